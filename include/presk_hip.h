@@ -236,6 +236,79 @@ void presk_hip_batch_release(presk_hip_batch *b);
  * host refuses it. */
 int presk_hip_dropout_mask(const void *key, double rate, const char *type, int64_t n, void *dst, void *stream);
 
+/* The losses of a large vocabulary and their gradients; no counterpart among
+ * the reference's nests, where a loss is `cross_entropy` over logits in memory
+ * (crates/presk-kernel/src/lower.rs:1459-1488).
+ *
+ * Of logits z [rows, vocab], with u = z / temperature:
+ *   lse[r]  = log sum_v exp(u[r, v])
+ *   loss[r] = T^2 * sum_v t[r, v] * (log t[r, v] - u[r, v] + lse[r])
+ *   mean    = the counted rows' mean loss (0 when none counts), and their number
+ *   dz[r]   = ct[r] * T * (exp(u[r] - lse[r]) - t[r])
+ * The target t[r] of `top` 0 is one column, index[r] (temperature 1): the
+ * softmax cross entropy.  With `top` k of 1 to 1024 it is the softmax of a
+ * teacher's k logits at the same temperature, teacher[r, j] at column
+ * index[r, j]; columns named twice have both weights.
+ * A slot whose index is negative, or whose teacher logit is -inf, is unused; a
+ * row with no used slot does not count: its loss and its row of dz are 0,
+ * whatever its logits are.  A slot at or past `vocab` makes its row's loss and
+ * cotangent NaN.  `ct` null: the mean's gradient, ct[r] = 1 / count.
+ *
+ * presk_hip_head_loss: z = x . w with x [rows, model] and w [model, vocab], or
+ * [vocab, model] when `tied`, in pieces of the vocabulary: the logits are not
+ * kept, whatever its size.  Gradients dx = dz . w^T and dw = x^T . dz, either
+ * of which may be null.  The products accumulate in f32; in 16-bit storage dz
+ * is rounded to the storage type before them (scaled to its range in f16).
+ * A row of x that does not count still enters dw times zero, so it must be
+ * finite.
+ * presk_hip_distill: z = x, given (model 0, w null, top >= 1); dx is dz.
+ *
+ * `what`: PRESK_HIP_LOSS_VALUE writes loss, lse (f32 [rows]) and mean (f32 [2]),
+ * those that are not null.  PRESK_HIP_LOSS_GRAD writes the gradients from the
+ * forward's lse and, with ct null, its mean.  Both: value and gradients in one
+ * call.  f16 outputs that overflow set bit 0 of *flag (if flag is not null), as
+ * a guarded nest's stores do.
+ * `work`: device memory of presk_hip_loss_workspace bytes (from the sizes and
+ * the nullness of the pointers alone), 16-byte aligned, this call's until it
+ * has run; nothing in it is kept between calls.  Every buffer is whole and
+ * row-major; an output may not meet another buffer.  Nothing is allocated, and
+ * only kernels are launched, so the calls may be captured.
+ * Storage types f32, bf16 and f16 (others are E7005); rows from 0, model and
+ * vocab below 2^22 (vocab of given logits below 2^30), and in f32 rows * model
+ * and model * vocab below 2^31. */
+typedef struct {
+    const char* dtype;
+    int64_t rows, model, vocab, top;
+    int32_t tied;
+    double temperature;
+    const void* x;
+    const void* w;
+    const int64_t* index;
+    const void* teacher;
+    float* loss;
+    float* lse;
+    float* mean;
+    const float* ct;
+    void* dx;
+    void* dw;
+    uint32_t* flag;
+    void* work;
+    size_t work_bytes;
+} presk_hip_loss;
+
+#define PRESK_HIP_LOSS_VALUE 1
+#define PRESK_HIP_LOSS_GRAD 2
+
+/* The workspace of presk_hip_head_loss (model >= 1) or presk_hip_distill (model
+ * 0) with these arguments; `work` and `work_bytes` are not read. */
+int presk_hip_loss_workspace(const presk_hip_loss* a, int what, size_t* bytes);
+int presk_hip_head_loss(const presk_hip_loss* a, int what, void* stream);
+int presk_hip_distill(const presk_hip_loss* a, int what, void* stream);
+/* Either as a step of a recorded sequence: the arguments are copied, the
+ * buffers (the workspace among them) must outlive the batch. */
+int presk_hip_batch_add_head_loss(presk_hip_batch* b, const presk_hip_loss* a, int what);
+int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int what);
+
 /* Seeded synthetic values written in place: n elements mean + std * z of
  * type "f32", "bf16" or "f16", z ~ N(0, 1) a function of (seed, element
  * index) alone (a splitmix64 hash and Box-Muller in f32).  Stands in for the

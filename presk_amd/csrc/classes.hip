@@ -530,19 +530,7 @@ struct GemmPlan : ClassPlan {
             if (n_bias) n_bias += nsz * bias_off;
         }
         if (seq) return gemm_seq_launch(a, stream);
-        // the clamped 16-byte loads need whole aligned vectors along the
-        // loaded axis: k when it is contiguous, else the rows
-        const int vec = storage == kF32 ? 4 : 8;
-        auto aligned = [&](const void* p, bool kcontig, long long rows, long long other_stride, const long long* bs) {
-            if ((uintptr_t)p % 16) return false;
-            if (other_stride % vec) return false;
-            if ((kcontig ? a.K : rows) % vec) return false;
-            for (int d = 0; d < a.nbatch; ++d)
-                if (bs[d] % vec) return false;
-            return true;
-        };
-        a.a_vec = aligned(a.A, a.a_kcontig, a.M, a.a_kcontig ? a.sa_m : a.sa_k, a.sa_b);
-        a.b_vec = aligned(a.B, a.b_kcontig, a.N, a.b_kcontig ? a.sb_n : a.sb_k, a.sb_b);
+        gemm_align(a);
         if (a.splits > 1) {
             if (!work) return hipErrorInvalidValue;
             a.work = (float*)work;
@@ -568,6 +556,22 @@ int storage_of(Ty t) {
 }
 
 }  // namespace
+
+// The clamped 16-byte loads need whole aligned vectors along the loaded
+// axis: k when it is contiguous, else the rows.
+void gemm_align(GemmArgs& g) {
+    const int vec = g.storage == kF32 ? 4 : 8;
+    auto aligned = [&](const void* p, bool kcontig, long long rows, long long other_stride, const long long* bs) {
+        if ((uintptr_t)p % 16) return false;
+        if (other_stride % vec) return false;
+        if ((kcontig ? g.K : rows) % vec) return false;
+        for (int d = 0; d < g.nbatch; ++d)
+            if (bs[d] % vec) return false;
+        return true;
+    };
+    g.a_vec = aligned(g.A, g.a_kcontig, g.M, g.a_kcontig ? g.sa_m : g.sa_k, g.sa_b);
+    g.b_vec = aligned(g.B, g.b_kcontig, g.N, g.b_kcontig ? g.sb_n : g.sb_k, g.sb_b);
+}
 
 bool tile_override(TileOverride* t, std::string* err) {
     *t = TileOverride{};
@@ -1544,5 +1548,7 @@ std::unique_ptr<ClassPlan> classify(const Kernel& k, int mode) {
     if (auto p = classify_gemm(k, mode == PRESK_HIP_EXACT)) return p;
     return nullptr;
 }
+
+void gemm_plan(GemmArgs& g) { plan_tiles(g, false); }
 
 }  // namespace presk

@@ -41,6 +41,10 @@ struct GemmArgs {
 };
 
 hipError_t gemm_launch(const GemmArgs& g, hipStream_t stream);
+// tiles and splits of a product whose M, N, K, strides and storage are set
+// (classes.hip), and at its launch, its pointers set, whether its vectors are whole
+void gemm_plan(GemmArgs& g);
+void gemm_align(GemmArgs& g);
 
 // f32 products as six bf16 products of operands split in three (gemm_split.hip)
 bool gemm_split_fits(const GemmArgs& g);

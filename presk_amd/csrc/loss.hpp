@@ -1,0 +1,148 @@
+// The losses of a large vocabulary (loss.hip, loss_rows.hip, loss_gemm.hpp):
+// softmax cross entropy and the divergence from a teacher's top logits, of
+// given logits or of a head's product x . w whose logits are never kept.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "gemm.hpp"
+#include "presk_hip.h"
+
+namespace presk {
+
+// What the ABI's arguments ask for, checked: "" or why not, the message
+// starting with its code.  `head`: of x . w, else of given logits.
+std::string loss_check(const presk_hip_loss& a, int what, bool head);
+std::string loss_check_buffers(const presk_hip_loss& a, int what, bool head);
+// the bytes of workspace a checked call needs
+size_t loss_workspace(const presk_hip_loss& a, int what, bool head);
+hipError_t loss_run(const presk_hip_loss& a, int what, bool head, hipStream_t s);
+
+// ---- what the kernels share -------------------------------------------------
+
+constexpr int kUnused = 0x7fffffff;    // a row's slot that names nothing (sorted last)
+constexpr int kOutside = 0x7ffffffe;   // one that names no column of the vocabulary
+constexpr int kParts = 1024;           // at most so many partial counts of a call's rows
+constexpr int kCols = 64;              // columns a `start` entry stands for
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// A row's target: `k` slots (column, weight) sorted by column, the weights'
+// sum of p log p (NaN where a slot names no column), and, where k > 4, each
+// 64-column block's first slot.
+struct LossTarget {
+    const int* col;              // [rows][k]
+    const float* p;              // [rows][k]
+    const float* ent;            // [rows]
+    const unsigned short* start; // [rows][nblocks + 1] or null
+    int k, nblocks;
+};
+
+// One 16-bit product of the head (loss_gemm.hpp).  Operands lie k-contiguous
+// (element (r, k) at r * s + k) or not ((r, k) at k * s + r).
+struct LossGemm {
+    const unsigned short *A, *B;
+    long long sa, sb;
+    int arows, brows;           // rows that exist (those past them are read from the last ones)
+    int ka, kb;                 // k that exist
+    int M, N, K;                // the product's extent (rows stored, k summed)
+    int tiles_m, tiles_n, splits;
+    // values: u = z * c, in units of log 2
+    float c;
+    LossTarget t;
+    int col0, cols;             // the product's first column of the vocabulary, and how many exist
+    long long rows;             // rows that exist
+    float *pm, *ps, *pa;        // a column tile's maximum, sum and target part: [tile][rows]
+    const float *lse, *coef;    // [rows]
+    unsigned short* P;          // the logits' cotangent, [prows][pld], zero past rows and cols
+    long long pld;
+    int prows;
+    // outputs
+    void* C;                    // 16-bit, row stride ldc (null: the f32 sums stay in acc)
+    long long ldc;
+    float* acc;                 // [M][N] f32: added to (acc_in), written where C is null
+    bool acc_in;
+    float* part;                // [splits][M][N] f32 (splits > 1)
+    const float* scale;         // the sums' factor, one float of device memory
+    unsigned* flag;
+};
+
+enum LossEpi { kEpiStats = 0, kEpiP = 1, kEpiOut = 2 };
+
+// tile rows and columns: 256 x 256 by eight waves, or 128 x 128 by four
+struct LossTile { int bm, bn; };
+hipError_t loss_gemm_bf16(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s);
+hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s);
+
+// ---- row kernels (loss_rows.hip) -------------------------------------------
+
+struct LossPrep {
+    const long long* index;
+    const void* teacher;
+    const float* ct;
+    int storage;
+    long long rows;
+    int vocab, top;
+    float c;                    // log2 e / T
+    int* col;
+    float *p, *ent;
+    unsigned short* start;
+    int nblocks;
+    int* count;                 // [parts]: counted rows
+    float* most;                // [parts]: their largest |ct|
+};
+// its blocks: `parts` of the counts
+int loss_parts(long long rows, int top);
+hipError_t loss_prep(const LossPrep& a, hipStream_t s);
+
+// partials -> a row's lse and loss, and the factor of its cotangent
+struct LossRows {
+    const float *pm, *ps, *pa;  // [slots][rows]
+    int slots;
+    LossTarget t;
+    long long rows;
+    float temperature;
+    float *lse, *loss;          // outputs, may be null
+    float* coef;                // [rows] or null
+    const float* ct;
+    const float* mean_in;       // {mean, count}: the count where the rows are not counted here
+    const int* count;
+    const float* most;
+    int parts;
+    float* scale;               // out (f16): the inverse of the factor in coef (null: none)
+};
+hipError_t loss_rows(const LossRows& a, hipStream_t s);
+hipError_t loss_mean(const float* loss, long long rows, const int* count, int parts, float* mean, hipStream_t s);
+
+// Logits in memory, [rows][ld] from column col0 on, `cols` of them.
+struct LossMatrix {
+    const void* z;
+    long long ld;
+    int storage;                // Storage
+    long long rows;
+    int col0, cols;
+    float c;
+    LossTarget t;
+};
+// partials [chunk][rows] from slot0 on
+int loss_chunks(long long rows, int cols);
+hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, hipStream_t s);
+// the logits' cotangent, coef * (softmax - target), stored as `to`
+hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, int to,
+                     unsigned* flag, hipStream_t s);
+
+// value and cotangent of whole rows, each read once and held in registers:
+// lse, loss (either may be null) and coef * (softmax - target) stored as m.storage
+bool loss_joint_fits(const LossMatrix& m);
+hipError_t loss_joint(const LossMatrix& m, float temperature, float* lse, float* loss, const float* coef, void* out, long long ldo,
+                      unsigned* flag, hipStream_t s);
+
+// [rows][cols] 16-bit from row stride lds to ldd, zero up to padded columns
+hipError_t loss_pack(const void* src, long long lds, long long rows, int cols, void* dst, int ldd, hipStream_t s);
+hipError_t loss_zero(void* dst, long long bytes, hipStream_t s);
+// the partials' sum, in split order, times scale (plus acc): into C (16-bit, ldc) or acc
+hipError_t loss_join(const LossGemm& g, int storage, hipStream_t s);
+
+}  // namespace presk

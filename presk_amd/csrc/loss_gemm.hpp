@@ -1,0 +1,481 @@
+// The 16-bit products of a head whose logits are not kept (loss.hip):
+//   kEpiStats  z = x . w, of which a column tile leaves each row's maximum, its
+//              sum of exponentials and its target's logits alone;
+//   kEpiP      z again, leaving the logits' cotangent coef * (exp(u - lse) - t)
+//              rounded to 16 bits, a piece of the vocabulary's;
+//   kEpiOut    dx += P . w^T and dw = x^T . P over that piece.
+// 32x32x16 MFMAs over tiles of 256 x 256 by eight waves (128 x 64 a wave, one
+// workgroup a CU) or 128 x 128 by four (64 x 64, two workgroups a CU), two
+// 64-deep k-blocks in LDS, loaded straight into it.  The MFMAs take the
+// operands' roles exchanged (D = B^T A^T), so that a lane holds one row's
+// columns, four consecutive ones at a time: a row's maximum and sum are lane
+// sums and one exchange between half-waves.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "devfmt.hpp"
+#include "loss.hpp"
+
+namespace presk {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+
+constexpr int BK = 64;
+
+// One operand's 64-deep block in LDS, 16-byte chunks placed by an XOR swizzle
+// (lane i of a wave's load fills slot i of the wave's 1 KB, the swizzle picks
+// the chunk that it fetches), so that the fragment reads meet no bank twice:
+//   k-contiguous, [row][8 chunks of 8 k]: chunk c of row r at 8 r + (c ^ ((r ^ (r >> 3)) & 7))
+//   else, [k][ROWS / 8 chunks of 8 rows]: chunk j of k-row r at
+//     (ROWS / 8) r + (j ^ (2 (r & 3) ^ 8 (r & 1)))
+// Loads past the operand are moved to where it ends: a row to the last row
+// (or last whole vector of rows), a k to the last k (or last whole vector), whose
+// products meet a zero of the other operand or are not stored.  The
+// addresses are the tile's origin (uniform, 64 bits) and a lane's 32-bit
+// offset in the block.  The loads are inline assembly without an output; the
+// kernel waits for them (wait_vm) before the barrier ahead of every read.
+template <bool KC, int ROWS, int NTH>
+struct Block16 {
+    static constexpr int CPR = KC ? 8 : ROWS / 8;
+    static constexpr int SLOTS = ROWS * BK / 8, ROUNDS = SLOTS / NTH, BYTES = SLOTS * 16;
+    static_assert(SLOTS % NTH == 0 && (KC || ROWS % 128 == 0), "whole rounds, the swizzle inside a k-row");
+    unsigned voff[ROUNDS];
+    const char* origin;
+    long long block_bytes;
+    unsigned lds0;
+    long long stride;
+    int nk;                     // k that exist
+
+    __device__ static __forceinline__ int swz(int r) {
+        return KC ? ((r ^ (r >> 3)) & 7) : ((2 * (r & 3)) ^ (8 * (r & 1)));
+    }
+    __device__ __forceinline__ void init(const unsigned short* p, int rows, long long s, int row0, int k_exist, unsigned tile) {
+        const int t = threadIdx.x;
+        stride = s;
+        nk = k_exist;
+        origin = (const char*)(p + (KC ? (long long)row0 * s : (long long)row0));
+        block_bytes = KC ? 2LL * BK : 2LL * BK * s;
+#pragma unroll
+        for (int q = 0; q < ROUNDS; ++q) {
+            const int slot = q * NTH + t, r = slot / CPR, c = (slot % CPR) ^ swz(r);
+            if (KC) {
+                const int row = row0 + r < rows ? r : rows - 1 - row0;
+                voff[q] = (unsigned)(2 * (row * s + 8 * c));
+            } else {
+                const int row = row0 + 8 * c + 8 <= rows ? 8 * c : rows - 8 - row0;
+                voff[q] = (unsigned)(2 * (r * s + row));
+            }
+        }
+        lds0 = __builtin_amdgcn_readfirstlane(tile + (unsigned)(t & ~63) * 16u);
+    }
+    __device__ __forceinline__ void issue(int kb, unsigned stage) const {
+        const char* const src = origin + kb * block_bytes;
+        const int left = nk - kb * BK;      // k of this block that exist
+        if (left >= BK) {
+#pragma unroll
+            for (int q = 0; q < ROUNDS; ++q)
+                asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+                             : : "v"(voff[q]), "s"(src), "s"(__builtin_amdgcn_readfirstlane(lds0 + stage + (unsigned)(q * NTH * 16))) : "memory", "m0");
+        } else {
+            // a block in which the operand ends, or one past its end (then
+            // the whole block is read from the last k): offsets may be negative,
+            // so the address is the lane's own
+            const int t = threadIdx.x;
+#pragma unroll
+            for (int q = 0; q < ROUNDS; ++q) {
+                const int slot = q * NTH + t, r = slot / CPR, c = (slot % CPR) ^ swz(r);
+                long long move = 0;
+                if (KC) {
+                    if (8 * c + 8 > left) move = 2LL * (left - 8 - 8 * c);
+                } else if (r >= left) {
+                    move = 2LL * (left - 1 - r) * stride;
+                }
+                const char* const at = src + voff[q] + move;
+                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+                             : : "v"(at), "s"(__builtin_amdgcn_readfirstlane(lds0 + stage + (unsigned)(q * NTH * 16))) : "memory", "m0");
+            }
+        }
+    }
+    // the 32x32x16 fragment: a lane's k = kk + 8 (lane >> 5) .. + 8 of row
+    // base + (lane & 31): one 16-byte read, or two transposing ones
+    __device__ static __forceinline__ u16x8 frag(const unsigned char* xs, int base, int kk, int lane) {
+        if constexpr (KC) {
+            const int r = base + (lane & 31), c = (kk >> 3) + (lane >> 5);
+            return *(const u16x8*)(xs + (r * 8 + (c ^ swz(r))) * 16);
+        } else {
+            const int L = lane & 15, g = lane >> 4;
+            const int r = kk + 8 * (g >> 1) + (L >> 2), col = base + 16 * (g & 1) + 4 * (L & 3);
+            const int off = r * ROWS * 2 + (((col >> 3) ^ swz(r)) << 4) + (col & 7) * 2;
+            const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(xs + off));
+            const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(xs + off + 4 * ROWS * 2));
+            u16x8 f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] = (unsigned short)lo[e];
+                f[4 + e] = (unsigned short)hi[e];
+            }
+            return f;
+        }
+    }
+};
+
+// at most N of this thread's vector-memory operations outstanding
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+template <int ST>
+__device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 acc) {
+    if constexpr (ST == kBF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+}
+
+template <int ST>
+__device__ __forceinline__ unsigned short narrow(float v, bool& ovf) {
+    if constexpr (ST == kBF16) return pk_f32_to_bf16(v);
+    ovf |= pk_overflows_f16(v);
+    return pk_f32_to_f16(v);
+}
+
+// The column, of the wave's 64, of a lane's sum e of column fragment j
+__device__ __forceinline__ int col_of(int j, int e, int lane) { return j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+
+template <int ST, bool AKC, bool BKC, int WM, int NW, int WAN, int EPI>
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(LossGemm g) {
+    constexpr int WN = 2, NTH = 64 * NW, WAM = NW / WAN, BM = WAM * WM * 32, BN = WAN * 64;
+    typedef Block16<AKC, BM, NTH> QA;
+    typedef Block16<BKC, BN, NTH> QB;
+    constexpr int STAGE = QA::BYTES + QB::BYTES, NS = 2, CLD = BN + 8;
+    constexpr int OPER = NS * STAGE, CTILE = EPI == kEpiStats ? 3 * WAN * BM * 4 : BM * CLD * 2;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[OPER > CTILE ? OPER : CTILE];
+
+    // Work order: workgroups are dealt to the 8 XCDs round robin; each XCD
+    // takes one run of items, tiles GROUP rows at a time across the columns,
+    // so that those in flight share panels in its L2.
+    const unsigned tiles = (unsigned)g.tiles_m * (unsigned)g.tiles_n, total = gridDim.x;
+    const unsigned xcd = blockIdx.x % 8, q8 = total / 8, r8 = total % 8;
+    const unsigned item = xcd * q8 + (xcd < r8 ? xcd : r8) + blockIdx.x / 8;
+    const int split = (int)(item / tiles);
+    const unsigned bid = item - (unsigned)split * tiles;
+    constexpr unsigned GROUP = BM == 256 ? 4 : 8;
+    const unsigned group_size = GROUP * (unsigned)g.tiles_n, grp = bid / group_size, first_m = grp * GROUP;
+    const unsigned gm = (unsigned)g.tiles_m - first_m < GROUP ? (unsigned)g.tiles_m - first_m : GROUP;
+    const unsigned in_grp = bid - grp * group_size, tn = in_grp / gm, tm = first_m + (in_grp - tn * gm);
+    const int m0 = (int)tm * BM, n0 = (int)tn * BN;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave / WAN * (WM * 32), wn = wave % WAN * 64;
+    f32x16 acc[WM][WN];
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
+
+    // split s of S takes k-blocks [s * n / S, (s + 1) * n / S)
+    const unsigned nkb = (unsigned)((g.K + BK - 1) / BK), ns = (unsigned)g.splits;
+    const int kb0 = (int)((unsigned)split * nkb / ns), nd = (int)(((unsigned)split + 1) * nkb / ns) - kb0;
+
+    // Block kt + 1 streams into one stage while block kt is multiplied out of
+    // the other; each 16-k step's fragments are read during the step before.
+    // Before a block's last step this thread's loads of the next block have
+    // landed, and a barrier has seen every thread's; it also retires every read
+    // of the stage that the loads after it overwrite.
+    QA qa;
+    QB qb;
+    const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
+    qa.init(g.A, g.arows, g.sa, m0, g.ka, lds);
+    qb.init(g.B, g.brows, g.sb, n0, g.kb, lds + QA::BYTES);
+    auto fetch = [&](int kb, int st) {
+        qa.issue(kb0 + kb, (unsigned)(st * STAGE));
+        qb.issue(kb0 + kb, (unsigned)(st * STAGE));
+    };
+    u16x8 a[WM], b[WN];
+    auto read = [&](const unsigned char* st, int kk) {
+#pragma unroll
+        for (int i = 0; i < WM; ++i) a[i] = QA::frag(st, wm + i * 32, kk, lane);
+#pragma unroll
+        for (int j = 0; j < WN; ++j) b[j] = QB::frag(st + QA::BYTES, wn + j * 32, kk, lane);
+    };
+    if (nd > 0) {
+        fetch(0, 0);
+        wait_vm<0>();
+        __syncthreads();
+        read(smem, 0);
+    }
+    auto block = [&](int kt, auto stage) {
+        constexpr int CUR = decltype(stage)::value;
+        if (kt + 1 < nd) fetch(kt + 1, CUR ^ 1);
+        const unsigned char* const st = smem + CUR * STAGE;
+#pragma unroll
+        for (int kk = 0; kk < BK; kk += 16) {
+            u16x8 ca[WM], cb[WN];
+#pragma unroll
+            for (int i = 0; i < WM; ++i) ca[i] = a[i];
+#pragma unroll
+            for (int j = 0; j < WN; ++j) cb[j] = b[j];
+            if (kk + 16 < BK) {
+                read(st, kk + 16);
+            } else if (kt + 1 < nd) {
+                wait_vm<0>();
+                __syncthreads();
+                read(smem + (CUR ^ 1) * STAGE, 0);
+            }
+            // the reads stay ahead of this step's MFMAs
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int j = 0; j < WN; ++j) acc[i][j] = mfma32<ST>(cb[j], ca[i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int kt = 0;
+    for (; kt + 2 <= nd; kt += 2) {
+        block(kt, std::integral_constant<int, 0>{});
+        block(kt + 1, std::integral_constant<int, 1>{});
+    }
+    if (kt < nd) block(kt, std::integral_constant<int, 0>{});
+    __syncthreads();    // the stages are the epilogue's from here
+
+    // The slots of row m's target in the wave's 64 columns: f(column, weight)
+    // for each, in order.
+    auto targets = [&](int m, auto f) {
+        const bool in = m < g.rows;
+        const int k = g.t.k, first = g.col0 + n0 + wn;
+        long long e = 0, end = 0;
+        if (in) {
+            e = (long long)m * k;
+            end = e + k;
+            if (g.t.start) {
+                const unsigned short* const s = g.t.start + (long long)m * (g.t.nblocks + 1);
+                const int blk = first / kCols < g.t.nblocks ? first / kCols : g.t.nblocks - 1;
+                const bool past = first / kCols >= g.t.nblocks;
+                end = e + (past ? 0 : s[blk + 1]);
+                e = e + (past ? 0 : s[blk]);
+            }
+        }
+        while (__any(e < end)) {
+            const bool on = e < end;
+            const int col = on ? g.t.col[e] - first : -1;
+            const float p = on ? g.t.p[e] : 0.f;
+            if (__any(col >= 0 && col < 64)) f(col, p);
+            ++e;
+        }
+    };
+
+    if constexpr (EPI == kEpiStats) {
+        float* const red = (float*)smem;    // [3][WAN][BM]
+        const int h = lane >> 5;
+        const bool edge = n0 + BN > g.cols;
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {
+            const int row = wm + i * 32 + (lane & 31);
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (n0 + wn + col_of(j, e, lane) >= g.cols) acc[i][j][e] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < WN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float mc = mx * g.c, base = mx == -INFINITY ? 0.f : mc;
+            float s = 0.f, ta = 0.f;
+#pragma unroll
+            for (int j = 0; j < WN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], g.c, -base));
+            targets(m0 + row, [&](int col, float p) {
+                float v = 0.f;
+                bool hit = false;
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (col == col_of(j, e, lane)) {
+                            v = acc[i][j][e];
+                            hit = true;
+                        }
+                if (hit) ta += p * (v * g.c);
+            });
+            s += __shfl_xor(s, 32);
+            ta += __shfl_xor(ta, 32);
+            if (h == 0) {
+                const int at = wave % WAN * BM + row;
+                red[at] = mc;
+                red[WAN * BM + at] = s;
+                red[2 * WAN * BM + at] = ta;
+            }
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < BM; r += NTH) {
+            if (m0 + r >= g.rows) continue;
+            float m = red[r], s = 0.f, ta = 0.f;
+#pragma unroll
+            for (int w = 1; w < WAN; ++w) m = fmaxf(m, red[w * BM + r]);
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < WAN; ++w) {
+                s += red[(WAN + w) * BM + r] * __builtin_amdgcn_exp2f(red[w * BM + r] - base);
+                ta += red[(2 * WAN + w) * BM + r];
+            }
+            const long long at = (long long)tn * g.rows + m0 + r;
+            g.pm[at] = m;
+            g.ps[at] = s;
+            g.pa[at] = ta;
+        }
+    } else if constexpr (EPI == kEpiP) {
+        unsigned short* const ct = (unsigned short*)smem;   // [BM][CLD]
+        bool ovf = false;
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {
+            const int row = wm + i * 32 + (lane & 31), m = m0 + row;
+            const bool in = m < g.rows;
+            const float lse = in ? g.lse[m] * kLog2e : 0.f, coef = in ? g.coef[m] : 0.f;
+#pragma unroll
+            for (int j = 0; j < WN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], g.c, -lse));
+            targets(m, [&](int col, float p) {
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (col == col_of(j, e, lane)) acc[i][j][e] -= p;
+            });
+#pragma unroll
+            for (int j = 0; j < WN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    u16x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int col = col_of(j, 4 * q + e, lane);
+                        const float x = coef == 0.f || n0 + wn + col >= g.cols ? 0.f : acc[i][j][4 * q + e] * coef;
+                        v[e] = narrow<ST>(x, ovf);
+                    }
+                    *(u16x4*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
+                }
+        }
+        __syncthreads();
+        constexpr int VPR = BN / 8;
+        for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
+            const int r = u / VPR, c = u % VPR * 8;
+            if (m0 + r < g.prows && n0 + c < g.pld)
+                *(u16x8*)(g.P + (long long)(m0 + r) * g.pld + n0 + c) = *(const u16x8*)&ct[r * CLD + c];
+        }
+    } else {
+        const float scale = g.scale ? *g.scale : 1.f;
+        if (g.splits > 1 || !g.C) {
+            // f32 sums: four consecutive columns of a row from the registers
+            float* const out = g.splits > 1 ? g.part + (long long)split * g.M * g.N : g.acc;
+            const bool add = g.splits <= 1 && g.acc_in, vec = g.N % 4 == 0;
+            const float f = g.splits > 1 ? 1.f : scale;
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                const int m = m0 + wm + i * 32 + (lane & 31);
+                if (m >= g.M) continue;
+                float* const row = out + (long long)m * g.N;
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int n = n0 + wn + col_of(j, 4 * q, lane);
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * f;
+                        if (vec && n < g.N) {
+                            if (add) v += *(const f32x4*)(row + n);
+                            *(f32x4*)(row + n) = v;
+                        } else {
+                            for (int e = 0; e < 4 && n + e < g.N; ++e) row[n + e] = add ? row[n + e] + v[e] : v[e];
+                        }
+                    }
+            }
+        } else {
+            unsigned short* const ct = (unsigned short*)smem;
+            bool ovf = false;
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                const int row = wm + i * 32 + (lane & 31), m = m0 + row;
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = wn + col_of(j, 4 * q, lane);
+                        u16x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = acc[i][j][4 * q + e] * scale;
+                            const bool in = m < g.M && n0 + c + e < g.N;
+                            if (g.acc_in && in) x += g.acc[(long long)m * g.N + n0 + c + e];
+                            bool o = false;
+                            v[e] = narrow<ST>(x, o);
+                            ovf |= o && in;
+                        }
+                        *(u16x4*)&ct[row * CLD + c] = v;
+                    }
+            }
+            if (ovf && g.flag) atomicOr(g.flag, 1u);
+            __syncthreads();
+            unsigned short* const C = (unsigned short*)g.C;
+            if (g.ldc % 8 == 0 && g.N % 8 == 0 && (size_t)C % 16 == 0) {
+                constexpr int VPR = BN / 8;
+                for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
+                    const int r = u / VPR, c = u % VPR * 8;
+                    if (m0 + r < g.M && n0 + c < g.N)
+                        *(u16x8*)(C + (long long)(m0 + r) * g.ldc + n0 + c) = *(const u16x8*)&ct[r * CLD + c];
+                }
+            } else {
+                for (int u = threadIdx.x; u < BM * BN; u += NTH) {
+                    const int r = u / BN, c = u % BN;
+                    if (m0 + r < g.M && n0 + c < g.N) C[(long long)(m0 + r) * g.ldc + n0 + c] = ct[r * CLD + c];
+                }
+            }
+        }
+    }
+}
+
+template <int ST, bool AKC, bool BKC, int EPI>
+hipError_t launch(const LossGemm& g, int tile, hipStream_t s) {
+    const unsigned grid = (unsigned)g.tiles_m * (unsigned)g.tiles_n * (unsigned)g.splits;
+    if (!grid) return hipSuccess;
+    if (tile == 256)
+        loss_gemm_kernel<ST, AKC, BKC, 4, 8, 4, EPI><<<grid, 512, 0, s>>>(g);
+    else
+        loss_gemm_kernel<ST, AKC, BKC, 2, 4, 2, EPI><<<grid, 256, 0, s>>>(g);
+    return hipGetLastError();
+}
+
+template <int ST>
+hipError_t dispatch(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s) {
+    if (epi == kEpiStats) return bkc ? launch<ST, true, true, kEpiStats>(g, tile, s) : launch<ST, true, false, kEpiStats>(g, tile, s);
+    if (epi == kEpiP) return bkc ? launch<ST, true, true, kEpiP>(g, tile, s) : launch<ST, true, false, kEpiP>(g, tile, s);
+    if (akc) return bkc ? launch<ST, true, true, kEpiOut>(g, tile, s) : launch<ST, true, false, kEpiOut>(g, tile, s);
+    return launch<ST, false, false, kEpiOut>(g, tile, s);
+}
+
+}  // namespace
+
+}  // namespace presk

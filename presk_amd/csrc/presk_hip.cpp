@@ -20,6 +20,7 @@
 
 #include "branches.hpp"
 #include "convert.hpp"
+#include "loss.hpp"
 #include "probe.hpp"
 #include "synth.hpp"
 #include "executor.hpp"
@@ -516,7 +517,8 @@ int presk_hip_time(const presk_hip_kernel* h, void* const* bufs, int64_t lo, int
 
 struct presk_hip_batch {
     // a kernel launch, or (k null) an edge conversion, or (k null, rate >= 0)
-    // a dropout mask: bufs {key, dst}, type in `to`
+    // a dropout mask: bufs {key, dst}, type in `to`, or (k null, what > 0) a
+    // loss over its own arguments
     struct Item {
         const presk_hip_kernel* k;
         std::vector<void*> bufs;
@@ -524,6 +526,9 @@ struct presk_hip_batch {
         int from = -1, to = -1;
         int64_t n = 0;
         double rate = -1.0;
+        presk_hip_loss loss{};
+        int what = 0;
+        bool head = false;
     };
     std::vector<Item> items;
     hipGraph_t graph = nullptr;
@@ -559,6 +564,10 @@ struct presk_hip_batch {
         return PRESK_HIP_OK;
     }
     static int run_one(const Item& it, hipStream_t s) {
+        if (it.what) {
+            hipError_t e = loss_run(it.loss, it.what, it.head, s);
+            return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, it.head ? "head loss" : "distillation");
+        }
         if (!it.k && it.rate >= 0.0) {
             hipError_t e = dropout_launch(it.bufs[0], it.rate, it.to, it.n, it.bufs[1], s);
             return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, "dropout mask");
@@ -820,6 +829,57 @@ int presk_hip_batch_add_convert(presk_hip_batch* b, const void* src, const char*
     b->items.push_back(it);
     return PRESK_HIP_OK;
 }
+
+}  // extern "C"
+
+namespace {
+
+// a loss's arguments and buffers, checked
+int check_loss(const presk_hip_loss* a, int what, bool head) {
+    if (!a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    std::string why = loss_check(*a, what, head);
+    if (why.empty()) why = loss_check_buffers(*a, what, head);
+    if (why.empty()) return PRESK_HIP_OK;
+    return fail(why.compare(0, 5, "E7005") == 0 ? PRESK_HIP_REFUSED : PRESK_HIP_ERR, why);
+}
+
+int run_loss(const presk_hip_loss* a, int what, bool head, void* stream) {
+    if (int rc = check_loss(a, what, head)) return rc;
+    hipError_t e = loss_run(*a, what, head, (hipStream_t)stream);
+    return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, head ? "head loss" : "distillation");
+}
+
+int add_loss(presk_hip_batch* b, const presk_hip_loss* a, int what, bool head) {
+    if (!b) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (int rc = check_loss(a, what, head)) return rc;
+    b->drop_graph();
+    presk_hip_batch::Item it{nullptr, {}, 0, 0};
+    it.loss = *a;
+    const std::string type = a->dtype;
+    it.loss.dtype = type == "f32" ? "f32" : type == "bf16" ? "bf16" : "f16";
+    it.what = what;
+    it.head = head;
+    b->items.push_back(it);
+    return PRESK_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int presk_hip_loss_workspace(const presk_hip_loss* a, int what, size_t* bytes) {
+    if (!a || !bytes) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    const bool head = a->model != 0;
+    const std::string why = loss_check(*a, what, head);
+    if (!why.empty()) return fail(why.compare(0, 5, "E7005") == 0 ? PRESK_HIP_REFUSED : PRESK_HIP_ERR, why);
+    *bytes = loss_workspace(*a, what, head);
+    return PRESK_HIP_OK;
+}
+
+int presk_hip_head_loss(const presk_hip_loss* a, int what, void* stream) { return run_loss(a, what, true, stream); }
+int presk_hip_distill(const presk_hip_loss* a, int what, void* stream) { return run_loss(a, what, false, stream); }
+int presk_hip_batch_add_head_loss(presk_hip_batch* b, const presk_hip_loss* a, int what) { return add_loss(b, a, what, true); }
+int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int what) { return add_loss(b, a, what, false); }
 
 int presk_hip_batch_graph(presk_hip_batch* b) { return presk_hip_batch_graph_branches(b, 1); }
 

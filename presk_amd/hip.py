@@ -28,7 +28,8 @@ SYMBOLS = ["presk_hip_init", "presk_hip_last_error", "presk_hip_compile", "presk
            "presk_hip_scalar_digest", "presk_hip_batch_create", "presk_hip_batch_add", "presk_hip_batch_graph", "presk_hip_batch_graph_branches",
            "presk_hip_batch_run", "presk_hip_batch_release", "presk_hip_convert", "presk_hip_batch_add_convert",
            "presk_hip_fill_normal", "presk_hip_dropout_mask", "presk_hip_batch_add_dropout",
-           "presk_hip_pskd_decode", "presk_hip_pskd_decode_idx", "presk_hip_mfma_probe"]
+           "presk_hip_pskd_decode", "presk_hip_pskd_decode_idx", "presk_hip_mfma_probe",
+           "presk_hip_loss_workspace", "presk_hip_head_loss", "presk_hip_distill", "presk_hip_batch_add_head_loss", "presk_hip_batch_add_distill"]
 
 
 class HipError(RuntimeError):
@@ -45,6 +46,14 @@ class Info(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_char * 32), ("order", ctypes.c_char * 32), ("guarded", ctypes.c_int32),
                 ("n_inputs", ctypes.c_int32), ("split_bound", ctypes.c_int64), ("flops", ctypes.c_double),
                 ("bytes", ctypes.c_double)]
+
+
+class LossArgs(ctypes.Structure):
+    """presk_hip_loss."""
+    _fields_ = [("dtype", ctypes.c_char_p), ("rows", ctypes.c_int64), ("model", ctypes.c_int64), ("vocab", ctypes.c_int64),
+                ("top", ctypes.c_int64), ("tied", ctypes.c_int32), ("temperature", ctypes.c_double)] + [
+                    (n, ctypes.c_void_p) for n in ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag", "work")
+                ] + [("work_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -93,6 +102,12 @@ def lib():
         L.presk_hip_dropout_mask.argtypes = [vp, ctypes.c_double, ctypes.c_char_p, i64, vp, vp]
         L.presk_hip_batch_add_dropout.argtypes = [vp, vp, ctypes.c_double, ctypes.c_char_p, i64, vp]
         L.presk_hip_batch_add_convert.argtypes = [vp, vp, ctypes.c_char_p, vp, ctypes.c_char_p, i64, vp]
+        la = ctypes.POINTER(LossArgs)
+        L.presk_hip_loss_workspace.argtypes = [la, i32, ctypes.POINTER(ctypes.c_size_t)]
+        L.presk_hip_head_loss.argtypes = [la, i32, vp]
+        L.presk_hip_distill.argtypes = [la, i32, vp]
+        L.presk_hip_batch_add_head_loss.argtypes = [vp, la, i32]
+        L.presk_hip_batch_add_distill.argtypes = [vp, la, i32]
         _lib = L
     return _lib
 
@@ -287,3 +302,131 @@ class HipExec:
                 raise HipError(OVERFLOW, f"E7007: the kernel `{text.split(' (')[0][7:]}` stored a finite value past the largest "
                                          f"finite number of {dtype} (an overflow of its storage)")
         return c
+
+
+# ---- the losses of a large vocabulary ---------------------------------------------
+
+VALUE, GRAD = 1, 2
+_WHAT = {"value": VALUE, "vjp": GRAD, "step": VALUE | GRAD}
+
+
+def _buffer(name: str, b, nbytes: int) -> int:
+    """The device pointer of a buffer of at least `nbytes` bytes: a
+    DeviceBuffer, or an array of another library that says where and how
+    large it is (torch's `data_ptr` and `nbytes`, contiguous)."""
+    if b is None:
+        return None
+    if hasattr(b, "data_ptr"):
+        if not b.is_cuda:
+            raise ValueError(f"{name} is not in device memory")
+        if not b.is_contiguous():
+            raise ValueError(f"{name} is not contiguous")
+        ptr, have = b.data_ptr(), b.nbytes
+    else:
+        ptr, have = b.ptr, b.nbytes
+    if have < nbytes:
+        raise ValueError(f"{name} has {have} bytes, {nbytes} needed")
+    return ptr
+
+
+class Distill:
+    """presk_hip_distill at fixed sizes: the divergence of given logits x
+    [rows, vocab] from the softmax of a teacher's `top` logits, teacher[r, j]
+    at column index[r, j] (i64; negative: unused), both at `temperature`.
+
+    `value` writes loss, lse (f32 [rows]) and mean (f32 [2]: the counted rows'
+    mean and their number), those given.  `vjp` writes the logits' cotangent
+    dx from the forward's lse, for a row's cotangent ct (f32 [rows]), or for
+    the mean's where mean is given in its place.  `value_and_grad` does both,
+    for ct or else the mean.  Buffers are DeviceBuffers or torch tensors;
+    `work` is workspace(kind) bytes of the caller's, or, not given, a buffer
+    this object keeps: calls that share a workspace run one after another (one
+    stream, or an object a stream)."""
+
+    head = False
+
+    def __init__(self, dtype: str, rows: int, vocab: int, top: int, temperature: float = 1.0):
+        self._set(dtype, rows, 0, vocab, top, False, temperature)
+
+    def _set(self, dtype, rows, model, vocab, top, tied, temperature):
+        self.dtype, self.rows, self.model, self.vocab, self.top = dtype, int(rows), int(model), int(vocab), int(top)
+        self.tied, self.temperature = bool(tied), float(temperature)
+        self._work, self._needs = None, {}
+        self.workspace("value")     # the sizes and the type are checked here
+
+    def _args(self) -> LossArgs:
+        a = LossArgs()
+        a.dtype, a.rows, a.model, a.vocab, a.top = self.dtype.encode(), self.rows, self.model, self.vocab, self.top
+        a.tied, a.temperature = int(self.tied), self.temperature
+        return a
+
+    def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
+        """Bytes of workspace for `value`, `vjp` or `step` (value_and_grad),
+        with the gradients asked for."""
+        key = (kind, dx, dw)
+        if key not in self._needs:
+            a, n = self._args(), ctypes.c_size_t()
+            # (only whether they are null is looked at)
+            a.dx, a.dw = (1 if dx else None), (1 if dw and self.head else None)
+            check(lib().presk_hip_loss_workspace(ctypes.byref(a), _WHAT[kind], ctypes.byref(n)))
+            self._needs[key] = n.value
+        return self._needs[key]
+
+    def args(self, kind: str, work=None, flag=None, **bufs) -> LossArgs:
+        """The call's arguments, each buffer checked against its size."""
+        e = STORAGE_BYTES[self.dtype]
+        n, k = self.rows, max(self.top, 1)
+        x, w = n * (self.model if self.head else self.vocab) * e, self.model * self.vocab * e
+        sizes = {"x": x, "w": w, "index": 8 * n * k, "teacher": e * n * self.top, "loss": 4 * n, "lse": 4 * n, "mean": 8, "ct": 4 * n,
+                 "dx": x, "dw": w}
+        a = self._args()
+        for name, b in bufs.items():
+            setattr(a, name, _buffer(name, b, sizes[name]))
+        a.flag = _buffer("flag", flag, 4)
+        need = self.workspace(kind, bufs.get("dx") is not None, bufs.get("dw") is not None)
+        if work is None:
+            if self._work is None or self._work.nbytes < need:
+                self._work = DeviceBuffer(need)
+            work = self._work
+        a.work, a.work_bytes = _buffer("work", work, need), work.nbytes
+        return a
+
+    def _call(self, kind, stream, **bufs):
+        a = self.args(kind, **bufs)
+        f = lib().presk_hip_head_loss if self.head else lib().presk_hip_distill
+        check(f(ctypes.byref(a), _WHAT[kind], stream))
+
+    def value(self, x, index, teacher, loss=None, lse=None, mean=None, work=None, stream=None):
+        self._call("value", stream, x=x, index=index, teacher=teacher, loss=loss, lse=lse, mean=mean, work=work)
+
+    def vjp(self, x, index, teacher, lse, dx, ct=None, mean=None, flag=None, work=None, stream=None):
+        self._call("vjp", stream, x=x, index=index, teacher=teacher, lse=lse, dx=dx, ct=ct, mean=mean, flag=flag, work=work)
+
+    def value_and_grad(self, x, index, teacher, dx, loss=None, lse=None, mean=None, ct=None, flag=None, work=None, stream=None):
+        self._call("step", stream, x=x, index=index, teacher=teacher, dx=dx, loss=loss, lse=lse, mean=mean, ct=ct, flag=flag, work=work)
+
+
+class HeadLoss(Distill):
+    """presk_hip_head_loss at fixed sizes: the loss of the logits x . w, which
+    are not kept.  x [rows, model]; w [model, vocab], or [vocab, model] when
+    `tied`; `top` 0: the softmax cross entropy against index[r] (negative: the
+    row does not count); `top` k: Distill's loss.  The methods are Distill's,
+    with w, and the gradients dx and dw, of which one may be left out."""
+
+    head = True
+
+    def __init__(self, dtype: str, rows: int, model: int, vocab: int, tied: bool = False, top: int = 0, temperature: float = 1.0):
+        if int(model) < 1:
+            raise ValueError(f"a head of model {model}")
+        self._set(dtype, rows, model, vocab, top, tied, temperature)
+
+    def value(self, x, w, index, teacher=None, loss=None, lse=None, mean=None, work=None, stream=None):
+        self._call("value", stream, x=x, w=w, index=index, teacher=teacher, loss=loss, lse=lse, mean=mean, work=work)
+
+    def vjp(self, x, w, index, lse, dx=None, dw=None, teacher=None, ct=None, mean=None, flag=None, work=None, stream=None):
+        self._call("vjp", stream, x=x, w=w, index=index, teacher=teacher, lse=lse, dx=dx, dw=dw, ct=ct, mean=mean, flag=flag, work=work)
+
+    def value_and_grad(self, x, w, index, dx=None, dw=None, teacher=None, loss=None, lse=None, mean=None, ct=None, flag=None, work=None,
+                       stream=None):
+        self._call("step", stream, x=x, w=w, index=index, teacher=teacher, dx=dx, dw=dw, loss=loss, lse=lse, mean=mean, ct=ct, flag=flag,
+                   work=work)
