@@ -204,6 +204,7 @@ struct Call {
     hipStream_t s;
     char* w;
     LossTarget t;
+    bool mean_done = false;
 
     template <typename T>
     T* at(size_t off) const { return (T*)(w + off); }
@@ -267,7 +268,7 @@ struct Call {
         return h.splits > 1 ? loss_join(g, q.st, s) : hipSuccess;
     }
 
-    hipError_t half(const float* lse) const {
+    hipError_t half(const float* lse) {
         Side x{(const unsigned short*)a.x, q.D, (int)q.rows, q.D};
         if (q.packx) {
             LOSS_TRY(loss_pack(a.x, q.D, q.rows, q.D, at<void>(q.xp), q.Dp, s));
@@ -289,8 +290,7 @@ struct Call {
             }
         }
         LOSS_TRY(rows_of());
-        if (!q.grad || (!a.dx && !a.dw)) return hipSuccess;
-        for (long long v = 0; v < q.V; v += q.piece) {
+        for (long long v = 0; v < q.V && q.grad; v += q.piece) {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
             const long long pld = up(n, 64);
             // (a vocabulary of one piece is packed already)
@@ -370,28 +370,54 @@ struct Call {
         m.t = t;
         return m;
     }
-    hipError_t single(const float* lse) const {
+    LossJoint joint_args(const LossMatrix& m, void* out, long long ldo) const {
+        LossJoint j{};
+        j.m = m;
+        j.temperature = (float)a.temperature;
+        j.lse = a.lse;
+        j.loss = loss_out();
+        j.ct = a.ct;
+        j.count = at<int>(q.count);
+        j.parts = q.parts;
+        j.out = out;
+        j.ldo = ldo;
+        j.flag = a.flag;
+        return j;
+    }
+    // the value of logits in memory, as far as the rows' sums: whole where one
+    // chunk has each row
+    hipError_t value_of(const LossMatrix& m, int slot) const {
+        const LossDone d{(float)a.temperature, lse_out(), loss_out()};
+        return loss_stats(m, at<float>(q.pm), at<float>(q.ps), at<float>(q.pa), slot, q.slots == 1 ? &d : nullptr, s);
+    }
+    hipError_t single(const float* lse) {
         const float* const x = (const float*)a.x;
         float* const z = at<float>(q.P);
         auto logits = [&](long long v, int n) {
             return gemm(product_z(q, a.tied, n), x, (const float*)a.w + (a.tied ? v * q.D : v), z, nullptr);
         };
-        if (q.value) {
+        // a vocabulary of one piece: its logits, then their cotangent in place
+        const LossMatrix whole = matrix(z, q.ldz, kF32, 0, q.V);
+        const bool once = q.value && q.grad && q.pieces == 1 && loss_joint_fits(whole);
+        if (once) {
+            LOSS_TRY(logits(0, q.V));
+            LOSS_TRY(loss_joint(joint_args(whole, z, q.ldz), s));
+        } else {
             int slot = 0;
-            for (long long v = 0; v < q.V; v += q.piece) {
+            for (long long v = 0; v < q.V && q.value; v += q.piece) {
                 const int n = (int)std::min<long long>(q.piece, q.V - v);
                 LOSS_TRY(logits(v, n));
-                LOSS_TRY(loss_stats(matrix(z, q.ldz, kF32, v, n), at<float>(q.pm), at<float>(q.ps), at<float>(q.pa), slot, s));
+                LOSS_TRY(value_of(matrix(z, q.ldz, kF32, v, n), slot));
                 slot += loss_chunks(q.rows, n);
             }
+            LOSS_TRY(rows_of());
         }
-        LOSS_TRY(rows_of());
-        if (!q.grad || (!a.dx && !a.dw)) return hipSuccess;
-        for (long long v = 0; v < q.V; v += q.piece) {
+        for (long long v = 0; v < q.V && q.grad; v += q.piece) {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
-            // (the logits of a vocabulary of one piece are still there)
-            if (!q.value || q.pieces > 1) LOSS_TRY(logits(v, n));
-            LOSS_TRY(loss_grad(matrix(z, q.ldz, kF32, v, n), lse, at<float>(q.coef), z, q.ldz, kF32, nullptr, s));
+            if (!once) {
+                LOSS_TRY(logits(v, n));
+                LOSS_TRY(loss_grad(matrix(z, q.ldz, kF32, v, n), lse, at<float>(q.coef), z, q.ldz, nullptr, s));
+            }
             float* const dx = (float*)a.dx;
             if (dx)
                 LOSS_TRY(gemm(product_dx(q, a.tied, n), z, (const float*)a.w + (a.tied ? v * q.D : v), dx, v ? dx : nullptr));
@@ -403,33 +429,31 @@ struct Call {
         return hipSuccess;
     }
 
-    hipError_t given(const float* lse) const {
+    hipError_t given(const float* lse) {
         LossMatrix m = matrix(a.x, q.V, q.st, 0, q.V);
-        if (q.value && q.grad && loss_joint_fits(m)) {
-            LossRows r = row_args();
-            r.slots = 0;
-            LOSS_TRY(loss_rows(r, s));
-            return loss_joint(m, (float)a.temperature, a.lse, loss_out(), at<float>(q.coef), a.dx, q.V, a.flag, s);
-        }
-        if (q.value) LOSS_TRY(loss_stats(m, at<float>(q.pm), at<float>(q.ps), at<float>(q.pa), 0, s));
+        if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, a.dx, q.V), s);
+        if (q.value) LOSS_TRY(value_of(m, 0));
         LOSS_TRY(rows_of());
         if (!q.grad) return hipSuccess;
-        return loss_grad(m, lse, at<float>(q.coef), a.dx, q.V, q.st, a.flag, s);
+        return loss_grad(m, lse, at<float>(q.coef), a.dx, q.V, a.flag, s);
     }
 
+    float* lse_out() const { return a.lse ? a.lse : at<float>(q.lse); }
     float* loss_out() const { return a.loss ? a.loss : at<float>(q.loss); }
     LossRows row_args() const {
         LossRows r{};
         r.pm = at<float>(q.pm);
         r.ps = at<float>(q.ps);
         r.pa = at<float>(q.pa);
-        r.slots = q.slots;
+        // (one chunk of logits in memory: the rows are done)
+        r.slots = q.slots == 1 && (!q.head || q.st == kF32) ? 0 : q.slots;
         r.t = t;
         r.rows = q.rows;
         r.temperature = (float)a.temperature;
         if (q.value) {
-            r.lse = a.lse ? a.lse : at<float>(q.lse);
+            r.lse = lse_out();
             r.loss = loss_out();
+            if (loss_rows_mean(q.rows)) r.mean = a.mean;
         }
         if (q.grad) {
             r.coef = at<float>(q.coef);
@@ -442,7 +466,13 @@ struct Call {
         r.parts = q.parts;
         return r;
     }
-    hipError_t rows_of() const { return loss_rows(row_args(), s); }
+    // the rows' sums joined, their cotangents' factors, and of few rows the mean
+    hipError_t rows_of() {
+        const LossRows r = row_args();
+        if (!r.slots && !r.coef && !r.mean) return hipSuccess;
+        mean_done = r.mean;
+        return loss_rows(r, s);
+    }
 
     hipError_t run() {
         LossPrep p{};
@@ -464,12 +494,12 @@ struct Call {
         t = LossTarget{p.col, p.p, p.ent, p.start, q.k, q.nblocks};
         if (q.rows) {
             LOSS_TRY(loss_prep(p, s));
-            const float* const lse = a.lse ? a.lse : at<float>(q.lse);
+            const float* const lse = lse_out();
             LOSS_TRY(!q.head ? given(lse) : q.st == kF32 ? single(lse) : half(lse));
         } else if (q.grad && q.head && a.dw) {
             LOSS_TRY(loss_zero(a.dw, (long long)q.D * q.V * q.esz, s));
         }
-        if (q.value && a.mean) LOSS_TRY(loss_mean(loss_out(), q.rows, p.count, q.parts, a.mean, s));
+        if (q.value && a.mean && !mean_done) LOSS_TRY(loss_mean(loss_out(), q.rows, p.count, q.parts, a.mean, s));
         return hipSuccess;
     }
 };
@@ -496,9 +526,11 @@ std::string loss_check(const presk_hip_loss& a, int what, bool head) {
     return "";
 }
 
+namespace {
+
 // The buffers of a checked call: their presence, alignment, and that no output
 // meets another buffer.
-std::string loss_check_buffers(const presk_hip_loss& a, int what, bool head) {
+std::string check_buffers(const presk_hip_loss& a, int what, bool head, size_t need) {
     const int st = storage_code(a.dtype);
     const char* const op = head ? "head loss" : "distillation";
     auto no = [&](const std::string& why) { return std::string("E10001: ") + op + ": " + why; };
@@ -537,15 +569,33 @@ std::string loss_check_buffers(const presk_hip_loss& a, int what, bool head) {
             if (&s != &o && o.out && s.p && o.p && s.bytes > 0 && o.bytes > 0 && (uintptr_t)s.p < (uintptr_t)o.p + o.bytes &&
                 (uintptr_t)o.p < (uintptr_t)s.p + s.bytes)
                 return no(std::string(o.name) + " meets " + s.name);
-    const size_t need = loss_workspace(a, what, head);
     if (a.work_bytes < need) return no("a workspace of " + std::to_string(a.work_bytes) + " bytes, " + std::to_string(need) + " needed");
     return "";
 }
 
-size_t loss_workspace(const presk_hip_loss& a, int what, bool head) { return std::max<size_t>(plan_of(a, what, head).total, 256); }
+size_t bytes_of(const Plan& q) { return std::max<size_t>(q.total, 256); }
+
+}  // namespace
+
+size_t loss_workspace(const presk_hip_loss& a, int what, bool head) { return bytes_of(plan_of(a, what, head)); }
+
+std::string loss_check_all(const presk_hip_loss& a, int what, bool head) {
+    std::string why = loss_check(a, what, head);
+    return why.empty() ? check_buffers(a, what, head, loss_workspace(a, what, head)) : why;
+}
 
 hipError_t loss_run(const presk_hip_loss& a, int what, bool head, hipStream_t s) {
     const Plan q = plan_of(a, what, head);
+    Call c{a, q, s, (char*)a.work, {}};
+    return c.run();
+}
+
+hipError_t loss_check_run(const presk_hip_loss& a, int what, bool head, hipStream_t s, std::string* why) {
+    *why = loss_check(a, what, head);
+    if (!why->empty()) return hipSuccess;
+    const Plan q = plan_of(a, what, head);
+    *why = check_buffers(a, what, head, bytes_of(q));
+    if (!why->empty()) return hipSuccess;
     Call c{a, q, s, (char*)a.work, {}};
     return c.run();
 }

@@ -12,13 +12,17 @@
 
 namespace presk {
 
-// What the ABI's arguments ask for, checked: "" or why not, the message
-// starting with its code.  `head`: of x . w, else of given logits.
+// What the ABI's arguments ask for, checked on the host: "" or why not, the
+// message starting with its code.  loss_check looks at the type and the sizes,
+// loss_check_all at the buffers and the workspace too.  `head`: of x . w, else
+// of given logits.
 std::string loss_check(const presk_hip_loss& a, int what, bool head);
-std::string loss_check_buffers(const presk_hip_loss& a, int what, bool head);
+std::string loss_check_all(const presk_hip_loss& a, int what, bool head);
 // the bytes of workspace a checked call needs
 size_t loss_workspace(const presk_hip_loss& a, int what, bool head);
+// the launches of a checked call, and with the check in front (`why` it was refused)
 hipError_t loss_run(const presk_hip_loss& a, int what, bool head, hipStream_t s);
+hipError_t loss_check_run(const presk_hip_loss& a, int what, bool head, hipStream_t s, std::string* why);
 
 // ---- what the kernels share -------------------------------------------------
 
@@ -112,7 +116,9 @@ struct LossRows {
     const float* most;
     int parts;
     float* scale;               // out (f16): the inverse of the factor in coef (null: none)
+    float* mean;                // {mean, count} or null: in the same launch where loss_rows_mean(rows)
 };
+bool loss_rows_mean(long long rows);
 hipError_t loss_rows(const LossRows& a, hipStream_t s);
 hipError_t loss_mean(const float* loss, long long rows, const int* count, int parts, float* mean, hipStream_t s);
 
@@ -126,18 +132,32 @@ struct LossMatrix {
     float c;
     LossTarget t;
 };
-// partials [chunk][rows] from slot0 on
+// partials [chunk][rows] from slot0 on; or, of one chunk, the rows' lse and loss
+// themselves (`done`, its outputs may be null)
+struct LossDone {
+    float temperature;
+    float *lse, *loss;
+};
 int loss_chunks(long long rows, int cols);
-hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, hipStream_t s);
-// the logits' cotangent, coef * (softmax - target), stored as `to`
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, int to,
-                     unsigned* flag, hipStream_t s);
-
-// value and cotangent of whole rows, each read once and held in registers:
-// lse, loss (either may be null) and coef * (softmax - target) stored as m.storage
+hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s);
+// the logits' cotangent, coef * (softmax - target), in the logits' type (in place or not)
+hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag,
+                     hipStream_t s);
+// both of whole rows, each read once and held in registers: lse, loss (either
+// may be null) and the cotangent for ct, or for the mean over `count` (null ct)
+struct LossJoint {
+    LossMatrix m;
+    float temperature;
+    float *lse, *loss;
+    const float* ct;
+    const int* count;
+    int parts;
+    void* out;
+    long long ldo;
+    unsigned* flag;
+};
 bool loss_joint_fits(const LossMatrix& m);
-hipError_t loss_joint(const LossMatrix& m, float temperature, float* lse, float* loss, const float* coef, void* out, long long ldo,
-                      unsigned* flag, hipStream_t s);
+hipError_t loss_joint(const LossJoint& a, hipStream_t s);
 
 // [rows][cols] 16-bit from row stride lds to ldd, zero up to padded columns
 hipError_t loss_pack(const void* src, long long lds, long long rows, int cols, void* dst, int ldd, hipStream_t s);

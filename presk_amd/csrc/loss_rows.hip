@@ -43,21 +43,42 @@ __device__ __forceinline__ typename Elem<ST>::S narrow(float v, bool& ovf) {
     }
 }
 
-// 16 bytes at any alignment of the element
-template <int ST>
-struct Vec {
-    typename Elem<ST>::S e[Elem<ST>::V];
-};
-template <int ST>
-__device__ __forceinline__ Vec<ST> load_vec(const typename Elem<ST>::S* p) {
-    Vec<ST> v;
+// 16 bytes of a row, at any alignment of the element, as four words
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 load_vec(const void* p) {
+    u32x4 v;
     __builtin_memcpy(&v, p, 16);
     return v;
 }
+__device__ __forceinline__ void store_vec(void* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
+// element e of a vector
 template <int ST>
-__device__ __forceinline__ void store_vec(typename Elem<ST>::S* p, const Vec<ST>& v) {
-    __builtin_memcpy(p, &v, 16);
+__device__ __forceinline__ float elem(u32x4 v, int e) {
+    if constexpr (ST == kF32) return pk_float(v[e]);
+    else return widen<ST>((unsigned short)(e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xffffu));
 }
+template <int ST>
+__device__ __forceinline__ void set_elem(u32x4& v, int e, typename Elem<ST>::S x) {
+    if constexpr (ST == kF32) v[e] = pk_bits(x);
+    else if (e & 1) v[e / 2] |= (unsigned)x << 16;
+    else v[e / 2] = x;
+}
+// A row's vectors start where its address is a multiple of 16: `head`
+// elements come before, `rest` after the `n` vectors.  Those at the ends go to
+// threads 0 .. head + rest - 1, one each (at most 14).
+template <int ST>
+struct Split {
+    int head, n, rest;
+    __device__ __forceinline__ Split(const void* row, int cols) {
+        constexpr int V = Elem<ST>::V, B = 16 / V;
+        head = (int)(((16 - ((size_t)row & 15)) & 15) / B);
+        if (head > cols) head = cols;
+        n = (cols - head) / V;
+        rest = cols - head - n * V;
+    }
+    __device__ __forceinline__ int edge(int t) const { return t < head ? t : head + n * Elem<ST>::V + t - head; }
+    __device__ __forceinline__ int edges() const { return head + rest; }
+};
 
 __device__ __forceinline__ float exp2_of(float z, float c, float base) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -base)); }
 // what is subtracted from u where the largest is m: a row of -inf has sum 0
@@ -116,60 +137,73 @@ __global__ void __launch_bounds__(256) prep_one_kernel(LossPrep a) {
 
 // A teacher's slots: the softmax of those in use, sorted by column (a slot's
 // place is how many come before it: columns below its own, or its own at an
-// earlier slot, so the order is one whatever runs first).
-template <int ST, int G>
+// earlier slot, so the order is one whatever runs first).  G threads a row, E
+// slots a thread.
+template <int ST, int G, int E>
 __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
-    constexpr int R = 256 / G, KM = G == 64 ? 64 : 1024;
-    __shared__ int in[R][KM], sorted[R][KM];
-    __shared__ float red[4];
-    __shared__ float tally[R][2];
+    constexpr int R = 256 / G, KM = G * E;
+    __shared__ __attribute__((aligned(16))) int in[R][KM], sorted[R][KM];
+    __shared__ float red[4], tally[R][2];
     const int g = threadIdx.x / G, t = threadIdx.x % G, k = a.top;
+    typedef typename Elem<ST>::S S;
     float n = 0.f, most = 0.f;
     for (long long r0 = (long long)blockIdx.x * R; r0 < a.rows; r0 += (long long)gridDim.x * R) {
         const long long r = r0 + g;
         const bool live = r < a.rows;
-        typedef typename Elem<ST>::S S;
-        auto logit = [&](int j) { return widen<ST>(((const S*)a.teacher)[r * k + j]); };
-        float top = -INFINITY, used = 0.f, bad = 0.f;
-        for (int j = t; j < k; j += G) {
-            int col = kUnused;
-            if (live) {
+        float x[E];
+        int col[E];
+        float top = -INFINITY, seen = 0.f;      // seen: 1 a used slot, 2 one outside the vocabulary
+#pragma unroll
+        for (int q = 0; q < E; ++q) {
+            const int j = t + q * G;
+            col[q] = kUnused;
+            x[q] = -INFINITY;
+            if (live && j < k) {
                 const long long i = a.index[r * k + j];
-                const float x = logit(j);
-                if (i >= 0 && x != -INFINITY) {
-                    col = i >= a.vocab ? kOutside : (int)i;
-                    if (i >= a.vocab) bad = 1.f;
-                    used = 1.f;
-                    top = x > top || x != x ? x : top;
+                x[q] = widen<ST>(((const S*)a.teacher)[r * k + j]);
+                if (i >= 0 && x[q] != -INFINITY) {
+                    col[q] = i >= a.vocab ? kOutside : (int)i;
+                    seen = fmaxf(seen, i >= a.vocab ? 2.f : 1.f);
+                    top = fmaxf(top, x[q]);     // (a NaN comes back in its term)
                 }
             }
-            in[g][j] = col;
+            in[g][j] = col[q];
         }
-        // (a NaN among them is lost to the maximum and comes back in its term)
-        top = all_of<G>(top, red, max_f);
-        used = all_of<G>(used, red, max_f);
-        bad = all_of<G>(bad, red, max_f);
-        __syncthreads();
+        top = all_of<G>(top, red, max_f) * a.c;
+        seen = all_of<G>(seen, red, max_f);
+        const float base = base_of(top);
         float total = 0.f;
-        for (int j = t; j < k; j += G)
-            if (in[g][j] != kUnused) total += exp2_of(logit(j), a.c, top * a.c);
-        total = all_of<G>(total, red, add_f);
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+            if (col[q] != kUnused) total += exp2_of(x[q], a.c, base);
+        total = all_of<G>(total, red, add_f);   // (and the barrier that `in` needs)
+        if constexpr (G == 64) __syncthreads();
+        int at[E];
+#pragma unroll
+        for (int q = 0; q < E; ++q) at[q] = 0;
+        for (int j = 0; j < k; j += 4) {
+            const int4 c4 = *(const int4*)&in[g][j];    // (past k: unused, after every slot in use)
+            const int c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int q = 0; q < E; ++q) at[q] += c[e] < col[q] || (c[e] == col[q] && j + e < t + q * G);
+        }
         const float l2 = __builtin_amdgcn_logf(total);
         float ent = 0.f;
-        for (int j = t; j < k; j += G) {
-            const int col = in[g][j];
-            int at = 0;
-            for (int q = 0; q < k; ++q) at += in[g][q] < col || (in[g][q] == col && q < j);
+#pragma unroll
+        for (int q = 0; q < E; ++q) {
+            if (t + q * G >= k) continue;
             float p = 0.f;
-            if (col != kUnused) {
-                const float u = __builtin_fmaf(logit(j), a.c, -(top * a.c));
+            if (col[q] != kUnused) {
+                const float u = __builtin_fmaf(x[q], a.c, -base);
                 p = __builtin_amdgcn_exp2f(u) / total;
                 if (p != 0.f) ent += p * ((u - l2) * kLn2);
             }
-            sorted[g][at] = col;
+            sorted[g][at[q]] = col[q];
             if (live) {
-                a.col[r * k + at] = col;
-                a.p[r * k + at] = p;
+                a.col[r * k + at[q]] = col[q];
+                a.p[r * k + at[q]] = p;
             }
         }
         ent = all_of<G>(ent, red, add_f);
@@ -186,8 +220,8 @@ __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
             }
         }
         if (live && t == 0) {
-            a.ent[r] = bad != 0.f ? NAN : ent;
-            if (used != 0.f) {
+            a.ent[r] = seen > 1.f ? NAN : ent;
+            if (seen != 0.f) {
                 n += 1.f;
                 if (a.ct) most = fmaxf(most, fabsf(a.ct[r]));
             }
@@ -211,43 +245,54 @@ __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
 
 // ---- a row's partial sums joined ------------------------------------------------
 
-// 32 rows a workgroup, eight threads a row, each over every eighth slot.
-__global__ void __launch_bounds__(256) rows_kernel(LossRows a) {
-    __shared__ float red[4];
-    const int q = threadIdx.x & 7;
-    const long long r = (long long)blockIdx.x * 32 + threadIdx.x / 8;
+// A row's loss from its largest u, its sum and its target's part: the largest
+// against the target's before anything is added to it.
+__device__ __forceinline__ float row_loss(const LossTarget& t, long long r, float temperature, float m, float log_s, float ta) {
+    if (t.col[r * t.k] == kUnused) return 0.f;
+    return temperature * temperature * (t.ent[r] + __builtin_fmaf(m - ta, kLn2, log_s));
+}
+
+// the mean of `rows` losses over `n` rows by T threads, in f64 (their order is
+// the strides', then a tree)
+template <int T>
+__device__ __forceinline__ void write_mean(const float* loss, long long rows, int n, float* mean) {
+    __shared__ double red[T / 64];
+    double s = 0.0;
+    for (long long r = threadIdx.x; r < rows; r += T) s += (double)loss[r];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < T / 64; ++w) s += red[w];
+        mean[0] = n ? (float)(s / n) : 0.f;
+        mean[1] = (float)n;
+    }
+}
+
+// T / G rows a workgroup, G threads a row, each over every G-th slot; with a
+// mean one workgroup has all the rows.
+template <int T, int G>
+__global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
+    __shared__ float red[T / 64];
+    const int q = threadIdx.x % G;
+    const long long r = (long long)blockIdx.x * (T / G) + threadIdx.x / G;
     const bool live = r < a.rows;
     float count = 0.f, most = 0.f;
-    if (a.coef) {
-        if (a.count) {
-            for (int i = threadIdx.x; i < a.parts; i += 256) {
-                count += (float)a.count[i];
-                most = fmaxf(most, a.most[i]);
-            }
-            count = all_of<256>(count, red, add_f);
-            most = all_of<256>(most, red, max_f);
+    if (a.coef || a.mean) {
+        for (int i = threadIdx.x; i < a.parts; i += T) {
+            count += (float)a.count[i];
+            most = fmaxf(most, a.most[i]);
         }
-        if (a.mean_in) count = a.mean_in[1];
-    }
-    float m = -INFINITY, s = 0.f, ta = 0.f;
-    if (live) {
-        for (int p = q; p < a.slots; p += 8) {
-            const long long at = (long long)p * a.rows + r;
-            join(m, s, a.pm[at], a.ps[at]);
-            ta += a.pa[at];
-        }
-    }
-#pragma unroll
-    for (int d = 1; d < 8; d *= 2) {
-        const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
-        join(m, s, m2, s2);
-        ta += __shfl_xor(ta, d);
+        count = all_of<T>(count, red, add_f);
+        most = all_of<T>(most, red, max_f);
     }
     if (a.coef) {
+        const float n = a.mean_in ? a.mean_in[1] : count;
         // f16: a power of two brings the largest cotangent to 2^14 .. 2^15
         int e = 0;
         if (a.scale) {
-            const float top = (a.ct ? most : 1.f / fmaxf(count, 1.f)) * a.temperature;
+            const float top = (a.ct ? most : 1.f / fmaxf(n, 1.f)) * a.temperature;
             if (top > 0.f && top < INFINITY) {
                 int x;
                 (void)frexpf(top, &x);
@@ -258,96 +303,99 @@ __global__ void __launch_bounds__(256) rows_kernel(LossRows a) {
         if (live && q == 0) {
             float f = 0.f;
             if (a.t.col[r * a.t.k] != kUnused) {
-                f = (a.ct ? a.ct[r] : 1.f / fmaxf(count, 1.f)) * a.temperature;
+                f = (a.ct ? a.ct[r] : 1.f / fmaxf(n, 1.f)) * a.temperature;
                 if (a.scale) f = ldexpf(f, e);
                 f += a.t.ent[r] != a.t.ent[r] ? NAN : 0.f;
             }
             a.coef[r] = f;
         }
     }
-    if (live && q == 0 && a.slots) {
-        const float ls = pk_logf(s);
-        if (a.lse) a.lse[r] = __builtin_fmaf(m, kLn2, ls);
-        if (a.loss) {
-            // the largest logit against the target's before anything is added to it
-            const float l = a.t.ent[r] + (__builtin_fmaf(m - ta, kLn2, ls));
-            a.loss[r] = a.t.col[r * a.t.k] == kUnused ? 0.f : a.temperature * a.temperature * l;
+    if (a.slots) {
+        float m = -INFINITY, s = 0.f, ta = 0.f;
+        if (live)
+            for (int p = q; p < a.slots; p += G) {
+                const long long at = (long long)p * a.rows + r;
+                join(m, s, a.pm[at], a.ps[at]);
+                ta += a.pa[at];
+            }
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) {
+            const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+            join(m, s, m2, s2);
+            ta += __shfl_xor(ta, d);
         }
+        if (live && q == 0) {
+            const float ls = pk_logf(s);
+            if (a.lse) a.lse[r] = __builtin_fmaf(m, kLn2, ls);
+            if (a.loss) a.loss[r] = row_loss(a.t, r, a.temperature, m, ls, ta);
+        }
+    }
+    if (a.mean) {
+        __threadfence_block();
+        __syncthreads();
+        write_mean<T>(a.loss, a.rows, (int)count, a.mean);
     }
 }
 
 __global__ void __launch_bounds__(1024) mean_kernel(const float* loss, long long rows, const int* count, int parts, float* mean) {
-    __shared__ double red[16];
-    __shared__ int nred[16];
-    double s = 0.0;
+    __shared__ int red[16];
     int n = 0;
-    for (long long r = threadIdx.x; r < rows; r += 1024) s += (double)loss[r];
     for (int i = threadIdx.x; i < parts; i += 1024) n += count[i];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        s += __shfl_xor(s, d);
-        n += __shfl_xor(n, d);
-    }
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = s;
-        nred[threadIdx.x >> 6] = n;
-    }
+    for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) {
-            s += red[w];
-            n += nred[w];
-        }
-        mean[0] = n ? (float)(s / n) : 0.f;
-        mean[1] = (float)n;
-    }
+    n = 0;
+    for (int w = 0; w < 16; ++w) n += red[w];
+    write_mean<1024>(loss, rows, n, mean);
 }
 
 // ---- logits in memory -------------------------------------------------------------
 
-// Columns [lo, hi) of row r by G threads: the largest, the sum, the target's part.
+// Columns [lo, hi) of row r by G threads: the largest u, the sum, the target's part.
 template <int ST, int G>
 __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int lo, int hi, int t, float* red, float& m, float& s,
                                           float& ta) {
     typedef typename Elem<ST>::S S;
     constexpr int V = Elem<ST>::V;
     const S* const z = (const S*)a.z + r * a.ld;
+    const Split<ST> sp(z + lo, hi - lo);
+    const S* const w = z + lo + sp.head;
     m = -INFINITY;
     s = 0.f;
     ta = 0.f;
-    const int whole = lo + (hi - lo) / V * V;
+    for (int e = t; e < a.t.k; e += G) {
+        const int col = a.t.col[r * a.t.k + e] - a.col0;
+        const float p = a.t.p[r * a.t.k + e];
+        if (col >= lo && col < hi && p != 0.f) ta += p * (widen<ST>(z[col]) * a.c);
+    }
     // four vectors in flight, their largest first, then one rescale for all
     constexpr int U = 4;
-    for (int i = lo + t * V; i < whole; i += U * G * V) {
-        Vec<ST> v[U];
+    for (int i = t; i < sp.n; i += U * G) {
+        u32x4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * G * V < whole) v[u] = load_vec<ST>(z + i + u * G * V);
+            if (i + u * G < sp.n) v[u] = load_vec(w + (long long)(i + u * G) * V);
         float x = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * G * V < whole)
+            if (i + u * G < sp.n)
 #pragma unroll
-                for (int e = 0; e < V; ++e) x = fmaxf(x, widen<ST>(v[u].e[e]));
+                for (int e = 0; e < V; ++e) x = fmaxf(x, elem<ST>(v[u], e));
         const float n = fmaxf(m, x * a.c), b = base_of(n);
         s *= __builtin_amdgcn_exp2f(m - b);
         m = n;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * G * V < whole)
+            if (i + u * G < sp.n)
 #pragma unroll
-                for (int e = 0; e < V; ++e) s += exp2_of(widen<ST>(v[u].e[e]), a.c, b);
+                for (int e = 0; e < V; ++e) s += exp2_of(elem<ST>(v[u], e), a.c, b);
     }
-    if (whole + t < hi) {
-        const float x = widen<ST>(z[whole + t]);
+    if (t < sp.edges()) {
+        const float x = widen<ST>(z[lo + sp.edge(t)]);
         const float n = fmaxf(m, x * a.c), b = base_of(n);
         s = s * __builtin_amdgcn_exp2f(m - b) + exp2_of(x, a.c, b);
         m = n;
-    }
-    for (int e = t; e < a.t.k; e += G) {
-        const int col = a.t.col[r * a.t.k + e] - a.col0;
-        const float p = a.t.p[r * a.t.k + e];
-        if (col >= lo && col < hi && p != 0.f) ta += p * (widen<ST>(z[col]) * a.c);
     }
     const float top = all_of<G>(m, red, max_f);
     s *= __builtin_amdgcn_exp2f(m - base_of(top));
@@ -358,7 +406,8 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
 
 // G 64: four rows a workgroup, a wave each; 256: a row's chunk a workgroup
 template <int ST, int G>
-__global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, float* ps, float* pa, int slot0, int chunk) {
+__global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, float* ps, float* pa, int slot0, int chunk,
+                                                    LossDone done, bool finish) {
     __shared__ float red[4];
     const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
     if (r >= a.rows) return;    // (whole waves; with G 256 never)
@@ -366,7 +415,12 @@ __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, flo
     const int lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
     float m, s, ta;
     row_stats<ST, G>(a, r, lo, hi, t, red, m, s, ta);
-    if (t == 0) {
+    if (t != 0) return;
+    if (finish) {
+        const float ls = pk_logf(s);
+        if (done.lse) done.lse[r] = __builtin_fmaf(m, kLn2, ls);
+        if (done.loss) done.loss[r] = row_loss(a.t, r, done.temperature, m, ls, ta);
+    } else {
         const long long at = (long long)(slot0 + blockIdx.y) * a.rows + r;
         pm[at] = m;
         ps[at] = s;
@@ -374,8 +428,8 @@ __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, flo
     }
 }
 
-// The cotangent of one target slot's column: `e` is the first slot that names
-// it; the weights of those after it that name it too are added in order.
+// Whether slot e is the first that names its column; the weights of those
+// after it that name it too are added in order.
 __device__ __forceinline__ bool first_of(const LossTarget& t, long long at, int e, float& p) {
     const int col = t.col[at + e];
     if (e > 0 && t.col[at + e - 1] == col) return false;
@@ -384,148 +438,156 @@ __device__ __forceinline__ bool first_of(const LossTarget& t, long long at, int 
     return true;
 }
 
-// out = coef * (2^(u - lse) - t).  One target a row is met as its column
-// passes; several are written after the row's other columns, by a thread each,
-// once the stores of this workgroup (or wave) have reached memory.
-template <int SI, int SO, int G>
+// c * (2^(u - l) - p), 0 where c is 0 whatever the logit
+template <int ST>
+__device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, float l, float p, float c, bool& ovf) {
+    return narrow<ST>(c == 0.f ? 0.f : (exp2_of(z, cf, l) - p) * c, ovf);
+}
+
+// out = coef * (2^(u - lse) - t).  The target's columns are written after the
+// row's others, by a thread each, once the stores of this workgroup (or wave)
+// have reached memory.
+template <int ST, int G>
 __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* lse, const float* coef, void* out, long long ldo,
                                                    unsigned* flag, int chunk) {
-    typedef typename Elem<SI>::S S;
-    typedef typename Elem<SO>::S T;
-    constexpr int V = SI == kF32 ? 4 : 8;
+    typedef typename Elem<ST>::S S;
+    constexpr int V = Elem<ST>::V;
     const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
     if (r >= a.rows) return;
     const int t = threadIdx.x % G, lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
-    const S* const z = (const S*)a.z + r * a.ld;
-    T* const o = (T*)out + r * ldo;
+    const S* const z = (const S*)a.z + r * a.ld + lo;
+    S* const o = (S*)out + r * ldo + lo;
     const float c = coef[r], l = lse[r] * kLog2e;
-    const int k = a.t.k, one = k == 1 ? a.t.col[r] - a.col0 : -1;
+    const int k = a.t.k, first = a.col0 + lo, n = hi - lo;
     const long long at = r * k;
     bool ovf = false;
-    // at most four slots a thread (1024 by 256; a wave has 64 or 1024 by 16)
+    // the logits of the target's columns, before the row is written (in place)
     constexpr int E = 1024 / G;
     float zt[E];
-    if (k > 1)
-        for (int q = 0; q < E; ++q) {
-            const int e = t + q * G;
-            zt[q] = 0.f;
-            if (e < k) {
-                const int col = a.t.col[at + e] - a.col0;
-                if (col >= lo && col < hi) zt[q] = widen<SI>(z[col]);
-            }
-        }
-    auto value = [&](float x, int col) {
-        const float g = exp2_of(x, a.c, l) - (col == one ? a.t.p[at] : 0.f);
-        return narrow<SO>(c == 0.f ? 0.f : g * c, ovf);
-    };
-    if (k > 1) {
-        // every thread's logits of the targets are read before the row is written
-        __builtin_amdgcn_s_waitcnt(0);
-        if constexpr (G > 64) __syncthreads();
+    for (int q = 0; q < E && t + q * G < k; ++q) {
+        const int col = a.t.col[at + t + q * G] - first;
+        zt[q] = col >= 0 && col < n ? widen<ST>(z[col]) : 0.f;
     }
-    const int whole = lo + (hi - lo) / V * V;
-    for (int i = lo + t * V; i < whole; i += G * V) {
-        const Vec<SI> v = load_vec<SI>(z + i);
-        struct { T e[V]; } w;
+    __builtin_amdgcn_s_waitcnt(0);
+    if constexpr (G > 64) __syncthreads();
+    const Split<ST> sp(z, n);
+    constexpr int U = 2;
+    for (int i = t; i < sp.n; i += U * G) {
+        u32x4 v[U];
 #pragma unroll
-        for (int e = 0; e < V; ++e) w.e[e] = value(widen<SI>(v.e[e]), i + e);
-        __builtin_memcpy(o + i, &w, sizeof w);
+        for (int u = 0; u < U; ++u)
+            if (i + u * G < sp.n) v[u] = load_vec(z + sp.head + (long long)(i + u * G) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * G < sp.n) {
+                u32x4 w{};
+#pragma unroll
+                for (int e = 0; e < V; ++e) set_elem<ST>(w, e, cotangent<ST>(elem<ST>(v[u], e), a.c, l, 0.f, c, ovf));
+                store_vec(o + sp.head + (long long)(i + u * G) * V, w);
+            }
     }
-    if (whole + t < hi) o[whole + t] = value(widen<SI>(z[whole + t]), whole + t);
-    if (k > 1) {
-        __builtin_amdgcn_s_waitcnt(0);
-        if constexpr (G > 64) __syncthreads();
-        for (int q = 0; q < E; ++q) {
-            const int e = t + q * G;
-            if (e >= k) break;
-            const int col = a.t.col[at + e] - a.col0;
-            float p;
-            if (col >= lo && col < hi && first_of(a.t, at, e, p))
-                o[col] = narrow<SO>(c == 0.f ? 0.f : (exp2_of(zt[q], a.c, l) - p) * c, ovf);
-        }
+    if (t < sp.edges()) o[sp.edge(t)] = cotangent<ST>(widen<ST>(z[sp.edge(t)]), a.c, l, 0.f, c, ovf);
+    __builtin_amdgcn_s_waitcnt(0);
+    if constexpr (G > 64) __syncthreads();
+    for (int q = 0; q < E && t + q * G < k; ++q) {
+        const int e = t + q * G, col = a.t.col[at + e] - first;
+        float p;
+        if (col >= 0 && col < n && first_of(a.t, at, e, p)) o[col] = cotangent<ST>(zt[q], a.c, l, p, c, ovf);
     }
-    if (SO == kF16 && ovf && flag) atomicOr(flag, 1u);
+    if (ST == kF16 && ovf && flag) atomicOr(flag, 1u);
 }
 
-// Whole rows, read once: R vectors a thread of G.
-template <int ST, int G, int R>
-__global__ void __launch_bounds__(G) joint_kernel(LossMatrix a, float temperature, float* lse, float* loss, const float* coef,
-                                                  void* out, long long ldo, unsigned* flag) {
+// Whole rows, read once: G threads a row (64: four rows a workgroup), R
+// vectors and E slots of the target each.
+template <int ST, int G, int R, int E>
+__global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kernel(LossJoint a) {
     typedef typename Elem<ST>::S S;
-    constexpr int V = Elem<ST>::V;
-    __shared__ float red[G / 64];
-    const long long r = blockIdx.x;
-    const int t = threadIdx.x, k = a.t.k, nv = a.cols / V, rest = a.cols - nv * V;
-    const S* const z = (const S*)a.z + r * a.ld;
+    constexpr int V = Elem<ST>::V, T = G < 256 ? 256 : G;
+    __shared__ float red[T / 64];
+    const LossTarget& tg = a.m.t;
+    const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
+    if (r >= a.m.rows) return;  // (whole waves; with more than one a row never)
+    const int t = threadIdx.x % G, k = tg.k, n = a.m.cols;
+    const S* const z = (const S*)a.m.z + r * a.m.ld;
     const long long at = r * k;
-    Vec<ST> v[R];
+    const float cf = a.m.c;
+    const Split<ST> sp(z, n);
+    u32x4 v[R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (t + i * G < nv) v[i] = load_vec<ST>(z + (long long)(t + i * G) * V);
-    const bool tail = t < rest;
-    const float last = tail ? widen<ST>(z[nv * V + t]) : -INFINITY;
-    constexpr int E = (1024 + G - 1) / G;
+        if (t + i * G < sp.n) v[i] = load_vec(z + sp.head + (long long)(t + i * G) * V);
+    const bool edge = t < sp.edges();
+    const float last = edge ? widen<ST>(z[sp.edge(t)]) : -INFINITY;
     float zt[E], ta = 0.f;
 #pragma unroll
     for (int q = 0; q < E; ++q) {
-        const int e = t + q * G;
         zt[q] = 0.f;
-        if (e < k) {
-            const int col = a.t.col[at + e];
-            const float p = a.t.p[at + e];
-            if (col < a.cols) {
+        if (t + q * G < k) {
+            const int col = tg.col[at + t + q * G];
+            const float p = tg.p[at + t + q * G];
+            if (col < n) {
                 zt[q] = widen<ST>(z[col]);
-                if (p != 0.f) ta += p * (zt[q] * a.c);
+                if (p != 0.f) ta += p * (zt[q] * cf);
             }
         }
     }
+    float c = a.temperature;
+    if (a.ct) {
+        c *= a.ct[r];
+    } else {
+        float count = 0.f;
+        for (int i = t; i < a.parts; i += G) count += (float)a.count[i];
+        c *= 1.f / fmaxf(all_of<G>(count, red, add_f), 1.f);
+    }
+    if (tg.col[at] == kUnused) c = 0.f;
+    else if (tg.ent[at / k] != tg.ent[at / k]) c = NAN;
     float m = last;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (t + i * G < nv)
+        if (t + i * G < sp.n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) m = fmaxf(m, widen<ST>(v[i].e[e]));
-    m = all_of<G>(m, red, max_f) * a.c;
+            for (int e = 0; e < V; ++e) m = fmaxf(m, elem<ST>(v[i], e));
+    // (every load of this thread has landed before the barriers below, and so
+    // before any thread writes the row: the output may be the input)
+    __builtin_amdgcn_s_waitcnt(0);
+    m = all_of<G>(m, red, max_f) * cf;
     const float b = base_of(m);
-    float s = tail ? exp2_of(last, a.c, b) : 0.f;
+    float s = edge ? exp2_of(last, cf, b) : 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (t + i * G < nv)
+        if (t + i * G < sp.n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += exp2_of(widen<ST>(v[i].e[e]), a.c, b);
+            for (int e = 0; e < V; ++e) s += exp2_of(elem<ST>(v[i], e), cf, b);
     s = all_of<G>(s, red, add_f);
     ta = all_of<G>(ta, red, add_f);
     const float ls = pk_logf(s), l = __builtin_fmaf(m, kLn2, ls);
     if (t == 0) {
-        if (lse) lse[r] = l;
-        if (loss)
-            loss[r] = a.t.col[at] == kUnused ? 0.f : temperature * temperature * (a.t.ent[r] + __builtin_fmaf(m - ta, kLn2, ls));
+        if (a.lse) a.lse[r] = l;
+        if (a.loss) a.loss[r] = row_loss(tg, r, a.temperature, m, ls, ta);
     }
-    const float c = coef[r], l2 = l * kLog2e;
-    S* const o = (S*)out + r * ldo;
+    const float l2 = l * kLog2e;
+    S* const o = (S*)a.out + r * a.ldo;
     bool ovf = false;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (t + i * G < nv) {
-            Vec<ST> w;
+        if (t + i * G < sp.n) {
+            u32x4 w{};
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                w.e[e] = narrow<ST>(c == 0.f ? 0.f : exp2_of(widen<ST>(v[i].e[e]), a.c, l2) * c, ovf);
-            store_vec<ST>(o + (long long)(t + i * G) * V, w);
+            for (int e = 0; e < V; ++e) set_elem<ST>(w, e, cotangent<ST>(elem<ST>(v[i], e), cf, l2, 0.f, c, ovf));
+            store_vec(o + sp.head + (long long)(t + i * G) * V, w);
         }
-    if (tail) o[nv * V + t] = narrow<ST>(c == 0.f ? 0.f : exp2_of(last, a.c, l2) * c, ovf);
+    if (edge) o[sp.edge(t)] = cotangent<ST>(last, cf, l2, 0.f, c, ovf);
     __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+    if constexpr (G > 64) __syncthreads();
 #pragma unroll
     for (int q = 0; q < E; ++q) {
         const int e = t + q * G;
         if (e >= k) break;
-        const int col = a.t.col[at + e];
+        const int col = tg.col[at + e];
         float p;
-        if (col < a.cols && first_of(a.t, at, e, p))
-            o[col] = narrow<ST>(c == 0.f ? 0.f : (exp2_of(zt[q], a.c, l2) - p) * c, ovf);
+        if (col < n && first_of(tg, at, e, p)) o[col] = cotangent<ST>(zt[q], cf, l2, p, c, ovf);
     }
-    if (ST == kF16 && ovf && flag) atomicOr(flag, 1u);
+    if (ST == kF16 && ovf && a.flag) atomicOr(a.flag, 1u);
 }
 
 // ---- copies ------------------------------------------------------------------------
@@ -583,51 +645,63 @@ __global__ void __launch_bounds__(256) join_kernel(LossGemm g) {
 
 unsigned blocks_of(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 16384); }
 
-template <int ST>
-hipError_t stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, int chunks, int chunk, hipStream_t s) {
-    if (m.cols <= 1024)
-        stats_kernel<ST, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, pm, ps, pa, slot0, m.cols);
-    else
-        stats_kernel<ST, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, pm, ps, pa, slot0, chunk);
-    return hipGetLastError();
-}
-
-template <int SI, int SO>
-hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag, int chunks,
-                int chunk, hipStream_t s) {
-    if (m.cols <= 1024)
-        grad_kernel<SI, SO, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, lse, coef, out, ldo, flag, m.cols);
-    else
-        grad_kernel<SI, SO, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, lse, coef, out, ldo, flag, chunk);
-    return hipGetLastError();
-}
-
 // a chunk's columns: whole vectors of a workgroup
 int chunk_cols(int cols, int chunks) { return ((cols + chunks - 1) / chunks + 2047) / 2048 * 2048; }
 
 template <int ST>
-hipError_t joint(const LossMatrix& m, float temperature, float* lse, float* loss, const float* coef, void* out, long long ldo,
-                 unsigned* flag, hipStream_t s) {
-    const int nv = m.cols / Elem<ST>::V;
-    const unsigned n = (unsigned)m.rows;
-    if (nv <= 256 * 4) joint_kernel<ST, 256, 4><<<n, 256, 0, s>>>(m, temperature, lse, loss, coef, out, ldo, flag);
-    else if (nv <= 512 * 8) joint_kernel<ST, 512, 8><<<n, 512, 0, s>>>(m, temperature, lse, loss, coef, out, ldo, flag);
-    else if (nv <= 1024 * 8) joint_kernel<ST, 1024, 8><<<n, 1024, 0, s>>>(m, temperature, lse, loss, coef, out, ldo, flag);
-    else joint_kernel<ST, 1024, 16><<<n, 1024, 0, s>>>(m, temperature, lse, loss, coef, out, ldo, flag);
+hipError_t stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s) {
+    const int chunks = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, chunks);
+    if (done && chunks > 1) return hipErrorInvalidValue;
+    const LossDone d = done ? *done : LossDone{};
+    if (m.cols <= 1024)
+        stats_kernel<ST, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, pm, ps, pa, slot0, m.cols, d, done);
+    else
+        stats_kernel<ST, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, pm, ps, pa, slot0, chunk, d, done);
+    return hipGetLastError();
+}
+
+template <int ST>
+hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag, hipStream_t s) {
+    const int chunks = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, chunks);
+    if (m.cols <= 1024)
+        grad_kernel<ST, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, lse, coef, out, ldo, flag, m.cols);
+    else
+        grad_kernel<ST, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, lse, coef, out, ldo, flag, chunk);
+    return hipGetLastError();
+}
+
+template <int ST, int G, int R>
+void joint_of(const LossJoint& a, unsigned grid, hipStream_t s) {
+    constexpr int T = G < 256 ? 256 : G;
+    if (a.m.t.k <= G) joint_kernel<ST, G, R, 1><<<grid, T, 0, s>>>(a);
+    else joint_kernel<ST, G, R, 1024 / G><<<grid, T, 0, s>>>(a);
+}
+
+template <int ST>
+hipError_t joint(const LossJoint& a, hipStream_t s) {
+    const int nv = a.m.cols / Elem<ST>::V;
+    const unsigned n = (unsigned)a.m.rows;
+    if (nv <= 64 * 4) joint_of<ST, 64, 4>(a, (n + 3) / 4, s);
+    else if (nv <= 256 * 4) joint_of<ST, 256, 4>(a, n, s);
+    else if (nv <= 512 * 8) joint_of<ST, 512, 8>(a, n, s);
+    else if (nv <= 1024 * 8) joint_of<ST, 1024, 8>(a, n, s);
+    else joint_of<ST, 1024, 16>(a, n, s);
     return hipGetLastError();
 }
 
 template <int ST>
 hipError_t prep(const LossPrep& a, unsigned grid, hipStream_t s) {
-    if (a.top <= 64) prep_top_kernel<ST, 64><<<grid, 256, 0, s>>>(a);
-    else prep_top_kernel<ST, 256><<<grid, 256, 0, s>>>(a);
+    if (a.top <= 64) prep_top_kernel<ST, 64, 1><<<grid, 256, 0, s>>>(a);
+    else if (a.top <= 128) prep_top_kernel<ST, 64, 2><<<grid, 256, 0, s>>>(a);
+    else if (a.top <= 256) prep_top_kernel<ST, 64, 4><<<grid, 256, 0, s>>>(a);
+    else prep_top_kernel<ST, 256, 4><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int loss_parts(long long rows, int top) {
-    const long long per = top == 0 ? 256 : top <= 64 ? 4 : 1;
+    const long long per = top == 0 ? 256 : top <= 256 ? 4 : 1;
     return (int)std::min<long long>((rows + per - 1) / per, kParts);
 }
 
@@ -646,9 +720,20 @@ hipError_t loss_prep(const LossPrep& a, hipStream_t s) {
     return hipErrorInvalidValue;
 }
 
+// few enough rows for one workgroup
+bool loss_rows_mean(long long rows) { return rows <= 128; }
+
 hipError_t loss_rows(const LossRows& a, hipStream_t s) {
     if (a.rows <= 0) return hipSuccess;
-    rows_kernel<<<(unsigned)((a.rows + 31) / 32), 256, 0, s>>>(a);
+    if (a.mean) {
+        if (!loss_rows_mean(a.rows) || !a.loss) return hipErrorInvalidValue;
+        if (a.rows <= 16) rows_kernel<1024, 64><<<1, 1024, 0, s>>>(a);
+        else rows_kernel<1024, 8><<<1, 1024, 0, s>>>(a);
+    } else if (a.rows <= 1024 && a.slots > 64) {
+        rows_kernel<256, 64><<<(unsigned)((a.rows + 3) / 4), 256, 0, s>>>(a);
+    } else {
+        rows_kernel<256, 8><<<(unsigned)((a.rows + 31) / 32), 256, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 
@@ -665,36 +750,35 @@ int loss_chunks(long long rows, int cols) {
     return (cols + chunk - 1) / chunk;
 }
 
-hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, hipStream_t s) {
+hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s) {
     if (m.rows <= 0 || m.cols <= 0) return hipSuccess;
-    const int n = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, n);
     switch (m.storage) {
-        case kF32: return stats<kF32>(m, pm, ps, pa, slot0, n, chunk, s);
-        case kBF16: return stats<kBF16>(m, pm, ps, pa, slot0, n, chunk, s);
-        case kF16: return stats<kF16>(m, pm, ps, pa, slot0, n, chunk, s);
+        case kF32: return stats<kF32>(m, pm, ps, pa, slot0, done, s);
+        case kBF16: return stats<kBF16>(m, pm, ps, pa, slot0, done, s);
+        case kF16: return stats<kF16>(m, pm, ps, pa, slot0, done, s);
     }
     return hipErrorInvalidValue;
 }
 
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, int to, unsigned* flag,
+hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag,
                      hipStream_t s) {
     if (m.rows <= 0 || m.cols <= 0) return hipSuccess;
-    const int n = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, n);
-    if (m.storage == kF32 && to == kF32) return grad<kF32, kF32>(m, lse, coef, out, ldo, flag, n, chunk, s);
-    if (m.storage == kBF16 && to == kBF16) return grad<kBF16, kBF16>(m, lse, coef, out, ldo, flag, n, chunk, s);
-    if (m.storage == kF16 && to == kF16) return grad<kF16, kF16>(m, lse, coef, out, ldo, flag, n, chunk, s);
+    switch (m.storage) {
+        case kF32: return grad<kF32>(m, lse, coef, out, ldo, flag, s);
+        case kBF16: return grad<kBF16>(m, lse, coef, out, ldo, flag, s);
+        case kF16: return grad<kF16>(m, lse, coef, out, ldo, flag, s);
+    }
     return hipErrorInvalidValue;
 }
 
 bool loss_joint_fits(const LossMatrix& m) { return m.cols / (m.storage == kF32 ? 4 : 8) <= 1024 * 16; }
 
-hipError_t loss_joint(const LossMatrix& m, float temperature, float* lse, float* loss, const float* coef, void* out, long long ldo,
-                      unsigned* flag, hipStream_t s) {
-    if (m.rows <= 0) return hipSuccess;
-    switch (m.storage) {
-        case kF32: return joint<kF32>(m, temperature, lse, loss, coef, out, ldo, flag, s);
-        case kBF16: return joint<kBF16>(m, temperature, lse, loss, coef, out, ldo, flag, s);
-        case kF16: return joint<kF16>(m, temperature, lse, loss, coef, out, ldo, flag, s);
+hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
+    if (a.m.rows <= 0) return hipSuccess;
+    switch (a.m.storage) {
+        case kF32: return joint<kF32>(a, s);
+        case kBF16: return joint<kBF16>(a, s);
+        case kF16: return joint<kF16>(a, s);
     }
     return hipErrorInvalidValue;
 }

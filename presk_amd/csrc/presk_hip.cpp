@@ -834,24 +834,21 @@ int presk_hip_batch_add_convert(presk_hip_batch* b, const void* src, const char*
 
 namespace {
 
-// a loss's arguments and buffers, checked
-int check_loss(const presk_hip_loss* a, int what, bool head) {
-    if (!a) return fail(PRESK_HIP_ERR, "E10001: null argument");
-    std::string why = loss_check(*a, what, head);
-    if (why.empty()) why = loss_check_buffers(*a, what, head);
-    if (why.empty()) return PRESK_HIP_OK;
+int refuse_loss(const std::string& why) {
     return fail(why.compare(0, 5, "E7005") == 0 ? PRESK_HIP_REFUSED : PRESK_HIP_ERR, why);
 }
 
 int run_loss(const presk_hip_loss* a, int what, bool head, void* stream) {
-    if (int rc = check_loss(a, what, head)) return rc;
-    hipError_t e = loss_run(*a, what, head, (hipStream_t)stream);
+    if (!a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    std::string why;
+    hipError_t e = loss_check_run(*a, what, head, (hipStream_t)stream, &why);
+    if (!why.empty()) return refuse_loss(why);
     return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, head ? "head loss" : "distillation");
 }
 
 int add_loss(presk_hip_batch* b, const presk_hip_loss* a, int what, bool head) {
-    if (!b) return fail(PRESK_HIP_ERR, "E10001: null argument");
-    if (int rc = check_loss(a, what, head)) return rc;
+    if (!b || !a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = loss_check_all(*a, what, head); !why.empty()) return refuse_loss(why);
     b->drop_graph();
     presk_hip_batch::Item it{nullptr, {}, 0, 0};
     it.loss = *a;
@@ -870,8 +867,7 @@ extern "C" {
 int presk_hip_loss_workspace(const presk_hip_loss* a, int what, size_t* bytes) {
     if (!a || !bytes) return fail(PRESK_HIP_ERR, "E10001: null argument");
     const bool head = a->model != 0;
-    const std::string why = loss_check(*a, what, head);
-    if (!why.empty()) return fail(why.compare(0, 5, "E7005") == 0 ? PRESK_HIP_REFUSED : PRESK_HIP_ERR, why);
+    if (const std::string why = loss_check(*a, what, head); !why.empty()) return refuse_loss(why);
     *bytes = loss_workspace(*a, what, head);
     return PRESK_HIP_OK;
 }

@@ -8,6 +8,7 @@ back to a CPU path: a missing library or a device error raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -52,8 +53,8 @@ class LossArgs(ctypes.Structure):
     """presk_hip_loss."""
     _fields_ = [("dtype", ctypes.c_char_p), ("rows", ctypes.c_int64), ("model", ctypes.c_int64), ("vocab", ctypes.c_int64),
                 ("top", ctypes.c_int64), ("tied", ctypes.c_int32), ("temperature", ctypes.c_double)] + [
-                    (n, ctypes.c_void_p) for n in ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag", "work")
-                ] + [("work_bytes", ctypes.c_size_t)]
+                    (n, ctypes.c_void_p) for n in ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag", "work")] + [
+                        ("work_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -310,6 +311,19 @@ VALUE, GRAD = 1, 2
 _WHAT = {"value": VALUE, "vjp": GRAD, "step": VALUE | GRAD}
 
 
+_LOSS_BUFFERS = ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag")
+
+
+@functools.lru_cache(maxsize=1024)
+def _loss_workspace(sizes: tuple, what: int, dx: bool, dw: bool) -> int:
+    """presk_hip_loss_workspace (of the sizes alone: whether dx and dw are null
+    is all that is looked at of the buffers)."""
+    a, n = LossArgs(sizes[0].encode(), *sizes[1:]), ctypes.c_size_t()
+    a.dx, a.dw = (1 if dx else None), (1 if dw else None)
+    check(lib().presk_hip_loss_workspace(ctypes.byref(a), what, ctypes.byref(n)))
+    return n.value
+
+
 def _buffer(name: str, b, nbytes: int) -> int:
     """The device pointer of a buffer of at least `nbytes` bytes: a
     DeviceBuffer, or an array of another library that says where and how
@@ -351,45 +365,28 @@ class Distill:
     def _set(self, dtype, rows, model, vocab, top, tied, temperature):
         self.dtype, self.rows, self.model, self.vocab, self.top = dtype, int(rows), int(model), int(vocab), int(top)
         self.tied, self.temperature = bool(tied), float(temperature)
-        self._work, self._needs = None, {}
+        self._sizes = (self.dtype, self.rows, self.model, self.vocab, self.top, self.tied, self.temperature)
+        self._work = None
         self.workspace("value")     # the sizes and the type are checked here
-
-    def _args(self) -> LossArgs:
-        a = LossArgs()
-        a.dtype, a.rows, a.model, a.vocab, a.top = self.dtype.encode(), self.rows, self.model, self.vocab, self.top
-        a.tied, a.temperature = int(self.tied), self.temperature
-        return a
+        e, n = STORAGE_BYTES[dtype], self.rows
+        x, w = n * (self.model if self.head else self.vocab) * e, self.model * self.vocab * e
+        self._bytes = (x, w, 8 * n * max(self.top, 1), e * n * self.top, 4 * n, 4 * n, 8, 4 * n, x, w, 4)
 
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
         """Bytes of workspace for `value`, `vjp` or `step` (value_and_grad),
         with the gradients asked for."""
-        key = (kind, dx, dw)
-        if key not in self._needs:
-            a, n = self._args(), ctypes.c_size_t()
-            # (only whether they are null is looked at)
-            a.dx, a.dw = (1 if dx else None), (1 if dw and self.head else None)
-            check(lib().presk_hip_loss_workspace(ctypes.byref(a), _WHAT[kind], ctypes.byref(n)))
-            self._needs[key] = n.value
-        return self._needs[key]
+        return _loss_workspace(self._sizes, _WHAT[kind], dx, dw and self.head)
 
-    def args(self, kind: str, work=None, flag=None, **bufs) -> LossArgs:
+    def args(self, kind: str, x=None, w=None, index=None, teacher=None, loss=None, lse=None, mean=None, ct=None, dx=None, dw=None,
+             flag=None, work=None) -> LossArgs:
         """The call's arguments, each buffer checked against its size."""
-        e = STORAGE_BYTES[self.dtype]
-        n, k = self.rows, max(self.top, 1)
-        x, w = n * (self.model if self.head else self.vocab) * e, self.model * self.vocab * e
-        sizes = {"x": x, "w": w, "index": 8 * n * k, "teacher": e * n * self.top, "loss": 4 * n, "lse": 4 * n, "mean": 8, "ct": 4 * n,
-                 "dx": x, "dw": w}
-        a = self._args()
-        for name, b in bufs.items():
-            setattr(a, name, _buffer(name, b, sizes[name]))
-        a.flag = _buffer("flag", flag, 4)
-        need = self.workspace(kind, bufs.get("dx") is not None, bufs.get("dw") is not None)
+        need = self.workspace(kind, dx is not None, dw is not None)
         if work is None:
             if self._work is None or self._work.nbytes < need:
                 self._work = DeviceBuffer(need)
             work = self._work
-        a.work, a.work_bytes = _buffer("work", work, need), work.nbytes
-        return a
+        bufs = map(_buffer, _LOSS_BUFFERS, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag), self._bytes)
+        return LossArgs(self.dtype.encode(), *self._sizes[1:], *bufs, _buffer("work", work, need), work.nbytes)
 
     def _call(self, kind, stream, **bufs):
         a = self.args(kind, **bufs)
