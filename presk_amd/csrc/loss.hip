@@ -35,20 +35,65 @@ constexpr int kPieceCols = 256;                 // a piece is a multiple of thes
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
-// Tile and splits of a 16-bit product of M x N over K.
+// Tile and splits of a 16-bit product of M x N over K.  256 x 256 tiles where
+// they come to three quarters of the CUs or more, else 128 x 128.
 struct Shape {
     int tile, tiles_m, tiles_n, splits;
 };
-Shape shape_of(long long M, long long N, long long K, bool split) {
-    Shape s{};
-    const long long big = up(M, 256) / 256 * (up(N, 256) / 256);
-    s.tile = big >= 192 ? 256 : 128;
-    s.tiles_m = (int)(up(M, s.tile) / s.tile);
-    s.tiles_n = (int)(up(N, s.tile) / s.tile);
-    s.splits = 1;
-    const long long t = (long long)s.tiles_m * s.tiles_n, nkb = up(K, 64) / 64;
-    if (split && t < 256) s.splits = (int)std::max<long long>(1, std::min<long long>({512 / t, nkb / 4, 64}));
+Shape tiled(long long M, long long N, int tile) { return Shape{tile, (int)(up(M, tile) / tile), (int)(up(N, tile) / tile), 1}; }
+long long tiles_of(const Shape& s) { return (long long)s.tiles_m * s.tiles_n; }
+
+Shape shape_of(long long M, long long N) {
+    const Shape s = tiled(M, N, 256);
+    return tiles_of(s) >= 192 ? s : tiled(M, N, 128);
+}
+
+// dx (Mx x Nx over Kx) and dw in one launch: their tiles are of one kind, and a K
+// that is longer than a CU's share of the work is cut into shares of it, four
+// 64-deep blocks at least.
+void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long Nw, long long Kw, Shape* x, Shape* w) {
+    auto both = [&](int tile) {
+        *x = tiled(Mx, Nx, tile);
+        *w = tiled(Mw, Nw, tile);
+        return tiles_of(*x) + tiles_of(*w);
+    };
+    if (both(256) < 192) both(128);
+    const long long kx = up(Kx, 64) / 64, kw = up(Kw, 64) / 64, slots = x->tile == 256 ? 256 : 512;
+    const double share = (double)(tiles_of(*x) * kx + tiles_of(*w) * kw) / (double)slots;
+    auto cut = [&](long long k) {
+        const long long n = (long long)((double)k / std::max(share, 1.0) + 0.5);
+        return (int)std::max<long long>(1, std::min<long long>({n, k / 4, 64}));
+    };
+    x->splits = cut(kx);
+    w->splits = cut(kw);
+}
+
+// f32 logits: as many shares of K as leave no CU idle, their planes joined as
+// they are read
+Shape logits_of(long long M, long long N, long long K) {
+    Shape s = shape_of(M, N);
+    const long long nkb = up(K, 64) / 64;
+    if (tiles_of(s) < 128) s.splits = (int)std::max<long long>(1, std::min<long long>({256 / tiles_of(s), nkb / 4, 8}));
     return s;
+}
+
+// A 16-bit piece's columns, at most `most`: the width whose tiles of the
+// cotangent's product end nearest whole rounds of the CUs.
+int piece_of(long long rows, long long V, long long most) {
+    if (most >= V) return (int)up(V, kPieceCols);
+    const long long rt = up(rows, 256) / 256, all = up(V, 256) / 256, top = most / 256;
+    long long best = top;
+    double cost = 1e300;
+    for (long long c = top; c >= 1 && c * 2 > top; --c) {
+        const long long n = all / c, rest = all - n * c;
+        const double t = (double)(n * ((rt * c + 255) / 256) + (rest ? (rt * rest + 255) / 256 : 0)) + 0.25 * (double)(n + (rest > 0));
+        if (t < cost) {
+            cost = t;
+            best = c;
+        }
+        if (top - c >= 255) break;
+    }
+    return (int)(best * 256);
 }
 
 struct Plan {
@@ -56,10 +101,11 @@ struct Plan {
     int st, esz, D, V, k, parts, slots, nblocks;
     long long rows, prows;
     float c;
-    bool packx, packw;
+    bool packx, packw, once, counted;   // once: f32 logits of the whole vocabulary; counted: counts are taken
     int Dp, piece, pieces, spiece;    // spiece: columns a pass of row sums takes at once
     long long ldz;
-    size_t col, p, ent, start, count, most, lse, loss, coef, scale, pm, ps, pa, xp, wp, P, acc, part, total;
+    Shape zs;                         // once
+    size_t col, p, ent, start, count, most, lse, loss, coef, scale, pm, ps, pa, xp, wp, P, z, acc, partx, partw, total;
 };
 
 GemmArgs product(long long M, long long N, long long K, long long sa_m, long long sa_k, long long sb_k, long long sb_n, long long sc_m) {
@@ -90,6 +136,12 @@ GemmArgs product_dw(const Plan& q, bool tied, long long n) {
     return tied ? product(n, q.D, q.rows, 1, q.ldz, q.D, 1, q.D) : product(q.D, n, q.rows, 1, q.D, q.ldz, 1, q.V);
 }
 
+// the gradients' products of a 16-bit piece of n columns (one that is not
+// asked for has no tiles)
+void pair_shapes(const Plan& q, const presk_hip_loss& a, int n, Shape* x, Shape* w) {
+    pair_of(a.dx ? q.rows : 0, q.D, up(n, 64), !a.dw ? 0 : a.tied ? n : q.D, a.tied ? q.D : n, q.prows, x, w);
+}
+
 Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     Plan q{};
     q.head = head;
@@ -102,7 +154,10 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     q.V = (int)a.vocab;
     q.k = (int)std::max<int64_t>(a.top, 1);
     q.c = (float)(1.4426950408889634074 / a.temperature);
-    q.parts = loss_parts(q.rows, (int)a.top);
+    // the counted rows' number is the mean's gradient's factor, their largest
+    // cotangent f16's scale
+    q.counted = a.top > 0 || (q.grad && (q.value || (head && q.st == kF16)));
+    q.parts = q.counted ? loss_parts(q.rows, (int)a.top) : 0;
     size_t at = 0;
     auto take = [&](long long bytes) {
         const size_t was = at;
@@ -112,9 +167,9 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     const bool half = head && q.st != kF32;
     q.prows = up(q.rows, 64);
     q.nblocks = (int)(up(q.V, kCols) / kCols);
-    q.col = take(4 * q.rows * q.k);
-    q.p = take(4 * q.rows * q.k);
-    q.ent = take(4 * q.rows);
+    q.col = take(4 * q.rows * a.top);
+    q.p = take(4 * q.rows * a.top);
+    q.ent = take(a.top ? 4 * q.rows : 0);
     q.start = take(half && q.k > 4 ? 2 * q.rows * (q.nblocks + 1) : 0);
     q.count = take(4 * q.parts);
     q.most = take(4 * q.parts);
@@ -133,42 +188,47 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         long long cols = kPieceBytes / (bytes * std::max<long long>(q.prows, 1)) / kPieceCols * kPieceCols;
         if (q.st == kF32) cols = std::min(cols, ((1ll << 31) - 1) / std::max<long long>(q.rows, 1) / kPieceCols * kPieceCols);
         cols = std::min(std::max<long long>(cols, kPieceCols), up(q.V, kPieceCols));
-        q.pieces = (int)(up(q.V, cols) / cols);
-        q.piece = (int)up((q.V + q.pieces - 1) / q.pieces, kPieceCols);
+        q.piece = half ? piece_of(q.rows, q.V, cols) : (int)up((q.V + up(q.V, cols) / cols - 1) / (up(q.V, cols) / cols), kPieceCols);
         q.pieces = (int)(up(q.V, q.piece) / q.piece);
     }
     if (half) {
         q.packx = q.D % 64 != 0;
         q.packw = (a.tied ? q.D : q.V) % 8 != 0;
         q.Dp = (int)up(q.D, 64);
-        q.spiece = q.V;
-        if (q.packw) q.spiece = q.piece;
+        q.ldz = up(q.V, 4);
+        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kPieceBytes && q.V <= 65536;
+        if (q.once) {
+            q.pieces = 1;
+            q.piece = (int)up(q.V, kPieceCols);
+        }
+        q.spiece = q.packw ? q.piece : q.V;
         // (a launch stays below 2^32 threads)
         const long long rt = up(q.rows, 128) / 128;
         if (rt * (up(q.spiece, 128) / 128) > kMany)
             q.spiece = (int)std::max<long long>(kPieceCols, kMany / rt * 128 / kPieceCols * kPieceCols);
-        q.slots = 0;
-        for (long long v = 0; v < q.V && q.value; v += q.spiece)
-            q.slots += shape_of(q.rows, std::min<long long>(q.spiece, q.V - v), q.D, false).tiles_n;
+        for (long long v = 0; v < q.V && q.value && !q.once; v += q.spiece)
+            q.slots += shape_of(q.rows, std::min<long long>(q.spiece, q.V - v)).tiles_n;
         q.xp = take(q.packx ? 2 * q.rows * q.Dp : 0);
         q.wp = take(!q.packw ? 0 : a.tied ? 2ll * q.piece * q.Dp : 2ll * q.D * up(q.piece, 64));
+        if (q.once) {
+            q.zs = logits_of(q.rows, q.V, q.D);
+            q.z = take(4ll * q.zs.splits * q.rows * q.ldz);
+        }
         if (q.grad) {
-            const long long n = std::min<long long>(q.piece, q.V), pld = up(n, 64);
-            q.P = take(2 * q.prows * pld);
+            q.P = take(2 * q.prows * up(std::min<long long>(q.piece, q.V), 64));
             q.acc = take(a.dx && q.pieces > 1 ? 4 * q.rows * q.D : 0);
-            long long part = 0;
+            long long px = 0, pw = 0;
             for (long long v = 0; v < q.V; v += q.piece) {
-                const long long w = std::min<long long>(q.piece, q.V - v);
-                const Shape x = shape_of(q.rows, q.D, up(w, 64), true);
-                const Shape y = shape_of(a.tied ? w : q.D, a.tied ? q.D : w, q.prows, true);
-                if (a.dx && x.splits > 1) part = std::max(part, 4 * x.splits * q.rows * q.D);
-                if (a.dw && y.splits > 1) part = std::max(part, 4ll * y.splits * q.D * w);
+                Shape x, w;
+                pair_shapes(q, a, (int)std::min<long long>(q.piece, q.V - v), &x, &w);
+                if (a.dx && x.splits > 1) px = std::max(px, 4 * x.splits * q.rows * q.D);
+                if (a.dw && w.splits > 1) pw = std::max(pw, 4ll * w.splits * q.D * std::min<long long>(q.piece, q.V - v));
             }
-            q.part = take(part);
+            q.partx = take(px);
+            q.partw = take(pw);
         }
     } else if (head) {
         q.ldz = up(std::min(q.piece, q.V), 4);
-        const long long n = std::min<long long>(q.piece, q.V);
         q.P = take(4 * q.rows * q.ldz);
         long long part = 0;
         auto splits = [&](const GemmArgs& g) {
@@ -181,8 +241,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
             if (q.grad && a.dw) splits(product_dw(q, a.tied, w));
             if (q.value) q.slots += loss_chunks(q.rows, (int)w);
         }
-        q.part = take(part);
-        (void)n;
+        q.partx = take(part);
     } else if (q.value) {
         q.slots = loss_chunks(q.rows, q.V);
     }
@@ -204,13 +263,14 @@ struct Call {
     hipStream_t s;
     char* w;
     LossTarget t;
+    LossPrep prep;
     bool mean_done = false;
 
     template <typename T>
     T* at(size_t off) const { return (T*)(w + off); }
 
-    hipError_t half_gemm(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile) const {
-        return q.st == kBF16 ? loss_gemm_bf16(g, epi, akc, bkc, tile, s) : loss_gemm_f16(g, epi, akc, bkc, tile, s);
+    hipError_t half_gemm(const LossGemm& g, LossEpi epi, int tile) const {
+        return q.st == kBF16 ? loss_gemm_bf16(g, epi, a.tied, tile, s) : loss_gemm_f16(g, epi, a.tied, tile, s);
     }
 
     // What the products of columns [v0, v0 + n) take of x and w.
@@ -249,7 +309,7 @@ struct Call {
         g.K = q.D;
         g.tiles_m = h.tiles_m;
         g.tiles_n = h.tiles_n;
-        g.splits = 1;
+        g.splits = h.splits;
         g.c = q.c;
         g.t = t;
         g.col0 = (int)v0;
@@ -257,15 +317,66 @@ struct Call {
         g.rows = q.rows;
         return g;
     }
-    hipError_t out(LossGemm g, const Shape& h, bool akc, bool bkc) const {
-        g.tiles_m = h.tiles_m;
-        g.tiles_n = h.tiles_n;
-        g.splits = h.splits;
-        g.part = at<float>(q.part);
-        g.scale = q.st == kF16 ? at<float>(q.scale) : nullptr;
-        g.flag = a.flag;
-        LOSS_TRY(half_gemm(g, kEpiOut, akc, bkc, h.tile));
-        return h.splits > 1 ? loss_join(g, q.st, s) : hipSuccess;
+    // dx and dw from columns [v, v + n)'s cotangent
+    hipError_t pair(const Side& x, const Side& w, long long v, int n) {
+        const long long pld = up(n, 64);
+        Shape hx, hw;
+        pair_shapes(q, a, n, &hx, &hw);
+        unsigned short* const P = at<unsigned short>(q.P);
+        LossGemm dx{}, dw{};
+        for (LossGemm* g : {&dx, &dw}) {
+            const Shape& h = g == &dx ? hx : hw;
+            g->tiles_m = h.tiles_m;
+            g->tiles_n = h.tiles_n;
+            g->splits = h.splits;
+            g->scale = q.st == kF16 ? at<float>(q.scale) : nullptr;
+            g->flag = a.flag;
+        }
+        if (a.dx) {
+            // dx[r][d] += sum over the piece of P[r][v] w(v, d); P is zero past the piece
+            dx.A = P;
+            dx.sa = pld;
+            dx.arows = (int)q.rows;
+            dx.ka = (int)pld;
+            dx.B = w.p;
+            dx.sb = w.stride;
+            dx.brows = a.tied ? w.k : q.D;
+            dx.kb = a.tied ? n : w.rows;
+            dx.M = (int)q.rows;
+            dx.N = q.D;
+            dx.K = (int)pld;
+            dx.acc = at<float>(q.acc);
+            dx.lda = q.D;
+            dx.acc_in = v > 0;
+            dx.part = at<float>(q.partx);
+            dx.C = v + n >= q.V ? a.dx : nullptr;
+            dx.ldc = q.D;
+        }
+        if (a.dw) {
+            const Side px{P, pld, (int)pld, (int)q.prows}, sx{x.p, x.stride, x.k, (int)q.rows};
+            const Side& A = a.tied ? px : sx;
+            const Side& B = a.tied ? sx : px;
+            dw.A = A.p;
+            dw.sa = A.stride;
+            dw.arows = A.rows;
+            dw.ka = A.k;
+            dw.B = B.p;
+            dw.sb = B.stride;
+            dw.brows = B.rows;
+            dw.kb = B.k;
+            dw.M = a.tied ? n : q.D;
+            dw.N = a.tied ? q.D : n;
+            dw.K = (int)q.prows;
+            dw.lda = dw.N;
+            dw.part = at<float>(q.partw);
+            dw.C = (unsigned short*)a.dw + (a.tied ? v * q.D : v);
+            dw.ldc = a.tied ? q.D : q.V;
+        }
+        LossMean m{};
+        if (q.value && a.mean && !mean_done) m = mean_args();
+        mean_done = mean_done || m.loss;
+        LOSS_TRY(q.st == kBF16 ? loss_pair_bf16(dx, dw, !a.tied, hx.tile, m, s) : loss_pair_f16(dx, dw, !a.tied, hx.tile, m, s));
+        return loss_join(dx, dw, q.st, s);
     }
 
     hipError_t half(const float* lse) {
@@ -275,75 +386,53 @@ struct Call {
             x = Side{at<unsigned short>(q.xp), q.Dp, (int)q.rows, q.Dp};
         }
         Side w;
+        if (q.once) {
+            // one piece: its logits in f32, their cotangent from whole rows
+            LOSS_TRY(weights(0, q.V, true, &w));
+            LossGemm g = logits(x, w, 0, q.V, q.zs);
+            g.acc = g.part = at<float>(q.z);
+            g.lda = q.ldz;
+            const LossPrep none{};
+            const LossPrep& p = a.top ? none : prep;
+            LOSS_TRY(q.st == kBF16 ? loss_logits_bf16(g, a.tied, q.zs.tile, p, s) : loss_logits_f16(g, a.tied, q.zs.tile, p, s));
+            LossMatrix m = matrix(at<float>(q.z), q.ldz, kF32, 0, q.V);
+            m.planes = q.zs.splits;
+            m.plane = q.rows * q.ldz;
+            LossJoint j = joint_args(m, at<void>(q.P), up(q.V, 64), q.st);
+            j.orows = q.prows;
+            j.scale = q.st == kF16 ? at<float>(q.scale) : nullptr;
+            j.flag = nullptr;
+            LOSS_TRY(loss_joint(j, s));
+            return pair(x, w, 0, q.V);
+        }
         if (q.value) {
             int slot = 0;
             for (long long v = 0; v < q.V; v += q.spiece) {
                 const int n = (int)std::min<long long>(q.spiece, q.V - v);
                 LOSS_TRY(weights(v, n, true, &w));
-                const Shape h = shape_of(q.rows, n, q.D, false);
+                const Shape h = shape_of(q.rows, n);
                 LossGemm g = logits(x, w, v, n, h);
                 g.pm = at<float>(q.pm) + slot * q.rows;
                 g.ps = at<float>(q.ps) + slot * q.rows;
                 g.pa = at<float>(q.pa) + slot * q.rows;
-                LOSS_TRY(half_gemm(g, kEpiStats, true, a.tied, h.tile));
+                LOSS_TRY(half_gemm(g, kEpiStats, h.tile));
                 slot += h.tiles_n;
             }
         }
         LOSS_TRY(rows_of());
         for (long long v = 0; v < q.V && q.grad; v += q.piece) {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
-            const long long pld = up(n, 64);
             // (a vocabulary of one piece is packed already)
             LOSS_TRY(weights(v, n, !(q.value && q.pieces == 1 && q.spiece >= q.V), &w));
-            const Shape h = shape_of(q.rows, n, q.D, false);
+            const Shape h = shape_of(q.rows, n);
             LossGemm g = logits(x, w, v, n, h);
             g.lse = lse;
             g.coef = at<float>(q.coef);
             g.P = at<unsigned short>(q.P);
-            g.pld = pld;
+            g.pld = up(n, 64);
             g.prows = (int)q.prows;
-            LOSS_TRY(half_gemm(g, kEpiP, true, a.tied, h.tile));
-            if (a.dx) {
-                // dx[r][d] += sum over the piece of P[r][v] w(v, d); P is zero past the piece
-                LossGemm d{};
-                d.A = g.P;
-                d.sa = pld;
-                d.arows = (int)q.rows;
-                d.ka = (int)pld;
-                d.B = w.p;
-                d.sb = w.stride;
-                d.brows = a.tied ? w.k : q.D;       // d
-                d.kb = a.tied ? n : w.rows;         // v
-                d.M = (int)q.rows;
-                d.N = q.D;
-                d.K = (int)pld;
-                d.acc = at<float>(q.acc);
-                d.acc_in = v > 0;
-                const bool last = v + n >= q.V;
-                d.C = last ? a.dx : nullptr;
-                d.ldc = q.D;
-                LOSS_TRY(out(d, shape_of(q.rows, q.D, pld, true), true, !a.tied));
-            }
-            if (a.dw) {
-                LossGemm d{};
-                const Side px{g.P, pld, (int)pld, (int)q.prows}, sx{x.p, x.stride, x.k, (int)q.rows};
-                const Side& A = a.tied ? px : sx;
-                const Side& B = a.tied ? sx : px;
-                d.A = A.p;
-                d.sa = A.stride;
-                d.arows = A.rows;
-                d.ka = A.k;
-                d.B = B.p;
-                d.sb = B.stride;
-                d.brows = B.rows;
-                d.kb = B.k;
-                d.M = a.tied ? n : q.D;
-                d.N = a.tied ? q.D : n;
-                d.K = (int)q.prows;
-                d.C = (unsigned short*)a.dw + (a.tied ? v * q.D : v);
-                d.ldc = a.tied ? q.D : q.V;
-                LOSS_TRY(out(d, shape_of(d.M, d.N, q.prows, true), false, false));
-            }
+            LOSS_TRY(half_gemm(g, kEpiP, h.tile));
+            LOSS_TRY(pair(x, w, v, n));
         }
         return hipSuccess;
     }
@@ -354,7 +443,7 @@ struct Call {
         g.C = C;
         g.bias = bias;
         g.bias_kind = bias ? 2 : 0;
-        g.work = at<float>(q.part);
+        g.work = at<float>(q.partx);
         gemm_align(g);
         return gemm_launch(g, s);
     }
@@ -368,9 +457,10 @@ struct Call {
         m.cols = n;
         m.c = q.c;
         m.t = t;
+        m.planes = 1;
         return m;
     }
-    LossJoint joint_args(const LossMatrix& m, void* out, long long ldo) const {
+    LossJoint joint_args(const LossMatrix& m, void* out, long long ldo, int to) const {
         LossJoint j{};
         j.m = m;
         j.temperature = (float)a.temperature;
@@ -378,8 +468,10 @@ struct Call {
         j.loss = loss_out();
         j.ct = a.ct;
         j.count = at<int>(q.count);
+        j.most = at<float>(q.most);
         j.parts = q.parts;
         j.out = out;
+        j.to = to;
         j.ldo = ldo;
         j.flag = a.flag;
         return j;
@@ -401,7 +493,7 @@ struct Call {
         const bool once = q.value && q.grad && q.pieces == 1 && loss_joint_fits(whole);
         if (once) {
             LOSS_TRY(logits(0, q.V));
-            LOSS_TRY(loss_joint(joint_args(whole, z, q.ldz), s));
+            LOSS_TRY(loss_joint(joint_args(whole, z, q.ldz, kF32), s));
         } else {
             int slot = 0;
             for (long long v = 0; v < q.V && q.value; v += q.piece) {
@@ -431,13 +523,14 @@ struct Call {
 
     hipError_t given(const float* lse) {
         LossMatrix m = matrix(a.x, q.V, q.st, 0, q.V);
-        if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, a.dx, q.V), s);
+        if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, a.dx, q.V, q.st), s);
         if (q.value) LOSS_TRY(value_of(m, 0));
         LOSS_TRY(rows_of());
         if (!q.grad) return hipSuccess;
         return loss_grad(m, lse, at<float>(q.coef), a.dx, q.V, a.flag, s);
     }
 
+    LossMean mean_args() const { return LossMean{loss_out(), q.rows, t.index, at<int>(q.count), q.parts, a.mean}; }
     float* lse_out() const { return a.lse ? a.lse : at<float>(q.lse); }
     float* loss_out() const { return a.loss ? a.loss : at<float>(q.loss); }
     LossRows row_args() const {
@@ -475,7 +568,7 @@ struct Call {
     }
 
     hipError_t run() {
-        LossPrep p{};
+        LossPrep& p = prep;
         p.index = (const long long*)a.index;
         p.teacher = a.teacher;
         p.ct = q.grad ? a.ct : nullptr;
@@ -491,15 +584,17 @@ struct Call {
         p.nblocks = q.nblocks;
         p.count = at<int>(q.count);
         p.most = at<float>(q.most);
-        t = LossTarget{p.col, p.p, p.ent, p.start, q.k, q.nblocks};
+        p.parts = q.parts;
+        t = LossTarget{a.top ? nullptr : p.index, q.V, p.col, p.p, p.ent, p.start, q.k, q.nblocks};
         if (q.rows) {
-            LOSS_TRY(loss_prep(p, s));
+            // (counts alone are taken beside the logits where those are one launch)
+            if (q.counted && (a.top || !q.once)) LOSS_TRY(loss_prep(p, s));
             const float* const lse = lse_out();
             LOSS_TRY(!q.head ? given(lse) : q.st == kF32 ? single(lse) : half(lse));
         } else if (q.grad && q.head && a.dw) {
             LOSS_TRY(loss_zero(a.dw, (long long)q.D * q.V * q.esz, s));
         }
-        if (q.value && a.mean && !mean_done) LOSS_TRY(loss_mean(loss_out(), q.rows, p.count, q.parts, a.mean, s));
+        if (q.value && a.mean && !mean_done) LOSS_TRY(loss_mean(mean_args(), s));
         return hipSuccess;
     }
 };
@@ -586,7 +681,7 @@ std::string loss_check_all(const presk_hip_loss& a, int what, bool head) {
 
 hipError_t loss_run(const presk_hip_loss& a, int what, bool head, hipStream_t s) {
     const Plan q = plan_of(a, what, head);
-    Call c{a, q, s, (char*)a.work, {}};
+    Call c{a, q, s, (char*)a.work, {}, {}};
     return c.run();
 }
 
@@ -596,7 +691,7 @@ hipError_t loss_check_run(const presk_hip_loss& a, int what, bool head, hipStrea
     const Plan q = plan_of(a, what, head);
     *why = check_buffers(a, what, head, bytes_of(q));
     if (!why->empty()) return hipSuccess;
-    Call c{a, q, s, (char*)a.work, {}};
+    Call c{a, q, s, (char*)a.work, {}, {}};
     return c.run();
 }
 

@@ -35,8 +35,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // A row's target: `k` slots (column, weight) sorted by column, the weights'
 // sum of p log p (NaN where a slot names no column), and, where k > 4, each
-// 64-column block's first slot.
+// 64-column block's first slot.  One column a row: the call's own index.
 struct LossTarget {
+    const long long* index;      // [rows] or null
+    int vocab;
     const int* col;              // [rows][k]
     const float* p;              // [rows][k]
     const float* ent;            // [rows]
@@ -66,24 +68,28 @@ struct LossGemm {
     // outputs
     void* C;                    // 16-bit, row stride ldc (null: the f32 sums stay in acc)
     long long ldc;
-    float* acc;                 // [M][N] f32: added to (acc_in), written where C is null
+    float* acc;                 // [M][lda] f32: added to (acc_in), written where C is null
+    long long lda;
     bool acc_in;
-    float* part;                // [splits][M][N] f32 (splits > 1)
+    float* part;                // [splits][M][lda] f32 (splits > 1)
     const float* scale;         // the sums' factor, one float of device memory
     unsigned* flag;
 };
 
 enum LossEpi { kEpiStats = 0, kEpiP = 1, kEpiOut = 2 };
 
-// tile rows and columns: 256 x 256 by eight waves, or 128 x 128 by four
-struct LossTile { int bm, bn; };
-hipError_t loss_gemm_bf16(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s);
-hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s);
-
-// ---- row kernels (loss_rows.hip) -------------------------------------------
-
+// What a launch of products may do beside them, in workgroups of its own: the
+// mean of the counted rows' losses, and the counts of rows of one column each.
+struct LossMean {
+    const float* loss;           // null: nothing
+    long long rows;
+    const long long* index;      // one column a row: which count; else
+    const int* count;            // the counts of `parts`
+    int parts;
+    float* mean;
+};
 struct LossPrep {
-    const long long* index;
+    const long long* index;      // null: nothing
     const void* teacher;
     const float* ct;
     int storage;
@@ -96,8 +102,22 @@ struct LossPrep {
     int nblocks;
     int* count;                 // [parts]: counted rows
     float* most;                // [parts]: their largest |ct|
+    int parts;
 };
-// its blocks: `parts` of the counts
+
+// tile: 256 (256 x 256 by eight waves) or 128 (128 x 128 by four)
+hipError_t loss_gemm_bf16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
+hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
+// z = x . w in f32 (kEpiOut, A k-contiguous), the rows' targets counted beside it
+hipError_t loss_logits_bf16(const LossGemm& g, bool bkc, int tile, const LossPrep& p, hipStream_t s);
+hipError_t loss_logits_f16(const LossGemm& g, bool bkc, int tile, const LossPrep& p, hipStream_t s);
+// dx and dw in one launch (either may have no tiles), and the mean
+hipError_t loss_pair_bf16(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s);
+hipError_t loss_pair_f16(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s);
+
+// ---- row kernels (loss_rows.hip) -------------------------------------------
+
+// workgroups of a call's preparation, each of which leaves one count
 int loss_parts(long long rows, int top);
 hipError_t loss_prep(const LossPrep& a, hipStream_t s);
 
@@ -120,7 +140,7 @@ struct LossRows {
 };
 bool loss_rows_mean(long long rows);
 hipError_t loss_rows(const LossRows& a, hipStream_t s);
-hipError_t loss_mean(const float* loss, long long rows, const int* count, int parts, float* mean, hipStream_t s);
+hipError_t loss_mean(const LossMean& m, hipStream_t s);
 
 // Logits in memory, [rows][ld] from column col0 on, `cols` of them.
 struct LossMatrix {
@@ -131,6 +151,8 @@ struct LossMatrix {
     int col0, cols;
     float c;
     LossTarget t;
+    int planes;                 // loss_joint in f32: the sum of so many, in order, ...
+    long long plane;            // ... so many elements apart
 };
 // partials [chunk][rows] from slot0 on; or, of one chunk, the rows' lse and loss
 // themselves (`done`, its outputs may be null)
@@ -151,9 +173,13 @@ struct LossJoint {
     float *lse, *loss;
     const float* ct;
     const int* count;
+    const float* most;
     int parts;
-    void* out;
+    float* scale;               // f16 products follow: the inverse of a power of two in the cotangent
+    void* out;                  // of type `to`: the logits' own, or 16 bits of f32 logits
+    int to;
     long long ldo;
+    long long orows;            // rows written, zero past m.rows; in 16 bits of f32 columns too, up to ldo
     unsigned* flag;
 };
 bool loss_joint_fits(const LossMatrix& m);
@@ -162,7 +188,8 @@ hipError_t loss_joint(const LossJoint& a, hipStream_t s);
 // [rows][cols] 16-bit from row stride lds to ldd, zero up to padded columns
 hipError_t loss_pack(const void* src, long long lds, long long rows, int cols, void* dst, int ldd, hipStream_t s);
 hipError_t loss_zero(void* dst, long long bytes, hipStream_t s);
-// the partials' sum, in split order, times scale (plus acc): into C (16-bit, ldc) or acc
-hipError_t loss_join(const LossGemm& g, int storage, hipStream_t s);
+// the partials' sums of two products (of those that are split), in split order,
+// times scale (plus acc): into C (16-bit, ldc) or acc
+hipError_t loss_join(const LossGemm& x, const LossGemm& w, int storage, hipStream_t s);
 
 }  // namespace presk

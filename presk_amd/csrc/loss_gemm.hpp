@@ -16,8 +16,7 @@
 
 #include <type_traits>
 
-#include "devfmt.hpp"
-#include "loss.hpp"
+#include "loss_dev.hpp"
 
 namespace presk {
 
@@ -157,21 +156,33 @@ __device__ __forceinline__ unsigned short narrow(float v, bool& ovf) {
 // The column, of the wave's 64, of a lane's sum e of column fragment j
 __device__ __forceinline__ int col_of(int j, int e, int lane) { return j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
 
-template <int ST, bool AKC, bool BKC, int WM, int NW, int WAN, int EPI>
-__global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(LossGemm g) {
-    constexpr int WN = 2, NTH = 64 * NW, WAM = NW / WAN, BM = WAM * WM * 32, BN = WAN * 64;
+// A tile: WAM x WAN waves of (WM x 32) x 64.
+template <int WM_, int NW_, int WAN_>
+struct Tile {
+    static constexpr int WM = WM_, NW = NW_, WAN = WAN_, NTH = 64 * NW, BM = NW / WAN * WM * 32, BN = WAN * 64;
+    static constexpr int STAGES = 2, STAGE = (BM + BN) * BK * 2, CLD = BN + 8;
+    static constexpr int OPER = STAGES * STAGE, CTILE = BM * CLD * 2;
+    static constexpr int BYTES = OPER > CTILE ? OPER : CTILE;   // of LDS
+};
+typedef Tile<4, 8, 4> Tile256;
+typedef Tile<2, 4, 2> Tile128;
+
+// Item `id` of `total` of a product, a tile and a range of k; `id` counts from a
+// workgroup whose number is a multiple of 8.
+template <int ST, bool AKC, bool BKC, typename TL, int EPI>
+__device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned total, unsigned char* smem) {
+    constexpr int WM = TL::WM, NW = TL::NW, WAN = TL::WAN, WN = 2, NTH = TL::NTH, BM = TL::BM, BN = TL::BN;
     typedef Block16<AKC, BM, NTH> QA;
     typedef Block16<BKC, BN, NTH> QB;
-    constexpr int STAGE = QA::BYTES + QB::BYTES, NS = 2, CLD = BN + 8;
-    constexpr int OPER = NS * STAGE, CTILE = EPI == kEpiStats ? 3 * WAN * BM * 4 : BM * CLD * 2;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[OPER > CTILE ? OPER : CTILE];
+    constexpr int STAGE = TL::STAGE, CLD = TL::CLD;
+    static_assert(QA::BYTES + QB::BYTES == STAGE && 3 * WAN * BM * 4 <= TL::BYTES, "the tile's LDS");
 
     // Work order: workgroups are dealt to the 8 XCDs round robin; each XCD
     // takes one run of items, tiles GROUP rows at a time across the columns,
     // so that those in flight share panels in its L2.
-    const unsigned tiles = (unsigned)g.tiles_m * (unsigned)g.tiles_n, total = gridDim.x;
-    const unsigned xcd = blockIdx.x % 8, q8 = total / 8, r8 = total % 8;
-    const unsigned item = xcd * q8 + (xcd < r8 ? xcd : r8) + blockIdx.x / 8;
+    const unsigned tiles = (unsigned)g.tiles_m * (unsigned)g.tiles_n;
+    const unsigned xcd = id % 8, q8 = total / 8, r8 = total % 8;
+    const unsigned item = xcd * q8 + (xcd < r8 ? xcd : r8) + id / 8;
     const int split = (int)(item / tiles);
     const unsigned bid = item - (unsigned)split * tiles;
     constexpr unsigned GROUP = BM == 256 ? 4 : 8;
@@ -273,8 +284,9 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
         }
         while (__any(e < end)) {
             const bool on = e < end;
-            const int col = on ? g.t.col[e] - first : -1;
-            const float p = on ? g.t.p[e] : 0.f;
+            const int s = (int)(e - (long long)m * k);
+            const int col = on ? slot_col(g.t, m, s) - first : -1;
+            const float p = on ? slot_p(g.t, m, s) : 0.f;
             if (__any(col >= 0 && col < 64)) f(col, p);
             ++e;
         }
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
             for (int j = 0; j < WN; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = fmaxf(mx, partner<32>(mx));
             const float mc = mx * g.c, base = mx == -INFINITY ? 0.f : mc;
             float s = 0.f, ta = 0.f;
 #pragma unroll
@@ -319,8 +331,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
                         }
                 if (hit) ta += p * (v * g.c);
             });
-            s += __shfl_xor(s, 32);
-            ta += __shfl_xor(ta, 32);
+            s += partner<32>(s);
+            ta += partner<32>(ta);
             if (h == 0) {
                 const int at = wave % WAN * BM + row;
                 red[at] = mc;
@@ -389,14 +401,14 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
         const float scale = g.scale ? *g.scale : 1.f;
         if (g.splits > 1 || !g.C) {
             // f32 sums: four consecutive columns of a row from the registers
-            float* const out = g.splits > 1 ? g.part + (long long)split * g.M * g.N : g.acc;
-            const bool add = g.splits <= 1 && g.acc_in, vec = g.N % 4 == 0;
+            float* const out = g.splits > 1 ? g.part + (long long)split * g.M * g.lda : g.acc;
+            const bool add = g.splits <= 1 && g.acc_in, vec = g.lda % 4 == 0;   // (then rows hold whole fours)
             const float f = g.splits > 1 ? 1.f : scale;
 #pragma unroll
             for (int i = 0; i < WM; ++i) {
                 const int m = m0 + wm + i * 32 + (lane & 31);
                 if (m >= g.M) continue;
-                float* const row = out + (long long)m * g.N;
+                float* const row = out + (long long)m * g.lda;
 #pragma unroll
                 for (int j = 0; j < WN; ++j)
 #pragma unroll
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
                         for (int e = 0; e < 4; ++e) {
                             float x = acc[i][j][4 * q + e] * scale;
                             const bool in = m < g.M && n0 + c + e < g.N;
-                            if (g.acc_in && in) x += g.acc[(long long)m * g.N + n0 + c + e];
+                            if (g.acc_in && in) x += g.acc[(long long)m * g.lda + n0 + c + e];
                             bool o = false;
                             v[e] = narrow<ST>(x, o);
                             ovf |= o && in;
@@ -457,23 +469,67 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 2 : 2) loss_gemm_kernel(Los
     }
 }
 
+template <int ST, bool AKC, bool BKC, typename TL, int EPI>
+__global__ void __launch_bounds__(TL::NTH, 2) loss_gemm_kernel(LossGemm g) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
+    tile_of<ST, AKC, BKC, TL, EPI>(g, blockIdx.x, gridDim.x, smem);
+}
+
+// the logits in f32, and in workgroups past their items the rows' counts
+template <int ST, bool BKC, typename TL>
+__global__ void __launch_bounds__(TL::NTH, 2) loss_logits_kernel(LossGemm g, unsigned items, LossPrep p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
+    if (blockIdx.x < items) tile_of<ST, true, BKC, TL, kEpiOut>(g, blockIdx.x, items, smem);
+    else prep_one<TL::NTH>(p, (int)(blockIdx.x - items));
+}
+
+// dx (A the cotangent, k-contiguous), dw (neither operand), the mean
+template <int ST, bool XBKC, typename TL>
+__global__ void __launch_bounds__(TL::NTH, 2) loss_pair_kernel(LossGemm x, LossGemm w, unsigned nx, unsigned nx8, unsigned nw, LossMean m) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
+    const unsigned id = blockIdx.x;
+    if (id < nx8) {
+        if (id < nx) tile_of<ST, true, XBKC, TL, kEpiOut>(x, id, nx, smem);
+    } else if (id < nx8 + nw) {
+        tile_of<ST, false, false, TL, kEpiOut>(w, id - nx8, nw, smem);
+    } else {
+        write_mean<TL::NTH>(m);
+    }
+}
+
+unsigned items_of(const LossGemm& g) { return (unsigned)g.tiles_m * (unsigned)g.tiles_n * (unsigned)g.splits; }
+
 template <int ST, bool AKC, bool BKC, int EPI>
 hipError_t launch(const LossGemm& g, int tile, hipStream_t s) {
-    const unsigned grid = (unsigned)g.tiles_m * (unsigned)g.tiles_n * (unsigned)g.splits;
+    const unsigned grid = items_of(g);
     if (!grid) return hipSuccess;
-    if (tile == 256)
-        loss_gemm_kernel<ST, AKC, BKC, 4, 8, 4, EPI><<<grid, 512, 0, s>>>(g);
-    else
-        loss_gemm_kernel<ST, AKC, BKC, 2, 4, 2, EPI><<<grid, 256, 0, s>>>(g);
+    if (tile == 256) loss_gemm_kernel<ST, AKC, BKC, Tile256, EPI><<<grid, 512, 0, s>>>(g);
+    else loss_gemm_kernel<ST, AKC, BKC, Tile128, EPI><<<grid, 256, 0, s>>>(g);
     return hipGetLastError();
 }
 
 template <int ST>
-hipError_t dispatch(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s) {
+hipError_t gemm(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s) {
     if (epi == kEpiStats) return bkc ? launch<ST, true, true, kEpiStats>(g, tile, s) : launch<ST, true, false, kEpiStats>(g, tile, s);
     if (epi == kEpiP) return bkc ? launch<ST, true, true, kEpiP>(g, tile, s) : launch<ST, true, false, kEpiP>(g, tile, s);
-    if (akc) return bkc ? launch<ST, true, true, kEpiOut>(g, tile, s) : launch<ST, true, false, kEpiOut>(g, tile, s);
-    return launch<ST, false, false, kEpiOut>(g, tile, s);
+    return hipErrorInvalidValue;
+}
+
+template <int ST, bool BKC>
+hipError_t logits_of(const LossGemm& g, int tile, const LossPrep& p, hipStream_t s) {
+    const unsigned n = items_of(g), grid = n + (p.index ? (unsigned)p.parts : 0);
+    if (tile == 256) loss_logits_kernel<ST, BKC, Tile256><<<grid, 512, 0, s>>>(g, n, p);
+    else loss_logits_kernel<ST, BKC, Tile128><<<grid, 256, 0, s>>>(g, n, p);
+    return hipGetLastError();
+}
+
+template <int ST, bool XBKC>
+hipError_t pair_of(const LossGemm& x, const LossGemm& w, int tile, const LossMean& m, hipStream_t s) {
+    const unsigned nx = items_of(x), nx8 = (nx + 7) / 8 * 8, nw = items_of(w), grid = nx8 + nw + (m.loss ? 1 : 0);
+    if (!grid) return hipSuccess;
+    if (tile == 256) loss_pair_kernel<ST, XBKC, Tile256><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
+    else loss_pair_kernel<ST, XBKC, Tile128><<<grid, 256, 0, s>>>(x, w, nx, nx8, nw, m);
+    return hipGetLastError();
 }
 
 }  // namespace

@@ -3,8 +3,14 @@
 
 namespace presk {
 
-hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool akc, bool bkc, int tile, hipStream_t s) {
-    return dispatch<kF16>(g, epi, akc, bkc, tile, s);
+hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s) {
+    return gemm<kF16>(g, epi, bkc, tile, s);
+}
+hipError_t loss_logits_f16(const LossGemm& g, bool bkc, int tile, const LossPrep& p, hipStream_t s) {
+    return bkc ? logits_of<kF16, true>(g, tile, p, s) : logits_of<kF16, false>(g, tile, p, s);
+}
+hipError_t loss_pair_f16(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s) {
+    return xbkc ? pair_of<kF16, true>(x, w, tile, m, s) : pair_of<kF16, false>(x, w, tile, m, s);
 }
 
 }  // namespace presk

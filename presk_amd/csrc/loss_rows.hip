@@ -8,8 +8,7 @@
 
 #include <algorithm>
 
-#include "devfmt.hpp"
-#include "loss.hpp"
+#include "loss_dev.hpp"
 
 namespace presk {
 
@@ -80,10 +79,6 @@ struct Split {
     __device__ __forceinline__ int edges() const { return head + rest; }
 };
 
-__device__ __forceinline__ float exp2_of(float z, float c, float base) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -base)); }
-// what is subtracted from u where the largest is m: a row of -inf has sum 0
-__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
-
 // (m, s) with another (m2, s2)
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     const float n = fmaxf(m, m2), b = base_of(n);
@@ -91,49 +86,10 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = n;
 }
 
-// Over G threads (64: a wave; more: the workgroup, through `red`, G / 64
-// floats): the same value in every one, the lanes met in a fixed tree.
-template <int G, typename F>
-__device__ __forceinline__ float all_of(float v, float* red, F op) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v = op(v, __shfl_xor(v, d));
-    if constexpr (G > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = red[0];
-#pragma unroll
-        for (int w = 1; w < G / 64; ++w) v = op(v, red[w]);
-    }
-    return v;
-}
-__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
-__device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
-
 // ---- targets ------------------------------------------------------------------
 
 // one column a row
-__global__ void __launch_bounds__(256) prep_one_kernel(LossPrep a) {
-    __shared__ float red[4];
-    float n = 0.f, most = 0.f;
-    for (long long r = (long long)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (long long)gridDim.x * 256) {
-        const long long y = a.index[r];
-        const bool on = y >= 0, out = y >= a.vocab;
-        a.col[r] = !on ? kUnused : out ? kOutside : (int)y;
-        a.p[r] = on && !out ? 1.f : 0.f;
-        a.ent[r] = out ? NAN : 0.f;
-        if (on) {
-            n += 1.f;
-            if (a.ct) most = fmaxf(most, fabsf(a.ct[r]));
-        }
-    }
-    n = all_of<256>(n, red, add_f);
-    most = all_of<256>(most, red, max_f);
-    if (threadIdx.x == 0) {
-        a.count[blockIdx.x] = (int)n;
-        a.most[blockIdx.x] = most;
-    }
-}
+__global__ void __launch_bounds__(256) prep_one_kernel(LossPrep a) { prep_one<256>(a, (int)blockIdx.x); }
 
 // A teacher's slots: the softmax of those in use, sorted by column (a slot's
 // place is how many come before it: columns below its own, or its own at an
@@ -248,26 +204,8 @@ __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
 // A row's loss from its largest u, its sum and its target's part: the largest
 // against the target's before anything is added to it.
 __device__ __forceinline__ float row_loss(const LossTarget& t, long long r, float temperature, float m, float log_s, float ta) {
-    if (t.col[r * t.k] == kUnused) return 0.f;
-    return temperature * temperature * (t.ent[r] + __builtin_fmaf(m - ta, kLn2, log_s));
-}
-
-// the mean of `rows` losses over `n` rows by T threads, in f64 (their order is
-// the strides', then a tree)
-template <int T>
-__device__ __forceinline__ void write_mean(const float* loss, long long rows, int n, float* mean) {
-    __shared__ double red[T / 64];
-    double s = 0.0;
-    for (long long r = threadIdx.x; r < rows; r += T) s += (double)loss[r];
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < T / 64; ++w) s += red[w];
-        mean[0] = n ? (float)(s / n) : 0.f;
-        mean[1] = (float)n;
-    }
+    if (!counts(t, r)) return 0.f;
+    return temperature * temperature * (row_ent(t, r) + __builtin_fmaf(m - ta, kLn2, log_s));
 }
 
 // T / G rows a workgroup, G threads a row, each over every G-th slot; with a
@@ -279,33 +217,21 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
     const long long r = (long long)blockIdx.x * (T / G) + threadIdx.x / G;
     const bool live = r < a.rows;
     float count = 0.f, most = 0.f;
-    if (a.coef || a.mean) {
+    if (a.coef) {
         for (int i = threadIdx.x; i < a.parts; i += T) {
             count += (float)a.count[i];
             most = fmaxf(most, a.most[i]);
         }
         count = all_of<T>(count, red, add_f);
         most = all_of<T>(most, red, max_f);
-    }
-    if (a.coef) {
         const float n = a.mean_in ? a.mean_in[1] : count;
-        // f16: a power of two brings the largest cotangent to 2^14 .. 2^15
-        int e = 0;
-        if (a.scale) {
-            const float top = (a.ct ? most : 1.f / fmaxf(n, 1.f)) * a.temperature;
-            if (top > 0.f && top < INFINITY) {
-                int x;
-                (void)frexpf(top, &x);
-                e = 15 - x < -100 ? -100 : 15 - x > 100 ? 100 : 15 - x;
-            }
-            if (blockIdx.x == 0 && threadIdx.x == 0) *a.scale = ldexpf(1.f, -e);
-        }
+        const int e = a.scale ? scale_exponent((a.ct ? most : 1.f / fmaxf(n, 1.f)) * a.temperature) : 0;
+        if (a.scale && blockIdx.x == 0 && threadIdx.x == 0) *a.scale = ldexpf(1.f, -e);
         if (live && q == 0) {
             float f = 0.f;
-            if (a.t.col[r * a.t.k] != kUnused) {
-                f = (a.ct ? a.ct[r] : 1.f / fmaxf(n, 1.f)) * a.temperature;
-                if (a.scale) f = ldexpf(f, e);
-                f += a.t.ent[r] != a.t.ent[r] ? NAN : 0.f;
+            if (counts(a.t, r)) {
+                f = ldexpf((a.ct ? a.ct[r] : 1.f / fmaxf(n, 1.f)) * a.temperature, e);
+                f += row_ent(a.t, r) != row_ent(a.t, r) ? NAN : 0.f;
             }
             a.coef[r] = f;
         }
@@ -333,22 +259,11 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
     if (a.mean) {
         __threadfence_block();
         __syncthreads();
-        write_mean<T>(a.loss, a.rows, (int)count, a.mean);
+        write_mean<T>(LossMean{a.loss, a.rows, a.t.index, a.count, a.parts, a.mean});
     }
 }
 
-__global__ void __launch_bounds__(1024) mean_kernel(const float* loss, long long rows, const int* count, int parts, float* mean) {
-    __shared__ int red[16];
-    int n = 0;
-    for (int i = threadIdx.x; i < parts; i += 1024) n += count[i];
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
-    __syncthreads();
-    n = 0;
-    for (int w = 0; w < 16; ++w) n += red[w];
-    write_mean<1024>(loss, rows, n, mean);
-}
+__global__ void __launch_bounds__(1024) mean_kernel(LossMean m) { write_mean<1024>(m); }
 
 // ---- logits in memory -------------------------------------------------------------
 
@@ -365,8 +280,8 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
     s = 0.f;
     ta = 0.f;
     for (int e = t; e < a.t.k; e += G) {
-        const int col = a.t.col[r * a.t.k + e] - a.col0;
-        const float p = a.t.p[r * a.t.k + e];
+        const int col = slot_col(a.t, r, e) - a.col0;
+        const float p = slot_p(a.t, r, e);
         if (col >= lo && col < hi && p != 0.f) ta += p * (widen<ST>(z[col]) * a.c);
     }
     // four vectors in flight, their largest first, then one rescale for all
@@ -404,13 +319,13 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
     ta = all_of<G>(ta, red, add_f);
 }
 
-// G 64: four rows a workgroup, a wave each; 256: a row's chunk a workgroup
+// G 16, 64: 16 or four rows a workgroup; 256: a row's chunk a workgroup
 template <int ST, int G>
 __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, float* ps, float* pa, int slot0, int chunk,
                                                     LossDone done, bool finish) {
     __shared__ float red[4];
-    const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
-    if (r >= a.rows) return;    // (whole waves; with G 256 never)
+    const long long r = G < 256 ? (long long)blockIdx.x * (256 / G) + threadIdx.x / G : (long long)blockIdx.x;
+    if (r >= a.rows) return;    // (all threads of a row; with G 256 never)
     const int t = threadIdx.x % G;
     const int lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
     float m, s, ta;
@@ -430,11 +345,11 @@ __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, flo
 
 // Whether slot e is the first that names its column; the weights of those
 // after it that name it too are added in order.
-__device__ __forceinline__ bool first_of(const LossTarget& t, long long at, int e, float& p) {
-    const int col = t.col[at + e];
-    if (e > 0 && t.col[at + e - 1] == col) return false;
-    p = t.p[at + e];
-    for (int q = e + 1; q < t.k && t.col[at + q] == col; ++q) p += t.p[at + q];
+__device__ __forceinline__ bool first_of(const LossTarget& t, long long r, int e, float& p) {
+    const int col = slot_col(t, r, e);
+    if (e > 0 && slot_col(t, r, e - 1) == col) return false;
+    p = slot_p(t, r, e);
+    for (int q = e + 1; q < t.k && slot_col(t, r, q) == col; ++q) p += slot_p(t, r, q);
     return true;
 }
 
@@ -459,13 +374,12 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
     S* const o = (S*)out + r * ldo + lo;
     const float c = coef[r], l = lse[r] * kLog2e;
     const int k = a.t.k, first = a.col0 + lo, n = hi - lo;
-    const long long at = r * k;
     bool ovf = false;
     // the logits of the target's columns, before the row is written (in place)
     constexpr int E = 1024 / G;
     float zt[E];
     for (int q = 0; q < E && t + q * G < k; ++q) {
-        const int col = a.t.col[at + t + q * G] - first;
+        const int col = slot_col(a.t, r, t + q * G) - first;
         zt[q] = col >= 0 && col < n ? widen<ST>(z[col]) : 0.f;
     }
     __builtin_amdgcn_s_waitcnt(0);
@@ -490,74 +404,115 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
     for (int q = 0; q < E && t + q * G < k; ++q) {
-        const int e = t + q * G, col = a.t.col[at + e] - first;
+        const int e = t + q * G, col = slot_col(a.t, r, e) - first;
         float p;
-        if (col >= 0 && col < n && first_of(a.t, at, e, p)) o[col] = cotangent<ST>(zt[q], a.c, l, p, c, ovf);
+        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<ST>(zt[q], a.c, l, p, c, ovf);
     }
     if (ST == kF16 && ovf && flag) atomicOr(flag, 1u);
 }
 
-// Whole rows, read once: G threads a row (64: four rows a workgroup), R
-// vectors and E slots of the target each.
-template <int ST, int G, int R, int E>
+// Whole rows, read once: G threads a row (16, 64: 16 or four rows a workgroup), R
+// vectors and E slots of the target each.  SI the logits' type, SO the output's.
+template <int SI, int SO, int G, int R, int E>
 __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kernel(LossJoint a) {
-    typedef typename Elem<ST>::S S;
-    constexpr int V = Elem<ST>::V, T = G < 256 ? 256 : G;
+    typedef typename Elem<SI>::S S;
+    typedef typename Elem<SO>::S O;
+    constexpr int V = Elem<SI>::V, T = G < 256 ? 256 : G;
     __shared__ float red[T / 64];
     const LossTarget& tg = a.m.t;
-    const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
-    if (r >= a.m.rows) return;  // (whole waves; with more than one a row never)
+    // (a wave's row is one, and its addresses are a uniform base and 32 bits)
+    const long long r = G == 16 ? (long long)blockIdx.x * 16 + threadIdx.x / 16
+                        : G == 64 ? (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : (long long)blockIdx.x;
     const int t = threadIdx.x % G, k = tg.k, n = a.m.cols;
+    O* const o = (O*)a.out + r * a.ldo;
+    // (all threads of a row)
+    if (r >= a.m.rows) {
+        if (r < a.orows)
+            for (long long c = t; c < a.ldo; c += G) o[c] = (O)0;
+        return;
+    }
     const S* const z = (const S*)a.m.z + r * a.m.ld;
-    const long long at = r * k;
     const float cf = a.m.c;
-    const Split<ST> sp(z, n);
+    const Split<SI> sp(z, n);
+    const char* const zb = (const char*)(z + sp.head);
+    const unsigned off = (unsigned)t * 16u;
     u32x4 v[R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (t + i * G < sp.n) v[i] = load_vec(z + sp.head + (long long)(t + i * G) * V);
+        if (t + i * G < sp.n) v[i] = load_vec(zb + i * G * 16 + off);
     const bool edge = t < sp.edges();
-    const float last = edge ? widen<ST>(z[sp.edge(t)]) : -INFINITY;
+    auto logit = [&](int col) {
+        float x = widen<SI>(z[col]);
+        if constexpr (SI == kF32)
+            for (int p = 1; p < a.m.planes; ++p) x += z[p * a.m.plane + col];
+        return x;
+    };
+    const float last = edge ? logit(sp.edge(t)) : -INFINITY;
+    if constexpr (SI == kF32)
+        for (int p = 1; p < a.m.planes; ++p)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (t + i * G < sp.n) {
+                    const u32x4 w = load_vec(zb + p * a.m.plane * 4 + i * G * 16 + off);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[i][e] = pk_bits(pk_float(v[i][e]) + pk_float(w[e]));
+                }
     float zt[E], ta = 0.f;
 #pragma unroll
     for (int q = 0; q < E; ++q) {
         zt[q] = 0.f;
         if (t + q * G < k) {
-            const int col = tg.col[at + t + q * G];
-            const float p = tg.p[at + t + q * G];
+            const int col = slot_col(tg, r, t + q * G);
+            const float p = slot_p(tg, r, t + q * G);
             if (col < n) {
-                zt[q] = widen<ST>(z[col]);
+                zt[q] = logit(col);
                 if (p != 0.f) ta += p * (zt[q] * cf);
             }
         }
     }
     float c = a.temperature;
-    if (a.ct) {
-        c *= a.ct[r];
-    } else {
-        float count = 0.f;
-        for (int i = t; i < a.parts; i += G) count += (float)a.count[i];
-        c *= 1.f / fmaxf(all_of<G>(count, red, add_f), 1.f);
+    if (!a.ct || a.scale) {
+        float count = 0.f, most = 0.f;
+        for (int i = t; i < a.parts; i += G) {
+            count += (float)a.count[i];
+            most = fmaxf(most, a.most[i]);
+        }
+        count = all_of<G>(count, red, add_f);
+        const float f = 1.f / fmaxf(count, 1.f);
+        if (!a.ct) c *= f;
+        if (a.scale) {
+            const int e = scale_exponent((a.ct ? all_of<G>(most, red, max_f) : f) * a.temperature);
+            c = ldexpf(c, e);
+            if (r == 0 && t == 0) *a.scale = ldexpf(1.f, -e);
+        }
     }
-    if (tg.col[at] == kUnused) c = 0.f;
-    else if (tg.ent[at / k] != tg.ent[at / k]) c = NAN;
+    if (a.ct) c *= a.ct[r];
+    if (!counts(tg, r)) c = 0.f;
+    else if (row_ent(tg, r) != row_ent(tg, r)) c = NAN;
     float m = last;
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (t + i * G < sp.n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) m = fmaxf(m, elem<ST>(v[i], e));
+            for (int e = 0; e < V; ++e) m = fmaxf(m, elem<SI>(v[i], e));
     // (every load of this thread has landed before the barriers below, and so
     // before any thread writes the row: the output may be the input)
     __builtin_amdgcn_s_waitcnt(0);
     m = all_of<G>(m, red, max_f) * cf;
     const float b = base_of(m);
+    // (the vectors stay packed between the passes: their elements widened once
+    // for all three would be twice the registers)
+    auto packed = [&]() {
+#pragma unroll
+        for (int i = 0; i < R; ++i) asm volatile("" : "+v"(v[i]));
+    };
+    packed();
     float s = edge ? exp2_of(last, cf, b) : 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (t + i * G < sp.n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += exp2_of(elem<ST>(v[i], e), cf, b);
+            for (int e = 0; e < V; ++e) s += exp2_of(elem<SI>(v[i], e), cf, b);
     s = all_of<G>(s, red, add_f);
     ta = all_of<G>(ta, red, add_f);
     const float ls = pk_logf(s), l = __builtin_fmaf(m, kLn2, ls);
@@ -566,28 +521,38 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
         if (a.loss) a.loss[r] = row_loss(tg, r, a.temperature, m, ls, ta);
     }
     const float l2 = l * kLog2e;
-    S* const o = (S*)a.out + r * a.ldo;
     bool ovf = false;
+    packed();
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (t + i * G < sp.n) {
-            u32x4 w{};
+            char* const at = (char*)(o + sp.head) + i * G * V * (int)sizeof(O) + (unsigned)t * (unsigned)(V * sizeof(O));
+            if constexpr (SI == SO) {
+                u32x4 w{};
 #pragma unroll
-            for (int e = 0; e < V; ++e) set_elem<ST>(w, e, cotangent<ST>(elem<ST>(v[i], e), cf, l2, 0.f, c, ovf));
-            store_vec(o + sp.head + (long long)(t + i * G) * V, w);
+                for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[i], e), cf, l2, 0.f, c, ovf));
+                store_vec(at, w);
+            } else {
+                O w[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[i], e), cf, l2, 0.f, c, ovf);
+                __builtin_memcpy(at, w, sizeof w);
+            }
         }
-    if (edge) o[sp.edge(t)] = cotangent<ST>(last, cf, l2, 0.f, c, ovf);
+    if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, l2, 0.f, c, ovf);
+    if constexpr (SI != SO)
+        for (long long q = n + t; q < a.ldo; q += G) o[q] = (O)0;
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
 #pragma unroll
     for (int q = 0; q < E; ++q) {
         const int e = t + q * G;
         if (e >= k) break;
-        const int col = tg.col[at + e];
+        const int col = slot_col(tg, r, e);
         float p;
-        if (col < n && first_of(tg, at, e, p)) o[col] = cotangent<ST>(zt[q], cf, l2, p, c, ovf);
+        if (col < n && first_of(tg, r, e, p)) o[col] = cotangent<SO>(zt[q], cf, l2, p, c, ovf);
     }
-    if (ST == kF16 && ovf && a.flag) atomicOr(a.flag, 1u);
+    if (SO == kF16 && ovf && a.flag) atomicOr(a.flag, 1u);
 }
 
 // ---- copies ------------------------------------------------------------------------
@@ -618,29 +583,34 @@ __global__ void __launch_bounds__(256) zero_kernel(unsigned char* dst, long long
 }
 
 template <int ST>
-__global__ void __launch_bounds__(256) join_kernel(LossGemm g) {
-    const long long n = (long long)g.M * g.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float s = g.part[i];
+__device__ __forceinline__ void join_at(const LossGemm& g, long long i) {
+    const long long n = (long long)g.M * g.lda, m = i / g.N, at = m * g.lda + (i - m * g.N);
+    float s = g.part[at];
     int p = 1;
     for (; p + 8 <= g.splits; p += 8) {
         float w[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) w[q] = g.part[(long long)(p + q) * n + i];
+        for (int q = 0; q < 8; ++q) w[q] = g.part[(long long)(p + q) * n + at];
 #pragma unroll
         for (int q = 0; q < 8; ++q) s += w[q];
     }
-    for (; p < g.splits; ++p) s += g.part[(long long)p * n + i];
+    for (; p < g.splits; ++p) s += g.part[(long long)p * n + at];
     if (g.scale) s *= *g.scale;
-    if (g.acc_in) s += g.acc[i];
+    if (g.acc_in) s += g.acc[at];
     if (g.C) {
         bool ovf = false;
-        const long long m = i / g.N;
         ((unsigned short*)g.C)[m * g.ldc + (i - m * g.N)] = narrow<ST>(s, ovf);
         if (ovf && g.flag) atomicOr(g.flag, 1u);
     } else {
-        g.acc[i] = s;
+        g.acc[at] = s;
     }
+}
+template <int ST>
+__global__ void __launch_bounds__(256) join_kernel(LossGemm x, LossGemm w, unsigned nx) {
+    const bool first = blockIdx.x < nx;
+    const long long i = (long long)(first ? blockIdx.x : blockIdx.x - nx) * 256 + threadIdx.x;
+    const LossGemm& g = first ? x : w;
+    if (i < (long long)g.M * g.N) join_at<ST>(g, i);
 }
 
 unsigned blocks_of(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 16384); }
@@ -653,7 +623,9 @@ hipError_t stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0
     const int chunks = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, chunks);
     if (done && chunks > 1) return hipErrorInvalidValue;
     const LossDone d = done ? *done : LossDone{};
-    if (m.cols <= 1024)
+    if (m.cols <= 256)
+        stats_kernel<ST, 16><<<dim3((unsigned)((m.rows + 15) / 16)), 256, 0, s>>>(m, pm, ps, pa, slot0, m.cols, d, done);
+    else if (m.cols <= 1024)
         stats_kernel<ST, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, pm, ps, pa, slot0, m.cols, d, done);
     else
         stats_kernel<ST, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, pm, ps, pa, slot0, chunk, d, done);
@@ -670,22 +642,25 @@ hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, void* 
     return hipGetLastError();
 }
 
-template <int ST, int G, int R>
-void joint_of(const LossJoint& a, unsigned grid, hipStream_t s) {
+template <int SI, int SO, int G, int R>
+void joint_of(const LossJoint& a, long long rows, hipStream_t s) {
     constexpr int T = G < 256 ? 256 : G;
-    if (a.m.t.k <= G) joint_kernel<ST, G, R, 1><<<grid, T, 0, s>>>(a);
-    else joint_kernel<ST, G, R, 1024 / G><<<grid, T, 0, s>>>(a);
+    constexpr int per = T / G;
+    const unsigned grid = (unsigned)((rows + per - 1) / per);
+    if (a.m.t.k <= G) joint_kernel<SI, SO, G, R, 1><<<grid, T, 0, s>>>(a);
+    else joint_kernel<SI, SO, G, R, G == 16 ? 4 : 1024 / G><<<grid, T, 0, s>>>(a);
 }
 
-template <int ST>
+template <int SI, int SO>
 hipError_t joint(const LossJoint& a, hipStream_t s) {
-    const int nv = a.m.cols / Elem<ST>::V;
-    const unsigned n = (unsigned)a.m.rows;
-    if (nv <= 64 * 4) joint_of<ST, 64, 4>(a, (n + 3) / 4, s);
-    else if (nv <= 256 * 4) joint_of<ST, 256, 4>(a, n, s);
-    else if (nv <= 512 * 8) joint_of<ST, 512, 8>(a, n, s);
-    else if (nv <= 1024 * 8) joint_of<ST, 1024, 8>(a, n, s);
-    else joint_of<ST, 1024, 16>(a, n, s);
+    const int nv = a.m.cols / Elem<SI>::V;
+    const long long n = std::max(a.m.rows, a.orows);
+    if (nv <= 16 * 4 && a.m.t.k <= 64) joint_of<SI, SO, 16, 4>(a, n, s);
+    else if (nv <= 64 * 4) joint_of<SI, SO, 64, 4>(a, n, s);
+    else if (nv <= 256 * 4) joint_of<SI, SO, 256, 4>(a, n, s);
+    else if (nv <= 512 * 8) joint_of<SI, SO, 512, 8>(a, n, s);
+    else if (nv <= 1024 * 8) joint_of<SI, SO, 1024, 8>(a, n, s);
+    else joint_of<SI, SO, 1024, 16>(a, n, s);
     return hipGetLastError();
 }
 
@@ -708,6 +683,7 @@ int loss_parts(long long rows, int top) {
 hipError_t loss_prep(const LossPrep& a, hipStream_t s) {
     const unsigned grid = (unsigned)loss_parts(a.rows, a.top);
     if (!grid) return hipSuccess;
+    if ((int)grid != a.parts) return hipErrorInvalidValue;
     if (a.top == 0) {
         prep_one_kernel<<<grid, 256, 0, s>>>(a);
         return hipGetLastError();
@@ -737,8 +713,8 @@ hipError_t loss_rows(const LossRows& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t loss_mean(const float* loss, long long rows, const int* count, int parts, float* mean, hipStream_t s) {
-    mean_kernel<<<1, 1024, 0, s>>>(loss, rows, count, parts, mean);
+hipError_t loss_mean(const LossMean& m, hipStream_t s) {
+    mean_kernel<<<1, 1024, 0, s>>>(m);
     return hipGetLastError();
 }
 
@@ -775,11 +751,11 @@ bool loss_joint_fits(const LossMatrix& m) { return m.cols / (m.storage == kF32 ?
 
 hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
     if (a.m.rows <= 0) return hipSuccess;
-    switch (a.m.storage) {
-        case kF32: return joint<kF32>(a, s);
-        case kBF16: return joint<kBF16>(a, s);
-        case kF16: return joint<kF16>(a, s);
-    }
+    if (a.m.storage == kF32 && a.to == kF32) return joint<kF32, kF32>(a, s);
+    if (a.m.storage == kBF16 && a.to == kBF16) return joint<kBF16, kBF16>(a, s);
+    if (a.m.storage == kF16 && a.to == kF16) return joint<kF16, kF16>(a, s);
+    if (a.m.storage == kF32 && a.to == kBF16) return joint<kF32, kBF16>(a, s);
+    if (a.m.storage == kF32 && a.to == kF16) return joint<kF32, kF16>(a, s);
     return hipErrorInvalidValue;
 }
 
@@ -796,12 +772,12 @@ hipError_t loss_zero(void* dst, long long bytes, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t loss_join(const LossGemm& g, int storage, hipStream_t s) {
-    const long long n = (long long)g.M * g.N;
-    if (n <= 0) return hipSuccess;
-    const unsigned grid = (unsigned)((n + 255) / 256);
-    if (storage == kBF16) join_kernel<kBF16><<<grid, 256, 0, s>>>(g);
-    else join_kernel<kF16><<<grid, 256, 0, s>>>(g);
+hipError_t loss_join(const LossGemm& x, const LossGemm& w, int storage, hipStream_t s) {
+    auto blocks = [](const LossGemm& g) { return g.splits > 1 ? (unsigned)(((long long)g.M * g.N + 255) / 256) : 0u; };
+    const unsigned nx = blocks(x), n = nx + blocks(w);
+    if (!n) return hipSuccess;
+    if (storage == kBF16) join_kernel<kBF16><<<n, 256, 0, s>>>(x, w, nx);
+    else join_kernel<kF16><<<n, 256, 0, s>>>(x, w, nx);
     return hipGetLastError();
 }
 
