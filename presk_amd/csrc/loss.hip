@@ -31,6 +31,7 @@ int storage_code(const char* name) {
 
 constexpr long long kMany = 1ll << 22;          // rows, model and a head's vocabulary stay below this
 constexpr long long kPieceBytes = 128ll << 20;  // a piece's logits or their cotangent
+constexpr long long kOnceBytes = 256ll << 20;   // f32 logits that are one piece: as many as the Infinity Cache holds
 constexpr int kPieceCols = 256;                 // a piece is a multiple of these
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
@@ -183,9 +184,10 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         return q;
     }
     if (head) {
-        // pieces of equal width, as wide as kPieceBytes allow
+        // one piece, or as wide as kPieceBytes allow (in f32 of equal width)
         const long long bytes = half ? 2 : 4;
         long long cols = kPieceBytes / (bytes * std::max<long long>(q.prows, 1)) / kPieceCols * kPieceCols;
+        if (4 * q.rows * up(q.V, 4) <= kOnceBytes) cols = up(q.V, kPieceCols);
         if (q.st == kF32) cols = std::min(cols, ((1ll << 31) - 1) / std::max<long long>(q.rows, 1) / kPieceCols * kPieceCols);
         cols = std::min(std::max<long long>(cols, kPieceCols), up(q.V, kPieceCols));
         q.piece = half ? piece_of(q.rows, q.V, cols) : (int)up((q.V + up(q.V, cols) / cols - 1) / (up(q.V, cols) / cols), kPieceCols);
@@ -196,7 +198,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         q.packw = (a.tied ? q.D : q.V) % 8 != 0;
         q.Dp = (int)up(q.D, 64);
         q.ldz = up(q.V, 4);
-        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kPieceBytes && q.V <= 65536;
+        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kOnceBytes && q.V <= 65536;
         if (q.once) {
             q.pieces = 1;
             q.piece = (int)up(q.V, kPieceCols);
@@ -530,7 +532,7 @@ struct Call {
         return loss_grad(m, lse, at<float>(q.coef), a.dx, q.V, a.flag, s);
     }
 
-    LossMean mean_args() const { return LossMean{loss_out(), q.rows, t.index, at<int>(q.count), q.parts, a.mean}; }
+    LossMean mean_args() const { return LossMean{loss_out(), q.rows, at<int>(q.count), q.parts, t.index, a.mean}; }
     float* lse_out() const { return a.lse ? a.lse : at<float>(q.lse); }
     float* loss_out() const { return a.loss ? a.loss : at<float>(q.loss); }
     LossRows row_args() const {

@@ -83,9 +83,9 @@ enum LossEpi { kEpiStats = 0, kEpiP = 1, kEpiOut = 2 };
 struct LossMean {
     const float* loss;           // null: nothing
     long long rows;
-    const long long* index;      // one column a row: which count; else
-    const int* count;            // the counts of `parts`
+    const int* count;            // the counts of `parts`, or, with none taken,
     int parts;
+    const long long* index;      // which of one column a row count
     float* mean;
 };
 struct LossPrep {

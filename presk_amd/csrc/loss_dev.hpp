@@ -122,7 +122,7 @@ __device__ __forceinline__ void write_mean(const LossMean& m) {
         for (int q = 0; q < 8; ++q) {
             const bool in = r0 + q * T < m.rows;
             l[q] = in ? m.loss[r0 + q * T] : 0.f;
-            y[q] = in && m.index ? m.index[r0 + q * T] : -1;
+            y[q] = in && !m.parts ? m.index[r0 + q * T] : -1;
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -130,8 +130,7 @@ __device__ __forceinline__ void write_mean(const LossMean& m) {
             n += y[q] >= 0;
         }
     }
-    if (!m.index)
-        for (int i = threadIdx.x; i < m.parts; i += T) n += m.count[i];
+    for (int i = threadIdx.x; i < m.parts; i += T) n += m.count[i];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         s += __shfl_xor(s, d);

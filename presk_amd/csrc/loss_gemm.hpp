@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "loss_dev.hpp"
 
@@ -138,6 +139,28 @@ __device__ __forceinline__ void wait_vm() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
+// Wait until the block about to be read has landed, `later` blocks issued
+// after it (NL loads a thread each) still in flight.
+template <int NL, int L>
+__device__ __forceinline__ void wait_blocks(int later) {
+    if constexpr (L == 0) {
+        wait_vm<0>();
+    } else {
+        if (later >= L) wait_vm<L * NL>();
+        else wait_blocks<NL, L - 1>(later);
+    }
+}
+
+// Blocks kt .. kt + sizeof(I) - 1 in stages I; the tail takes those below n.
+template <typename F, int... I>
+__device__ __forceinline__ void stage_round(F& f, int kt, std::integer_sequence<int, I...>) {
+    (f(kt + I, std::integral_constant<int, I>{}), ...);
+}
+template <typename F, int... I>
+__device__ __forceinline__ void stage_tail(F& f, int kt, int n, std::integer_sequence<int, I...>) {
+    ((kt + I < n ? f(kt + I, std::integral_constant<int, I>{}) : void()), ...);
+}
+
 template <int ST>
 __device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 acc) {
     if constexpr (ST == kBF16)
@@ -157,15 +180,16 @@ __device__ __forceinline__ unsigned short narrow(float v, bool& ovf) {
 __device__ __forceinline__ int col_of(int j, int e, int lane) { return j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
 
 // A tile: WAM x WAN waves of (WM x 32) x 64.
-template <int WM_, int NW_, int WAN_>
+template <int WM_, int NW_, int WAN_, int STAGES_>
 struct Tile {
     static constexpr int WM = WM_, NW = NW_, WAN = WAN_, NTH = 64 * NW, BM = NW / WAN * WM * 32, BN = WAN * 64;
-    static constexpr int STAGES = 2, STAGE = (BM + BN) * BK * 2, CLD = BN + 8;
+    static constexpr int STAGES = STAGES_, STAGE = (BM + BN) * BK * 2, CLD = BN + 8;
     static constexpr int OPER = STAGES * STAGE, CTILE = BM * CLD * 2;
     static constexpr int BYTES = OPER > CTILE ? OPER : CTILE;   // of LDS
 };
-typedef Tile<4, 8, 4> Tile256;
-typedef Tile<2, 4, 2> Tile128;
+typedef Tile<4, 8, 4, 2> Tile256;
+typedef Tile<2, 4, 2, 2> Tile128;
+typedef Tile<1, 8, 2, 4> Tile128x8;
 
 // Item `id` of `total` of a product, a tile and a range of k; `id` counts from a
 // workgroup whose number is a multiple of 8.
@@ -203,13 +227,15 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
     const unsigned nkb = (unsigned)((g.K + BK - 1) / BK), ns = (unsigned)g.splits;
     const int kb0 = (int)((unsigned)split * nkb / ns), nd = (int)(((unsigned)split + 1) * nkb / ns) - kb0;
 
-    // Block kt + 1 streams into one stage while block kt is multiplied out of
-    // the other; each 16-k step's fragments are read during the step before.
-    // Before a block's last step this thread's loads of the next block have
-    // landed, and a barrier has seen every thread's; it also retires every read
-    // of the stage that the loads after it overwrite.
+    // Blocks kt + 1 .. kt + STAGES - 1 stream into their stages while block kt
+    // is multiplied; each 16-k step's fragments are read during the step
+    // before.  Before a block's last step this thread's loads of the next
+    // block have landed, and a barrier has seen every thread's; it also retires
+    // every read of the stage that the loads after it overwrite.
     QA qa;
     QB qb;
+    constexpr int NS = TL::STAGES, LA = NS - 1, NL = QA::ROUNDS + QB::ROUNDS;
+    static_assert(LA * NL < 64, "vmcnt holds the loads in flight");
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
     qa.init(g.A, g.arows, g.sa, m0, g.ka, lds);
     qb.init(g.B, g.brows, g.sb, n0, g.kb, lds + QA::BYTES);
@@ -225,14 +251,15 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
         for (int j = 0; j < WN; ++j) b[j] = QB::frag(st + QA::BYTES, wn + j * 32, kk, lane);
     };
     if (nd > 0) {
-        fetch(0, 0);
-        wait_vm<0>();
+        const int pre = nd < LA ? nd : LA;
+        for (int kb = 0; kb < pre; ++kb) fetch(kb, kb);
+        wait_blocks<NL, LA - 1>(pre - 1);
         __syncthreads();
         read(smem, 0);
     }
     auto block = [&](int kt, auto stage) {
         constexpr int CUR = decltype(stage)::value;
-        if (kt + 1 < nd) fetch(kt + 1, CUR ^ 1);
+        if (kt + LA < nd) fetch(kt + LA, (CUR + LA) % NS);
         const unsigned char* const st = smem + CUR * STAGE;
 #pragma unroll
         for (int kk = 0; kk < BK; kk += 16) {
@@ -244,9 +271,10 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
             if (kk + 16 < BK) {
                 read(st, kk + 16);
             } else if (kt + 1 < nd) {
-                wait_vm<0>();
+                const int last = kt + LA < nd - 1 ? kt + LA : nd - 1;   // the last block issued
+                wait_blocks<NL, LA - 1>(last - (kt + 1));
                 __syncthreads();
-                read(smem + (CUR ^ 1) * STAGE, 0);
+                read(smem + (CUR + 1) % NS * STAGE, 0);
             }
             // the reads stay ahead of this step's MFMAs
             __builtin_amdgcn_sched_barrier(0);
@@ -258,11 +286,8 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
         }
     };
     int kt = 0;
-    for (; kt + 2 <= nd; kt += 2) {
-        block(kt, std::integral_constant<int, 0>{});
-        block(kt + 1, std::integral_constant<int, 1>{});
-    }
-    if (kt < nd) block(kt, std::integral_constant<int, 0>{});
+    for (; kt + NS <= nd; kt += NS) stage_round(block, kt, std::make_integer_sequence<int, NS>{});
+    stage_tail(block, kt, nd, std::make_integer_sequence<int, NS - 1>{});
     __syncthreads();    // the stages are the epilogue's from here
 
     // The slots of row m's target in the wave's 64 columns: f(column, weight)
@@ -504,6 +529,7 @@ hipError_t launch(const LossGemm& g, int tile, hipStream_t s) {
     const unsigned grid = items_of(g);
     if (!grid) return hipSuccess;
     if (tile == 256) loss_gemm_kernel<ST, AKC, BKC, Tile256, EPI><<<grid, 512, 0, s>>>(g);
+    else if (tile == 130) loss_gemm_kernel<ST, AKC, BKC, Tile128x8, EPI><<<grid, 512, 0, s>>>(g);
     else loss_gemm_kernel<ST, AKC, BKC, Tile128, EPI><<<grid, 256, 0, s>>>(g);
     return hipGetLastError();
 }
@@ -519,6 +545,7 @@ template <int ST, bool BKC>
 hipError_t logits_of(const LossGemm& g, int tile, const LossPrep& p, hipStream_t s) {
     const unsigned n = items_of(g), grid = n + (p.index ? (unsigned)p.parts : 0);
     if (tile == 256) loss_logits_kernel<ST, BKC, Tile256><<<grid, 512, 0, s>>>(g, n, p);
+    else if (tile == 130) loss_logits_kernel<ST, BKC, Tile128x8><<<grid, 512, 0, s>>>(g, n, p);
     else loss_logits_kernel<ST, BKC, Tile128><<<grid, 256, 0, s>>>(g, n, p);
     return hipGetLastError();
 }
@@ -528,6 +555,7 @@ hipError_t pair_of(const LossGemm& x, const LossGemm& w, int tile, const LossMea
     const unsigned nx = items_of(x), nx8 = (nx + 7) / 8 * 8, nw = items_of(w), grid = nx8 + nw + (m.loss ? 1 : 0);
     if (!grid) return hipSuccess;
     if (tile == 256) loss_pair_kernel<ST, XBKC, Tile256><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
+    else if (tile == 130) loss_pair_kernel<ST, XBKC, Tile128x8><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
     else loss_pair_kernel<ST, XBKC, Tile128><<<grid, 256, 0, s>>>(x, w, nx, nx8, nw, m);
     return hipGetLastError();
 }

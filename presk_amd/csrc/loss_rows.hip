@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) prep_one_kernel(LossPrep a) { prep_one<25
 template <int ST, int G, int E>
 __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
     constexpr int R = 256 / G, KM = G * E;
-    __shared__ __attribute__((aligned(16))) int in[R][KM], sorted[R][KM];
+    __shared__ __attribute__((aligned(16))) int in[R][KM + 4], sorted[R][KM];  // (rows four banks apart)
     __shared__ float red[4], tally[R][2];
     const int g = threadIdx.x / G, t = threadIdx.x % G, k = a.top;
     typedef typename Elem<ST>::S S;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
         for (int q = 0; q < E; ++q)
             if (col[q] != kUnused) total += exp2_of(x[q], a.c, base);
         total = all_of<G>(total, red, add_f);   // (and the barrier that `in` needs)
-        if constexpr (G == 64) __syncthreads();
+        if constexpr (G <= 64) __syncthreads();
         int at[E];
 #pragma unroll
         for (int q = 0; q < E; ++q) at[q] = 0;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
     if (a.mean) {
         __threadfence_block();
         __syncthreads();
-        write_mean<T>(LossMean{a.loss, a.rows, a.t.index, a.count, a.parts, a.mean});
+        write_mean<T>(LossMean{a.loss, a.rows, a.count, a.parts, a.t.index, a.mean});
     }
 }
 
@@ -666,7 +666,9 @@ hipError_t joint(const LossJoint& a, hipStream_t s) {
 
 template <int ST>
 hipError_t prep(const LossPrep& a, unsigned grid, hipStream_t s) {
-    if (a.top <= 64) prep_top_kernel<ST, 64, 1><<<grid, 256, 0, s>>>(a);
+    if (a.top <= 16) prep_top_kernel<ST, 16, 1><<<grid, 256, 0, s>>>(a);
+    else if (a.top <= 32) prep_top_kernel<ST, 16, 2><<<grid, 256, 0, s>>>(a);
+    else if (a.top <= 64) prep_top_kernel<ST, 16, 4><<<grid, 256, 0, s>>>(a);
     else if (a.top <= 128) prep_top_kernel<ST, 64, 2><<<grid, 256, 0, s>>>(a);
     else if (a.top <= 256) prep_top_kernel<ST, 64, 4><<<grid, 256, 0, s>>>(a);
     else prep_top_kernel<ST, 256, 4><<<grid, 256, 0, s>>>(a);
@@ -676,7 +678,7 @@ hipError_t prep(const LossPrep& a, unsigned grid, hipStream_t s) {
 }  // namespace
 
 int loss_parts(long long rows, int top) {
-    const long long per = top == 0 ? 256 : top <= 256 ? 4 : 1;
+    const long long per = top == 0 ? 256 : top <= 64 ? 16 : top <= 256 ? 4 : 1;
     return (int)std::min<long long>((rows + per - 1) / per, kParts);
 }
 
