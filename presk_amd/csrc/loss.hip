@@ -36,37 +36,56 @@ constexpr int kPieceCols = 256;                 // a piece is a multiple of thes
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
-// Tile and splits of a 16-bit product of M x N over K.  256 x 256 tiles where
-// they come to three quarters of the CUs or more, else 128 x 128.
+// Tile and splits of a 16-bit product of M x N over K: 256 x 256 tiles where
+// they come to three quarters of the CUs or more (2048 x 4096 x 32000 446 us, on
+// 128 x 128 tiles 546), else 128 x 128: two workgroups a CU, or, where no CU
+// has two of them anyway, one of eight waves with three blocks in flight (8 x 4096
+// x 32000, 250 tiles, 58.7 -> 46.7 us with its weights partly in cache; 1024
+// tiles of 4096 x 512 x 2048 76.8 us, deep 81.3).
 struct Shape {
     int tile, tiles_m, tiles_n, splits;
 };
-Shape tiled(long long M, long long N, int tile) { return Shape{tile, (int)(up(M, tile) / tile), (int)(up(N, tile) / tile), 1}; }
+Shape tiled(long long M, long long N, int tile) {
+    const int n = tile == 256 ? 256 : 128;
+    return Shape{tile, (int)(up(M, n) / n), (int)(up(N, n) / n), 1};
+}
 long long tiles_of(const Shape& s) { return (long long)s.tiles_m * s.tiles_n; }
 
 Shape shape_of(long long M, long long N) {
-    const Shape s = tiled(M, N, 256);
-    return tiles_of(s) >= 192 ? s : tiled(M, N, 128);
+    const Shape s = tiled(M, N, 256), t = tiled(M, N, 128);
+    return tiles_of(s) >= 192 ? s : tiles_of(t) > 256 ? t : tiled(M, N, kDeep128);
 }
 
 // dx (Mx x Nx over Kx) and dw in one launch: their tiles are of one kind, and a K
 // that is longer than a CU's share of the work is cut into shares of it, four
-// 64-deep blocks at least.
+// 64-deep blocks at least.  The deep tiles where one round of the CUs holds
+// every item (4096 x 512 x 2048 76.8 -> 69.2 us; 512 x 2048 x 8192, 1100 items,
+// 98 us, deep 104); two a CU are kept to one round where fewer cuts do that
+// (777 x 500 x 10007, 316 tiles of dw and 28 of dx cut 9 ways 105 us, 6 ways 93).
 void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long Nw, long long Kw, Shape* x, Shape* w) {
-    auto both = [&](int tile) {
+    const long long kx = up(Kx, 64) / 64, kw = up(Kw, 64) / 64;
+    auto items = [&]() { return tiles_of(*x) * x->splits + tiles_of(*w) * w->splits; };
+    auto both = [&](int tile, long long slots) {
         *x = tiled(Mx, Nx, tile);
         *w = tiled(Mw, Nw, tile);
+        const double share = std::max((double)(tiles_of(*x) * kx + tiles_of(*w) * kw) / (double)slots, 1.0);
+        auto cut = [&](long long k) {
+            const long long n = (long long)((double)k / share + 0.5);
+            return (int)std::max<long long>(1, std::min<long long>({n, k / 4, 64}));
+        };
+        x->splits = cut(kx);
+        w->splits = cut(kw);
+        for (Shape* s : {x, w}) {
+            const long long over = items() - slots, t = std::max<long long>(tiles_of(*s), 1);
+            const long long less = s->splits - (over + t - 1) / t;
+            if (over > 0 && 2 * less > s->splits) s->splits = (int)less;
+        }
         return tiles_of(*x) + tiles_of(*w);
     };
-    if (both(256) < 192) both(128);
-    const long long kx = up(Kx, 64) / 64, kw = up(Kw, 64) / 64, slots = x->tile == 256 ? 256 : 512;
-    const double share = (double)(tiles_of(*x) * kx + tiles_of(*w) * kw) / (double)slots;
-    auto cut = [&](long long k) {
-        const long long n = (long long)((double)k / std::max(share, 1.0) + 0.5);
-        return (int)std::max<long long>(1, std::min<long long>({n, k / 4, 64}));
-    };
-    x->splits = cut(kx);
-    w->splits = cut(kw);
+    if (both(256, 256) >= 192) return;
+    both(kDeep128, 256);
+    if (items() <= 256) return;
+    both(128, 512);
 }
 
 // f32 logits: as many shares of K as leave no CU idle, their planes joined as
@@ -281,20 +300,25 @@ struct Call {
         long long stride;
         int rows, k;    // of w: columns and k that exist, as the logits' product sees them
     };
-    hipError_t weights(long long v0, int n, bool pack, Side* o) const {
+    bool x_packed = false;
+    Side states() const {
+        return q.packx ? Side{at<unsigned short>(q.xp), q.Dp, (int)q.rows, q.Dp}
+                       : Side{(const unsigned short*)a.x, q.D, (int)q.rows, q.D};
+    }
+    // w's side of columns [v0, v0 + n); what has to be packed, x the first
+    // time, is (w not where `held`)
+    hipError_t weights(long long v0, int n, bool held, Side* o) {
         const unsigned short* const wt = (const unsigned short*)a.w + (a.tied ? v0 * q.D : v0);
-        if (!q.packw) {
-            *o = Side{wt, a.tied ? q.D : q.V, n, q.D};
-            return hipSuccess;
-        }
+        LossPack px{}, pw{};
+        if (q.packx && !x_packed) px = LossPack{a.x, q.D, q.rows, q.D, at<void>(q.xp), q.Dp};
+        x_packed = true;
         unsigned short* const dst = at<unsigned short>(q.wp);
-        if (a.tied) {
-            *o = Side{dst, q.Dp, n, q.Dp};
-            return pack ? loss_pack(wt, q.D, n, q.D, dst, q.Dp, s) : hipSuccess;
-        }
         const int ld = (int)up(n, 64);
-        *o = Side{dst, ld, ld, q.D};
-        return pack ? loss_pack(wt, q.V, q.D, n, dst, ld, s) : hipSuccess;
+        if (!q.packw) *o = Side{wt, a.tied ? q.D : q.V, n, q.D};
+        else if (a.tied) *o = Side{dst, q.Dp, n, q.Dp};
+        else *o = Side{dst, ld, ld, q.D};
+        if (q.packw && !held) pw = a.tied ? LossPack{wt, q.D, n, q.D, dst, q.Dp} : LossPack{wt, q.V, q.D, n, dst, ld};
+        return loss_pack(px, pw, s);
     }
     LossGemm logits(const Side& x, const Side& w, long long v0, int n, const Shape& h) const {
         LossGemm g{};
@@ -382,15 +406,11 @@ struct Call {
     }
 
     hipError_t half(const float* lse) {
-        Side x{(const unsigned short*)a.x, q.D, (int)q.rows, q.D};
-        if (q.packx) {
-            LOSS_TRY(loss_pack(a.x, q.D, q.rows, q.D, at<void>(q.xp), q.Dp, s));
-            x = Side{at<unsigned short>(q.xp), q.Dp, (int)q.rows, q.Dp};
-        }
+        const Side x = states();
         Side w;
         if (q.once) {
             // one piece: its logits in f32, their cotangent from whole rows
-            LOSS_TRY(weights(0, q.V, true, &w));
+            LOSS_TRY(weights(0, q.V, false, &w));
             LossGemm g = logits(x, w, 0, q.V, q.zs);
             g.acc = g.part = at<float>(q.z);
             g.lda = q.ldz;
@@ -411,7 +431,7 @@ struct Call {
             int slot = 0;
             for (long long v = 0; v < q.V; v += q.spiece) {
                 const int n = (int)std::min<long long>(q.spiece, q.V - v);
-                LOSS_TRY(weights(v, n, true, &w));
+                LOSS_TRY(weights(v, n, false, &w));
                 const Shape h = shape_of(q.rows, n);
                 LossGemm g = logits(x, w, v, n, h);
                 g.pm = at<float>(q.pm) + slot * q.rows;
@@ -425,7 +445,7 @@ struct Call {
         for (long long v = 0; v < q.V && q.grad; v += q.piece) {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
             // (a vocabulary of one piece is packed already)
-            LOSS_TRY(weights(v, n, !(q.value && q.pieces == 1 && q.spiece >= q.V), &w));
+            LOSS_TRY(weights(v, n, q.value && q.pieces == 1 && q.spiece >= q.V, &w));
             const Shape h = shape_of(q.rows, n);
             LossGemm g = logits(x, w, v, n, h);
             g.lse = lse;

@@ -105,7 +105,9 @@ struct LossPrep {
     int parts;
 };
 
-// tile: 256 (256 x 256 by eight waves) or 128 (128 x 128 by four)
+// tile: 256 (256 x 256 by eight waves), 128 (128 x 128 by four) or kDeep128
+// (128 x 128 by eight, more blocks in flight)
+constexpr int kDeep128 = 130;
 hipError_t loss_gemm_bf16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
 hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
 // z = x . w in f32 (kEpiOut, A k-contiguous), the rows' targets counted beside it
@@ -185,8 +187,16 @@ struct LossJoint {
 bool loss_joint_fits(const LossMatrix& m);
 hipError_t loss_joint(const LossJoint& a, hipStream_t s);
 
-// [rows][cols] 16-bit from row stride lds to ldd, zero up to padded columns
-hipError_t loss_pack(const void* src, long long lds, long long rows, int cols, void* dst, int ldd, hipStream_t s);
+// [rows][cols] 16-bit from row stride lds to ldd (a multiple of 8), zero past
+// cols: two of them, either may have no rows
+struct LossPack {
+    const void* src;
+    long long lds, rows;
+    int cols;
+    void* dst;
+    int ldd;
+};
+hipError_t loss_pack(const LossPack& a, const LossPack& b, hipStream_t s);
 hipError_t loss_zero(void* dst, long long bytes, hipStream_t s);
 // the partials' sums of two products (of those that are split), in split order,
 // times scale (plus acc): into C (16-bit, ldc) or acc

@@ -558,23 +558,25 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
 // ---- copies ------------------------------------------------------------------------
 
 // rows of `cols` elements into rows of `ldd`, eight elements a thread, zero
-// past cols
-__global__ void __launch_bounds__(256) pack_kernel(const unsigned short* src, long long lds, long long rows, int cols,
-                                                   unsigned short* dst, int ldd) {
-    const unsigned vpr = (unsigned)ldd / 8;
-    const long long n = rows * vpr;
-    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < n; u += (long long)gridDim.x * 256) {
+// past cols; the first nb workgroups take a's
+__global__ void __launch_bounds__(256) pack_kernel(LossPack a, LossPack b, unsigned nb) {
+    const bool first = blockIdx.x < nb;
+    const LossPack& k = first ? a : b;
+    const long long at = first ? blockIdx.x : blockIdx.x - nb, stride = first ? nb : gridDim.x - nb;
+    const unsigned vpr = (unsigned)k.ldd / 8;
+    const long long n = k.rows * vpr;
+    for (long long u = at * 256 + threadIdx.x; u < n; u += stride * 256) {
         const long long r = u / vpr;
         const int c = (int)(u - r * vpr) * 8;
-        const unsigned short* const p = src + r * lds + c;
+        const unsigned short* const p = (const unsigned short*)k.src + r * k.lds + c;
         u16x8 v;
-        if (c + 8 <= cols) {
+        if (c + 8 <= k.cols) {
             __builtin_memcpy(&v, p, 16);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : (unsigned short)0;
+            for (int e = 0; e < 8; ++e) v[e] = c + e < k.cols ? p[e] : (unsigned short)0;
         }
-        *(u16x8*)(dst + r * ldd + c) = v;
+        *(u16x8*)((unsigned short*)k.dst + r * k.ldd + c) = v;
     }
 }
 
@@ -761,10 +763,11 @@ hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
     return hipErrorInvalidValue;
 }
 
-hipError_t loss_pack(const void* src, long long lds, long long rows, int cols, void* dst, int ldd, hipStream_t s) {
-    const long long n = rows * (ldd / 8);
-    if (n <= 0) return hipSuccess;
-    pack_kernel<<<blocks_of(n), 256, 0, s>>>((const unsigned short*)src, lds, rows, cols, (unsigned short*)dst, ldd);
+hipError_t loss_pack(const LossPack& a, const LossPack& b, hipStream_t s) {
+    auto blocks = [](const LossPack& k) { return k.rows > 0 ? blocks_of(k.rows * (k.ldd / 8)) : 0u; };
+    const unsigned na = blocks(a), n = na + blocks(b);
+    if (!n) return hipSuccess;
+    pack_kernel<<<n, 256, 0, s>>>(a, b, na);
     return hipGetLastError();
 }
 
