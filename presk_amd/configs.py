@@ -148,32 +148,30 @@ def storage_inputs(p: Program, host: dict) -> dict:
     under its name and its f32 scales under `<name>#scales`."""
     from . import quant as Q
     env = {}
-    for ln in p.launches:
-        for name, (ty, count) in zip(ln.ins, _input_specs(ln.low)):
-            ty = p.input_types.get(name, ty) if ty != "i64" else ty
-            if name in host and name not in env:
-                v = host[name]
-                if ty == "i64":
-                    env[name] = np.ascontiguousarray(v, dtype=np.int64).ravel()
-                elif name in p.quant:
-                    q, over, axes = p.quant[name]
-                    qt = Q.quantize(np.asarray(v, np.float32).astype(np.float64), [a.len for a in axes],
-                                    Q.Quant(q.bits, over, q.scheme))
-                    env[name], env[name + "#scales"] = qt.data, qt.scales
-                elif np.asarray(v).dtype == np.float64:
-                    # the host's f64 values (literals, drawn inputs): one Buf::of
-                    env[name] = encode64(np.asarray(v).reshape(-1)[:max(count, 1)], ty)
-                else:
-                    env[name] = encode(np.asarray(v, np.float32).reshape(-1)[:max(count, 1)], ty)
+    for name, (ty, count) in p.input_specs():
+        ty = p.input_types.get(name, ty) if ty != "i64" else ty
+        if name in host and name not in env:
+            v = host[name]
+            if ty == "i64":
+                env[name] = np.ascontiguousarray(v, dtype=np.int64).ravel()
+            elif name in p.quant:
+                q, over, axes = p.quant[name]
+                qt = Q.quantize(np.asarray(v, np.float32).astype(np.float64), [a.len for a in axes],
+                                Q.Quant(q.bits, over, q.scheme))
+                env[name], env[name + "#scales"] = qt.data, qt.scales
+            elif np.asarray(v).dtype == np.float64:
+                # the host's f64 values (literals, drawn inputs): one Buf::of
+                env[name] = encode64(np.asarray(v).reshape(-1)[:max(count, 1)], ty)
+            else:
+                env[name] = encode(np.asarray(v, np.float32).reshape(-1)[:max(count, 1)], ty)
     return env
 
 
 def load_inputs(p: Program, host: dict):
     """Declares and uploads every host input in the program's storage type."""
     specs = {}
-    for ln in p.launches:
-        for name, (ty, count) in zip(ln.ins, _input_specs(ln.low)):
-            specs.setdefault(name, (p.input_types.get(name, ty) if ty != "i64" else ty, count))
+    for name, (ty, count) in p.input_specs():
+        specs.setdefault(name, (p.input_types.get(name, ty) if ty != "i64" else ty, count))
     for name, arr in storage_inputs(p, host).items():
         if name.endswith("#scales"):
             ty, count = "f32", arr.size

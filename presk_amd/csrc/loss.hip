@@ -61,7 +61,9 @@ Shape shape_of(long long M, long long N) {
 // 64-deep blocks at least.  The deep tiles where one round of the CUs holds
 // every item (4096 x 512 x 2048 76.8 -> 69.2 us; 512 x 2048 x 8192, 1100 items,
 // 98 us, deep 104); two a CU are kept to one round where fewer cuts do that
-// (777 x 500 x 10007, 316 tiles of dw and 28 of dx cut 9 ways 105 us, 6 ways 93).
+// (777 x 500 x 10007, 316 tiles of dw and 28 of dx cut 7 ways, 512 items and
+// the mean, 105 us, 6 ways 89).
+constexpr int kBeside = 8;      // workgroups of the launch that are no item: the mean's, and dx's padding to 8
 void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long Nw, long long Kw, Shape* x, Shape* w) {
     const long long kx = up(Kx, 64) / 64, kw = up(Kw, 64) / 64;
     auto items = [&]() { return tiles_of(*x) * x->splits + tiles_of(*w) * w->splits; };
@@ -76,7 +78,7 @@ void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long N
         x->splits = cut(kx);
         w->splits = cut(kw);
         for (Shape* s : {x, w}) {
-            const long long over = items() - slots, t = std::max<long long>(tiles_of(*s), 1);
+            const long long over = items() - (slots - kBeside), t = std::max<long long>(tiles_of(*s), 1);
             const long long less = s->splits - (over + t - 1) / t;
             if (over > 0 && 2 * less > s->splits) s->splits = (int)less;
         }
@@ -84,7 +86,7 @@ void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long N
     };
     if (both(256, 256) >= 192) return;
     both(kDeep128, 256);
-    if (items() <= 256) return;
+    if (items() <= 256 - kBeside) return;
     both(128, 512);
 }
 

@@ -262,6 +262,27 @@ class Builder:
     def cross_entropy_vjp(self, logits, y, ct, name=None):
         return self._prim(lambda dt: L.cross_entropy_vjp([self.op(logits), self.op(y), self.op(ct)], dt), [logits, y, ct], name)
 
+    def head_loss(self, x, w, y, kind):
+        """The mean cross entropy of x . w against y without the logits, as one
+        step (hip.HeadLoss; `kind` "value", or "step" with the gradients of x
+        and w): no nests of the interpreter's, so FAST and one storage type
+        only.  Returns {"loss": its mean and the counted rows (f32 [2]),
+        "ce": each row's loss (f32)} and, with the gradients, "dx" and "dw"."""
+        from . import hip
+        if self.p.mode != hip.FAST or self.realize is not None:
+            raise ValueError("E7005: a head's loss without its logits is built in FAST mode and one storage type")
+        ax = self.axes[x]
+        rows = math.prod(a.len for a in ax[:-1])
+        out = {"loss": "loss", "ce": "ce"}
+        bufs = {"x": self.base.get(x, x), "w": w, "index": y, "mean": "loss", "loss": "ce", "lse": "lse"}
+        if kind == "step":
+            out.update(dx="d.xf", dw="d.head")
+            bufs.update(dx="d.xf", dw="d.head")
+            self.input("d.xf", ax), self.input("d.head", self.axes[w])
+        self.input("loss", A(2)), self.input("ce", ax[:-1]), self.input("lse", ax[:-1])
+        self.p.add_loss(kind, self.dt, rows, self.axes[w][-1].len, bufs, model=ax[-1].len)
+        return out
+
     def dropout_mask(self, x, slot: int, rate: float, name=None):
         """`DropoutMask(rate, key, x)`: a mask of x's shape and the site's
         type, drawn from key `slot` of the program's key table."""
@@ -411,7 +432,7 @@ def site_keys(s: GptShape, step_key: bytes) -> list:
 
 
 def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realize=None, dropout: float = 0.0,
-          step_key: bytes | None = None, optimizer: bool = False) -> tuple:
+          step_key: bytes | None = None, optimizer: bool = False, fused_head: bool = False) -> tuple:
     """The program of config 3 (`train=False`: loss only) or config 4.
     Returns (program, builder, names) with names["loss"] and, for training,
     names["grads"][param] = buffer of its gradient.  `realize`: a
@@ -420,7 +441,10 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
     kernel reads its inputs converted at its edge.  `dropout`: the rate of
     the program's dropout sites (the course's 0.2) with training masks drawn
     from `step_key` (Key::from_seed(0) by default); 0 leaves them out (x * 1,
-    the configs' reading)."""
+    the configs' reading).  `fused_head`: the head, the loss and their
+    reverse mode as one step that keeps no logits (FAST, one storage type):
+    names["loss"] is then f32 [2], the mean loss and the counted tokens, and
+    there is no names["logits"]."""
     from . import hip, keys
     tag = dtype if realize is None else "mixed"
     p = Program(f"gpt-{'step' if train else 'forward'}-{tag}", mode=hip.FAST if mode is None else mode)
@@ -514,19 +538,26 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
                           xn2=xn2, ln2=ln2, u=u, g=g))
         x = xo
     xf, lnf = _layernorm(b, x, "lnf.g", "lnf.b", train, "lnf")
-    logits = b.dot(xf, "head", name="logits")
-    ce = b.cross_entropy(logits, "y", name="ce")
-    loss = b.mean_all(ce, name="loss")
-    names = {"loss": loss, "logits": logits, "grads": {}}
+    if fused_head:
+        head = b.head_loss(xf, "head", "y", "step" if train else "value")
+        names = {"loss": head["loss"], "grads": {}}
+    else:
+        logits = b.dot(xf, "head", name="logits")
+        ce = b.cross_entropy(logits, "y", name="ce")
+        loss = b.mean_all(ce, name="loss")
+        names = {"loss": loss, "logits": logits, "grads": {}}
     if not train:
         return p, b, names
     G = names["grads"]
     # ---- reverse mode -------------------------------------------------------
-    with b.func("MiniGPT.apply.vjp"):
-        dce = b.mean_vjp("one", ce, None)
-        dlogits = b.cross_entropy_vjp(logits, "y", dce)
-        dxf = b.dot_vjp_l(dlogits, "head")
-        G["head"] = b.dot_vjp_r(xf, dlogits, name="d.head")
+    if fused_head:
+        dxf, G["head"] = head["dx"], head["dw"]
+    else:
+        with b.func("MiniGPT.apply.vjp"):
+            dce = b.mean_vjp("one", ce, None)
+            dlogits = b.cross_entropy_vjp(logits, "y", dce)
+            dxf = b.dot_vjp_l(dlogits, "head")
+            G["head"] = b.dot_vjp_r(xf, dlogits, name="d.head")
     dx, G["lnf.g"], G["lnf.b"] = _layernorm_vjp(b, lnf, dxf, "lnf")
     for l in reversed(range(s.L)):
         pr, sv = f"b{l}.", saved[l]

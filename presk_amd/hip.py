@@ -308,7 +308,7 @@ class HipExec:
 # ---- the losses of a large vocabulary ---------------------------------------------
 
 VALUE, GRAD = 1, 2
-_WHAT = {"value": VALUE, "vjp": GRAD, "step": VALUE | GRAD}
+LOSS_WHAT = {"value": VALUE, "vjp": GRAD, "step": VALUE | GRAD}
 
 
 _LOSS_BUFFERS = ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag")
@@ -375,7 +375,7 @@ class Distill:
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
         """Bytes of workspace for `value`, `vjp` or `step` (value_and_grad),
         with the gradients asked for."""
-        return _loss_workspace(self._sizes, _WHAT[kind], dx, dw and self.head)
+        return _loss_workspace(self._sizes, LOSS_WHAT[kind], dx, dw and self.head)
 
     def args(self, kind: str, x=None, w=None, index=None, teacher=None, loss=None, lse=None, mean=None, ct=None, dx=None, dw=None,
              flag=None, work=None) -> LossArgs:
@@ -391,7 +391,7 @@ class Distill:
     def _call(self, kind, stream, **bufs):
         a = self.args(kind, **bufs)
         f = lib().presk_hip_head_loss if self.head else lib().presk_hip_distill
-        check(f(ctypes.byref(a), _WHAT[kind], stream))
+        check(f(ctypes.byref(a), LOSS_WHAT[kind], stream))
 
     def value(self, x, index, teacher, loss=None, lse=None, mean=None, work=None, stream=None):
         self._call("value", stream, x=x, index=index, teacher=teacher, loss=loss, lse=lse, mean=mean, work=work)

@@ -268,9 +268,12 @@ def params_layout(s: LlamaShape):
     return Layout.from_paths(pairs), rename
 
 
-def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None) -> tuple:
+def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None, score: bool = False) -> tuple:
     """The program of `Llama.apply` (the logits).  Returns (program,
-    builder, names) with names["logits"]."""
+    builder, names) with names["logits"].  `score`: the loss of the targets `y`
+    (i64 [batch, seq]; negative: not counted) in the logits' place, which are
+    not kept (FAST, one storage type): names["ce"] each token's, f32,
+    names["loss"] their mean and number, f32 [2]."""
     from . import hip
     p = Program(f"llama-forward-{dtype if realize is None else 'mixed'}", mode=hip.FAST if mode is None else mode)
     b = Builder(p, dtype, realize)
@@ -303,6 +306,9 @@ def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None) -> tuple:
             x = b.binary("add", x2, f, name=pr + "out")
     xn = _rmsnorm(b, x, "norm.g", "norm")
     with b.func("Llama.apply"):
+        if score:
+            b.input("y", A(("batch", s.B), ("seq", s.T)), "idx")
+            return p, b, b.head_loss(xn, "head", "y", "value")
         logits = b.dot(xn, "head", name="logits")
     return p, b, {"logits": logits}
 
@@ -338,11 +344,9 @@ def contraction_flops(s: LlamaShape) -> float:
 
 def input_specs(p: Program) -> dict:
     """name -> (storage type, element count) of every program input."""
-    from .configs import _input_specs
     specs = {}
-    for ln in p.launches:
-        for name, (ty, count) in zip(ln.ins, _input_specs(ln.low)):
-            specs.setdefault(name, (p.input_types.get(name, ty) if ty != "i64" else ty, count))
+    for name, (ty, count) in p.input_specs():
+        specs.setdefault(name, (p.input_types.get(name, ty) if ty != "i64" else ty, count))
     return specs
 
 
@@ -361,6 +365,8 @@ def load_device_inputs(p: Program, s: LlamaShape, seed: int = 5):
         hip.check(lib.presk_hip_fill_normal(buf.ptr, ty.encode(), count, seed * 1000003 + i, mean, std, None))
     rng = np.random.default_rng(seed)
     host = {"ids": rng.integers(0, s.V, size=(s.B, s.T), dtype=np.int64)}
+    if "y" in specs:
+        host["y"] = rng.integers(0, s.V, size=(s.B, s.T), dtype=np.int64)
     host.update({k: np.array([v], np.float64) for k, v in scalar_values(s).items()})
     for name, arr in configs.storage_inputs(p, host).items():
         ty, count = specs[name]

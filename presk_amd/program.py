@@ -94,6 +94,49 @@ class Launch:
         self.table = None
 
 
+class LossStep:
+    """A loss of a large vocabulary (hip.HeadLoss, or hip.Distill where `model`
+    is 0) as a step of a program: `bufs` names the call's buffers; it runs
+    before launch `at`."""
+
+    # the arguments a call writes, those of its value only when it has one
+    VALUE, GRAD = ("loss", "lse", "mean"), ("dx", "dw")
+
+    def __init__(self, at, kind, dtype, rows, vocab, model, top, tied, temperature, bufs):
+        self.at, self.kind, self.dtype, self.bufs = at, kind, dtype, dict(bufs)
+        self.rows, self.vocab, self.model, self.top, self.tied, self.temperature = rows, vocab, model, top, tied, temperature
+        self.op = self.args = None
+
+    def specs(self) -> dict:
+        """argument -> (storage type, element count)."""
+        n, k = self.rows, max(self.top, 1)
+        x, w = n * (self.model or self.vocab), self.model * self.vocab
+        return {"x": (self.dtype, x), "w": (self.dtype, w), "index": ("i64", n * k), "teacher": (self.dtype, n * self.top),
+                "loss": ("f32", n), "lse": ("f32", n), "mean": ("f32", 2), "ct": ("f32", n), "dx": (self.dtype, x), "dw": (self.dtype, w)}
+
+    def writes(self) -> list:
+        names = (self.VALUE if self.kind != "vjp" else ()) + (self.GRAD if self.kind != "value" else ())
+        return [a for a in names if a in self.bufs]
+
+    def reads(self) -> list:
+        return [a for a in self.bufs if a not in self.writes()]
+
+    def prepare(self, bufs: Buffers, flag, name: str):
+        specs = self.specs()
+        if self.model:
+            self.op = hip.HeadLoss(self.dtype, self.rows, self.model, self.vocab, self.tied, self.top, self.temperature)
+        else:
+            self.op = hip.Distill(self.dtype, self.rows, self.vocab, self.top, self.temperature)
+        for a in self.reads():
+            ty, count = bufs.meta[self.bufs[a]]
+            if ty != specs[a][0] or count < specs[a][1]:
+                raise ValueError(f"E7005: {name} reads {self.bufs[a]}, {ty}[{count}], as {a}, {specs[a][0]}[{specs[a][1]}]")
+        for a in self.writes():
+            bufs.alloc(self.bufs[a], *specs[a])
+        work = bufs.alloc(name + ".work", "int8", self.op.workspace(self.kind, "dx" in self.bufs, "dw" in self.bufs))
+        self.args = self.op.args(self.kind, work=work, flag=flag, **{a: bufs.dev[b] for a, b in self.bufs.items()})
+
+
 class Program:
     """Launches in order on one stream; `run` enqueues them all."""
 
@@ -107,8 +150,9 @@ class Program:
         # a host input's storage type when it is not its first reader's (a
         # mixed realization's parameters at rest)
         self.input_types: dict = {}
-        # the prepared sequence: ("launch", Launch) and, where a kernel reads a
-        # buffer of another storage type, ("convert", src, from, dst, to, n)
+        # the prepared sequence: ("launch", Launch), ("loss", LossStep) and,
+        # where a kernel reads a buffer of another storage type, ("convert",
+        # src, from, dst, to, n)
         self.steps: list = []
         # training dropout masks (name, key slot, rate, storage type, count),
         # drawn on the device from a table of 32-byte keys (set_keys) before
@@ -119,6 +163,29 @@ class Program:
         # integer weights: buffer -> (Quant, its quantised axis, its axes),
         # stored as `int8`/`int4` with f32 scales in `<buffer>#scales`
         self.quant: dict = {}
+        # losses of a large vocabulary (LossStep), between the launches
+        self.losses: list = []
+
+    def add_loss(self, kind: str, dtype: str, rows: int, vocab: int, bufs: dict, model: int = 0, top: int = 0, tied: bool = False,
+                 temperature: float = 1.0) -> dict:
+        """Appends the loss of a head x . w (`model` its states' width) or of
+        given logits x (`model` 0): `kind` "value", "vjp" or "step" (both);
+        `bufs` the buffer of each argument of hip.HeadLoss, outputs among
+        them.  Returns bufs."""
+        self.losses.append(LossStep(len(self.launches), kind, dtype, int(rows), int(vocab), int(model), int(top), bool(tied),
+                                    float(temperature), bufs))
+        return bufs
+
+    def input_specs(self):
+        """(name, (storage type, element count)) of everything a step reads, in
+        order; a name read twice comes twice."""
+        from .configs import _input_specs
+        for i, ln in enumerate(self.launches + [None]):
+            for st in self.losses:
+                if st.at == i:
+                    yield from ((st.bufs[a], st.specs()[a]) for a in st.reads())
+            if ln is not None:
+                yield from zip(ln.ins, _input_specs(ln.low))
 
     def add(self, low: L.Lowered, ins: list, out: str, scales=()) -> str:
         """Appends one launch of `low` reading buffers `ins`, writing `out`
@@ -191,7 +258,14 @@ class Program:
         for name, slot, rate, ty, count in self.masks:
             self.bufs.alloc(name, ty, count)
             self.steps.append(("dropout", name, slot, rate, ty, count))
-        for ln in self.launches:
+        def losses(i):
+            for n, st in enumerate(self.losses):
+                if st.at == i:
+                    st.prepare(self.bufs, self._flag, f"loss{n}")
+                    self.steps.append(("loss", st))
+
+        for i, ln in enumerate(self.launches):
+            losses(i)
             c = ln.compiled
             ty = ln.low.dtype if ln.low.out_kind == "real" else "i64"
             names = []
@@ -213,6 +287,7 @@ class Program:
                 ptrs.append(self._flag.ptr)
             ln.table = (ctypes.c_void_p * len(ptrs))(*ptrs)
             self.steps.append(("launch", ln))
+        losses(len(self.launches))
         self._flag.zero()
         return self
 
@@ -225,6 +300,12 @@ class Program:
         _, src, frm, dst, to, n = step
         hip.check(hip.lib().presk_hip_convert(self.bufs.dev[src].ptr, frm.encode(), self.bufs.dev[dst].ptr, to.encode(),
                                               n, self._flag.ptr, stream))
+
+    def _loss(self, step, stream=None):
+        st = step[1]
+        lib = hip.lib()
+        call = lib.presk_hip_head_loss if st.model else lib.presk_hip_distill
+        hip.check(call(ctypes.byref(st.args), hip.LOSS_WHAT[st.kind], stream))
 
     def record(self, graph: bool = True, branches: int = 1):
         """Hands the prepared launch sequence to the executor: `run` then
@@ -245,6 +326,10 @@ class Program:
                 _, src, frm, dst, to, n = st
                 hip.check(lib.presk_hip_batch_add_convert(b, self.bufs.dev[src].ptr, frm.encode(), self.bufs.dev[dst].ptr,
                                                           to.encode(), n, self._flag.ptr))
+                continue
+            if st[0] == "loss":
+                add = lib.presk_hip_batch_add_head_loss if st[1].model else lib.presk_hip_batch_add_distill
+                hip.check(add(b, ctypes.byref(st[1].args), hip.LOSS_WHAT[st[1].kind]))
                 continue
             c = st[1].compiled
             hip.check(lib.presk_hip_batch_add(b, c.handle, st[1].table, 0, max(c.split_bound, 0)))
@@ -274,6 +359,9 @@ class Program:
                 continue
             if st[0] == "convert":
                 self._convert(st, stream)
+                continue
+            if st[0] == "loss":
+                self._loss(st, stream)
                 continue
             c = st[1].compiled
             rc = lib.presk_hip_run(c.handle, st[1].table, 0, max(c.split_bound, 0), stream)
