@@ -257,8 +257,10 @@ int presk_hip_dropout_mask(const void *key, double rate, const char *type, int64
  * presk_hip_head_loss: z = x . w with x [rows, model] and w [model, vocab], or
  * [vocab, model] when `tied`, in pieces of the vocabulary: the logits are not
  * kept, whatever its size.  Gradients dx = dz . w^T and dw = x^T . dz, either
- * of which may be null.  The products accumulate in f32; in 16-bit storage dz
- * is rounded to the storage type before them (scaled to its range in f16).
+ * of which may be null.  The products accumulate in f32; in 16-bit storage the
+ * factor ct[r] * (exp(u[r] - lse[r]) - t[r]) of dz is rounded to the storage type
+ * before them (by a power of two in f16's range), T and the mean's 1 / count
+ * come after.
  * A row of x that does not count still enters dw times zero, so it must be
  * finite.
  * presk_hip_distill: z = x, given (model 0, w null, top >= 1); dx is dz.

@@ -357,7 +357,7 @@ struct Call {
             g->tiles_m = h.tiles_m;
             g->tiles_n = h.tiles_n;
             g->splits = h.splits;
-            g->scale = q.st == kF16 ? at<float>(q.scale) : nullptr;
+            g->scale = at<float>(q.scale);
             g->flag = a.flag;
         }
         if (a.dx) {
@@ -424,7 +424,7 @@ struct Call {
             m.plane = q.rows * q.ldz;
             LossJoint j = joint_args(m, at<void>(q.P), up(q.V, 64), q.st);
             j.orows = q.prows;
-            j.scale = q.st == kF16 ? at<float>(q.scale) : nullptr;
+            j.scale = at<float>(q.scale);
             j.flag = nullptr;
             LOSS_TRY(loss_joint(j, s));
             return pair(x, w, 0, q.V);
@@ -576,7 +576,8 @@ struct Call {
             r.coef = at<float>(q.coef);
             r.ct = a.ct;
             r.mean_in = !a.ct && !q.value ? a.mean : nullptr;
-            r.scale = q.head && q.st == kF16 ? at<float>(q.scale) : nullptr;
+            r.scale = q.head && q.st != kF32 ? at<float>(q.scale) : nullptr;
+            r.shift = q.st == kF16;
         }
         r.count = at<int>(q.count);
         r.most = at<float>(q.most);

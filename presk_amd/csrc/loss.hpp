@@ -137,7 +137,8 @@ struct LossRows {
     const int* count;
     const float* most;
     int parts;
-    float* scale;               // out (f16): the inverse of the factor in coef (null: none)
+    float* scale;               // out: the factor of all rows, which coef is without (null: it has it)
+    bool shift;                 // f16: coef by a power of two that its range holds best
     float* mean;                // {mean, count} or null: in the same launch where loss_rows_mean(rows)
 };
 bool loss_rows_mean(long long rows);
@@ -177,7 +178,7 @@ struct LossJoint {
     const int* count;
     const float* most;
     int parts;
-    float* scale;               // f16 products follow: the inverse of a power of two in the cotangent
+    float* scale;               // as in LossRows (f16 outputs shifted), where products follow
     void* out;                  // of type `to`: the logits' own, or 16 bits of f32 logits
     int to;
     long long ldo;
