@@ -239,13 +239,14 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         }
         if (q.grad) {
             q.P = take(2 * q.prows * up(std::min<long long>(q.piece, q.V), 64));
-            q.acc = take(a.dx && q.pieces > 1 ? 4 * q.rows * q.D : 0);
+            q.acc = take(a.dx && q.pieces > 1 ? 4 * q.rows * up(q.D, 4) : 0);
             long long px = 0, pw = 0;
             for (long long v = 0; v < q.V; v += q.piece) {
                 Shape x, w;
                 pair_shapes(q, a, (int)std::min<long long>(q.piece, q.V - v), &x, &w);
-                if (a.dx && x.splits > 1) px = std::max(px, 4 * x.splits * q.rows * q.D);
-                if (a.dw && w.splits > 1) pw = std::max(pw, 4ll * w.splits * q.D * std::min<long long>(q.piece, q.V - v));
+                if (a.dx && x.splits > 1) px = std::max(px, 4 * x.splits * q.rows * up(q.D, 4));
+                const long long n = std::min<long long>(q.piece, q.V - v);
+                if (a.dw && w.splits > 1) pw = std::max(pw, 4ll * w.splits * (a.tied ? n * up(q.D, 4) : q.D * up(n, 4)));
             }
             q.partx = take(px);
             q.partw = take(pw);
@@ -374,7 +375,7 @@ struct Call {
             dx.N = q.D;
             dx.K = (int)pld;
             dx.acc = at<float>(q.acc);
-            dx.lda = q.D;
+            dx.lda = up(q.D, 4);
             dx.acc_in = v > 0;
             dx.part = at<float>(q.partx);
             dx.C = v + n >= q.V ? a.dx : nullptr;
@@ -395,7 +396,7 @@ struct Call {
             dw.M = a.tied ? n : q.D;
             dw.N = a.tied ? q.D : n;
             dw.K = (int)q.prows;
-            dw.lda = dw.N;
+            dw.lda = up(dw.N, 4);
             dw.part = at<float>(q.partw);
             dw.C = (unsigned short*)a.dw + (a.tied ? v * q.D : v);
             dw.ldc = a.tied ? q.D : q.V;

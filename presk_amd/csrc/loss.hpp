@@ -69,7 +69,7 @@ struct LossGemm {
     void* C;                    // 16-bit, row stride ldc (null: the f32 sums stay in acc)
     long long ldc;
     float* acc;                 // [M][lda] f32: added to (acc_in), written where C is null
-    long long lda;
+    long long lda;              // (a multiple of 4)
     bool acc_in;
     float* part;                // [splits][M][lda] f32 (splits > 1)
     const float* scale;         // the sums' factor, one float of device memory

@@ -169,11 +169,16 @@ __device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 acc) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
 }
 
+// two values rounded into one word, the first in its low half
 template <int ST>
-__device__ __forceinline__ unsigned short narrow(float v, bool& ovf) {
-    if constexpr (ST == kBF16) return pk_f32_to_bf16(v);
-    ovf |= pk_overflows_f16(v);
-    return pk_f32_to_f16(v);
+__device__ __forceinline__ unsigned narrow2(float a, float b) {
+    if constexpr (ST == kBF16) {
+        unsigned r;
+        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+        return r;
+    } else {
+        return (unsigned)pk_f32_to_f16(a) | (unsigned)pk_f32_to_f16(b) << 16;
+    }
 }
 
 // The column, of the wave's 64, of a lane's sum e of column fragment j
@@ -391,8 +396,9 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
             g.pa[at] = ta;
         }
     } else if constexpr (EPI == kEpiP) {
+        // (f16 cotangents stay below 2^15: no overflow to look for)
         unsigned short* const ct = (unsigned short*)smem;   // [BM][CLD]
-        bool ovf = false;
+        const bool edge = n0 + BN > g.cols;
 #pragma unroll
         for (int i = 0; i < WM; ++i) {
             const int row = wm + i * 32 + (lane & 31), m = m0 + row;
@@ -409,18 +415,24 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
                     for (int e = 0; e < 16; ++e)
                         if (col == col_of(j, e, lane)) acc[i][j][e] -= p;
             });
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (n0 + wn + col_of(j, e, lane) >= g.cols) acc[i][j][e] = 0.f;
+            }
 #pragma unroll
             for (int j = 0; j < WN; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    u16x4 v;
+                    float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int col = col_of(j, 4 * q + e, lane);
-                        const float x = coef == 0.f || n0 + wn + col >= g.cols ? 0.f : acc[i][j][4 * q + e] * coef;
-                        v[e] = narrow<ST>(x, ovf);
-                    }
-                    *(u16x4*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
+                    for (int e = 0; e < 4; ++e) x[e] = coef == 0.f ? 0.f : acc[i][j][4 * q + e] * coef;
+                    uint2 v;
+                    v.x = narrow2<ST>(x[0], x[1]);
+                    v.y = narrow2<ST>(x[2], x[3]);
+                    *(uint2*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
                 }
         }
         __syncthreads();
@@ -432,11 +444,14 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
         }
     } else {
         const float scale = g.scale ? *g.scale : 1.f;
-        if (g.splits > 1 || !g.C) {
-            // f32 sums: four consecutive columns of a row from the registers
+        if (g.splits > 1 || !g.C || g.acc_in) {
+            // four consecutive columns of a row from the registers: f32 sums
+            // (rows hold whole fours), or with those of the pieces before
+            // added the 16-bit result
             float* const out = g.splits > 1 ? g.part + (long long)split * g.M * g.lda : g.acc;
-            const bool add = g.splits <= 1 && g.acc_in, vec = g.lda % 4 == 0;   // (then rows hold whole fours)
+            const bool add = g.splits <= 1 && g.acc_in, last = add && g.C;
             const float f = g.splits > 1 ? 1.f : scale;
+            bool ovf = false;
 #pragma unroll
             for (int i = 0; i < WM; ++i) {
                 const int m = m0 + wm + i * 32 + (lane & 31);
@@ -447,56 +462,69 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int n = n0 + wn + col_of(j, 4 * q, lane);
+                        if (n >= g.N) continue;
                         f32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * f;
-                        if (vec && n < g.N) {
-                            if (add) v += *(const f32x4*)(row + n);
+                        if (add) v += *(const f32x4*)(row + n);
+                        if (!last) {
                             *(f32x4*)(row + n) = v;
-                        } else {
-                            for (int e = 0; e < 4 && n + e < g.N; ++e) row[n + e] = add ? row[n + e] + v[e] : v[e];
+                            continue;
                         }
+                        unsigned short* const at = (unsigned short*)g.C + (long long)m * g.ldc + n;
+                        const uint2 h{narrow2<ST>(v[0], v[1]), narrow2<ST>(v[2], v[3])};
+                        if (n + 4 <= g.N) {
+                            __builtin_memcpy(at, &h, 8);
+                        } else {
+                            at[0] = (unsigned short)h.x;
+                            if (n + 1 < g.N) at[1] = (unsigned short)(h.x >> 16);
+                            if (n + 2 < g.N) at[2] = (unsigned short)h.y;
+                        }
+                        if constexpr (ST == kF16)
+                            for (int e = 0; e < 4; ++e) ovf |= n + e < g.N && pk_overflows_f16(v[e]);
                     }
             }
+            if (ovf && g.flag) atomicOr(g.flag, 1u);
         } else {
             unsigned short* const ct = (unsigned short*)smem;
-            bool ovf = false;
+            // the largest finite value (past the operands' ends stand values
+            // from inside them, or 0)
+            unsigned worst = 0;
 #pragma unroll
             for (int i = 0; i < WM; ++i) {
-                const int row = wm + i * 32 + (lane & 31), m = m0 + row;
+                const int row = wm + i * 32 + (lane & 31);
 #pragma unroll
                 for (int j = 0; j < WN; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int c = wn + col_of(j, 4 * q, lane);
-                        u16x4 v;
+                        float x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float x = acc[i][j][4 * q + e] * scale;
-                            const bool in = m < g.M && n0 + c + e < g.N;
-                            if (g.acc_in && in) x += g.acc[(long long)m * g.lda + n0 + c + e];
-                            bool o = false;
-                            v[e] = narrow<ST>(x, o);
-                            ovf |= o && in;
+                            x[e] = acc[i][j][4 * q + e] * scale;
+                            if constexpr (ST == kF16) {
+                                const unsigned b = pk_bits(x[e]) & 0x7fffffffu;
+                                worst = max(worst, b < 0x7f800000u ? b : 0u);
+                            }
                         }
-                        *(u16x4*)&ct[row * CLD + c] = v;
+                        uint2 v;
+                        v.x = narrow2<ST>(x[0], x[1]);
+                        v.y = narrow2<ST>(x[2], x[3]);
+                        *(uint2*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
                     }
             }
-            if (ovf && g.flag) atomicOr(g.flag, 1u);
+            if (ST == kF16 && g.flag && pk_overflows_f16(pk_float(worst))) atomicOr(g.flag, 1u);
             __syncthreads();
+            // 16 bytes a thread, at whatever element a row starts
             unsigned short* const C = (unsigned short*)g.C;
-            if (g.ldc % 8 == 0 && g.N % 8 == 0 && (size_t)C % 16 == 0) {
-                constexpr int VPR = BN / 8;
-                for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
-                    const int r = u / VPR, c = u % VPR * 8;
-                    if (m0 + r < g.M && n0 + c < g.N)
-                        *(u16x8*)(C + (long long)(m0 + r) * g.ldc + n0 + c) = *(const u16x8*)&ct[r * CLD + c];
-                }
-            } else {
-                for (int u = threadIdx.x; u < BM * BN; u += NTH) {
-                    const int r = u / BN, c = u % BN;
-                    if (m0 + r < g.M && n0 + c < g.N) C[(long long)(m0 + r) * g.ldc + n0 + c] = ct[r * CLD + c];
-                }
+            constexpr int VPR = BN / 8;
+            for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
+                const int r = u / VPR, c = u % VPR * 8;
+                if (m0 + r >= g.M) continue;
+                unsigned short* const at = C + (long long)(m0 + r) * g.ldc + n0 + c;
+                if (n0 + c + 8 <= g.N)
+                    __builtin_memcpy(at, &ct[r * CLD + c], 16);
+                else
+                    for (int e = 0; n0 + c + e < g.N; ++e) at[e] = ct[r * CLD + c + e];
             }
         }
     }
