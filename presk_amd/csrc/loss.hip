@@ -415,7 +415,7 @@ struct Call {
             // one piece: its logits in f32, their cotangent from whole rows
             LOSS_TRY(weights(0, q.V, false, &w));
             LossGemm g = logits(x, w, 0, q.V, q.zs);
-            g.acc = g.part = at<float>(q.z);
+            g.part = at<float>(q.z);
             g.lda = q.ldz;
             const LossPrep none{};
             const LossPrep& p = a.top ? none : prep;

@@ -71,12 +71,12 @@ struct LossGemm {
     float* acc;                 // [M][lda] f32: added to (acc_in), written where C is null
     long long lda;              // (a multiple of 4)
     bool acc_in;
-    float* part;                // [splits][M][lda] f32 (splits > 1)
+    float* part;                // [splits][M][lda] f32 (splits > 1, and logits)
     const float* scale;         // the sums' factor, one float of device memory
     unsigned* flag;
 };
 
-enum LossEpi { kEpiStats = 0, kEpiP = 1, kEpiOut = 2 };
+enum LossEpi { kEpiStats, kEpiP, kEpiZ, kEpiDx, kEpiDw };
 
 // What a launch of products may do beside them, in workgroups of its own: the
 // mean of the counted rows' losses, and the counts of rows of one column each.
@@ -110,7 +110,7 @@ struct LossPrep {
 constexpr int kDeep128 = 130;
 hipError_t loss_gemm_bf16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
 hipError_t loss_gemm_f16(const LossGemm& g, LossEpi epi, bool bkc, int tile, hipStream_t s);
-// z = x . w in f32 (kEpiOut, A k-contiguous), the rows' targets counted beside it
+// z = x . w in f32 (kEpiZ, A k-contiguous), the rows' targets counted beside it
 hipError_t loss_logits_bf16(const LossGemm& g, bool bkc, int tile, const LossPrep& p, hipStream_t s);
 hipError_t loss_logits_f16(const LossGemm& g, bool bkc, int tile, const LossPrep& p, hipStream_t s);
 // dx and dw in one launch (either may have no tiles), and the mean

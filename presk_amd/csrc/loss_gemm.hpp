@@ -444,14 +444,30 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
         }
     } else {
         const float scale = g.scale ? *g.scale : 1.f;
-        if (g.splits > 1 || !g.C || g.acc_in) {
-            // four consecutive columns of a row from the registers: f32 sums
-            // (rows hold whole fours), or with those of the pieces before
-            // added the 16-bit result
-            float* const out = g.splits > 1 ? g.part + (long long)split * g.M * g.lda : g.acc;
-            const bool add = g.splits <= 1 && g.acc_in, last = add && g.C;
-            const float f = g.splits > 1 ? 1.f : scale;
-            bool ovf = false;
+        const bool sums = EPI == kEpiZ || g.splits > 1 || !g.C;   // f32 (rows hold whole fours)
+        float* const out = EPI == kEpiZ || g.splits > 1 ? g.part + (long long)split * g.M * g.lda : g.acc;
+        float f = EPI == kEpiZ || g.splits > 1 ? 1.f : scale;
+        if (EPI == kEpiDx && g.splits <= 1 && g.acc_in) {
+            // the pieces before
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                const int m = m0 + wm + i * 32 + (lane & 31);
+                const float* const row = out + (long long)m * g.lda;
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int n = n0 + wn + col_of(j, 4 * q, lane);
+                        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                        if (m < g.M && n < g.N) v = *(const f32x4*)(row + n);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = acc[i][j][4 * q + e] * f + v[e];
+                    }
+            }
+            f = 1.f;
+        }
+        if (sums) {
+            // four consecutive columns of a row from the registers
 #pragma unroll
             for (int i = 0; i < WM; ++i) {
                 const int m = m0 + wm + i * 32 + (lane & 31);
@@ -462,29 +478,12 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int n = n0 + wn + col_of(j, 4 * q, lane);
-                        if (n >= g.N) continue;
                         f32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * f;
-                        if (add) v += *(const f32x4*)(row + n);
-                        if (!last) {
-                            *(f32x4*)(row + n) = v;
-                            continue;
-                        }
-                        unsigned short* const at = (unsigned short*)g.C + (long long)m * g.ldc + n;
-                        const uint2 h{narrow2<ST>(v[0], v[1]), narrow2<ST>(v[2], v[3])};
-                        if (n + 4 <= g.N) {
-                            __builtin_memcpy(at, &h, 8);
-                        } else {
-                            at[0] = (unsigned short)h.x;
-                            if (n + 1 < g.N) at[1] = (unsigned short)(h.x >> 16);
-                            if (n + 2 < g.N) at[2] = (unsigned short)h.y;
-                        }
-                        if constexpr (ST == kF16)
-                            for (int e = 0; e < 4; ++e) ovf |= n + e < g.N && pk_overflows_f16(v[e]);
+                        if (n < g.N) *(f32x4*)(row + n) = v;
                     }
             }
-            if (ovf && g.flag) atomicOr(g.flag, 1u);
         } else {
             unsigned short* const ct = (unsigned short*)smem;
             // the largest finite value (past the operands' ends stand values
@@ -500,7 +499,7 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
                         float x[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            x[e] = acc[i][j][4 * q + e] * scale;
+                            x[e] = acc[i][j][4 * q + e] * f;
                             if constexpr (ST == kF16) {
                                 const unsigned b = pk_bits(x[e]) & 0x7fffffffu;
                                 worst = max(worst, b < 0x7f800000u ? b : 0u);
@@ -521,10 +520,12 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
                 const int r = u / VPR, c = u % VPR * 8;
                 if (m0 + r >= g.M) continue;
                 unsigned short* const at = C + (long long)(m0 + r) * g.ldc + n0 + c;
+                const u16x8 v = *(const u16x8*)&ct[r * CLD + c];
                 if (n0 + c + 8 <= g.N)
-                    __builtin_memcpy(at, &ct[r * CLD + c], 16);
+                    __builtin_memcpy(at, &v, 16);
                 else
-                    for (int e = 0; n0 + c + e < g.N; ++e) at[e] = ct[r * CLD + c + e];
+                    for (int e = 0; e < 7; ++e)
+                        if (n0 + c + e < g.N) at[e] = v[e];
             }
         }
     }
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(TL::NTH, 2) loss_gemm_kernel(LossGemm g) {
 template <int ST, bool BKC, typename TL>
 __global__ void __launch_bounds__(TL::NTH, 2) loss_logits_kernel(LossGemm g, unsigned items, LossPrep p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
-    if (blockIdx.x < items) tile_of<ST, true, BKC, TL, kEpiOut>(g, blockIdx.x, items, smem);
+    if (blockIdx.x < items) tile_of<ST, true, BKC, TL, kEpiZ>(g, blockIdx.x, items, smem);
     else prep_one<TL::NTH>(p, (int)(blockIdx.x - items));
 }
 
@@ -550,9 +551,9 @@ __global__ void __launch_bounds__(TL::NTH, 2) loss_pair_kernel(LossGemm x, LossG
     __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
     const unsigned id = blockIdx.x;
     if (id < nx8) {
-        if (id < nx) tile_of<ST, true, XBKC, TL, kEpiOut>(x, id, nx, smem);
+        if (id < nx) tile_of<ST, true, XBKC, TL, kEpiDx>(x, id, nx, smem);
     } else if (id < nx8 + nw) {
-        tile_of<ST, false, false, TL, kEpiOut>(w, id - nx8, nw, smem);
+        tile_of<ST, false, false, TL, kEpiDw>(w, id - nx8, nw, smem);
     } else {
         write_mean<TL::NTH>(m);
     }
