@@ -31,7 +31,8 @@ int storage_code(const char* name) {
 
 constexpr long long kMany = 1ll << 22;          // rows, model and a head's vocabulary stay below this
 constexpr long long kPieceBytes = 128ll << 20;  // a piece's logits or their cotangent
-constexpr long long kOnceBytes = 256ll << 20;   // f32 logits that are one piece: as many as the Infinity Cache holds
+constexpr long long kOnceBytes = 256ll << 20;   // f32 logits that are one piece: as many as the Infinity Cache holds, ...
+constexpr long long kKeepBytes = 4ll << 30;     // ... and where the gradient follows the value, so that they stay for it
 constexpr int kPieceCols = 256;                 // a piece is a multiple of these
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
@@ -123,7 +124,7 @@ struct Plan {
     int st, esz, D, V, k, parts, slots, nblocks;
     long long rows, prows;
     float c;
-    bool packx, packw, once, counted;   // once: f32 logits of the whole vocabulary; counted: counts are taken
+    bool packx, packw, once, joint, counted;   // once: f32 logits of the whole vocabulary, joint: in one kernel's registers; counted: counts are taken
     int Dp, piece, pieces, spiece;    // spiece: columns a pass of row sums takes at once
     long long ldz;
     Shape zs;                         // once
@@ -208,7 +209,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         // one piece, or as wide as kPieceBytes allow (in f32 of equal width)
         const long long bytes = half ? 2 : 4;
         long long cols = kPieceBytes / (bytes * std::max<long long>(q.prows, 1)) / kPieceCols * kPieceCols;
-        if (4 * q.rows * up(q.V, 4) <= kOnceBytes) cols = up(q.V, kPieceCols);
+        if (4 * q.rows * up(q.V, 4) <= (q.value && q.grad ? kKeepBytes : kOnceBytes)) cols = up(q.V, kPieceCols);
         if (q.st == kF32) cols = std::min(cols, ((1ll << 31) - 1) / std::max<long long>(q.rows, 1) / kPieceCols * kPieceCols);
         cols = std::min(std::max<long long>(cols, kPieceCols), up(q.V, kPieceCols));
         q.piece = half ? piece_of(q.rows, q.V, cols) : (int)up((q.V + up(q.V, cols) / cols - 1) / (up(q.V, cols) / cols), kPieceCols);
@@ -219,8 +220,13 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         q.packw = (a.tied ? q.D : q.V) % 8 != 0;
         q.Dp = (int)up(q.D, 64);
         q.ldz = up(q.V, 4);
-        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kOnceBytes && q.V <= 65536;
+        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kKeepBytes;
         if (q.once) {
+            LossMatrix m{};
+            m.storage = kF32;
+            m.cols = q.V;
+            q.joint = loss_joint_fits(m);
+            if (!q.joint) q.slots = loss_chunks(q.rows, q.V);
             q.pieces = 1;
             q.piece = (int)up(q.V, kPieceCols);
         }
@@ -234,7 +240,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         q.xp = take(q.packx ? 2 * q.rows * q.Dp : 0);
         q.wp = take(!q.packw ? 0 : a.tied ? 2ll * q.piece * q.Dp : 2ll * q.D * up(q.piece, 64));
         if (q.once) {
-            q.zs = logits_of(q.rows, q.V, q.D);
+            q.zs = q.joint ? logits_of(q.rows, q.V, q.D) : shape_of(q.rows, q.V);
             q.z = take(4ll * q.zs.splits * q.rows * q.ldz);
         }
         if (q.grad) {
@@ -423,11 +429,17 @@ struct Call {
             LossMatrix m = matrix(at<float>(q.z), q.ldz, kF32, 0, q.V);
             m.planes = q.zs.splits;
             m.plane = q.rows * q.ldz;
-            LossJoint j = joint_args(m, at<void>(q.P), up(q.V, 64), q.st);
-            j.orows = q.prows;
-            j.scale = at<float>(q.scale);
-            j.flag = nullptr;
-            LOSS_TRY(loss_joint(j, s));
+            const LossTo to{at<void>(q.P), q.st, up(q.V, 64), q.prows};
+            if (q.joint) {
+                LossJoint j = joint_args(m, to);
+                j.scale = at<float>(q.scale);
+                j.flag = nullptr;
+                LOSS_TRY(loss_joint(j, s));
+            } else {
+                LOSS_TRY(value_of(m, 0));
+                LOSS_TRY(rows_of());
+                LOSS_TRY(loss_grad(m, lse, at<float>(q.coef), to, nullptr, s));
+            }
             return pair(x, w, 0, q.V);
         }
         if (q.value) {
@@ -485,7 +497,7 @@ struct Call {
         m.planes = 1;
         return m;
     }
-    LossJoint joint_args(const LossMatrix& m, void* out, long long ldo, int to) const {
+    LossJoint joint_args(const LossMatrix& m, const LossTo& to) const {
         LossJoint j{};
         j.m = m;
         j.temperature = (float)a.temperature;
@@ -495,9 +507,7 @@ struct Call {
         j.count = at<int>(q.count);
         j.most = at<float>(q.most);
         j.parts = q.parts;
-        j.out = out;
         j.to = to;
-        j.ldo = ldo;
         j.flag = a.flag;
         return j;
     }
@@ -515,10 +525,11 @@ struct Call {
         };
         // a vocabulary of one piece: its logits, then their cotangent in place
         const LossMatrix whole = matrix(z, q.ldz, kF32, 0, q.V);
+        const LossTo to{z, kF32, q.ldz, q.rows};
         const bool once = q.value && q.grad && q.pieces == 1 && loss_joint_fits(whole);
         if (once) {
             LOSS_TRY(logits(0, q.V));
-            LOSS_TRY(loss_joint(joint_args(whole, z, q.ldz, kF32), s));
+            LOSS_TRY(loss_joint(joint_args(whole, to), s));
         } else {
             int slot = 0;
             for (long long v = 0; v < q.V && q.value; v += q.piece) {
@@ -532,8 +543,8 @@ struct Call {
         for (long long v = 0; v < q.V && q.grad; v += q.piece) {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
             if (!once) {
-                LOSS_TRY(logits(v, n));
-                LOSS_TRY(loss_grad(matrix(z, q.ldz, kF32, v, n), lse, at<float>(q.coef), z, q.ldz, nullptr, s));
+                if (!q.value || q.pieces > 1) LOSS_TRY(logits(v, n));
+                LOSS_TRY(loss_grad(matrix(z, q.ldz, kF32, v, n), lse, at<float>(q.coef), to, nullptr, s));
             }
             float* const dx = (float*)a.dx;
             if (dx)
@@ -548,11 +559,12 @@ struct Call {
 
     hipError_t given(const float* lse) {
         LossMatrix m = matrix(a.x, q.V, q.st, 0, q.V);
-        if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, a.dx, q.V, q.st), s);
+        const LossTo to{a.dx, q.st, q.V, q.rows};
+        if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, to), s);
         if (q.value) LOSS_TRY(value_of(m, 0));
         LOSS_TRY(rows_of());
         if (!q.grad) return hipSuccess;
-        return loss_grad(m, lse, at<float>(q.coef), a.dx, q.V, a.flag, s);
+        return loss_grad(m, lse, at<float>(q.coef), to, a.flag, s);
     }
 
     LossMean mean_args() const { return LossMean{loss_out(), q.rows, at<int>(q.count), q.parts, t.index, a.mean}; }
@@ -564,7 +576,7 @@ struct Call {
         r.ps = at<float>(q.ps);
         r.pa = at<float>(q.pa);
         // (one chunk of logits in memory: the rows are done)
-        r.slots = q.slots == 1 && (!q.head || q.st == kF32) ? 0 : q.slots;
+        r.slots = q.slots == 1 && (!q.head || q.st == kF32 || q.once) ? 0 : q.slots;
         r.t = t;
         r.rows = q.rows;
         r.temperature = (float)a.temperature;
@@ -633,7 +645,6 @@ std::string loss_check(const presk_hip_loss& a, int what, bool head) {
     auto no = [&](const std::string& why) { return std::string("E10001: ") + op + ": " + why; };
     if (st < 0) return std::string("E7005: ") + op + " in storage type `" + (a.dtype ? a.dtype : "") + "` (f32, bf16 or f16)";
     if (what < 1 || what > 3) return no("what is neither VALUE nor GRAD nor both");
-    const bool value = what & PRESK_HIP_LOSS_VALUE, grad = what & PRESK_HIP_LOSS_GRAD;
     if (a.rows < 0 || a.rows >= kMany) return no("rows " + std::to_string(a.rows) + " not in [0, 2^22)");
     if (head ? a.model < 1 || a.model >= kMany : a.model != 0)
         return no("model " + std::to_string(a.model) + (head ? " not in [1, 2^22)" : ", which is 0 where the logits are given"));

@@ -165,9 +165,15 @@ struct LossDone {
 };
 int loss_chunks(long long rows, int cols);
 hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s);
-// the logits' cotangent, coef * (softmax - target), in the logits' type (in place or not)
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag,
-                     hipStream_t s);
+// Where a cotangent goes: in the logits' type (in place or not), or f32 logits'
+// in 16 bits, zero then past their columns, and past their rows up to `rows`.
+struct LossTo {
+    void* p;
+    int storage;
+    long long ld, rows;
+};
+// the logits' cotangent, coef * (softmax - target)
+hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s);
 // both of whole rows, each read once and held in registers: lse, loss (either
 // may be null) and the cotangent for ct, or for the mean over `count` (null ct)
 struct LossJoint {
@@ -179,10 +185,7 @@ struct LossJoint {
     const float* most;
     int parts;
     float* scale;               // as in LossRows (f16 outputs shifted), where products follow
-    void* out;                  // of type `to`: the logits' own, or 16 bits of f32 logits
-    int to;
-    long long ldo;
-    long long orows;            // rows written, zero past m.rows; in 16 bits of f32 columns too, up to ldo
+    LossTo to;
     unsigned* flag;
 };
 bool loss_joint_fits(const LossMatrix& m);

@@ -375,17 +375,22 @@ __device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, flo
 
 // out = coef * (2^(u - lse) - t).  The target's columns are written after the
 // row's others, by a thread each, once the stores of this workgroup (or wave)
-// have reached memory.
-template <int ST, int G>
-__global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* lse, const float* coef, void* out, long long ldo,
-                                                   unsigned* flag, int chunk) {
-    typedef typename Elem<ST>::S S;
-    constexpr int V = Elem<ST>::V;
+// have reached memory.  SI the logits' type, SO the output's.
+template <int SI, int SO, int G>
+__global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* lse, const float* coef, LossTo to, unsigned* flag,
+                                                   int chunk) {
+    typedef typename Elem<SI>::S S;
+    typedef typename Elem<SO>::S O;
+    constexpr int V = Elem<SI>::V;
     const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
-    if (r >= a.rows) return;
     const int t = threadIdx.x % G, lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
+    O* const o = (O*)to.p + r * to.ld + lo;
+    const int end = (int)((hi == a.cols && SI != SO ? to.ld : hi) - lo);   // columns written
+    if (r >= a.rows) {
+        for (int q = t; q < end && r < to.rows; q += G) o[q] = (O)0;
+        return;
+    }
     const S* const z = (const S*)a.z + r * a.ld + lo;
-    S* const o = (S*)out + r * ldo + lo;
     const float c = coef[r], l = lse[r] * kLog2e;
     const int k = a.t.k, first = a.col0 + lo, n = hi - lo;
     bool ovf = false;
@@ -394,11 +399,11 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
     float zt[E];
     for (int q = 0; q < E && t + q * G < k; ++q) {
         const int col = slot_col(a.t, r, t + q * G) - first;
-        zt[q] = col >= 0 && col < n ? widen<ST>(z[col]) : 0.f;
+        zt[q] = col >= 0 && col < n ? widen<SI>(z[col]) : 0.f;
     }
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
-    const Split<ST> sp(z, n);
+    const Split<SI> sp(z, n);
     constexpr int U = 2;
     for (int i = t; i < sp.n; i += U * G) {
         u32x4 v[U];
@@ -408,21 +413,30 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i + u * G < sp.n) {
-                u32x4 w{};
+                O* const at = o + sp.head + (long long)(i + u * G) * V;
+                if constexpr (SI == SO) {
+                    u32x4 w{};
 #pragma unroll
-                for (int e = 0; e < V; ++e) set_elem<ST>(w, e, cotangent<ST>(elem<ST>(v[u], e), a.c, l, 0.f, c, ovf));
-                store_vec(o + sp.head + (long long)(i + u * G) * V, w);
+                    for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[u], e), a.c, l, 0.f, c, ovf));
+                    store_vec(at, w);
+                } else {
+                    O w[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[u], e), a.c, l, 0.f, c, ovf);
+                    __builtin_memcpy(at, w, sizeof w);
+                }
             }
     }
-    if (t < sp.edges()) o[sp.edge(t)] = cotangent<ST>(widen<ST>(z[sp.edge(t)]), a.c, l, 0.f, c, ovf);
+    if (t < sp.edges()) o[sp.edge(t)] = cotangent<SO>(widen<SI>(z[sp.edge(t)]), a.c, l, 0.f, c, ovf);
+    for (int q = n + t; q < end; q += G) o[q] = (O)0;
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
     for (int q = 0; q < E && t + q * G < k; ++q) {
         const int e = t + q * G, col = slot_col(a.t, r, e) - first;
         float p;
-        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<ST>(zt[q], a.c, l, p, c, ovf);
+        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<SO>(zt[q], a.c, l, p, c, ovf);
     }
-    if (ST == kF16 && ovf && flag) atomicOr(flag, 1u);
+    if (SO == kF16 && ovf && flag) atomicOr(flag, 1u);
 }
 
 // Whole rows, read once: G threads a row (16, 64: 16 or four rows a workgroup), R
@@ -441,11 +455,11 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
     const long long r = G == 16 ? (long long)blockIdx.x * 16 + threadIdx.x / 16
                         : G == 64 ? (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : (long long)blockIdx.x;
     const int t = threadIdx.x % G, k = tg.k, n = a.m.cols;
-    O* const o = (O*)a.out + r * a.ldo;
+    O* const o = (O*)a.to.p + r * a.to.ld;
     // (all threads of a row)
     if (r >= a.m.rows) {
-        if (r < a.orows)
-            for (long long c = t; c < a.ldo; c += G) o[c] = (O)0;
+        if (r < a.to.rows)
+            for (long long c = t; c < a.to.ld; c += G) o[c] = (O)0;
         return;
     }
     const S* const z = (const S*)a.m.z + r * a.m.ld;
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
         }
     if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, l2, 0.f, c, ovf);
     if constexpr (SI != SO)
-        for (long long q = n + t; q < a.ldo; q += G) o[q] = (O)0;
+        for (long long q = n + t; q < a.to.ld; q += G) o[q] = (O)0;
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
 #pragma unroll
@@ -651,13 +665,12 @@ hipError_t stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0
     return hipGetLastError();
 }
 
-template <int ST>
-hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag, hipStream_t s) {
+template <int SI, int SO>
+hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
     const int chunks = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, chunks);
-    if (m.cols <= 1024)
-        grad_kernel<ST, 64><<<dim3((unsigned)((m.rows + 3) / 4)), 256, 0, s>>>(m, lse, coef, out, ldo, flag, m.cols);
-    else
-        grad_kernel<ST, 256><<<dim3((unsigned)m.rows, (unsigned)chunks), 256, 0, s>>>(m, lse, coef, out, ldo, flag, chunk);
+    const unsigned rows = (unsigned)std::max(m.rows, to.rows);
+    if (m.cols <= 1024) grad_kernel<SI, SO, 64><<<dim3((rows + 3) / 4), 256, 0, s>>>(m, lse, coef, to, flag, m.cols);
+    else grad_kernel<SI, SO, 256><<<dim3(rows, (unsigned)chunks), 256, 0, s>>>(m, lse, coef, to, flag, chunk);
     return hipGetLastError();
 }
 
@@ -673,7 +686,7 @@ void joint_of(const LossJoint& a, long long rows, hipStream_t s) {
 template <int SI, int SO, bool NT>
 hipError_t joint(const LossJoint& a, hipStream_t s) {
     const int nv = a.m.cols / Elem<SI>::V;
-    const long long n = std::max(a.m.rows, a.orows);
+    const long long n = std::max(a.m.rows, a.to.rows);
     if (nv <= 16 * 4 && a.m.t.k <= 64) joint_of<SI, SO, 16, 4, NT>(a, n, s);
     else if (nv <= 64 * 4) joint_of<SI, SO, 64, 4, NT>(a, n, s);
     else if (nv <= 256 * 4) joint_of<SI, SO, 256, 4, NT>(a, n, s);
@@ -686,7 +699,7 @@ hipError_t joint(const LossJoint& a, hipStream_t s) {
 // do not fit the last of them (256 MiB)
 template <int ST>
 hipError_t joint_rows(const LossJoint& a, hipStream_t s) {
-    const bool nt = a.out != a.m.z && 2 * a.m.rows * a.m.cols * (ST == kF32 ? 4 : 2) > (256ll << 20);
+    const bool nt = a.to.p != a.m.z && 2 * a.m.rows * a.m.cols * (ST == kF32 ? 4 : 2) > (256ll << 20);
     return nt ? joint<ST, ST, true>(a, s) : joint<ST, ST, false>(a, s);
 }
 
@@ -764,14 +777,13 @@ hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int 
     return hipErrorInvalidValue;
 }
 
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, void* out, long long ldo, unsigned* flag,
-                     hipStream_t s) {
+hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
     if (m.rows <= 0 || m.cols <= 0) return hipSuccess;
-    switch (m.storage) {
-        case kF32: return grad<kF32>(m, lse, coef, out, ldo, flag, s);
-        case kBF16: return grad<kBF16>(m, lse, coef, out, ldo, flag, s);
-        case kF16: return grad<kF16>(m, lse, coef, out, ldo, flag, s);
-    }
+    if (m.storage == kF32 && to.storage == kF32) return grad<kF32, kF32>(m, lse, coef, to, flag, s);
+    if (m.storage == kBF16 && to.storage == kBF16) return grad<kBF16, kBF16>(m, lse, coef, to, flag, s);
+    if (m.storage == kF16 && to.storage == kF16) return grad<kF16, kF16>(m, lse, coef, to, flag, s);
+    if (m.storage == kF32 && to.storage == kBF16) return grad<kF32, kBF16>(m, lse, coef, to, flag, s);
+    if (m.storage == kF32 && to.storage == kF16) return grad<kF32, kF16>(m, lse, coef, to, flag, s);
     return hipErrorInvalidValue;
 }
 
@@ -779,11 +791,11 @@ bool loss_joint_fits(const LossMatrix& m) { return m.cols / (m.storage == kF32 ?
 
 hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
     if (a.m.rows <= 0) return hipSuccess;
-    if (a.m.storage == kF32 && a.to == kF32) return joint_rows<kF32>(a, s);
-    if (a.m.storage == kBF16 && a.to == kBF16) return joint_rows<kBF16>(a, s);
-    if (a.m.storage == kF16 && a.to == kF16) return joint_rows<kF16>(a, s);
-    if (a.m.storage == kF32 && a.to == kBF16) return joint<kF32, kBF16, false>(a, s);
-    if (a.m.storage == kF32 && a.to == kF16) return joint<kF32, kF16, false>(a, s);
+    if (a.m.storage == kF32 && a.to.storage == kF32) return joint_rows<kF32>(a, s);
+    if (a.m.storage == kBF16 && a.to.storage == kBF16) return joint_rows<kBF16>(a, s);
+    if (a.m.storage == kF16 && a.to.storage == kF16) return joint_rows<kF16>(a, s);
+    if (a.m.storage == kF32 && a.to.storage == kBF16) return joint<kF32, kBF16, false>(a, s);
+    if (a.m.storage == kF32 && a.to.storage == kF16) return joint<kF32, kF16, false>(a, s);
     return hipErrorInvalidValue;
 }
 

@@ -249,8 +249,8 @@ def test_head_value_then_vjp_equals_both(dt, tied, top):
 
 
 def test_head_value_and_grad_of_several_pieces_is_value_then_vjp():
-    """More than a piece in 16-bit storage: the same launches, the same bits."""
-    k = Case("bf16", 40000, 2000, d=64, seed=3, ct=False)
+    """16-bit storage, more logits than are kept: the same launches, the same bits."""
+    k = Case("bf16", 40000, 28000, d=64, seed=3, ct=False)
     both, v = k.run("step"), k.run("value")
     g = k.run("vjp", lse=v["lse"], mean=v["mean"])
     for m, x in {**v, **g}.items():
@@ -264,7 +264,18 @@ def test_head_value_and_grad_of_several_pieces_is_value_then_vjp():
 ], ids=str)
 def test_head_in_several_pieces(dt, rows, d, vocab, tied, top):
     k = Case(dt, rows, vocab, d=d, tied=tied, top=top, seed=5)
-    k.check(k.run("step"))
+    v = k.run("value")
+    for got in (k.run("step"), v, k.run("vjp", lse=v["lse"], mean=v["mean"])):
+        k.check(got)
+
+
+# more columns than a workgroup's registers hold of a row
+@pytest.mark.parametrize("tied,top", [(False, 0), (True, 0), (True, 7), (False, 1000)])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_head_of_long_rows(dt, tied, top):
+    for rows in (3, 70):
+        k = Case(dt, rows, 66001 if tied else 70003, d=40, tied=tied, top=top, seed=8)
+        k.check(k.run("step"))
 
 
 @pytest.mark.parametrize("dt,rows,d,vocab,tied", [("bf16", 2048, 1024, 8192, False), ("f16", 1999, 1021, 9001, False),

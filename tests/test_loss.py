@@ -89,15 +89,17 @@ def test_steps_of_a_sequence_are_checked_when_they_are_added():
 
 
 def test_the_workspace_does_not_grow_with_the_vocabulary():
-    """A head's workspace is its pieces': between a vocabulary of 64 Ki and
-    one of 4 Mi it grows by the row sums' partials alone (12 bytes a row and
-    column tile of at least 128)."""
+    """Past 4 GiB of f32 logits a head's workspace is its pieces': between a
+    vocabulary of 128 Ki and one of 4 Mi it grows by the row sums' partials
+    alone (12 bytes a row and column tile of at least 128).  Up to there it is
+    the logits' and their 16-bit cotangent's."""
     for dt in ("bf16", "f16", "f32"):
         rows, model = 8192, 256
-        sizes = [hip.HeadLoss(dt, rows, model, v).workspace("step") for v in (1 << 16, (1 << 22) - 64)]
+        sizes = [hip.HeadLoss(dt, rows, model, v).workspace("step") for v in ((1 << 17) + 64, (1 << 22) - 64)]
         tiles = (1 << 22) // 128
         assert sizes[1] - sizes[0] <= 12 * rows * tiles + (1 << 20), (dt, sizes)
         assert sizes[1] < rows * (1 << 22)     # a byte a logit
+        assert hip.HeadLoss(dt, rows, model, 1 << 17).workspace("step") < 6.5 * (1 << 30)
     # a gradient that is not asked for takes none
     op = hip.HeadLoss("bf16", 65536, 4096, 50000)
     assert op.workspace("step", dx=False) < op.workspace("step")
