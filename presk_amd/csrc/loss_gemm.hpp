@@ -467,22 +467,33 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
             f = 1.f;
         }
         if (sums) {
-            // four consecutive columns of a row from the registers
+            // 32 rows of the wave's 64 columns at a time through its own LDS,
+            // so that a store is four rows' 256 bytes and not 32 rows' 32
+            constexpr int LD = 68;
+            static_assert(NW * 32 * LD * 4 <= TL::BYTES, "the waves' rows");
+            float* const rows = (float*)smem + wave * (32 * LD);
 #pragma unroll
             for (int i = 0; i < WM; ++i) {
-                const int m = m0 + wm + i * 32 + (lane & 31);
-                if (m >= g.M) continue;
-                float* const row = out + (long long)m * g.lda;
 #pragma unroll
                 for (int j = 0; j < WN; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int n = n0 + wn + col_of(j, 4 * q, lane);
                         f32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * f;
-                        if (n < g.N) *(f32x4*)(row + n) = v;
+                        *(f32x4*)&rows[(lane & 31) * LD + col_of(j, 4 * q, lane)] = v;
                     }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    const int r = 4 * p + (lane >> 4), c = 4 * (lane & 15);
+                    const f32x4 v = *(const f32x4*)&rows[r * LD + c];
+                    const int m = m0 + wm + i * 32 + r, n = n0 + wn + c;
+                    if (m < g.M && n < g.N) *(f32x4*)(out + (long long)m * g.lda + n) = v;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
         } else {
             unsigned short* const ct = (unsigned short*)smem;
