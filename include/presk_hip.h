@@ -255,8 +255,9 @@ int presk_hip_dropout_mask(const void *key, double rate, const char *type, int64
  * cotangent NaN.  `ct` null: the mean's gradient, ct[r] = 1 / count.
  *
  * presk_hip_head_loss: z = x . w with x [rows, model] and w [model, vocab], or
- * [vocab, model] when `tied`, in pieces of the vocabulary: the logits are not
- * kept, whatever its size.  Gradients dx = dz . w^T and dw = x^T . dz, either
+ * [vocab, model] when `tied`.  The logits are the workspace's: value and
+ * gradient in one call keep up to 4 GiB of them in f32, past that, and for
+ * either alone, they come in pieces of the vocabulary.  Gradients dx = dz . w^T and dw = x^T . dz, either
  * of which may be null.  The products accumulate in f32; in 16-bit storage the
  * factor ct[r] * (exp(u[r] - lse[r]) - t[r]) of dz is rounded to the storage type
  * before them (by a power of two in f16's range), T and the mean's 1 / count

@@ -19,7 +19,8 @@ struct Span {
 // One step of the sequence, as the batch records it: a launch of a compiled
 // kernel over its pointer table (`k` its IR, `handle` the compiled kernel),
 // or, with no kernel, an edge conversion (bufs {src, dst, flag}, types
-// `from` and `to`) or, with `rate` >= 0, a dropout mask (bufs {key, dst}).
+// `from` and `to`) or, with `rate` >= 0, a dropout mask (bufs {key, dst}), or,
+// with neither, a step that names its spans itself.
 struct BranchStep {
     const Kernel* k = nullptr;
     const void* handle = nullptr;
@@ -27,6 +28,7 @@ struct BranchStep {
     int from = -1, to = -1;
     int64_t n = 0;
     double rate = -1.0;
+    std::vector<Span> rd, wr;
 };
 
 inline size_t spec_bytes(const BufSpec& s) {
@@ -56,6 +58,9 @@ inline void step_spans(const BranchStep& it, std::vector<Span>* rd, std::vector<
     } else if (it.rate >= 0.0) {
         add(rd, it.bufs[0], 32);   // the ChaCha20 key
         add(wr, it.bufs[1], (size_t)it.n * code_bytes(it.to));
+    } else if (it.bufs.empty()) {
+        *rd = it.rd;
+        *wr = it.wr;
     } else {
         add(rd, it.bufs[0], (size_t)it.n * code_bytes(it.from));
         add(wr, it.bufs[1], (size_t)it.n * code_bytes(it.to));

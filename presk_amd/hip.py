@@ -324,15 +324,27 @@ def _loss_workspace(sizes: tuple, what: int, dx: bool, dw: bool) -> int:
     return n.value
 
 
-def _buffer(name: str, b, nbytes: int) -> int:
+# a torch dtype's name in the executor's terms, by the dtype object
+_TORCH_TYPES: dict = {}
+_TORCH_NAMES = {"torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
+
+
+def _buffer(name: str, b, nbytes: int, ty: str | None = None) -> int:
     """The device pointer of a buffer of at least `nbytes` bytes: a
-    DeviceBuffer, or an array of another library that says where and how
-    large it is (torch's `data_ptr` and `nbytes`, contiguous)."""
-    if b is None:
-        return None
+    DeviceBuffer, or a tensor of another library that says where and how
+    large it is (torch's `data_ptr` and `nbytes`, contiguous, on the device in
+    use, of type `ty`)."""
     if hasattr(b, "data_ptr"):
-        if not b.is_cuda:
+        at = b.get_device()
+        if at < 0:
             raise ValueError(f"{name} is not in device memory")
+        if at != _initialized and _initialized not in (None, -1):
+            raise ValueError(f"{name} is on device {at}, not {_initialized}")
+        have = _TORCH_TYPES.get(b.dtype)
+        if have is None:
+            have = _TORCH_TYPES[b.dtype] = _TORCH_NAMES.get(str(b.dtype), str(b.dtype))
+        if have != ty and ty is not None:
+            raise ValueError(f"{name} is {have}, not {ty}")
         if not b.is_contiguous():
             raise ValueError(f"{name} is not contiguous")
         ptr, have = b.data_ptr(), b.nbytes
@@ -354,8 +366,9 @@ class Distill:
     the mean's where mean is given in its place.  `value_and_grad` does both,
     for ct or else the mean.  Buffers are DeviceBuffers or torch tensors;
     `work` is workspace(kind) bytes of the caller's, or, not given, a buffer
-    this object keeps: calls that share a workspace run one after another (one
-    stream, or an object a stream)."""
+    this object keeps (with any smaller one it has outgrown, which a captured
+    call may still use): calls that share a workspace, their captured graphs
+    among them, run one after another (one stream, or an object a stream)."""
 
     head = False
 
@@ -366,11 +379,13 @@ class Distill:
         self.dtype, self.rows, self.model, self.vocab, self.top = dtype, int(rows), int(model), int(vocab), int(top)
         self.tied, self.temperature = bool(tied), float(temperature)
         self._sizes = (self.dtype, self.rows, self.model, self.vocab, self.top, self.tied, self.temperature)
-        self._work = None
+        self._work, self._outgrown = None, []
         self.workspace("value")     # the sizes and the type are checked here
         e, n = STORAGE_BYTES[dtype], self.rows
         x, w = n * (self.model if self.head else self.vocab) * e, self.model * self.vocab * e
-        self._bytes = (x, w, 8 * n * max(self.top, 1), e * n * self.top, 4 * n, 4 * n, 8, 4 * n, x, w, 4)
+        self._specs = tuple(zip(_LOSS_BUFFERS, (x, w, 8 * n * max(self.top, 1), e * n * self.top, 4 * n, 4 * n, 8, 4 * n, x, w, 4),
+                                (dtype, dtype, "i64", dtype, "f32", "f32", "f32", "f32", dtype, dtype, None)))
+        self._head_args = (dtype.encode(), *self._sizes[1:])
 
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
         """Bytes of workspace for `value`, `vjp` or `step` (value_and_grad),
@@ -383,10 +398,12 @@ class Distill:
         need = self.workspace(kind, dx is not None, dw is not None)
         if work is None:
             if self._work is None or self._work.nbytes < need:
+                self._outgrown.append(self._work)
                 self._work = DeviceBuffer(need)
             work = self._work
-        bufs = map(_buffer, _LOSS_BUFFERS, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag), self._bytes)
-        return LossArgs(self.dtype.encode(), *self._sizes[1:], *bufs, _buffer("work", work, need), work.nbytes)
+        bufs = [None if b is None else _buffer(s[0], b, s[1], s[2])
+                for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
+        return LossArgs(*self._head_args, *bufs, _buffer("work", work, need), work.nbytes)
 
     def _call(self, kind, stream, **bufs):
         a = self.args(kind, **bufs)
@@ -405,7 +422,7 @@ class Distill:
 
 class HeadLoss(Distill):
     """presk_hip_head_loss at fixed sizes: the loss of the logits x . w, which
-    are not kept.  x [rows, model]; w [model, vocab], or [vocab, model] when
+    are the workspace's.  x [rows, model]; w [model, vocab], or [vocab, model] when
     `tied`; `top` 0: the softmax cross entropy against index[r] (negative: the
     row does not count); `top` k: Distill's loss.  The methods are Distill's,
     with w, and the gradients dx and dw, of which one may be left out."""

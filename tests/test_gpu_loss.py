@@ -564,3 +564,24 @@ def test_the_bindings_own_workspace():
     op.value(**k.ins(), loss=loss)
     hip.sync()
     same(loss, k.run("value")["loss"], "loss")
+
+
+def test_the_bindings_own_workspace_captured_and_outgrown():
+    """A captured call's workspace stays when a later call needs a larger one."""
+    k = Case("bf16", 30, 3000, d=64, seed=1, ct=False)
+    op, loss, s, graph = k.op(), torch.empty(30, device=DEV), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    want = k.run("value")["loss"]
+    with torch.cuda.stream(s):
+        op.value(**k.ins(), loss=loss, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            op.value(**k.ins(), loss=loss, stream=s.cuda_stream)
+    first = op._work
+    for _ in range(3):
+        op.value_and_grad(**k.ins(), dx=torch.empty_like(k.x), dw=torch.empty_like(k.w))
+        torch.cuda.synchronize()
+        loss.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(loss, want, "loss")
+    assert op._work is not first and first in op._outgrown

@@ -131,3 +131,38 @@ def test_the_binding_checks_sizes():
         hip.HeadLoss("f64", 4, 64, 100)
     with pytest.raises(hip.HipError, match="top 0"):
         hip.Distill("f32", 4, 100, 0)
+
+
+def test_the_binding_checks_tensors_types_and_places():
+    torch = pytest.importorskip("torch")
+
+    class Tensor:
+        """A tensor in device memory as far as the checks look."""
+
+        def __init__(self, dtype, n, cuda=True, contiguous=True, device=0):
+            self.dtype, self.nbytes, self.whole, self.device = dtype, n, contiguous, device if cuda else -1
+
+        def get_device(self):
+            return self.device
+
+        def data_ptr(self):
+            return 1 << 24
+
+        def is_contiguous(self):
+            return self.whole
+
+    op = hip.HeadLoss("bf16", 4, 64, 100)
+    x, w, i, f = (Tensor(t, 1 << 20) for t in (torch.bfloat16, torch.bfloat16, torch.int64, torch.float32))
+    assert op.args("value", x=x, w=w, index=i, loss=f, work=Tensor(torch.uint8, 1 << 20)).rows == 4
+    for bad, why in [({"x": Tensor(torch.float16, 1 << 20)}, "x is f16, not bf16"), ({"w": f}, "w is f32, not bf16"),
+                     ({"index": Tensor(torch.int32, 1 << 20)}, "index is torch.int32, not i64"), ({"loss": x}, "loss is bf16, not f32"),
+                     ({"x": Tensor(torch.bfloat16, 1 << 20, cuda=False)}, "x is not in device memory"),
+                     ({"x": Tensor(torch.bfloat16, 1 << 20, contiguous=False)}, "x is not contiguous")]:
+        with pytest.raises(ValueError, match=why):
+            op.args("value", **{**dict(x=x, w=w, index=i, loss=f, work=Tensor(torch.uint8, 1 << 20)), **bad})
+    was, hip._initialized = hip._initialized, 0
+    try:
+        with pytest.raises(ValueError, match="x is on device 1, not 0"):
+            op.args("value", x=Tensor(torch.bfloat16, 1 << 20, device=1), w=w, index=i, loss=f, work=x)
+    finally:
+        hip._initialized = was
