@@ -128,7 +128,9 @@ struct Plan {
     int st, esz, D, V, k, parts, slots, nblocks;
     long long rows, prows;
     float c;
-    bool packx, packw, once, joint, counted;   // once: f32 logits of the whole vocabulary, joint: in one kernel's registers; counted: counts are taken
+    bool packx, packw;
+    bool once, joint;                 // f32 logits of the whole vocabulary are kept; a row of them fits a workgroup's registers
+    bool blocks, counted;             // the slots' blocks are listed (`start`); the rows are counted
     int Dp, piece, pieces, spiece;    // spiece: columns a pass of row sums takes at once
     long long ldz;
     Shape zs;                         // once
@@ -192,12 +194,14 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         return was;
     };
     const bool half = head && q.st != kF32;
+    q.once = half && q.rows && q.value && q.grad && 4 * q.rows * up(q.V, 4) <= kKeepBytes;
     q.prows = up(q.rows, 64);
     q.nblocks = (int)(up(q.V, kCols) / kCols);
     q.col = take(4 * q.rows * a.top);
     q.p = take(4 * q.rows * a.top);
     q.ent = take(a.top ? 4 * q.rows : 0);
-    q.start = take(half && q.k > 4 ? 2 * q.rows * (q.nblocks + 1) : 0);
+    q.blocks = half && q.k > 4 && !q.once;
+    q.start = take(q.blocks ? 2 * q.rows * (q.nblocks + 1) : 0);
     q.count = take(4 * q.parts);
     q.most = take(4 * q.parts);
     q.lse = take(4 * q.rows);
@@ -224,7 +228,6 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
         q.packw = (a.tied ? q.D : q.V) % 8 != 0;
         q.Dp = (int)up(q.D, 64);
         q.ldz = up(q.V, 4);
-        q.once = q.value && q.grad && 4 * q.rows * q.ldz <= kKeepBytes;
         if (q.once) {
             LossMatrix m{};
             m.storage = kF32;
@@ -622,7 +625,7 @@ struct Call {
         p.col = at<int>(q.col);
         p.p = at<float>(q.p);
         p.ent = at<float>(q.ent);
-        p.start = q.head && q.st != kF32 && q.k > 4 ? at<unsigned short>(q.start) : nullptr;
+        p.start = q.blocks ? at<unsigned short>(q.start) : nullptr;
         p.nblocks = q.nblocks;
         p.count = at<int>(q.count);
         p.most = at<float>(q.most);

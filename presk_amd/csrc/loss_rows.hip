@@ -100,13 +100,15 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // ---- targets ------------------------------------------------------------------
 
-// one column a row
+// one column a row: bound by its launch (16384 rows 3.5 us)
 __global__ void __launch_bounds__(256) prep_one_kernel(LossPrep a) { prep_one<256>(a, (int)blockIdx.x); }
 
 // A teacher's slots: the softmax of those in use, sorted by column (a slot's
 // place is how many come before it: columns below its own, or its own at an
-// earlier slot, so the order is one whatever runs first).  G threads a row, E
-// slots a thread.
+// earlier slot, so the order is one whatever runs first).  k^2 comparisons a row
+// out of LDS: G threads a row, E slots a thread, as many rows a workgroup as
+// their slots fit.  4096 rows of 64 slots 12 us, 30 with the list of blocks
+// that the products without kept logits look their slots up in.
 template <int ST, int G, int E>
 __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) {
     constexpr int R = 256 / G, KM = G * E;
@@ -221,7 +223,9 @@ __device__ __forceinline__ float row_loss(const LossTarget& t, long long r, floa
 }
 
 // T / G rows a workgroup, G threads a row, each over every G-th slot; with a
-// mean one workgroup has all the rows.
+// mean one workgroup has all the rows.  Bound by the partials' bytes and its
+// launch: 8192 rows of 125 slots, 12 MB, 12.5 us; few rows of many slots take a
+// wave each (8 rows of 250 and their mean 6.5 us).
 template <int T, int G>
 __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
     __shared__ float red[T / 64];
@@ -277,6 +281,8 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
     }
 }
 
+// the mean, in 64 bits, by one workgroup where no other launch has a place for
+// it: 16384 rows 6.3 us, 256 rows 2.2
 __global__ void __launch_bounds__(1024) mean_kernel(LossMean m) { write_mean<1024>(m); }
 
 // ---- logits in memory -------------------------------------------------------------
@@ -333,7 +339,9 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
     ta = all_of<G>(ta, red, add_f);
 }
 
-// G 16, 64: 16 or four rows a workgroup; 256: a row's chunk a workgroup
+// G 16, 64: 16 or four rows a workgroup; 256: a row's chunk a workgroup.  Bound
+// by the logits' bytes, for few rows by its launch (64 x 50257 in f32, 12.9 MB
+// out of the Infinity Cache, 4.9 us; 256 x 65 4.4).
 template <int ST, int G>
 __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, float* ps, float* pa, int slot0, int chunk,
                                                     LossDone done, bool finish) {
@@ -375,7 +383,9 @@ __device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, flo
 
 // out = coef * (2^(u - lse) - t).  The target's columns are written after the
 // row's others, by a thread each, once the stores of this workgroup (or wave)
-// have reached memory.  SI the logits' type, SO the output's.
+// have reached memory.  SI the logits' type, SO the output's.  Bound by the
+// bytes in and out; where value and gradient are one call and a row fits a
+// workgroup's registers, joint_kernel reads the logits once instead of twice.
 template <int SI, int SO, int G>
 __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* lse, const float* coef, LossTo to, unsigned* flag,
                                                    int chunk) {
@@ -443,7 +453,8 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
 // vectors and E slots of the target each.  SI the logits' type, SO the output's.
 // Bound by its row's bytes in and out: 8192 x 32000 in bf16, 1.05 GB, 215 us
 // with the row past the caches (NT), 235 without; of 0.26 GB, which the
-// Infinity Cache holds, 68 with and 63 without (8192 x 8000).
+// Infinity Cache holds, 68 with and 63 without (8192 x 8000); f32 logits of
+// 8192 x 32000 into bf16, 1.57 GB, 277 with and 300 without.
 template <int SI, int SO, int G, int R, int E, bool NT>
 __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kernel(LossJoint a) {
     typedef typename Elem<SI>::S S;
@@ -589,7 +600,9 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
 // ---- copies ------------------------------------------------------------------------
 
 // rows of `cols` elements into rows of `ldd`, eight elements a thread, zero
-// past cols; the first nb workgroups take a's
+// past cols; the first nb workgroups take a's.  Bound by its bytes, read at odd
+// addresses: half of 1021 x 50257 in 16 bits and its states, 107 MB in and
+// out, 20.8 us.
 __global__ void __launch_bounds__(256) pack_kernel(LossPack a, LossPack b, unsigned nb) {
     const bool first = blockIdx.x < nb;
     const LossPack& k = first ? a : b;
@@ -794,8 +807,9 @@ hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
     if (a.m.storage == kF32 && a.to.storage == kF32) return joint_rows<kF32>(a, s);
     if (a.m.storage == kBF16 && a.to.storage == kBF16) return joint_rows<kBF16>(a, s);
     if (a.m.storage == kF16 && a.to.storage == kF16) return joint_rows<kF16>(a, s);
-    if (a.m.storage == kF32 && a.to.storage == kBF16) return joint<kF32, kBF16, false>(a, s);
-    if (a.m.storage == kF32 && a.to.storage == kF16) return joint<kF32, kF16, false>(a, s);
+    const bool nt = 4 * a.m.rows * a.m.ld > (256ll << 20);
+    if (a.m.storage == kF32 && a.to.storage == kBF16) return nt ? joint<kF32, kBF16, true>(a, s) : joint<kF32, kBF16, false>(a, s);
+    if (a.m.storage == kF32 && a.to.storage == kF16) return nt ? joint<kF32, kF16, true>(a, s) : joint<kF32, kF16, false>(a, s);
     return hipErrorInvalidValue;
 }
 
