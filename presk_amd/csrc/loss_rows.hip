@@ -628,35 +628,51 @@ __global__ void __launch_bounds__(256) zero_kernel(unsigned char* dst, long long
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < bytes; i += (long long)gridDim.x * 256) dst[i] = 0;
 }
 
+// Four columns of a row a thread, eight splits' loads in flight: bound by the
+// partials' bytes (dx of 1999 x 1021 over 25 K columns 8.2 us, 12.2 with one
+// column a thread).
 template <int ST>
-__device__ __forceinline__ void join_at(const LossGemm& g, long long i) {
-    const long long n = (long long)g.M * g.lda, m = i / g.N, at = m * g.lda + (i - m * g.N);
-    float s = g.part[at];
+__device__ __forceinline__ void join_at(const LossGemm& g, unsigned i) {
+    const unsigned quads = (unsigned)g.lda / 4, m = i / quads;
+    const int c = (int)(i - m * quads) * 4;
+    const long long n = (long long)g.M * g.lda, at = (long long)m * g.lda + c;
+    f32x4 s = *(const f32x4*)(g.part + at);
     int p = 1;
     for (; p + 8 <= g.splits; p += 8) {
-        float w[8];
+        f32x4 w[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) w[q] = g.part[(long long)(p + q) * n + at];
+        for (int q = 0; q < 8; ++q) w[q] = *(const f32x4*)(g.part + (long long)(p + q) * n + at);
 #pragma unroll
         for (int q = 0; q < 8; ++q) s += w[q];
     }
-    for (; p < g.splits; ++p) s += g.part[(long long)p * n + at];
+    for (; p < g.splits; ++p) s += *(const f32x4*)(g.part + (long long)p * n + at);
     if (g.scale) s *= *g.scale;
-    if (g.acc_in) s += g.acc[at];
-    if (g.C) {
-        bool ovf = false;
-        ((unsigned short*)g.C)[m * g.ldc + (i - m * g.N)] = narrow<ST>(s, ovf);
-        if (ovf && g.flag) atomicOr(g.flag, 1u);
-    } else {
-        g.acc[at] = s;
+    if (g.acc_in) s += *(const f32x4*)(g.acc + at);
+    if (!g.C) {
+        *(f32x4*)(g.acc + at) = s;
+        return;
     }
+    unsigned short* const out = (unsigned short*)g.C + (long long)m * g.ldc + c;
+    bool ovf = false;
+    unsigned short h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bool o = false;
+        h[e] = narrow<ST>(s[e], o);
+        ovf |= o && c + e < g.N;
+    }
+    if (c + 4 <= g.N) __builtin_memcpy(out, h, 8);
+    else
+        for (int e = 0; e < 3; ++e)
+            if (c + e < g.N) out[e] = h[e];
+    if (ovf && g.flag) atomicOr(g.flag, 1u);
 }
 template <int ST>
 __global__ void __launch_bounds__(256) join_kernel(LossGemm x, LossGemm w, unsigned nx) {
     const bool first = blockIdx.x < nx;
-    const long long i = (long long)(first ? blockIdx.x : blockIdx.x - nx) * 256 + threadIdx.x;
+    const unsigned i = (first ? blockIdx.x : blockIdx.x - nx) * 256 + threadIdx.x;
     const LossGemm& g = first ? x : w;
-    if (i < (long long)g.M * g.N) join_at<ST>(g, i);
+    if (i < (unsigned)g.M * ((unsigned)g.lda / 4)) join_at<ST>(g, i);
 }
 
 unsigned blocks_of(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 16384); }
@@ -828,8 +844,9 @@ hipError_t loss_zero(void* dst, long long bytes, hipStream_t s) {
 }
 
 hipError_t loss_join(const LossGemm& x, const LossGemm& w, int storage, hipStream_t s) {
-    auto blocks = [](const LossGemm& g) { return g.splits > 1 ? (unsigned)(((long long)g.M * g.N + 255) / 256) : 0u; };
-    const unsigned nx = blocks(x), n = nx + blocks(w);
+    auto quads = [](const LossGemm& g) { return g.splits > 1 ? g.M * (g.lda / 4) : 0; };
+    if (quads(x) >= 1ll << 30 || quads(w) >= 1ll << 30) return hipErrorInvalidValue;    // (few tiles are split)
+    const unsigned nx = (unsigned)(quads(x) + 255) / 256, n = nx + (unsigned)(quads(w) + 255) / 256;
     if (!n) return hipSuccess;
     if (storage == kBF16) join_kernel<kBF16><<<n, 256, 0, s>>>(x, w, nx);
     else join_kernel<kF16><<<n, 256, 0, s>>>(x, w, nx);
