@@ -301,7 +301,7 @@ struct Call {
     char* w;
     LossTarget t;
     LossPrep prep;
-    bool mean_done = false;
+    bool mean_done = false, beside = false;     // beside: given logits' sums are one launch with the targets
 
     template <typename T>
     T* at(size_t off) const { return (T*)(w + off); }
@@ -568,6 +568,10 @@ struct Call {
         LossMatrix m = matrix(a.x, q.V, q.st, 0, q.V);
         const LossTo to{a.dx, q.st, q.V, q.rows};
         if (q.value && q.grad && loss_joint_fits(m)) return loss_joint(joint_args(m, to), s);
+        if (beside) {
+            LOSS_TRY(loss_stats_beside(m, at<float>(q.pm), at<float>(q.ps), prep, s));
+            return rows_of(m);
+        }
         if (q.value) LOSS_TRY(value_of(m, 0));
         LOSS_TRY(rows_of());
         if (!q.grad) return hipSuccess;
@@ -605,8 +609,10 @@ struct Call {
         return r;
     }
     // the rows' sums joined, their cotangents' factors, and of few rows the mean
-    hipError_t rows_of() {
-        const LossRows r = row_args();
+    hipError_t rows_of(const LossMatrix& late = LossMatrix{}) {
+        LossRows r = row_args();
+        r.z = late;
+        if (late.z) r.slots = q.slots;
         if (!r.slots && !r.coef && !r.mean) return hipSuccess;
         mean_done = r.mean;
         return loss_rows(r, s);
@@ -633,7 +639,8 @@ struct Call {
         t = LossTarget{a.top ? nullptr : p.index, q.V, p.col, p.p, p.ent, p.start, q.k, q.nblocks};
         if (q.rows) {
             // (counts alone are taken beside the logits where those are one launch)
-            if (q.counted && (a.top || !q.once)) LOSS_TRY(loss_prep(p, s));
+            beside = !q.head && !q.grad && loss_beside(matrix(a.x, q.V, q.st, 0, q.V), p.top);
+            if (q.counted && (a.top || !q.once) && !beside) LOSS_TRY(loss_prep(p, s));
             const float* const lse = lse_out();
             LOSS_TRY(!q.head ? given(lse) : q.st == kF32 ? single(lse) : half(lse));
         } else if (q.grad && q.head && a.dw) {

@@ -133,11 +133,25 @@ hipError_t loss_pair_f16(const LossGemm& x, const LossGemm& w, bool xbkc, int ti
 int loss_parts(long long rows, int top);
 hipError_t loss_prep(const LossPrep& a, hipStream_t s);
 
+// Logits in memory, [rows][ld] from column col0 on, `cols` of them.
+struct LossMatrix {
+    const void* z;
+    long long ld;
+    int storage;                // Storage
+    long long rows;
+    int col0, cols;
+    float c;
+    LossTarget t;
+    int planes;                 // loss_joint in f32: the sum of so many, in order, ...
+    long long plane;            // ... so many elements apart
+};
+
 // partials -> a row's lse and loss, and the factor of its cotangent
 struct LossRows {
     const float *pm, *ps, *pa;  // [slots][rows]
     int slots;
     LossTarget t;
+    LossMatrix z;               // given logits whose target's part is taken here (null: it is in pa)
     long long rows;
     float temperature;
     float *lse, *loss;          // outputs, may be null
@@ -155,18 +169,6 @@ bool loss_rows_mean(long long rows);
 hipError_t loss_rows(const LossRows& a, hipStream_t s);
 hipError_t loss_mean(const LossMean& m, hipStream_t s);
 
-// Logits in memory, [rows][ld] from column col0 on, `cols` of them.
-struct LossMatrix {
-    const void* z;
-    long long ld;
-    int storage;                // Storage
-    long long rows;
-    int col0, cols;
-    float c;
-    LossTarget t;
-    int planes;                 // loss_joint in f32: the sum of so many, in order, ...
-    long long plane;            // ... so many elements apart
-};
 // partials [chunk][rows] from slot0 on; or, of one chunk, the rows' lse and loss
 // themselves (`done`, its outputs may be null)
 struct LossDone {
@@ -175,6 +177,10 @@ struct LossDone {
 };
 int loss_chunks(long long rows, int cols);
 hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s);
+// the same partials of few rows, without the target's part, beside loss_prep
+// of a teacher's slots in one launch
+bool loss_beside(const LossMatrix& m, int top);
+hipError_t loss_stats_beside(const LossMatrix& m, float* pm, float* ps, const LossPrep& p, hipStream_t s);
 // Where a cotangent goes: in the logits' type (in place or not), or f32 logits'
 // in 16 bits, zero then past their columns, and past their rows up to `rows`.
 struct LossTo {

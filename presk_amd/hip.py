@@ -324,6 +324,19 @@ def _loss_workspace(sizes: tuple, what: int, dx: bool, dw: bool) -> int:
     return n.value
 
 
+@functools.lru_cache(maxsize=1024)
+def _loss_layout(sizes: tuple) -> tuple:
+    """(each buffer's name, bytes and type; the arguments before the buffers) of
+    sizes and a type that are checked here."""
+    dtype, n, model, vocab, top = sizes[:5]
+    _loss_workspace(sizes, VALUE, True, True)
+    e = STORAGE_BYTES[dtype]
+    x, w = n * (model or vocab) * e, model * vocab * e
+    return (tuple(zip(_LOSS_BUFFERS, (x, w, 8 * n * max(top, 1), e * n * top, 4 * n, 4 * n, 8, 4 * n, x, w, 4),
+                      (dtype, dtype, "i64", dtype, "f32", "f32", "f32", "f32", dtype, dtype, None))),
+            (dtype.encode(), *sizes[1:]))
+
+
 # a torch dtype's name in the executor's terms, by the dtype object
 _TORCH_TYPES: dict = {}
 _TORCH_NAMES = {"torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
@@ -380,12 +393,7 @@ class Distill:
         self.tied, self.temperature = bool(tied), float(temperature)
         self._sizes = (self.dtype, self.rows, self.model, self.vocab, self.top, self.tied, self.temperature)
         self._work, self._outgrown = None, []
-        self.workspace("value")     # the sizes and the type are checked here
-        e, n = STORAGE_BYTES[dtype], self.rows
-        x, w = n * (self.model if self.head else self.vocab) * e, self.model * self.vocab * e
-        self._specs = tuple(zip(_LOSS_BUFFERS, (x, w, 8 * n * max(self.top, 1), e * n * self.top, 4 * n, 4 * n, 8, 4 * n, x, w, 4),
-                                (dtype, dtype, "i64", dtype, "f32", "f32", "f32", "f32", dtype, dtype, None)))
-        self._head_args = (dtype.encode(), *self._sizes[1:])
+        self._specs, self._fixed = _loss_layout(self._sizes)
 
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
         """Bytes of workspace for `value`, `vjp` or `step` (value_and_grad),
@@ -403,7 +411,7 @@ class Distill:
             work = self._work
         bufs = [None if b is None else _buffer(s[0], b, s[1], s[2])
                 for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
-        return LossArgs(*self._head_args, *bufs, _buffer("work", work, need), work.nbytes)
+        return LossArgs(*self._fixed, *bufs, _buffer("work", work, need), work.nbytes)
 
     def _call(self, kind, stream, **bufs):
         a = self.args(kind, **bufs)
