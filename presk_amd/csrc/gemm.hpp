@@ -38,6 +38,7 @@ struct GemmArgs {
     bool staged;                    // 16-bit operands staged through registers (gemm_ragged.hip), bm x bn tiles
     bool split3;                    // f32 on the bf16 matrix cores (gemm_split.hip): 128 rows, 192, 128 (eight or four waves) or 64 columns
     bool stream;                    // K of at most two k-blocks may stream B's tiles across a kept A panel
+    bool planes;                    // the partials of splits > 1 are the result: nothing adds them into C
 };
 
 hipError_t gemm_launch(const GemmArgs& g, hipStream_t stream);

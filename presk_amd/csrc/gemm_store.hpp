@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) split_reduce_kernel(GemmArgs g) {
 // (nothing to do where K is not split)
 template <int ST>
 hipError_t split_reduce(const GemmArgs& g, hipStream_t stream) {
-    if (g.splits <= 1) return hipSuccess;
+    if (g.splits <= 1 || g.planes) return hipSuccess;
     split_reduce_kernel<ST><<<(unsigned)((g.M * g.N + 255) / 256), 256, 0, stream>>>(g);
     return hipGetLastError();
 }

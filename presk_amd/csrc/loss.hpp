@@ -142,7 +142,7 @@ struct LossMatrix {
     int col0, cols;
     float c;
     LossTarget t;
-    int planes;                 // loss_joint in f32: the sum of so many, in order, ...
+    int planes;                 // loss_stats and loss_joint in f32: the sum of so many, in order, ...
     long long plane;            // ... so many elements apart
 };
 

@@ -312,10 +312,16 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
     m = -INFINITY;
     s = 0.f;
     ta = 0.f;
+    auto logit = [&](int col) {
+        float x = widen<ST>(z[col]);
+        if constexpr (ST == kF32)
+            for (int p = 1; p < a.planes; ++p) x += z[p * a.plane + col];
+        return x;
+    };
     for (int e = t; e < a.t.k; e += G) {
         const int col = slot_col(a.t, r, e) - a.col0;
         const float p = slot_p(a.t, r, e);
-        if (col >= lo && col < hi && p != 0.f) ta += p * (widen<ST>(z[col]) * a.c);
+        if (col >= lo && col < hi && p != 0.f) ta += p * (logit(col) * a.c);
     }
     // four vectors in flight, their largest first, then one rescale for all
     constexpr int U = 4;
@@ -324,6 +330,15 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i + u * G < sp.n) v[u] = load_vec(w + (long long)(i + u * G) * V);
+        if constexpr (ST == kF32)
+            for (int p = 1; p < a.planes; ++p)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i + u * G < sp.n) {
+                        const u32x4 y = load_vec(w + p * a.plane + (long long)(i + u * G) * V);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) v[u][e] = pk_bits(pk_float(v[u][e]) + pk_float(y[e]));
+                    }
         float x = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -340,7 +355,7 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
                 for (int e = 0; e < V; ++e) s += exp2_of(elem<ST>(v[u], e), a.c, b);
     }
     if (t < sp.edges()) {
-        const float x = widen<ST>(z[lo + sp.edge(t)]);
+        const float x = logit(lo + sp.edge(t));
         const float n = fmaxf(m, x * a.c), b = base_of(n);
         s = s * __builtin_amdgcn_exp2f(m - b) + exp2_of(x, a.c, b);
         m = n;
