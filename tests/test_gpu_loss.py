@@ -269,6 +269,13 @@ def test_head_in_several_pieces(dt, rows, d, vocab, tied, top):
         k.check(got)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_head_of_nearly_all_the_logits_that_are_kept(dt):
+    """4.2 GB of f32 logits, whose byte offsets pass 2^31, in one piece."""
+    k = Case(dt, 40000, 26000, d=72, seed=9)
+    k.check(k.run("step"))
+
+
 # more columns than a workgroup's registers hold of a row
 @pytest.mark.parametrize("tied,top", [(False, 0), (True, 0), (True, 7), (False, 1000)])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
