@@ -326,14 +326,16 @@ def _loss_workspace(sizes: tuple, what: int, dx: bool, dw: bool) -> int:
 
 @functools.lru_cache(maxsize=1024)
 def _loss_layout(sizes: tuple) -> tuple:
-    """(each buffer's name, bytes and type; the arguments before the buffers) of
-    sizes and a type that are checked here."""
-    dtype, n, model, vocab, top = sizes[:5]
+    """(each buffer's name, bytes, type and row length; the arguments before the
+    buffers) of sizes and a type that are checked here."""
+    dtype, n, model, vocab, top, tied = sizes[:6]
     _loss_workspace(sizes, VALUE, True, True)
     e = STORAGE_BYTES[dtype]
     x, w = n * (model or vocab) * e, model * vocab * e
+    xr, wr, tr = model or vocab, model if tied else vocab, top or None
     return (tuple(zip(_LOSS_BUFFERS, (x, w, 8 * n * max(top, 1), e * n * top, 4 * n, 4 * n, 8, 4 * n, x, w, 4),
-                      (dtype, dtype, "i64", dtype, "f32", "f32", "f32", "f32", dtype, dtype, None))),
+                      (dtype, dtype, "i64", dtype, "f32", "f32", "f32", "f32", dtype, dtype, None),
+                      (xr, wr, tr, tr, None, None, None, None, xr, wr, None))),
             (dtype.encode(), *sizes[1:]))
 
 
@@ -342,11 +344,11 @@ _TORCH_TYPES: dict = {}
 _TORCH_NAMES = {"torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
 
 
-def _buffer(name: str, b, nbytes: int, ty: str | None = None) -> int:
+def _buffer(name: str, b, nbytes: int, ty: str | None = None, row: int | None = None) -> int:
     """The device pointer of a buffer of at least `nbytes` bytes: a
     DeviceBuffer, or a tensor of another library that says where and how
     large it is (torch's `data_ptr` and `nbytes`, contiguous, on the device in
-    use, of type `ty`)."""
+    use, of type `ty`, its last axis `row` long where it has several)."""
     if hasattr(b, "data_ptr"):
         at = b.get_device()
         if at < 0:
@@ -358,6 +360,8 @@ def _buffer(name: str, b, nbytes: int, ty: str | None = None) -> int:
             have = _TORCH_TYPES[b.dtype] = _TORCH_NAMES.get(str(b.dtype), str(b.dtype))
         if have != ty and ty is not None:
             raise ValueError(f"{name} is {have}, not {ty}")
+        if row is not None and b.ndim > 1 and b.shape[-1] != row:
+            raise ValueError(f"{name} has rows of {b.shape[-1]}, not {row}")
         if not b.is_contiguous():
             raise ValueError(f"{name} is not contiguous")
         ptr, have = b.data_ptr(), b.nbytes
@@ -409,7 +413,7 @@ class Distill:
                 self._outgrown.append(self._work)
                 self._work = DeviceBuffer(need)
             work = self._work
-        bufs = [None if b is None else _buffer(s[0], b, s[1], s[2])
+        bufs = [None if b is None else _buffer(s[0], b, *s[1:])
                 for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
         return LossArgs(*self._fixed, *bufs, _buffer("work", work, need), work.nbytes)
 

@@ -139,7 +139,8 @@ def test_the_binding_checks_tensors_types_and_places():
     class Tensor:
         """A tensor in device memory as far as the checks look."""
 
-        def __init__(self, dtype, n, cuda=True, contiguous=True, device=0):
+        def __init__(self, dtype, n, cuda=True, contiguous=True, device=0, shape=(1,)):
+            self.shape, self.ndim = shape, len(shape)
             self.dtype, self.nbytes, self.whole, self.device = dtype, n, contiguous, device if cuda else -1
 
         def get_device(self):
@@ -156,6 +157,7 @@ def test_the_binding_checks_tensors_types_and_places():
     assert op.args("value", x=x, w=w, index=i, loss=f, work=Tensor(torch.uint8, 1 << 20)).rows == 4
     for bad, why in [({"x": Tensor(torch.float16, 1 << 20)}, "x is f16, not bf16"), ({"w": f}, "w is f32, not bf16"),
                      ({"index": Tensor(torch.int32, 1 << 20)}, "index is torch.int32, not i64"), ({"loss": x}, "loss is bf16, not f32"),
+                     ({"w": Tensor(torch.bfloat16, 1 << 20, shape=(100, 64))}, "w has rows of 64, not 100"),
                      ({"x": Tensor(torch.bfloat16, 1 << 20, cuda=False)}, "x is not in device memory"),
                      ({"x": Tensor(torch.bfloat16, 1 << 20, contiguous=False)}, "x is not contiguous")]:
         with pytest.raises(ValueError, match=why):
