@@ -442,9 +442,9 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
     the program's dropout sites (the course's 0.2) with training masks drawn
     from `step_key` (Key::from_seed(0) by default); 0 leaves them out (x * 1,
     the configs' reading).  `fused_head`: the head, the loss and their
-    reverse mode as one step that keeps no logits (FAST, one storage type):
-    names["loss"] is then f32 [2], the mean loss and the counted tokens, and
-    there is no names["logits"]."""
+    reverse mode as one step, the logits no buffer of the program (FAST, one
+    storage type): names["loss"] is then f32 [2], the mean loss and the counted
+    tokens, and there is no names["logits"]."""
     from . import hip, keys
     tag = dtype if realize is None else "mixed"
     p = Program(f"gpt-{'step' if train else 'forward'}-{tag}", mode=hip.FAST if mode is None else mode)

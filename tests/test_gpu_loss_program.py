@@ -1,4 +1,4 @@
-"""Programs whose head's loss keeps no logits (gpt.build(fused_head=True),
+"""Programs whose head and loss are one step (gpt.build(fused_head=True),
 llama.build(score=True)) on the device, against the same programs with the
 logits, in the interpreter's order."""
 import numpy as np
