@@ -253,6 +253,9 @@ int presk_hip_dropout_mask(const void *key, double rate, const char *type, int64
  * row with no used slot does not count: its loss and its row of dz are 0,
  * whatever its logits are.  A slot at or past `vocab` makes its row's loss and
  * cotangent NaN.  `ct` null: the mean's gradient, ct[r] = 1 / count.
+ * Given and teachers' logits may be the type's lowest value (a mask): a row of
+ * nothing else is uniform, in the value and in both together; the gradient
+ * alone knows such a row by its f32 lse, in which its log sum is lost.
  *
  * presk_hip_head_loss: z = x . w with x [rows, model] and w [model, vocab], or
  * [vocab, model] when `tied`.  The logits are the workspace's: value and

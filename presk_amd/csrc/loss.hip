@@ -127,14 +127,14 @@ struct Plan {
     bool head, value, grad;
     int st, esz, D, V, k, parts, slots, nblocks;
     long long rows, prows;
-    float c;
+    float c, nat;                     // log2 e / T and 1 / T
     bool packx, packw;
     bool once, joint;                 // f32 logits of the whole vocabulary are kept; a row of them fits a workgroup's registers
     bool blocks, counted;             // the slots' blocks are listed (`start`); the rows are counted
     int Dp, piece, pieces, spiece;    // spiece: columns a pass of row sums takes at once
     long long ldz;
     Shape zs;                         // once
-    size_t col, p, ent, start, count, most, lse, loss, coef, scale, pm, ps, pa, xp, wp, P, z, acc, partx, partw, total;
+    size_t col, p, ent, start, count, most, lse, loss, top, sum, coef, scale, pm, ps, pa, xp, wp, P, z, acc, partx, partw, total;
 };
 
 GemmArgs product(long long M, long long N, long long K, long long sa_m, long long sa_k, long long sb_k, long long sb_n, long long sc_m) {
@@ -183,6 +183,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     q.V = (int)a.vocab;
     q.k = (int)std::max<int64_t>(a.top, 1);
     q.c = (float)(1.4426950408889634074 / a.temperature);
+    q.nat = (float)(1.0 / a.temperature);
     // the counted rows' number is the mean's gradient's factor, their largest
     // cotangent f16's scale
     q.counted = a.top > 0 || (q.grad && (q.value || (head && q.st == kF16)));
@@ -206,6 +207,8 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     q.most = take(4 * q.parts);
     q.lse = take(4 * q.rows);
     q.loss = take(4 * q.rows);
+    q.top = take(q.value && q.grad ? 4 * q.rows : 0);
+    q.sum = take(q.value && q.grad ? 4 * q.rows : 0);
     q.coef = take(q.grad ? 4 * q.rows : 0);
     q.scale = take(4);
     q.slots = 0;
@@ -445,7 +448,7 @@ struct Call {
             } else {
                 LOSS_TRY(value_of(m, 0));
                 LOSS_TRY(rows_of());
-                LOSS_TRY(loss_grad(m, lse, at<float>(q.coef), to, nullptr, s));
+                LOSS_TRY(grad_of(m, lse, to, nullptr));
             }
             return pair(x, w, 0, q.V);
         }
@@ -500,6 +503,7 @@ struct Call {
         m.col0 = (int)v0;
         m.cols = n;
         m.c = q.c;
+        m.nat = q.nat;
         m.t = t;
         m.planes = 1;
         return m;
@@ -521,8 +525,13 @@ struct Call {
     // the value of logits in memory, as far as the rows' sums: whole where one
     // chunk has each row
     hipError_t value_of(const LossMatrix& m, int slot) const {
-        const LossDone d{(float)a.temperature, lse_out(), loss_out()};
+        const LossDone d{(float)a.temperature, lse_out(), loss_out(), top_out(), sum_out()};
         return loss_stats(m, at<float>(q.pm), at<float>(q.ps), at<float>(q.pa), slot, q.slots == 1 ? &d : nullptr, s);
+    }
+    // the cotangent of logits in memory, from what this call kept of their rows
+    // or, of a gradient alone, from the forward's lse
+    hipError_t grad_of(const LossMatrix& m, const float* lse, const LossTo& to, unsigned* flag) const {
+        return loss_grad(m, top_out(), q.value ? sum_out() : lse, at<float>(q.coef), to, flag, s);
     }
     hipError_t single(const float* lse) {
         const float* const x = (const float*)a.x;
@@ -562,7 +571,7 @@ struct Call {
             const int n = (int)std::min<long long>(q.piece, q.V - v);
             if (!once) {
                 if (!q.value || q.pieces > 1) LOSS_TRY(logits(v, n, false, &m));
-                LOSS_TRY(loss_grad(m, lse, at<float>(q.coef), to, nullptr, s));
+                LOSS_TRY(grad_of(m, lse, to, nullptr));
             }
             float* const dx = (float*)a.dx;
             if (dx)
@@ -583,15 +592,20 @@ struct Call {
             LOSS_TRY(loss_stats_beside(m, at<float>(q.pm), at<float>(q.ps), prep, s));
             return rows_of(m);
         }
-        if (q.value) LOSS_TRY(value_of(m, 0));
-        LOSS_TRY(rows_of());
+        // (the targets of a row in several chunks are looked up once those are joined)
+        LossMatrix sums = m;
+        if (q.slots > 1) sums.t.k = 0;
+        if (q.value) LOSS_TRY(value_of(sums, 0));
+        LOSS_TRY(rows_of(q.slots > 1 ? m : LossMatrix{}));
         if (!q.grad) return hipSuccess;
-        return loss_grad(m, lse, at<float>(q.coef), to, a.flag, s);
+        return grad_of(m, lse, to, a.flag);
     }
 
     LossMean mean_args() const { return LossMean{loss_out(), q.rows, at<int>(q.count), q.parts, t.index, a.mean}; }
     float* lse_out() const { return a.lse ? a.lse : at<float>(q.lse); }
     float* loss_out() const { return a.loss ? a.loss : at<float>(q.loss); }
+    float* top_out() const { return q.value && q.grad ? at<float>(q.top) : nullptr; }
+    float* sum_out() const { return q.value && q.grad ? at<float>(q.sum) : nullptr; }
     LossRows row_args() const {
         LossRows r{};
         r.pm = at<float>(q.pm);
@@ -599,12 +613,18 @@ struct Call {
         r.pa = at<float>(q.pa);
         // (one chunk of logits in memory: the rows are done)
         r.slots = q.slots == 1 && (!q.head || q.st == kF32 || q.once) ? 0 : q.slots;
+        // (kEpiStats leaves its sums in log 2, the row kernels in the logits' units)
+        const bool scaled = q.head && q.st != kF32 && !q.once;
+        r.unit = scaled ? 1.f : q.c;
+        r.nat = scaled ? kLn2 : q.nat;
         r.t = t;
         r.rows = q.rows;
         r.temperature = (float)a.temperature;
         if (q.value) {
             r.lse = lse_out();
             r.loss = loss_out();
+            r.top = top_out();
+            r.sum = sum_out();
             if (loss_rows_mean(q.rows)) r.mean = a.mean;
         }
         if (q.grad) {

@@ -140,7 +140,7 @@ struct LossMatrix {
     int storage;                // Storage
     long long rows;
     int col0, cols;
-    float c;
+    float c, nat;               // log2 e / T and 1 / T
     LossTarget t;
     int planes;                 // loss_stats and loss_joint in f32: the sum of so many, in order, ...
     long long plane;            // ... so many elements apart
@@ -150,11 +150,13 @@ struct LossMatrix {
 struct LossRows {
     const float *pm, *ps, *pa;  // [slots][rows]
     int slots;
+    float unit, nat;            // of pm and pa: in log 2, and in natural logarithms of u
     LossTarget t;
     LossMatrix z;               // given logits whose target's part is taken here (null: it is in pa)
     long long rows;
     float temperature;
     float *lse, *loss;          // outputs, may be null
+    float *top, *sum;           // the two parts of lse: the largest logit and log s (null: not kept)
     float* coef;                // [rows] or null
     const float* ct;
     const float* mean_in;       // {mean, count}: the count where the rows are not counted here
@@ -173,7 +175,7 @@ hipError_t loss_mean(const LossMean& m, hipStream_t s);
 // themselves (`done`, its outputs may be null)
 struct LossDone {
     float temperature;
-    float *lse, *loss;
+    float *lse, *loss, *top, *sum;
 };
 int loss_chunks(long long rows, int cols);
 hipError_t loss_stats(const LossMatrix& m, float* pm, float* ps, float* pa, int slot0, const LossDone* done, hipStream_t s);
@@ -188,8 +190,9 @@ struct LossTo {
     int storage;
     long long ld, rows;
 };
-// the logits' cotangent, coef * (softmax - target)
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s);
+// the logits' cotangent, coef * (softmax - target), from the rows' lse or, with
+// `top`, from its two parts, which hold more of it
+hipError_t loss_grad(const LossMatrix& m, const float* top, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s);
 // both of whole rows, each read once and held in registers: lse, loss (either
 // may be null) and the cotangent for ct, or for the mean over `count` (null ct)
 struct LossJoint {

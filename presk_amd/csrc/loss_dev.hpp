@@ -10,10 +10,11 @@ namespace presk {
 
 namespace {
 
-__device__ __forceinline__ float exp2_of(float z, float c, float base) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -base)); }
-// what is subtracted from u where the largest is m: a row of -inf has sum 0
+// 2^((z - base) c): the difference first, in the logits' own units, so that a
+// type's lowest value (a mask) beside another stays finite, which z c need not
+__device__ __forceinline__ float exp2_of(float z, float c, float base) { return __builtin_amdgcn_exp2f((z - base) * c); }
+// what is subtracted from z where the largest is m: a row of -inf has sum 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
-
 
 // Lane i's partner at step D of a reduction over 2 D lanes whose steps below D
 // are done (each half of them holds one value): register moves, no LDS.

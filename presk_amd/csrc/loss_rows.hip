@@ -1,9 +1,10 @@
 // The row kernels of the losses (loss.hpp): a call's targets, the row sums and
 // cotangents of logits in memory, and what joins a row's partial sums.
 //
-// A row's logits are taken as u = z * c in units of log 2 (c = log2 e / T), its
-// sum of exponentials as sum 2^(u - m) with m the largest u: one fma and one
-// v_exp_f32 (1 ulp) an element.
+// A row's sum of exponentials is taken as sum 2^((z - m) c), c = log2 e / T and m
+// the largest logit: a difference, a product and one v_exp_f32 (1 ulp) an
+// element.  Largest logits and targets stay in the logits' units: a row of the
+// type's lowest value alone, which a mask may leave, has a finite loss.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -91,10 +92,10 @@ struct Split {
     __device__ __forceinline__ int edges() const { return head + rest; }
 };
 
-// (m, s) with another (m2, s2)
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+// (m, s) with another (m2, s2), the largest in `unit`s of log 2
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float unit) {
     const float n = fmaxf(m, m2), b = base_of(n);
-    s = s * __builtin_amdgcn_exp2f(m - b) + s2 * __builtin_amdgcn_exp2f(m2 - b);
+    s = s * exp2_of(m, unit, b) + s2 * exp2_of(m2, unit, b);
     m = n;
 }
 
@@ -139,7 +140,7 @@ __device__ __forceinline__ void prep_top(const LossPrep& a, unsigned block, unsi
             }
             in[g][j] = col[q];
         }
-        top = all_of<G>(top, red, max_f) * a.c;
+        top = all_of<G>(top, red, max_f);
         seen = all_of<G>(seen, red, max_f);
         const float base = base_of(top);
         float total = 0.f;
@@ -166,7 +167,7 @@ __device__ __forceinline__ void prep_top(const LossPrep& a, unsigned block, unsi
             if (t + q * G >= k) continue;
             float p = 0.f;
             if (col[q] != kUnused) {
-                const float u = __builtin_fmaf(x[q], a.c, -base);
+                const float u = (x[q] - base) * a.c;
                 p = __builtin_amdgcn_exp2f(u) / total;
                 if (p != 0.f) ent += p * ((u - l2) * kLn2);
             }
@@ -217,11 +218,12 @@ __global__ void __launch_bounds__(256) prep_top_kernel(LossPrep a) { prep_top<ST
 
 // ---- a row's partial sums joined ------------------------------------------------
 
-// A row's loss from its largest u, its sum and its target's part: the largest
-// against the target's before anything is added to it.
-__device__ __forceinline__ float row_loss(const LossTarget& t, long long r, float temperature, float m, float log_s, float ta) {
+// A row's loss from its sum and how far its target lies below its largest logit
+// (`gap`, of which `nat` is 1 of u): the largest against the target's before
+// anything is added to it.
+__device__ __forceinline__ float row_loss(const LossTarget& t, long long r, float temperature, float gap, float nat, float log_s) {
     if (!counts(t, r)) return 0.f;
-    return temperature * temperature * (row_ent(t, r) + __builtin_fmaf(m - ta, kLn2, log_s));
+    return temperature * temperature * (row_ent(t, r) + __builtin_fmaf(gap, nat, log_s));
 }
 
 // T / G rows a workgroup, G threads a row, each over every G-th slot; with a
@@ -261,10 +263,16 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
         if (live)
             for (int p = q; p < a.slots; p += G) {
                 const long long at = (long long)p * a.rows + r;
-                join(m, s, a.pm[at], a.ps[at]);
+                join(m, s, a.pm[at], a.ps[at], a.unit);
                 if (!a.z.z) ta += a.pa[at];
             }
-        // the target's part, where the sums were taken beside the targets
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) {
+            const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+            join(m, s, m2, s2, a.unit);
+        }
+        // given logits' target, below the largest
+        float gap = 0.f;
         if (live && a.z.z)
             for (int e = q; e < a.t.k; e += G) {
                 const int col = slot_col(a.t, r, e);
@@ -273,18 +281,22 @@ __global__ void __launch_bounds__(T) rows_kernel(LossRows a) {
                 const long long at = r * a.z.ld + col;
                 const float z = a.z.storage == kF32 ? ((const float*)a.z.z)[at] : a.z.storage == kBF16 ? widen<kBF16>(((const unsigned short*)a.z.z)[at])
                                                                                                        : widen<kF16>(((const unsigned short*)a.z.z)[at]);
-                ta += p * (z * a.z.c);
+                gap += p * (m - z);
             }
 #pragma unroll
         for (int d = 1; d < G; d *= 2) {
-            const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
-            join(m, s, m2, s2);
             ta += __shfl_xor(ta, d);
+            gap += __shfl_xor(gap, d);
         }
+        if (!a.z.z) gap = m - ta;
         if (live && q == 0) {
             const float ls = pk_logf(s);
-            if (a.lse) a.lse[r] = __builtin_fmaf(m, kLn2, ls);
-            if (a.loss) a.loss[r] = row_loss(a.t, r, a.temperature, m, ls, ta);
+            if (a.lse) a.lse[r] = __builtin_fmaf(m, a.nat, ls);
+            if (a.loss) a.loss[r] = row_loss(a.t, r, a.temperature, gap, a.nat, ls);
+            if (a.top) {
+                a.top[r] = m;
+                a.sum[r] = ls;
+            }
         }
     }
     if (a.mean) {
@@ -300,10 +312,11 @@ __global__ void __launch_bounds__(1024) mean_kernel(LossMean m) { write_mean<102
 
 // ---- logits in memory -------------------------------------------------------------
 
-// Columns [lo, hi) of row r by G threads: the largest u, the sum, the target's part.
+// Columns [lo, hi) of row r by G threads: the largest logit, the sum and the
+// target's part, or of a whole row how far that lies below the largest (`gap`).
 template <int ST, int G>
-__device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int lo, int hi, int t, float* red, float& m, float& s,
-                                          float& ta) {
+__device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int lo, int hi, int t, float* red, bool gap, float& m,
+                                          float& s, float& ta) {
     typedef typename Elem<ST>::S S;
     constexpr int V = Elem<ST>::V;
     const S* const z = (const S*)a.z + r * a.ld;
@@ -318,11 +331,6 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
             for (int p = 1; p < a.planes; ++p) x += z[p * a.plane + col];
         return x;
     };
-    for (int e = t; e < a.t.k; e += G) {
-        const int col = slot_col(a.t, r, e) - a.col0;
-        const float p = slot_p(a.t, r, e);
-        if (col >= lo && col < hi && p != 0.f) ta += p * (logit(col) * a.c);
-    }
     // four vectors in flight, their largest first, then one rescale for all
     constexpr int U = 4;
     for (int i = t; i < sp.n; i += U * G) {
@@ -345,8 +353,8 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
             if (i + u * G < sp.n)
 #pragma unroll
                 for (int e = 0; e < V; ++e) x = fmaxf(x, elem<ST>(v[u], e));
-        const float n = fmaxf(m, x * a.c), b = base_of(n);
-        s *= __builtin_amdgcn_exp2f(m - b);
+        const float n = fmaxf(m, x), b = base_of(n);
+        s *= exp2_of(m, a.c, b);
         m = n;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -356,13 +364,18 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
     }
     if (t < sp.edges()) {
         const float x = logit(lo + sp.edge(t));
-        const float n = fmaxf(m, x * a.c), b = base_of(n);
-        s = s * __builtin_amdgcn_exp2f(m - b) + exp2_of(x, a.c, b);
+        const float n = fmaxf(m, x), b = base_of(n);
+        s = s * exp2_of(m, a.c, b) + exp2_of(x, a.c, b);
         m = n;
     }
     const float top = all_of<G>(m, red, max_f);
-    s *= __builtin_amdgcn_exp2f(m - base_of(top));
+    s *= exp2_of(m, a.c, base_of(top));
     m = top;
+    for (int e = t; e < a.t.k; e += G) {
+        const int col = slot_col(a.t, r, e) - a.col0;
+        const float p = slot_p(a.t, r, e);
+        if (col >= lo && col < hi && p != 0.f) ta += p * (gap ? m - logit(col) : logit(col));
+    }
     s = all_of<G>(s, red, add_f);
     ta = all_of<G>(ta, red, add_f);
 }
@@ -379,12 +392,16 @@ __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, flo
     const int t = threadIdx.x % G;
     const int lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
     float m, s, ta;
-    row_stats<ST, G>(a, r, lo, hi, t, red, m, s, ta);
+    row_stats<ST, G>(a, r, lo, hi, t, red, finish, m, s, ta);
     if (t != 0) return;
     if (finish) {
         const float ls = pk_logf(s);
-        if (done.lse) done.lse[r] = __builtin_fmaf(m, kLn2, ls);
-        if (done.loss) done.loss[r] = row_loss(a.t, r, done.temperature, m, ls, ta);
+        if (done.lse) done.lse[r] = __builtin_fmaf(m, a.nat, ls);
+        if (done.loss) done.loss[r] = row_loss(a.t, r, done.temperature, ta, a.nat, ls);
+        if (done.top) {
+            done.top[r] = m;
+            done.sum[r] = ls;
+        }
     } else {
         const long long at = (long long)(slot0 + blockIdx.y) * a.rows + r;
         pm[at] = m;
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(256) stats_beside_kernel(LossMatrix a, float* 
     const long long r = id / (unsigned)chunks;
     const int lo = (int)c * chunk;
     float m, s, ta;
-    row_stats<ST, 256>(a, r, lo, min(a.cols, lo + chunk), threadIdx.x, red, m, s, ta);
+    row_stats<ST, 256>(a, r, lo, min(a.cols, lo + chunk), threadIdx.x, red, false, m, s, ta);
     if (threadIdx.x != 0) return;
     pm[c * a.rows + r] = m;
     ps[c * a.rows + r] = s;
@@ -424,10 +441,10 @@ __device__ __forceinline__ bool first_of(const LossTarget& t, long long r, int e
     return true;
 }
 
-// c * (2^(u - l) - p), 0 where c is 0 whatever the logit
+// c * (2^((z - b) cf - l) - p), 0 where c is 0 whatever the logit
 template <int ST>
-__device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, float l, float p, float c, bool& ovf) {
-    return narrow<ST>(c == 0.f ? 0.f : (exp2_of(z, cf, l) - p) * c, ovf);
+__device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, float b, float l, float p, float c, bool& ovf) {
+    return narrow<ST>(c == 0.f ? 0.f : (__builtin_amdgcn_exp2f(__builtin_fmaf(z - b, cf, -l)) - p) * c, ovf);
 }
 
 // out = coef * (2^(u - lse) - t).  The target's columns are written after the
@@ -436,8 +453,8 @@ __device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, flo
 // bytes in and out; where value and gradient are one call and a row fits a
 // workgroup's registers, joint_kernel reads the logits once instead of twice.
 template <int SI, int SO, int G>
-__global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* lse, const float* coef, LossTo to, unsigned* flag,
-                                                   int chunk) {
+__global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* top, const float* lse, const float* coef, LossTo to,
+                                                   unsigned* flag, int chunk) {
     typedef typename Elem<SI>::S S;
     typedef typename Elem<SO>::S O;
     constexpr int V = Elem<SI>::V;
@@ -450,7 +467,7 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
         return;
     }
     const S* const z = (const S*)a.z + r * a.ld + lo;
-    const float c = coef[r], l = lse[r] * kLog2e;
+    const float c = coef[r], b = top ? base_of(top[r]) : lse[r] / a.nat, l = top ? lse[r] * kLog2e : 0.f;
     const int k = a.t.k, first = a.col0 + lo, n = hi - lo;
     bool ovf = false;
     // the logits of the target's columns, before the row is written (in place)
@@ -476,24 +493,24 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* ls
                 if constexpr (SI == SO) {
                     u32x4 w{};
 #pragma unroll
-                    for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[u], e), a.c, l, 0.f, c, ovf));
+                    for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, ovf));
                     store_vec(at, w);
                 } else {
                     O w[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[u], e), a.c, l, 0.f, c, ovf);
+                    for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, ovf);
                     __builtin_memcpy(at, w, sizeof w);
                 }
             }
     }
-    if (t < sp.edges()) o[sp.edge(t)] = cotangent<SO>(widen<SI>(z[sp.edge(t)]), a.c, l, 0.f, c, ovf);
+    if (t < sp.edges()) o[sp.edge(t)] = cotangent<SO>(widen<SI>(z[sp.edge(t)]), a.c, b, l, 0.f, c, ovf);
     for (int q = n + t; q < end; q += G) o[q] = (O)0;
     __builtin_amdgcn_s_waitcnt(0);
     if constexpr (G > 64) __syncthreads();
     for (int q = 0; q < E && t + q * G < k; ++q) {
         const int e = t + q * G, col = slot_col(a.t, r, e) - first;
         float p;
-        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<SO>(zt[q], a.c, l, p, c, ovf);
+        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<SO>(zt[q], a.c, b, l, p, c, ovf);
     }
     if (SO == kF16 && ovf && flag) atomicOr(flag, 1u);
 }
@@ -548,16 +565,15 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
 #pragma unroll
                     for (int e = 0; e < V; ++e) v[i][e] = pk_bits(pk_float(v[i][e]) + pk_float(w[e]));
                 }
-    float zt[E], ta = 0.f;
+    float zt[E], pt[E];
 #pragma unroll
     for (int q = 0; q < E; ++q) {
-        zt[q] = 0.f;
+        zt[q] = pt[q] = 0.f;
         if (t + q * G < k) {
             const int col = slot_col(tg, r, t + q * G);
-            const float p = slot_p(tg, r, t + q * G);
             if (col < n) {
                 zt[q] = logit(col);
-                if (p != 0.f) ta += p * (zt[q] * cf);
+                pt[q] = slot_p(tg, r, t + q * G);
             }
         }
     }
@@ -589,8 +605,12 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
     // (every load of this thread has landed before the barriers below, and so
     // before any thread writes the row: the output may be the input)
     __builtin_amdgcn_s_waitcnt(0);
-    m = all_of<G>(m, red, max_f) * cf;
+    m = all_of<G>(m, red, max_f);
     const float b = base_of(m);
+    float gap = 0.f;
+#pragma unroll
+    for (int q = 0; q < E; ++q)
+        if (pt[q] != 0.f) gap += pt[q] * (m - zt[q]);
     // (the vectors stay packed between the passes: their elements widened once
     // for all three would be twice the registers)
     auto packed = [&]() {
@@ -605,13 +625,13 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
 #pragma unroll
             for (int e = 0; e < V; ++e) s += exp2_of(elem<SI>(v[i], e), cf, b);
     s = all_of<G>(s, red, add_f);
-    ta = all_of<G>(ta, red, add_f);
-    const float ls = pk_logf(s), l = __builtin_fmaf(m, kLn2, ls);
+    gap = all_of<G>(gap, red, add_f);
+    const float ls = pk_logf(s);
     if (t == 0) {
-        if (a.lse) a.lse[r] = l;
-        if (a.loss) a.loss[r] = row_loss(tg, r, a.temperature, m, ls, ta);
+        if (a.lse) a.lse[r] = __builtin_fmaf(m, a.m.nat, ls);
+        if (a.loss) a.loss[r] = row_loss(tg, r, a.temperature, gap, a.m.nat, ls);
     }
-    const float l2 = l * kLog2e;
+    const float l2 = ls * kLog2e;
     bool ovf = false;
     packed();
 #pragma unroll
@@ -621,16 +641,16 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
             if constexpr (SI == SO) {
                 u32x4 w{};
 #pragma unroll
-                for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[i], e), cf, l2, 0.f, c, ovf));
+                for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, ovf));
                 store_row<NT>(at, w);
             } else {
                 O w[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[i], e), cf, l2, 0.f, c, ovf);
+                for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, ovf);
                 __builtin_memcpy(at, w, sizeof w);
             }
         }
-    if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, l2, 0.f, c, ovf);
+    if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, b, l2, 0.f, c, ovf);
     if constexpr (SI != SO)
         for (long long q = n + t; q < a.to.ld; q += G) o[q] = (O)0;
     __builtin_amdgcn_s_waitcnt(0);
@@ -641,7 +661,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
         if (e >= k) break;
         const int col = slot_col(tg, r, e);
         float p;
-        if (col < n && first_of(tg, r, e, p)) o[col] = cotangent<SO>(zt[q], cf, l2, p, c, ovf);
+        if (col < n && first_of(tg, r, e, p)) o[col] = cotangent<SO>(zt[q], cf, b, l2, p, c, ovf);
     }
     if (SO == kF16 && ovf && a.flag) atomicOr(a.flag, 1u);
 }
@@ -755,11 +775,11 @@ hipError_t stats_beside(LossMatrix m, float* pm, float* ps, const LossPrep& p, h
 }
 
 template <int SI, int SO>
-hipError_t grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
+hipError_t grad(const LossMatrix& m, const float* top, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
     const int chunks = loss_chunks(m.rows, m.cols), chunk = chunk_cols(m.cols, chunks);
     const unsigned rows = (unsigned)std::max(m.rows, to.rows);
-    if (m.cols <= 1024) grad_kernel<SI, SO, 64><<<dim3((rows + 3) / 4), 256, 0, s>>>(m, lse, coef, to, flag, m.cols);
-    else grad_kernel<SI, SO, 256><<<dim3(rows, (unsigned)chunks), 256, 0, s>>>(m, lse, coef, to, flag, chunk);
+    if (m.cols <= 1024) grad_kernel<SI, SO, 64><<<dim3((rows + 3) / 4), 256, 0, s>>>(m, top, lse, coef, to, flag, m.cols);
+    else grad_kernel<SI, SO, 256><<<dim3(rows, (unsigned)chunks), 256, 0, s>>>(m, top, lse, coef, to, flag, chunk);
     return hipGetLastError();
 }
 
@@ -878,13 +898,13 @@ hipError_t loss_stats_beside(const LossMatrix& m, float* pm, float* ps, const Lo
     return hipErrorInvalidValue;
 }
 
-hipError_t loss_grad(const LossMatrix& m, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
+hipError_t loss_grad(const LossMatrix& m, const float* top, const float* lse, const float* coef, const LossTo& to, unsigned* flag, hipStream_t s) {
     if (m.rows <= 0 || m.cols <= 0) return hipSuccess;
-    if (m.storage == kF32 && to.storage == kF32) return grad<kF32, kF32>(m, lse, coef, to, flag, s);
-    if (m.storage == kBF16 && to.storage == kBF16) return grad<kBF16, kBF16>(m, lse, coef, to, flag, s);
-    if (m.storage == kF16 && to.storage == kF16) return grad<kF16, kF16>(m, lse, coef, to, flag, s);
-    if (m.storage == kF32 && to.storage == kBF16) return grad<kF32, kBF16>(m, lse, coef, to, flag, s);
-    if (m.storage == kF32 && to.storage == kF16) return grad<kF32, kF16>(m, lse, coef, to, flag, s);
+    if (m.storage == kF32 && to.storage == kF32) return grad<kF32, kF32>(m, top, lse, coef, to, flag, s);
+    if (m.storage == kBF16 && to.storage == kBF16) return grad<kBF16, kBF16>(m, top, lse, coef, to, flag, s);
+    if (m.storage == kF16 && to.storage == kF16) return grad<kF16, kF16>(m, top, lse, coef, to, flag, s);
+    if (m.storage == kF32 && to.storage == kBF16) return grad<kF32, kBF16>(m, top, lse, coef, to, flag, s);
+    if (m.storage == kF32 && to.storage == kF16) return grad<kF32, kF16>(m, top, lse, coef, to, flag, s);
     return hipErrorInvalidValue;
 }
 

@@ -1,0 +1,117 @@
+"""The losses on the device where a mask is the type's lowest value, against
+float64 under the bounds of tests/test_gpu_loss.py (its Case).
+
+A row's loss and cotangent do not change when its logits, or its teacher's,
+are all moved by one number, so the reference takes both below their row's
+largest: a difference to the largest that the kernels take too, within half a
+step of itself.  What lies 200 T or more below it (e^-200 of the largest: no
+part of a sum in f32 or in the compared digits) stands at -200 T there, so that
+the bounds, which grow with a logit, stay those of the others."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from presk_amd import hip  # noqa: E402
+from tests.test_gpu_loss import DEV, E24, T, Case  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def device():
+    hip.init(0)
+    yield
+    torch.cuda.synchronize()
+
+
+def below(x, t):
+    x = x.double()
+    return (x - x.amax(-1, keepdim=True)).clamp_min(-200.0 * t)
+
+
+def reference(k, teacher_only=False):
+    s = Case(k.dtype, k.rows, k.vocab, d=k.d, tied=k.tied, top=k.top, t=k.t, seed=0)
+    s.index, s.ct = k.index, k.ct
+    s.x, s.w = (k.x, k.w) if k.d else (below(k.x, k.t), None)
+    s.teacher = below(k.teacher, k.t)
+    return s.exact()
+
+
+def check(got, r, e, names, rows=None):
+    for m in names:
+        off, bound = (got[m].double() - r[m]).abs(), e[m]
+        bad = ~(off <= bound)
+        if rows is not None:
+            bad = bad[rows]
+        assert not bool(bad.any()), (m, bad.nonzero()[:4].tolist())
+
+
+LOW = [(dt, *s) for dt in ("f32", "bf16", "f16") for s in [
+    # rows, vocab, top, T: each of the row kernels' widths, one chunk and several,
+    # slots beside the sums and before them
+    (12, 50, 4, 1.0), (12, 1000, 4, 2.0), (12, 5000, 4, 1.0), (12, 5000, 70, 1.0), (200, 5000, 4, 1.5), (12, 70000, 4, 1.0),
+    (1100, 70000, 3, 1.0), (12, 140000, 5, 2.0), (12, 140000, 100, 1.0),
+]]
+
+
+@pytest.mark.parametrize("c", LOW, ids=str)
+def test_distill_of_rows_and_slots_at_the_lowest_value(c):
+    """Rows whose mask leaves nothing (softmax uniform), half masked rows, and
+    teachers' slots of the lowest value, some and all of a row's."""
+    dt, rows, vocab, top, t = c
+    low = torch.finfo(T[dt]).min
+    k = Case(dt, rows, vocab, top=top, t=t, seed=rows + vocab, pad=False, ct=True)
+    k.index = torch.stack([torch.randperm(vocab // 2, device=DEV)[:top] if top <= vocab // 2 else torch.arange(top, device=DEV)
+                           for _ in range(rows)]).contiguous()
+    k.x[0], k.x[3] = low, low
+    k.x[1, vocab // 2:] = low
+    k.teacher[2], k.teacher[3] = low, low
+    k.teacher[4, 1:] = low
+    k.index[5] = -1
+    k.x[5] = low
+    r, e = reference(k)
+    got = k.run("step")
+    check(got, r, e, ("loss", "dx"))
+    value = k.run("value")
+    check(value, r, e, ("loss",))
+    scale = k.x.double().amax(-1) / t
+    for v in (got, value):
+        off = (v["lse"].double() - (r["lse"] + scale)).abs()
+        assert bool((off <= e["lse"] + (scale.abs() + r["lse"].abs()) * 4 * E24).all())
+    # the gradient alone knows of a row its f32 lse, in which log V is lost
+    # beside the lowest value of the wider types
+    whole = torch.ones(rows, dtype=torch.bool, device=DEV)
+    whole[0] = whole[3] = False
+    g = k.run("vjp", lse=value["lse"])
+    # (the lse is in the logits' own place, and half a step of it, of T's product
+    # and of the difference to it moves an exponent)
+    q, moved = torch.softmax(below(k.x, t) / t, -1), torch.expm1(8 * E24 * scale.abs())
+    e["dx"] = e["dx"] + 2 * q * (moved * k.ct.double() * t)[:, None]
+    check(g, r, e, ("dx",), whole)
+    assert bool(g["dx"].isfinite().all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(9, 300), (9, 5000), (300, 4000)])
+def test_distill_of_a_target_at_the_lowest_value(dt, rows, vocab):
+    """A masked column that the teacher wants: a loss of the logits' own size,
+    not an infinity, where f32 holds it."""
+    k = Case(dt, rows, vocab, top=1, t=1.0, seed=1, pad=False, ct=True)
+    low = torch.finfo(T[dt]).min
+    k.x[4, 7], k.index[4] = low, 7
+    want = float(k.x[4].double().amax()) - low
+    for kind in ("step", "value"):
+        got = float(k.run(kind)["loss"][4])
+        assert abs(got - want) <= want * 2.0 ** -10, (kind, got, want)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("top", [3, 6, 100, 300])
+def test_head_of_a_teacher_at_the_lowest_value(dt, top):
+    k = Case(dt, 70, 900, d=64, top=top, t=2.0, seed=top, ct=True)
+    low = torch.finfo(T[dt]).min
+    k.teacher[0], k.teacher[3, 1:] = low, low
+    k.index[0] = torch.arange(top, device=DEV)
+    r, e = reference(k)
+    for kind in ("step", "value"):
+        check(k.run(kind), r, e, ("loss", "lse") + (("dx", "dw") if kind == "step" else ()))
