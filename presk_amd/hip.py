@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import sys
 
 import numpy as np
 
@@ -372,6 +373,18 @@ def _buffer(name: str, b, nbytes: int, ty: str | None = None, row: int | None = 
     return ptr
 
 
+def _stream_of(bufs, stream):
+    """The stream of a call over these buffers: the caller's, or, where it names
+    none and a buffer is torch's, torch's current one, on which the tensors
+    were made and are read next (0 is the null stream)."""
+    torch = sys.modules.get("torch")
+    if stream is None and torch is not None:
+        for b in bufs:
+            if isinstance(b, torch.Tensor) and b.is_cuda:
+                return torch.cuda.current_stream(b.get_device()).cuda_stream
+    return stream
+
+
 class Distill:
     """presk_hip_distill at fixed sizes: the divergence of given logits x
     [rows, vocab] from the softmax of a teacher's `top` logits, teacher[r, j]
@@ -381,11 +394,12 @@ class Distill:
     mean and their number), those given.  `vjp` writes the logits' cotangent
     dx from the forward's lse, for a row's cotangent ct (f32 [rows]), or for
     the mean's where mean is given in its place.  `value_and_grad` does both,
-    for ct or else the mean.  Buffers are DeviceBuffers or torch tensors;
-    `work` is workspace(kind) bytes of the caller's, or, not given, a buffer
-    this object keeps (with any smaller one it has outgrown, which a captured
-    call may still use): calls that share a workspace, their captured graphs
-    among them, run one after another (one stream, or an object a stream)."""
+    for ct or else the mean.  Buffers are DeviceBuffers or torch tensors; a call
+    with tensors that names no stream goes to torch's current one, others to
+    the null stream.  `work` is workspace(kind) bytes of the caller's, or, not
+    given, a buffer that this object keeps for the call's stream (with any
+    smaller one outgrown, which a captured call may still use): calls that
+    share a workspace, their captured graphs among them, run one after another."""
 
     head = False
 
@@ -396,7 +410,8 @@ class Distill:
         self.dtype, self.rows, self.model, self.vocab, self.top = dtype, int(rows), int(model), int(vocab), int(top)
         self.tied, self.temperature = bool(tied), float(temperature)
         self._sizes = (self.dtype, self.rows, self.model, self.vocab, self.top, self.tied, self.temperature)
-        self._work, self._outgrown = None, []
+        self._work = None       # the workspace last used of the object's own
+        self._works = {}        # stream -> those taken for it, the largest last
         self._specs, self._fixed = _loss_layout(self._sizes)
 
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
@@ -404,21 +419,30 @@ class Distill:
         with the gradients asked for."""
         return _loss_workspace(self._sizes, LOSS_WHAT[kind], dx, dw and self.head)
 
+    @property
+    def _outgrown(self) -> list:
+        return [b for own in self._works.values() for b in own if b is not self._work]
+
+    def _own_work(self, need: int, stream):
+        own = self._works.setdefault(getattr(stream, "value", stream) or 0, [])
+        if not own or own[-1].nbytes < need:
+            own.append(DeviceBuffer(need))
+        self._work = own[-1]
+        return self._work
+
     def args(self, kind: str, x=None, w=None, index=None, teacher=None, loss=None, lse=None, mean=None, ct=None, dx=None, dw=None,
-             flag=None, work=None) -> LossArgs:
-        """The call's arguments, each buffer checked against its size."""
+             flag=None, work=None, stream=None) -> LossArgs:
+        """The arguments of a call on `stream`, each buffer checked against its size."""
         need = self.workspace(kind, dx is not None, dw is not None)
         if work is None:
-            if self._work is None or self._work.nbytes < need:
-                self._outgrown.append(self._work)
-                self._work = DeviceBuffer(need)
-            work = self._work
+            work = self._own_work(need, stream)
         bufs = [None if b is None else _buffer(s[0], b, *s[1:])
                 for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
         return LossArgs(*self._fixed, *bufs, _buffer("work", work, need), work.nbytes)
 
     def _call(self, kind, stream, **bufs):
-        a = self.args(kind, **bufs)
+        stream = _stream_of(bufs.values(), stream)
+        a = self.args(kind, stream=stream, **bufs)
         f = lib().presk_hip_head_loss if self.head else lib().presk_hip_distill
         check(f(ctypes.byref(a), LOSS_WHAT[kind], stream))
 

@@ -115,3 +115,27 @@ def test_head_of_a_teacher_at_the_lowest_value(dt, top):
     r, e = reference(k)
     for kind in ("step", "value"):
         check(k.run(kind), r, e, ("loss", "lse") + (("dx", "dw") if kind == "step" else ()))
+
+
+def test_a_call_without_a_stream_follows_torchs_current_one():
+    """Inputs made on a side stream, late, and the outputs read there: the call
+    that names no stream lies between."""
+    n, v = 64, 2000
+    k = Case("f32", n, v, top=4, seed=1, ct=False)
+    want = k.run("value")["loss"]
+    x, loss, op = torch.zeros_like(k.x), torch.empty(n, device=DEV), k.op()
+    late = torch.randn(4096, 4096, device=DEV)
+    op.value(k.x, k.index, k.teacher, loss=loss)
+    torch.cuda.synchronize()
+    for own in (True, False):
+        work = None if own else torch.empty(op.workspace("value"), dtype=torch.uint8, device=DEV)
+        x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                torch.mm(late, late)
+            x.copy_(k.x)
+            op.value(x, k.index, k.teacher, loss=loss, work=work)
+            got = loss.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), own
