@@ -345,17 +345,17 @@ _TORCH_TYPES: dict = {}
 _TORCH_NAMES = {"torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
 
 
-def _buffer(name: str, b, nbytes: int, ty: str | None = None, row: int | None = None) -> int:
+def _buffer(name: str, b, device, nbytes: int, ty: str | None = None, row: int | None = None) -> int:
     """The device pointer of a buffer of at least `nbytes` bytes: a
     DeviceBuffer, or a tensor of another library that says where and how
-    large it is (torch's `data_ptr` and `nbytes`, contiguous, on the device in
-    use, of type `ty`, its last axis `row` long where it has several)."""
+    large it is (torch's `data_ptr` and `nbytes`, contiguous, on `device`, any
+    where that is not known, of type `ty`, its last axis `row` long where it has several)."""
     if hasattr(b, "data_ptr"):
         at = b.get_device()
         if at < 0:
             raise ValueError(f"{name} is not in device memory")
-        if at != _initialized and _initialized not in (None, -1):
-            raise ValueError(f"{name} is on device {at}, not {_initialized}")
+        if at != device and device not in (None, -1):
+            raise ValueError(f"{name} is on device {at}, not {device}")
         have = _TORCH_TYPES.get(b.dtype)
         if have is None:
             have = _TORCH_TYPES[b.dtype] = _TORCH_NAMES.get(str(b.dtype), str(b.dtype))
@@ -373,16 +373,20 @@ def _buffer(name: str, b, nbytes: int, ty: str | None = None, row: int | None = 
     return ptr
 
 
-def _stream_of(bufs, stream):
-    """The stream of a call over these buffers: the caller's, or, where it names
-    none and a buffer is torch's, torch's current one, on which the tensors
+def _place_of(bufs, stream) -> tuple:
+    """(device, stream) of a call over these buffers.  With a tensor of torch's
+    among them: the current device, on which the kernels run, and the caller's
+    stream or, where it names none, torch's current one, on which the tensors
     were made and are read next (0 is the null stream)."""
     torch = sys.modules.get("torch")
-    if stream is None and torch is not None:
+    if torch is not None:
         for b in bufs:
             if isinstance(b, torch.Tensor) and b.is_cuda:
-                return torch.cuda.current_stream(b.get_device()).cuda_stream
-    return stream
+                now = torch.cuda.current_device()
+                if now != _initialized and _initialized not in (None, -1):
+                    raise ValueError(f"the current device is {now}, not {_initialized}")
+                return now, torch.cuda.current_stream(now).cuda_stream if stream is None else stream
+    return _initialized, stream
 
 
 class Distill:
@@ -431,18 +435,20 @@ class Distill:
         return self._work
 
     def args(self, kind: str, x=None, w=None, index=None, teacher=None, loss=None, lse=None, mean=None, ct=None, dx=None, dw=None,
-             flag=None, work=None, stream=None) -> LossArgs:
-        """The arguments of a call on `stream`, each buffer checked against its size."""
+             flag=None, work=None, stream=None, device=None) -> LossArgs:
+        """The arguments of a call on `stream`, each buffer checked against its
+        size and `device` (the one initialised)."""
+        device = _initialized if device is None else device
         need = self.workspace(kind, dx is not None, dw is not None)
         if work is None:
             work = self._own_work(need, stream)
-        bufs = [None if b is None else _buffer(s[0], b, *s[1:])
+        bufs = [None if b is None else _buffer(s[0], b, device, *s[1:])
                 for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
-        return LossArgs(*self._fixed, *bufs, _buffer("work", work, need), work.nbytes)
+        return LossArgs(*self._fixed, *bufs, _buffer("work", work, device, need), work.nbytes)
 
     def _call(self, kind, stream, **bufs):
-        stream = _stream_of(bufs.values(), stream)
-        a = self.args(kind, stream=stream, **bufs)
+        device, stream = _place_of(bufs.values(), stream)
+        a = self.args(kind, stream=stream, device=device, **bufs)
         f = lib().presk_hip_head_loss if self.head else lib().presk_hip_distill
         check(f(ctypes.byref(a), LOSS_WHAT[kind], stream))
 

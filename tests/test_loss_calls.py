@@ -87,3 +87,18 @@ def test_the_own_workspace_is_a_streams(calls):
     op._works[0x10][0].nbytes = 16
     op.value(Memory(1024), Memory(64), Memory(32), loss=Memory(16), stream=0x10)
     assert calls[-1][0] not in w and small in op._outgrown and op._work not in op._outgrown
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(calls, monkeypatch):
+    """Also where the executor was not initialised by device, or torch's
+    current device was changed after that."""
+    op = hip.Distill("f32", 4, 64, 2)
+    for initialized in (None, -1, 0):
+        monkeypatch.setattr(hip, "_initialized", initialized)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+        for stream in (None, 0, 0x7000):
+            with pytest.raises(ValueError, match="is on device 0, not 1" if initialized != 0 else "current device is 1, not 0"):
+                op.value(**inputs(), stream=stream)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        op.value(**inputs())
+    assert len(calls) == 3
