@@ -262,25 +262,32 @@ class Builder:
     def cross_entropy_vjp(self, logits, y, ct, name=None):
         return self._prim(lambda dt: L.cross_entropy_vjp([self.op(logits), self.op(y), self.op(ct)], dt), [logits, y, ct], name)
 
-    def head_loss(self, x, w, y, kind):
-        """The mean cross entropy of x . w against y without the logits, as one
-        step (hip.HeadLoss; `kind` "value", or "step" with the gradients of x
-        and w): no nests of the interpreter's, so FAST and one storage type
-        only.  Returns {"loss": its mean and the counted rows (f32 [2]),
-        "ce": each row's loss (f32)} and, with the gradients, "dx" and "dw"."""
+    def head_loss(self, x, w, y, kind, name=""):
+        """The mean cross entropy of x . w against y, its logits no buffer of the
+        program, as one step (hip.HeadLoss; `kind` "value", or "step" with the
+        gradients of x and w): no nests of the interpreter's, so FAST and one
+        storage type only.  Returns {"loss": its mean and the counted rows (f32
+        [2]), "ce": each row's loss (f32)} and, with the gradients, "dx" and
+        "dw"; a second head of a program has a `name`, which its buffers'
+        begin with."""
         from . import hip
         if self.p.mode != hip.FAST or self.realize is not None:
             raise ValueError("E7005: a head's loss without its logits is built in FAST mode and one storage type")
+        if kind not in ("value", "step"):
+            raise ValueError(f"a head's loss of kind {kind!r}, not value or step")
         ax = self.axes[x]
         rows = math.prod(a.len for a in ax[:-1])
-        out = {"loss": "loss", "ce": "ce"}
-        bufs = {"x": self.base.get(x, x), "w": w, "index": y, "mean": "loss", "loss": "ce", "lse": "lse"}
+        out = {k: name + b for k, b in (("loss", "loss"), ("ce", "ce"))}
+        bufs = {**{k: self.base.get(b, b) for k, b in (("x", x), ("w", w), ("index", y))},
+                "mean": name + "loss", "loss": name + "ce", "lse": name + "lse"}
         if kind == "step":
-            out.update(dx="d.xf", dw="d.head")
-            bufs.update(dx="d.xf", dw="d.head")
-            self.input("d.xf", ax), self.input("d.head", self.axes[w])
-        self.input("loss", A(2)), self.input("ce", ax[:-1]), self.input("lse", ax[:-1])
+            grads = {"dx": name + "d.xf", "dw": name + "d.head"}
+            out.update(grads)
+            bufs.update(grads)
         self.p.add_loss(kind, self.dt, rows, self.axes[w][-1].len, bufs, model=ax[-1].len)
+        if kind == "step":
+            self.input(out["dx"], ax), self.input(out["dw"], self.axes[w])
+        self.input(out["loss"], A(2)), self.input(out["ce"], ax[:-1]), self.input(bufs["lse"], ax[:-1])
         return out
 
     def dropout_mask(self, x, slot: int, rate: float, name=None):

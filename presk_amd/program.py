@@ -171,10 +171,22 @@ class Program:
         """Appends the loss of a head x . w (`model` its states' width) or of
         given logits x (`model` 0): `kind` "value", "vjp" or "step" (both);
         `bufs` the buffer of each argument of hip.HeadLoss, outputs among
-        them.  Returns bufs."""
-        self.losses.append(LossStep(len(self.launches), kind, dtype, int(rows), int(vocab), int(model), int(top), bool(tied),
-                                    float(temperature), bufs))
+        them, which no other step writes.  Returns bufs."""
+        if kind not in hip.LOSS_WHAT:
+            raise ValueError(f"a loss of kind {kind!r}, not one of {', '.join(hip.LOSS_WHAT)}")
+        st = LossStep(len(self.launches), kind, dtype, int(rows), int(vocab), int(model), int(top), bool(tied), float(temperature), bufs)
+        if unknown := sorted(set(bufs) - set(st.specs())):
+            raise ValueError(f"a loss has no argument {unknown[0]}")
+        written = {ln.out for ln in self.launches} | {m[0] for m in self.masks} | self._loss_outputs()
+        for a in st.writes():
+            if bufs[a] in written:
+                raise ValueError(f"buffer {bufs[a]}, a loss's {a}, is another step's output")
+            written.add(bufs[a])
+        self.losses.append(st)
         return bufs
+
+    def _loss_outputs(self) -> set:
+        return {st.bufs[a] for st in self.losses for a in st.writes()}
 
     def input_specs(self):
         """(name, (storage type, element count)) of everything a step reads, in
@@ -190,6 +202,8 @@ class Program:
     def add(self, low: L.Lowered, ins: list, out: str, scales=()) -> str:
         """Appends one launch of `low` reading buffers `ins`, writing `out`
         (and `scales`, the scales of its integer inputs)."""
+        if out in self._loss_outputs():
+            raise ValueError(f"buffer {out} is a loss's output")
         self.launches.append(Launch(low, list(ins), out, scales))
         return out
 
