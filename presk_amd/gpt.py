@@ -278,7 +278,8 @@ class Builder:
         ax = self.axes[x]
         rows = math.prod(a.len for a in ax[:-1])
         out = {k: name + b for k, b in (("loss", "loss"), ("ce", "ce"))}
-        bufs = {"x": self.base.get(x, x), "w": w, "index": y, "mean": name + "loss", "loss": name + "ce", "lse": name + "lse"}
+        bufs = {**{k: self.base.get(b, b) for k, b in (("x", x), ("w", w), ("index", y))},
+                "mean": name + "loss", "loss": name + "ce", "lse": name + "lse"}
         if kind == "step":
             grads = {"dx": name + "d.xf", "dw": name + "d.head"}
             out.update(grads)

@@ -57,3 +57,12 @@ def test_two_heads_of_one_program():
     assert not set(first.values()) & set(second.values()) and len(p.losses) == 2
     with pytest.raises(ValueError, match="kind 'vjp'"):
         b.head_loss("x", "w", "y", "vjp", name="third.")
+
+
+def test_a_views_buffer_is_its_bases():
+    p = Program("t", hip.FAST)
+    b = Builder(p, "f32")
+    b.input("x", A(("rows", 8), ("model", 64))), b.input("flat", A(("n", 6400))), b.input("ids", A(("b", 2), ("s", 4)), "idx")
+    b.view("flat", A(("model", 64), ("vocab", 100)), "w"), b.view("ids", A(("rows", 8)), "y")
+    b.head_loss("x", "w", "y", "value")
+    assert [name for name, _ in p.input_specs()] == ["x", "flat", "ids"]
