@@ -139,3 +139,59 @@ def test_a_call_without_a_stream_follows_torchs_current_one():
             got = loss.clone()
         torch.cuda.synchronize()
         assert torch.equal(got, want), own
+
+
+def along(k, name):
+    """A direction of x or w with rows (columns of a head's weights) of one
+    length, against which each row's mean loss is steep, and the largest range
+    that the logits / T of a row change by along it: (v, ranges)."""
+    base = getattr(k, name).double().requires_grad_()
+    x, w = (base, k.w) if name == "x" else (k.x, base)
+    z = x.double()
+    if k.d:
+        z = z @ (w.t() if k.tied else w).double()
+    p = torch.softmax((k.teacher.double() / k.t).masked_fill(k.index < 0, -torch.inf), -1).nan_to_num(0.0) if k.top else (k.index >= 0).double()[:, None]
+    at = k.index.reshape(k.rows, -1).clamp_min(0)
+    u = z / k.t
+    # (the reference's direction alone; the loss itself is the device's)
+    v, = torch.autograd.grad((p.sum(-1) * torch.logsumexp(u, -1) - (p * u.gather(1, at)).sum(-1)).sum(), base)
+    v = v / v.norm(dim=-1, keepdim=True).clamp_min(1e-30)
+    x, w = (v, k.w) if name == "x" else (k.x, v)
+    a = x.double()
+    if k.d:
+        a = a @ (w.t() if k.tied else w).double()
+    return v, (a.amax(-1) - a.amin(-1)) / k.t
+
+
+@pytest.mark.parametrize("d,tied,top,t", [(48, False, 5, 2.0), (48, True, 3, 1.5), (48, False, 0, 1.0), (0, False, 5, 2.0)], ids=str)
+def test_gradients_are_the_values_steep_differences(d, tied, top, t):
+    """f(h) - f(-h) = 2 h f' + h^3 / 3 f''' of the mean f along a line of x or w,
+    on which the logits are linear: f''' is T^2 times the mean of the third
+    central moments of a row's change a / T under its softmax, at most R^3 /
+    (6 sqrt 3) of a change of range R.  Beside it stand both values' errors and
+    the gradient's own.  h leaves that an eighth of the difference or less, so a
+    gradient of 0, of the other sign, or with a factor of T too many or too few
+    is outside it."""
+    k = Case("f32", 40, 200, d=d, tied=tied, top=top, t=t, seed=3, ct=False)
+    got = k.run("step")
+    _, e = k.exact()
+    for name, grad in (("x", "dx"), ("w", "dw"))[:2 if d else 1]:
+        v, ranges = along(k, name)
+        h = 0.5 / float(ranges.max())
+        base = getattr(k, name)
+        vals, ends, off = [], [], 0.0
+        for s in (h, -h):
+            setattr(k, name, (base + s * v).float().contiguous())
+            ends.append(getattr(k, name).double())
+            vals.append(float(k.run("value")["mean"][0]))
+            off += float(k.exact()[1]["mean"])
+        setattr(k, name, base)
+        step = ends[0] - ends[1]
+        slope, change = float((got[grad].double() * step).sum()), vals[0] - vals[1]
+        third = t * t * float((ranges ** 3).mean()) / (6 * 3 ** 0.5)
+        err = off + h ** 3 / 3 * third + float((e[grad] * step.abs()).sum())
+        print(name, "change", change, "slope", slope, "bound", err)
+        assert abs(change - slope) <= err
+        assert err <= abs(slope) / 8
+        for wrong in (0.0, -slope) + ((slope / t, slope * t) if t != 1.0 else ()):
+            assert abs(change - wrong) > err, wrong
