@@ -195,3 +195,25 @@ def test_gradients_are_the_values_steep_differences(d, tied, top, t):
         assert err <= abs(slope) / 8
         for wrong in (0.0, -slope) + ((slope / t, slope * t) if t != 1.0 else ()):
             assert abs(change - wrong) > err, wrong
+
+
+def test_two_streams_at_once():
+    """Calls in turn on two streams with nothing waited for between them, each
+    object with the workspace that it keeps for its stream, one object on both
+    among them: the bits of the calls alone."""
+    cases = [Case("bf16", 500, 3000, d=256, seed=1, ct=False), Case("f16", 300, 9000, top=20, t=2.0, seed=2),
+             Case("f32", 400, 1500, d=96, tied=True, top=7, seed=3, ct=False)]
+    want = [k.run("step") for k in cases]
+    ops, streams, rounds = [k.op() for k in cases], [torch.cuda.Stream() for _ in range(2)], 6
+    outs = [[[{m: torch.empty_like(x) for m, x in w.items()} for w in want] for _ in streams] for _ in range(rounds)]
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        for s, made in zip(streams, outs[i]):
+            with torch.cuda.stream(s):
+                for k, op, o in zip(cases, ops, made):
+                    op.value_and_grad(**k.ins(), **o, ct=k.ct)
+    torch.cuda.synchronize()
+    for i in range(rounds):
+        for made in outs[i]:
+            for w, o in zip(want, made):
+                assert [m for m in w if not torch.equal(w[m], o[m])] == [], i
