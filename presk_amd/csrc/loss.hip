@@ -703,26 +703,6 @@ std::string loss_check(const presk_hip_loss& a, int what, bool head) {
     return "";
 }
 
-std::array<LossBuffer, 12> loss_buffers(const presk_hip_loss& a, int what, bool head) {
-    const bool value = what & PRESK_HIP_LOSS_VALUE, grad = what & PRESK_HIP_LOSS_GRAD;
-    const long long esz = storage_code(a.dtype) == kF32 ? 4 : 2, k = std::max<int64_t>(a.top, 1);
-    const long long nx = a.rows * (head ? a.model : a.vocab) * esz, nw = head ? a.model * a.vocab * esz : 0;
-    return {{
-        {"x", a.x, nx, (int)esz, false, true},
-        {"w", a.w, nw, (int)esz, false, head},
-        {"index", a.index, 8 * a.rows * k, 8, false, true},
-        {"teacher", a.teacher, esz * a.rows * a.top, (int)esz, false, a.top > 0},
-        {"ct", a.ct, grad ? 4 * a.rows : 0, 4, false, false},
-        {"loss", a.loss, value ? 4 * a.rows : 0, 4, value, false},
-        {"lse", a.lse, 4 * a.rows, 4, value, !value},
-        {"mean", a.mean, 8, 4, value, !value && !a.ct},
-        {"dx", a.dx, grad ? nx : 0, (int)esz, true, grad && !head},
-        {"dw", a.dw, grad ? nw : 0, (int)esz, true, false},
-        {"flag", a.flag, 4, 4, true, false},
-        {"work", a.work, (long long)a.work_bytes, 16, true, true},
-    }};
-}
-
 namespace {
 
 // The buffers of a checked call: their presence, alignment, and that no output

@@ -5,10 +5,10 @@
 
 #include <hip/hip_runtime.h>
 
-#include <array>
 #include <string>
 
 #include "gemm.hpp"
+#include "loss_buffers.hpp"
 #include "presk_hip.h"
 
 namespace presk {
@@ -19,15 +19,6 @@ namespace presk {
 // of given logits.
 std::string loss_check(const presk_hip_loss& a, int what, bool head);
 std::string loss_check_all(const presk_hip_loss& a, int what, bool head);
-// a checked call's buffers
-struct LossBuffer {
-    const char* name;
-    const void* p;
-    long long bytes;
-    int align;
-    bool out, need;
-};
-std::array<LossBuffer, 12> loss_buffers(const presk_hip_loss& a, int what, bool head);
 // the bytes of workspace a checked call needs
 size_t loss_workspace(const presk_hip_loss& a, int what, bool head);
 // the launches of a checked call, and with the check in front (`why` it was refused)

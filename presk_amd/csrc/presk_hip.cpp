@@ -760,10 +760,7 @@ std::vector<BranchStep> branch_steps(const presk_hip_batch& b) {
         st.to = it.to;
         st.n = it.n;
         st.rate = it.rate;
-        if (it.what)
-            for (const LossBuffer& f : loss_buffers(it.loss, it.what, it.head))
-                if (f.p && f.bytes > 0 && f.p != it.loss.flag)
-                    (f.out ? st.wr : st.rd).push_back({(uintptr_t)f.p, (uintptr_t)f.p + (size_t)f.bytes});
+        if (it.what) loss_spans(it.loss, it.what, it.head, &st.rd, &st.wr);
         out.push_back(std::move(st));
     }
     return out;
