@@ -11,9 +11,13 @@
 // products over the whole vocabulary leaves the row sums (kEpiStats) and no
 // logits; for the gradient one goes over it a piece at a time, the cotangent of
 // a piece (kEpiP) entering dx, whose sum over the pieces stays in f32, and the
-// piece's part of dw.  Together that is four products, and a workspace that
-// does not grow with the vocabulary.  8192 x 4096 x 32000 in bf16, loss and
-// gradients: 5.45 ms with the logits kept, 7.06 computed twice.
+// piece's part of dw.  Together that is four products.  8192 x 4096 x 32000 in
+// bf16, loss and gradients: 5.45 ms with the logits kept, 7.06 computed twice.
+// The workspace of pieces: a piece's cotangent, 128 MiB or, of many rows, that of
+// 256 columns; 12 bytes a row and column tile (256 columns, of few rows 128) of
+// the whole vocabulary for the value's row sums; and with more than four slots a
+// row 2 bytes a row and 64 columns for the lists of their blocks.  So it grows
+// with the vocabulary, by an 85th to a 51st of what its f32 logits would take.
 // In f32 the logits are products of gemm.hpp in the workspace, a piece at a
 // time or all, and row kernels turn them into their cotangent in place.
 #include "loss.hpp"
