@@ -263,8 +263,8 @@ int presk_hip_dropout_mask(const void *key, double rate, const char *type, int64
  * either alone, they come in pieces of the vocabulary.  Gradients dx = dz . w^T and dw = x^T . dz, either
  * of which may be null.  The products accumulate in f32; in 16-bit storage the
  * factor ct[r] * (exp(u[r] - lse[r]) - t[r]) of dz is rounded to the storage type
- * before them (by a power of two in f16's range), T and the mean's 1 / count
- * come after.
+ * before them (by a power of two in f16's range; of up to 64 rows what the
+ * rounding left enters too, rounded itself), T and the mean's 1 / count come after.
  * A row of x that does not count still enters dw times zero, so it must be
  * finite.
  * presk_hip_distill: z = x, given (model 0, w null, top >= 1); dx is dz.

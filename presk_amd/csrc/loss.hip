@@ -42,6 +42,15 @@ constexpr long long kPieceBytes = 128ll << 20;  // a piece's logits or their cot
 constexpr long long kOnceBytes = 256ll << 20;   // f32 logits that are one piece: as many as the Infinity Cache holds, ...
 constexpr long long kKeepBytes = 4ll << 30;     // ... and where the gradient follows the value, so that they stay for it
 constexpr int kPieceCols = 256;                 // a piece is a multiple of these
+// 16-bit storage: up to so many rows the cotangent enters dx and dw in two 16-bit
+// parts, its rounding and what that left; past them its rounding alone, whose
+// errors average over the rows (the gradients' whole error against the outputs'
+// rounding alone: 1.34 to 1.46 times it over 200 sizes of more rows; of fewer up
+// to 2.1, 43 of 382 gradients over 1.5; in two parts 1.00).  The second part is
+// half as many products again or more: 8 x 4096 x 32000 in bf16, both gradients,
+// 205 us in one part and 259 in two; 65 rows 226 and 287; 8192 rows 5.33 and 8.57
+// ms.
+constexpr int kFineRows = 64;
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
@@ -134,6 +143,7 @@ struct Plan {
     float c, nat;                     // log2 e / T and 1 / T
     bool packx, packw;
     bool once, joint;                 // f32 logits of the whole vocabulary are kept; a row of them fits a workgroup's registers
+    bool two;                         // the 16-bit cotangent is in two parts
     bool blocks, counted;             // the slots' blocks are listed (`start`); the rows are counted
     int Dp, piece, pieces, spiece;    // spiece: columns a pass of row sums takes at once
     long long ldz;
@@ -172,7 +182,7 @@ GemmArgs product_dw(const Plan& q, bool tied, long long n) {
 // the gradients' products of a 16-bit piece of n columns (one that is not
 // asked for has no tiles)
 void pair_shapes(const Plan& q, const presk_hip_loss& a, int n, Shape* x, Shape* w) {
-    pair_of(a.dx ? q.rows : 0, q.D, up(n, 64), !a.dw ? 0 : a.tied ? n : q.D, a.tied ? q.D : n, q.prows, x, w);
+    pair_of(a.dx ? q.rows : 0, q.D, up(n, 64) << q.two, !a.dw ? 0 : a.tied ? n : q.D, a.tied ? q.D : n, q.prows << q.two, x, w);
 }
 
 Plan plan_of(const presk_hip_loss& a, int what, bool head) {
@@ -201,6 +211,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
     const bool half = head && q.st != kF32;
     q.once = half && q.rows && q.value && q.grad && 4 * q.rows * up(q.V, 4) <= kKeepBytes;
     q.prows = up(q.rows, 64);
+    q.two = half && q.grad && q.rows <= kFineRows;
     q.nblocks = (int)(up(q.V, kCols) / kCols);
     q.col = take(4 * q.rows * a.top);
     q.p = take(4 * q.rows * a.top);
@@ -258,7 +269,7 @@ Plan plan_of(const presk_hip_loss& a, int what, bool head) {
             q.z = take(4ll * q.zs.splits * q.rows * q.ldz);
         }
         if (q.grad) {
-            q.P = take(2 * q.prows * up(std::min<long long>(q.piece, q.V), 64));
+            q.P = take((2 * q.prows * up(std::min<long long>(q.piece, q.V), 64)) << q.two);
             q.acc = take(a.dx && q.pieces > 1 ? 4 * q.rows * up(q.D, 4) : 0);
             long long px = 0, pw = 0;
             for (long long v = 0; v < q.V; v += q.piece) {
@@ -380,6 +391,7 @@ struct Call {
             g->splits = h.splits;
             g->scale = at<float>(q.scale);
             g->flag = a.flag;
+            g->two = q.two;
         }
         if (a.dx) {
             // dx[r][d] += sum over the piece of P[r][v] w(v, d); P is zero past the piece
@@ -395,6 +407,7 @@ struct Call {
             dx.N = q.D;
             dx.K = (int)pld;
             dx.acc = at<float>(q.acc);
+            dx.a2 = 2 * q.prows * pld;
             dx.lda = up(q.D, 4);
             dx.acc_in = v > 0;
             dx.part = at<float>(q.partx);
@@ -416,6 +429,7 @@ struct Call {
             dw.M = a.tied ? n : q.D;
             dw.N = a.tied ? q.D : n;
             dw.K = (int)q.prows;
+            (a.tied ? dw.a2 : dw.b2) = 2 * q.prows * pld;
             dw.lda = up(dw.N, 4);
             dw.part = at<float>(q.partw);
             dw.C = (unsigned short*)a.dw + (a.tied ? v * q.D : v);
@@ -443,7 +457,7 @@ struct Call {
             LossMatrix m = matrix(at<float>(q.z), q.ldz, kF32, 0, q.V);
             m.planes = q.zs.splits;
             m.plane = q.rows * q.ldz;
-            const LossTo to{at<void>(q.P), q.st, up(q.V, 64), q.prows};
+            const LossTo to{at<void>(q.P), q.st, up(q.V, 64), q.prows, q.two ? q.prows * up(q.V, 64) : 0};
             if (q.joint) {
                 LossJoint j = joint_args(m, to);
                 j.scale = at<float>(q.scale);
@@ -481,6 +495,7 @@ struct Call {
             g.coef = at<float>(q.coef);
             g.P = at<unsigned short>(q.P);
             g.pld = up(n, 64);
+            g.plow = q.two ? q.prows * g.pld : 0;
             g.prows = (int)q.prows;
             LOSS_TRY(half_gemm(g, kEpiP, h.tile));
             LOSS_TRY(pair(x, w, v, n));

@@ -55,6 +55,8 @@ struct LossGemm {
     int arows, brows;           // rows that exist (those past them are read from the last ones)
     int ka, kb;                 // k that exist
     int M, N, K;                // the product's extent (rows stored, k summed)
+    bool two;                   // dx, dw: one operand is in two parts, summed (a2 or b2 bytes apart)
+    long long a2, b2;
     int tiles_m, tiles_n, splits;
     // values: u = z * c, in units of log 2
     float c;
@@ -64,7 +66,7 @@ struct LossGemm {
     float *pm, *ps, *pa;        // a column tile's maximum, sum and target part: [tile][rows]
     const float *lse, *coef;    // [rows]
     unsigned short* P;          // the logits' cotangent, [prows][pld], zero past rows and cols
-    long long pld;
+    long long pld, plow;        // elements from P to its second part (0: none)
     int prows;
     // outputs
     void* C;                    // 16-bit, row stride ldc (null: the f32 sums stay in acc)
@@ -180,6 +182,7 @@ struct LossTo {
     void* p;
     int storage;
     long long ld, rows;
+    long long low;              // 16 bits of f32: elements to what the rounding left, rounded itself (0: not kept)
 };
 // the logits' cotangent, coef * (softmax - target), from the rows' lse or, with
 // `top`, from its two parts, which hold more of it

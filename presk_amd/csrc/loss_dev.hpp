@@ -34,6 +34,9 @@ __device__ __forceinline__ float partner(float v) {
     }
 }
 
+// what the rounding of v to 16 bits left of it (nothing beside an infinity)
+__device__ __forceinline__ float left_of(float v, float rounded) { return __builtin_fabsf(rounded) < INFINITY ? v - rounded : 0.f; }
+
 // Over G threads (16, 64: as many lanes of a wave; more: the workgroup,
 // through `red`, G / 64 floats): the same value in every one, met in a fixed tree.
 template <int G, typename F>

@@ -89,8 +89,9 @@ struct Block16 {
         }
         lds0 = __builtin_amdgcn_readfirstlane(tile + (unsigned)(t & ~63) * 16u);
     }
-    __device__ __forceinline__ void issue(int kb, unsigned stage) const {
-        const char* const src = origin + kb * block_bytes;
+    // block kb, `part` bytes further on
+    __device__ __forceinline__ void issue(int kb, unsigned stage, long long part) const {
+        const char* const src = origin + kb * block_bytes + part;
         const int left = nk - kb * BK;      // k of this block that exist
         if (left >= BK) {
 #pragma unroll
@@ -206,7 +207,7 @@ typedef Tile<1, 8, 2, 4> Tile128x8;    // one, three blocks ahead
 
 // Item `id` of `total` of a product, a tile and a range of k; `id` counts from a
 // workgroup whose number is a multiple of 8.
-template <int ST, bool AKC, bool BKC, typename TL, int EPI>
+template <int ST, bool AKC, bool BKC, typename TL, int EPI, bool TWO = false>
 __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned total, unsigned char* smem) {
     constexpr int WM = TL::WM, NW = TL::NW, WAN = TL::WAN, WN = 2, NTH = TL::NTH, BM = TL::BM, BN = TL::BN;
     typedef Block16<AKC, BM, NTH> QA;
@@ -237,7 +238,10 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
         for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
 
     // split s of S takes k-blocks [s * n / S, (s + 1) * n / S)
-    const unsigned nkb = (unsigned)((g.K + BK - 1) / BK), ns = (unsigned)g.splits;
+    // (TWO, an operand in two parts: a block of each in turn, against the other
+    // operand's same block)
+    constexpr int two = TWO;
+    const unsigned nkb = (unsigned)((g.K + BK - 1) / BK) << two, ns = (unsigned)g.splits;
     const int kb0 = (int)((unsigned)split * nkb / ns), nd = (int)(((unsigned)split + 1) * nkb / ns) - kb0;
 
     // Blocks kt + 1 .. kt + STAGES - 1 stream into their stages while block kt
@@ -252,10 +256,8 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
     qa.init(g.A, g.arows, g.sa, m0, g.ka, lds);
     qb.init(g.B, g.brows, g.sb, n0, g.kb, lds + QA::BYTES);
-    auto fetch = [&](int kb, int st) {
-        qa.issue(kb0 + kb, (unsigned)(st * STAGE));
-        qb.issue(kb0 + kb, (unsigned)(st * STAGE));
-    };
+    auto fetch_a = [&](int kb, int st) { qa.issue((kb0 + kb) >> two, (unsigned)(st * STAGE), (kb0 + kb) & two ? g.a2 : 0); };
+    auto fetch_b = [&](int kb, int st) { qb.issue((kb0 + kb) >> two, (unsigned)(st * STAGE), (kb0 + kb) & two ? g.b2 : 0); };
     u16x8 a[WM], b[WN];
     auto read = [&](const unsigned char* st, int kk) {
 #pragma unroll
@@ -265,7 +267,10 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
     };
     if (nd > 0) {
         const int pre = nd < LA ? nd : LA;
-        for (int kb = 0; kb < pre; ++kb) fetch(kb, kb);
+        for (int kb = 0; kb < pre; ++kb) {
+            fetch_a(kb, kb);
+            fetch_b(kb, kb);
+        }
         wait_blocks<NL, LA - 1>(pre - 1);
         __syncthreads();
         read(smem, 0);
@@ -279,8 +284,8 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
             // (8192 x 4096 x 32000, loss and gradients, 7.17 ms, 7.06 so, 7.00
             // with the MFMAs' priority)
             if (kt + LA < nd) {
-                if (kk == 0) qa.issue(kb0 + kt + LA, (unsigned)((CUR + LA) % NS * STAGE));
-                if (kk == 16) qb.issue(kb0 + kt + LA, (unsigned)((CUR + LA) % NS * STAGE));
+                if (kk == 0) fetch_a(kt + LA, (CUR + LA) % NS);
+                if (kk == 16) fetch_b(kt + LA, (CUR + LA) % NS);
             }
             u16x8 ca[WM], cb[WN];
 #pragma unroll
@@ -433,22 +438,41 @@ __device__ __forceinline__ void tile_of(const LossGemm& g, unsigned id, unsigned
 #pragma unroll
             for (int j = 0; j < WN; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = coef == 0.f ? 0.f : acc[i][j][4 * q + e] * coef;
-                    uint2 v;
-                    v.x = narrow2<ST>(x[0], x[1]);
-                    v.y = narrow2<ST>(x[2], x[3]);
-                    *(uint2*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
-                }
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = coef == 0.f ? 0.f : acc[i][j][e] * coef;
         }
-        __syncthreads();
-        constexpr int VPR = BN / 8;
-        for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
-            const int r = u / VPR, c = u % VPR * 8;
-            if (m0 + r < g.prows && n0 + c < g.pld)
-                *(u16x8*)(g.P + (long long)(m0 + r) * g.pld + n0 + c) = *(const u16x8*)&ct[r * CLD + c];
+        // the tile rounded, then, of a P in two parts, what that left
+        for (long long part = 0;; part = g.plow) {
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                const int row = wm + i * 32 + (lane & 31);
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint2 v;
+                        v.x = narrow2<ST>(acc[i][j][4 * q], acc[i][j][4 * q + 1]);
+                        v.y = narrow2<ST>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                        *(uint2*)&ct[row * CLD + wn + col_of(j, 4 * q, lane)] = v;
+                    }
+            }
+            __syncthreads();
+            constexpr int VPR = BN / 8;
+            for (int u = threadIdx.x; u < BM * VPR; u += NTH) {
+                const int r = u / VPR, c = u % VPR * 8;
+                if (m0 + r < g.prows && n0 + c < g.pld)
+                    *(u16x8*)(g.P + part + (long long)(m0 + r) * g.pld + n0 + c) = *(const u16x8*)&ct[r * CLD + c];
+            }
+            if (part == g.plow) break;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const unsigned short h = ST == kBF16 ? pk_f32_to_bf16(acc[i][j][e]) : pk_f32_to_f16(acc[i][j][e]);
+                        acc[i][j][e] = left_of(acc[i][j][e], ST == kBF16 ? pk_bf16_to_f32(h) : pk_f16_to_f32(h));
+                    }
         }
     } else {
         const float scale = g.scale ? *g.scale : 1.f;
@@ -565,14 +589,14 @@ __global__ void __launch_bounds__(TL::NTH, 2) loss_logits_kernel(LossGemm g, uns
 }
 
 // dx (A the cotangent, k-contiguous), dw (neither operand), the mean
-template <int ST, bool XBKC, typename TL>
+template <int ST, bool XBKC, typename TL, bool TWO>
 __global__ void __launch_bounds__(TL::NTH, 2) loss_pair_kernel(LossGemm x, LossGemm w, unsigned nx, unsigned nx8, unsigned nw, LossMean m) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[TL::BYTES];
     const unsigned id = blockIdx.x;
     if (id < nx8) {
-        if (id < nx) tile_of<ST, true, XBKC, TL, kEpiDx>(x, id, nx, smem);
+        if (id < nx) tile_of<ST, true, XBKC, TL, kEpiDx, TWO>(x, id, nx, smem);
     } else if (id < nx8 + nw) {
-        tile_of<ST, false, false, TL, kEpiDw>(w, id - nx8, nw, smem);
+        tile_of<ST, false, false, TL, kEpiDw, TWO>(w, id - nx8, nw, smem);
     } else {
         write_mean<TL::NTH>(m);
     }
@@ -606,14 +630,20 @@ hipError_t logits_of(const LossGemm& g, int tile, const LossPrep& p, hipStream_t
     return hipGetLastError();
 }
 
-template <int ST, bool XBKC>
+template <int ST, bool XBKC, bool TWO>
 hipError_t pair_of(const LossGemm& x, const LossGemm& w, int tile, const LossMean& m, hipStream_t s) {
     const unsigned nx = items_of(x), nx8 = (nx + 7) / 8 * 8, nw = items_of(w), grid = nx8 + nw + (m.loss ? 1 : 0);
     if (!grid) return hipSuccess;
-    if (tile == 256) loss_pair_kernel<ST, XBKC, Tile256><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
-    else if (tile == kDeep128) loss_pair_kernel<ST, XBKC, Tile128x8><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
-    else loss_pair_kernel<ST, XBKC, Tile128><<<grid, 256, 0, s>>>(x, w, nx, nx8, nw, m);
+    if (tile == 256) loss_pair_kernel<ST, XBKC, Tile256, TWO><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
+    else if (tile == kDeep128) loss_pair_kernel<ST, XBKC, Tile128x8, TWO><<<grid, 512, 0, s>>>(x, w, nx, nx8, nw, m);
+    else loss_pair_kernel<ST, XBKC, Tile128, TWO><<<grid, 256, 0, s>>>(x, w, nx, nx8, nw, m);
     return hipGetLastError();
+}
+
+template <int ST>
+hipError_t pair(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s) {
+    if (x.two) return xbkc ? pair_of<ST, true, true>(x, w, tile, m, s) : pair_of<ST, false, true>(x, w, tile, m, s);
+    return xbkc ? pair_of<ST, true, false>(x, w, tile, m, s) : pair_of<ST, false, false>(x, w, tile, m, s);
 }
 
 }  // namespace

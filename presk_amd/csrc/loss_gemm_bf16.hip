@@ -10,7 +10,7 @@ hipError_t loss_logits_bf16(const LossGemm& g, bool bkc, int tile, const LossPre
     return bkc ? logits_of<kBF16, true>(g, tile, p, s) : logits_of<kBF16, false>(g, tile, p, s);
 }
 hipError_t loss_pair_bf16(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s) {
-    return xbkc ? pair_of<kBF16, true>(x, w, tile, m, s) : pair_of<kBF16, false>(x, w, tile, m, s);
+    return pair<kBF16>(x, w, xbkc, tile, m, s);
 }
 
 }  // namespace presk

@@ -10,7 +10,7 @@ hipError_t loss_logits_f16(const LossGemm& g, bool bkc, int tile, const LossPrep
     return bkc ? logits_of<kF16, true>(g, tile, p, s) : logits_of<kF16, false>(g, tile, p, s);
 }
 hipError_t loss_pair_f16(const LossGemm& x, const LossGemm& w, bool xbkc, int tile, const LossMean& m, hipStream_t s) {
-    return xbkc ? pair_of<kF16, true>(x, w, tile, m, s) : pair_of<kF16, false>(x, w, tile, m, s);
+    return pair<kF16>(x, w, xbkc, tile, m, s);
 }
 
 }  // namespace presk

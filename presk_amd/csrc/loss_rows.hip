@@ -441,10 +441,13 @@ __device__ __forceinline__ bool first_of(const LossTarget& t, long long r, int e
     return true;
 }
 
-// c * (2^((z - b) cf - l) - p), 0 where c is 0 whatever the logit
+// c * (2^((z - b) cf - l) - p), 0 where c is 0 whatever the logit; `part` 1: what
+// its rounding leaves
 template <int ST>
-__device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, float b, float l, float p, float c, bool& ovf) {
-    return narrow<ST>(c == 0.f ? 0.f : (__builtin_amdgcn_exp2f(__builtin_fmaf(z - b, cf, -l)) - p) * c, ovf);
+__device__ __forceinline__ typename Elem<ST>::S cotangent(float z, float cf, float b, float l, float p, float c, int part, bool& ovf) {
+    const float v = c == 0.f ? 0.f : (__builtin_amdgcn_exp2f(__builtin_fmaf(z - b, cf, -l)) - p) * c;
+    const typename Elem<ST>::S h = narrow<ST>(v, ovf);
+    return part ? narrow<ST>(left_of(v, widen<ST>(h)), ovf) : h;
 }
 
 // out = coef * (2^(u - lse) - t).  The target's columns are written after the
@@ -460,10 +463,12 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* to
     constexpr int V = Elem<SI>::V;
     const long long r = G == 64 ? (long long)blockIdx.x * 4 + threadIdx.x / 64 : (long long)blockIdx.x;
     const int t = threadIdx.x % G, lo = (int)blockIdx.y * chunk, hi = min(a.cols, lo + chunk);
-    O* const o = (O*)to.p + r * to.ld + lo;
+    O* o = (O*)to.p + r * to.ld + lo;
     const int end = (int)((hi == a.cols && SI != SO ? to.ld : hi) - lo);   // columns written
+    const int parts = SI != SO && to.low ? 2 : 1;
     if (r >= a.rows) {
-        for (int q = t; q < end && r < to.rows; q += G) o[q] = (O)0;
+        for (int q = t; q < end && r < to.rows; q += G)
+            for (int part = 0; part < parts; ++part) o[q + part * to.low] = (O)0;
         return;
     }
     const S* const z = (const S*)a.z + r * a.ld + lo;
@@ -481,36 +486,38 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* to
     if constexpr (G > 64) __syncthreads();
     const Split<SI> sp(z, n);
     constexpr int U = 2;
-    for (int i = t; i < sp.n; i += U * G) {
-        u32x4 v[U];
+    for (int part = 0; part < parts; ++part, o += to.low) {
+        for (int i = t; i < sp.n; i += U * G) {
+            u32x4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + u * G < sp.n) v[u] = load_vec(z + sp.head + (long long)(i + u * G) * V);
+            for (int u = 0; u < U; ++u)
+                if (i + u * G < sp.n) v[u] = load_vec(z + sp.head + (long long)(i + u * G) * V);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + u * G < sp.n) {
-                O* const at = o + sp.head + (long long)(i + u * G) * V;
-                if constexpr (SI == SO) {
-                    u32x4 w{};
+            for (int u = 0; u < U; ++u)
+                if (i + u * G < sp.n) {
+                    O* const at = o + sp.head + (long long)(i + u * G) * V;
+                    if constexpr (SI == SO) {
+                        u32x4 w{};
 #pragma unroll
-                    for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, ovf));
-                    store_vec(at, w);
-                } else {
-                    O w[V];
+                        for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, 0, ovf));
+                        store_vec(at, w);
+                    } else {
+                        O w[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, ovf);
-                    __builtin_memcpy(at, w, sizeof w);
+                        for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[u], e), a.c, b, l, 0.f, c, part, ovf);
+                        __builtin_memcpy(at, w, sizeof w);
+                    }
                 }
-            }
-    }
-    if (t < sp.edges()) o[sp.edge(t)] = cotangent<SO>(widen<SI>(z[sp.edge(t)]), a.c, b, l, 0.f, c, ovf);
-    for (int q = n + t; q < end; q += G) o[q] = (O)0;
-    __builtin_amdgcn_s_waitcnt(0);
-    if constexpr (G > 64) __syncthreads();
-    for (int q = 0; q < E && t + q * G < k; ++q) {
-        const int e = t + q * G, col = slot_col(a.t, r, e) - first;
-        float p;
-        if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<SO>(zt[q], a.c, b, l, p, c, ovf);
+        }
+        if (t < sp.edges()) o[sp.edge(t)] = cotangent<SO>(widen<SI>(z[sp.edge(t)]), a.c, b, l, 0.f, c, part, ovf);
+        for (int q = n + t; q < end; q += G) o[q] = (O)0;
+        __builtin_amdgcn_s_waitcnt(0);
+        if constexpr (G > 64) __syncthreads();
+        for (int q = 0; q < E && t + q * G < k; ++q) {
+            const int e = t + q * G, col = slot_col(a.t, r, e) - first;
+            float p;
+            if (col >= 0 && col < n && first_of(a.t, r, e, p)) o[col] = cotangent<SO>(zt[q], a.c, b, l, p, c, part, ovf);
+        }
     }
     if (SO == kF16 && ovf && flag) atomicOr(flag, 1u);
 }
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(256) grad_kernel(LossMatrix a, const float* to
 // with the row past the caches (NT), 235 without; of 0.26 GB, which the
 // Infinity Cache holds, 68 with and 63 without (8192 x 8000); f32 logits of
 // 8192 x 32000 into bf16, 1.57 GB, 277 with and 300 without.
-template <int SI, int SO, int G, int R, int E, bool NT>
+template <int SI, int SO, int G, int R, int E, bool NT, bool TWO>
 __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kernel(LossJoint a) {
     typedef typename Elem<SI>::S S;
     typedef typename Elem<SO>::S O;
@@ -532,11 +539,13 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
     const long long r = G == 16 ? (long long)blockIdx.x * 16 + threadIdx.x / 16
                         : G == 64 ? (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : (long long)blockIdx.x;
     const int t = threadIdx.x % G, k = tg.k, n = a.m.cols;
-    O* const o = (O*)a.to.p + r * a.to.ld;
+    O* o = (O*)a.to.p + r * a.to.ld;
+    constexpr int parts = TWO ? 2 : 1;
     // (all threads of a row)
     if (r >= a.m.rows) {
         if (r < a.to.rows)
-            for (long long c = t; c < a.to.ld; c += G) o[c] = (O)0;
+            for (long long c = t; c < a.to.ld; c += G)
+                for (int part = 0; part < parts; ++part) o[c + part * a.to.low] = (O)0;
         return;
     }
     const S* const z = (const S*)a.m.z + r * a.m.ld;
@@ -633,35 +642,37 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, R <= 8 ? 8 : 4) joint_kerne
     }
     const float l2 = ls * kLog2e;
     bool ovf = false;
-    packed();
+    for (int part = 0; part < parts; ++part, o += a.to.low) {
+        packed();
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-        if (t + i * G < sp.n) {
-            char* const at = (char*)(o + sp.head) + i * G * V * (int)sizeof(O) + (unsigned)t * (unsigned)(V * sizeof(O));
-            if constexpr (SI == SO) {
-                u32x4 w{};
+        for (int i = 0; i < R; ++i)
+            if (t + i * G < sp.n) {
+                char* const at = (char*)(o + sp.head) + i * G * V * (int)sizeof(O) + (unsigned)t * (unsigned)(V * sizeof(O));
+                if constexpr (SI == SO) {
+                    u32x4 w{};
 #pragma unroll
-                for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, ovf));
-                store_row<NT>(at, w);
-            } else {
-                O w[V];
+                    for (int e = 0; e < V; ++e) set_elem<SO>(w, e, cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, 0, ovf));
+                    store_row<NT>(at, w);
+                } else {
+                    O w[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, ovf);
-                __builtin_memcpy(at, w, sizeof w);
+                    for (int e = 0; e < V; ++e) w[e] = cotangent<SO>(elem<SI>(v[i], e), cf, b, l2, 0.f, c, part, ovf);
+                    __builtin_memcpy(at, w, sizeof w);
+                }
             }
-        }
-    if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, b, l2, 0.f, c, ovf);
-    if constexpr (SI != SO)
-        for (long long q = n + t; q < a.to.ld; q += G) o[q] = (O)0;
-    __builtin_amdgcn_s_waitcnt(0);
-    if constexpr (G > 64) __syncthreads();
+        if (edge) o[sp.edge(t)] = cotangent<SO>(last, cf, b, l2, 0.f, c, part, ovf);
+        if constexpr (SI != SO)
+            for (long long q = n + t; q < a.to.ld; q += G) o[q] = (O)0;
+        __builtin_amdgcn_s_waitcnt(0);
+        if constexpr (G > 64) __syncthreads();
 #pragma unroll
-    for (int q = 0; q < E; ++q) {
-        const int e = t + q * G;
-        if (e >= k) break;
-        const int col = slot_col(tg, r, e);
-        float p;
-        if (col < n && first_of(tg, r, e, p)) o[col] = cotangent<SO>(zt[q], cf, b, l2, p, c, ovf);
+        for (int q = 0; q < E; ++q) {
+            const int e = t + q * G;
+            if (e >= k) break;
+            const int col = slot_col(tg, r, e);
+            float p;
+            if (col < n && first_of(tg, r, e, p)) o[col] = cotangent<SO>(zt[q], cf, b, l2, p, c, part, ovf);
+        }
     }
     if (SO == kF16 && ovf && a.flag) atomicOr(a.flag, 1u);
 }
@@ -783,25 +794,25 @@ hipError_t grad(const LossMatrix& m, const float* top, const float* lse, const f
     return hipGetLastError();
 }
 
-template <int SI, int SO, int G, int R, bool NT>
+template <int SI, int SO, int G, int R, bool NT, bool TWO>
 void joint_of(const LossJoint& a, long long rows, hipStream_t s) {
     constexpr int T = G < 256 ? 256 : G;
     constexpr int per = T / G;
     const unsigned grid = (unsigned)((rows + per - 1) / per);
-    if (a.m.t.k <= G) joint_kernel<SI, SO, G, R, 1, NT><<<grid, T, 0, s>>>(a);
-    else joint_kernel<SI, SO, G, R, G == 16 ? 4 : 1024 / G, NT><<<grid, T, 0, s>>>(a);
+    if (a.m.t.k <= G) joint_kernel<SI, SO, G, R, 1, NT, TWO><<<grid, T, 0, s>>>(a);
+    else joint_kernel<SI, SO, G, R, G == 16 ? 4 : 1024 / G, NT, TWO><<<grid, T, 0, s>>>(a);
 }
 
-template <int SI, int SO, bool NT>
+template <int SI, int SO, bool NT, bool TWO = false>
 hipError_t joint(const LossJoint& a, hipStream_t s) {
     const int nv = a.m.cols / Elem<SI>::V;
     const long long n = std::max(a.m.rows, a.to.rows);
-    if (nv <= 16 * 4 && a.m.t.k <= 64) joint_of<SI, SO, 16, 4, NT>(a, n, s);
-    else if (nv <= 64 * 4) joint_of<SI, SO, 64, 4, NT>(a, n, s);
-    else if (nv <= 256 * 4) joint_of<SI, SO, 256, 4, NT>(a, n, s);
-    else if (nv <= 512 * 8) joint_of<SI, SO, 512, 8, NT>(a, n, s);
-    else if (nv <= 1024 * 8) joint_of<SI, SO, 1024, 8, NT>(a, n, s);
-    else joint_of<SI, SO, 1024, 16, NT>(a, n, s);
+    if (nv <= 16 * 4 && a.m.t.k <= 64) joint_of<SI, SO, 16, 4, NT, TWO>(a, n, s);
+    else if (nv <= 64 * 4) joint_of<SI, SO, 64, 4, NT, TWO>(a, n, s);
+    else if (nv <= 256 * 4) joint_of<SI, SO, 256, 4, NT, TWO>(a, n, s);
+    else if (nv <= 512 * 8) joint_of<SI, SO, 512, 8, NT, TWO>(a, n, s);
+    else if (nv <= 1024 * 8) joint_of<SI, SO, 1024, 8, NT, TWO>(a, n, s);
+    else joint_of<SI, SO, 1024, 16, NT, TWO>(a, n, s);
     return hipGetLastError();
 }
 // of the caller's logits into the caller's buffer: past the caches where the two
@@ -915,10 +926,12 @@ hipError_t loss_joint(const LossJoint& a, hipStream_t s) {
     if (a.m.storage == kF32 && a.to.storage == kF32) return joint_rows<kF32>(a, s);
     if (a.m.storage == kBF16 && a.to.storage == kBF16) return joint_rows<kBF16>(a, s);
     if (a.m.storage == kF16 && a.to.storage == kF16) return joint_rows<kF16>(a, s);
-    const bool nt = 4 * a.m.rows * a.m.ld > (256ll << 20);
-    if (a.m.storage == kF32 && a.to.storage == kBF16) return nt ? joint<kF32, kBF16, true>(a, s) : joint<kF32, kBF16, false>(a, s);
-    if (a.m.storage == kF32 && a.to.storage == kF16) return nt ? joint<kF32, kF16, true>(a, s) : joint<kF32, kF16, false>(a, s);
-    return hipErrorInvalidValue;
+    if (a.m.storage != kF32 || (a.to.storage != kBF16 && a.to.storage != kF16)) return hipErrorInvalidValue;
+    // (two parts are few rows', which the caches hold)
+    const bool bf = a.to.storage == kBF16;
+    if (a.to.low) return bf ? joint<kF32, kBF16, false, true>(a, s) : joint<kF32, kF16, false, true>(a, s);
+    if (4 * a.m.rows * a.m.ld > (256ll << 20)) return bf ? joint<kF32, kBF16, true>(a, s) : joint<kF32, kF16, true>(a, s);
+    return bf ? joint<kF32, kBF16, false>(a, s) : joint<kF32, kF16, false>(a, s);
 }
 
 hipError_t loss_pack(const LossPack& a, const LossPack& b, hipStream_t s) {

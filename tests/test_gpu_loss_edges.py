@@ -12,7 +12,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from presk_amd import hip  # noqa: E402
-from tests.test_gpu_loss import DEV, E24, T, Case  # noqa: E402
+from tests.test_gpu_loss import DEV, E24, HALF, TINY, Case, T  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,44 @@ def test_two_streams_at_once():
         for made in outs[i]:
             for w, o in zip(want, made):
                 assert [m for m in w if not torch.equal(w[m], o[m])] == [], i
+
+
+FINE = [(dt, *s) for dt in ("bf16", "f16") for s in [
+    # rows, d, vocab, tied, top, T: one piece with a row in a workgroup's
+    # registers, longer rows, and (the gradient alone) tiles of the products;
+    # sizes that are and are not whole vectors
+    (1, 64, 500, False, 0, 1.0), (3, 45, 1272, True, 0, 1.0), (3, 96, 770, False, 18, 2.0), (8, 200, 5003, False, 2, 1.0),
+    (21, 1168, 400, False, 1, 2.0), (64, 320, 1347, False, 0, 1.0), (64, 40, 6656, True, 9, 1.5), (17, 40, 70003, False, 0, 1.0),
+    (5, 72, 66001, True, 7, 1.0), (33, 4096, 640, False, 0, 1.0),
+]]
+
+
+@pytest.mark.parametrize("c", FINE, ids=str)
+def test_few_rows_have_the_cotangents_f32_bits(c):
+    """Gradients of at most 64 rows in 16-bit storage: the bounds of f32 storage,
+    what two 16-bit parts leave of a cotangent (half a step of half a step; in
+    f16 a part's own range ends 2^-38 below the largest), and the rounding of
+    the outputs.  As a whole they are as far off as that rounding alone."""
+    dt, rows, d, vocab, tied, top, t = c
+    k = Case(dt, rows, vocab, d=d, tied=tied, top=top, t=t, seed=rows + vocab, pad=rows > 2, ct=True)
+    k.dtype = "f32"
+    r, e = k.exact()
+    k.dtype = dt
+    x, w = k.x.double(), (k.w.t() if tied else k.w).double().contiguous()
+    at = k.index.reshape(rows, -1)
+    p = torch.softmax((k.teacher.double() / t).masked_fill(at < 0, -torch.inf), -1).nan_to_num(0.0) if top else (at >= 0).double()
+    coef = torch.where((at >= 0).any(-1), k.ct.double() * t, 0.0)[:, None]
+    g = (torch.softmax(x @ w / t, -1).scatter_add(1, at.clamp_min(0), -p) * coef).abs()
+    left = HALF[dt] ** 2 * g + (2.0 ** -38 * coef.amax() if dt == "f16" else 0.0)
+    more = {"dx": left @ w.t().abs().contiguous(), "dw": x.t().abs().contiguous() @ left}
+    if tied:
+        more["dw"] = more["dw"].t()
+    lse = k.run("value")["lse"]
+    for got in (k.run("step"), k.run("vjp", lse=lse), k.run("step", dw=False), k.run("step", dx=False)):
+        for m in {"dx", "dw"} & set(got):
+            y, ey = r[m], e[m] + more[m]
+            off = (got[m].double() - y).abs()
+            bound = ey + HALF[dt] * (y.abs() + ey) + TINY[dt]
+            assert bool((off <= bound).all()), (m, float((off / bound).max()))
+            rounded = float((y.to(T[dt]).double() - y).norm())
+            assert float(off.norm()) <= 1.1 * rounded, (m, float(off.norm()) / rounded)
