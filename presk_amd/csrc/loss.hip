@@ -12,7 +12,7 @@
 // logits; for the gradient one goes over it a piece at a time, the cotangent of
 // a piece (kEpiP) entering dx, whose sum over the pieces stays in f32, and the
 // piece's part of dw.  Together that is four products.  8192 x 4096 x 32000 in
-// bf16, loss and gradients: 5.45 ms with the logits kept, 7.06 computed twice.
+// bf16, loss and gradients: 5.7 ms with the logits kept, 7.4 in two calls.
 // The workspace of pieces: a piece's cotangent, 128 MiB or, of many rows, that of
 // 256 columns; 12 bytes a row and column tile (256 columns, of few rows 128) of
 // the whole vocabulary for the value's row sums; and with more than four slots a
@@ -44,12 +44,11 @@ constexpr long long kKeepBytes = 4ll << 30;     // ... and where the gradient fo
 constexpr int kPieceCols = 256;                 // a piece is a multiple of these
 // 16-bit storage: up to so many rows the cotangent enters dx and dw in two 16-bit
 // parts, its rounding and what that left; past them its rounding alone, whose
-// errors average over the rows (the gradients' whole error against the outputs'
-// rounding alone: 1.34 to 1.46 times it over 200 sizes of more rows; of fewer up
-// to 2.1, 43 of 382 gradients over 1.5; in two parts 1.00).  The second part is
-// half as many products again or more: 8 x 4096 x 32000 in bf16, both gradients,
-// 205 us in one part and 259 in two; 65 rows 226 and 287; 8192 rows 5.33 and 8.57
-// ms.
+// errors average (the gradients' whole error against that of f32 cotangents, whose
+// outputs are rounded: 1.3 to 1.48 times it over 200 sizes of more rows; of fewer
+// up to 2.1, 43 of 382 gradients over 1.5; in two parts 1.00).  The second part
+// doubles two products: 8 x 4096 x 32000 in bf16, both gradients, 205 us in one
+// part and 259 in two; 65 rows 226 and 287; 8192 rows 5.33 and 8.57 ms.
 constexpr int kFineRows = 64;
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }

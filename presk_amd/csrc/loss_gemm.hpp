@@ -13,11 +13,13 @@
 // A^T), so that a lane holds one row's columns, four consecutive ones at a
 // time: a row's maximum and sum are lane sums and one exchange between
 // half-waves.
-// Bound by the matrix cores, busy 61 % of the cycles with no LDS conflict, at
-// the clock their power leaves: 8192 x 4096 x 32000 in bf16, kEpiStats 1670 us
-// (1286 TFLOP/s), kEpiP 452 a quarter of it (1188), kEpiZ with its 1.05 GB
-// 1802 (1192), dx and dw 3421 (1255); the library's plain product of that size
-// 1233 TFLOP/s.
+// Bound by the matrix cores at the clock their power leaves, 7 % apart from card
+// to card.  4096 x 32000 in bf16: kEpiStats of 2048 rows 430 to 480 us (1250 to
+// 1120 TFLOP/s), the matrix cores busy 58 % of the cycles with no LDS conflict;
+// of 8192 rows kEpiZ with its 1.05 GB 1.80 to 2.03 ms (1190 to 1060), busy 66 %
+// with 2 % of the LDS cycles conflicts, dx and dw 3.42 to 3.89 (1255 to 1105),
+// 69 % with 0.6 %; the library's plain product of that size 1233 to 1257
+// TFLOP/s.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -382,7 +382,7 @@ __device__ __forceinline__ void row_stats(const LossMatrix& a, long long r, int 
 
 // G 16, 64: 16 or four rows a workgroup; 256: a row's chunk a workgroup.  Bound
 // by the logits' bytes, for few rows by its launch (64 x 50257 in f32, 12.9 MB
-// out of the Infinity Cache, 4.9 us; 256 x 65 4.4).
+// out of the Infinity Cache, 5.2 us; 256 x 65 4.9).
 template <int ST, int G>
 __global__ void __launch_bounds__(256) stats_kernel(LossMatrix a, float* pm, float* ps, float* pa, int slot0, int chunk,
                                                     LossDone done, bool finish) {
