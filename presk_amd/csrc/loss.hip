@@ -47,8 +47,8 @@ constexpr int kPieceCols = 256;                 // a piece is a multiple of thes
 // errors average (the gradients' whole error against that of f32 cotangents, whose
 // outputs are rounded: 1.3 to 1.48 times it over 200 sizes of more rows; of fewer
 // up to 2.1, 43 of 382 gradients over 1.5; in two parts 1.00).  The second part
-// doubles two products: 8 x 4096 x 32000 in bf16, both gradients, 205 us in one
-// part and 259 in two; 65 rows 226 and 287; 8192 rows 5.33 and 8.57 ms.
+// doubles two products: 8 x 4096 x 32000 in bf16, value and gradients, 205 us in
+// one part and 245 in two; 65 rows 226 and 287; 8192 rows 5.33 and 8.57 ms.
 constexpr int kFineRows = 64;
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
@@ -79,7 +79,8 @@ Shape shape_of(long long M, long long N) {
 // every item (4096 x 512 x 2048 76.8 -> 69.2 us; 512 x 2048 x 8192, 1100 items,
 // 98 us, deep 104); two a CU are kept to one round where fewer cuts do that
 // (777 x 500 x 10007, 316 tiles of dw and 28 of dx cut 7 ways, 512 items and
-// the mean, 105 us, 6 ways 89).
+// the mean, 105 us, 6 ways 89).  The few rows of a cotangent in two parts take no
+// 256-row tiles (8 x 4096 x 32000, value and gradients, 264 -> 245 us).
 constexpr int kBeside = 8;      // workgroups of the launch that are no item: the mean's, and dx's padding to 8
 void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long Nw, long long Kw, Shape* x, Shape* w) {
     const long long kx = up(Kx, 64) / 64, kw = up(Kw, 64) / 64;
@@ -101,7 +102,7 @@ void pair_of(long long Mx, long long Nx, long long Kx, long long Mw, long long N
         }
         return tiles_of(*x) + tiles_of(*w);
     };
-    if (both(256, 256) >= 192) return;
+    if ((Mx == 0 || Mx > kFineRows) && both(256, 256) >= 192) return;
     both(kDeep128, 256);
     if (items() <= 256 - kBeside) return;
     both(128, 512);
