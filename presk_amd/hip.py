@@ -415,7 +415,7 @@ class Distill:
         self.tied, self.temperature = bool(tied), float(temperature)
         self._sizes = (self.dtype, self.rows, self.model, self.vocab, self.top, self.tied, self.temperature)
         self._work = None       # the workspace last used of the object's own
-        self._works = {}        # stream -> those taken for it, the largest last
+        self._works = {}        # device and stream -> those taken for it, the largest last
         self._specs, self._fixed = _loss_layout(self._sizes)
 
     def workspace(self, kind: str, dx: bool = True, dw: bool = True) -> int:
@@ -427,8 +427,8 @@ class Distill:
     def _outgrown(self) -> list:
         return [b for own in self._works.values() for b in own if b is not self._work]
 
-    def _own_work(self, need: int, stream):
-        own = self._works.setdefault(getattr(stream, "value", stream) or 0, [])
+    def _own_work(self, need: int, device, stream):
+        own = self._works.setdefault((device, getattr(stream, "value", stream) or 0), [])
         if not own or own[-1].nbytes < need:
             own.append(DeviceBuffer(need))
         self._work = own[-1]
@@ -441,7 +441,7 @@ class Distill:
         device = _initialized if device is None else device
         need = self.workspace(kind, dx is not None, dw is not None)
         if work is None:
-            work = self._own_work(need, stream)
+            work = self._own_work(need, device, stream)
         bufs = [None if b is None else _buffer(s[0], b, device, *s[1:])
                 for s, b in zip(self._specs, (x, w, index, teacher, loss, lse, mean, ct, dx, dw, flag))]
         return LossArgs(*self._fixed, *bufs, _buffer("work", work, device, need), work.nbytes)

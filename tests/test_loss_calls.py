@@ -14,6 +14,8 @@ CURRENT = 0x5000
 class Tensor(torch.Tensor):
     """A tensor that says it is in device memory."""
 
+    at = 0
+
     @staticmethod
     def of(t):
         return t.as_subclass(Tensor)
@@ -21,7 +23,7 @@ class Tensor(torch.Tensor):
     is_cuda = True
 
     def get_device(self):
-        return 0
+        return Tensor.at
 
 
 class Library:
@@ -83,8 +85,8 @@ def test_the_own_workspace_is_a_streams(calls):
         op.value(Memory(1024), Memory(64), Memory(32), loss=Memory(16), stream=s)
     w = [a for a, _ in calls]
     assert w[0] == w[2] != w[1] == w[5] and w[3] == w[4] not in (w[0], w[1])
-    small = op._works[0x10][0]
-    op._works[0x10][0].nbytes = 16
+    small, = (b for own in op._works.values() for b in own if b.ptr == w[0])
+    small.nbytes = 16
     op.value(Memory(1024), Memory(64), Memory(32), loss=Memory(16), stream=0x10)
     assert calls[-1][0] not in w and small in op._outgrown and op._work not in op._outgrown
 
@@ -102,3 +104,15 @@ def test_tensors_of_another_device_than_the_current_one_are_refused(calls, monke
         monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
         op.value(**inputs())
     assert len(calls) == 3
+
+
+def test_the_own_workspace_is_a_devices(calls, monkeypatch):
+    """The null streams of two devices are two."""
+    op = hip.Distill("f32", 4, 64, 2)
+    monkeypatch.setattr(hip, "_initialized", None)
+    for at in (0, 1, 0):
+        monkeypatch.setattr(Tensor, "at", at)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: at)
+        op.value(**inputs(), stream=0)
+    w = [a for a, _ in calls]
+    assert w[0] == w[2] != w[1]
