@@ -315,6 +315,122 @@ int presk_hip_distill(const presk_hip_loss* a, int what, void* stream);
 int presk_hip_batch_add_head_loss(presk_hip_batch* b, const presk_hip_loss* a, int what);
 int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int what);
 
+/* Attention of grouped heads without its weights in memory, and its gradients; no
+ * counterpart among the reference's nests, where it is `ein`, `div`, `softmax` and
+ * `ein` over weights in memory (crates/presk-kernel/src/lower.rs:250-303).
+ *
+ * Of queries q [batch, q_len, heads, head_dim] and keys and values k, v [batch,
+ * k_len, kv_heads, head_dim], head h reading key head h / (heads / kv_heads):
+ *   s[i, j] = scale * (q[i] . k[j]) over the keys that query i may read
+ *   lse[i]  = log sum_j exp(s[i, j])              (-inf where it reads none)
+ *   o[i]    = sum_j exp(s[i, j] - lse[i]) v[j]    (0 where it reads none)
+ * and, of o's cotangent dout, with p = exp(s - lse):
+ *   dv[j] = sum_i p[i, j] dout[i],  ds[i, j] = p[i, j] (dout[i] . v[j] - dout[i] . o[i])
+ *   dq[i] = scale sum_j ds[i, j] k[j],  dk[j] = scale sum_i ds[i, j] q[i]
+ * dk and dv summed over the heads of their group as well.
+ * Query i of sequence b stands at position first[b] + i among the keys.  It may
+ * read key j below lens[b] (null: k_len; taken into [0, k_len]) where
+ *   causal:         j <= first[b] + i, and with a window also j > first[b] + i - window;
+ *   mask_cols > 0:  j < first[b], or mask[b, i, j - first[b]] is not 0, whose
+ *                   columns end at mask_cols (a tree of drafted tokens over a
+ *                   cache; a mask of all keys has first 0 and k_len columns);
+ *   neither:        always.
+ * `first` null: k_len - q_len (the queries are the last keys), of a mask k_len -
+ * mask_cols.  A key at or past lens[b] is not read, whatever it holds, and its
+ * rows of dk and dv are 0; one that only some queries read enters the others
+ * times 0, so it must be finite.
+ * A tensor's element (b, i, h, d) is at p + b * batch + i * seq + h * head + d,
+ * strides in elements and not negative, those of an input over batch or heads 0
+ * where it is shared.  Rows of whole 16-byte vectors (address, strides and
+ * head_dim) are loaded as such, others element by element.
+ * Products accumulate in f32, and so do the sums of a softmax; in 16-bit storage
+ * the weights p and their cotangents ds are rounded to the storage type before
+ * the products they enter.
+ *
+ * `what`: PRESK_HIP_ATTN_VALUE writes o and, where it is not null, lse (f32 [batch,
+ * heads, q_len]).  PRESK_HIP_ATTN_GRAD writes those of dq, dk and dv whose p is
+ * not null from the forward's o and lse.  f16 outputs that overflow set bit 0 of
+ * *flag (if flag is not null).
+ * `work`: device memory of presk_hip_attention_workspace bytes (from the sizes
+ * alone), 16-byte aligned, this call's until it has run; nothing in it is kept
+ * between calls.  An output may not meet another buffer (tensors whose rows lie
+ * between each other's do not).  Nothing is allocated, and only kernels are
+ * launched, so the calls may be captured; lens, first and mask are read then.
+ * Storage types f32 (head_dim to 128), bf16 and f16 (to 256), others are E7005;
+ * q_len, k_len, mask_cols and window below 2^28; a row's stride (seq) at least
+ * head_dim elements and below 2^25 bytes. */
+typedef struct {
+    void* p;
+    int64_t batch, seq, head;
+} presk_hip_heads;
+
+typedef struct {
+    const char* dtype;
+    int64_t batch, heads, kv_heads, q_len, k_len, head_dim, window, mask_cols;
+    int32_t causal;
+    double scale;
+    presk_hip_heads q, k, v, o, dout, dq, dk, dv;
+    float* lse;
+    const int64_t* lens;
+    const int64_t* first;
+    const uint8_t* mask;
+    int64_t mask_batch, mask_row;
+    uint32_t* flag;
+    void* work;
+    size_t work_bytes;
+} presk_hip_attn;
+
+#define PRESK_HIP_ATTN_VALUE 1
+#define PRESK_HIP_ATTN_GRAD 2
+
+int presk_hip_attention_workspace(const presk_hip_attn* a, int what, size_t* bytes);
+int presk_hip_attention(const presk_hip_attn* a, int what, void* stream);
+/* As a step of a recorded sequence: the arguments are copied, the buffers (the
+ * workspace among them) must outlive the batch. */
+int presk_hip_batch_add_attention(presk_hip_batch* b, const presk_hip_attn* a, int what);
+
+/* The norm of each head of the queries and keys and their rotation by position in
+ * one pass, and its gradients; among the reference's nests the rotation is `slice`,
+ * `cos`, `sin`, products and `concat` (examples/coverage/llama.psk:36-48).
+ *
+ * Of a head's x (q [batch, seq, heads, head_dim] and k [.., kv_heads, ..]; kv_heads 0:
+ * q alone), with `norm`:  u = g * x / sqrt(mean(x^2) + eps), gains gq for every head
+ * of q and gk for those of k ([head_dim], null: ones); without it u = x.  Of the first
+ * `rotary` elements of u, pair r turns by at[b, i] * freq[r] (f64 radians, freq
+ * [rotary / 2], at i64 [batch, seq], null: i):
+ *   y0 = u0 cos - u1 sin,  y1 = u1 cos + u0 sin
+ * pair r being elements r and r + rotary / 2, or with `even` 2 r and 2 r + 1.  The
+ * others of y are those of u.
+ * PRESK_HIP_ROT_VALUE writes yq and yk (which may be q and k themselves);
+ * PRESK_HIP_ROT_GRAD, from their cotangents dyq and dyk and, with `norm`, q and k,
+ * writes dq and dk (which may be dyq and dyk) and those of dgq and dgk ([head_dim])
+ * that are not null.  Sums in f32, angles in f64 (so that one of 2^30
+ * radians is right to 2^-23); tensors, f16's flag, `work` (null and 0 bytes do but for a gradient with
+ * `norm`), streams and graphs as presk_hip_attention's. */
+typedef struct {
+    const char* dtype;
+    int64_t batch, seq, heads, kv_heads, head_dim, rotary;
+    int32_t norm, even;
+    double eps;
+    presk_hip_heads q, k, yq, yk, dyq, dyk, dq, dk;
+    const double* freq;
+    const int64_t* at;
+    const void* gq;
+    const void* gk;
+    void* dgq;
+    void* dgk;
+    uint32_t* flag;
+    void* work;
+    size_t work_bytes;
+} presk_hip_rot;
+
+#define PRESK_HIP_ROT_VALUE 1
+#define PRESK_HIP_ROT_GRAD 2
+
+int presk_hip_head_rotary_workspace(const presk_hip_rot* a, int what, size_t* bytes);
+int presk_hip_head_rotary(const presk_hip_rot* a, int what, void* stream);
+int presk_hip_batch_add_head_rotary(presk_hip_batch* b, const presk_hip_rot* a, int what);
+
 /* Seeded synthetic values written in place: n elements mean + std * z of
  * type "f32", "bf16" or "f16", z ~ N(0, 1) a function of (seed, element
  * index) alone (a splitmix64 hash and Box-Muller in f32).  Stands in for the

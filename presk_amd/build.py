@@ -19,7 +19,8 @@ OUT = os.path.join(PKG, "libpresk_hip.so")
 BUILD = os.path.join(PKG, "_build")
 
 SOURCES = ["ir.cpp", "hipgen.cpp", "presk_hip.cpp", "selftest.hip", "classes.hip", "gemm.hip", "gemm_split.hip", "gemm_ragged.hip", "gemm_quant.hip", "gemm_seq.hip", "reduce.hip", "rows.hip", "wrows.hip", "scatter.hip", "convert.hip", "synth.hip", "probe.hip",
-           "loss.hip", "loss_rows.hip", "loss_gemm_bf16.hip", "loss_gemm_f16.hip"]
+           "loss.hip", "loss_rows.hip", "loss_gemm_bf16.hip", "loss_gemm_f16.hip",
+           "attn.hip", "attn_f32.hip", "attn_bf16.hip", "attn_f16.hip", "rotary.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # f32 semantics the parity rests on: no contraction into FMA, IEEE denormals,

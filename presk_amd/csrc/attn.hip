@@ -1,0 +1,248 @@
+// Attention: what a call checks, its workspace and its launches (attn.hpp).
+#include "attn.hpp"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "heads.hpp"
+
+namespace presk {
+
+namespace {
+
+int storage_code(const char* name) {
+    const std::string t = name ? name : "";
+    return t == "f32" ? kF32 : t == "bf16" ? kBF16 : t == "f16" ? kF16 : -1;
+}
+
+long long up(long long n, long long to) { return (n + to - 1) / to * to; }
+
+// A row's bits and a column's, 32 of a byte mask a thread.
+__global__ void __launch_bounds__(256) attn_mask_kernel(AttnMask m) {
+    const long long n = (long long)m.nbatch * m.tq * m.words, t = (long long)m.nbatch * m.cols * m.words_t;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at < n) {
+        const int w = (int)(at % m.words);
+        const long long line = at / m.words, b = line / m.tq, i = line - b * m.tq;
+        const unsigned char* const src = m.mask + b * m.batch + i * m.row + 32LL * w;
+        const int left = m.cols - 32 * w < 32 ? m.cols - 32 * w : 32;
+        unsigned bits = 0;
+        if (left == 32 && ((uintptr_t)src & 3) == 0) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const unsigned v = ((const unsigned*)src)[q];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bits |= (v >> (8 * e) & 0xff ? 1u : 0u) << (4 * q + e);
+            }
+        } else {
+            for (int e = 0; e < left; ++e) bits |= (src[e] ? 1u : 0u) << e;
+        }
+        m.bits[at] = bits;
+    } else if (m.bits_t && at - n < t) {
+        // columns innermost, so that a wave reads a row's bytes beside each other
+        const long long k = at - n;
+        const int c = (int)(k % m.cols);
+        const long long line = k / m.cols, b = line / m.words_t;
+        const int w = (int)(line - b * m.words_t);
+        const unsigned char* const src = m.mask + b * m.batch + 32LL * w * m.row + c;
+        const int left = m.tq - 32 * w < 32 ? m.tq - 32 * w : 32;
+        unsigned bits = 0;
+        for (int e = 0; e < left; ++e) bits |= (src[e * m.row] ? 1u : 0u) << e;
+        m.bits_t[(b * m.cols + c) * m.words_t + w] = bits;
+    }
+}
+
+// What a checked call launches.
+struct Plan {
+    int st, nd, pack = 1, splits = 1;
+    int words = 0, words_t = 0, nbits = 0;
+    size_t bits = 0, bits_t = 0, part = 0, ml = 0, rows = 0, total = 0;     // offsets in the workspace
+};
+
+// Splits of the keys: as many shares as fill two workgroups a CU, of two tiles
+// at least.
+int splits_of(long long items, long long tk) {
+    if (items <= 0 || items >= 256) return 1;
+    return (int)std::max<long long>(1, std::min<long long>({512 / items, tk / 128, 64}));
+}
+
+Plan plan_of(const presk_hip_attn& a, int what) {
+    Plan p;
+    p.st = storage_code(a.dtype);
+    p.nd = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+    const long long all = a.batch * a.heads * a.q_len;
+    auto take = [&](long long bytes) {
+        const size_t at = p.total;
+        p.total += (size_t)up(bytes, 256);
+        return at;
+    };
+    const bool grad = what == PRESK_HIP_ATTN_GRAD;
+    if (a.mask_cols) {
+        // (a mask that the sequences share is taken as theirs: the workspace is
+        // one of the sizes alone)
+        p.words = (int)up(a.mask_cols, 32) / 32;
+        p.words_t = (int)up(a.q_len, 32) / 32;
+        p.bits = take(4 * a.batch * a.q_len * p.words);
+        if (grad) p.bits_t = take(4 * a.batch * a.mask_cols * p.words_t);
+    }
+    if (grad) {
+        p.rows = take(8 * all);
+        return p;
+    }
+    const long long per = a.heads / a.kv_heads;
+    if (a.q_len < kAttnTile) p.pack = (int)per;
+    const long long items = up(a.q_len * p.pack, kAttnTile) / kAttnTile * a.batch * (a.heads / p.pack);
+    p.splits = splits_of(items, a.k_len);
+    if (p.splits > 1) {
+        p.part = take(4 * all * p.splits * p.nd * 32);
+        p.ml = take(8 * all * p.splits);
+    }
+    return p;
+}
+
+size_t bytes_of(const Plan& p) { return std::max<size_t>(p.total, 256); }
+
+std::vector<HeadsBuffer> tensors(const presk_hip_attn& a, bool grad) {
+    const auto q = [&](const char* n, const presk_hip_heads& t, bool out, bool need) {
+        return HeadsBuffer{n, &t, a.batch, a.q_len, a.heads, a.head_dim, out, need};
+    };
+    const auto k = [&](const char* n, const presk_hip_heads& t, bool out, bool need) {
+        return HeadsBuffer{n, &t, a.batch, a.k_len, a.kv_heads, a.head_dim, out, need};
+    };
+    std::vector<HeadsBuffer> v{q("q", a.q, false, true), k("k", a.k, false, true), k("v", a.v, false, true), q("o", a.o, !grad, true)};
+    if (grad) {
+        v.push_back(q("dout", a.dout, false, true));
+        v.push_back(q("dq", a.dq, true, false));
+        v.push_back(k("dk", a.dk, true, false));
+        v.push_back(k("dv", a.dv, true, false));
+    }
+    return v;
+}
+
+std::vector<PlainBuffer> others(const presk_hip_attn& a, bool grad, int64_t work) {
+    const int64_t mask = a.mask_cols && a.q_len && a.batch ? (a.batch - 1) * a.mask_batch + (a.q_len - 1) * a.mask_row + a.mask_cols : 0;
+    return {{"lse", a.lse, 4 * a.batch * a.heads * a.q_len, 4, !grad, grad},
+            {"lens", a.lens, 8 * a.batch, 8, false, false},
+            {"first", a.first, 8 * a.batch, 8, false, false},
+            {"mask", a.mask, mask, 1, false, true},
+            {"flag", a.flag, 4, 4, true, false},
+            {"work", a.work, work, 16, true, true}};
+}
+
+}  // namespace
+
+std::string attn_check(const presk_hip_attn& a, int what) {
+    auto no = [&](const std::string& why) { return std::string("E10001: attention: ") + why; };
+    auto size = [&](const char* n, int64_t v) { return no(std::string(n) + " " + std::to_string(v)); };
+    const int st = storage_code(a.dtype);
+    if (st < 0) return std::string("E7005: attention in storage type `") + (a.dtype ? a.dtype : "") + "` (f32, bf16 or f16)";
+    if (what != PRESK_HIP_ATTN_VALUE && what != PRESK_HIP_ATTN_GRAD) return no("what is neither VALUE nor GRAD");
+    constexpr int64_t kMany = 1ll << 28;
+    if (a.batch < 0 || a.batch >= 1 << 24) return size("batch", a.batch);
+    if (a.heads < 1 || a.heads >= 1 << 16) return size("heads", a.heads);
+    if (a.kv_heads < 1 || a.heads % a.kv_heads) return no("heads " + std::to_string(a.heads) + " are not whole groups of kv_heads " + std::to_string(a.kv_heads));
+    if (a.q_len < 0 || a.q_len >= kMany) return size("q_len", a.q_len);
+    if (a.k_len < 0 || a.k_len >= kMany) return size("k_len", a.k_len);
+    if (a.head_dim < 1 || a.head_dim > 256) return size("head_dim", a.head_dim);
+    if (st == kF32 && a.head_dim > 128) return "E7005: attention: head_dim " + std::to_string(a.head_dim) + " in f32 (to 128)";
+    if (a.window < 0 || a.window >= kMany) return size("window", a.window);
+    if (a.window && !a.causal) return no("a window without causal");
+    if (a.mask_cols < 0 || a.mask_cols >= kMany) return size("mask_cols", a.mask_cols);
+    if (a.mask_cols && a.causal) return no("a mask and causal");
+    if (!(a.scale >= 1e-20 && a.scale <= 1e20)) return no("a scale of " + std::to_string(a.scale) + ", not in [1e-20, 1e20]");
+    // workgroups of a launch
+    const int64_t most = std::max(a.heads * (up(a.q_len, 16) / 16), a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile));
+    if (a.batch * most >= 1ll << 31) return no("batch * heads * length past what a launch holds");
+    if (a.mask_cols && a.batch * std::max(a.q_len * (up(a.mask_cols, 32) / 32), a.mask_cols * (up(a.q_len, 32) / 32)) >= 1ll << 38)
+        return no("a mask past what a launch holds");
+    return "";
+}
+
+std::string attn_check_all(const presk_hip_attn& a, int what) {
+    auto no = [&](const std::string& why) { return std::string("E10001: attention: ") + why; };
+    if (std::string why = attn_check(a, what); !why.empty()) return why;
+    const bool grad = what == PRESK_HIP_ATTN_GRAD;
+    const int esz = storage_code(a.dtype) == kF32 ? 4 : 2;
+    if (a.mask_cols) {
+        if (a.mask_batch < 0 || a.mask_batch > 1ll << 40 || a.mask_row < 0 || a.mask_row > 1ll << 40) return no("a mask with a negative stride");
+    }
+    if (grad && !a.dq.p && !a.dk.p && !a.dv.p && a.batch * (a.q_len + a.k_len) > 0) return no("a gradient without an output");
+    if (std::string why = buffers_check(tensors(a, grad), others(a, grad, (int64_t)a.work_bytes), esz); !why.empty()) return no(why);
+    const size_t need = bytes_of(plan_of(a, what));
+    if (a.work_bytes < need) return no("a workspace of " + std::to_string(a.work_bytes) + " bytes, " + std::to_string(need) + " needed");
+    return "";
+}
+
+size_t attn_workspace(const presk_hip_attn& a, int what) { return bytes_of(plan_of(a, what)); }
+
+void attn_spans(const presk_hip_attn& a, int what, std::vector<Span>* rd, std::vector<Span>* wr) {
+    const bool grad = what == PRESK_HIP_ATTN_GRAD;
+    buffers_spans(tensors(a, grad), others(a, grad, (int64_t)a.work_bytes), storage_code(a.dtype) == kF32 ? 4 : 2, rd, wr);
+}
+
+hipError_t attn_run(const presk_hip_attn& a, int what, hipStream_t s) {
+    const Plan p = plan_of(a, what);
+    const int esz = p.st == kF32 ? 4 : 2;
+    char* const work = (char*)a.work;
+    auto tensor = [&](const presk_hip_heads& t, int64_t seq, int64_t heads) {
+        auto whole = [&](int64_t n, int64_t stride) { return n < 2 || stride * esz % 16 == 0; };
+        const bool vec = (uintptr_t)t.p % 16 == 0 && a.head_dim * esz % 16 == 0 && whole(a.batch, t.batch) && whole(seq, t.seq) && whole(heads, t.head);
+        return AttnTensor{t.p, t.batch, t.seq, t.head, vec};
+    };
+    auto queries = [&](const presk_hip_heads& t) { return tensor(t, a.q_len, a.heads); };
+    auto keys = [&](const presk_hip_heads& t) { return tensor(t, a.k_len, a.kv_heads); };
+    AttnArgs g{};
+    g.q = queries(a.q);
+    g.k = keys(a.k);
+    g.v = keys(a.v);
+    g.o = queries(a.o);
+    g.dout = queries(a.dout);
+    g.dq = queries(a.dq);
+    g.dk = keys(a.dk);
+    g.dv = keys(a.dv);
+    g.lse = a.lse;
+    g.lens = (const long long*)a.lens;
+    g.first = (const long long*)a.first;
+    g.first0 = a.k_len - (a.mask_cols ? a.mask_cols : a.q_len);
+    g.batch = (int)a.batch;
+    g.heads = (int)a.heads;
+    g.kv = (int)a.kv_heads;
+    g.per = (int)(a.heads / a.kv_heads);
+    g.tq = (int)a.q_len;
+    g.tk = (int)a.k_len;
+    g.d = (int)a.head_dim;
+    g.causal = a.causal != 0;
+    g.window = (int)a.window;
+    g.cols = (int)a.mask_cols;
+    g.c = (float)(a.scale * 1.4426950408889634);
+    g.scale = (float)a.scale;
+    g.flag = a.flag;
+    g.pack = p.pack;
+    g.splits = p.splits;
+    g.part = (float*)(work + p.part);
+    g.part_ml = (float*)(work + p.ml);
+    g.rows = (float*)(work + p.rows);
+    if (a.mask_cols && a.batch && a.q_len) {
+        const bool grad = what == PRESK_HIP_ATTN_GRAD;
+        const int nb = a.mask_batch || a.batch == 1 ? (int)a.batch : 1;
+        AttnMask m{a.mask, a.mask_batch, a.mask_row, nb, g.tq, g.cols, p.words, p.words_t, (unsigned*)(work + p.bits),
+                   grad ? (unsigned*)(work + p.bits_t) : nullptr};
+        const long long n = (long long)nb * g.tq * m.words + (grad ? (long long)nb * g.cols * m.words_t : 0);
+        attn_mask_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(m);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        g.bits = m.bits;
+        g.bits_t = m.bits_t;
+        g.words = m.words;
+        g.words_t = m.words_t;
+        g.bits_batch = nb > 1 ? g.tq : 0;
+        g.bits_t_batch = nb > 1 ? g.cols : 0;
+    }
+    if (what == PRESK_HIP_ATTN_GRAD)
+        return p.st == kF32 ? attn_bwd_f32(g, p.nd, s) : p.st == kBF16 ? attn_bwd_bf16(g, p.nd, s) : attn_bwd_f16(g, p.nd, s);
+    return p.st == kF32 ? attn_fwd_f32(g, p.nd, s) : p.st == kBF16 ? attn_fwd_bf16(g, p.nd, s) : attn_fwd_f16(g, p.nd, s);
+}
+
+}  // namespace presk

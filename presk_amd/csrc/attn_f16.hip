@@ -1,0 +1,9 @@
+// Attention in f16 (attn_dev.hpp).
+#include "attn_dev.hpp"
+
+namespace presk {
+
+hipError_t attn_fwd_f16(const AttnArgs& a, int nd, hipStream_t s) { return fwd_nd<kF16>(a, nd, s); }
+hipError_t attn_bwd_f16(const AttnArgs& a, int nd, hipStream_t s) { return bwd_nd<kF16>(a, nd, s); }
+
+}  // namespace presk

@@ -18,10 +18,12 @@
 #include <sstream>
 #include <unordered_map>
 
+#include "attn.hpp"
 #include "branches.hpp"
 #include "convert.hpp"
 #include "loss.hpp"
 #include "probe.hpp"
+#include "rotary.hpp"
 #include "synth.hpp"
 #include "executor.hpp"
 
@@ -518,7 +520,8 @@ int presk_hip_time(const presk_hip_kernel* h, void* const* bufs, int64_t lo, int
 struct presk_hip_batch {
     // a kernel launch, or (k null) an edge conversion, or (k null, rate >= 0)
     // a dropout mask: bufs {key, dst}, type in `to`, or (k null, what > 0) a
-    // loss over its own arguments
+    // loss over its own arguments, or (k null, call set) another operator, with
+    // the spans it reads and writes
     struct Item {
         const presk_hip_kernel* k;
         std::vector<void*> bufs;
@@ -529,6 +532,9 @@ struct presk_hip_batch {
         presk_hip_loss loss{};
         int what = 0;
         bool head = false;
+        std::function<hipError_t(hipStream_t)> call;
+        const char* call_name = nullptr;
+        std::vector<Span> rd, wr;
     };
     std::vector<Item> items;
     hipGraph_t graph = nullptr;
@@ -567,6 +573,10 @@ struct presk_hip_batch {
         if (it.what) {
             hipError_t e = loss_run(it.loss, it.what, it.head, s);
             return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, it.head ? "head loss" : "distillation");
+        }
+        if (it.call) {
+            hipError_t e = it.call(s);
+            return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, it.call_name);
         }
         if (!it.k && it.rate >= 0.0) {
             hipError_t e = dropout_launch(it.bufs[0], it.rate, it.to, it.n, it.bufs[1], s);
@@ -761,6 +771,7 @@ std::vector<BranchStep> branch_steps(const presk_hip_batch& b) {
         st.n = it.n;
         st.rate = it.rate;
         if (it.what) loss_spans(it.loss, it.what, it.head, &st.rd, &st.wr);
+        if (it.call) st.rd = it.rd, st.wr = it.wr;
         out.push_back(std::move(st));
     }
     return out;
@@ -861,9 +872,67 @@ int add_loss(presk_hip_batch* b, const presk_hip_loss* a, int what, bool head) {
     return PRESK_HIP_OK;
 }
 
+const char* type_name(const std::string& type) { return type == "f32" ? "f32" : type == "bf16" ? "bf16" : "f16"; }
+
 }  // namespace
 
 extern "C" {
+
+int presk_hip_attention_workspace(const presk_hip_attn* a, int what, size_t* bytes) {
+    if (!a || !bytes) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = attn_check(*a, what); !why.empty()) return refuse_loss(why);
+    *bytes = attn_workspace(*a, what);
+    return PRESK_HIP_OK;
+}
+
+int presk_hip_attention(const presk_hip_attn* a, int what, void* stream) {
+    if (!a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = attn_check_all(*a, what); !why.empty()) return refuse_loss(why);
+    hipError_t e = attn_run(*a, what, (hipStream_t)stream);
+    return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, "attention");
+}
+
+int presk_hip_batch_add_attention(presk_hip_batch* b, const presk_hip_attn* a, int what) {
+    if (!b || !a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = attn_check_all(*a, what); !why.empty()) return refuse_loss(why);
+    b->drop_graph();
+    presk_hip_batch::Item it{nullptr, {}, 0, 0};
+    presk_hip_attn copy = *a;
+    copy.dtype = type_name(a->dtype);
+    it.call = [copy, what](hipStream_t s) { return attn_run(copy, what, s); };
+    it.call_name = "attention";
+    attn_spans(copy, what, &it.rd, &it.wr);
+    b->items.push_back(it);
+    return PRESK_HIP_OK;
+}
+
+int presk_hip_head_rotary_workspace(const presk_hip_rot* a, int what, size_t* bytes) {
+    if (!a || !bytes) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = rotary_check(*a, what); !why.empty()) return refuse_loss(why);
+    *bytes = rotary_workspace(*a, what);
+    return PRESK_HIP_OK;
+}
+
+int presk_hip_head_rotary(const presk_hip_rot* a, int what, void* stream) {
+    if (!a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = rotary_check_all(*a, what); !why.empty()) return refuse_loss(why);
+    hipError_t e = rotary_run(*a, what, (hipStream_t)stream);
+    return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, "head rotary");
+}
+
+int presk_hip_batch_add_head_rotary(presk_hip_batch* b, const presk_hip_rot* a, int what) {
+    if (!b || !a) return fail(PRESK_HIP_ERR, "E10001: null argument");
+    if (const std::string why = rotary_check_all(*a, what); !why.empty()) return refuse_loss(why);
+    b->drop_graph();
+    presk_hip_batch::Item it{nullptr, {}, 0, 0};
+    presk_hip_rot copy = *a;
+    copy.dtype = type_name(a->dtype);
+    it.call = [copy, what](hipStream_t s) { return rotary_run(copy, what, s); };
+    it.call_name = "head rotary";
+    rotary_spans(copy, what, &it.rd, &it.wr);
+    b->items.push_back(it);
+    return PRESK_HIP_OK;
+}
 
 int presk_hip_loss_workspace(const presk_hip_loss* a, int what, size_t* bytes) {
     if (!a || !bytes) return fail(PRESK_HIP_ERR, "E10001: null argument");

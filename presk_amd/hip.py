@@ -31,7 +31,9 @@ SYMBOLS = ["presk_hip_init", "presk_hip_last_error", "presk_hip_compile", "presk
            "presk_hip_batch_run", "presk_hip_batch_release", "presk_hip_convert", "presk_hip_batch_add_convert",
            "presk_hip_fill_normal", "presk_hip_dropout_mask", "presk_hip_batch_add_dropout",
            "presk_hip_pskd_decode", "presk_hip_pskd_decode_idx", "presk_hip_mfma_probe",
-           "presk_hip_loss_workspace", "presk_hip_head_loss", "presk_hip_distill", "presk_hip_batch_add_head_loss", "presk_hip_batch_add_distill"]
+           "presk_hip_loss_workspace", "presk_hip_head_loss", "presk_hip_distill", "presk_hip_batch_add_head_loss", "presk_hip_batch_add_distill",
+           "presk_hip_attention_workspace", "presk_hip_attention", "presk_hip_batch_add_attention",
+           "presk_hip_head_rotary_workspace", "presk_hip_head_rotary", "presk_hip_batch_add_head_rotary"]
 
 
 class HipError(RuntimeError):
@@ -56,6 +58,31 @@ class LossArgs(ctypes.Structure):
                 ("top", ctypes.c_int64), ("tied", ctypes.c_int32), ("temperature", ctypes.c_double)] + [
                     (n, ctypes.c_void_p) for n in ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag", "work")] + [
                         ("work_bytes", ctypes.c_size_t)]
+
+
+class Heads(ctypes.Structure):
+    """presk_hip_heads."""
+    _fields_ = [("p", ctypes.c_void_p), ("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class AttnArgs(ctypes.Structure):
+    """presk_hip_attn."""
+    _fields_ = [("dtype", ctypes.c_char_p)] + [
+        (n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_len", "k_len", "head_dim", "window", "mask_cols")] + [
+            ("causal", ctypes.c_int32), ("scale", ctypes.c_double)] + [
+                (n, Heads) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] + [
+                    (n, ctypes.c_void_p) for n in ("lse", "lens", "first", "mask")] + [
+                        ("mask_batch", ctypes.c_int64), ("mask_row", ctypes.c_int64), ("flag", ctypes.c_void_p), ("work", ctypes.c_void_p),
+                        ("work_bytes", ctypes.c_size_t)]
+
+
+class RotArgs(ctypes.Structure):
+    """presk_hip_rot."""
+    _fields_ = [("dtype", ctypes.c_char_p)] + [
+        (n, ctypes.c_int64) for n in ("batch", "seq", "heads", "kv_heads", "head_dim", "rotary")] + [
+            ("norm", ctypes.c_int32), ("even", ctypes.c_int32), ("eps", ctypes.c_double)] + [
+                (n, Heads) for n in ("q", "k", "yq", "yk", "dyq", "dyk", "dq", "dk")] + [
+                    (n, ctypes.c_void_p) for n in ("freq", "at", "gq", "gk", "dgq", "dgk", "flag", "work")] + [("work_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -110,6 +137,11 @@ def lib():
         L.presk_hip_distill.argtypes = [la, i32, vp]
         L.presk_hip_batch_add_head_loss.argtypes = [vp, la, i32]
         L.presk_hip_batch_add_distill.argtypes = [vp, la, i32]
+        for name, args in (("attention", AttnArgs), ("head_rotary", RotArgs)):
+            pa = ctypes.POINTER(args)
+            getattr(L, f"presk_hip_{name}_workspace").argtypes = [pa, i32, ctypes.POINTER(ctypes.c_size_t)]
+            getattr(L, f"presk_hip_{name}").argtypes = [pa, i32, vp]
+            getattr(L, f"presk_hip_batch_add_{name}").argtypes = [vp, pa, i32]
         _lib = L
     return _lib
 
@@ -342,7 +374,7 @@ def _loss_layout(sizes: tuple) -> tuple:
 
 # a torch dtype's name in the executor's terms, by the dtype object
 _TORCH_TYPES: dict = {}
-_TORCH_NAMES = {"torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
+_TORCH_NAMES = {"torch.float64": "f64", "torch.float32": "f32", "torch.bfloat16": "bf16", "torch.float16": "f16", "torch.int64": "i64"}
 
 
 def _buffer(name: str, b, device, nbytes: int, ty: str | None = None, row: int | None = None) -> int:
@@ -485,4 +517,243 @@ class HeadLoss(Distill):
     def value_and_grad(self, x, w, index, dx=None, dw=None, teacher=None, loss=None, lse=None, mean=None, ct=None, flag=None, work=None,
                        stream=None):
         self._call("step", stream, x=x, w=w, index=index, teacher=teacher, dx=dx, dw=dw, loss=loss, lse=lse, mean=mean, ct=ct, flag=flag,
+                   work=work)
+
+
+# ---- a block's attention ------------------------------------------------------------
+
+
+_HEAD_AXES = {"bshd": (0, 1, 2), "bhsd": (0, 2, 1)}    # where a layout has batch, seq and head
+_NOWHERE = Heads()
+
+
+class _HeadsCall:
+    """What the operators over tensors of heads share: their tensors' checks,
+    their workspace and their calls.  A tensor is a DeviceBuffer, dense in
+    `layout`, or a torch tensor of that layout's four axes with any strides whose
+    last is 1 (a slice of a packed projection, of a longer cache)."""
+
+    _name: str                  # of the library's calls
+    _kinds: dict                # what a call is -> its code
+    _tensors: dict              # a tensor's name -> whether it is a key's
+    _lengths: tuple             # of queries and keys
+
+    def _init(self, layout: str):
+        if layout not in _HEAD_AXES:
+            raise ValueError(f"a layout {layout!r}, not one of {', '.join(_HEAD_AXES)}")
+        self.layout = layout
+        self._works = {}        # device and stream -> the workspaces taken for it, the largest last
+        self._need = {}         # kind -> bytes of workspace
+        n = ctypes.c_size_t()
+        for kind, what in self._kinds.items():
+            check(getattr(lib(), f"presk_hip_{self._name}_workspace")(ctypes.byref(self._args()), what, ctypes.byref(n)))
+            self._need[kind] = n.value
+
+    def workspace(self, kind: str) -> int:
+        """Bytes of workspace for `value` or `vjp`."""
+        return self._need[kind]
+
+    def _shape(self, name: str) -> tuple:
+        """(batch, seq, heads, head_dim) of a tensor."""
+        k = self._tensors[name]
+        return (self.batch, self._lengths[k], self.kv_heads if k else self.heads, self.head_dim)
+
+    def elements(self, name: str) -> int:
+        b, s, h, d = self._shape(name)
+        return b * s * h * d
+
+    def _heads(self, name: str, t, device) -> Heads:
+        if t is None:
+            return _NOWHERE
+        shape = self._shape(name)
+        ab, as_, ah = _HEAD_AXES[self.layout]
+        if not hasattr(t, "data_ptr"):
+            need = self.elements(name) * STORAGE_BYTES[self.dtype]
+            if t.nbytes < need:
+                raise ValueError(f"{name} has {t.nbytes} bytes, {need} needed")
+            b, s, h, d = shape
+            return Heads(t.ptr, s * h * d, h * d if self.layout == "bshd" else d, d if self.layout == "bshd" else s * d)
+        at = _place(name, t, device)
+        have = _type_name(t)
+        if have != self.dtype:
+            raise ValueError(f"{name} is {have}, not {self.dtype}")
+        want = (shape[0], shape[1], shape[2], shape[3]) if self.layout == "bshd" else (shape[0], shape[2], shape[1], shape[3])
+        if tuple(t.shape) != want:
+            raise ValueError(f"{name} is {list(t.shape)}, not {list(want)}")
+        st = t.stride()
+        if st[3] != 1 and shape[3] > 1 and t.numel():
+            raise ValueError(f"{name}'s heads are not contiguous")
+        return Heads(at, st[ab], st[as_], st[ah])
+
+    def _own_work(self, need: int, device, stream):
+        own = self._works.setdefault((device, getattr(stream, "value", stream) or 0), [])
+        if not own or own[-1].nbytes < need:
+            own.append(DeviceBuffer(need))
+        return own[-1]
+
+    def args(self, kind: str, work=None, stream=None, device=None, **bufs):
+        """The arguments of a call on `stream`, each buffer checked against its
+        size and `device` (the one initialised)."""
+        device = _initialized if device is None else device
+        if work is None and self._works_for(kind):
+            work = self._own_work(self._need[kind], device, stream)
+        a = self._args()
+        for name, b in bufs.items():
+            if name in self._tensors:
+                setattr(a, "dout" if name == "do" else name, self._heads(name, b, device))
+            elif b is not None:
+                self._other(a, name, b, device)
+        if work is not None:
+            a.work, a.work_bytes = _buffer("work", work, device, self._need[kind]), work.nbytes
+        return a
+
+    def _works_for(self, kind: str) -> bool:
+        return True
+
+    def _call(self, kind, stream, **bufs):
+        device, stream = _place_of(bufs.values(), stream)
+        a = self.args(kind, stream=stream, device=device, **bufs)
+        check(getattr(lib(), "presk_hip_" + self._name)(ctypes.byref(a), self._kinds[kind], stream))
+
+
+def _place(name: str, t, device) -> int:
+    """The address of a tensor of another library, which is on `device`."""
+    at = t.get_device()
+    if at < 0:
+        raise ValueError(f"{name} is not in device memory")
+    if at != device and device not in (None, -1):
+        raise ValueError(f"{name} is on device {at}, not {device}")
+    return t.data_ptr()
+
+
+def _type_name(t) -> str:
+    have = _TORCH_TYPES.get(t.dtype)
+    if have is None:
+        have = _TORCH_TYPES[t.dtype] = _TORCH_NAMES.get(str(t.dtype), str(t.dtype))
+    return have
+
+
+class Attention(_HeadsCall):
+    """presk_hip_attention at fixed sizes: softmax(scale q k^T) v of q [batch,
+    q_len, heads, head_dim] and k, v [batch, k_len, kv_heads, head_dim] (axes in that
+    order, `layout` "bshd", or "bhsd"), head h with key head h // (heads //
+    kv_heads), without the weights in memory; `scale` head_dim ** -0.5 unless given.
+
+    Query i of a sequence stands at position first + i among its keys and reads
+    those below `lens` (i64 [batch]; none given: k_len): all of them; with `causal`
+    those up to its position, with a `window` the last so many of these; with
+    `mask_cols` those before `first` and, of the next mask_cols, those whose byte
+    of its row of `mask` ([batch, q_len, mask_cols] or, shared, [q_len, mask_cols];
+    bool or uint8) is not 0.  `first` (i64 [batch]) not given: the queries (the
+    mask's columns) are the last keys.  A query that reads no key has output 0, lse
+    -inf and no gradients.
+
+    `value` writes o and, given, lse (f32 [batch, heads, q_len]).  `vjp`, from the
+    forward's o and lse and the cotangent do, writes those of dq, dk and dv that
+    are given.  Buffers are DeviceBuffers or torch tensors; a call with tensors
+    that names no stream goes to torch's current one, others to the null stream.
+    `work` is workspace(kind) bytes of the caller's, or, not given, a buffer that
+    this object keeps for the call's stream: calls that share a workspace, their
+    captured graphs among them, run one after another."""
+
+    _name, _kinds = "attention", {"value": 1, "vjp": 2}
+    _tensors = {"q": False, "k": True, "v": True, "o": False, "do": False, "dq": False, "dk": True, "dv": True}
+
+    def __init__(self, dtype: str, batch: int, heads: int, kv_heads: int, q_len: int, k_len: int, head_dim: int, causal: bool = False,
+                 window: int = 0, mask_cols: int = 0, scale: float | None = None, layout: str = "bshd"):
+        self.dtype, self.batch, self.heads, self.kv_heads = dtype, int(batch), int(heads), int(kv_heads)
+        self.q_len, self.k_len, self.head_dim = int(q_len), int(k_len), int(head_dim)
+        self.causal, self.window, self.mask_cols = bool(causal), int(window), int(mask_cols)
+        self.scale = float(scale) if scale is not None else max(self.head_dim, 1) ** -0.5
+        self._lengths = (self.q_len, self.k_len)
+        self._init(layout)
+
+    def _args(self) -> AttnArgs:
+        return AttnArgs(self.dtype.encode(), self.batch, self.heads, self.kv_heads, self.q_len, self.k_len, self.head_dim, self.window,
+                        self.mask_cols, self.causal, self.scale)
+
+    def _other(self, a, name, b, device):
+        if name == "mask":
+            if not self.mask_cols:
+                raise ValueError("a mask of no columns (mask_cols)")
+            a.mask, a.mask_batch, a.mask_row = self._mask(b, device)
+            return
+        n, ty = {"lse": (4 * self.batch * self.heads * self.q_len, "f32"), "lens": (8 * self.batch, "i64"), "first": (8 * self.batch, "i64"),
+                 "flag": (4, None)}[name]
+        setattr(a, name, _buffer(name, b, device, n, ty))
+
+    def _mask(self, m, device) -> tuple:
+        if not hasattr(m, "data_ptr"):
+            return _buffer("mask", m, device, self.batch * self.q_len * self.mask_cols), self.q_len * self.mask_cols, self.mask_cols
+        at = _place("mask", m, device)
+        if str(m.dtype) not in ("torch.bool", "torch.uint8"):
+            raise ValueError(f"mask is {m.dtype}, not bool or uint8")
+        want = (self.q_len, self.mask_cols)
+        if tuple(m.shape) not in (want, (self.batch,) + want):
+            raise ValueError(f"mask is {list(m.shape)}, not {[self.batch, *want]} or {list(want)}")
+        st = m.stride()
+        if st[-1] != 1 and self.mask_cols > 1 and m.numel():
+            raise ValueError("mask's rows are not contiguous")
+        return at, st[0] if m.ndim == 3 else 0, st[-2]
+
+    def value(self, q, k, v, o, lse=None, lens=None, first=None, mask=None, flag=None, work=None, stream=None):
+        self._call("value", stream, q=q, k=k, v=v, o=o, lse=lse, lens=lens, first=first, mask=mask, flag=flag, work=work)
+
+    def vjp(self, q, k, v, o, lse, do, dq=None, dk=None, dv=None, lens=None, first=None, mask=None, flag=None, work=None, stream=None):
+        self._call("vjp", stream, q=q, k=k, v=v, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, lens=lens, first=first, mask=mask, flag=flag,
+                   work=work)
+
+
+def rotary_frequencies(rotary: int, base: float = 1e4) -> np.ndarray:
+    """The rotation's radians a position, f64 [rotary / 2]: base ** (-2 r / rotary)."""
+    return base ** (-2.0 * np.arange(rotary // 2) / max(rotary, 1))
+
+
+class HeadRotary(_HeadsCall):
+    """presk_hip_head_rotary at fixed sizes: each head of q [batch, seq, heads,
+    head_dim] and k [batch, seq, kv_heads, head_dim] (kv_heads 0: q alone; axes by
+    `layout`, as Attention's) normed, with `norm`, by its root mean square and the
+    gains gq and gk ([head_dim]; not given: ones), and its first `rotary` elements
+    (all, unless given) turned by the token's position: pair r by at * freq[r]
+    radians, freq f64 [rotary / 2] (rotary_frequencies) and `at` i64 [batch, seq]
+    (not given: 0, 1, ..).  `pairs` "half": elements r and r + rotary / 2; "even":
+    2 r and 2 r + 1.
+
+    `value` writes yq and yk, which may be q and k.  `vjp`, from the cotangents dyq
+    and dyk and, with `norm`, q and k, writes dq and dk (which may be dyq and dyk)
+    and those of dgq and dgk that are given.  Buffers, streams and `work` as
+    Attention's; only a gradient with `norm` needs any workspace."""
+
+    _name, _kinds = "head_rotary", {"value": 1, "vjp": 2}
+    _tensors = {"q": False, "k": True, "yq": False, "yk": True, "dyq": False, "dyk": True, "dq": False, "dk": True}
+
+    def __init__(self, dtype: str, batch: int, seq: int, heads: int, kv_heads: int, head_dim: int, rotary: int | None = None,
+                 norm: bool = False, eps: float = 1e-6, pairs: str = "half", layout: str = "bshd"):
+        if pairs not in ("half", "even"):
+            raise ValueError(f"pairs {pairs!r}, not half or even")
+        self.dtype, self.batch, self.seq, self.heads, self.kv_heads = dtype, int(batch), int(seq), int(heads), int(kv_heads)
+        self.head_dim, self.rotary = int(head_dim), int(head_dim if rotary is None else rotary)
+        self.norm, self.eps, self.pairs = bool(norm), float(eps), pairs
+        self._lengths = (self.seq, self.seq)
+        self._init(layout)
+
+    def _args(self) -> RotArgs:
+        return RotArgs(self.dtype.encode(), self.batch, self.seq, self.heads, self.kv_heads, self.head_dim, self.rotary, self.norm,
+                       self.pairs == "even", self.eps)
+
+    def _other(self, a, name, b, device):
+        g = (self.head_dim * STORAGE_BYTES[self.dtype], self.dtype)
+        n, ty = {"freq": (4 * self.rotary, "f64"), "at": (8 * self.batch * self.seq, "i64"), "flag": (4, None), "gq": g, "gk": g, "dgq": g,
+                 "dgk": g}[name]
+        setattr(a, name, _buffer(name, b, device, n, ty))
+
+    def _works_for(self, kind: str) -> bool:
+        return self.norm and kind == "vjp"
+
+    def value(self, q, freq, yq, k=None, yk=None, at=None, gq=None, gk=None, flag=None, work=None, stream=None):
+        self._call("value", stream, q=q, k=k, yq=yq, yk=yk, freq=freq, at=at, gq=gq, gk=gk, flag=flag, work=work)
+
+    def vjp(self, freq, dyq, dq, dyk=None, dk=None, q=None, k=None, at=None, gq=None, gk=None, dgq=None, dgk=None, flag=None, work=None,
+            stream=None):
+        self._call("vjp", stream, q=q, k=k, dyq=dyq, dyk=dyk, dq=dq, dk=dk, freq=freq, at=at, gq=gq, gk=gk, dgq=dgq, dgk=dgk, flag=flag,
                    work=work)

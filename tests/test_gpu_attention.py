@@ -1,0 +1,357 @@
+"""hip.Attention on the device against float64 (tests/attention_oracle.py), within
+what the roundings that it makes may add."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from presk_amd import hip  # noqa: E402
+from tests import attention_oracle as A  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def tensors(dtype, batch, heads, kv, tq, tk, d, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g).to(A.TORCH[dtype])  # noqa: E731
+    return n(batch, tq, heads, d), n(batch, tk, kv, d), n(batch, tk, kv, d), n(batch, tq, heads, d)
+
+
+def put(x, layout="bshd"):
+    if x is None:
+        return None
+    x = x.to(DEV)
+    return x.transpose(1, 2).contiguous() if layout == "bhsd" else x
+
+
+def run(dtype, q, k, v, do, layout="bshd", scale=None, causal=False, window=0, lens=None, first=None, mask=None, grad=True):
+    """The operator's value and gradients against float64."""
+    hip.init(0)
+    b, tq, h, d = q.shape
+    tk, kv = k.shape[1], k.shape[2]
+    op = hip.Attention(dtype, b, h, kv, tq, tk, d, causal=causal, window=window, mask_cols=0 if mask is None else mask.shape[-1], scale=scale,
+                       layout=layout)
+    Q, K, V, DO = (put(x, layout) for x in (q, k, v, do))
+    where = {n: x.to(DEV) for n, x in (("lens", lens), ("first", first), ("mask", mask)) if x is not None}
+    o = torch.full_like(Q, 9.0)
+    lse = torch.full((b, h, tq), 9.0, device=DEV)
+    op.value(Q, K, V, o, lse=lse, **where)
+    back = (lambda x: x.transpose(1, 2)) if layout == "bhsd" else (lambda x: x)
+    ok = A.allowed(b, tq, tk, causal, window, lens, first, mask)
+    case = A.Case(dtype, q, k, v, ok, op.scale, do)
+    worst = {n: A.check(n, back(g) if n == "o" else g, *case.value()[n]) for n, g in (("o", o), ("lse", lse))}
+    if grad:
+        grads = {n: torch.full_like(x, 9.0) for n, x in (("dq", Q), ("dk", K), ("dv", V))}
+        op.vjp(Q, K, V, o, lse, DO, **grads, **where)
+        want = case.vjp(back(o).cpu(), lse.cpu())
+        worst.update((n, A.check(n, back(g), *want[n])) for n, g in grads.items())
+    torch.cuda.synchronize()
+    print({n: round(w, 3) for n, w in worst.items()}, flush=True)
+
+
+# batch, heads, key heads, queries, keys, head
+SIZES = [(1, 1, 1, 1, 1, 64), (2, 4, 2, 5, 77, 64), (1, 3, 1, 33, 65, 128), (2, 2, 2, 128, 128, 64), (1, 2, 1, 200, 131, 80),
+         (2, 6, 3, 129, 300, 128), (3, 5, 5, 64, 64, 8), (1, 8, 2, 1, 700, 128), (1, 2, 2, 17, 31, 96)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_against_float64(dtype, causal, size):
+    run(dtype, *tensors(dtype, *size, seed=sum(size)), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("size", [(1, 2, 1, 70, 150, 256), (1, 2, 2, 1, 400, 200), (2, 4, 1, 40, 33, 136)], ids=str)
+def test_wide_heads(dtype, size):
+    run(dtype, *tensors(dtype, *size), causal=size[3] <= size[4])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [1, 3, 20, 33, 65, 101])
+def test_heads_that_are_no_whole_vectors(dtype, d):
+    run(dtype, *tensors(dtype, 2, 4, 2, 37, 90, d), causal=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
+def test_windows(dtype, window):
+    run(dtype, *tensors(dtype, 1, 4, 2, 150, 210, 64), causal=True, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["all", "causal", "window"])
+def test_sequences_of_unequal_lengths(dtype, kind):
+    """Lengths of nothing, of one key and past the end; queries before the
+    first key, and past the last."""
+    q, k, v, do = tensors(dtype, 6, 4, 2, 40, 170, 64)
+    lens = torch.tensor([0, 1, 170, 1000, 63, -5])
+    first = torch.tensor([0, -20, 130, 200, 23, 7])
+    for b, n in enumerate(lens.clamp(0, 170).tolist()):
+        # what lies past a sequence's end is not read
+        k[b, n:], v[b, n:] = math.nan, math.inf
+    run(dtype, q, k, v, do, causal=kind != "all", window=25 if kind == "window" else 0, lens=lens, first=first)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("size", [(2, 4, 2, 100, 100, 64), (2, 2, 2, 45, 333, 128)], ids=str)
+def test_masks_of_all_keys(dtype, shared, size):
+    """Rows and columns that are masked whole, and a mask that every sequence
+    shares."""
+    q, k, v, do = tensors(dtype, *size)
+    mask = torch.rand(size[0], size[3], size[4], generator=torch.Generator().manual_seed(1)) < 0.4
+    mask[:, 3] = False
+    mask[:, :, 40:] = mask[:, :, 40:] & (torch.arange(40, size[4]) % 7 > 2)
+    mask[:, 7:20, :70] = True
+    run(dtype, q, k, v, do, mask=mask[1] if shared else mask)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("per", [1, 4])
+def test_trees_of_drafted_tokens(dtype, per):
+    """A mask over the last keys of a cache, as bytes; what lies past it is not
+    read."""
+    b, tq, tk = 4, 13, 500
+    q, k, v, do = tensors(dtype, b, 2 * per, 2, tq, tk, 64)
+    lens = torch.tensor([13, 500, 77, 300])
+    parent = (torch.rand(b, tq, generator=torch.Generator().manual_seed(2)) * torch.arange(tq)).long()
+    mask = torch.zeros(b, tq, tq, dtype=torch.uint8)
+    for i in range(tq):
+        if i:
+            mask[:, i] = mask[torch.arange(b), parent[:, i]]
+        mask[:, i, i] = 255
+    run(dtype, q, k, v, do, lens=lens, first=lens - tq, mask=mask)
+    run(dtype, q, k, v, do, first=torch.tensor([0, 400, -3, 480]), mask=mask)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_heads_before_rows(dtype):
+    run(dtype, *tensors(dtype, 2, 6, 2, 50, 81, 64), layout="bhsd", causal=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_slices_of_packed_projections(dtype):
+    """Queries, keys, values and their gradients side by side in one buffer's rows."""
+    hip.init(0)
+    b, n, h, kv, d = 2, 90, 4, 2, 64
+    q, k, v, do = tensors(dtype, b, h, kv, n, n, d)
+    packed = torch.cat((q, k, v), 2).to(DEV)
+    cut = lambda x: x.split((h, kv, kv), 2)  # noqa: E731
+    Q, K, V = cut(packed)
+    grads = torch.full_like(packed, 9.0)
+    dq, dk, dv = cut(grads)
+    op = hip.Attention(dtype, b, h, kv, n, n, d, causal=True)
+    o, lse = torch.empty_like(do, device=DEV), torch.empty(b, h, n, device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    op.vjp(Q, K, V, o, lse, do.to(DEV), dq=dq, dk=dk, dv=dv)
+    case = A.Case(dtype, q, k, v, A.allowed(b, n, n, True), op.scale, do)
+    A.check("o", o, *case.value()["o"])
+    want = case.vjp(o.cpu(), lse.cpu())
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        A.check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_that_start_anywhere(dtype):
+    """Addresses and strides that are no multiples of 16 bytes, beside ones that are."""
+    hip.init(0)
+    b, n, h, d = 2, 70, 3, 64
+    q, k, v, do = tensors(dtype, b, h, h, n, n, d)
+
+    def odd(x):
+        wide = torch.full((b, n + 1, h, d + 3), 9.0, dtype=x.dtype, device=DEV)
+        y = wide[:, 1:, :, 1:d + 1]
+        y.copy_(x)
+        return y, wide
+
+    op = hip.Attention(dtype, b, h, h, n, n, d, causal=True)
+    (Q, _), (K, _), (DO, _) = odd(q), odd(k), odd(do)
+    (o, ow), (dq, qw), (dv, vw) = odd(q), odd(q), odd(v)
+    lse, dk, V = torch.empty(b, h, n, device=DEV), torch.empty_like(k, device=DEV), v.to(DEV)
+    op.value(Q, K, V, o, lse=lse)
+    op.vjp(Q, K, V, o, lse, DO, dq=dq, dk=dk, dv=dv)
+    case = A.Case(dtype, q, k, v, A.allowed(b, n, n, True), op.scale, do)
+    A.check("o", o, *case.value()["o"])
+    want = case.vjp(o.cpu(), lse.cpu())
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        A.check(name, got, *want[name])
+    for wide in (ow, qw, vw):
+        assert (wide[..., 0] == 9).all() and (wide[..., d + 1:] == 9).all() and (wide[:, 0] == 9).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_keys_that_the_batch_shares(dtype):
+    """Stride 0 over the batch: a prefix of all sequences."""
+    hip.init(0)
+    b, tq, tk, h, d = 3, 9, 140, 2, 64
+    q, k, v, do = tensors(dtype, b, h, h, tq, tk, d)
+    k, v = k[:1].expand(b, -1, -1, -1), v[:1].expand(b, -1, -1, -1)
+    op = hip.Attention(dtype, b, h, h, tq, tk, d)
+    o, lse = torch.empty_like(q, device=DEV), torch.empty(b, h, tq, device=DEV)
+    op.value(q.to(DEV), k[:1].to(DEV).expand_as(k), v[:1].to(DEV).expand_as(v), o, lse=lse)
+    case = A.Case(dtype, q, k, v, A.allowed(b, tq, tk), op.scale, do)
+    A.check("o", o, *case.value()["o"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scores_far_apart(dtype):
+    """Scores of thousands, and a scale of its own: the weights are one key's."""
+    q, k, v, do = tensors(dtype, 1, 2, 2, 40, 100, 64)
+    run(dtype, q * 8, k * 8, v, do, scale=2.0, causal=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scores_that_are_equal(dtype):
+    """Weights of 1 / keys each."""
+    q, k, v, do = tensors(dtype, 1, 2, 2, 40, 1500, 64)
+    run(dtype, q * 0, k, v, do)
+
+
+def test_no_queries_and_no_keys():
+    hip.init(0)
+    for tq, tk in ((0, 5), (5, 0), (0, 0)):
+        q, k, v, do = (x.to(DEV) for x in tensors("bf16", 2, 2, 2, tq, tk, 64))
+        op = hip.Attention("bf16", 2, 2, 2, tq, tk, 64)
+        o, lse = torch.full_like(q, 9.0), torch.full((2, 2, tq), 9.0, device=DEV)
+        op.value(q, k, v, o, lse=lse)
+        dq, dk, dv = torch.full_like(q, 9.0), torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+        op.vjp(q, k, v, o, lse, do, dq=dq, dk=dk, dv=dv)
+        assert (o == 0).all() and (lse == -math.inf).all() and (dq == 0).all() and (dk == 0).all() and (dv == 0).all()
+
+
+def test_a_gradient_alone():
+    """Any of the three by itself is the one that comes with the others."""
+    hip.init(0)
+    q, k, v, do = (x.to(DEV) for x in tensors("bf16", 1, 4, 2, 100, 130, 64))
+    op = hip.Attention("bf16", 1, 4, 2, 100, 130, 64, causal=True)
+    o, lse = torch.empty_like(q), torch.empty(1, 4, 100, device=DEV)
+    op.value(q, k, v, o, lse=lse)
+    like = {"dq": q, "dk": k, "dv": v}
+    all_ = {n: torch.empty_like(x) for n, x in like.items()}
+    op.vjp(q, k, v, o, lse, do, **all_)
+    for n, x in like.items():
+        one = torch.full_like(x, 9.0)
+        op.vjp(q, k, v, o, lse, do, **{n: one})
+        assert torch.equal(one, all_[n])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradients_by_differences(dtype):
+    """Of sum(o * do) along a random direction, from float32 values."""
+    hip.init(0)
+    b, tq, tk, h, kv, d = 1, 20, 50, 4, 2, 32
+    q, k, v, do = (x.float() for x in tensors(dtype, b, h, kv, tq, tk, d))
+    dirs = [x.double() for x in tensors("f32", b, h, kv, tq, tk, d, seed=5)[:3]]
+    ok = A.allowed(b, tq, tk, True)
+
+    def f(t):
+        c = A.Case("f32", *(x.double() + t * y for x, y in zip((q, k, v), dirs)), ok, d ** -0.5)
+        return float((c.value()["o"][0] * do.double()).sum())
+
+    slope = (f(1e-4) - f(-1e-4)) / 2e-4
+    ty = A.TORCH[dtype]
+    Q, K, V, DO = (x.to(ty).to(DEV) for x in (q, k, v, do))
+    op = hip.Attention(dtype, b, h, kv, tq, tk, d, causal=True)
+    o, lse = torch.empty_like(Q), torch.empty(b, h, tq, device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    grads = [torch.empty_like(x) for x in (Q, K, V)]
+    op.vjp(Q, K, V, o, lse, DO, *grads)
+    got = sum(float((g.cpu().double() * y).sum()) for g, y in zip(grads, dirs))
+    # the gradient's own roundings, independent: a few half steps of its terms'
+    # root mean square, and the differences' 1e-6
+    terms = math.sqrt(sum(float((g.cpu().double() * y).square().sum()) for g, y in zip(grads, dirs)))
+    assert abs(got - slope) <= 16 * A.HALF[dtype] * terms + 1e-6 * (1 + abs(slope)), (got, slope, terms)
+
+
+def test_a_captured_call_replays():
+    """A captured value and gradient over lengths and masks that change."""
+    hip.init(0)
+    b, tq, tk, h, kv, d = 2, 6, 300, 4, 2, 64
+    q, k, v, do = (x.to(DEV) for x in tensors("bf16", b, h, kv, tq, tk, d))
+    mask = torch.ones(b, tq, tq, dtype=torch.bool, device=DEV).tril()
+    lens, first = torch.tensor([40, 50], device=DEV), torch.tensor([34, 44], device=DEV)
+    op = hip.Attention("bf16", b, h, kv, tq, tk, d, mask_cols=tq)
+    o, lse = torch.empty_like(q), torch.empty(b, h, tq, device=DEV)
+    grads = [torch.empty_like(x) for x in (q, k, v)]
+    works = [torch.empty(op.workspace(n), dtype=torch.uint8, device=DEV) for n in ("value", "vjp")]
+
+    def call(o, lse, grads, works):
+        op.value(q, k, v, o, lse=lse, lens=lens, first=first, mask=mask, work=works[0])
+        op.vjp(q, k, v, o, lse, do, *grads, lens=lens, first=first, mask=mask, work=works[1])
+
+    call(o, lse, grads, works)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(o, lse, grads, works)
+    for step in range(4):
+        lens.add_(50), first.add_(50)
+        mask[:, step + 1, step] = False
+        q.mul_(1.1)
+        for x in (o, lse, *grads):
+            x.fill_(9.0)
+        graph.replay()
+        got = [x.clone() for x in (o, lse, *grads)]
+        again = [torch.empty_like(x) for x in got]
+        call(again[0], again[1], again[2:], [torch.empty_like(w) for w in works])
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, again)), step
+
+
+def test_two_streams():
+    """Calls of one object on two streams with no wait between them."""
+    hip.init(0)
+    ins = [[x.to(DEV) for x in tensors("bf16", 2, 4, 1, 1, 2000, 128, seed=s)] for s in (1, 2)]
+    op = hip.Attention("bf16", 2, 4, 1, 1, 2000, 128)
+    alone = []
+    for q, k, v, _ in ins:
+        o = torch.empty_like(q)
+        op.value(q, k, v, o)
+        alone.append(o)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    outs = [[torch.empty_like(i[0]) for _ in range(8)] for i in ins]
+    torch.cuda.synchronize()
+    for r in range(8):
+        for s, (q, k, v, _), o in zip(streams, ins, outs):
+            with torch.cuda.stream(s):
+                op.value(q, k, v, o[r])
+    torch.cuda.synchronize()
+    for o, want in zip(outs, alone):
+        assert all(torch.equal(x, want) for x in o)
+
+
+def test_f16_gradients_that_overflow_set_the_flag():
+    hip.init(0)
+    q, k, v, do = (x.to(DEV) for x in tensors("f16", 1, 2, 2, 40, 40, 64))
+    op = hip.Attention("f16", 1, 2, 2, 40, 40, 64)
+    o, lse = torch.empty_like(q), torch.empty(1, 2, 40, device=DEV)
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    grads = [torch.empty_like(x) for x in (q, k, v)]
+    op.value(q, k, v, o, lse=lse, flag=flag)
+    op.vjp(q, k, v, o, lse, do, *grads, flag=flag)
+    assert int(flag) == 0
+    op.vjp(q, k, v, o, lse, (do.float() * 0 + 60000).half(), *grads, flag=flag)
+    assert int(flag) == 1
+
+
+def test_a_long_cache():
+    """Keys whose elements lie past 2^31 elements and 2^32 bytes: the last ones'
+    rows alone are read, by a window."""
+    hip.init(0)
+    tk, kv, d, w = 1 << 20, 17, 128, 200
+    k = torch.zeros(1, tk, kv, d, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    g = torch.Generator().manual_seed(3)
+    kl, vl = (torch.randn(1, w, kv, d, generator=g).bfloat16() for _ in range(2))
+    k[:, -w:], v[:, -w:] = kl.to(DEV), vl.to(DEV)
+    q = torch.randn(1, 3, kv, d, generator=g).bfloat16()
+    op = hip.Attention("bf16", 1, kv, kv, 3, tk, d, causal=True, window=w - 2)
+    o = torch.empty_like(q, device=DEV)
+    op.value(q.to(DEV), k, v, o)
+    case = A.Case("bf16", q, kl, vl, A.allowed(1, 3, w, True, w - 2), op.scale)
+    A.check("o", o, *case.value()["o"])
