@@ -56,8 +56,8 @@ struct AttnArgs {
     // rows; the keys are cut into `splits`, whose sums are joined after
     int pack, splits;
     float *part, *part_ml;       // [split][batch][heads][tq][ND * 32] and [split][batch][heads][tq]{max, sum}
-    // what the backward pass needs of a row: {-lse / scale, -sum do o}
-    float* rows;                 // [batch][heads][tq][2]
+    // what the backward pass needs of a row: -lse log2 e and -sum do o
+    float* rows;                 // [2][batch][heads][tq]
 };
 
 // bits of a byte mask

@@ -33,7 +33,7 @@ struct Geo {
     static constexpr int ROW = PITCH * ES, CPR = ROW / 16, EPC = 16 / ES;
     static constexpr int STEPS = ND * 32 / (2 * EPC);     // 16-byte reads of a row a lane (its half of each pair of chunks)
     static constexpr int TILE = ROW <= 256 ? 64 : 32;     // rows of a tile
-    __device__ static __forceinline__ int swz(int r) {
+    __host__ __device__ static constexpr int swz(int r) {
         if constexpr (CPR == 8) return ((r & 2) << 1) | ((r & 4) >> 1) | ((r ^ (r >> 3)) & 1);
         else return ((r & 1) << 2) | (((r >> 1) ^ (r >> 3)) & 1) << 3 | (r & 2) | ((r >> 2) & 1);
     }
@@ -85,56 +85,93 @@ struct Weights<kF32> {
 // The tile row, of 32, of a lane's sum e.
 __device__ __forceinline__ int row_of(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
 
-// A lane's part of row `row` of a tile at step `st`.
+// Where a lane reads a tile: LDS addresses, of a tile's 32 rows by adding whole
+// tiles to them.  A step's and a piece's chunks are a base's with bits flipped, so
+// that a lane holds one address and not one a step: `row` its part of row lane &
+// 31, `col` its first element of the transposed 32 rows.
 template <int ST, int ND>
-__device__ __forceinline__ typename FragOf<ST>::T frag_row(const unsigned char* xs, int row, int st, int h) {
+struct Places {
     typedef Geo<ST, ND> G;
-    return *(const typename FragOf<ST>::T*)(xs + row * G::ROW + (((2 * st + h) ^ G::swz(row)) << 4));
+    unsigned row, col;
+    __device__ __forceinline__ void init(int lane) {
+        const int h = lane >> 5, r = lane & 31;
+        row = (unsigned)(r * G::ROW + ((h ^ G::swz(r)) << 4));
+        if constexpr (ST == kF32) {
+            const int el = ND * r;
+            col = (unsigned)(4 * h * G::ROW + (((el >> 2) ^ h) << 4 | (el & 3) << 2));
+        } else {
+            const int L = lane & 15, g = (lane >> 4) & 1, q = 4 * h + (L >> 2);
+            col = (unsigned)(q * G::ROW + (((2 * g + ((L & 3) >> 1)) ^ G::swz(q)) << 4) + 8 * (L & 1));
+        }
+    }
+    // at `at` bytes of LDS.  The compiler does not see that they stay the same
+    // from tile to tile, or it would keep every step's.
+    __device__ __forceinline__ Places from(unsigned at) const {
+        Places p{row + at, col + at};
+        asm volatile("" : "+v"(p.row), "+v"(p.col));
+        return p;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T lds_read(unsigned at) {
+    return *(__attribute__((address_space(3))) T*)at;
 }
 
-// acc[dt] += X^T . w over the tile's rows row0 .. row0 + 31.  Of acc[dt]'s sum e
-// a lane's element of the head is dim_of(dt, e).
-template <int ST, int ND>
-__device__ __forceinline__ void mma_col(const unsigned char* xs, int row0, const Weights<ST>& w, f32x16 (&acc)[ND], int lane) {
+// A lane's part of its row at step `st` (its half of chunks 2 st and 2 st + 1).
+template <int ST>
+__device__ __forceinline__ typename FragOf<ST>::T frag_row(unsigned row, int st, unsigned off = 0) {
+    return lds_read<typename FragOf<ST>::T>((row ^ (unsigned)(st << 5)) + off);
+}
+
+// acc[n][dt] += X^T . w[n] over 32 rows of a tile, for NB blocks of kept rows.  f32
+// takes a lane's elements of the head as ND consecutive ones.
+template <int ST, int ND, int NB, bool TIGHT = false>
+__device__ __forceinline__ void mma_col(unsigned col, unsigned off, const Weights<ST> (&w)[NB], f32x16 (&acc)[NB][ND]) {
     typedef Geo<ST, ND> G;
-    const int h = lane >> 5;
     if constexpr (ST == kF32) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int r = row0 + row_of(e, h), m = lane & 31, el = ND * m;
-            const unsigned char* const at = xs + r * G::ROW + ((((el >> 2) ^ G::swz(r)) << 4) | ((el & 3) << 2));
+            // (the row without the half-wave's 4, which `col` has)
+            const int r = 8 * (e >> 2) + (e & 3);
+            const unsigned at = (col ^ (unsigned)(G::swz(r) << 4)) + (unsigned)(r * G::ROW) + off;
             float x[ND];
             if constexpr (ND == 4) {
-                const f32x4 v = *(const f32x4*)at;
+                const f32x4 v = lds_read<f32x4>(at);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = v[i];
             } else {
-                const f32x2 v = *(const f32x2*)at;
+                const f32x2 v = lds_read<f32x2>(at);
                 x[0] = v[0], x[1] = v[1];
             }
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[dt], w.w[e], acc[dt], 0, 0, 0);
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) acc[n][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[dt], w[n].w[e], acc[n][dt], 0, 0, 0);
         }
     } else {
-        const int L = lane & 15, g = (lane >> 4) & 1;
+        constexpr unsigned FLIP = (unsigned)((G::swz(8) ^ G::swz(0)) << 4);      // of a row 8 further on
+        // (TIGHT: a fragment's reads one ahead of its products, and no further)
+        v4i16 a, b;
+        auto read = [&](int n) {
+            const int s = n / ND, dt = n % ND;
+            a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)((col ^ (unsigned)(dt << 6)) + (unsigned)(16 * s * G::ROW) + off));
+            b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)((col ^ (unsigned)(dt << 6) ^ FLIP) + (unsigned)((16 * s + 8) * G::ROW) + off));
+        };
+        read(0);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int r = row0 + 16 * s + 4 * h + (L >> 2);
+        for (int i = 0; i < 2 * ND; ++i) {
+            u16x8 f;
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
-                const int col = dt * 32 + 16 * g + 4 * (L & 3);
-                const int lo = r * G::ROW + (((col >> 3) ^ G::swz(r)) << 4) + (col & 7) * 2;
-                const int hi = (r + 8) * G::ROW + (((col >> 3) ^ G::swz(r + 8)) << 4) + (col & 7) * 2;
-                const v4i16 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(xs + lo));
-                const v4i16 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(xs + hi));
-                u16x8 f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[e] = (unsigned short)a[e];
-                    f[4 + e] = (unsigned short)b[e];
-                }
-                acc[dt] = mfma32<ST>(f, w.w[s], acc[dt]);
+            for (int e = 0; e < 4; ++e) {
+                f[e] = (unsigned short)a[e];
+                f[4 + e] = (unsigned short)b[e];
             }
+            if (i + 1 < 2 * ND) read(i + 1);
+            if (TIGHT) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) acc[n][i % ND] = mfma32<ST>(f, w[n].w[i / ND], acc[n][i % ND]);
+            if (TIGHT) __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -162,12 +199,15 @@ __device__ __forceinline__ const void* row_at(const AttnTensor& t, int b, long l
     return (const char*)t.p + n * (ST == kF32 ? 4 : 2);
 }
 
-// A kept row: a lane's 16 bytes of every step.
+// A kept row: a lane's 16 bytes of every step.  Rows that are no whole vectors
+// pass through the lane's own 16 bytes a step of `lds` (the wave's 1 KB a step),
+// in a loop that is not unrolled.
 template <int ST, int ND>
-__device__ __forceinline__ void load_kept(const AttnTensor& t, int b, long long i, int head, int d, bool in, int h,
+__device__ __forceinline__ void load_kept(const AttnTensor& t, int b, long long i, int head, int d, bool in, int lane, unsigned char* lds,
                                           typename FragOf<ST>::T (&x)[Geo<ST, ND>::STEPS]) {
     typedef typename FragOf<ST>::T F;
     const void* const row = row_at<ST>(t, b, in ? i : 0, head);
+    const int h = lane >> 5;
     if (t.vec) {
 #pragma unroll
         for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) {
@@ -175,8 +215,11 @@ __device__ __forceinline__ void load_kept(const AttnTensor& t, int b, long long 
             x[st] = in && c * Geo<ST, ND>::EPC < d ? *(const F*)((const char*)row + 16 * c) : F{};
         }
     } else {
+        F* const mine = (F*)lds + lane;
+#pragma unroll 1
+        for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) mine[64 * st] = chunk_of<ST>(row, 2 * st + h, d, in);
 #pragma unroll
-        for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) x[st] = chunk_of<ST>(row, 2 * st + h, d, in);
+        for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) x[st] = mine[64 * st];
     }
 }
 
@@ -230,9 +273,20 @@ struct Rows {
                              : : "v"(off), "s"(buf), "s"(__builtin_amdgcn_readfirstlane(lds0 + at + (unsigned)(q * NTH * 16))) : "memory", "m0");
             }
         } else {
+            const int n = left < ROWS ? left : ROWS;
+            const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), (short)0, (int)((n - 1) * stride + d * G::ES), 0x00020000);
+#pragma unroll 1
             for (int q = 0; q < ROUNDS; ++q) {
                 const int slot = q * NTH + tid, r = slot / G::CPR, c = (slot % G::CPR) ^ G::swz(r);
-                *(typename FragOf<ST>::T*)(smem + at + slot * 16) = chunk_of<ST>(src + (r < left ? r : 0) * stride, c, d, r < left);
+                const unsigned off = (unsigned)(r * (int)stride + 16 * c);
+                typename FragOf<ST>::T f;
+#pragma unroll
+                for (int e = 0; e < G::EPC; ++e) {
+                    const int o = c * G::EPC + e < d ? (int)(off + e * G::ES) : (int)0x80000000u;
+                    if constexpr (ST == kF32) f[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buf, o, 0, 0));
+                    else f[e] = __builtin_amdgcn_raw_buffer_load_b16(buf, o, 0, 0);
+                }
+                *(typename FragOf<ST>::T*)(smem + at + slot * 16) = f;
             }
         }
     }
@@ -240,31 +294,26 @@ struct Rows {
 
 // ---- stores -----------------------------------------------------------------------
 
-// A lane's row of sums times f into the storage type.
-template <int ST, int ND>
-__device__ __forceinline__ void store_kept(const AttnTensor& t, int b, long long i, int head, int d, const f32x16 (&acc)[ND], float f, int h,
-                                           bool in, unsigned* flag) {
-    if (!in) return;
-    void* const row = const_cast<void*>(row_at<ST>(t, b, i, head));
+// A wave's 32 rows of sums, a lane's times its own f, in the storage type: through
+// the wave's 32 rows of `lds` (which no other wave reads any more), so that a row
+// leaves in 16-byte vectors beside each other.  `where(r)`: row r's address, null
+// where there is none.
+template <int ST, int ND, typename W>
+__device__ __forceinline__ void store_kept(const f32x16 (&acc)[ND], float f, int d, bool vec, bool live, W where, unsigned char* lds, int lane,
+                                           unsigned* flag) {
+    typedef Geo<ST, ND> G;
+    typedef typename FragOf<ST>::T F;
+    const int h = lane >> 5, r = lane & 31;
     bool ovf = false;
     if constexpr (ST == kF32) {
-        float* const out = (float*)row;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int at = ND * row_of(e, h);
-            if (t.vec) {
-                if (at < d) {
-                    if constexpr (ND == 4) *(f32x4*)(out + at) = f32x4{acc[0][e] * f, acc[1][e] * f, acc[2][e] * f, acc[3][e] * f};
-                    else *(f32x2*)(out + at) = f32x2{acc[0][e] * f, acc[1][e] * f};
-                }
-            } else {
-#pragma unroll
-                for (int dt = 0; dt < ND; ++dt)
-                    if (at + dt < d) out[at + dt] = acc[dt][e] * f;
-            }
+            unsigned char* const to = lds + r * G::ROW + ((((at >> 2) ^ G::swz(r)) << 4) | ((at & 3) << 2));
+            if constexpr (ND == 4) *(f32x4*)to = f32x4{acc[0][e] * f, acc[1][e] * f, acc[2][e] * f, acc[3][e] * f};
+            else *(f32x2*)to = f32x2{acc[0][e] * f, acc[1][e] * f};
         }
     } else {
-        unsigned short* const out = (unsigned short*)row;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -272,22 +321,34 @@ __device__ __forceinline__ void store_kept(const AttnTensor& t, int b, long long
                 const int at = dt * 32 + 8 * g + 4 * h;
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = acc[dt][4 * g + e] * f;
-                if (at >= d) continue;
-                if (ST == kF16)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) ovf |= pk_overflows_f16(x[e]);
-                const unsigned lo = pack2<ST>(x[0], x[1]), hi = pack2<ST>(x[2], x[3]);
-                if (t.vec) {
-                    *(unsigned long long*)(out + at) = lo | (unsigned long long)hi << 32;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at + e < d) out[at + e] = (unsigned short)((e < 2 ? lo : hi) >> (16 * (e & 1)));
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = acc[dt][4 * g + e] * f;
+                    if (ST == kF16) ovf |= pk_overflows_f16(x[e]);
                 }
+                *(unsigned long long*)(lds + r * G::ROW + ((((at >> 3) ^ G::swz(r)) << 4) | ((at & 4) << 1))) =
+                    pack2<ST>(x[0], x[1]) | (unsigned long long)pack2<ST>(x[2], x[3]) << 32;
             }
     }
-    if (ovf && flag) atomicOr(flag, 1u);
+    if (ovf && live && flag) atomicOr(flag, 1u);
+    constexpr int EPC = G::EPC;
+#pragma unroll 1
+    for (int u = lane; u < 32 * G::CPR; u += 64) {
+        const int row = u / G::CPR, c = u % G::CPR;
+        if (c * EPC >= d) continue;
+        char* const to = (char*)where(row);
+        if (!to) continue;
+        const F v = *(const F*)(lds + row * G::ROW + ((c ^ G::swz(row)) << 4));
+        if (vec) {
+            *(F*)(to + 16 * c) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPC; ++e)
+                if (c * EPC + e < d) {
+                    if constexpr (ST == kF32) ((float*)to)[c * EPC + e] = v[e];
+                    else ((unsigned short*)to)[c * EPC + e] = v[e];
+                }
+        }
+    }
 }
 
 // ---- which keys a query reads -------------------------------------------------------
@@ -324,6 +385,17 @@ __device__ __forceinline__ unsigned bits_at(const unsigned* line, int words, int
     return (unsigned)(((unsigned long long)hi << 32 | lo) >> (rel & 31));
 }
 
+// Bits [lo, hi) of 32.
+__device__ __forceinline__ unsigned range_of(int lo, int hi) {
+    const unsigned from = lo <= 0 ? ~0u : lo < 32 ? ~0u << lo : 0u, to = hi >= 32 ? ~0u : hi > 0 ? ~0u >> (32 - hi) : 0u;
+    return from & to;
+}
+// x where bit row_of(e, h) of a lane's 32 is set, else `no`; `bits` are shifted by 4 h.
+__device__ __forceinline__ float where_bit(unsigned bits, int e, float x, float no) {
+    const int m = (int)(bits << (31 - 8 * (e >> 2) - (e & 3))) >> 31;
+    return __builtin_bit_cast(float, (m & __builtin_bit_cast(int, x)) | (~m & __builtin_bit_cast(int, no)));
+}
+
 // Work order: workgroups are dealt to the 8 XCDs round robin; each takes one
 // run of items, so that those of a head share its keys in one L2.
 __device__ __forceinline__ unsigned item_of(unsigned id, unsigned total) {
@@ -340,8 +412,8 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
     typedef Rows<ST, ND, G::TILE, 256> Tile;
     constexpr int NB = G::TILE / 32;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * Tile::BYTES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int rows = a.tq * a.pack, tiles = (rows + kAttnTile - 1) / kAttnTile, groups = a.heads / a.pack;
     const unsigned item = item_of(blockIdx.x, gridDim.x);
@@ -383,46 +455,54 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
         kt.issue(k0, khi - k0, stage, smem, tid);
         vt.issue(k0, khi - k0, stage, smem + Tile::BYTES, tid);
     };
-    if (nt > 0) fetch(0);
+    unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
     typename FragOf<ST>::T q[G::STEPS];
-    load_kept<ST, ND>(a.q, b, i, head, a.d, live, h, q);
+    load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
+    if (!a.q.vec) __syncthreads();
+    if (nt > 0) fetch(0);
 
-    f32x16 o[ND];
+    f32x16 o[1][ND];
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt) o[dt] = f32x16{};
+    for (int dt = 0; dt < ND; ++dt) o[0][dt] = f32x16{};
     float m = -INFINITY, l = 0.f;       // in log 2; this lane's part of the sum
+    // what any of the wave's rows reads
+    const int w0 = r0 + wave * 32, w1 = w0 + 31 < r1 ? w0 + 31 : r1;
+    const int wlo = keys.lo(a, (w0 < r1 ? w0 : r1) / a.pack), whi = w0 <= r1 ? keys.hi(a, w1 / a.pack) : 0;
 
-    for (int t = 0; t < nt; ++t) {
-        wait_vm<0>();
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+    Places<ST, ND> places;
+    places.init(lane);
+    places = places.from(lds);
+    auto body = [&](bool masked, int t) {
         const int k0 = klo + t * G::TILE;
-        const unsigned char* const ks = smem + (t & 1) * 2 * Tile::BYTES;
-        const unsigned char* const vs = ks + Tile::BYTES;
+        const Places<ST, ND> at = places.from((unsigned)(t & 1) * 2 * Tile::BYTES);
         f32x16 s[NB];
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-            s[kb] = f32x16{};
-#pragma unroll
-            for (int st = 0; st < G::STEPS; ++st) s[kb] = mma_row<ST>(frag_row<ST, ND>(ks, kb * 32 + (lane & 31), st, h), q[st], s[kb]);
-        }
-        if (k0 < surelo || k0 + G::TILE > surehi) {
-#pragma unroll
-            for (int kb = 0; kb < NB; ++kb) {
-                const int base = k0 + kb * 32;
-                const unsigned bits = a.cols ? bits_at(line, a.words, base - keys.first) : ~0u;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int c = row_of(e, h), j = base + c;
-                    s[kb][e] = j >= rlo && j < rhi && (bits >> c & 1) ? s[kb][e] : -INFINITY;
-                }
-            }
-        }
+        bool any[NB];
         float mx = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
+        for (int kb = 0; kb < NB; ++kb) {
+            const int base = k0 + kb * 32;
+            unsigned bits = ~0u;
+            any[kb] = true;
+            if (masked) {
+                // keys that no row of the wave reads are passed over
+                any[kb] = base < whi && base + 32 > wlo;
+                if (any[kb] && a.cols && base + 32 > keys.first) {
+                    bits = bits_at(line, a.words, base - keys.first);
+                    any[kb] = __any(bits);
+                }
+                if (!any[kb]) continue;
+            }
+            s[kb] = f32x16{};
+#pragma unroll
+            for (int st = 0; st < G::STEPS; ++st) s[kb] = mma_row<ST>(frag_row<ST>(at.row, st, kb * 32 * G::ROW), q[st], s[kb]);
+            if (masked) {
+                bits = (bits & range_of(rlo - base, rhi - base)) >> (4 * h);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] = where_bit(bits, e, s[kb][e], -INFINITY);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+        }
         mx = fmaxf(mx, partner<32>(mx)) * a.c;
         // the sums stay at an older maximum until one passes it by 2^8
         if (__any(mx > m + 8.f)) {
@@ -432,11 +512,12 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[dt][e] *= f;
+                for (int e = 0; e < 16; ++e) o[0][dt][e] *= f;
         }
         const float base = base_of(m);
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
+            if (!any[kb]) continue;
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -444,10 +525,17 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
                 sum += s[kb][e];
             }
             l += sum;
-            Weights<ST> w;
-            w.set(s[kb]);
-            mma_col<ST, ND>(vs, kb * 32, w, o, lane);
+            Weights<ST> w[1];
+            w[0].set(s[kb]);
+            mma_col<ST, ND, 1>(at.col, Tile::BYTES + kb * 32 * G::ROW, w, o);
         }
+    };
+    for (int t = 0; t < nt; ++t) {
+        wait_vm<0>();
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1);
+        const int k0 = klo + t * G::TILE;
+        body(k0 < surelo || k0 + G::TILE > surehi, t);
     }
 
     l += partner<32>(l);
@@ -460,12 +548,16 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
             for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *(f32x4*)(out + dt * 32 + 8 * g + 4 * h) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+                    *(f32x4*)(out + dt * 32 + 8 * g + 4 * h) = f32x4{o[0][dt][4 * g], o[0][dt][4 * g + 1], o[0][dt][4 * g + 2], o[0][dt][4 * g + 3]};
             if (h == 0) *(f32x2*)(a.part_ml + 2 * n) = f32x2{m, l};
         }
         return;
     }
-    store_kept<ST, ND>(a.o, b, i, head, a.d, o, l == 0.f ? 0.f : 1.f / l, h, live, a.flag);
+    __syncthreads();
+    store_kept<ST, ND>(o[0], l == 0.f ? 0.f : 1.f / l, a.d, a.o.vec, live, [&](int n) -> const void* {
+        const int x = r0 + wave * 32 + n;
+        return x < rows ? row_at<ST>(a.o, b, x / a.pack, hx * a.pack + x % a.pack) : nullptr;
+    }, own, lane, a.flag);
     if (a.lse && live && h == 0) a.lse[row] = l == 0.f ? -INFINITY : (base_of(m) + __builtin_log2f(l)) * kLn2;
 }
 
@@ -513,8 +605,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 
 // ---- the gradients --------------------------------------------------------------------
 
-// A row's {-lse / scale, -sum do o}: the scores' products start from the one, the
-// weights' cotangents from the other.  16 lanes a row.
+// A row's -lse log2 e, and behind all of them its -sum do o.  16 lanes a row.
 template <int ST>
 __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
     const long long all = (long long)a.batch * a.heads * a.tq, row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -543,41 +634,34 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
         const long long at = ((long long)b * a.heads + head) * a.tq + i;
         const float lse = a.lse[at];
         // (a row that reads nothing: its weights are zero by the keys it may read)
-        *(f32x2*)(a.rows + 2 * at) = f32x2{lse == -INFINITY ? 0.f : -lse / a.scale, -s};
+        a.rows[at] = -base_of(lse) * kLog2e;
+        a.rows[all + at] = -s;
     }
 }
 
-// The weights and their cotangents, from the products that started from the
-// rows' sums: p = exp2(c s), ds = p dp.  In f16 the weights, most of them far below
-// one, enter their product times 2^8.
+// In f16 the weights, most of them far below one, enter their product times 2^8.
 constexpr float kShift = 8.f;
 
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
-// the queries'.
-template <int ST, int ND>
-__global__ void __launch_bounds__(256, ND == 8 || (ST == kF32 && ND == 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
+// the queries', NB blocks of 32 rows a wave.
+template <int ST, int ND, int NB>
+__global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
     typedef Rows<ST, ND, G::TILE, 256> Tile;
-    constexpr int NB = G::TILE / 32;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * Tile::BYTES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    constexpr int WROWS = 32 * NB, ROWS = 4 * WROWS;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
-    const int tiles = (a.tq + kAttnTile - 1) / kAttnTile;
+    const int tiles = (a.tq + ROWS - 1) / ROWS;
     const unsigned at = item_of(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
     const int b = unit / a.heads, head = unit % a.heads, hk = head / a.per;
-    const int r0 = tile * kAttnTile, r1 = (a.tq < r0 + kAttnTile ? a.tq : r0 + kAttnTile) - 1;
+    const int r0 = tile * ROWS, r1 = (a.tq < r0 + ROWS ? a.tq : r0 + ROWS) - 1;
 
     Keys keys;
     keys.init(a, b);
     const int klo = keys.lo(a, r0), khi = keys.hi(a, r1), surelo = keys.lo(a, r1), surehi = keys.sure(a, r0);
     const int nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
-
-    const int r = r0 + wave * 32 + (lane & 31);
-    const bool live = r < a.tq;
-    const int i = live ? r : r1;
-    const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
-    const unsigned* const line = a.cols ? a.bits + ((long long)b * a.bits_batch + i) * a.words : nullptr;
 
     Tile kt, vt;
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
@@ -589,169 +673,298 @@ __global__ void __launch_bounds__(256, ND == 8 || (ST == kF32 && ND == 4) ? 1 : 
         kt.issue(k0, khi - k0, stage, smem, tid);
         vt.issue(k0, khi - k0, stage, smem + Tile::BYTES, tid);
     };
-    if (nt > 0) fetch(0);
-    typename FragOf<ST>::T q[G::STEPS], dout[G::STEPS];
-    load_kept<ST, ND>(a.q, b, i, head, a.d, live, h, q);
-    load_kept<ST, ND>(a.dout, b, i, head, a.d, live, h, dout);
-    const f32x2 st2 = *(const f32x2*)(a.rows + 2 * (((long long)b * a.heads + head) * a.tq + i));
+    unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
 
-    f32x16 dq[ND];
+    const int w0 = r0 + wave * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
+    const int wlo = keys.lo(a, w0 < r1 ? w0 : r1), whi = w0 <= r1 ? keys.hi(a, w1) : 0;
+    typename FragOf<ST>::T q[NB][G::STEPS], dout[NB][G::STEPS];
+    float lse[NB], delta[NB];
+    f32x16 dq[NB][ND];
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt) dq[dt] = f32x16{};
+    for (int n = 0; n < NB; ++n) {
+        const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
+        load_kept<ST, ND>(a.q, b, i, head, a.d, r <= r1, lane, own, q[n]);
+        load_kept<ST, ND>(a.dout, b, i, head, a.d, r <= r1, lane, own, dout[n]);
+        const float* const x = a.rows + ((long long)b * a.heads + head) * a.tq + i;
+        lse[n] = x[0], delta[n] = x[(long long)a.batch * a.heads * a.tq];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dq[n][dt] = f32x16{};
+    }
+    if (!a.q.vec || !a.dout.vec) __syncthreads();
+    if (nt > 0) fetch(0);
 
+    Places<ST, ND> places;
+    places.init(lane);
+    places = places.from(lds);
+    auto body = [&](bool masked, int t, int kb) {
+        const int base = klo + t * G::TILE + kb * 32;
+        const Places<ST, ND> at = places.from((unsigned)((t & 1) * 2 * Tile::BYTES + kb * 32 * G::ROW));
+        unsigned bits[NB];
+        if (masked) {
+            // keys that no row of the wave reads are passed over
+            if (base >= whi || base + 32 <= wlo) return;
+            unsigned all = 0;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
+                bits[n] = ~0u;
+                if (a.cols && base + 32 > keys.first)
+                    bits[n] = bits_at(a.bits + ((long long)b * a.bits_batch + i) * a.words, a.words, base - keys.first);
+                all |= bits[n];
+            }
+            if (!__any(all)) return;
+        }
+        f32x16 s[NB], dp[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = dp[n] = f32x16{};
+#pragma unroll
+        for (int st = 0; st < G::STEPS; ++st) {
+            const auto fk = frag_row<ST>(at.row, st), fv = frag_row<ST>(at.row, st, Tile::BYTES);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                s[n] = mma_row<ST>(fk, q[n][st], s[n]);
+                dp[n] = mma_row<ST>(fv, dout[n][st], dp[n]);
+            }
+        }
+        Weights<ST> w[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], a.c, lse[n])) * (dp[n][e] + delta[n]);
+            if (masked) {
+                const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
+                const unsigned in = (bits[n] & range_of(keys.lo(a, i) - base, keys.hi(a, i) - base)) >> (4 * h);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] = where_bit(in, e, s[n][e], 0.f);
+            }
+            w[n].set(s[n]);
+        }
+        mma_col<ST, ND, NB>(at.col, 0, w, dq);
+    };
     for (int t = 0; t < nt; ++t) {
         wait_vm<0>();
         __syncthreads();
         if (t + 1 < nt) fetch(t + 1);
         const int k0 = klo + t * G::TILE;
-        const unsigned char* const ks = smem + (t & 1) * 2 * Tile::BYTES;
-        const unsigned char* const vs = ks + Tile::BYTES;
-        const bool sure = k0 >= surelo && k0 + G::TILE <= surehi;
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-            f32x16 s, dp;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = st2[0], dp[e] = st2[1];
-#pragma unroll
-            for (int st = 0; st < G::STEPS; ++st) {
-                s = mma_row<ST>(frag_row<ST, ND>(ks, kb * 32 + (lane & 31), st, h), q[st], s);
-                dp = mma_row<ST>(frag_row<ST, ND>(vs, kb * 32 + (lane & 31), st, h), dout[st], dp);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * a.c) * dp[e];
-            if (!sure) {
-                const int base = k0 + kb * 32;
-                const unsigned bits = a.cols ? bits_at(line, a.words, base - keys.first) : ~0u;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int c = row_of(e, h), j = base + c;
-                    s[e] = j >= rlo && j < rhi && (bits >> c & 1) ? s[e] : 0.f;
-                }
-            }
-            Weights<ST> w;
-            w.set(s);
-            mma_col<ST, ND>(ks, kb * 32, w, dq, lane);
-        }
+#pragma unroll 1
+        for (int kb = 0; kb < G::TILE / 32; ++kb) body(k0 < surelo || k0 + G::TILE > surehi, t, kb);
     }
-    store_kept<ST, ND>(a.dq, b, i, head, a.d, dq, a.scale, h, live, a.flag);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+        store_kept<ST, ND>(dq[n], a.scale, a.d, a.dq.vec, w0 + 32 * n + (lane & 31) <= r1, [&](int x) -> const void* {
+            const int r = w0 + 32 * n + x;
+            return r <= r1 ? row_at<ST>(a.dq, b, r, head) : nullptr;
+        }, own, lane, a.flag);
 }
 
-// The keys' and values' gradients: a workgroup keeps 128 keys of a key head, 32 a
-// wave, and the rows of all heads of its group that read any of them pass by.
-template <int ST, int ND>
-__global__ void __launch_bounds__(256, ND == 8 || (ST == kF32 && ND == 4) ? 1 : 2) attn_dkv_kernel(AttnArgs a) {
+// The keys' and values' gradients (DK, DV): a workgroup keeps 128 NB keys of a key
+// head, NB blocks of 32 a wave, and the rows of all heads of its group that read
+// any of them pass by.
+template <int ST, int ND, int NB, int QT, bool DK, bool DV, bool VL, int OCC>
+__global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, 32, 256> Tile;
-    constexpr int STAGE = 2 * Tile::BYTES + 256;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    typedef Rows<ST, ND, QT, 256> Tile;
+    constexpr int WKEYS = 32 * NB, KEYS = 4 * WKEYS, STAGE = 2 * Tile::BYTES + 512;
+    typedef Rows<ST, ND, KEYS, 256> Kept;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + (VL ? Kept::BYTES : 0)];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
-    const int tiles = (a.tk + kAttnTile - 1) / kAttnTile;
+    const int tiles = (a.tk + KEYS - 1) / KEYS;
     const unsigned at = item_of(blockIdx.x, gridDim.x);
     const int tile = (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
     const int b = unit / a.kv, hk = unit % a.kv;
-    const int k0 = tile * kAttnTile, k1 = a.tk < k0 + kAttnTile ? a.tk : k0 + kAttnTile;
+    const int k0 = tile * KEYS, k1 = a.tk < k0 + KEYS ? a.tk : k0 + KEYS;
 
     Keys keys;
     keys.init(a, b);
-    // queries [ilo, ihi) read any of the keys
-    int ilo = 0, ihi = a.tq;
-    const int last = (k1 < keys.len ? k1 : keys.len) - 1;
-    if (a.causal) {
-        ilo = k0 - keys.first > 0 ? k0 - keys.first : 0;
-        if (a.window) {
-            const long long e = (long long)last - keys.first + a.window;
-            ihi = (int)(e < ihi ? e : ihi);
+    // queries [ilo, ihi) read any of the keys from jlo on, below jhi
+    auto queries = [&](int jlo, int jhi, int* ilo, int* ihi) {
+        const int last = (jhi < keys.len ? jhi : keys.len) - 1;
+        *ilo = 0, *ihi = a.tq;
+        if (a.causal) {
+            *ilo = jlo - keys.first > 0 ? jlo - keys.first : 0;
+            if (a.window) {
+                const long long e = (long long)last - keys.first + a.window;
+                *ihi = (int)(e < a.tq ? e : a.tq);
+            }
         }
-    }
-    if (a.cols && k0 >= keys.first + a.cols) ihi = 0;
-    if (last < k0) ihi = 0;
-    const int nt1 = ihi > ilo ? (ihi - ilo + 31) / 32 : 0, nt = nt1 * a.per;
-
-    // this lane's key
-    const int j = k0 + wave * 32 + (lane & 31);
-    const bool exists = j < a.tk, live = exists && j < keys.len;
-    const int jw = k0 + wave * 32;      // the wave's first
-    // queries [qlo, qhi) read it (and of a mask's columns those whose bit is set)
-    const int qlo = a.causal ? j - keys.first : 0;
-    const long long qend = a.window ? (long long)j - keys.first + a.window : a.tq;
-    const int qhi = (int)(qend < a.tq ? qend : a.tq);
-    const int col = j - keys.first;
-    const unsigned* const line =
-        a.cols && col >= 0 && col < a.cols ? a.bits_t + ((long long)b * a.bits_t_batch + col) * a.words_t : nullptr;
+        if (last < jlo || (a.cols && jlo >= keys.first + a.cols)) *ihi = 0;
+    };
+    int ilo, ihi, wlo, whi;
+    queries(k0, k1, &ilo, &ihi);
+    const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0, nt = nt1 * a.per;
+    const int jw = k0 + wave * WKEYS;      // the wave's first key
+    queries(jw, jw + WKEYS < k1 ? jw + WKEYS : k1, &wlo, &whi);
 
     Tile qt, dt_;
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
+    int fi = ilo, fg = 0;       // the next tile's first row, and its head in the group
     auto fetch = [&](int t) {
-        const int g = t / nt1, i0 = ilo + (t - g * nt1) * 32, head = hk * a.per + g;
+        const int i0 = fi, head = hk * a.per + fg;
         const unsigned stage = (unsigned)(t & 1) * STAGE;
+        fi += QT;
+        if (fi >= ihi) fi = ilo, ++fg;
         if (i0 == ilo) {
             qt.init(a.q, b, head, a.d, tid, lds);
             dt_.init(a.dout, b, head, a.d, tid, lds + Tile::BYTES);
         }
-        const int left = a.tq - i0;
+        const int left = ihi - i0;
         qt.issue(i0, left, stage, smem, tid);
         dt_.issue(i0, left, stage, smem + Tile::BYTES, tid);
-        if (wave == 0) {
-            const float* const src = a.rows + 2 * (((long long)b * a.heads + head) * a.tq + i0);
-            const i32x4 buf = buffer_of(src, (unsigned)((left < 32 ? left : 32) * 8));
+        if (wave < 2) {
+            // (the lanes past the rows write zeros into the rest of 256 bytes)
+            const float* const src = a.rows + (wave ? (long long)a.batch * a.heads * a.tq : 0) + ((long long)b * a.heads + head) * a.tq + i0;
+            const i32x4 buf = buffer_of(src, (unsigned)((left < QT ? left : QT) * 4));
             asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds"
-                         : : "v"(lane * 4), "s"(buf), "s"(__builtin_amdgcn_readfirstlane(lds + stage + 2 * Tile::BYTES)) : "memory", "m0");
+                         : : "v"(lane * 4), "s"(buf), "s"(__builtin_amdgcn_readfirstlane(lds + stage + 2 * Tile::BYTES + wave * 256)) : "memory", "m0");
         }
     };
-    if (nt > 0) fetch(0);
-    typename FragOf<ST>::T k[G::STEPS], v[G::STEPS];
-    load_kept<ST, ND>(a.k, b, j, hk, a.d, live, h, k);
-    load_kept<ST, ND>(a.v, b, j, hk, a.d, live, h, v);
-    f32x16 dk[ND], dv[ND];
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt) dk[dt] = dv[dt] = f32x16{};
 
-    for (int t = 0; t < nt; ++t) {
+    unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
+    typename FragOf<ST>::T k[NB][G::STEPS], v[VL ? 1 : NB][G::STEPS];
+    f32x16 dk[NB][ND], dv[NB][ND];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int j = jw + 32 * n + (lane & 31);
+        const bool live = j < k1 && j < keys.len;
+        load_kept<ST, ND>(a.k, b, j, hk, a.d, live, lane, own, k[n]);
+        if (DK && !VL) load_kept<ST, ND>(a.v, b, j, hk, a.d, live, lane, own, v[n]);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dk[n][dt] = dv[n][dt] = f32x16{};
+    }
+    if (!a.k.vec || !a.v.vec) __syncthreads();
+    if (nt > 0) {
+        if (VL) {
+            Kept vt;
+            vt.init(a.v, b, hk, a.d, tid, lds);
+            vt.issue(k0, (k1 < keys.len ? k1 : keys.len) - k0, 2 * STAGE, smem, tid);
+        }
+        fetch(0);
+    }
+
+    // the tile's rows sub * 32 on, which are the queries i0 on
+    Places<ST, ND> places;
+    places.init(lane);
+    places = places.from(lds);
+    auto body = [&](bool masked, int t, int sub, int i0) {
+        const unsigned stage = (unsigned)(t & 1) * STAGE;
+        const Places<ST, ND> at = places.from(stage + (unsigned)(sub * 32 * G::ROW));
+        const f32x4* const stats = (const f32x4*)(smem + stage + 2 * Tile::BYTES + 128 * sub + 16 * h);
+        unsigned bits[NB];
+        if (masked) {
+            // rows that read none of the wave's keys are passed over
+            if (i0 + 31 < wlo || i0 >= whi) return;
+            unsigned all = 0;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int col = jw + 32 * n + (lane & 31) - keys.first;
+                bits[n] = ~0u;
+                if (a.cols && col >= 0)
+                    bits[n] = col < a.cols ? bits_at(a.bits_t + ((long long)b * a.bits_t_batch + col) * a.words_t, a.words_t, i0) : 0u;
+                all |= bits[n];
+            }
+            if (!__any(all)) return;
+        }
+        const unsigned kept = VL ? places.from((unsigned)(2 * STAGE + wave * WKEYS * G::ROW)).row : 0u;
+        f32x16 s[NB], dp[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = dp[n] = f32x16{};
+        // a step's reads a step ahead of its products, and no further, or the
+        // registers do not hold them
+        typedef typename FragOf<ST>::T F;
+        F fq, fd, fv[NB];
+        auto read = [&](int st) {
+            fq = frag_row<ST>(at.row, st);
+            if (DK) {
+                fd = frag_row<ST>(at.row, st, Tile::BYTES);
+                if (VL)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) fv[n] = frag_row<ST>(kept, st, 32 * n * G::ROW);
+            }
+        };
+        read(0);
+#pragma unroll
+        for (int st = 0; st < G::STEPS; ++st) {
+            const F cq = fq, cd = fd;
+            F cv[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) cv[n] = VL ? fv[n] : v[VL ? 0 : n][st];
+            if (st + 1 < G::STEPS) read(st + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                s[n] = mma_row<ST>(cq, k[n][st], s[n]);
+                if (DK) dp[n] = mma_row<ST>(cd, cv[n], dp[n]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        Weights<ST> w[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = stats[2 * g];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[n][4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][4 * g + e], a.c, ST == kF16 ? x[e] + kShift : x[e]));
+            }
+            if (masked) {
+                const int j = jw + 32 * n + (lane & 31);
+                // queries [qlo, qhi) of these 32 read it (and of a mask's columns those whose bit is set)
+                const int qlo = a.causal ? j - keys.first - i0 : 0;
+                const long long end = a.window ? (long long)j - keys.first + a.window - i0 : 32;
+                const unsigned in = (bits[n] & range_of(qlo, (int)(end < 32 ? end : 32))) >> (4 * h);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[n][e] = where_bit(in, e, s[n][e], 0.f);
+            }
+            if (DV) w[n].set(s[n]);
+        }
+        if (DV) mma_col<ST, ND, NB, true>(at.col, Tile::BYTES, w, dv);
+        if (DK) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 x = stats[16 + 2 * g];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = s[n][4 * g + e];
+                        s[n][4 * g + e] = (ST == kF16 ? y * 0.00390625f : y) * (dp[n][4 * g + e] + x[e]);
+                    }
+                }
+                w[n].set(s[n]);
+            }
+            mma_col<ST, ND, NB, true>(at.col, 0, w, dk);
+        }
+    };
+    for (int t = 0, ti = ilo; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
         wait_vm<0>();
         __syncthreads();
         if (t + 1 < nt) fetch(t + 1);
-        const int i0 = ilo + t % nt1 * 32;
-        const unsigned char* const qs = smem + (t & 1) * STAGE;
-        const unsigned char* const ds_ = qs + Tile::BYTES;
-        const float* const stats = (const float*)(qs + 2 * Tile::BYTES);
-        f32x16 s, dp;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 x = *(const f32x4*)(stats + 2 * (8 * g + 4 * h)), y = *(const f32x4*)(stats + 2 * (8 * g + 4 * h) + 4);
-            s[4 * g] = x[0], s[4 * g + 1] = x[2], s[4 * g + 2] = y[0], s[4 * g + 3] = y[2];
-            dp[4 * g] = x[1], dp[4 * g + 1] = x[3], dp[4 * g + 2] = y[1], dp[4 * g + 3] = y[3];
+#pragma unroll 1
+        for (int sub = 0; sub < QT / 32; ++sub) {
+            const int i0 = ti + 32 * sub;
+            const bool sure = (!a.causal || (jw + WKEYS - 1 <= keys.first + i0 && (!a.window || jw > keys.first + i0 + 31 - a.window))) &&
+                              (!a.cols || jw + WKEYS <= keys.first) && i0 < ihi;
+            body(!sure, t, sub, i0);
         }
-#pragma unroll
-        for (int st = 0; st < G::STEPS; ++st) s = mma_row<ST>(frag_row<ST, ND>(qs, lane & 31, st, h), k[st], s);
-#pragma unroll
-        for (int st = 0; st < G::STEPS; ++st) dp = mma_row<ST>(frag_row<ST, ND>(ds_, lane & 31, st, h), v[st], dp);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            s[e] = ST == kF16 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c, kShift)) : __builtin_amdgcn_exp2f(s[e] * a.c);
-        const bool sure = (!a.causal || (jw + 31 <= keys.first + i0 && (!a.window || jw > keys.first + i0 + 31 - a.window))) &&
-                          (!a.cols || jw + 32 <= keys.first);
-        if (!sure) {
-            const unsigned bits = !a.cols || col < 0 ? ~0u : line ? bits_at(line, a.words_t, i0) : 0u;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int c = row_of(e, h), i = i0 + c;
-                s[e] = i >= qlo && i < qhi && (bits >> c & 1) ? s[e] : 0.f;
-            }
-        }
-        Weights<ST> w;
-        w.set(s);
-        mma_col<ST, ND>(ds_, 0, w, dv, lane);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = ST == kF16 ? s[e] * 0.00390625f * dp[e] : s[e] * dp[e];
-        w.set(s);
-        mma_col<ST, ND>(qs, 0, w, dk, lane);
     }
-    if (!live)
+    __syncthreads();
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) dk[dt] = dv[dt] = f32x16{};
-    if (a.dk.p) store_kept<ST, ND>(a.dk, b, j, hk, a.d, dk, a.scale, h, exists, a.flag);
-    if (a.dv.p) store_kept<ST, ND>(a.dv, b, j, hk, a.d, dv, ST == kF16 ? 0.00390625f : 1.f, h, exists, a.flag);
+    for (int n = 0; n < NB; ++n) {
+        const int j = jw + 32 * n + (lane & 31);
+        const bool exists = j < k1;
+        // (what a key past the sequence's end was given is dropped)
+        if (j >= keys.len)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dk[n][dt] = dv[n][dt] = f32x16{};
+        auto where = [&](const AttnTensor& t) {
+            return [&, t](int x) -> const void* { return jw + 32 * n + x < k1 ? row_at<ST>(t, b, jw + 32 * n + x, hk) : nullptr; };
+        };
+        if (DK && a.dk.p) store_kept<ST, ND>(dk[n], a.scale, a.d, a.dk.vec, exists, where(a.dk), own, lane, a.flag);
+        if (DV && a.dv.p) store_kept<ST, ND>(dv[n], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), own, lane, a.flag);
+    }
 }
 
 // ---- launches -----------------------------------------------------------------------------
@@ -769,13 +982,33 @@ hipError_t fwd(const AttnArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int ST, int ND, int NB>
+void dq_launch(const AttnArgs& a, hipStream_t s) {
+    attn_dq_kernel<ST, ND, NB><<<(unsigned)((long long)((a.tq + 128 * NB - 1) / (128 * NB)) * a.batch * a.heads), 256, 0, s>>>(a);
+}
+template <int ST, int ND, int NB, int QT, bool DK, bool DV, bool VL, int OCC>
+void dkv_launch(const AttnArgs& a, hipStream_t s) {
+    attn_dkv_kernel<ST, ND, NB, QT, DK, DV, VL, OCC><<<(unsigned)((long long)((a.tk + 128 * NB - 1) / (128 * NB)) * a.batch * a.kv), 256, 0, s>>>(a);
+}
+
 template <int ST, int ND>
 hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     const long long all = (long long)a.batch * a.heads * a.tq;
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
-    if (a.dq.p && all) attn_dq_kernel<ST, ND><<<(unsigned)((a.tq + kAttnTile - 1) / kAttnTile * a.batch * a.heads), 256, 0, s>>>(a);
-    if ((a.dk.p || a.dv.p) && a.batch && a.tk)
-        attn_dkv_kernel<ST, ND><<<(unsigned)((a.tk + kAttnTile - 1) / kAttnTile * a.batch * a.kv), 256, 0, s>>>(a);
+    if (a.dq.p && all) dq_launch<ST, ND, 1>(a, s);
+    if ((a.dk.p || a.dv.p) && a.batch && a.tk) {
+        if constexpr (ND == 8) {
+            // (both sums of 256 elements and both kept rows do not fit the registers)
+            if (a.dk.p) dkv_launch<ST, ND, 1, 32, true, false, false, 1>(a, s);
+            if (a.dv.p) dkv_launch<ST, ND, 1, 32, false, true, false, 1>(a, s);
+        } else if constexpr (ST == kF32) {
+            dkv_launch<ST, ND, 1, ND == 4 ? 32 : 64, true, true, false, ND == 4 ? 1 : 2>(a, s);
+        } else if constexpr (ND == 4) {
+            dkv_launch<ST, ND, 1, 32, true, true, true, 2>(a, s);
+        } else {
+            dkv_launch<ST, ND, 1, 64, true, true, false, 2>(a, s);
+        }
+    }
     return hipGetLastError();
 }
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import sys
 
 import numpy as np
@@ -58,31 +59,6 @@ class LossArgs(ctypes.Structure):
                 ("top", ctypes.c_int64), ("tied", ctypes.c_int32), ("temperature", ctypes.c_double)] + [
                     (n, ctypes.c_void_p) for n in ("x", "w", "index", "teacher", "loss", "lse", "mean", "ct", "dx", "dw", "flag", "work")] + [
                         ("work_bytes", ctypes.c_size_t)]
-
-
-class Heads(ctypes.Structure):
-    """presk_hip_heads."""
-    _fields_ = [("p", ctypes.c_void_p), ("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("head", ctypes.c_int64)]
-
-
-class AttnArgs(ctypes.Structure):
-    """presk_hip_attn."""
-    _fields_ = [("dtype", ctypes.c_char_p)] + [
-        (n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_len", "k_len", "head_dim", "window", "mask_cols")] + [
-            ("causal", ctypes.c_int32), ("scale", ctypes.c_double)] + [
-                (n, Heads) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] + [
-                    (n, ctypes.c_void_p) for n in ("lse", "lens", "first", "mask")] + [
-                        ("mask_batch", ctypes.c_int64), ("mask_row", ctypes.c_int64), ("flag", ctypes.c_void_p), ("work", ctypes.c_void_p),
-                        ("work_bytes", ctypes.c_size_t)]
-
-
-class RotArgs(ctypes.Structure):
-    """presk_hip_rot."""
-    _fields_ = [("dtype", ctypes.c_char_p)] + [
-        (n, ctypes.c_int64) for n in ("batch", "seq", "heads", "kv_heads", "head_dim", "rotary")] + [
-            ("norm", ctypes.c_int32), ("even", ctypes.c_int32), ("eps", ctypes.c_double)] + [
-                (n, Heads) for n in ("q", "k", "yq", "yk", "dyq", "dyk", "dq", "dk")] + [
-                    (n, ctypes.c_void_p) for n in ("freq", "at", "gq", "gk", "dgq", "dgk", "flag", "work")] + [("work_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -137,11 +113,10 @@ def lib():
         L.presk_hip_distill.argtypes = [la, i32, vp]
         L.presk_hip_batch_add_head_loss.argtypes = [vp, la, i32]
         L.presk_hip_batch_add_distill.argtypes = [vp, la, i32]
-        for name, args in (("attention", AttnArgs), ("head_rotary", RotArgs)):
-            pa = ctypes.POINTER(args)
-            getattr(L, f"presk_hip_{name}_workspace").argtypes = [pa, i32, ctypes.POINTER(ctypes.c_size_t)]
-            getattr(L, f"presk_hip_{name}").argtypes = [pa, i32, vp]
-            getattr(L, f"presk_hip_batch_add_{name}").argtypes = [vp, pa, i32]
+        for name in ("attention", "head_rotary"):
+            getattr(L, f"presk_hip_{name}_workspace").argtypes = [vp, i32, ctypes.POINTER(ctypes.c_size_t)]
+            getattr(L, f"presk_hip_{name}").argtypes = [vp, i32, vp]
+            getattr(L, f"presk_hip_batch_add_{name}").argtypes = [vp, vp, i32]
         _lib = L
     return _lib
 
@@ -523,8 +498,28 @@ class HeadLoss(Distill):
 # ---- a block's attention ------------------------------------------------------------
 
 
-_HEAD_AXES = {"bshd": (0, 1, 2), "bhsd": (0, 2, 1)}    # where a layout has batch, seq and head
-_NOWHERE = Heads()
+_HEADS_KINDS = {"value": 1, "vjp": 2}
+_LAYOUTS = ("bshd", "bhsd")
+# storage types' names where the C side finds them, for the process's life
+_C_NAMES = {t: ctypes.create_string_buffer(t.encode()) for t in ("f32", "bf16", "f16")}
+_NO_HEADS = (0, 0, 0, 0)
+
+
+def _c_name(dtype: str) -> int:
+    if dtype not in _C_NAMES:
+        _C_NAMES[dtype] = ctypes.create_string_buffer(str(dtype).encode())
+    return ctypes.addressof(_C_NAMES[dtype])
+
+
+@functools.lru_cache(maxsize=4096)
+def _heads_workspace(cls, fixed: tuple) -> dict:
+    """The workspaces of an operator's sizes, which are checked here."""
+    n, need = ctypes.c_size_t(), {}
+    args = cls._pack(fixed, {}, 0, 0)
+    for kind, what in _HEADS_KINDS.items():
+        check(getattr(lib(), f"presk_hip_{cls._name}_workspace")(args, what, ctypes.byref(n)))
+        need[kind] = n.value
+    return need
 
 
 class _HeadsCall:
@@ -534,56 +529,50 @@ class _HeadsCall:
     last is 1 (a slice of a packed projection, of a longer cache)."""
 
     _name: str                  # of the library's calls
-    _kinds: dict                # what a call is -> its code
     _tensors: dict              # a tensor's name -> whether it is a key's
-    _lengths: tuple             # of queries and keys
 
-    def _init(self, layout: str):
-        if layout not in _HEAD_AXES:
-            raise ValueError(f"a layout {layout!r}, not one of {', '.join(_HEAD_AXES)}")
+    def _init(self, layout: str, fixed: tuple, lengths: tuple):
+        if layout not in _LAYOUTS:
+            raise ValueError(f"a layout {layout!r}, not one of {', '.join(_LAYOUTS)}")
         self.layout = layout
+        self._fixed = fixed
+        self._need = _heads_workspace(type(self), fixed)
         self._works = {}        # device and stream -> the workspaces taken for it, the largest last
-        self._need = {}         # kind -> bytes of workspace
-        n = ctypes.c_size_t()
-        for kind, what in self._kinds.items():
-            check(getattr(lib(), f"presk_hip_{self._name}_workspace")(ctypes.byref(self._args()), what, ctypes.byref(n)))
-            self._need[kind] = n.value
+        b, d, rows_first = self.batch, self.head_dim, layout == "bshd"
+        # of queries and of keys: a tensor's axes, and a dense one's strides
+        self._specs = []
+        for s, h in ((lengths[0], self.heads), (lengths[1], self.kv_heads)):
+            self._specs.append(((b, s, h, d), s * h * d, h * d, d) if rows_first else ((b, h, s, d), s * h * d, d, s * d))
 
     def workspace(self, kind: str) -> int:
         """Bytes of workspace for `value` or `vjp`."""
         return self._need[kind]
 
-    def _shape(self, name: str) -> tuple:
-        """(batch, seq, heads, head_dim) of a tensor."""
-        k = self._tensors[name]
-        return (self.batch, self._lengths[k], self.kv_heads if k else self.heads, self.head_dim)
-
     def elements(self, name: str) -> int:
-        b, s, h, d = self._shape(name)
-        return b * s * h * d
+        """The element count of a tensor."""
+        return self.batch * self._specs[self._tensors[name]][1]
 
-    def _heads(self, name: str, t, device) -> Heads:
-        if t is None:
-            return _NOWHERE
-        shape = self._shape(name)
-        ab, as_, ah = _HEAD_AXES[self.layout]
+    def _heads(self, name: str, t, device) -> tuple:
+        """(address, strides of batch, row and head) of a tensor that is checked here."""
+        shape, *strides = self._specs[self._tensors[name]]
         if not hasattr(t, "data_ptr"):
             need = self.elements(name) * STORAGE_BYTES[self.dtype]
             if t.nbytes < need:
                 raise ValueError(f"{name} has {t.nbytes} bytes, {need} needed")
-            b, s, h, d = shape
-            return Heads(t.ptr, s * h * d, h * d if self.layout == "bshd" else d, d if self.layout == "bshd" else s * d)
-        at = _place(name, t, device)
-        have = _type_name(t)
-        if have != self.dtype:
+            return (t.ptr, *strides)
+        at = t.get_device()
+        if at < 0:
+            raise ValueError(f"{name} is not in device memory")
+        if at != device and device not in (None, -1):
+            raise ValueError(f"{name} is on device {at}, not {device}")
+        if (have := _type_name(t)) != self.dtype:
             raise ValueError(f"{name} is {have}, not {self.dtype}")
-        want = (shape[0], shape[1], shape[2], shape[3]) if self.layout == "bshd" else (shape[0], shape[2], shape[1], shape[3])
-        if tuple(t.shape) != want:
-            raise ValueError(f"{name} is {list(t.shape)}, not {list(want)}")
-        st = t.stride()
-        if st[3] != 1 and shape[3] > 1 and t.numel():
+        if t.shape != shape:
+            raise ValueError(f"{name} is {list(t.shape)}, not {list(shape)}")
+        sb, s1, s2, one = t.stride()
+        if one != 1 and self.head_dim > 1 and t.numel():
             raise ValueError(f"{name}'s heads are not contiguous")
-        return Heads(at, st[ab], st[as_], st[ah])
+        return (t.data_ptr(), sb, s1, s2) if self.layout == "bshd" else (t.data_ptr(), sb, s2, s1)
 
     def _own_work(self, need: int, device, stream):
         own = self._works.setdefault((device, getattr(stream, "value", stream) or 0), [])
@@ -591,21 +580,16 @@ class _HeadsCall:
             own.append(DeviceBuffer(need))
         return own[-1]
 
-    def args(self, kind: str, work=None, stream=None, device=None, **bufs):
-        """The arguments of a call on `stream`, each buffer checked against its
+    def args(self, kind: str, work=None, stream=None, device=None, **bufs) -> bytes:
+        """The C call's arguments on `stream`, each buffer checked against its
         size and `device` (the one initialised)."""
         device = _initialized if device is None else device
         if work is None and self._works_for(kind):
             work = self._own_work(self._need[kind], device, stream)
-        a = self._args()
-        for name, b in bufs.items():
-            if name in self._tensors:
-                setattr(a, "dout" if name == "do" else name, self._heads(name, b, device))
-            elif b is not None:
-                self._other(a, name, b, device)
-        if work is not None:
-            a.work, a.work_bytes = _buffer("work", work, device, self._need[kind]), work.nbytes
-        return a
+        got = {n: self._heads(n, b, device) if n in self._tensors else self._other(n, b, device) for n, b in bufs.items() if b is not None}
+        if work is None:
+            return self._pack(self._fixed, got, 0, 0)
+        return self._pack(self._fixed, got, _buffer("work", work, device, self._need[kind]), work.nbytes)
 
     def _works_for(self, kind: str) -> bool:
         return True
@@ -613,17 +597,7 @@ class _HeadsCall:
     def _call(self, kind, stream, **bufs):
         device, stream = _place_of(bufs.values(), stream)
         a = self.args(kind, stream=stream, device=device, **bufs)
-        check(getattr(lib(), "presk_hip_" + self._name)(ctypes.byref(a), self._kinds[kind], stream))
-
-
-def _place(name: str, t, device) -> int:
-    """The address of a tensor of another library, which is on `device`."""
-    at = t.get_device()
-    if at < 0:
-        raise ValueError(f"{name} is not in device memory")
-    if at != device and device not in (None, -1):
-        raise ValueError(f"{name} is on device {at}, not {device}")
-    return t.data_ptr()
+        check(self._launch(lib())(a, _HEADS_KINDS[kind], stream))
 
 
 def _type_name(t) -> str:
@@ -656,7 +630,10 @@ class Attention(_HeadsCall):
     this object keeps for the call's stream: calls that share a workspace, their
     captured graphs among them, run one after another."""
 
-    _name, _kinds = "attention", {"value": 1, "vjp": 2}
+    _name = "attention"
+    _launch = staticmethod(lambda lib: lib.presk_hip_attention)
+    # presk_hip_attn
+    _struct = struct.Struct("@P8qid" + "Pqqq" * 8 + "4P2qPPN")
     _tensors = {"q": False, "k": True, "v": True, "o": False, "do": False, "dq": False, "dk": True, "dv": True}
 
     def __init__(self, dtype: str, batch: int, heads: int, kv_heads: int, q_len: int, k_len: int, head_dim: int, causal: bool = False,
@@ -665,27 +642,33 @@ class Attention(_HeadsCall):
         self.q_len, self.k_len, self.head_dim = int(q_len), int(k_len), int(head_dim)
         self.causal, self.window, self.mask_cols = bool(causal), int(window), int(mask_cols)
         self.scale = float(scale) if scale is not None else max(self.head_dim, 1) ** -0.5
-        self._lengths = (self.q_len, self.k_len)
-        self._init(layout)
+        self._init(layout, (self.dtype, self.batch, self.heads, self.kv_heads, self.q_len, self.k_len, self.head_dim, self.window,
+                            self.mask_cols, self.causal, self.scale), (self.q_len, self.k_len))
+        rows = 4 * self.batch * self.heads * self.q_len
+        self._others = {"lse": (rows, "f32"), "lens": (8 * self.batch, "i64"), "first": (8 * self.batch, "i64"), "flag": (4, None)}
 
-    def _args(self) -> AttnArgs:
-        return AttnArgs(self.dtype.encode(), self.batch, self.heads, self.kv_heads, self.q_len, self.k_len, self.head_dim, self.window,
-                        self.mask_cols, self.causal, self.scale)
+    @classmethod
+    def _pack(cls, fixed, got, work, work_bytes) -> bytes:
+        g = got.get
+        h = [x for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for x in g(n, _NO_HEADS)]
+        return cls._struct.pack(_c_name(fixed[0]), *fixed[1:], *h, g("lse", 0), g("lens", 0), g("first", 0), *g("mask", (0, 0, 0)),
+                                g("flag", 0), work, work_bytes)
 
-    def _other(self, a, name, b, device):
-        if name == "mask":
-            if not self.mask_cols:
-                raise ValueError("a mask of no columns (mask_cols)")
-            a.mask, a.mask_batch, a.mask_row = self._mask(b, device)
-            return
-        n, ty = {"lse": (4 * self.batch * self.heads * self.q_len, "f32"), "lens": (8 * self.batch, "i64"), "first": (8 * self.batch, "i64"),
-                 "flag": (4, None)}[name]
-        setattr(a, name, _buffer(name, b, device, n, ty))
+    def _other(self, name, b, device):
+        if name != "mask":
+            return _buffer(name, b, device, *self._others[name])
+        if not self.mask_cols:
+            raise ValueError("a mask of no columns (mask_cols)")
+        return self._mask(b, device)
 
     def _mask(self, m, device) -> tuple:
         if not hasattr(m, "data_ptr"):
             return _buffer("mask", m, device, self.batch * self.q_len * self.mask_cols), self.q_len * self.mask_cols, self.mask_cols
-        at = _place("mask", m, device)
+        at = m.get_device()
+        if at < 0:
+            raise ValueError("mask is not in device memory")
+        if at != device and device not in (None, -1):
+            raise ValueError(f"mask is on device {at}, not {device}")
         if str(m.dtype) not in ("torch.bool", "torch.uint8"):
             raise ValueError(f"mask is {m.dtype}, not bool or uint8")
         want = (self.q_len, self.mask_cols)
@@ -694,7 +677,7 @@ class Attention(_HeadsCall):
         st = m.stride()
         if st[-1] != 1 and self.mask_cols > 1 and m.numel():
             raise ValueError("mask's rows are not contiguous")
-        return at, st[0] if m.ndim == 3 else 0, st[-2]
+        return m.data_ptr(), st[0] if m.ndim == 3 else 0, st[-2]
 
     def value(self, q, k, v, o, lse=None, lens=None, first=None, mask=None, flag=None, work=None, stream=None):
         self._call("value", stream, q=q, k=k, v=v, o=o, lse=lse, lens=lens, first=first, mask=mask, flag=flag, work=work)
@@ -724,7 +707,10 @@ class HeadRotary(_HeadsCall):
     and those of dgq and dgk that are given.  Buffers, streams and `work` as
     Attention's; only a gradient with `norm` needs any workspace."""
 
-    _name, _kinds = "head_rotary", {"value": 1, "vjp": 2}
+    _name = "head_rotary"
+    _launch = staticmethod(lambda lib: lib.presk_hip_head_rotary)
+    # presk_hip_rot
+    _struct = struct.Struct("@P6qiid" + "Pqqq" * 8 + "8PN")
     _tensors = {"q": False, "k": True, "yq": False, "yk": True, "dyq": False, "dyk": True, "dq": False, "dk": True}
 
     def __init__(self, dtype: str, batch: int, seq: int, heads: int, kv_heads: int, head_dim: int, rotary: int | None = None,
@@ -734,18 +720,21 @@ class HeadRotary(_HeadsCall):
         self.dtype, self.batch, self.seq, self.heads, self.kv_heads = dtype, int(batch), int(seq), int(heads), int(kv_heads)
         self.head_dim, self.rotary = int(head_dim), int(head_dim if rotary is None else rotary)
         self.norm, self.eps, self.pairs = bool(norm), float(eps), pairs
-        self._lengths = (self.seq, self.seq)
-        self._init(layout)
+        self._init(layout, (self.dtype, self.batch, self.seq, self.heads, self.kv_heads, self.head_dim, self.rotary, self.norm,
+                            self.pairs == "even", self.eps), (self.seq, self.seq))
+        gain = (self.head_dim * STORAGE_BYTES[self.dtype], self.dtype)
+        self._others = {"freq": (4 * self.rotary, "f64"), "at": (8 * self.batch * self.seq, "i64"), "flag": (4, None),
+                        "gq": gain, "gk": gain, "dgq": gain, "dgk": gain}
 
-    def _args(self) -> RotArgs:
-        return RotArgs(self.dtype.encode(), self.batch, self.seq, self.heads, self.kv_heads, self.head_dim, self.rotary, self.norm,
-                       self.pairs == "even", self.eps)
+    @classmethod
+    def _pack(cls, fixed, got, work, work_bytes) -> bytes:
+        g = got.get
+        h = [x for n in ("q", "k", "yq", "yk", "dyq", "dyk", "dq", "dk") for x in g(n, _NO_HEADS)]
+        return cls._struct.pack(_c_name(fixed[0]), *fixed[1:], *h, *(g(n, 0) for n in ("freq", "at", "gq", "gk", "dgq", "dgk", "flag")),
+                                work, work_bytes)
 
-    def _other(self, a, name, b, device):
-        g = (self.head_dim * STORAGE_BYTES[self.dtype], self.dtype)
-        n, ty = {"freq": (4 * self.rotary, "f64"), "at": (8 * self.batch * self.seq, "i64"), "flag": (4, None), "gq": g, "gk": g, "dgq": g,
-                 "dgk": g}[name]
-        setattr(a, name, _buffer(name, b, device, n, ty))
+    def _other(self, name, b, device):
+        return _buffer(name, b, device, *self._others[name])
 
     def _works_for(self, kind: str) -> bool:
         return self.norm and kind == "vjp"
