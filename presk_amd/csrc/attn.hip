@@ -20,53 +20,66 @@ int storage_code(const char* name) {
 
 long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
-// A row's bits and a column's, 32 of a byte mask a thread.
+// 4 bytes' truth as 4 bits.
+__device__ __forceinline__ unsigned truths(unsigned v) {
+    return ((((v & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v) >> 7 & 0x01010101u) * 0x01020408u >> 24;
+}
+
+// A byte mask's bits by rows and by columns, and which of its blocks of 32 x 32
+// hold any: a wave takes 32 rows and 64 columns, a lane 32 columns of a row, from
+// which a column's bits are a vote.  Reads each byte once (2 x 1024 x 1024 8 us).
 __global__ void __launch_bounds__(256) attn_mask_kernel(AttnMask m) {
-    const long long n = (long long)m.nbatch * m.tq * m.words, t = (long long)m.nbatch * m.cols * m.words_t;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at < n) {
-        const int w = (int)(at % m.words);
-        const long long line = at / m.words, b = line / m.tq, i = line - b * m.tq;
+    const int lane = threadIdx.x & 63, blocks = (m.tq + 31) / 32, pairs = (m.words + 1) / 2;
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= (long long)m.nbatch * blocks * pairs) return;
+    const int w = 2 * (int)(unit % pairs) + (lane >> 5);
+    const long long line = unit / pairs, b = line / blocks;
+    const int rb = (int)(line - b * blocks), i = 32 * rb + (lane & 31);
+    unsigned bits = 0;
+    if (i < m.tq && w < m.words) {
         const unsigned char* const src = m.mask + b * m.batch + i * m.row + 32LL * w;
         const int left = m.cols - 32 * w < 32 ? m.cols - 32 * w : 32;
-        unsigned bits = 0;
         if (left == 32 && ((uintptr_t)src & 3) == 0) {
+            unsigned v[8];
+            if (((uintptr_t)src & 15) == 0) {
+                *(uint4*)v = ((const uint4*)src)[0];
+                *(uint4*)(v + 4) = ((const uint4*)src)[1];
+            } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const unsigned v = ((const unsigned*)src)[q];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bits |= (v >> (8 * e) & 0xff ? 1u : 0u) << (4 * q + e);
+                for (int q = 0; q < 8; ++q) v[q] = ((const unsigned*)src)[q];
             }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) bits |= truths(v[q]) << (4 * q);
         } else {
             for (int e = 0; e < left; ++e) bits |= (src[e] ? 1u : 0u) << e;
         }
-        m.bits[at] = bits;
-    } else if (m.bits_t && at - n < t) {
-        // columns innermost, so that a wave reads a row's bytes beside each other
-        const long long k = at - n;
-        const int c = (int)(k % m.cols);
-        const long long line = k / m.cols, b = line / m.words_t;
-        const int w = (int)(line - b * m.words_t);
-        const unsigned char* const src = m.mask + b * m.batch + 32LL * w * m.row + c;
-        const int left = m.tq - 32 * w < 32 ? m.tq - 32 * w : 32;
-        unsigned bits = 0;
-        for (int e = 0; e < left; ++e) bits |= (src[e * m.row] ? 1u : 0u) << e;
-        m.bits_t[(b * m.cols + c) * m.words_t + w] = bits;
+        m.bits[(b * m.tq + i) * m.words + w] = bits;
     }
+    const unsigned long long any = __ballot(bits != 0);
+    if ((lane & 31) == 0 && w < m.words) m.any[line * m.words + w] = (unsigned)(any >> lane) != 0;
+    if (!m.bits_t) return;
+    unsigned col = 0;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+        const unsigned long long set = __ballot(bits >> c & 1);
+        if ((lane & 31) == c) col = (unsigned)(set >> (lane & 32));
+    }
+    const int c = 32 * w + (lane & 31);
+    if (c < m.cols) m.bits_t[(b * m.cols + c) * m.words_t + rb] = col;
 }
 
 // What a checked call launches.
 struct Plan {
-    int st, nd, pack = 1, splits = 1;
+    int st, nd, pack = 1, splits = 1, chunk = 0;
     int words = 0, words_t = 0, nbits = 0;
-    size_t bits = 0, bits_t = 0, part = 0, ml = 0, rows = 0, total = 0;     // offsets in the workspace
+    size_t bits = 0, bits_t = 0, any = 0, part = 0, ml = 0, rows = 0, total = 0;     // offsets in the workspace
 };
 
-// Splits of the keys: as many shares as fill two workgroups a CU, of two tiles
-// at least.
-int splits_of(long long items, long long tk) {
-    if (items <= 0 || items >= 256) return 1;
-    return (int)std::max<long long>(1, std::min<long long>({512 / items, tk / 128, 64}));
+// Keys a split of `items` workgroups' ranges: as many splits as come to `want`
+// workgroups, of `least` keys at least.
+int chunk_of(long long items, long long tk, long long want, long long least) {
+    const long long splits = std::max<long long>(1, want / std::max<long long>(items, 1));
+    return (int)std::min<long long>(up(std::max<long long>((tk + splits - 1) / splits, least), 128), 1 << 28);
 }
 
 Plan plan_of(const presk_hip_attn& a, int what) {
@@ -87,6 +100,7 @@ Plan plan_of(const presk_hip_attn& a, int what) {
         p.words_t = (int)up(a.q_len, 32) / 32;
         p.bits = take(4 * a.batch * a.q_len * p.words);
         if (grad) p.bits_t = take(4 * a.batch * a.mask_cols * p.words_t);
+        p.any = take(a.batch * p.words_t * p.words);
     }
     if (grad) {
         p.rows = take(8 * all);
@@ -94,8 +108,10 @@ Plan plan_of(const presk_hip_attn& a, int what) {
     }
     const long long per = a.heads / a.kv_heads;
     if (a.q_len < kAttnTile) p.pack = (int)per;
-    const long long items = up(a.q_len * p.pack, kAttnTile) / kAttnTile * a.batch * (a.heads / p.pack);
-    p.splits = splits_of(items, a.k_len);
+    const long long rows = a.q_len * p.pack, units = a.batch * (a.heads / p.pack);
+    if (rows <= kAttnFew) p.chunk = chunk_of(units, a.k_len, 1024, 256);
+    else if (up(rows, kAttnTile) / kAttnTile * units < 128) p.chunk = chunk_of(up(rows, kAttnTile) / kAttnTile * units, a.k_len, 512, 256);
+    p.splits = p.chunk ? (int)std::max<long long>(1, (a.k_len + p.chunk - 1) / p.chunk) : 1;
     if (p.splits > 1) {
         p.part = take(4 * all * p.splits * p.nd * 32);
         p.ml = take(8 * all * p.splits);
@@ -156,7 +172,7 @@ std::string attn_check(const presk_hip_attn& a, int what) {
     // workgroups of a launch
     const int64_t most = std::max(a.heads * (up(a.q_len, 16) / 16), a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile));
     if (a.batch * most >= 1ll << 31) return no("batch * heads * length past what a launch holds");
-    if (a.mask_cols && a.batch * std::max(a.q_len * (up(a.mask_cols, 32) / 32), a.mask_cols * (up(a.q_len, 32) / 32)) >= 1ll << 38)
+    if (a.mask_cols && a.batch * up(a.q_len, 32) * (up(a.mask_cols, 64) / 32) >= 1ll << 31)
         return no("a mask past what a launch holds");
     return "";
 }
@@ -222,6 +238,7 @@ hipError_t attn_run(const presk_hip_attn& a, int what, hipStream_t s) {
     g.flag = a.flag;
     g.pack = p.pack;
     g.splits = p.splits;
+    g.chunk = p.chunk;
     g.part = (float*)(work + p.part);
     g.part_ml = (float*)(work + p.ml);
     g.rows = (float*)(work + p.rows);
@@ -229,12 +246,13 @@ hipError_t attn_run(const presk_hip_attn& a, int what, hipStream_t s) {
         const bool grad = what == PRESK_HIP_ATTN_GRAD;
         const int nb = a.mask_batch || a.batch == 1 ? (int)a.batch : 1;
         AttnMask m{a.mask, a.mask_batch, a.mask_row, nb, g.tq, g.cols, p.words, p.words_t, (unsigned*)(work + p.bits),
-                   grad ? (unsigned*)(work + p.bits_t) : nullptr};
-        const long long n = (long long)nb * g.tq * m.words + (grad ? (long long)nb * g.cols * m.words_t : 0);
-        attn_mask_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(m);
+                   grad ? (unsigned*)(work + p.bits_t) : nullptr, (unsigned char*)(work + p.any)};
+        const long long n = (long long)nb * p.words_t * ((p.words + 1) / 2);
+        attn_mask_kernel<<<(unsigned)((n + 3) / 4), 256, 0, s>>>(m);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         g.bits = m.bits;
         g.bits_t = m.bits_t;
+        g.any = a.mask_cols > 64 ? m.any : nullptr;     // (the few columns of a tree are one tile anyway)
         g.words = m.words;
         g.words_t = m.words_t;
         g.bits_batch = nb > 1 ? g.tq : 0;

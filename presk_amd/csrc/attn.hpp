@@ -50,11 +50,12 @@ struct AttnArgs {
     const unsigned *bits, *bits_t;
     int words, words_t;
     long long bits_batch, bits_t_batch;   // rows (columns) from one sequence's to the next one's (0: shared)
+    const unsigned char* any;    // [sequences][blocks of 32 rows][words]: whether 32 x 32 of the mask hold any; null: few columns
     float c, scale;              // scale log2 e, scale
     unsigned* flag;
     // the few rows' form: `pack` heads of a group stand beside each other as
     // rows; the keys are cut into `splits`, whose sums are joined after
-    int pack, splits;
+    int pack, splits, chunk;     // `chunk` keys a split
     float *part, *part_ml;       // [split][batch][heads][tq][ND * 32] and [split][batch][heads][tq]{max, sum}
     // what the backward pass needs of a row: -lse log2 e and -sum do o
     float* rows;                 // [2][batch][heads][tq]
@@ -66,9 +67,11 @@ struct AttnMask {
     long long batch, row;
     int nbatch, tq, cols, words, words_t;
     unsigned *bits, *bits_t;     // bits_t null: not wanted
+    unsigned char* any;
 };
 
 constexpr int kAttnTile = 128;   // rows of a workgroup
+constexpr int kAttnFew = 32;     // rows that are one block of a wave
 
 // nd: 32-wide pieces of a head, 2, 4 or (16-bit) 8
 hipError_t attn_fwd_f32(const AttnArgs& a, int nd, hipStream_t s);

@@ -76,6 +76,15 @@ struct Weights {
         }
     }
 };
+// What that rounding left of p, in its place.
+template <int ST>
+__device__ __forceinline__ void left_in(f32x16& p, const Weights<ST>& w) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const unsigned short u = w.w[e >> 3][e & 7];
+        p[e] = left_of(p[e], ST == kBF16 ? pk_bf16_to_f32(u) : pk_f16_to_f32(u));
+    }
+}
 template <>
 struct Weights<kF32> {
     f32x16 w;
@@ -377,6 +386,44 @@ struct Keys {
     }
 };
 
+// Whether the cotangents of the weights of queries i0 .. i1 enter their products
+// in two parts, the rounding to 16 bits and what it left: where one of them reads
+// fewer than 64 keys (or a mask says which).  Such rows have the largest
+// gradients, and theirs are the errors of the stored output too; together with
+// the rounding of the weights' cotangents these pass what the gradients' own
+// rounding adds (documents of 256 tokens in bf16, 1.53 times a float32
+// computation's error, so 1.2).
+template <int ST>
+__device__ __forceinline__ bool fine_of(const AttnArgs& a, const Keys& keys, int i0, int i1) {
+    return ST != kF32 && (a.cols || keys.hi(a, i0) - keys.lo(a, i0) < 64 || keys.hi(a, i1) - keys.lo(a, i1) < 64);
+}
+
+// The first and past the last set of `n` flags of 0 or not, `stride` apart, in lines
+// l0 .. l1 `line` apart; (n, 0) where none is.  By a wave.
+__device__ __forceinline__ void flagged(const unsigned char* f, int n, long long stride, int l0, int l1, long long line, int* lo, int* hi) {
+    const int lane = threadIdx.x & 63;
+    *lo = n, *hi = 0;
+    for (int w = 0; w < n; w += 64) {
+        int any = 0;
+        if (w + lane < n)
+            for (int l = l0; l <= l1; ++l) any |= f[(w + lane) * stride + l * line];
+        const unsigned long long set = __ballot(any);
+        if (!set) continue;
+        if (*hi == 0) *lo = w + __builtin_ctzll(set);
+        *hi = w + 64 - __builtin_clzll(set);
+    }
+}
+// A mask's part of the keys [lo, hi) that the queries i0 .. i1 read.
+__device__ __forceinline__ void by_mask(const AttnArgs& a, const Keys& keys, int b, int i0, int i1, int* lo, int* hi) {
+    if (!a.any) return;
+    const int blocks = (a.tq + 31) / 32;
+    int w0, w1;
+    flagged(a.any + (a.bits_batch ? (long long)b * blocks * a.words : 0), a.words, 1, i0 / 32, i1 / 32, a.words, &w0, &w1);
+    const int end = w1 ? keys.first + 32 * w1 : keys.first, from = keys.first + 32 * w0;
+    if (end < *hi) *hi = end;
+    if (keys.first <= 0 && from > *lo) *lo = from;
+}
+
 // 32 bits of a mask's line from `rel` on: ones before it, zeros past it.
 __device__ __forceinline__ unsigned bits_at(const unsigned* line, int words, int rel) {
     if (rel <= -32) return ~0u;
@@ -401,6 +448,14 @@ __device__ __forceinline__ float where_bit(unsigned bits, int e, float x, float 
 __device__ __forceinline__ unsigned item_of(unsigned id, unsigned total) {
     const unsigned xcd = id % 8, q8 = total / 8, r8 = total % 8;
     return xcd * q8 + (xcd < r8 ? xcd : r8) + id / 8;
+}
+
+// Split `split` of the keys [lo, hi): `chunk` of them, the same for sequences of
+// any length, so that its workgroups take equally long or have nothing to do.
+__device__ __forceinline__ void cut(const AttnArgs& a, int split, int* lo, int* hi) {
+    const long long from = *lo + (long long)split * a.chunk, to = from + a.chunk;
+    *hi = to < *hi ? (int)to : *hi;
+    *lo = from < *hi ? (int)from : *hi;
 }
 
 // ---- the value ----------------------------------------------------------------------
@@ -428,14 +483,12 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
     keys.init(a, b);
     const int ifirst = r0 / a.pack, ilast = r1 / a.pack;
     int klo = keys.lo(a, ifirst), khi = keys.hi(a, ilast);
+    by_mask(a, keys, b, ifirst, ilast, &klo, &khi);
     const int surelo = keys.lo(a, ilast), surehi = keys.sure(a, ifirst);
     int nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
     if (a.splits > 1) {
-        const int t0 = (int)((long long)nt * split / a.splits), t1 = (int)((long long)nt * (split + 1) / a.splits);
-        const int end = klo + t1 * G::TILE;
-        klo += t0 * G::TILE;
-        khi = end < khi ? end : khi;
-        nt = t1 - t0;
+        cut(a, split, &klo, &khi);
+        nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
     }
 
     // this lane's row
@@ -561,46 +614,215 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
     if (a.lse && live && h == 0) a.lse[row] = l == 0.f ? -INFINITY : (base_of(m) + __builtin_log2f(l)) * kLn2;
 }
 
-// The splits' sums of a row joined: 64 lanes a row, ND / 2 elements a lane.
+// The sum in place `at` of a row's (dt, row_of) as an element of the head.
 template <int ST, int ND>
+__device__ __forceinline__ bool put(void* row, int at, int d, float v) {
+    const int e = ST == kF32 ? ND * (at & 31) + (at >> 5) : at;
+    if (e >= d) return false;
+    if constexpr (ST == kF32) ((float*)row)[e] = v;
+    else if constexpr (ST == kBF16) ((unsigned short*)row)[e] = pk_f32_to_bf16(v);
+    else ((unsigned short*)row)[e] = pk_f32_to_f16(v);
+    return ST == kF16 && pk_overflows_f16(v);
+}
+
+// Few rows (a group's heads beside each other, 32 at most) over many keys: all
+// of a workgroup's NW waves have the same rows, and blocks of 32 keys in turn,
+// which each loads for itself two at a time, so that no wave waits for another
+// until their sums meet in LDS at the end.
+template <int ST, int ND, int NW>
+__global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
+    typedef Geo<ST, ND> G;
+    typedef Rows<ST, ND, 32, 64> Tile;
+    constexpr int STAGE = 2 * Tile::BYTES, WAVE = 2 * STAGE, NL = 2 * Tile::ROUNDS;
+    static_assert(ND * 4096 <= WAVE, "a wave's sums in its part of LDS");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[NW * WAVE];
+    __shared__ float ml[NW][32][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+
+    const int rows = a.tq * a.pack, groups = a.heads / a.pack;
+    const unsigned item = item_of(blockIdx.x, gridDim.x);
+    const int split = (int)(item % (unsigned)a.splits), unit = (int)(item / (unsigned)a.splits);
+    const int b = unit / groups, hx = unit % groups, hk = hx * a.pack / a.per;
+
+    Keys keys;
+    keys.init(a, b);
+    int klo = keys.lo(a, 0), khi = keys.hi(a, a.tq - 1);
+    const int surelo = keys.lo(a, a.tq - 1), surehi = keys.sure(a, 0);
+    cut(a, split, &klo, &khi);
+    const int nblk = khi > klo ? (khi - klo + 31) / 32 : 0, nt = (nblk - wave + NW - 1) / NW;
+
+    Tile kt, vt;
+    const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem + (unsigned)(wave * WAVE);
+    unsigned char* const own = smem + wave * WAVE;
+    kt.init(a.k, b, hk, a.d, lane, lds);
+    vt.init(a.v, b, hk, a.d, lane, lds + Tile::BYTES);
+    auto fetch = [&](int t) {
+        const unsigned stage = (unsigned)(t & 1) * STAGE;
+        const int k0 = klo + (t * NW + wave) * 32;
+        kt.issue(k0, khi - k0, stage, own, lane);
+        vt.issue(k0, khi - k0, stage, own + Tile::BYTES, lane);
+    };
+
+    // this lane's row
+    const int r = lane & 31;
+    const bool live = r < rows;
+    const int i = live ? r / a.pack : a.tq - 1, head = hx * a.pack + (live ? r % a.pack : 0);
+    const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
+    const unsigned* const line = a.cols ? a.bits + ((long long)b * a.bits_batch + i) * a.words : nullptr;
+    typename FragOf<ST>::T q[G::STEPS];
+    if (!a.q.vec) {
+        load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
+        __builtin_amdgcn_s_waitcnt(0xc07f);     // LDS: the reads are done before a tile lands there
+        if (nt > 0) fetch(0);
+    } else {
+        if (nt > 0) fetch(0);
+        load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
+    }
+    const bool whole = a.k.vec && a.v.vec;
+
+    f32x16 o[1][ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) o[0][dt] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+    Places<ST, ND> places;
+    places.init(lane);
+    places = places.from(lds);
+    for (int t = 0; t < nt; ++t) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);     // LDS: the last block's reads are done before its stage is loaded again
+        if (t + 1 < nt) fetch(t + 1);
+        if (t + 1 < nt && whole) wait_vm<NL>();
+        else wait_vm<0>();
+        const int k0 = klo + (t * NW + wave) * 32;
+        const Places<ST, ND> at = places.from((unsigned)(t & 1) * STAGE);
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int st = 0; st < G::STEPS; ++st) s = mma_row<ST>(frag_row<ST>(at.row, st), q[st], s);
+        if (k0 < surelo || k0 + 32 > surehi) {
+            unsigned bits = a.cols && k0 + 32 > keys.first ? bits_at(line, a.words, k0 - keys.first) : ~0u;
+            bits = (bits & range_of(rlo - k0, rhi - k0)) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = where_bit(bits, e, s[e], -INFINITY);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(mx, partner<32>(mx)) * a.c;
+        if (__any(mx > m + 8.f)) {
+            const float top = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - base_of(top));
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[0][dt][e] *= f;
+        }
+        const float base = base_of(m);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c, -base));
+            sum += s[e];
+        }
+        l += sum;
+        Weights<ST> w[1];
+        w[0].set(s);
+        mma_col<ST, ND, 1>(at.col, Tile::BYTES, w, o);
+    }
+    l += partner<32>(l);
+
+    // the waves' sums, each in the wave's own part of LDS as its lanes hold them
+    f32x4* const sums = (f32x4*)own + lane;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) sums[64 * (4 * dt + g)] = f32x4{o[0][dt][4 * g], o[0][dt][4 * g + 1], o[0][dt][4 * g + 2], o[0][dt][4 * g + 3]};
+    if (h == 0) ml[wave][r][0] = m, ml[wave][r][1] = l;
+    __syncthreads();
+    float top = -INFINITY, f[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][r][0]);
+    const float base = base_of(top);
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(ml[w][r][0] - base);
+        l += ml[w][r][1] * f[w];
+    }
+    const long long all = (long long)a.batch * a.heads * a.tq, row = ((long long)b * a.heads + head) * a.tq + i, n = split * all + row;
+    if (wave == 0 && h == 0 && live) {
+        if (a.splits > 1) *(f32x2*)(a.part_ml + 2 * n) = f32x2{top, l};
+        else if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (base + __builtin_log2f(l)) * kLn2;
+    }
+    if (a.splits > 1 && l == 0.f) return;       // (the join reads no sums of it; no barrier follows)
+    const float whole_f = l == 0.f ? 0.f : 1.f / l;
+    void* const out = live ? const_cast<void*>(row_at<ST>(a.o, b, i, head)) : nullptr;
+    bool ovf = false;
+    for (int x = wave; x < 4 * ND; x += NW) {
+        f32x4 v = f32x4{};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const f32x4 y = ((const f32x4*)(smem + w * WAVE) + lane)[64 * x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += y[e] * f[w];
+        }
+        const int at = (x >> 2) * 32 + 8 * (x & 3) + 4 * h;     // its place among a row's sums
+        if (!live) continue;
+        if (a.splits > 1) {
+            *(f32x4*)(a.part + n * (ND * 32) + at) = v;
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ovf |= put<ST, ND>(out, at + e, a.d, v[e] * whole_f);
+    }
+    if (ovf && a.flag) atomicOr(a.flag, 1u);
+}
+
+// The splits' sums of a row joined, in order: by a wave (64 lanes, ND / 2 elements a
+// lane), or, of many splits, by a workgroup's four, a quarter of them each.
+template <int ST, int ND, int WAVES>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
-    const long long all = (long long)a.batch * a.heads * a.tq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ float sums[4][ND * 32], sl[4];
+    const long long all = (long long)a.batch * a.heads * a.tq;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long row = WAVES == 4 ? blockIdx.x : (long long)blockIdx.x * 4 + wave;
     if (row >= all) return;
-    const int lane = threadIdx.x & 63;
+    const f32x2* const mls = (const f32x2*)a.part_ml + row;
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * all + row)]);
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, mls[s * all][0]);
+    m = all_of<64>(m, nullptr, max_f);
     const float base = base_of(m);
     float l = 0.f, x[ND / 2];
 #pragma unroll
     for (int q = 0; q < ND / 2; ++q) x[q] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const long long n = s * all + row;
-        const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * n);
-        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
-        l += ml[1] * f;
+#pragma unroll 4
+    for (int s = WAVES == 4 ? wave : 0; s < a.splits; s += WAVES) {
+        const f32x2 v = mls[s * all];
+        const float f = __builtin_amdgcn_exp2f(v[0] - base);
+        l += v[1] * f;
+        // (a split without keys has no sums)
 #pragma unroll
-        for (int q = 0; q < ND / 2; ++q) x[q] += a.part[n * (ND * 32) + q * 64 + lane] * f;
+        for (int q = 0; q < ND / 2; ++q) x[q] += v[1] == 0.f ? 0.f : a.part[(s * all + row) * (ND * 32) + q * 64 + lane] * f;
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
     const int i = (int)(row % a.tq), head = (int)(row / a.tq % a.heads), b = (int)(row / a.tq / a.heads);
     void* const out = const_cast<void*>(row_at<ST>(a.o, b, i, head));
     bool ovf = false;
+    if constexpr (WAVES == 4) {
 #pragma unroll
-    for (int q = 0; q < ND / 2; ++q) {
-        // (an element's place among a split's sums: attn_fwd_kernel's lanes)
-        const int at = q * 64 + lane;
-        const int e = ST == kF32 ? ND * (at & 31) + (at >> 5) : at;
-        if (e >= a.d) continue;
-        const float v = x[q] * f;
-        if constexpr (ST == kF32) ((float*)out)[e] = v;
-        else if constexpr (ST == kBF16) ((unsigned short*)out)[e] = pk_f32_to_bf16(v);
-        else {
-            ovf |= pk_overflows_f16(v);
-            ((unsigned short*)out)[e] = pk_f32_to_f16(v);
-        }
+        for (int q = 0; q < ND / 2; ++q) sums[wave][q * 64 + lane] = x[q];
+        if (lane == 0) sl[wave] = l;
+        __syncthreads();
+        l = sl[0] + sl[1] + sl[2] + sl[3];
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if constexpr (WAVES == 4) {
+        for (int at = threadIdx.x; at < ND * 32; at += 256)
+            ovf |= put<ST, ND>(out, at, a.d, (sums[0][at] + sums[1][at] + sums[2][at] + sums[3][at]) * f);
+    } else {
+#pragma unroll
+        for (int q = 0; q < ND / 2; ++q) ovf |= put<ST, ND>(out, q * 64 + lane, a.d, x[q] * f);
     }
     if (ovf && a.flag) atomicOr(a.flag, 1u);
-    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (base + __builtin_log2f(l)) * kLn2;
+    if (a.lse && (WAVES == 4 ? threadIdx.x : lane) == 0) a.lse[row] = l == 0.f ? -INFINITY : (base + __builtin_log2f(l)) * kLn2;
 }
 
 // ---- the gradients --------------------------------------------------------------------
@@ -660,7 +882,9 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
 
     Keys keys;
     keys.init(a, b);
-    const int klo = keys.lo(a, r0), khi = keys.hi(a, r1), surelo = keys.lo(a, r1), surehi = keys.sure(a, r0);
+    int klo = keys.lo(a, r0), khi = keys.hi(a, r1);
+    by_mask(a, keys, b, r0, r1, &klo, &khi);
+    const int surelo = keys.lo(a, r1), surehi = keys.sure(a, r0);
     const int nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
 
     Tile kt, vt;
@@ -677,6 +901,7 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
 
     const int w0 = r0 + wave * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
     const int wlo = keys.lo(a, w0 < r1 ? w0 : r1), whi = w0 <= r1 ? keys.hi(a, w1) : 0;
+    const bool fine = fine_of<ST>(a, keys, w0 < r1 ? w0 : r1, w1);
     typename FragOf<ST>::T q[NB][G::STEPS], dout[NB][G::STEPS];
     float lse[NB], delta[NB];
     f32x16 dq[NB][ND];
@@ -740,6 +965,15 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
             w[n].set(s[n]);
         }
         mma_col<ST, ND, NB>(at.col, 0, w, dq);
+        if constexpr (ST != kF32)
+            if (fine) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    left_in<ST>(s[n], w[n]);
+                    w[n].set(s[n]);
+                }
+                mma_col<ST, ND, NB>(at.col, 0, w, dq);
+            }
     };
     for (int t = 0; t < nt; ++t) {
         wait_vm<0>();
@@ -793,6 +1027,12 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
     };
     int ilo, ihi, wlo, whi;
     queries(k0, k1, &ilo, &ihi);
+    if (a.any && k0 >= keys.first && ihi > 0) {
+        const int blocks = (a.tq + 31) / 32, c0 = k0 - keys.first, c1 = (k1 < keys.first + a.cols ? k1 : keys.first + a.cols) - 1 - keys.first;
+        flagged(a.any + (a.bits_batch ? (long long)b * blocks * a.words : 0), blocks, a.words, c0 / 32, c1 / 32, 1, &ilo, &ihi);
+        ilo *= 32;
+        ihi = 32 * ihi < a.tq ? 32 * ihi : a.tq;
+    }
     const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0, nt = nt1 * a.per;
     const int jw = k0 + wave * WKEYS;      // the wave's first key
     queries(jw, jw + WKEYS < k1 ? jw + WKEYS : k1, &wlo, &whi);
@@ -936,6 +1176,15 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
                 w[n].set(s[n]);
             }
             mma_col<ST, ND, NB, true>(at.col, 0, w, dk);
+            if constexpr (ST != kF32)
+                if (fine_of<ST>(a, keys, i0, i0 + 31 < a.tq ? i0 + 31 : a.tq - 1)) {
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        left_in<ST>(s[n], w[n]);
+                        w[n].set(s[n]);
+                    }
+                    mma_col<ST, ND, NB, true>(at.col, 0, w, dk);
+                }
         }
     };
     for (int t = 0, ti = ilo; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
@@ -971,14 +1220,17 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
 
 template <int ST, int ND>
 hipError_t fwd(const AttnArgs& a, hipStream_t s) {
-    const long long rows = (long long)a.tq * a.pack;
-    const long long grid = (rows + kAttnTile - 1) / kAttnTile * a.batch * (a.heads / a.pack) * a.splits;
-    if (!grid) return hipSuccess;
-    attn_fwd_kernel<ST, ND><<<(unsigned)grid, 256, 0, s>>>(a);
-    if (a.splits > 1) {
-        const long long all = (long long)a.batch * a.heads * a.tq;
-        attn_join_kernel<ST, ND><<<(unsigned)((all + 3) / 4), 256, 0, s>>>(a);
+    const long long rows = (long long)a.tq * a.pack, units = (long long)a.batch * (a.heads / a.pack), all = (long long)a.batch * a.heads * a.tq;
+    if (!all) return hipSuccess;
+    if (rows <= kAttnFew) {
+        // as many waves as 128 KB of LDS have two blocks of keys and values each for
+        constexpr int NW = Geo<ST, ND>::ROW > 256 ? 2 : 4;
+        attn_few_kernel<ST, ND, NW><<<(unsigned)(units * a.splits), 64 * NW, 0, s>>>(a);
+    } else {
+        attn_fwd_kernel<ST, ND><<<(unsigned)((rows + kAttnTile - 1) / kAttnTile * units * a.splits), 256, 0, s>>>(a);
     }
+    if (a.splits > 16) attn_join_kernel<ST, ND, 4><<<(unsigned)all, 256, 0, s>>>(a);
+    else if (a.splits > 1) attn_join_kernel<ST, ND, 1><<<(unsigned)((all + 3) / 4), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
