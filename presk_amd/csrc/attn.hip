@@ -172,7 +172,7 @@ std::string attn_check(const presk_hip_attn& a, int what) {
     // workgroups of a launch
     const int64_t most = std::max(a.heads * (up(a.q_len, 16) / 16), a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile));
     if (a.batch * most >= 1ll << 31) return no("batch * heads * length past what a launch holds");
-    if (a.mask_cols && a.batch * up(a.q_len, 32) * (up(a.mask_cols, 64) / 32) >= 1ll << 31)
+    if (a.mask_cols && a.batch * up(a.q_len, 32) * (up(a.mask_cols, 32) / 32) >= 1ll << 30)
         return no("a mask past what a launch holds");
     return "";
 }

@@ -23,6 +23,8 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // A tile's rows of ND * 32 elements in LDS, PITCH of them apart, 16-byte chunk c
 // of row r at chunk c ^ swz(r): eight (and sixteen) consecutive rows' same chunk,
@@ -54,12 +56,12 @@ __device__ __forceinline__ f32x16 mma_row(typename FragOf<ST>::T a, typename Fra
     }
 }
 
+// Two values rounded into one word.  (The compiler's own conversion: it knows that
+// an exponential's result needs a wait before it is read, which assembly would not get.)
 template <int ST>
 __device__ __forceinline__ unsigned pack2(float a, float b) {
-    unsigned r;
-    if constexpr (ST == kBF16) asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    else asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+    if constexpr (ST == kBF16) return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    else return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
 // The weights of 32 tile rows as a product's operand.
@@ -424,13 +426,25 @@ __device__ __forceinline__ void by_mask(const AttnArgs& a, const Keys& keys, int
     if (keys.first <= 0 && from > *lo) *lo = from;
 }
 
-// 32 bits of a mask's line from `rel` on: ones before it, zeros past it.
-__device__ __forceinline__ unsigned bits_at(const unsigned* line, int words, int rel) {
-    if (rel <= -32) return ~0u;
-    const int q = rel >> 5;
-    const unsigned lo = q < 0 ? ~0u : q < words ? line[q] : 0u, hi = q + 1 < words ? line[q + 1] : 0u;
-    return (unsigned)(((unsigned long long)hi << 32 | lo) >> (rel & 31));
-}
+// 32 bits of a mask's line from `rel` on: ones before it, zeros past it.  The line
+// begins `line` words (below 2^30) from `bits`.  The two words are loaded a tile
+// ahead (`load`, then `landed` where the tile's own loads have), as a wait for them
+// where they are used would be one for the next tile's loads as well.
+struct MaskBits {
+    unsigned lo, hi;
+    __device__ __forceinline__ void load(const unsigned* bits, unsigned line, int words, int rel) {
+        const int q = rel >> 5;
+        auto word = [&](int w) { return *(const unsigned*)((const char*)bits + 4u * (line + (unsigned)(w < 0 ? 0 : w < words ? w : words - 1))); };
+        lo = word(q);
+        hi = word(q + 1);
+    }
+    __device__ __forceinline__ void landed() { asm volatile("" : "+v"(lo), "+v"(hi)); }
+    __device__ __forceinline__ unsigned at(int words, int rel) const {
+        const int q = rel >> 5;
+        const unsigned a = q < 0 ? ~0u : q < words ? lo : 0u, b = q + 1 < 0 ? ~0u : q + 1 < words ? hi : 0u;
+        return (unsigned)(((unsigned long long)b << 32 | a) >> (rel & 31));
+    }
+};
 
 // Bits [lo, hi) of 32.
 __device__ __forceinline__ unsigned range_of(int lo, int hi) {
@@ -460,22 +474,57 @@ __device__ __forceinline__ void cut(const AttnArgs& a, int split, int* lo, int* 
 
 // ---- the value ----------------------------------------------------------------------
 
+// Sums to and from LDS as a wave's lanes hold them, 16 bytes a lane at a time.
+template <int ND>
+__device__ __forceinline__ void give(unsigned char* at, int lane, const f32x16 (&acc)[ND], bool now) {
+    if (!now) return;
+    f32x4* const to = (f32x4*)at + lane;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) to[64 * (4 * dt + g)] = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+}
+// acc = f acc + g (those)
+template <int ND>
+__device__ __forceinline__ void take(const unsigned char* at, int lane, f32x16 (&acc)[ND], float f, float g) {
+    const f32x4* const from = (const f32x4*)at + lane;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 x = from[64 * (4 * dt + q)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[dt][4 * q + e] = acc[dt][4 * q + e] * f + x[e] * g;
+        }
+}
+
 // One workgroup: 128 rows of a head (of a group's heads beside each other), 32 a
-// wave, over the keys that any of them reads, or a share of those.
-template <int ST, int ND>
-__global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
+// wave, over the keys that any of them reads, or a share of those.  SW 2: eight
+// waves, two of which share 32 rows and take half of each tile's keys each.
+template <int ST, int ND, int SW>
+__global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, G::TILE, 256> Tile;
-    constexpr int NB = G::TILE / 32;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES];
+    typedef Rows<ST, ND, G::TILE, 256 * SW> Tile;
+    constexpr int NB = G::TILE / 32 / SW;
+    static_assert(NB >= 1, "a tile has a block for each");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES + (SW == 2 ? 2048 : 0)];
+    constexpr int PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;     // of LDS for the waves of the same rows
+    static_assert(4 * Tile::BYTES >= 4 * PAIR, "the waves' sums in LDS");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
+    const int rw = wave & 3, kw = wave >> 2;      // which rows, and which of a tile's keys
     const int rows = a.tq * a.pack, tiles = (rows + kAttnTile - 1) / kAttnTile, groups = a.heads / a.pack;
     const unsigned item = item_of(blockIdx.x, gridDim.x);
     const int split = (int)(item % (unsigned)a.splits);
     const unsigned at = item / (unsigned)a.splits;
-    // (a head's tiles from the last on: the longest ones first where they are causal)
-    const int tile = tiles - 1 - (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
+    // a head's tiles from the last on, the longest ones first where they are causal
+    // (where all workgroups are on the chip at once, two a CU, an XCD's second 32
+    // from the first on, so that a CU has a long one and a short one: 32 heads x
+    // 2048 x 128, causal, 71 -> 62 us)
+    const int unit = (int)(at / (unsigned)tiles);
+    const int turn = (int)(at % (unsigned)tiles);
+    const bool second = SW == 1 && gridDim.x <= 512 && (int)(blockIdx.x / 8) - (int)(turn * a.splits + split) >= 32;
+    const int tile = second ? turn : tiles - 1 - turn;
     const int b = unit / groups, hx = unit % groups, hk = hx * a.pack / a.per;
     const int r0 = tile * kAttnTile, r1 = (rows < r0 + kAttnTile ? rows : r0 + kAttnTile) - 1;
 
@@ -492,11 +541,11 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
     }
 
     // this lane's row
-    const int r = r0 + wave * 32 + (lane & 31);
+    const int r = r0 + rw * 32 + (lane & 31);
     const bool live = r < rows;
     const int i = (live ? r : r1) / a.pack, head = hx * a.pack + (live ? r : r1) % a.pack;
     const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
-    const unsigned* const line = a.cols ? a.bits + ((long long)b * a.bits_batch + i) * a.words : nullptr;
+    const unsigned line = (unsigned)((b * a.bits_batch + i) * a.words);
 
     Tile kt, vt;
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
@@ -519,28 +568,34 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
     for (int dt = 0; dt < ND; ++dt) o[0][dt] = f32x16{};
     float m = -INFINITY, l = 0.f;       // in log 2; this lane's part of the sum
     // what any of the wave's rows reads
-    const int w0 = r0 + wave * 32, w1 = w0 + 31 < r1 ? w0 + 31 : r1;
+    const int w0 = r0 + rw * 32, w1 = w0 + 31 < r1 ? w0 + 31 : r1;
     const int wlo = keys.lo(a, (w0 < r1 ? w0 : r1) / a.pack), whi = w0 <= r1 ? keys.hi(a, w1 / a.pack) : 0;
 
     Places<ST, ND> places;
     places.init(lane);
     places = places.from(lds);
+    MaskBits ahead[NB], now[NB];
+    auto load_bits = [&](int t) {
+        if (a.cols)
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) ahead[kb].load(a.bits, line, a.words, klo + t * G::TILE + (kw * NB + kb) * 32 - keys.first);
+    };
     auto body = [&](bool masked, int t) {
         const int k0 = klo + t * G::TILE;
-        const Places<ST, ND> at = places.from((unsigned)(t & 1) * 2 * Tile::BYTES);
+        const Places<ST, ND> at = places.from((unsigned)((t & 1) * 2 * Tile::BYTES + kw * NB * 32 * G::ROW));
         f32x16 s[NB];
         bool any[NB];
         float mx = -INFINITY;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
-            const int base = k0 + kb * 32;
+            const int base = k0 + (kw * NB + kb) * 32;
             unsigned bits = ~0u;
             any[kb] = true;
             if (masked) {
                 // keys that no row of the wave reads are passed over
                 any[kb] = base < whi && base + 32 > wlo;
-                if (any[kb] && a.cols && base + 32 > keys.first) {
-                    bits = bits_at(line, a.words, base - keys.first);
+                if (any[kb] && a.cols) {
+                    bits = now[kb].at(a.words, base - keys.first);
                     any[kb] = __any(bits);
                 }
                 if (!any[kb]) continue;
@@ -583,15 +638,42 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
             mma_col<ST, ND, 1>(at.col, Tile::BYTES + kb * 32 * G::ROW, w, o);
         }
     };
+    if (nt > 0) load_bits(0);
     for (int t = 0; t < nt; ++t) {
         wait_vm<0>();
+        if (a.cols)
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                ahead[kb].landed();
+                now[kb] = ahead[kb];
+            }
         __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+        if (t + 1 < nt) {
+            fetch(t + 1);
+            load_bits(t + 1);
+        }
         const int k0 = klo + t * G::TILE;
         body(k0 < surelo || k0 + G::TILE > surehi, t);
     }
 
     l += partner<32>(l);
+    unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same rows
+    if constexpr (SW == 2) {
+        // their sums meet
+        __syncthreads();
+        give<ND>(pair, lane, o[0], kw == 1);
+        float* const mls = (float*)(smem + 4 * PAIR) + 128 * rw + lane;
+        if (kw == 1) mls[0] = m, mls[64] = l;
+        __syncthreads();
+        if (kw == 1) return;    // (no barrier follows)
+        const float m1 = mls[0], l1 = mls[64], top = fmaxf(m, m1), base = base_of(top);
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+        take<ND>(pair, lane, o[0], f0, f1);
+        m = top;
+        l = l * f0 + l1 * f1;
+    } else {
+        __syncthreads();
+    }
     const long long row = ((long long)b * a.heads + head) * a.tq + i;
     if (a.splits > 1) {
         const long long all = (long long)a.batch * a.heads * a.tq, n = (long long)split * all + row;
@@ -606,11 +688,10 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(AttnArgs a) {
         }
         return;
     }
-    __syncthreads();
     store_kept<ST, ND>(o[0], l == 0.f ? 0.f : 1.f / l, a.d, a.o.vec, live, [&](int n) -> const void* {
-        const int x = r0 + wave * 32 + n;
+        const int x = r0 + rw * 32 + n;
         return x < rows ? row_at<ST>(a.o, b, x / a.pack, hx * a.pack + x % a.pack) : nullptr;
-    }, own, lane, a.flag);
+    }, pair, lane, a.flag);
     if (a.lse && live && h == 0) a.lse[row] = l == 0.f ? -INFINITY : (base_of(m) + __builtin_log2f(l)) * kLn2;
 }
 
@@ -668,7 +749,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
     const bool live = r < rows;
     const int i = live ? r / a.pack : a.tq - 1, head = hx * a.pack + (live ? r % a.pack : 0);
     const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
-    const unsigned* const line = a.cols ? a.bits + ((long long)b * a.bits_batch + i) * a.words : nullptr;
+    const unsigned line = (unsigned)((b * a.bits_batch + i) * a.words);
     typename FragOf<ST>::T q[G::STEPS];
     if (!a.q.vec) {
         load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
@@ -698,7 +779,12 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
 #pragma unroll
         for (int st = 0; st < G::STEPS; ++st) s = mma_row<ST>(frag_row<ST>(at.row, st), q[st], s);
         if (k0 < surelo || k0 + 32 > surehi) {
-            unsigned bits = a.cols && k0 + 32 > keys.first ? bits_at(line, a.words, k0 - keys.first) : ~0u;
+            unsigned bits = ~0u;
+            if (a.cols && k0 + 32 > keys.first) {
+                MaskBits m;
+                m.load(a.bits, line, a.words, k0 - keys.first);
+                bits = m.at(a.words, k0 - keys.first);
+            }
             bits = (bits & range_of(rlo - k0, rhi - k0)) >> (4 * h);
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = where_bit(bits, e, s[e], -INFINITY);
@@ -865,15 +951,18 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
 constexpr float kShift = 8.f;
 
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
-// the queries', NB blocks of 32 rows a wave.
-template <int ST, int ND, int NB>
-__global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
+// the queries'.
+template <int ST, int ND, int SW>
+__global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, G::TILE, 256> Tile;
-    constexpr int WROWS = 32 * NB, ROWS = 4 * WROWS;
+    typedef Rows<ST, ND, G::TILE, 256 * SW> Tile;
+    constexpr int NB = 1;
+    constexpr int WROWS = 32 * NB, ROWS = 4 * WROWS, PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;
+    static_assert(4 * Tile::BYTES >= 4 * PAIR, "the waves' sums in LDS");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
+    const int rw = wave & 3, kw = wave >> 2;      // which rows, and which of a tile's keys
     const int tiles = (a.tq + ROWS - 1) / ROWS;
     const unsigned at = item_of(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
@@ -899,7 +988,7 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
     };
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
 
-    const int w0 = r0 + wave * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
+    const int w0 = r0 + rw * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
     const int wlo = keys.lo(a, w0 < r1 ? w0 : r1), whi = w0 <= r1 ? keys.hi(a, w1) : 0;
     const bool fine = fine_of<ST>(a, keys, w0 < r1 ? w0 : r1, w1);
     typename FragOf<ST>::T q[NB][G::STEPS], dout[NB][G::STEPS];
@@ -921,6 +1010,14 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
     Places<ST, ND> places;
     places.init(lane);
     places = places.from(lds);
+    constexpr int MINE = G::TILE / 32 / SW;     // blocks of a tile that are the wave's
+    MaskBits ahead[MINE], now[MINE];
+    const unsigned line = (unsigned)((b * a.bits_batch + (w0 + (lane & 31) <= r1 ? w0 + (lane & 31) : r1)) * a.words);
+    auto load_bits = [&](int t) {
+        if (a.cols)
+#pragma unroll
+            for (int x = 0; x < MINE; ++x) ahead[x].load(a.bits, line, a.words, klo + t * G::TILE + (kw + SW * x) * 32 - keys.first);
+    };
     auto body = [&](bool masked, int t, int kb) {
         const int base = klo + t * G::TILE + kb * 32;
         const Places<ST, ND> at = places.from((unsigned)((t & 1) * 2 * Tile::BYTES + kb * 32 * G::ROW));
@@ -928,16 +1025,9 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
         if (masked) {
             // keys that no row of the wave reads are passed over
             if (base >= whi || base + 32 <= wlo) return;
-            unsigned all = 0;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
-                bits[n] = ~0u;
-                if (a.cols && base + 32 > keys.first)
-                    bits[n] = bits_at(a.bits + ((long long)b * a.bits_batch + i) * a.words, a.words, base - keys.first);
-                all |= bits[n];
-            }
-            if (!__any(all)) return;
+            bits[0] = ~0u;
+            if (a.cols) bits[0] = (MINE == 1 || kb < SW ? now[0] : now[MINE - 1]).at(a.words, base - keys.first);
+            if (!__any(bits[0])) return;
         }
         f32x16 s[NB], dp[NB];
 #pragma unroll
@@ -975,35 +1065,54 @@ __global__ void __launch_bounds__(256, NB * ND >= 8 || (ST == kF32 && NB * ND >=
                 mma_col<ST, ND, NB>(at.col, 0, w, dq);
             }
     };
+    if (nt > 0) load_bits(0);
     for (int t = 0; t < nt; ++t) {
         wait_vm<0>();
+        if (a.cols)
+#pragma unroll
+            for (int x = 0; x < MINE; ++x) {
+                ahead[x].landed();
+                now[x] = ahead[x];
+            }
         __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+        if (t + 1 < nt) {
+            fetch(t + 1);
+            load_bits(t + 1);
+        }
         const int k0 = klo + t * G::TILE;
 #pragma unroll 1
-        for (int kb = 0; kb < G::TILE / 32; ++kb) body(k0 < surelo || k0 + G::TILE > surehi, t, kb);
+        for (int kb = kw; kb < G::TILE / 32; kb += SW) body(k0 < surelo || k0 + G::TILE > surehi, t, kb);
     }
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-        store_kept<ST, ND>(dq[n], a.scale, a.d, a.dq.vec, w0 + 32 * n + (lane & 31) <= r1, [&](int x) -> const void* {
-            const int r = w0 + 32 * n + x;
-            return r <= r1 ? row_at<ST>(a.dq, b, r, head) : nullptr;
-        }, own, lane, a.flag);
+    unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same rows
+    if constexpr (SW == 2) {
+        give<ND>(pair, lane, dq[0], kw == 1);
+        __syncthreads();
+        if (kw == 1) return;
+        take<ND>(pair, lane, dq[0], 1.f, 1.f);
+    }
+    store_kept<ST, ND>(dq[0], a.scale, a.d, a.dq.vec, w0 + (lane & 31) <= r1, [&](int x) -> const void* {
+        return w0 + x <= r1 ? row_at<ST>(a.dq, b, w0 + x, head) : nullptr;
+    }, pair, lane, a.flag);
 }
 
-// The keys' and values' gradients (DK, DV): a workgroup keeps 128 NB keys of a key
-// head, NB blocks of 32 a wave, and the rows of all heads of its group that read
-// any of them pass by.
-template <int ST, int ND, int NB, int QT, bool DK, bool DV, bool VL, int OCC>
-__global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
+// The keys' and values' gradients (DK, DV): a workgroup keeps 128 keys of a key
+// head, 32 a wave, and the rows of all heads of its group that read any of them
+// pass by, QT at a time.  SW 2: eight waves, two of which share 32 keys and take
+// half of each tile's rows each.  VL: the values are kept in LDS, as the registers
+// that two waves a SIMD have do not hold them too, and with eight waves, whose one
+// workgroup a CU has the room, the keys beside them.
+template <int ST, int ND, int SW, int QT, bool DK, bool DV, bool VL, int OCC>
+__global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, QT, 256> Tile;
-    constexpr int WKEYS = 32 * NB, KEYS = 4 * WKEYS, STAGE = 2 * Tile::BYTES + 512;
-    typedef Rows<ST, ND, KEYS, 256> Kept;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + (VL ? Kept::BYTES : 0)];
+    typedef Rows<ST, ND, QT, 256 * SW> Tile;
+    constexpr int NB = 1, WKEYS = 32 * NB, KEYS = 4 * WKEYS, STAGE = 2 * Tile::BYTES + 512, PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;
+    typedef Rows<ST, ND, KEYS, 256 * SW> Kept;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + (VL ? SW * Kept::BYTES : 0)];
+    constexpr bool KL = VL && SW == 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
+    const int rw = wave & 3, kw = wave >> 2;      // which keys, and which of a tile's rows
     const int tiles = (a.tk + KEYS - 1) / KEYS;
     const unsigned at = item_of(blockIdx.x, gridDim.x);
     const int tile = (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
@@ -1034,7 +1143,7 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
         ihi = 32 * ihi < a.tq ? 32 * ihi : a.tq;
     }
     const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0, nt = nt1 * a.per;
-    const int jw = k0 + wave * WKEYS;      // the wave's first key
+    const int jw = k0 + rw * WKEYS;      // the wave's first key
     queries(jw, jw + WKEYS < k1 ? jw + WKEYS : k1, &wlo, &whi);
 
     Tile qt, dt_;
@@ -1062,13 +1171,13 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
     };
 
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
-    typename FragOf<ST>::T k[NB][G::STEPS], v[VL ? 1 : NB][G::STEPS];
+    typename FragOf<ST>::T k[KL ? 1 : NB][G::STEPS], v[VL ? 1 : NB][G::STEPS];
     f32x16 dk[NB][ND], dv[NB][ND];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const int j = jw + 32 * n + (lane & 31);
         const bool live = j < k1 && j < keys.len;
-        load_kept<ST, ND>(a.k, b, j, hk, a.d, live, lane, own, k[n]);
+        if (!KL) load_kept<ST, ND>(a.k, b, j, hk, a.d, live, lane, own, k[n]);
         if (DK && !VL) load_kept<ST, ND>(a.v, b, j, hk, a.d, live, lane, own, v[n]);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) dk[n][dt] = dv[n][dt] = f32x16{};
@@ -1079,10 +1188,28 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
             Kept vt;
             vt.init(a.v, b, hk, a.d, tid, lds);
             vt.issue(k0, (k1 < keys.len ? k1 : keys.len) - k0, 2 * STAGE, smem, tid);
+            if (KL) {
+                vt.init(a.k, b, hk, a.d, tid, lds);
+                vt.issue(k0, (k1 < keys.len ? k1 : keys.len) - k0, 2 * STAGE + Kept::BYTES, smem, tid);
+            }
         }
         fetch(0);
     }
 
+    // a mask's words of this lane's key (its rows come 32 at a time from a multiple
+    // of 32 on), loaded a tile ahead as the queries' are
+    constexpr int MINE = QT / 32 / SW;      // blocks of a tile that are the wave's
+    const int col = jw + (lane & 31) - keys.first;
+    const unsigned line = (unsigned)((b * a.bits_t_batch + (col < 0 ? 0 : col < a.cols ? col : a.cols - 1)) * a.words_t);
+    unsigned ahead[MINE], now[MINE];
+    auto load_bits = [&](int i0) {
+        if (a.cols)
+#pragma unroll
+            for (int x = 0; x < MINE; ++x) {
+                const int w = i0 / 32 + kw + SW * x;
+                ahead[x] = *(const unsigned*)((const char*)a.bits_t + 4u * (line + (unsigned)(w < a.words_t ? w : a.words_t - 1)));
+            }
+    };
     // the tile's rows sub * 32 on, which are the queries i0 on
     Places<ST, ND> places;
     places.init(lane);
@@ -1095,27 +1222,20 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
         if (masked) {
             // rows that read none of the wave's keys are passed over
             if (i0 + 31 < wlo || i0 >= whi) return;
-            unsigned all = 0;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int col = jw + 32 * n + (lane & 31) - keys.first;
-                bits[n] = ~0u;
-                if (a.cols && col >= 0)
-                    bits[n] = col < a.cols ? bits_at(a.bits_t + ((long long)b * a.bits_t_batch + col) * a.words_t, a.words_t, i0) : 0u;
-                all |= bits[n];
-            }
-            if (!__any(all)) return;
+            bits[0] = !a.cols || col < 0 ? ~0u : col < a.cols ? MINE == 1 || sub < SW ? now[0] : now[MINE - 1] : 0u;
+            if (!__any(bits[0])) return;
         }
-        const unsigned kept = VL ? places.from((unsigned)(2 * STAGE + wave * WKEYS * G::ROW)).row : 0u;
+        const unsigned kept = VL ? places.from((unsigned)(2 * STAGE + rw * WKEYS * G::ROW)).row : 0u;
         f32x16 s[NB], dp[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = dp[n] = f32x16{};
         // a step's reads a step ahead of its products, and no further, or the
         // registers do not hold them
         typedef typename FragOf<ST>::T F;
-        F fq, fd, fv[NB];
+        F fq, fd, fv[NB], fk;
         auto read = [&](int st) {
             fq = frag_row<ST>(at.row, st);
+            if (KL) fk = frag_row<ST>(kept, st, Kept::BYTES);
             if (DK) {
                 fd = frag_row<ST>(at.row, st, Tile::BYTES);
                 if (VL)
@@ -1126,7 +1246,7 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
         read(0);
 #pragma unroll
         for (int st = 0; st < G::STEPS; ++st) {
-            const F cq = fq, cd = fd;
+            const F cq = fq, cd = fd, ck = KL ? fk : k[0][KL ? 0 : st];
             F cv[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n) cv[n] = VL ? fv[n] : v[VL ? 0 : n][st];
@@ -1134,7 +1254,7 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                s[n] = mma_row<ST>(cq, k[n][st], s[n]);
+                s[n] = mma_row<ST>(cq, ck, s[n]);
                 if (DK) dp[n] = mma_row<ST>(cd, cv[n], dp[n]);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -1187,12 +1307,22 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
                 }
         }
     };
+    if (nt > 0) load_bits(ilo);
     for (int t = 0, ti = ilo; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
         wait_vm<0>();
+        if (a.cols)
+#pragma unroll
+            for (int x = 0; x < MINE; ++x) {
+                asm volatile("" : "+v"(ahead[x]));
+                now[x] = ahead[x];
+            }
         __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+        if (t + 1 < nt) {
+            fetch(t + 1);
+            load_bits(ti + QT < ihi ? ti + QT : ilo);
+        }
 #pragma unroll 1
-        for (int sub = 0; sub < QT / 32; ++sub) {
+        for (int sub = kw; sub < QT / 32; sub += SW) {
             const int i0 = ti + 32 * sub;
             const bool sure = (!a.causal || (jw + WKEYS - 1 <= keys.first + i0 && (!a.window || jw > keys.first + i0 + 31 - a.window))) &&
                               (!a.cols || jw + WKEYS <= keys.first) && i0 < ihi;
@@ -1200,23 +1330,41 @@ __global__ void __launch_bounds__(256, OCC) attn_dkv_kernel(AttnArgs a) {
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int j = jw + 32 * n + (lane & 31);
-        const bool exists = j < k1;
-        // (what a key past the sequence's end was given is dropped)
-        if (j >= keys.len)
-#pragma unroll
-            for (int dt = 0; dt < ND; ++dt) dk[n][dt] = dv[n][dt] = f32x16{};
-        auto where = [&](const AttnTensor& t) {
-            return [&, t](int x) -> const void* { return jw + 32 * n + x < k1 ? row_at<ST>(t, b, jw + 32 * n + x, hk) : nullptr; };
-        };
-        if (DK && a.dk.p) store_kept<ST, ND>(dk[n], a.scale, a.d, a.dk.vec, exists, where(a.dk), own, lane, a.flag);
-        if (DV && a.dv.p) store_kept<ST, ND>(dv[n], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), own, lane, a.flag);
+    unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same keys
+    if constexpr (SW == 2) {
+        static_assert(sizeof(smem) >= 4 * PAIR, "the waves' sums in LDS");
+        give<ND>(pair, lane, dk[0], kw == 1);
+        __syncthreads();
+        if (kw == 0) take<ND>(pair, lane, dk[0], 1.f, 1.f);
+        __syncthreads();
+        give<ND>(pair, lane, dv[0], kw == 1);
+        __syncthreads();
+        if (kw == 1) return;
+        take<ND>(pair, lane, dv[0], 1.f, 1.f);
     }
+    const int j = jw + (lane & 31);
+    const bool exists = j < k1;
+    // (what a key past the sequence's end was given is dropped)
+    if (j >= keys.len)
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dk[0][dt] = dv[0][dt] = f32x16{};
+    auto where = [&](const AttnTensor& t) {
+        return [&, t](int x) -> const void* { return jw + x < k1 ? row_at<ST>(t, b, jw + x, hk) : nullptr; };
+    };
+    if (DK && a.dk.p) store_kept<ST, ND>(dk[0], a.scale, a.d, a.dk.vec, exists, where(a.dk), pair, lane, a.flag);
+    if (DV && a.dv.p) store_kept<ST, ND>(dv[0], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), pair, lane, a.flag);
 }
 
 // ---- launches -----------------------------------------------------------------------------
+
+// Workgroups of eight waves where four would leave SIMDs with a wave or none, which
+// then waits for its own results: where a round of the CUs holds them all (2 x 12
+// heads x 1024 x 64, 192 of them, 27 -> 17 us), and causal ones of up to two, whose
+// longest would be by themselves in the end.
+template <int ST, int ND>
+bool eight(long long grid) {
+    return Geo<ST, ND>::TILE == 64 && grid <= 256;
+}
 
 template <int ST, int ND>
 hipError_t fwd(const AttnArgs& a, hipStream_t s) {
@@ -1227,38 +1375,42 @@ hipError_t fwd(const AttnArgs& a, hipStream_t s) {
         constexpr int NW = Geo<ST, ND>::ROW > 256 ? 2 : 4;
         attn_few_kernel<ST, ND, NW><<<(unsigned)(units * a.splits), 64 * NW, 0, s>>>(a);
     } else {
-        attn_fwd_kernel<ST, ND><<<(unsigned)((rows + kAttnTile - 1) / kAttnTile * units * a.splits), 256, 0, s>>>(a);
+        const long long grid = (rows + kAttnTile - 1) / kAttnTile * units * a.splits;
+        if (eight<ST, ND>(grid)) {
+            if constexpr (Geo<ST, ND>::TILE == 64) attn_fwd_kernel<ST, ND, 2><<<(unsigned)grid, 512, 0, s>>>(a);
+        } else {
+            attn_fwd_kernel<ST, ND, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+        }
     }
     if (a.splits > 16) attn_join_kernel<ST, ND, 4><<<(unsigned)all, 256, 0, s>>>(a);
     else if (a.splits > 1) attn_join_kernel<ST, ND, 1><<<(unsigned)((all + 3) / 4), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
-template <int ST, int ND, int NB>
-void dq_launch(const AttnArgs& a, hipStream_t s) {
-    attn_dq_kernel<ST, ND, NB><<<(unsigned)((long long)((a.tq + 128 * NB - 1) / (128 * NB)) * a.batch * a.heads), 256, 0, s>>>(a);
-}
-template <int ST, int ND, int NB, int QT, bool DK, bool DV, bool VL, int OCC>
-void dkv_launch(const AttnArgs& a, hipStream_t s) {
-    attn_dkv_kernel<ST, ND, NB, QT, DK, DV, VL, OCC><<<(unsigned)((long long)((a.tk + 128 * NB - 1) / (128 * NB)) * a.batch * a.kv), 256, 0, s>>>(a);
-}
-
 template <int ST, int ND>
 hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     const long long all = (long long)a.batch * a.heads * a.tq;
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
-    if (a.dq.p && all) dq_launch<ST, ND, 1>(a, s);
+    if (a.dq.p && all) {
+        const long long grid = (long long)((a.tq + 127) / 128) * a.batch * a.heads;
+        if (eight<ST, ND>(grid)) {
+            if constexpr (Geo<ST, ND>::TILE == 64) attn_dq_kernel<ST, ND, 2><<<(unsigned)grid, 512, 0, s>>>(a);
+        } else {
+            attn_dq_kernel<ST, ND, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+        }
+    }
     if ((a.dk.p || a.dv.p) && a.batch && a.tk) {
+        const long long grid = (long long)((a.tk + 127) / 128) * a.batch * a.kv;
         if constexpr (ND == 8) {
             // (both sums of 256 elements and both kept rows do not fit the registers)
-            if (a.dk.p) dkv_launch<ST, ND, 1, 32, true, false, false, 1>(a, s);
-            if (a.dv.p) dkv_launch<ST, ND, 1, 32, false, true, false, 1>(a, s);
-        } else if constexpr (ST == kF32) {
-            dkv_launch<ST, ND, 1, ND == 4 ? 32 : 64, true, true, false, ND == 4 ? 1 : 2>(a, s);
-        } else if constexpr (ND == 4) {
-            dkv_launch<ST, ND, 1, 32, true, true, true, 2>(a, s);
+            if (a.dk.p) attn_dkv_kernel<ST, ND, 1, 32, true, false, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+            if (a.dv.p) attn_dkv_kernel<ST, ND, 1, 32, false, true, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+        } else if constexpr (ST == kF32 && ND == 4) {
+            attn_dkv_kernel<ST, ND, 1, 32, true, true, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+        } else if (eight<ST, ND>(grid)) {
+            attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2><<<(unsigned)grid, 512, 0, s>>>(a);
         } else {
-            dkv_launch<ST, ND, 1, 64, true, true, false, 2>(a, s);
+            attn_dkv_kernel<ST, ND, 1, ND == 4 ? 32 : 64, true, true, ND == 4, 2><<<(unsigned)grid, 256, 0, s>>>(a);
         }
     }
     return hipGetLastError();
