@@ -3,12 +3,15 @@
 //   y = (u0 cos a - u1 sin a, u1 cos a + u0 sin a) of a pair (u0, u1), a = position * freq,
 // and back: du the pair turned by -a, dg = sum du n, dx = (dn - n mean(dn n)) / sqrt(..)
 // with dn = g du.
-// A wave takes a token and some of its heads: a head is `lanes` lanes, each with two
-// runs of EC elements that are each other's partners, so that no lane needs
-// another's; the angles, the same for all of a token's heads, are worked out
-// once.  They are turns in f64, of which whole quarters drop out before f32: a
-// position of 10^6 keeps what an angle near zero has.
-// Bound by its bytes, x read and y written once.
+// A wave takes a token and some of its heads of q, or of k: a head is `lanes` lanes,
+// each with two runs of EC elements that are each other's partners, so that no lane
+// needs another's; the angles, the same for all heads, are worked out once a wave.
+// They are turns in f64, of which whole quarters drop out before f32: a position of
+// 10^6 keeps what an angle near zero has.
+// Bound by its bytes, x read and y written once, as long as the work on them stays
+// at a few instructions an element: one kernel that told q from k and pairs from
+// halves as it went took 47 an element, and 44 us for 2 x 4096 x (32 + 8) heads x 128
+// in bf16, normed, and 114 for their gradients.
 #include "rotary.hpp"
 
 #include <hip/hip_runtime.h>
@@ -37,17 +40,24 @@ struct RotTensor {
     long long batch, seq, head;
 };
 
+// One of q and k.
+struct RotSide {
+    RotTensor in, x, y;          // what is turned (the forward's x, or dy), the forward's x, and the output
+    const void* g;               // gains or null
+    void* dg;
+    int heads, chunks;           // heads of a token, and how many waves take them
+    int blocks;                  // workgroups
+};
+
 struct RotArgs {
-    RotTensor x[2], y[2];        // q and k; of the gradient dy and dx, and the forward's x
-    RotTensor in[2];
-    const void* g[2];            // gains or null
+    RotSide side[2];
     const double* freq;
     const long long* at;         // [batch][seq] or null
-    int batch, seq, heads[2], d, rotary, norm, even;
-    float eps;
+    int batch, seq, d, rotary;
+    float eps, per_d, sign;      // per_d 1 / d; sign -1 turns back
     int lanes;                   // of a head, a power of two
-    int per_wave, chunks;        // heads a wave takes of a token, and how many such there are
-    float* part;                 // [workgroups][2][d]: the gains' gradients
+    int per_wave;                // heads a wave takes of a token
+    float* part;                 // [workgroups][d]: the gains' gradients
     unsigned* flag;
 };
 
@@ -63,8 +73,8 @@ __device__ __forceinline__ float widen(typename Elem<ST>::T v) {
 template <int ST>
 __device__ __forceinline__ typename Elem<ST>::T narrow(float v) {
     if constexpr (ST == kF32) return v;
-    else if constexpr (ST == kBF16) return pk_f32_to_bf16(v);
-    else return pk_f32_to_f16(v);
+    else if constexpr (ST == kBF16) return __builtin_bit_cast(unsigned short, (__bf16)v);
+    else return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
 template <int ST, int EC>
@@ -105,12 +115,20 @@ __device__ __forceinline__ float over_lanes(float v, int lanes) {
     return v;
 }
 
-template <int ST, int EC, bool GRAD>
+enum RotMode { kTurn, kNormed, kNormedGrad };
+
+template <int ST, int EC, bool EVEN, RotMode MODE>
 __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
     typedef typename Elem<ST>::T T;
     typedef Run<ST, EC> R;
+    constexpr bool GRAD = MODE == kNormedGrad;
     constexpr int K = EC == 1 ? 2 : 1;      // pairs of runs a lane (a head of 256 single elements)
-    const int lane = threadIdx.x & 63, sub = lane / a.lanes, mine = lane % a.lanes, beside = 64 / a.lanes;
+    constexpr int U = 2;                    // heads a lane whose loads are under way together (more of them cost waves)
+    const bool second = blockIdx.x >= (unsigned)a.side[0].blocks;
+    const RotSide& c = a.side[second];
+    const int block = (int)blockIdx.x - (second ? a.side[0].blocks : 0);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int sub = lane / a.lanes, mine = lane % a.lanes, beside = 64 / a.lanes;
     const int pairs = a.rotary / (2 * EC), all = (a.d + 2 * EC - 1) / (2 * EC);
 
     // the first elements of this lane's two runs
@@ -121,205 +139,184 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
         const int p = mine + k * a.lanes;
         turns[k] = p < pairs;
         in[k] = p < all;
-        if (turns[k]) {
-            e0[k] = a.even ? 2 * EC * p : EC * p;
-            e1[k] = a.even ? 2 * EC * p + EC : a.rotary / 2 + EC * p;
-        } else {
-            e0[k] = 2 * EC * p;
-            e1[k] = e0[k] + EC;
-        }
+        const bool half = turns[k] && !EVEN;
+        e0[k] = half ? EC * p : 2 * EC * p;
+        e1[k] = half ? a.rotary / 2 + EC * p : 2 * EC * p + EC;
         in1[k] = in[k] && e1[k] < a.d;
     }
     // gains, and their gradients' sums
-    float g0[2][K][EC], g1[2][K][EC], s0[2][K][EC], s1[2][K][EC];
+    float g0[K][EC], g1[K][EC], s0[K][EC], s1[K][EC];
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < EC; ++e) {
+            const T* const g = (const T*)c.g;
+            g0[k][e] = g && in[k] ? widen<ST>(g[e0[k] + e]) : 1.f;
+            g1[k][e] = g && in1[k] ? widen<ST>(g[e1[k] + e]) : 1.f;
+            s0[k][e] = s1[k][e] = 0.f;
+        }
+    bool ovf = false;
+
+    const long long units = (long long)a.batch * a.seq * c.chunks;
+    for (long long unit = (long long)block * 4 + wave; unit < units; unit += (long long)c.blocks * 4) {
+        const long long token = unit / c.chunks;
+        const int first = (int)(unit - token * c.chunks) * a.per_wave;
+        const int end = first + a.per_wave < c.heads ? first + a.per_wave : c.heads;
+        const long long b = token / a.seq, i = token - b * a.seq;
+        auto start = [&](const RotTensor& t) { return (T*)t.p + b * t.batch + i * t.seq; };
+        T *const ip = start(c.in), *const xp = start(c.x), *const yp = start(c.y);
+        R ri0[U][K], ri1[U][K], rx0[GRAD ? U : 1][K], rx1[GRAD ? U : 1][K];
+        auto fetch = [&](int h0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int head = h0 + u * beside + sub;
+                auto load = [&](const T* p, R (&r0)[K], R (&r1)[K]) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        r0[k] = R{}, r1[k] = R{};
+                        if (head < end && in[k]) r0[k] = *(const R*)(p + e0[k]);
+                        if (head < end && in1[k]) r1[k] = *(const R*)(p + e1[k]);
+                    }
+                };
+                load(ip + head * c.in.head, ri0[u], ri1[u]);
+                if constexpr (GRAD) load(xp + head * c.x.head, rx0[u], rx1[u]);
+            }
+        };
+        fetch(first);       // (under way while the angles are worked out)
+        const double at = (double)(a.at ? a.at[token] : i);
+        float cs[K][EC], sn[K][EC];
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < EC; ++e) {
-                const T* const g = (const T*)a.g[w];
-                g0[w][k][e] = g && in[k] ? widen<ST>(g[e0[k] + e]) : 1.f;
-                g1[w][k][e] = g && in1[k] ? widen<ST>(g[e1[k] + e]) : 1.f;
-                s0[w][k][e] = s1[w][k][e] = 0.f;
-            }
-    bool ovf = false;
-
-    const long long units = (long long)a.batch * a.seq * a.chunks;
-    for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (long long)gridDim.x * 4) {
-        const long long token = unit / a.chunks;
-        const int first = (int)(unit - token * a.chunks) * a.per_wave;
-        const long long b = token / a.seq, i = token - b * a.seq;
-        const double at = (double)(a.at ? a.at[token] : i);
-        float cs[K][EC], sn[K][EC];
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-#pragma unroll
-            for (int e = 0; e < EC; ++e) {
                 cs[k][e] = 1.f, sn[k][e] = 0.f;
-                // neighbours: the run's pairs are (e0 + 2 j, e0 + 2 j + 1), EC of them in the two runs
+                // (neighbours paired: the two runs' EC pairs in order)
                 if (turns[k]) turned(at * a.freq[EC * (mine + k * a.lanes) + e] * 0.6366197723675814, &cs[k][e], &sn[k][e]);
+                sn[k][e] *= a.sign;
             }
-        }
-        const int total = a.heads[0] + a.heads[1], end = first + a.per_wave < total ? first + a.per_wave : total;
-        for (int h0 = first; h0 < end; h0 += beside) {
-            const int hh = h0 + sub;
-            const bool live = hh < end;
-            const int w = live && hh >= a.heads[0], head = live ? hh - (w ? a.heads[0] : 0) : 0;
-            auto row = [&](const RotTensor& t0, const RotTensor& t1) {
-                const RotTensor& t = w ? t1 : t0;
-                return (T*)t.p + b * t.batch + i * t.seq + head * t.head;
-            };
-            const T* const xs = !GRAD ? row(a.x[0], a.x[1]) : a.norm ? row(a.in[0], a.in[1]) : nullptr;
-            const T* const ds = GRAD ? row(a.x[0], a.x[1]) : nullptr;
-            // the head's elements, normed; of the gradient its cotangent too
-            float x0[K][EC], x1[K][EC], d0[K][EC], d1[K][EC];
-            auto load = [&](const T* p, float (&u)[K][EC], float (&v)[K][EC]) {
+        for (int h0 = first; h0 < end; h0 += U * beside) {
+            if (h0 > first) fetch(h0);
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    R r0{}, r1{};
-                    if (live && in[k]) r0 = *(const R*)(p + e0[k]);
-                    if (live && in1[k]) r1 = *(const R*)(p + e1[k]);
-#pragma unroll
-                    for (int e = 0; e < EC; ++e) u[k][e] = widen<ST>(r0.v[e]), v[k][e] = widen<ST>(r1.v[e]);
-                }
-            };
-            if (xs) load(xs, x0, x1);
-            if (GRAD) load(ds, d0, d1);
-            float rstd = 1.f;
-            if (a.norm) {
-                float ss = 0.f;
+            for (int u = 0; u < U; ++u) {
+                const int head = h0 + u * beside + sub;
+                float v0[K][EC], v1[K][EC], x0[K][EC], x1[K][EC], rstd = 1.f;
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int e = 0; e < EC; ++e) ss += x0[k][e] * x0[k][e] + x1[k][e] * x1[k][e];
-                ss = over_lanes(ss, a.lanes);
-                rstd = 1.f / sqrtf(ss / (float)a.d + a.eps);
-            }
-            auto gain = [&](const float (&g)[2][K][EC], int k, int e) { return w ? g[1][k][e] : g[0][k][e]; };
-            // a run's pairs: with neighbours paired, element j of the two runs read as one is turned with j ^ 1
-            auto turn = [&](float (&u)[K][EC], float (&v)[K][EC], float sign) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (EC > 1 && a.even) {
-                        float z[2 * EC];
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) z[e] = u[k][e], z[EC + e] = v[k][e];
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) {
-                            const float p = z[2 * e], q = z[2 * e + 1], s = sn[k][e] * sign;
-                            z[2 * e] = p * cs[k][e] - q * s;
-                            z[2 * e + 1] = q * cs[k][e] + p * s;
-                        }
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) u[k][e] = z[e], v[k][e] = z[EC + e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < EC; ++e) {
-                            const float p = u[k][e], q = v[k][e], s = sn[k][e] * sign;
-                            u[k][e] = p * cs[k][e] - q * s;
-                            v[k][e] = q * cs[k][e] + p * s;
-                        }
+                    for (int e = 0; e < EC; ++e) {
+                        v0[k][e] = widen<ST>(ri0[u][k].v[e]), v1[k][e] = widen<ST>(ri1[u][k].v[e]);
+                        if constexpr (GRAD) x0[k][e] = widen<ST>(rx0[u][k].v[e]), x1[k][e] = widen<ST>(rx1[u][k].v[e]);
                     }
-                }
-            };
-            if (!GRAD) {
-                if (a.norm)
+                if constexpr (MODE != kTurn) {
+                    float ss = 0.f;
 #pragma unroll
                     for (int k = 0; k < K; ++k)
 #pragma unroll
                         for (int e = 0; e < EC; ++e) {
-                            x0[k][e] = x0[k][e] * rstd * gain(g0, k, e);
-                            x1[k][e] = x1[k][e] * rstd * gain(g1, k, e);
+                            const float p = GRAD ? x0[k][e] : v0[k][e], q = GRAD ? x1[k][e] : v1[k][e];
+                            ss = __builtin_fmaf(p, p, __builtin_fmaf(q, q, ss));
                         }
-                turn(x0, x1, 1.f);
-            } else {
-                turn(d0, d1, -1.f);
-                if (a.norm) {
+                    // the hardware's root, refined once
+                    const float m = __builtin_fmaf(over_lanes(ss, a.lanes), a.per_d, a.eps), r = __builtin_amdgcn_rsqf(m);
+                    rstd = !(m >= 1e-30f && m <= 1e30f) ? 1.f / sqrtf(m) : __builtin_fmaf(__builtin_fmaf(-m * r, r, 1.f), 0.5f * r, r);
+                }
+                if constexpr (MODE == kNormed)
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int e = 0; e < EC; ++e) v0[k][e] *= rstd * g0[k][e], v1[k][e] *= rstd * g1[k][e];
+                // turned: pair e of the two runs, or of the one that they make
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int e = 0; e < EC; ++e) {
+                        float& p = EVEN && EC > 1 ? (2 * e < EC ? v0[k][2 * e % EC] : v1[k][2 * e % EC]) : v0[k][e];
+                        float& q = EVEN && EC > 1 ? (2 * e < EC ? v0[k][(2 * e + 1) % EC] : v1[k][(2 * e + 1) % EC]) : v1[k][e];
+                        const float p0 = p;
+                        p = __builtin_fmaf(p0, cs[k][e], -(q * sn[k][e]));
+                        q = __builtin_fmaf(q, cs[k][e], p0 * sn[k][e]);
+                    }
+                if constexpr (GRAD) {
                     float m = 0.f;
 #pragma unroll
                     for (int k = 0; k < K; ++k)
 #pragma unroll
                         for (int e = 0; e < EC; ++e) {
                             x0[k][e] *= rstd, x1[k][e] *= rstd;
-                            const float t0 = d0[k][e] * x0[k][e], t1 = d1[k][e] * x1[k][e];
                             // (a lane without a head has zeros)
-                            s0[0][k][e] += w ? 0.f : t0, s0[1][k][e] += w ? t0 : 0.f;
-                            s1[0][k][e] += w ? 0.f : t1, s1[1][k][e] += w ? t1 : 0.f;
-                            d0[k][e] *= gain(g0, k, e), d1[k][e] *= gain(g1, k, e);
-                            m += d0[k][e] * x0[k][e] + d1[k][e] * x1[k][e];
+                            s0[k][e] = __builtin_fmaf(v0[k][e], x0[k][e], s0[k][e]), s1[k][e] = __builtin_fmaf(v1[k][e], x1[k][e], s1[k][e]);
+                            v0[k][e] *= g0[k][e], v1[k][e] *= g1[k][e];
+                            m = __builtin_fmaf(v0[k][e], x0[k][e], __builtin_fmaf(v1[k][e], x1[k][e], m));
                         }
-                    m = over_lanes(m, a.lanes) / (float)a.d;
+                    m = over_lanes(m, a.lanes) * a.per_d;
 #pragma unroll
                     for (int k = 0; k < K; ++k)
 #pragma unroll
                         for (int e = 0; e < EC; ++e) {
-                            d0[k][e] = rstd * (d0[k][e] - x0[k][e] * m);
-                            d1[k][e] = rstd * (d1[k][e] - x1[k][e] * m);
+                            v0[k][e] = rstd * __builtin_fmaf(-x0[k][e], m, v0[k][e]);
+                            v1[k][e] = rstd * __builtin_fmaf(-x1[k][e], m, v1[k][e]);
                         }
                 }
-            }
-            T* const out = row(a.y[0], a.y[1]);
-            auto store = [&](const float (&u)[K][EC], const float (&v)[K][EC]) {
+                T* const out = yp + head * c.y.head;
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     R r0, r1;
+                    bool over = false;
 #pragma unroll
                     for (int e = 0; e < EC; ++e) {
-                        r0.v[e] = narrow<ST>(u[k][e]), r1.v[e] = narrow<ST>(v[k][e]);
-                        if (ST == kF16) ovf |= live && in[k] && (pk_overflows_f16(u[k][e]) || (in1[k] && pk_overflows_f16(v[k][e])));
+                        r0.v[e] = narrow<ST>(v0[k][e]), r1.v[e] = narrow<ST>(v1[k][e]);
+                        if (ST == kF16) over |= pk_overflows_f16(v0[k][e]) || pk_overflows_f16(v1[k][e]);
                     }
-                    if (live && in[k]) *(R*)(out + e0[k]) = r0;
-                    if (live && in1[k]) *(R*)(out + e1[k]) = r1;
+                    if (head < end) {
+                        if (in[k]) *(R*)(out + e0[k]) = r0;
+                        if (in1[k]) *(R*)(out + e1[k]) = r1;
+                        ovf |= over;
+                    }
                 }
-            };
-            if (GRAD) store(d0, d1);
-            else store(x0, x1);
+            }
         }
     }
     if (ovf && a.flag) atomicOr(a.flag, 1u);
-    if (GRAD && a.part) {
+    if constexpr (GRAD) {
         // the heads beside each other, then the four waves
-        __shared__ float red[4][2][256];
+        __shared__ float red[4][256];
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int e = 0; e < EC; ++e) {
-                    float u = s0[w][k][e], v = s1[w][k][e];
-                    for (int step = a.lanes; step < 64; step *= 2) u += __shfl_xor(u, step), v += __shfl_xor(v, step);
-                    if (sub == 0) {
-                        if (in[k]) red[threadIdx.x >> 6][w][e0[k] + e] = u;
-                        if (in1[k]) red[threadIdx.x >> 6][w][e1[k] + e] = v;
-                    }
+            for (int e = 0; e < EC; ++e) {
+                float u = s0[k][e], v = s1[k][e];
+                for (int step = a.lanes; step < 64; step *= 2) u += __shfl_xor(u, step), v += __shfl_xor(v, step);
+                if (sub == 0) {
+                    if (in[k]) red[wave][e0[k] + e] = u;
+                    if (in1[k]) red[wave][e1[k] + e] = v;
                 }
+            }
         __syncthreads();
-        for (int c = threadIdx.x; c < 2 * a.d; c += 256) {
-            const int w = c / a.d, e = c - w * a.d;
-            a.part[(long long)blockIdx.x * 2 * a.d + c] = red[0][w][e] + red[1][w][e] + red[2][w][e] + red[3][w][e];
-        }
+        for (int e = threadIdx.x; e < a.d; e += 256)
+            a.part[(long long)blockIdx.x * a.d + e] = red[0][e] + red[1][e] + red[2][e] + red[3][e];
     }
 }
 
-// The gains' gradients: 64 of their elements a workgroup, the partial sums 16
-// rows apart a wave, in order, then the waves'.
+// The gains' gradients: 64 of their elements a workgroup (of q's, then of k's), a
+// sixteenth of the partial sums a wave, in order, then the waves'.
 template <int ST>
-__global__ void __launch_bounds__(1024) rotary_gains_kernel(const float* part, int parts, int d, void* dgq, void* dgk, unsigned* flag) {
+__global__ void __launch_bounds__(1024) rotary_gains_kernel(const float* part, int parts_q, int parts_k, int d, void* dgq, void* dgk, unsigned* flag) {
     __shared__ float red[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+    const int blocks = (d + 63) / 64, second = (int)blockIdx.x >= blocks;
+    const int c = ((int)blockIdx.x - second * blocks) * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+    void* const out = second ? dgk : dgq;
+    if (!out) return;
+    const int first = second ? parts_q : 0, last = first + (second ? parts_k : parts_q);
     float s = 0.f;
-    if (c < 2 * d)
+    if (c < d)
 #pragma unroll 8
-        for (int p = wave; p < parts; p += 16) s += part[(long long)p * 2 * d + c];
+        for (int p = first + wave; p < last; p += 16) s += part[(long long)p * d + c];
     red[wave][threadIdx.x & 63] = s;
     __syncthreads();
-    if (wave || c >= 2 * d) return;
+    if (wave || c >= d) return;
     s = 0.f;
     for (int w = 0; w < 16; ++w) s += red[w][threadIdx.x];
-    void* const out = c < d ? dgq : dgk;
-    if (!out) return;
-    ((typename Elem<ST>::T*)out)[c < d ? c : c - d] = narrow<ST>(s);
+    ((typename Elem<ST>::T*)out)[c] = narrow<ST>(s);
     if (ST == kF16 && flag && pk_overflows_f16(s)) atomicOr(flag, 1u);
 }
 
@@ -331,7 +328,7 @@ struct Plan {
 };
 
 // Workgroups of a gradient with gains: each leaves one row of partial sums, so
-// that they are no more than fill the chip twice.
+// that they are no more than fill the chip.
 constexpr int kParts = 1024;
 
 Plan plan_of(const presk_hip_rot& a, int what) {
@@ -340,8 +337,8 @@ Plan plan_of(const presk_hip_rot& a, int what) {
     p.gains = what == PRESK_HIP_ROT_GRAD && a.norm;
     if (p.gains) {
         const long long waves = a.batch * a.seq * (a.heads + a.kv_heads);
-        p.parts = (int)std::max<long long>(1, std::min<long long>(kParts, (waves + 3) / 4));
-        p.total = (size_t)up(8 * p.parts * a.head_dim, 256);
+        p.parts = (int)std::max<long long>(2, std::min<long long>(kParts, (waves + 3) / 4 + 1));
+        p.total = (size_t)up(4 * p.parts * a.head_dim, 256);
     }
     return p;
 }
@@ -371,15 +368,22 @@ std::vector<PlainBuffer> others(const presk_hip_rot& a, bool grad, int64_t work)
             {"work", a.work, work, 16, true, grad && a.norm}};
 }
 
-template <int ST, bool GRAD>
-hipError_t launch(RotArgs& g, int ec, unsigned grid, hipStream_t s) {
-    if constexpr (ST != kF32)
-        if (ec == 8) {
-            rotary_kernel<ST, 8, GRAD><<<grid, 256, 0, s>>>(g);
-            return hipGetLastError();
-        }
-    if (ec == 4) rotary_kernel<ST, 4, GRAD><<<grid, 256, 0, s>>>(g);
-    else rotary_kernel<ST, 1, GRAD><<<grid, 256, 0, s>>>(g);
+template <int ST, int EC, bool EVEN>
+void launch_mode(const RotArgs& g, RotMode mode, unsigned grid, hipStream_t s) {
+    if (mode == kTurn) rotary_kernel<ST, EC, EVEN, kTurn><<<grid, 256, 0, s>>>(g);
+    else if (mode == kNormed) rotary_kernel<ST, EC, EVEN, kNormed><<<grid, 256, 0, s>>>(g);
+    else rotary_kernel<ST, EC, EVEN, kNormedGrad><<<grid, 256, 0, s>>>(g);
+}
+template <int ST, int EC>
+void launch_even(const RotArgs& g, bool even, RotMode mode, unsigned grid, hipStream_t s) {
+    // (single elements are paired by their places alone)
+    if (even) launch_mode<ST, EC, true>(g, mode, grid, s);
+    else launch_mode<ST, EC, false>(g, mode, grid, s);
+}
+template <int ST>
+hipError_t launch(const RotArgs& g, int ec, bool even, RotMode mode, unsigned grid, hipStream_t s) {
+    if (ec == 4) launch_even<ST, 4>(g, even, mode, grid, s);
+    else launch_even<ST, 1>(g, even, mode, grid, s);
     return hipGetLastError();
 }
 
@@ -429,20 +433,19 @@ hipError_t rotary_run(const presk_hip_rot& a, int what, hipStream_t s) {
     const int esz = p.st == kF32 ? 4 : 2;
     RotArgs g{};
     auto tensor = [](const presk_hip_heads& t) { return RotTensor{t.p, t.batch, t.seq, t.head}; };
-    g.x[0] = tensor(grad ? a.dyq : a.q), g.x[1] = tensor(grad ? a.dyk : a.k);
-    g.y[0] = tensor(grad ? a.dq : a.yq), g.y[1] = tensor(grad ? a.dk : a.yk);
-    g.in[0] = tensor(a.q), g.in[1] = tensor(a.k);
-    g.g[0] = a.gq, g.g[1] = a.gk;
+    g.side[0] = RotSide{tensor(grad ? a.dyq : a.q), tensor(a.q), tensor(grad ? a.dq : a.yq), a.gq, a.dgq, (int)a.heads, 0, 0};
+    g.side[1] = RotSide{tensor(grad ? a.dyk : a.k), tensor(a.k), tensor(grad ? a.dk : a.yk), a.gk, a.dgk, (int)a.kv_heads, 0, 0};
     g.freq = a.freq;
     g.at = (const long long*)a.at;
-    g.batch = (int)a.batch, g.seq = (int)a.seq, g.heads[0] = (int)a.heads, g.heads[1] = (int)a.kv_heads;
-    g.d = (int)a.head_dim, g.rotary = (int)a.rotary, g.norm = a.norm != 0, g.even = a.even != 0;
-    g.eps = (float)a.eps;
+    g.batch = (int)a.batch, g.seq = (int)a.seq, g.d = (int)a.head_dim, g.rotary = (int)a.rotary;
+    g.eps = (float)a.eps, g.per_d = 1.f / (float)a.head_dim, g.sign = grad ? -1.f : 1.f;
     g.flag = a.flag;
+    g.part = (float*)a.work;
     const long long tokens = a.batch * a.seq;
     if (tokens) {
-        // runs of 16 bytes where every tensor's rows, and the halves that are
-        // paired, are whole ones
+        // runs of 4 elements where every tensor's rows, and the halves that are
+        // paired, are whole ones (of 8 in 16 bits the registers hold two waves a SIMD
+        // of a gradient: 83 us, of 4 60; the value 44 and 33)
         auto fits = [&](int ec) {
             if (g.d % (2 * ec) || g.rotary % (2 * ec)) return false;
             for (const HeadsBuffer& b : tensors(a, grad)) {
@@ -451,43 +454,45 @@ hipError_t rotary_run(const presk_hip_rot& a, int what, hipStream_t s) {
             }
             return true;
         };
-        const int ec = p.st != kF32 && fits(8) ? 8 : fits(4) ? 4 : 1;
+        const int ec = fits(4) ? 4 : 1;
         const int pairs = (g.d + 2 * ec - 1) / (2 * ec);
         g.lanes = 1;
         while (g.lanes < pairs && g.lanes < 64) g.lanes *= 2;
         // heads a wave: all of a token's, or as few as keep the chip full
-        const int beside = 64 / g.lanes, total = g.heads[0] + g.heads[1];
-        g.per_wave = (int)up(total, beside);
-        while (g.per_wave > beside && tokens * ((total + g.per_wave - 1) / g.per_wave) < 4096) g.per_wave = (int)up(g.per_wave / 2, beside);
-        g.chunks = (total + g.per_wave - 1) / g.per_wave;
-        const long long waves = tokens * g.chunks;
-        long long grid = (waves + 3) / 4;
-        if (p.gains) {
-            grid = std::min<long long>(grid, p.parts);
-            g.part = (float*)a.work;
-        } else {
-            grid = std::min<long long>(grid, 1 << 20);
+        const int beside = 64 / g.lanes, most = std::max(g.side[0].heads, g.side[1].heads);
+        g.per_wave = (int)up(most, beside);
+        while (g.per_wave > beside && tokens * ((most + g.per_wave - 1) / g.per_wave) < 4096) g.per_wave = (int)up(g.per_wave / 2, beside);
+        long long units[2], all = 0;
+        for (int n = 0; n < 2; ++n) {
+            g.side[n].chunks = (g.side[n].heads + g.per_wave - 1) / g.per_wave;
+            units[n] = tokens * g.side[n].chunks;
+            all += (units[n] + 3) / 4;
         }
-        hipError_t e;
-        if (p.st == kF32) e = grad ? launch<kF32, true>(g, ec, (unsigned)grid, s) : launch<kF32, false>(g, ec, (unsigned)grid, s);
-        else if (p.st == kBF16) e = grad ? launch<kBF16, true>(g, ec, (unsigned)grid, s) : launch<kBF16, false>(g, ec, (unsigned)grid, s);
-        else e = grad ? launch<kF16, true>(g, ec, (unsigned)grid, s) : launch<kF16, false>(g, ec, (unsigned)grid, s);
+        // workgroups: enough for every wave, or, of a gradient with gains, one for
+        // each row of partial sums, shared out by the heads
+        const long long limit = p.gains ? p.parts : 1 << 22;
+        const double share = (double)a.heads / (double)(a.heads + a.kv_heads);
+        for (int n = 0; n < 2; ++n) {
+            const long long need = (units[n] + 3) / 4;
+            const long long part = std::max<long long>(1, (long long)((double)(limit - 1) * (n ? 1.0 - share : share)));
+            g.side[n].blocks = (int)(all <= limit ? need : std::min(need, part));
+        }
+        const unsigned grid = (unsigned)(g.side[0].blocks + g.side[1].blocks);
+        const RotMode mode = !a.norm ? kTurn : grad ? kNormedGrad : kNormed;
+        const bool even = a.even != 0;
+        hipError_t e = p.st == kF32 ? launch<kF32>(g, ec, even, mode, grid, s)
+                       : p.st == kBF16 ? launch<kBF16>(g, ec, even, mode, grid, s)
+                                       : launch<kF16>(g, ec, even, mode, grid, s);
         if (e != hipSuccess) return e;
-        if (!p.gains || (!a.dgq && !a.dgk)) return hipSuccess;
-        const unsigned cols = (unsigned)((2 * g.d + 63) / 64);
-        if (p.st == kF32) rotary_gains_kernel<kF32><<<cols, 1024, 0, s>>>(g.part, (int)grid, g.d, a.dgq, a.dgk, a.flag);
-        else if (p.st == kBF16) rotary_gains_kernel<kBF16><<<cols, 1024, 0, s>>>(g.part, (int)grid, g.d, a.dgq, a.dgk, a.flag);
-        else rotary_gains_kernel<kF16><<<cols, 1024, 0, s>>>(g.part, (int)grid, g.d, a.dgq, a.dgk, a.flag);
-        return hipGetLastError();
     }
-    if (p.gains && (a.dgq || a.dgk)) {
-        // no tokens: the gains' gradients are zero
-        const unsigned cols = (unsigned)((2 * g.d + 63) / 64);
-        if (p.st == kF32) rotary_gains_kernel<kF32><<<cols, 1024, 0, s>>>(nullptr, 0, g.d, a.dgq, a.dgk, nullptr);
-        else rotary_gains_kernel<kBF16><<<cols, 1024, 0, s>>>(nullptr, 0, g.d, a.dgq, a.dgk, nullptr);
-        return hipGetLastError();
-    }
-    return hipSuccess;
+    if (!p.gains || (!a.dgq && !a.dgk)) return hipSuccess;
+    // (of no tokens: zeros)
+    const unsigned cols = 2 * (unsigned)((g.d + 63) / 64);
+    const int pq = g.side[0].blocks, pk = g.side[1].blocks;
+    if (p.st == kF32) rotary_gains_kernel<kF32><<<cols, 1024, 0, s>>>(g.part, pq, pk, g.d, a.dgq, a.dgk, a.flag);
+    else if (p.st == kBF16) rotary_gains_kernel<kBF16><<<cols, 1024, 0, s>>>(g.part, pq, pk, g.d, a.dgq, a.dgk, a.flag);
+    else rotary_gains_kernel<kF16><<<cols, 1024, 0, s>>>(g.part, pq, pk, g.d, a.dgq, a.dgk, a.flag);
+    return hipGetLastError();
 }
 
 }  // namespace presk
