@@ -159,6 +159,9 @@ def storage_inputs(p: Program, host: dict) -> dict:
                 qt = Q.quantize(np.asarray(v, np.float32).astype(np.float64), [a.len for a in axes],
                                 Q.Quant(q.bits, over, q.scheme))
                 env[name], env[name + "#scales"] = qt.data, qt.scales
+            elif ty == "int8":
+                # a mask's bytes
+                env[name] = np.ascontiguousarray(v, dtype=np.uint8).ravel()
             elif np.asarray(v).dtype == np.float64:
                 # the host's f64 values (literals, drawn inputs): one Buf::of
                 env[name] = encode64(np.asarray(v).reshape(-1)[:max(count, 1)], ty)

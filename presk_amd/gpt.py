@@ -290,6 +290,65 @@ class Builder:
         self.input(out["loss"], A(2)), self.input(out["ce"], ax[:-1]), self.input(bufs["lse"], ax[:-1])
         return out
 
+    def _heads_op(self, what: str):
+        """Whether the program may have an operator that is no nest of the
+        interpreter's: in FAST mode and one storage type."""
+        from . import hip
+        if self.p.mode != hip.FAST or self.realize is not None:
+            raise ValueError(f"E7005: {what} is built in FAST mode and one storage type")
+
+    def _bases(self, bufs: dict) -> dict:
+        return {a: self.base.get(b, b) for a, b in bufs.items()}
+
+    def _attention_sizes(self, q, k, heads, kv_heads, causal) -> dict:
+        """hip.Attention's sizes of q [batch, seq, heads * hd] and k [batch, seq, kv_heads * hd]."""
+        (batch, n, model), kx = (a.len for a in self.axes[q]), self.axes[k]
+        return dict(dtype=self.dt, batch=batch, heads=heads, kv_heads=kv_heads, q_len=n, k_len=kx[1].len, head_dim=model // heads,
+                    causal=causal)
+
+    def attention(self, q, k, v, heads: int, kv_heads: int, causal: bool = True, keep: bool = False, name=None):
+        """softmax(q k^T / sqrt(hd)) v of the projections q [batch, seq, heads * hd]
+        and k, v [batch, seq, kv_heads * hd], the weights no buffer of the program,
+        as one step (hip.Attention).  `keep`: also the rows' sums of exponentials,
+        which its gradient reads.  Returns o [batch, seq, heads * hd] and theirs
+        (f32 [batch, heads, seq], or None)."""
+        self._heads_op("attention without its weights")
+        name = self._name(name)
+        bufs = {**self._bases({"q": q, "k": k, "v": v}), "o": name}
+        if keep:
+            bufs["lse"] = name + ".lse"
+        sizes = self._attention_sizes(q, k, heads, kv_heads, causal)
+        self.p.add_attention("value", bufs, **sizes)
+        self.input(name, self.axes[q])
+        if keep:
+            self.input(bufs["lse"], A(("batch", sizes["batch"]), ("heads", heads), ("seq", sizes["q_len"])))
+        return name, bufs.get("lse")
+
+    def attention_vjp(self, q, k, v, o, lse, do, heads: int, kv_heads: int, causal: bool = True, name=None):
+        """The cotangents of q, k and v of `attention`, from its o and lse and o's cotangent."""
+        self._heads_op("attention without its weights")
+        name = self._name(name)
+        out = {"dq": name + ".dq", "dk": name + ".dk", "dv": name + ".dv"}
+        bufs = {**self._bases({"q": q, "k": k, "v": v, "o": o, "lse": lse, "do": do}), **out}
+        self.p.add_attention("vjp", bufs, **self._attention_sizes(q, k, heads, kv_heads, causal))
+        for n, x in zip(out.values(), (q, k, v)):
+            self.input(n, self.axes[x])
+        return tuple(out.values())
+
+    def head_rotary(self, q, k, freq, heads: int, kv_heads: int, name=None):
+        """Each head of the projections q and k turned by its position in the
+        sequence (hip.HeadRotary, `freq` f64 [hd / 2] radians a position): their
+        turned copies."""
+        self._heads_op("a rotation of whole heads")
+        name = self._name(name)
+        batch, n, model = (a.len for a in self.axes[q])
+        out = {"yq": name + ".q", "yk": name + ".k"}
+        self.p.add_head_rotary("value", {**self._bases({"q": q, "k": k, "freq": freq}), **out}, dtype=self.dt, batch=batch, seq=n, heads=heads,
+                               kv_heads=kv_heads, head_dim=model // heads)
+        for b_, x in zip(out.values(), (q, k)):
+            self.input(b_, self.axes[x])
+        return tuple(out.values())
+
     def dropout_mask(self, x, slot: int, rate: float, name=None):
         """`DropoutMask(rate, key, x)`: a mask of x's shape and the site's
         type, drawn from key `slot` of the program's key table."""
@@ -439,7 +498,7 @@ def site_keys(s: GptShape, step_key: bytes) -> list:
 
 
 def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realize=None, dropout: float = 0.0,
-          step_key: bytes | None = None, optimizer: bool = False, fused_head: bool = False) -> tuple:
+          step_key: bytes | None = None, optimizer: bool = False, fused_head: bool = False, fused_attention: bool = False) -> tuple:
     """The program of config 3 (`train=False`: loss only) or config 4.
     Returns (program, builder, names) with names["loss"] and, for training,
     names["grads"][param] = buffer of its gradient.  `realize`: a
@@ -451,7 +510,9 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
     the configs' reading).  `fused_head`: the head, the loss and their
     reverse mode as one step, the logits no buffer of the program (FAST, one
     storage type): names["loss"] is then f32 [2], the mean loss and the counted
-    tokens, and there is no names["logits"]."""
+    tokens, and there is no names["logits"].  `fused_attention`: each layer's
+    attention and its reverse mode as one step each, the weights no buffers of the
+    program (FAST, one storage type, no dropout)."""
     from . import hip, keys
     tag = dtype if realize is None else "mixed"
     p = Program(f"gpt-{'step' if train else 'forward'}-{tag}", mode=hip.FAST if mode is None else mode)
@@ -480,9 +541,11 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
     b.input("two", A())         # real(2) of pow(2)'s and sqrt's adjoints
     b.input("one", A())         # the loss's cotangent
     drop = dropout > 0.0
+    if drop and fused_attention:
+        raise ValueError("E7005: attention without its weights has no dropout of them")
     if drop:
         p.set_keys(site_keys(s, step_key if step_key is not None else keys.from_seed(0)))
-    mask = b.causal_mask(s.T, "mask")
+    mask = None if fused_attention else b.causal_mask(s.T, "mask")
     pos_ids = b.positions(s.T, "pos_ids")
     with b.func("Embedding.apply"):
         te = b.embed("tok", "ids", name="te")
@@ -508,18 +571,23 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
             q = b.dot(xn1, pr + "wq", pr + "wq.b", name=pr + "q")
             k = b.dot(xn1, pr + "wk", pr + "wk.b", name=pr + "k")
             v = b.dot(xn1, pr + "wv", pr + "wv.b", name=pr + "v")
-            qh = b.split_heads(q, H, HD, name=pr + "qh")
-            kh = b.split_heads(k, H, HD, name=pr + "kh")
-            vh = b.split_heads(v, H, HD, name=pr + "vh")
-            sc = b.ein(qh, kh, lbl_q, lbl_k, lbl_s, name=pr + "scores")
-            sc2 = b.binary("div", sc, "scale", name=pr + "scaled")
-            a = b.masked_softmax(sc2, mask, "seq2", name=pr + "probs")
-            ad, ma = a, None
-            if drop:
-                ma = b.dropout_mask(a, 1 + 3 * l, dropout, name=pr + "m.att")
-                ad = b.binary("mul", a, ma, name=pr + "probs_d")
-            o = b.ein(ad, vh, lbl_s, lbl_k, lbl_q, name=pr + "o")
-            om = b.merge_heads(o, H, HD, name=pr + "om")
+            ma = None
+            if fused_attention:
+                qh, kh, vh, a = q, k, v, None
+                om, ad = b.attention(q, k, v, H, H, keep=train, name=pr + "om")      # (ad: the rows' sums)
+            else:
+                qh = b.split_heads(q, H, HD, name=pr + "qh")
+                kh = b.split_heads(k, H, HD, name=pr + "kh")
+                vh = b.split_heads(v, H, HD, name=pr + "vh")
+                sc = b.ein(qh, kh, lbl_q, lbl_k, lbl_s, name=pr + "scores")
+                sc2 = b.binary("div", sc, "scale", name=pr + "scaled")
+                a = b.masked_softmax(sc2, mask, "seq2", name=pr + "probs")
+                ad = a
+                if drop:
+                    ma = b.dropout_mask(a, 1 + 3 * l, dropout, name=pr + "m.att")
+                    ad = b.binary("mul", a, ma, name=pr + "probs_d")
+                o = b.ein(ad, vh, lbl_s, lbl_k, lbl_q, name=pr + "o")
+                om = b.merge_heads(o, H, HD, name=pr + "om")
             ao = b.dot(om, pr + "wo", pr + "wo.b", name=pr + "ao")
         mr = mf = None
         with b.func("Block.apply"):
@@ -587,21 +655,24 @@ def build(s: GptShape, dtype: str = "f32", train: bool = True, mode=None, realiz
             dom = b.dot_vjp_l(dao, pr + "wo")
             G[pr + "wo"] = b.dot_vjp_r(sv["om"], dao, name="d." + pr + "wo")
             G[pr + "wo.b"] = b.sum_to(dao, pr + "wo.b", name="d." + pr + "wo.b")
-            do = b.split_heads(dom, H, HD)
-            da = b.ein(do, sv["vh"], lbl_q, lbl_k, lbl_s, like=sv["a"])
-            dvh = b.ein(do, sv["ad"], lbl_q, lbl_s, lbl_k, like=sv["vh"])
-            # the dropped weights ad = a * ma: a's cotangent da * ma
-            if sv["ma"] is not None:
-                da = b.binary("mul", da, sv["ma"])
-            # softmax: a * (da - broadcast(sum(da * a)))
-            t = b.binary("mul", da, sv["a"])
-            ssum = b.sum(t, "seq2")
-            sb = b.broadcast_like(ssum, da)
-            dsc2 = b.fused([("sub", [("in", 0), ("in", 1)]), ("mul", [("in", 2), ("step", 0)])], [da, sb, sv["a"]], da)
-            dsc = b.binary("div", dsc2, "scale")
-            dqh = b.ein(dsc, sv["kh"], lbl_s, lbl_k, lbl_q, like=sv["qh"])
-            dkh = b.ein(dsc, sv["qh"], lbl_s, lbl_q, lbl_k, like=sv["kh"])
-            dq, dk, dv = b.merge_heads(dqh, H, HD), b.merge_heads(dkh, H, HD), b.merge_heads(dvh, H, HD)
+            if fused_attention:
+                dq, dk, dv = b.attention_vjp(sv["qh"], sv["kh"], sv["vh"], sv["om"], sv["ad"], dom, H, H, name=pr + "att")
+            else:
+                do = b.split_heads(dom, H, HD)
+                da = b.ein(do, sv["vh"], lbl_q, lbl_k, lbl_s, like=sv["a"])
+                dvh = b.ein(do, sv["ad"], lbl_q, lbl_s, lbl_k, like=sv["vh"])
+                # the dropped weights ad = a * ma: a's cotangent da * ma
+                if sv["ma"] is not None:
+                    da = b.binary("mul", da, sv["ma"])
+                # softmax: a * (da - broadcast(sum(da * a)))
+                t = b.binary("mul", da, sv["a"])
+                ssum = b.sum(t, "seq2")
+                sb = b.broadcast_like(ssum, da)
+                dsc2 = b.fused([("sub", [("in", 0), ("in", 1)]), ("mul", [("in", 2), ("step", 0)])], [da, sb, sv["a"]], da)
+                dsc = b.binary("div", dsc2, "scale")
+                dqh = b.ein(dsc, sv["kh"], lbl_s, lbl_k, lbl_q, like=sv["qh"])
+                dkh = b.ein(dsc, sv["qh"], lbl_s, lbl_q, lbl_k, like=sv["kh"])
+                dq, dk, dv = b.merge_heads(dqh, H, HD), b.merge_heads(dkh, H, HD), b.merge_heads(dvh, H, HD)
             dxq = b.dot_vjp_l(dq, pr + "wq")
             dxk = b.dot_vjp_l(dk, pr + "wk")
             dxv = b.dot_vjp_l(dv, pr + "wv")

@@ -132,6 +132,12 @@ def scalar_values(s: LlamaShape) -> dict:
     return {"two": 2.0, "hdr": float(s.HD), "base": float(s.base), "eps": float(s.eps)}
 
 
+def rope_frequencies(s: LlamaShape) -> np.ndarray:
+    """The rotation's radians a position of each pair of a head, f64 [HD / 2]."""
+    from . import hip
+    return hip.rotary_frequencies(s.HD, s.base)
+
+
 def _rmsnorm(b: Builder, x, g, tag):
     """RMSNorm.apply: `let ms = mean(axis model, x * x); x / sqrt(ms + eps) * g`.
     Groups: `x * x` alone (its consumer is a reduction), {ms + eps, sqrt}
@@ -214,6 +220,19 @@ def _attention(b: Builder, s: LlamaShape, pr, x, mask, phi):
         return b.ein(o, w2, la, lb, out_y, name=pr + "ao")
 
 
+def _fused_attention(b: Builder, s: LlamaShape, pr, x):
+    """`_attention` with the rotation of the queries' and keys' heads and the
+    attention one step each (hip.HeadRotary, hip.Attention): the projections' heads
+    stay where the products leave them, [batch, seq, heads, hd]."""
+    with b.func("Attention.apply"):
+        q = b.dot(x, pr + "attn.wq", name=pr + "qp")
+        k = b.dot(x, pr + "attn.wk", name=pr + "kp")
+        v = b.dot(x, pr + "attn.wv", name=pr + "vd")
+        q, k = b.head_rotary(q, k, "rope.freq", s.H, s.G, name=pr + "rot")
+        o, _ = b.attention(q, k, v, s.H, s.G, name=pr + "o")
+        return b.dot(o, pr + "attn.wo", name=pr + "ao")
+
+
 def _swiglu(b: Builder, pr, x):
     """`down.apply(silu(gate.apply(x)) * up.apply(x))`; silu's body
     `x * sigmoid(x)` is one group of its own function."""
@@ -268,12 +287,15 @@ def params_layout(s: LlamaShape):
     return Layout.from_paths(pairs), rename
 
 
-def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None, score: bool = False) -> tuple:
+def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None, score: bool = False,
+          fused_attention: bool = False) -> tuple:
     """The program of `Llama.apply` (the logits).  Returns (program,
     builder, names) with names["logits"].  `score`: the loss of the targets `y`
     (i64 [batch, seq]; negative: not counted) in the logits' place, which are
     not kept (FAST, one storage type): names["ce"] each token's, f32,
-    names["loss"] their mean and number, f32 [2]."""
+    names["loss"] their mean and number, f32 [2].  `fused_attention`: each
+    layer's rotation and attention one step each, the scores and weights no
+    buffers of the program (FAST, one storage type)."""
     from . import hip
     p = Program(f"llama-forward-{dtype if realize is None else 'mixed'}", mode=hip.FAST if mode is None else mode)
     b = Builder(p, dtype, realize)
@@ -291,15 +313,17 @@ def build(s: LlamaShape, dtype: str = "bf16", mode=None, realize=None, score: bo
     b.input("ids", A(("batch", s.B), ("seq", s.T)), "idx")
     for name in SCALARS:
         b.input(name, A())
-    mask = b.causal_mask(s.T, "mask")
+    if fused_attention:
+        b.input("rope.freq", A(("rot", s.HD // 2)))
+    mask = None if fused_attention else b.causal_mask(s.T, "mask")
     with b.func("Llama.apply"):
         x = b.embed("tok", "ids", name="x0")
-    phi = _angles(b, s)
+    phi = None if fused_attention else _angles(b, s)
     for l in range(s.L):
         pr = f"b{l}."
         with b.func("Block.apply"):
             h = _rmsnorm(b, x, pr + "n1.g", pr + "n1")
-            ao = _attention(b, s, pr, h, mask, phi)
+            ao = _fused_attention(b, s, pr, h) if fused_attention else _attention(b, s, pr, h, mask, phi)
             x2 = b.binary("add", x, ao, name=pr + "x")
             h2 = _rmsnorm(b, x2, pr + "n2.g", pr + "n2")
             f = _swiglu(b, pr, h2)
@@ -328,6 +352,7 @@ def host_inputs(s: LlamaShape, seed: int = 5) -> dict:
     out["ids"] = rng.integers(0, s.V, size=(s.B, s.T), dtype=np.int64)
     for k, v in scalar_values(s).items():
         out[k] = np.array([v], np.float64)
+    out["rope.freq"] = rope_frequencies(s)
     return out
 
 
@@ -368,6 +393,7 @@ def load_device_inputs(p: Program, s: LlamaShape, seed: int = 5):
     if "y" in specs:
         host["y"] = rng.integers(0, s.V, size=(s.B, s.T), dtype=np.int64)
     host.update({k: np.array([v], np.float64) for k, v in scalar_values(s).items()})
+    host["rope.freq"] = rope_frequencies(s)
     for name, arr in configs.storage_inputs(p, host).items():
         ty, count = specs[name]
         p.declare(name, ty, max(count, 1))

@@ -137,6 +137,56 @@ class LossStep:
         self.args = self.op.args(self.kind, work=work, flag=flag, **{a: bufs.dev[b] for a, b in self.bufs.items()})
 
 
+class HeadsStep:
+    """Attention or head rotation (`op` hip.Attention or hip.HeadRotary over
+    `sizes`, its constructor's arguments) as a step of a program: `bufs` names the
+    call's buffers; it runs before launch `at`."""
+
+    WRITES = {"Attention": {"value": ("o", "lse"), "vjp": ("dq", "dk", "dv")},
+              "HeadRotary": {"value": ("yq", "yk"), "vjp": ("dq", "dk", "dgq", "dgk")}}
+
+    def __init__(self, at, op, kind, sizes, bufs):
+        self.at, self.name, self.kind, self.sizes, self.bufs = at, op, kind, dict(sizes), dict(bufs)
+        self.op = getattr(hip, op)(**self.sizes)
+        self.args = None
+
+    def specs(self) -> dict:
+        """argument -> (storage type, element count)."""
+        op = self.op
+        out = {a: (op.dtype, op.elements(a)) for a in op._tensors}
+        if self.name == "Attention":
+            out.update(lse=("f32", op.batch * op.heads * op.q_len), lens=("i64", op.batch), first=("i64", op.batch),
+                       mask=("int8", op.batch * op.q_len * op.mask_cols))
+        else:
+            out.update(freq=("f64", op.rotary // 2), at=("i64", op.batch * op.seq))
+            out.update((a, (op.dtype, op.head_dim)) for a in ("gq", "gk", "dgq", "dgk"))
+        return out
+
+    def writes(self) -> list:
+        return [a for a in self.WRITES[self.name][self.kind] if a in self.bufs]
+
+    def reads(self) -> list:
+        return [a for a in self.bufs if a not in self.writes()]
+
+    def prepare(self, bufs: Buffers, flag, name: str):
+        specs = self.specs()
+        for a in self.reads():
+            ty, count = bufs.meta[self.bufs[a]]
+            if ty != specs[a][0] or count < specs[a][1]:
+                raise ValueError(f"E7005: {name} reads {self.bufs[a]}, {ty}[{count}], as {a}, {specs[a][0]}[{specs[a][1]}]")
+        for a in self.writes():
+            bufs.alloc(self.bufs[a], *specs[a])
+        work = bufs.alloc(name + ".work", "int8", self.op.workspace(self.kind)) if self.op._works_for(self.kind) else None
+        self.args = self.op.args(self.kind, work=work, flag=flag, **{a: bufs.dev[b] for a, b in self.bufs.items()})
+
+    def call(self, stream):
+        return self.op._launch(hip.lib())(self.args, hip._HEADS_KINDS[self.kind], stream)
+
+    def record(self, batch):
+        add = getattr(hip.lib(), "presk_hip_batch_add_" + self.op._name)
+        return add(batch, self.args, hip._HEADS_KINDS[self.kind])
+
+
 class Program:
     """Launches in order on one stream; `run` enqueues them all."""
 
@@ -150,7 +200,8 @@ class Program:
         # a host input's storage type when it is not its first reader's (a
         # mixed realization's parameters at rest)
         self.input_types: dict = {}
-        # the prepared sequence: ("launch", Launch), ("loss", LossStep) and,
+        # the prepared sequence: ("launch", Launch), ("loss", LossStep), ("op",
+        # HeadsStep) and,
         # where a kernel reads a buffer of another storage type, ("convert",
         # src, from, dst, to, n)
         self.steps: list = []
@@ -163,8 +214,10 @@ class Program:
         # integer weights: buffer -> (Quant, its quantised axis, its axes),
         # stored as `int8`/`int4` with f32 scales in `<buffer>#scales`
         self.quant: dict = {}
-        # losses of a large vocabulary (LossStep), between the launches
+        # losses of a large vocabulary (LossStep), between the launches, and
+        # attention and head rotations (HeadsStep)
         self.losses: list = []
+        self.ops: list = []
 
     def add_loss(self, kind: str, dtype: str, rows: int, vocab: int, bufs: dict, model: int = 0, top: int = 0, tied: bool = False,
                  temperature: float = 1.0) -> dict:
@@ -177,33 +230,63 @@ class Program:
         st = LossStep(len(self.launches), kind, dtype, int(rows), int(vocab), int(model), int(top), bool(tied), float(temperature), bufs)
         if unknown := sorted(set(bufs) - set(st.specs())):
             raise ValueError(f"a loss has no argument {unknown[0]}")
-        written = {ln.out for ln in self.launches} | {m[0] for m in self.masks} | self._loss_outputs()
-        for a in st.writes():
-            if bufs[a] in written:
-                raise ValueError(f"buffer {bufs[a]}, a loss's {a}, is another step's output")
-            written.add(bufs[a])
-        self.losses.append(st)
+        self._insert(self.losses, st, "a loss's")
         return bufs
 
-    def _loss_outputs(self) -> set:
-        return {st.bufs[a] for st in self.losses for a in st.writes()}
+    def _insert(self, steps: list, st, whose: str):
+        written = {ln.out for ln in self.launches} | {m[0] for m in self.masks} | self._outputs(self.losses) | self._outputs(self.ops)
+        for a in st.writes():
+            if st.bufs[a] in written:
+                raise ValueError(f"buffer {st.bufs[a]}, {whose} {a}, is another step's output")
+            written.add(st.bufs[a])
+        # (steps before the same launch run in the order they came)
+        st.turn = len(self.losses) + len(self.ops)
+        steps.append(st)
+
+    def add_attention(self, kind: str, bufs: dict, **sizes) -> dict:
+        """Appends hip.Attention(**sizes)'s `kind` "value" or "vjp"; `bufs` the
+        buffer of each argument of the call, outputs among them, which no other
+        step writes (tensors dense in the layout).  Returns bufs."""
+        return self._add_op("Attention", "attention's", kind, bufs, sizes)
+
+    def add_head_rotary(self, kind: str, bufs: dict, **sizes) -> dict:
+        """Appends hip.HeadRotary(**sizes)'s `kind` "value" or "vjp", as add_attention."""
+        return self._add_op("HeadRotary", "a rotation's", kind, bufs, sizes)
+
+    def _add_op(self, op, whose, kind, bufs, sizes):
+        if kind not in hip._HEADS_KINDS:
+            raise ValueError(f"{whose} kind is {kind!r}, not {' or '.join(hip._HEADS_KINDS)}")
+        st = HeadsStep(len(self.launches), op, kind, sizes, bufs)
+        if unknown := sorted(set(bufs) - set(st.specs())):
+            raise ValueError(f"{whose} call has no argument {unknown[0]}")
+        self._insert(self.ops, st, whose)
+        return bufs
+
+    @staticmethod
+    def _outputs(steps) -> set:
+        return {st.bufs[a] for st in steps for a in st.writes()}
+
+    def _before(self, i: int) -> list:
+        """The losses and operators that run before launch i, in order."""
+        return sorted((st for st in self.losses + self.ops if st.at == i), key=lambda st: st.turn)
 
     def input_specs(self):
         """(name, (storage type, element count)) of everything a step reads, in
         order; a name read twice comes twice."""
         from .configs import _input_specs
         for i, ln in enumerate(self.launches + [None]):
-            for st in self.losses:
-                if st.at == i:
-                    yield from ((st.bufs[a], st.specs()[a]) for a in st.reads())
+            for st in self._before(i):
+                specs = st.specs()
+                yield from ((st.bufs[a], specs[a]) for a in st.reads())
             if ln is not None:
                 yield from zip(ln.ins, _input_specs(ln.low))
 
     def add(self, low: L.Lowered, ins: list, out: str, scales=()) -> str:
         """Appends one launch of `low` reading buffers `ins`, writing `out`
         (and `scales`, the scales of its integer inputs)."""
-        if out in self._loss_outputs():
-            raise ValueError(f"buffer {out} is a loss's output")
+        for steps, whose in ((self.losses, "a loss's"), (self.ops, "an operator's")):
+            if out in self._outputs(steps):
+                raise ValueError(f"buffer {out} is {whose} output")
         self.launches.append(Launch(low, list(ins), out, scales))
         return out
 
@@ -272,14 +355,14 @@ class Program:
         for name, slot, rate, ty, count in self.masks:
             self.bufs.alloc(name, ty, count)
             self.steps.append(("dropout", name, slot, rate, ty, count))
-        def losses(i):
-            for n, st in enumerate(self.losses):
-                if st.at == i:
-                    st.prepare(self.bufs, self._flag, f"loss{n}")
-                    self.steps.append(("loss", st))
+        def before(i):
+            for st in self._before(i):
+                loss = isinstance(st, LossStep)
+                st.prepare(self.bufs, self._flag, f"loss{self.losses.index(st)}" if loss else f"op{self.ops.index(st)}")
+                self.steps.append(("loss" if loss else "op", st))
 
         for i, ln in enumerate(self.launches):
-            losses(i)
+            before(i)
             c = ln.compiled
             ty = ln.low.dtype if ln.low.out_kind == "real" else "i64"
             names = []
@@ -301,7 +384,7 @@ class Program:
                 ptrs.append(self._flag.ptr)
             ln.table = (ctypes.c_void_p * len(ptrs))(*ptrs)
             self.steps.append(("launch", ln))
-        losses(len(self.launches))
+        before(len(self.launches))
         self._flag.zero()
         return self
 
@@ -345,6 +428,9 @@ class Program:
                 add = lib.presk_hip_batch_add_head_loss if st[1].model else lib.presk_hip_batch_add_distill
                 hip.check(add(b, ctypes.byref(st[1].args), hip.LOSS_WHAT[st[1].kind]))
                 continue
+            if st[0] == "op":
+                hip.check(st[1].record(b))
+                continue
             c = st[1].compiled
             hip.check(lib.presk_hip_batch_add(b, c.handle, st[1].table, 0, max(c.split_bound, 0)))
         if graph:
@@ -376,6 +462,9 @@ class Program:
                 continue
             if st[0] == "loss":
                 self._loss(st, stream)
+                continue
+            if st[0] == "op":
+                hip.check(st[1].call(stream))
                 continue
             c = st[1].compiled
             rc = lib.presk_hip_run(c.handle, st[1].table, 0, max(c.split_bound, 0), stream)
