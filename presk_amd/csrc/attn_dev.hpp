@@ -464,6 +464,12 @@ __device__ __forceinline__ unsigned item_of(unsigned id, unsigned total) {
     return xcd * q8 + (xcd < r8 ? xcd : r8) + id / 8;
 }
 
+// The place of an item among its XCD's.
+__device__ __forceinline__ unsigned turn_of(unsigned item, unsigned total) {
+    const unsigned q8 = total / 8, r8 = total % 8, more = r8 * (q8 + 1);      // (the items of the XCDs that have one more)
+    return item < more ? item % (q8 + 1) : (item - more) % q8;
+}
+
 // Split `split` of the keys [lo, hi): `chunk` of them, the same for sequences of
 // any length, so that its workgroups take equally long or have nothing to do.
 __device__ __forceinline__ void cut(const AttnArgs& a, int split, int* lo, int* hi) {
@@ -518,12 +524,12 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     const int split = (int)(item % (unsigned)a.splits);
     const unsigned at = item / (unsigned)a.splits;
     // a head's tiles from the last on, the longest ones first where they are causal
-    // (where all workgroups are on the chip at once, two a CU, an XCD's second 32
-    // from the first on, so that a CU has a long one and a short one: 32 heads x
-    // 2048 x 128, causal, 71 -> 62 us)
+    // (where all workgroups are on the chip at once, two a CU, the heads that begin
+    // past an XCD's first 32 from the first on, so that a CU has a long one and a short
+    // one: 32 heads x 2048 x 128, causal, 71 -> 62 us)
     const int unit = (int)(at / (unsigned)tiles);
     const int turn = (int)(at % (unsigned)tiles);
-    const bool second = SW == 1 && gridDim.x <= 512 && (int)(blockIdx.x / 8) - (int)(turn * a.splits + split) >= 32;
+    const bool second = SW == 1 && gridDim.x <= 512 && turn_of((unsigned)unit * (unsigned)(tiles * a.splits), gridDim.x) >= 32;
     const int tile = second ? turn : tiles - 1 - turn;
     const int b = unit / groups, hx = unit % groups, hk = hx * a.pack / a.per;
     const int r0 = tile * kAttnTile, r1 = (rows < r0 + kAttnTile ? rows : r0 + kAttnTile) - 1;

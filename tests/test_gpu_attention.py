@@ -76,6 +76,15 @@ def test_heads_that_are_no_whole_vectors(dtype, d):
     run(dtype, *tensors(dtype, 2, 4, 2, 37, 90, d), causal=True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [(5, 20, 20, 300, 300, 64), (3, 14, 7, 1000, 1000, 128), (5, 4, 1, 300, 2000, 64), (1, 7, 7, 640, 2600, 128),
+                                  (9, 16, 2, 55, 600, 80)], ids=str)
+def test_all_workgroups_on_the_chip_at_once(dtype, size):
+    """A number of tiles, or of their shares of the keys, that the XCDs do not divide:
+    each is some workgroup's."""
+    run(dtype, *tensors(dtype, *size, seed=3), causal=True, grad=False)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
 def test_windows(dtype, window):
