@@ -27,7 +27,8 @@ __device__ __forceinline__ unsigned truths(unsigned v) {
 
 // A byte mask's bits by rows and by columns, and which of its blocks of 32 x 32
 // hold any: a wave takes 32 rows and 64 columns, a lane 32 columns of a row, from
-// which a column's bits are a vote.  Reads each byte once (2 x 1024 x 1024 8 us).
+// which a column's bits are a vote.  Reads each byte once (2 x 1024 x 1024 3.8 us,
+// of which 3 are a launch's).
 __global__ void __launch_bounds__(256) attn_mask_kernel(AttnMask m) {
     const int lane = threadIdx.x & 63, blocks = (m.tq + 31) / 32, pairs = (m.words + 1) / 2;
     const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(256) attn_mask_kernel(AttnMask m) {
 
 // What a checked call launches.
 struct Plan {
-    int st, nd, pack = 1, splits = 1, chunk = 0;
+    int st, nd, pack = 1, splits = 1, chunk = 0, parts = 1;
     int words = 0, words_t = 0, nbits = 0;
     size_t bits = 0, bits_t = 0, any = 0, part = 0, ml = 0, rows = 0, total = 0;     // offsets in the workspace
 };
@@ -104,13 +105,32 @@ Plan plan_of(const presk_hip_attn& a, int what) {
     }
     if (grad) {
         p.rows = take(8 * all);
+        // the keys' and values' gradients in parts of their rows, where one
+        // workgroup's tiles of 64 rows are more than a CU's share of all tiles, the
+        // queries' among them (of a causal square's the longest has twice the mean):
+        // to a workgroup a CU, and four tiles each at least (32 heads in groups of
+        // four x 1024 x 128, causal, all gradients: 133 -> 82 us in four parts, 40
+        // heads in groups of eight x 2048: 481 -> 250 in three)
+        const long long units = a.batch * a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile), per = a.heads / a.kv_heads;
+        const long long span = a.window ? std::min<long long>(a.window + kAttnTile, 1 << 28) : 1 << 28;
+        const long long own = per * (up(std::min<long long>(a.q_len, span), 64) / 64);
+        const long long queries = a.batch * a.heads * (up(a.q_len, kAttnTile) / kAttnTile) * (up(std::min<long long>(a.k_len, span), 64) / 64);
+        if (p.nd <= (p.st == kF32 ? 2 : 4) && units && own) {
+            const long long mean = std::max<long long>(1, (units * own + queries) / (a.causal && !a.window ? 512 : 256));
+            p.parts = (int)std::max<long long>(1, std::min({256 / units, own / 4, (own + mean / 2) / mean}));
+        }
+        if (p.parts > 1) p.part = take(8 * p.parts * a.batch * a.kv_heads * a.k_len * p.nd * 32);
         return p;
     }
     const long long per = a.heads / a.kv_heads;
     if (a.q_len < kAttnTile) p.pack = (int)per;
     const long long rows = a.q_len * p.pack, units = a.batch * (a.heads / p.pack);
+    // few rows in shares of the keys that come to four rounds of the CUs, a workgroup
+    // each (32 sequences' single tokens over 8192 keys: 1024 132 us, 768 137, 2048
+    // 145); others to one (8 x 24 drafted tokens over 4096: 34 us with the join, in
+    // two rounds 35, in four 41)
     if (rows <= kAttnFew) p.chunk = chunk_of(units, a.k_len, 1024, 256);
-    else if (up(rows, kAttnTile) / kAttnTile * units < 128) p.chunk = chunk_of(up(rows, kAttnTile) / kAttnTile * units, a.k_len, 512, 256);
+    else if (up(rows, kAttnTile) / kAttnTile * units < 128) p.chunk = chunk_of(up(rows, kAttnTile) / kAttnTile * units, a.k_len, 256, 256);
     p.splits = p.chunk ? (int)std::max<long long>(1, (a.k_len + p.chunk - 1) / p.chunk) : 1;
     if (p.splits > 1) {
         p.part = take(4 * all * p.splits * p.nd * 32);
@@ -239,6 +259,7 @@ hipError_t attn_run(const presk_hip_attn& a, int what, hipStream_t s) {
     g.pack = p.pack;
     g.splits = p.splits;
     g.chunk = p.chunk;
+    g.parts = p.parts;
     g.part = (float*)(work + p.part);
     g.part_ml = (float*)(work + p.ml);
     g.rows = (float*)(work + p.rows);

@@ -57,6 +57,8 @@ struct AttnArgs {
     // rows; the keys are cut into `splits`, whose sums are joined after
     int pack, splits, chunk;     // `chunk` keys a split
     float *part, *part_ml;       // [split][batch][heads][tq][ND * 32] and [split][batch][heads][tq]{max, sum}
+    // the keys' and values' gradients: `parts` of their rows, summed after
+    int parts;                   // (`part`: [dk, dv][part][batch][kv][tk][ND * 32])
     // what the backward pass needs of a row: -lse log2 e and -sum do o
     float* rows;                 // [2][batch][heads][tq]
 };

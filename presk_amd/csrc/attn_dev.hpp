@@ -393,8 +393,8 @@ struct Keys {
 // fewer than 64 keys (or a mask says which).  Such rows have the largest
 // gradients, and theirs are the errors of the stored output too; together with
 // the rounding of the weights' cotangents these pass what the gradients' own
-// rounding adds (documents of 256 tokens in bf16, 1.53 times a float32
-// computation's error, so 1.2).
+// rounding adds (documents of 256 tokens in bf16: 1.53 times the error of a float32
+// computation whose outputs are rounded, in two parts 1.35).
 template <int ST>
 __device__ __forceinline__ bool fine_of(const AttnArgs& a, const Keys& keys, int i0, int i1) {
     return ST != kF32 && (a.cols || keys.hi(a, i0) - keys.lo(a, i0) < 64 || keys.hi(a, i1) - keys.lo(a, i1) < 64);
@@ -464,6 +464,31 @@ __device__ __forceinline__ unsigned item_of(unsigned id, unsigned total) {
     return xcd * q8 + (xcd < r8 ? xcd : r8) + id / 8;
 }
 
+// Item `unit` of the heads, `n` of them a key head: a key head's of all sequences
+// after each other, so that an XCD's run has sequences of different lengths (8 of
+// 704 to 2048 keys, 32 heads in groups of four, all keys: 555 -> 481 us, the
+// gradients 1740 -> 1510; 8 of 128 to 1024, 16 heads: 84 -> 67, 261 -> 216).
+__device__ __forceinline__ void head_of(const AttnArgs& a, int unit, int n, int* b, int* hk, int* head) {
+    const int at = unit / n;
+    *b = at % a.batch;
+    *hk = at / a.batch;
+    *head = *hk * n + unit % n;
+}
+
+// A share of a sequence's keys and its key head, of workgroups that have the whole
+// group's rows: a share's heads, whose rows lie beside each other, on one XCD; a
+// sequence's shares on different ones, a longer sequence's last ones in the end (32
+// sequences of 2048 to 8192 keys, 8 key heads x 128: 150 us where an XCD has a run
+// of a head's shares, 140 a run of a sequence's, 132 so).
+__device__ __forceinline__ void share_of(const AttnArgs& a, unsigned id, int* b, int* hk, int* split) {
+    const unsigned kv = (unsigned)a.kv, batch = (unsigned)a.batch, rounds = batch * (unsigned)a.splits / 8, whole = 8 * rounds * kv;
+    const unsigned at = id < whole ? id / 8 : id - whole;
+    const unsigned share = id < whole ? at / kv * 8 + id % 8 : 8 * rounds + at / kv;
+    *hk = (int)(at % kv);
+    *split = (int)(share / batch);
+    *b = (int)((share % batch + batch - (unsigned)*split % batch) % batch);
+}
+
 // The place of an item among its XCD's.
 __device__ __forceinline__ unsigned turn_of(unsigned item, unsigned total) {
     const unsigned q8 = total / 8, r8 = total % 8, more = r8 * (q8 + 1);      // (the items of the XCDs that have one more)
@@ -504,14 +529,22 @@ __device__ __forceinline__ void take(const unsigned char* at, int lane, f32x16 (
         }
 }
 
+// f32's heads of 64 elements in tiles of 32 keys, so that a CU has three workgroups
+// (64 x 6 heads x 256 x 64, causal: 66 -> 63 us, the gradient 90 -> 87)
+template <int ST, int ND, int SW>
+constexpr bool three() { return ST == kF32 && ND == 2 && SW == 1; }
+template <int ST, int ND, int SW>
+constexpr int tile_of() { return three<ST, ND, SW>() ? 32 : Geo<ST, ND>::TILE; }
+
 // One workgroup: 128 rows of a head (of a group's heads beside each other), 32 a
 // wave, over the keys that any of them reads, or a share of those.  SW 2: eight
 // waves, two of which share 32 rows and take half of each tile's keys each.
 template <int ST, int ND, int SW>
-__global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : 2) attn_fwd_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, G::TILE, 256 * SW> Tile;
-    constexpr int NB = G::TILE / 32 / SW;
+    constexpr int TILE = tile_of<ST, ND, SW>();
+    typedef Rows<ST, ND, TILE, 256 * SW> Tile;
+    constexpr int NB = TILE / 32 / SW;
     static_assert(NB >= 1, "a tile has a block for each");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES + (SW == 2 ? 2048 : 0)];
     constexpr int PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;     // of LDS for the waves of the same rows
@@ -519,7 +552,7 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int rw = wave & 3, kw = wave >> 2;      // which rows, and which of a tile's keys
-    const int rows = a.tq * a.pack, tiles = (rows + kAttnTile - 1) / kAttnTile, groups = a.heads / a.pack;
+    const int rows = a.tq * a.pack, tiles = (rows + kAttnTile - 1) / kAttnTile;
     const unsigned item = item_of(blockIdx.x, gridDim.x);
     const int split = (int)(item % (unsigned)a.splits);
     const unsigned at = item / (unsigned)a.splits;
@@ -531,7 +564,8 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     const int turn = (int)(at % (unsigned)tiles);
     const bool second = SW == 1 && gridDim.x <= 512 && turn_of((unsigned)unit * (unsigned)(tiles * a.splits), gridDim.x) >= 32;
     const int tile = second ? turn : tiles - 1 - turn;
-    const int b = unit / groups, hx = unit % groups, hk = hx * a.pack / a.per;
+    int b, hk, hx;
+    head_of(a, unit, a.per / a.pack, &b, &hk, &hx);
     const int r0 = tile * kAttnTile, r1 = (rows < r0 + kAttnTile ? rows : r0 + kAttnTile) - 1;
 
     Keys keys;
@@ -540,10 +574,10 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     int klo = keys.lo(a, ifirst), khi = keys.hi(a, ilast);
     by_mask(a, keys, b, ifirst, ilast, &klo, &khi);
     const int surelo = keys.lo(a, ilast), surehi = keys.sure(a, ifirst);
-    int nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
+    int nt = khi > klo ? (khi - klo + TILE - 1) / TILE : 0;
     if (a.splits > 1) {
         cut(a, split, &klo, &khi);
-        nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
+        nt = khi > klo ? (khi - klo + TILE - 1) / TILE : 0;
     }
 
     // this lane's row
@@ -559,7 +593,7 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     vt.init(a.v, b, hk, a.d, tid, lds + Tile::BYTES);
     auto fetch = [&](int t) {
         const unsigned stage = (unsigned)(t & 1) * 2 * Tile::BYTES;
-        const int k0 = klo + t * G::TILE;
+        const int k0 = klo + t * TILE;
         kt.issue(k0, khi - k0, stage, smem, tid);
         vt.issue(k0, khi - k0, stage, smem + Tile::BYTES, tid);
     };
@@ -584,10 +618,10 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     auto load_bits = [&](int t) {
         if (a.cols)
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) ahead[kb].load(a.bits, line, a.words, klo + t * G::TILE + (kw * NB + kb) * 32 - keys.first);
+            for (int kb = 0; kb < NB; ++kb) ahead[kb].load(a.bits, line, a.words, klo + t * TILE + (kw * NB + kb) * 32 - keys.first);
     };
     auto body = [&](bool masked, int t) {
-        const int k0 = klo + t * G::TILE;
+        const int k0 = klo + t * TILE;
         const Places<ST, ND> at = places.from((unsigned)((t & 1) * 2 * Tile::BYTES + kw * NB * 32 * G::ROW));
         f32x16 s[NB];
         bool any[NB];
@@ -658,8 +692,8 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
             fetch(t + 1);
             load_bits(t + 1);
         }
-        const int k0 = klo + t * G::TILE;
-        body(k0 < surelo || k0 + G::TILE > surehi, t);
+        const int k0 = klo + t * TILE;
+        body(k0 < surelo || k0 + TILE > surehi, t);
     }
 
     l += partner<32>(l);
@@ -683,14 +717,14 @@ __global__ void __launch_bounds__(256 * SW, 2) attn_fwd_kernel(AttnArgs a) {
     const long long row = ((long long)b * a.heads + head) * a.tq + i;
     if (a.splits > 1) {
         const long long all = (long long)a.batch * a.heads * a.tq, n = (long long)split * all + row;
-        if (live) {
+        if (live && h == 0) *(f32x2*)(a.part_ml + 2 * n) = f32x2{m, l};
+        if (live && l != 0.f) {     // (the join reads no sums of a row without keys)
             float* const out = a.part + n * (ND * 32);
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *(f32x4*)(out + dt * 32 + 8 * g + 4 * h) = f32x4{o[0][dt][4 * g], o[0][dt][4 * g + 1], o[0][dt][4 * g + 2], o[0][dt][4 * g + 3]};
-            if (h == 0) *(f32x2*)(a.part_ml + 2 * n) = f32x2{m, l};
         }
         return;
     }
@@ -726,10 +760,9 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
     __shared__ float ml[NW][32][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
-    const int rows = a.tq * a.pack, groups = a.heads / a.pack;
-    const unsigned item = item_of(blockIdx.x, gridDim.x);
-    const int split = (int)(item % (unsigned)a.splits), unit = (int)(item / (unsigned)a.splits);
-    const int b = unit / groups, hx = unit % groups, hk = hx * a.pack / a.per;
+    const int rows = a.tq * a.pack;
+    int b, hk, split;
+    share_of(a, blockIdx.x, &b, &hk, &split);
 
     Keys keys;
     keys.init(a, b);
@@ -753,7 +786,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
     // this lane's row
     const int r = lane & 31;
     const bool live = r < rows;
-    const int i = live ? r / a.pack : a.tq - 1, head = hx * a.pack + (live ? r % a.pack : 0);
+    const int i = live ? r / a.pack : a.tq - 1, head = hk * a.pack + (live ? r % a.pack : 0);
     const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
     const unsigned line = (unsigned)((b * a.bits_batch + i) * a.words);
     typename FragOf<ST>::T q[G::STEPS];
@@ -870,37 +903,60 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
 }
 
 // The splits' sums of a row joined, in order: by a wave (64 lanes, ND / 2 elements a
-// lane), or, of many splits, by a workgroup's four, a quarter of them each.
+// lane), or, of many splits, by a workgroup's four, every fourth of them each.  A
+// lane takes a split's maximum and sum, then all lanes the sums of those splits
+// that have any, four loads at a time on the way.
 template <int ST, int ND, int WAVES>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+    constexpr int E = ND / 2;
+    typedef float V __attribute__((ext_vector_type(E)));
     __shared__ float sums[4][ND * 32], sl[4];
     const long long all = (long long)a.batch * a.heads * a.tq;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long row = WAVES == 4 ? blockIdx.x : (long long)blockIdx.x * 4 + wave;
     if (row >= all) return;
     const f32x2* const mls = (const f32x2*)a.part_ml + row;
-    float m = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, mls[s * all][0]);
+    const int first = WAVES == 4 ? wave : 0;
+    f32x2 ml = f32x2{-INFINITY, 0.f};
+    if (first + WAVES * lane < a.splits) ml = mls[(first + WAVES * lane) * all];
+    float m = ml[0];
+    for (int s = WAVES == 4 ? lane : lane + 64; s < a.splits; s += 64) m = fmaxf(m, mls[s * all][0]);
     m = all_of<64>(m, nullptr, max_f);
     const float base = base_of(m);
-    float l = 0.f, x[ND / 2];
+    float l = 0.f, x[E];
 #pragma unroll
-    for (int q = 0; q < ND / 2; ++q) x[q] = 0.f;
-#pragma unroll 4
-    for (int s = WAVES == 4 ? wave : 0; s < a.splits; s += WAVES) {
-        const f32x2 v = mls[s * all];
-        const float f = __builtin_amdgcn_exp2f(v[0] - base);
-        l += v[1] * f;
+    for (int q = 0; q < E; ++q) x[q] = 0.f;
+    for (int s0 = first; s0 < a.splits; s0 += 64 * WAVES) {
+        if (s0 > first) ml = s0 + WAVES * lane < a.splits ? mls[(s0 + WAVES * lane) * all] : f32x2{-INFINITY, 0.f};
+        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+        l += ml[1] * f;
         // (a split without keys has no sums)
+        for (unsigned long long have = __ballot(ml[1] != 0.f); have;) {
+            const int n = __builtin_popcountll(have);
+            V v[4];
+            float g[4];
 #pragma unroll
-        for (int q = 0; q < ND / 2; ++q) x[q] += v[1] == 0.f ? 0.f : a.part[(s * all + row) * (ND * 32) + q * 64 + lane] * f;
+            for (int j = 0; j < 4; ++j) {
+                const int k = __builtin_ctzll(have);
+                g[j] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
+                v[j] = *((const V*)(a.part + ((s0 + WAVES * k) * all + row) * (ND * 32)) + lane);
+                if (j < 3 && j + 1 < n) have &= have - 1;
+            }
+            have &= have - 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < n)
+#pragma unroll
+                    for (int q = 0; q < E; ++q) x[q] += v[j][q] * g[j];
+        }
     }
+    l = all_of<64>(l, nullptr, add_f);
     const int i = (int)(row % a.tq), head = (int)(row / a.tq % a.heads), b = (int)(row / a.tq / a.heads);
     void* const out = const_cast<void*>(row_at<ST>(a.o, b, i, head));
     bool ovf = false;
     if constexpr (WAVES == 4) {
 #pragma unroll
-        for (int q = 0; q < ND / 2; ++q) sums[wave][q * 64 + lane] = x[q];
+        for (int q = 0; q < E; ++q) sums[wave][E * lane + q] = x[q];
         if (lane == 0) sl[wave] = l;
         __syncthreads();
         l = sl[0] + sl[1] + sl[2] + sl[3];
@@ -911,7 +967,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
             ovf |= put<ST, ND>(out, at, a.d, (sums[0][at] + sums[1][at] + sums[2][at] + sums[3][at]) * f);
     } else {
 #pragma unroll
-        for (int q = 0; q < ND / 2; ++q) ovf |= put<ST, ND>(out, q * 64 + lane, a.d, x[q] * f);
+        for (int q = 0; q < E; ++q) ovf |= put<ST, ND>(out, E * lane + q, a.d, x[q] * f);
     }
     if (ovf && a.flag) atomicOr(a.flag, 1u);
     if (a.lse && (WAVES == 4 ? threadIdx.x : lane) == 0) a.lse[row] = l == 0.f ? -INFINITY : (base + __builtin_log2f(l)) * kLn2;
@@ -959,20 +1015,23 @@ constexpr float kShift = 8.f;
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
 // the queries'.
 template <int ST, int ND, int SW>
-__global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
+constexpr int dq_lds() { return 4 * Rows<ST, ND, tile_of<ST, ND, SW>(), 256 * SW>::BYTES; }
+template <int ST, int ND, int SW>
+__device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned total, unsigned char* smem) {
     typedef Geo<ST, ND> G;
-    typedef Rows<ST, ND, G::TILE, 256 * SW> Tile;
+    constexpr int TILE = tile_of<ST, ND, SW>();
+    typedef Rows<ST, ND, TILE, 256 * SW> Tile;
     constexpr int NB = 1;
     constexpr int WROWS = 32 * NB, ROWS = 4 * WROWS, PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;
     static_assert(4 * Tile::BYTES >= 4 * PAIR, "the waves' sums in LDS");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Tile::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int rw = wave & 3, kw = wave >> 2;      // which rows, and which of a tile's keys
     const int tiles = (a.tq + ROWS - 1) / ROWS;
-    const unsigned at = item_of(blockIdx.x, gridDim.x);
+    const unsigned at = item_of(id, total);
     const int tile = tiles - 1 - (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
-    const int b = unit / a.heads, head = unit % a.heads, hk = head / a.per;
+    int b, hk, head;
+    head_of(a, unit, a.per, &b, &hk, &head);
     const int r0 = tile * ROWS, r1 = (a.tq < r0 + ROWS ? a.tq : r0 + ROWS) - 1;
 
     Keys keys;
@@ -980,7 +1039,7 @@ __global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ?
     int klo = keys.lo(a, r0), khi = keys.hi(a, r1);
     by_mask(a, keys, b, r0, r1, &klo, &khi);
     const int surelo = keys.lo(a, r1), surehi = keys.sure(a, r0);
-    const int nt = khi > klo ? (khi - klo + G::TILE - 1) / G::TILE : 0;
+    const int nt = khi > klo ? (khi - klo + TILE - 1) / TILE : 0;
 
     Tile kt, vt;
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
@@ -988,7 +1047,7 @@ __global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ?
     vt.init(a.v, b, hk, a.d, tid, lds + Tile::BYTES);
     auto fetch = [&](int t) {
         const unsigned stage = (unsigned)(t & 1) * 2 * Tile::BYTES;
-        const int k0 = klo + t * G::TILE;
+        const int k0 = klo + t * TILE;
         kt.issue(k0, khi - k0, stage, smem, tid);
         vt.issue(k0, khi - k0, stage, smem + Tile::BYTES, tid);
     };
@@ -1016,16 +1075,16 @@ __global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ?
     Places<ST, ND> places;
     places.init(lane);
     places = places.from(lds);
-    constexpr int MINE = G::TILE / 32 / SW;     // blocks of a tile that are the wave's
+    constexpr int MINE = TILE / 32 / SW;     // blocks of a tile that are the wave's
     MaskBits ahead[MINE], now[MINE];
     const unsigned line = (unsigned)((b * a.bits_batch + (w0 + (lane & 31) <= r1 ? w0 + (lane & 31) : r1)) * a.words);
     auto load_bits = [&](int t) {
         if (a.cols)
 #pragma unroll
-            for (int x = 0; x < MINE; ++x) ahead[x].load(a.bits, line, a.words, klo + t * G::TILE + (kw + SW * x) * 32 - keys.first);
+            for (int x = 0; x < MINE; ++x) ahead[x].load(a.bits, line, a.words, klo + t * TILE + (kw + SW * x) * 32 - keys.first);
     };
     auto body = [&](bool masked, int t, int kb) {
-        const int base = klo + t * G::TILE + kb * 32;
+        const int base = klo + t * TILE + kb * 32;
         const Places<ST, ND> at = places.from((unsigned)((t & 1) * 2 * Tile::BYTES + kb * 32 * G::ROW));
         unsigned bits[NB];
         if (masked) {
@@ -1085,9 +1144,9 @@ __global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ?
             fetch(t + 1);
             load_bits(t + 1);
         }
-        const int k0 = klo + t * G::TILE;
+        const int k0 = klo + t * TILE;
 #pragma unroll 1
-        for (int kb = kw; kb < G::TILE / 32; kb += SW) body(k0 < surelo || k0 + G::TILE > surehi, t, kb);
+        for (int kb = kw; kb < TILE / 32; kb += SW) body(k0 < surelo || k0 + TILE > surehi, t, kb);
     }
     __syncthreads();
     unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same rows
@@ -1107,22 +1166,32 @@ __global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ?
 // pass by, QT at a time.  SW 2: eight waves, two of which share 32 keys and take
 // half of each tile's rows each.  VL: the values are kept in LDS, as the registers
 // that two waves a SIMD have do not hold them too, and with eight waves, whose one
-// workgroup a CU has the room, the keys beside them.
-template <int ST, int ND, int SW, int QT, bool DK, bool DV, bool VL, int OCC>
-__global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
+// workgroup a CU has the room, the keys beside them.  DQ: the queries' workgroups
+// follow the `nkv` of the keys in one launch, where either would leave CUs idle
+// (3 x 10 heads, 5 of keys, 777 x 1021 x 80, 120 and 210 workgroups: 38 + 18 -> 41
+// us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves a
+// tile's rows may be in parts of theirs (AttnArgs::parts), whose sums in f32
+// attn_sum_kernel adds.
+template <int ST, int ND, int SW, int QT, bool DK, bool DV, bool VL, int OCC, bool DQ>
+__global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, unsigned nkv) {
     typedef Geo<ST, ND> G;
     typedef Rows<ST, ND, QT, 256 * SW> Tile;
     constexpr int NB = 1, WKEYS = 32 * NB, KEYS = 4 * WKEYS, STAGE = 2 * Tile::BYTES + 512, PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;
     typedef Rows<ST, ND, KEYS, 256 * SW> Kept;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + (VL ? SW * Kept::BYTES : 0)];
     constexpr bool KL = VL && SW == 2;
+    constexpr int MINE_LDS = 2 * STAGE + (VL ? SW * Kept::BYTES : 0);
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[DQ && dq_lds<ST, ND, SW>() > MINE_LDS ? dq_lds<ST, ND, SW>() : MINE_LDS];
+    if constexpr (DQ)
+        if (blockIdx.x >= nkv) return dq_of<ST, ND, SW>(a, blockIdx.x - nkv, gridDim.x - nkv, smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int rw = wave & 3, kw = wave >> 2;      // which keys, and which of a tile's rows
     const int tiles = (a.tk + KEYS - 1) / KEYS;
-    const unsigned at = item_of(blockIdx.x, gridDim.x);
+    unsigned at = item_of(blockIdx.x, DQ ? nkv : gridDim.x);
+    const int part = SW == 2 ? (int)(at % (unsigned)a.parts) : 0;
+    if (SW == 2) at /= (unsigned)a.parts;
     const int tile = (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
-    const int b = unit / a.kv, hk = unit % a.kv;
+    const int b = unit % a.batch, hk = unit / a.batch;
     const int k0 = tile * KEYS, k1 = a.tk < k0 + KEYS ? a.tk : k0 + KEYS;
 
     Keys keys;
@@ -1148,19 +1217,28 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
         ilo *= 32;
         ihi = 32 * ihi < a.tq ? 32 * ihi : a.tq;
     }
-    const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0, nt = nt1 * a.per;
+    // tiles of rows, head after head, and of those this part's [t0, nt)
+    const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0;
+    int nt = nt1 * a.per, t0 = 0;
+    int fi = ilo, fg = 0;       // the next tile's first row, and its head in the group
+    if (SW == 2 && a.parts > 1) {
+        const int share = (nt + a.parts - 1) / a.parts;
+        t0 = part * share < nt ? part * share : nt;
+        nt = t0 + share < nt ? t0 + share : nt;
+        if (t0 < nt) fi = ilo + t0 % nt1 * QT, fg = t0 / nt1;
+    }
+    const int i00 = fi;
     const int jw = k0 + rw * WKEYS;      // the wave's first key
     queries(jw, jw + WKEYS < k1 ? jw + WKEYS : k1, &wlo, &whi);
 
     Tile qt, dt_;
     const unsigned lds = (unsigned)(size_t)(lds_void_t*)smem;
-    int fi = ilo, fg = 0;       // the next tile's first row, and its head in the group
     auto fetch = [&](int t) {
         const int i0 = fi, head = hk * a.per + fg;
         const unsigned stage = (unsigned)(t & 1) * STAGE;
         fi += QT;
         if (fi >= ihi) fi = ilo, ++fg;
-        if (i0 == ilo) {
+        if (i0 == ilo || t == t0) {
             qt.init(a.q, b, head, a.d, tid, lds);
             dt_.init(a.dout, b, head, a.d, tid, lds + Tile::BYTES);
         }
@@ -1189,7 +1267,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
         for (int dt = 0; dt < ND; ++dt) dk[n][dt] = dv[n][dt] = f32x16{};
     }
     if (!a.k.vec || !a.v.vec) __syncthreads();
-    if (nt > 0) {
+    if (nt > t0) {
         if (VL) {
             Kept vt;
             vt.init(a.v, b, hk, a.d, tid, lds);
@@ -1199,7 +1277,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
                 vt.issue(k0, (k1 < keys.len ? k1 : keys.len) - k0, 2 * STAGE + Kept::BYTES, smem, tid);
             }
         }
-        fetch(0);
+        fetch(t0);
     }
 
     // a mask's words of this lane's key (its rows come 32 at a time from a multiple
@@ -1313,8 +1391,8 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
                 }
         }
     };
-    if (nt > 0) load_bits(ilo);
-    for (int t = 0, ti = ilo; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
+    if (nt > t0) load_bits(i00);
+    for (int t = t0, ti = i00; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
         wait_vm<0>();
         if (a.cols)
 #pragma unroll
@@ -1354,6 +1432,19 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
     if (j >= keys.len)
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) dk[0][dt] = dv[0][dt] = f32x16{};
+    if (SW == 2 && a.parts > 1) {
+        // (kw 0: the waves that have both halves)
+        const long long all = (long long)a.batch * a.kv * a.tk, row = part * all + ((long long)b * a.kv + hk) * a.tk + j;
+        if (exists)
+#pragma unroll
+            for (int g = 0; g < 4 * ND; ++g) {
+                float* const to = a.part + row * (ND * 32) + g / 4 * 32 + 8 * (g & 3) + 4 * h;
+                const f32x16 &x = dk[0][g / 4], &y = dv[0][g / 4];
+                *(f32x4*)to = f32x4{x[g % 4 * 4], x[g % 4 * 4 + 1], x[g % 4 * 4 + 2], x[g % 4 * 4 + 3]};
+                *(f32x4*)(to + a.parts * all * (ND * 32)) = f32x4{y[g % 4 * 4], y[g % 4 * 4 + 1], y[g % 4 * 4 + 2], y[g % 4 * 4 + 3]};
+            }
+        return;
+    }
     auto where = [&](const AttnTensor& t) {
         return [&, t](int x) -> const void* { return jw + x < k1 ? row_at<ST>(t, b, jw + x, hk) : nullptr; };
     };
@@ -1361,12 +1452,55 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a) {
     if (DV && a.dv.p) store_kept<ST, ND>(dv[0], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), pair, lane, a.flag);
 }
 
+template <int ST, int ND, int SW>
+__global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : ND >= 8 || (ST == kF32 && ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[dq_lds<ST, ND, SW>()];
+    dq_of<ST, ND, SW>(a, blockIdx.x, gridDim.x, smem);
+}
+// The parts of the keys' and values' gradients summed, in order: four elements a
+// thread, all of the one tensor's before the other's.
+template <int ST, int ND>
+__global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
+    const long long all = (long long)a.batch * a.kv * a.tk, n = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = n / (8 * ND), line = row % all;
+    if (row >= 2 * all) return;
+    const bool value = row >= all;
+    const AttnTensor& t = value ? a.dv : a.dk;
+    const int at = (int)(n % (8 * ND)) * 4;
+    if (!t.p || (ST != kF32 && at >= a.d)) return;
+    const float* const from = a.part + ((value ? a.parts : 0) * all + line) * (ND * 32) + at;
+    f32x4 x = f32x4{};
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) {
+        const f32x4 y = *(const f32x4*)(from + p * all * (ND * 32));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += y[e];
+    }
+    const float f = value ? ST == kF16 ? 0.00390625f : 1.f : a.scale;
+    const int j = (int)(line % a.tk), hk = (int)(line / a.tk % a.kv), b = (int)(line / a.tk / a.kv);
+    void* const out = const_cast<void*>(row_at<ST>(t, b, j, hk));
+    bool ovf = false;
+    if (ST != kF32 && t.vec) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] *= f;
+            ovf |= ST == kF16 && pk_overflows_f16(x[e]);
+        }
+        if constexpr (ST != kF32)
+            *(unsigned long long*)((unsigned short*)out + at) = pack2<ST>(x[0], x[1]) | (unsigned long long)pack2<ST>(x[2], x[3]) << 32;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ovf |= put<ST, ND>(out, at + e, a.d, x[e] * f);
+    }
+    if (ovf && a.flag) atomicOr(a.flag, 1u);
+}
+
 // ---- launches -----------------------------------------------------------------------------
 
 // Workgroups of eight waves where four would leave SIMDs with a wave or none, which
 // then waits for its own results: where a round of the CUs holds them all (2 x 12
-// heads x 1024 x 64, 192 of them, 27 -> 17 us), and causal ones of up to two, whose
-// longest would be by themselves in the end.
+// heads x 1024 x 64 with a mask, 192 of them: the value 27 -> 20 us, the queries'
+// gradient 35 -> 24, the keys' 38 -> 27; of 384 of them, causal, 23 -> 26).
 template <int ST, int ND>
 bool eight(long long grid) {
     return Geo<ST, ND>::TILE == 64 && grid <= 256;
@@ -1397,26 +1531,35 @@ template <int ST, int ND>
 hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     const long long all = (long long)a.batch * a.heads * a.tq;
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
-    if (a.dq.p && all) {
-        const long long grid = (long long)((a.tq + 127) / 128) * a.batch * a.heads;
-        if (eight<ST, ND>(grid)) {
-            if constexpr (Geo<ST, ND>::TILE == 64) attn_dq_kernel<ST, ND, 2><<<(unsigned)grid, 512, 0, s>>>(a);
+    const long long nq = a.dq.p ? (long long)((a.tq + 127) / 128) * a.batch * a.heads : 0;
+    long long nkv = a.dk.p || a.dv.p ? (long long)((a.tk + 127) / 128) * a.batch * a.kv * a.parts : 0;
+    if constexpr (Geo<ST, ND>::TILE == 64)
+        if (nkv && eight<ST, ND>(nkv)) {
+            if (nq && nq <= 1024) attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
+            else attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
+            if (a.parts > 1) {
+                const long long n = 2LL * a.batch * a.kv * a.tk * 8 * ND;
+                attn_sum_kernel<ST, ND><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+            }
+            if (!nq || nq <= 1024) return hipGetLastError();
+            nkv = 0;
+        }
+    if (nq) {
+        if (eight<ST, ND>(nq)) {
+            if constexpr (Geo<ST, ND>::TILE == 64) attn_dq_kernel<ST, ND, 2><<<(unsigned)nq, 512, 0, s>>>(a);
         } else {
-            attn_dq_kernel<ST, ND, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+            attn_dq_kernel<ST, ND, 1><<<(unsigned)nq, 256, 0, s>>>(a);
         }
     }
-    if ((a.dk.p || a.dv.p) && a.batch && a.tk) {
-        const long long grid = (long long)((a.tk + 127) / 128) * a.batch * a.kv;
+    if (nkv) {
         if constexpr (ND == 8) {
             // (both sums of 256 elements and both kept rows do not fit the registers)
-            if (a.dk.p) attn_dkv_kernel<ST, ND, 1, 32, true, false, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
-            if (a.dv.p) attn_dkv_kernel<ST, ND, 1, 32, false, true, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
+            if (a.dk.p) attn_dkv_kernel<ST, ND, 1, 32, true, false, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
+            if (a.dv.p) attn_dkv_kernel<ST, ND, 1, 32, false, true, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         } else if constexpr (ST == kF32 && ND == 4) {
-            attn_dkv_kernel<ST, ND, 1, 32, true, true, false, 1><<<(unsigned)grid, 256, 0, s>>>(a);
-        } else if (eight<ST, ND>(grid)) {
-            attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2><<<(unsigned)grid, 512, 0, s>>>(a);
+            attn_dkv_kernel<ST, ND, 1, 32, true, true, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         } else {
-            attn_dkv_kernel<ST, ND, 1, ND == 4 ? 32 : 64, true, true, ND == 4, 2><<<(unsigned)grid, 256, 0, s>>>(a);
+            attn_dkv_kernel<ST, ND, 1, ND == 4 ? 32 : 64, true, true, ND == 4, 2, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         }
     }
     return hipGetLastError();

@@ -85,6 +85,32 @@ def test_all_workgroups_on_the_chip_at_once(dtype, size):
     run(dtype, *tensors(dtype, *size, seed=3), causal=True, grad=False)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["all", "causal", "window", "lengths", "mask", "dk", "dv"])
+@pytest.mark.parametrize("d", [20, 64, 128])
+def test_few_keys_and_many_rows(dtype, kind, d):
+    """Keys' gradients that one workgroup a tile would leave CUs idle for: in parts
+    of the rows, of which some may have none."""
+    b, h, kv, tq, tk = 2, 6, 2, 610, 200
+    q, k, v, do = tensors(dtype, b, h, kv, tq, tk, d, seed=d)
+    g = torch.Generator().manual_seed(d)
+    if kind in ("dk", "dv"):
+        hip.init(0)
+        op = hip.Attention(dtype, b, h, kv, tq, tk, d)
+        Q, K, V, DO = (x.to(DEV) for x in (q, k, v, do))
+        o, lse = torch.empty_like(Q), torch.empty(b, h, tq, device=DEV)
+        op.value(Q, K, V, o, lse=lse)
+        both = {"dk": torch.empty_like(K), "dv": torch.empty_like(V)}
+        op.vjp(Q, K, V, o, lse, DO, **both)
+        alone = torch.full_like(K, 9.0)
+        op.vjp(Q, K, V, o, lse, DO, **{kind: alone})
+        assert torch.equal(alone, both[kind])
+        return
+    more = {"all": {}, "causal": {"causal": True, "first": torch.tensor([0, -300])}, "window": {"causal": True, "window": 50, "first": torch.tensor([-400, 0])},
+            "lengths": {"lens": torch.tensor([0, 131])}, "mask": {"mask": torch.rand(tq, tk, generator=g) < 0.3}}[kind]
+    run(dtype, q, k, v, do, **more)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
 def test_windows(dtype, window):
