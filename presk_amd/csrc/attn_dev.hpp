@@ -1500,7 +1500,8 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
 // Workgroups of eight waves where four would leave SIMDs with a wave or none, which
 // then waits for its own results: where a round of the CUs holds them all (2 x 12
 // heads x 1024 x 64 with a mask, 192 of them: the value 27 -> 20 us, the queries'
-// gradient 35 -> 24, the keys' 38 -> 27; of 384 of them, causal, 23 -> 26).
+// gradient 35 -> 24, the keys' 38 -> 27; but 384 of 2 x 24 heads, causal, 23 ->
+// 29).
 template <int ST, int ND>
 bool eight(long long grid) {
     return Geo<ST, ND>::TILE == 64 && grid <= 256;
@@ -1534,7 +1535,7 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     const long long nq = a.dq.p ? (long long)((a.tq + 127) / 128) * a.batch * a.heads : 0;
     long long nkv = a.dk.p || a.dv.p ? (long long)((a.tk + 127) / 128) * a.batch * a.kv * a.parts : 0;
     if constexpr (Geo<ST, ND>::TILE == 64)
-        if (nkv && eight<ST, ND>(nkv)) {
+        if (nkv && (a.parts > 1 || eight<ST, ND>(nkv))) {      // (parts are those kernels' alone)
             if (nq && nq <= 1024) attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
             else attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
             if (a.parts > 1) {
