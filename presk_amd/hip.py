@@ -502,7 +502,7 @@ _HEADS_KINDS = {"value": 1, "vjp": 2}
 _LAYOUTS = ("bshd", "bhsd")
 # storage types' names where the C side finds them, for the process's life
 _C_NAMES = {t: ctypes.create_string_buffer(t.encode()) for t in ("f32", "bf16", "f16")}
-_NO_HEADS = (0, 0, 0, 0)
+_NO_HEADS, _NO_MASK = (0, 0, 0, 0), (0, 0, 0)
 
 
 def _c_name(dtype: str) -> int:
@@ -512,14 +512,22 @@ def _c_name(dtype: str) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _heads_workspace(cls, fixed: tuple) -> dict:
-    """The workspaces of an operator's sizes, which are checked here."""
+def _heads_sizes(cls, fixed: tuple, layout: str, batch: int, lengths: tuple, heads: tuple, d: int) -> tuple:
+    """What follows from an operator's sizes, which are checked here: its
+    arguments' head, its workspaces, and of queries' and of keys' tensors the axes
+    and a dense one's strides of batch, row and head."""
+    if layout not in _LAYOUTS:
+        raise ValueError(f"a layout {layout!r}, not one of {', '.join(_LAYOUTS)}")
+    head = (_c_name(fixed[0]), *fixed[1:])
     n, need = ctypes.c_size_t(), {}
     args = cls._pack(fixed, {}, 0, 0)
     for kind, what in _HEADS_KINDS.items():
         check(getattr(lib(), f"presk_hip_{cls._name}_workspace")(args, what, ctypes.byref(n)))
         need[kind] = n.value
-    return need
+    specs = []
+    for m, h in zip(lengths, heads):
+        specs.append(((batch, m, h, d), m * h * d, h * d, d) if layout == "bshd" else ((batch, h, m, d), m * h * d, d, m * d))
+    return head, need, specs
 
 
 class _HeadsCall:
@@ -529,20 +537,15 @@ class _HeadsCall:
     last is 1 (a slice of a packed projection, of a longer cache)."""
 
     _name: str                  # of the library's calls
-    _tensors: dict              # a tensor's name -> whether it is a key's
+    # a C call's arguments after the sizes: a tensor's name -> whether it is a
+    # key's, then the other buffers, then the workspace
+    _tensors: dict
+    _plain: tuple
 
     def _init(self, layout: str, fixed: tuple, lengths: tuple):
-        if layout not in _LAYOUTS:
-            raise ValueError(f"a layout {layout!r}, not one of {', '.join(_LAYOUTS)}")
-        self.layout = layout
-        self._fixed = fixed
-        self._need = _heads_workspace(type(self), fixed)
+        self.layout, self._fixed = layout, fixed
+        self._head, self._need, self._specs = _heads_sizes(type(self), fixed, layout, self.batch, lengths, (self.heads, self.kv_heads), self.head_dim)
         self._works = {}        # device and stream -> the workspaces taken for it, the largest last
-        b, d, rows_first = self.batch, self.head_dim, layout == "bshd"
-        # of queries and of keys: a tensor's axes, and a dense one's strides
-        self._specs = []
-        for s, h in ((lengths[0], self.heads), (lengths[1], self.kv_heads)):
-            self._specs.append(((b, s, h, d), s * h * d, h * d, d) if rows_first else ((b, h, s, d), s * h * d, d, s * d))
 
     def workspace(self, kind: str) -> int:
         """Bytes of workspace for `value` or `vjp`."""
@@ -565,12 +568,12 @@ class _HeadsCall:
             raise ValueError(f"{name} is not in device memory")
         if at != device and device not in (None, -1):
             raise ValueError(f"{name} is on device {at}, not {device}")
-        if (have := _type_name(t)) != self.dtype:
-            raise ValueError(f"{name} is {have}, not {self.dtype}")
+        if _TORCH_TYPES.get(t.dtype) != self.dtype and _type_name(t) != self.dtype:
+            raise ValueError(f"{name} is {_type_name(t)}, not {self.dtype}")
         if t.shape != shape:
             raise ValueError(f"{name} is {list(t.shape)}, not {list(shape)}")
         sb, s1, s2, one = t.stride()
-        if one != 1 and self.head_dim > 1 and t.numel():
+        if one != 1 and shape[3] > 1 and t.numel():
             raise ValueError(f"{name}'s heads are not contiguous")
         return (t.data_ptr(), sb, s1, s2) if self.layout == "bshd" else (t.data_ptr(), sb, s2, s1)
 
@@ -583,20 +586,41 @@ class _HeadsCall:
     def args(self, kind: str, work=None, stream=None, device=None, **bufs) -> bytes:
         """The C call's arguments on `stream`, each buffer checked against its
         size and `device` (the one initialised)."""
-        device = _initialized if device is None else device
+        if unknown := sorted(set(bufs) - set(self._tensors) - set(self._plain)):
+            raise TypeError(f"{self._name} has no argument {unknown[0]}")
+        return self._args(kind, work, stream, _initialized if device is None else device, bufs)
+
+    @classmethod
+    def _pack(cls, fixed, got, work, work_bytes) -> bytes:
+        """Those of buffers' addresses (and strides)."""
+        h = [x for n in cls._tensors for x in got.get(n, _NO_HEADS)]
+        for n in cls._plain:
+            h += got.get(n, _NO_MASK) if n == "mask" else (got.get(n, 0),)
+        return cls._struct.pack(_c_name(fixed[0]), *fixed[1:], *h, work, work_bytes)
+
+    def _args(self, kind, work, stream, device, bufs: dict) -> bytes:
         if work is None and self._works_for(kind):
             work = self._own_work(self._need[kind], device, stream)
-        got = {n: self._heads(n, b, device) if n in self._tensors else self._other(n, b, device) for n, b in bufs.items() if b is not None}
+        given, got = bufs.get, []
+        for n in self._tensors:
+            b = given(n)
+            got += _NO_HEADS if b is None else self._heads(n, b, device)
+        for n in self._plain:
+            b = given(n)
+            if n == "mask":
+                got += _NO_MASK if b is None else self._mask(b, device)
+            else:
+                got.append(0 if b is None else _buffer(n, b, device, *self._others[n]))
         if work is None:
-            return self._pack(self._fixed, got, 0, 0)
-        return self._pack(self._fixed, got, _buffer("work", work, device, self._need[kind]), work.nbytes)
+            return self._struct.pack(*self._head, *got, 0, 0)
+        return self._struct.pack(*self._head, *got, _buffer("work", work, device, self._need[kind]), work.nbytes)
 
     def _works_for(self, kind: str) -> bool:
         return True
 
-    def _call(self, kind, stream, **bufs):
+    def _call(self, kind, stream, work, bufs: dict):
         device, stream = _place_of(bufs.values(), stream)
-        a = self.args(kind, stream=stream, device=device, **bufs)
+        a = self._args(kind, work, stream, device, bufs)
         check(self._launch(lib())(a, _HEADS_KINDS[kind], stream))
 
 
@@ -635,6 +659,7 @@ class Attention(_HeadsCall):
     # presk_hip_attn
     _struct = struct.Struct("@P8qid" + "Pqqq" * 8 + "4P2qPPN")
     _tensors = {"q": False, "k": True, "v": True, "o": False, "do": False, "dq": False, "dk": True, "dv": True}
+    _plain = ("lse", "lens", "first", "mask", "flag")
 
     def __init__(self, dtype: str, batch: int, heads: int, kv_heads: int, q_len: int, k_len: int, head_dim: int, causal: bool = False,
                  window: int = 0, mask_cols: int = 0, scale: float | None = None, layout: str = "bshd"):
@@ -647,21 +672,9 @@ class Attention(_HeadsCall):
         rows = 4 * self.batch * self.heads * self.q_len
         self._others = {"lse": (rows, "f32"), "lens": (8 * self.batch, "i64"), "first": (8 * self.batch, "i64"), "flag": (4, None)}
 
-    @classmethod
-    def _pack(cls, fixed, got, work, work_bytes) -> bytes:
-        g = got.get
-        h = [x for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for x in g(n, _NO_HEADS)]
-        return cls._struct.pack(_c_name(fixed[0]), *fixed[1:], *h, g("lse", 0), g("lens", 0), g("first", 0), *g("mask", (0, 0, 0)),
-                                g("flag", 0), work, work_bytes)
-
-    def _other(self, name, b, device):
-        if name != "mask":
-            return _buffer(name, b, device, *self._others[name])
+    def _mask(self, m, device) -> tuple:
         if not self.mask_cols:
             raise ValueError("a mask of no columns (mask_cols)")
-        return self._mask(b, device)
-
-    def _mask(self, m, device) -> tuple:
         if not hasattr(m, "data_ptr"):
             return _buffer("mask", m, device, self.batch * self.q_len * self.mask_cols), self.q_len * self.mask_cols, self.mask_cols
         at = m.get_device()
@@ -680,11 +693,11 @@ class Attention(_HeadsCall):
         return m.data_ptr(), st[0] if m.ndim == 3 else 0, st[-2]
 
     def value(self, q, k, v, o, lse=None, lens=None, first=None, mask=None, flag=None, work=None, stream=None):
-        self._call("value", stream, q=q, k=k, v=v, o=o, lse=lse, lens=lens, first=first, mask=mask, flag=flag, work=work)
+        self._call("value", stream, work, {"q": q, "k": k, "v": v, "o": o, "lse": lse, "lens": lens, "first": first, "mask": mask, "flag": flag})
 
     def vjp(self, q, k, v, o, lse, do, dq=None, dk=None, dv=None, lens=None, first=None, mask=None, flag=None, work=None, stream=None):
-        self._call("vjp", stream, q=q, k=k, v=v, o=o, lse=lse, do=do, dq=dq, dk=dk, dv=dv, lens=lens, first=first, mask=mask, flag=flag,
-                   work=work)
+        self._call("vjp", stream, work, {"q": q, "k": k, "v": v, "o": o, "lse": lse, "do": do, "dq": dq, "dk": dk, "dv": dv, "lens": lens,
+                                         "first": first, "mask": mask, "flag": flag})
 
 
 def rotary_frequencies(rotary: int, base: float = 1e4) -> np.ndarray:
@@ -712,6 +725,7 @@ class HeadRotary(_HeadsCall):
     # presk_hip_rot
     _struct = struct.Struct("@P6qiid" + "Pqqq" * 8 + "8PN")
     _tensors = {"q": False, "k": True, "yq": False, "yk": True, "dyq": False, "dyk": True, "dq": False, "dk": True}
+    _plain = ("freq", "at", "gq", "gk", "dgq", "dgk", "flag")
 
     def __init__(self, dtype: str, batch: int, seq: int, heads: int, kv_heads: int, head_dim: int, rotary: int | None = None,
                  norm: bool = False, eps: float = 1e-6, pairs: str = "half", layout: str = "bshd"):
@@ -726,23 +740,13 @@ class HeadRotary(_HeadsCall):
         self._others = {"freq": (4 * self.rotary, "f64"), "at": (8 * self.batch * self.seq, "i64"), "flag": (4, None),
                         "gq": gain, "gk": gain, "dgq": gain, "dgk": gain}
 
-    @classmethod
-    def _pack(cls, fixed, got, work, work_bytes) -> bytes:
-        g = got.get
-        h = [x for n in ("q", "k", "yq", "yk", "dyq", "dyk", "dq", "dk") for x in g(n, _NO_HEADS)]
-        return cls._struct.pack(_c_name(fixed[0]), *fixed[1:], *h, *(g(n, 0) for n in ("freq", "at", "gq", "gk", "dgq", "dgk", "flag")),
-                                work, work_bytes)
-
-    def _other(self, name, b, device):
-        return _buffer(name, b, device, *self._others[name])
-
     def _works_for(self, kind: str) -> bool:
         return self.norm and kind == "vjp"
 
     def value(self, q, freq, yq, k=None, yk=None, at=None, gq=None, gk=None, flag=None, work=None, stream=None):
-        self._call("value", stream, q=q, k=k, yq=yq, yk=yk, freq=freq, at=at, gq=gq, gk=gk, flag=flag, work=work)
+        self._call("value", stream, work, {"q": q, "k": k, "yq": yq, "yk": yk, "freq": freq, "at": at, "gq": gq, "gk": gk, "flag": flag})
 
     def vjp(self, freq, dyq, dq, dyk=None, dk=None, q=None, k=None, at=None, gq=None, gk=None, dgq=None, dgk=None, flag=None, work=None,
             stream=None):
-        self._call("vjp", stream, q=q, k=k, dyq=dyq, dyk=dyk, dq=dq, dk=dk, freq=freq, at=at, gq=gq, gk=gk, dgq=dgq, dgk=dgk, flag=flag,
-                   work=work)
+        self._call("vjp", stream, work, {"q": q, "k": k, "dyq": dyq, "dyk": dyk, "dq": dq, "dk": dk, "freq": freq, "at": at, "gq": gq, "gk": gk,
+                                         "dgq": dgq, "dgk": dgk, "flag": flag})
