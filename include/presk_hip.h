@@ -343,9 +343,12 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * strides in elements and not negative, those of an input over batch or heads 0
  * where it is shared.  Rows of whole 16-byte vectors (address, strides and
  * head_dim) are loaded as such, others element by element.
- * Products accumulate in f32, and so do the sums of a softmax; in 16-bit storage
+ * Products accumulate in f32, and so do the sums of a softmax.  In 16-bit storage
  * the weights p and their cotangents ds are rounded to the storage type before
- * the products they enter.
+ * the products they enter, ds with what that rounding left as a second term where
+ * queries read fewer than 64 keys or a mask says which.  f32 elements enter as
+ * three bf16 parts, which are all of them, and six of their nine products (the
+ * rest is below 2^-24); one that is infinite, or above 0x1.ffp127, gives NaN.
  *
  * `what`: PRESK_HIP_ATTN_VALUE writes o and, where it is not null, lse (f32 [batch,
  * heads, q_len]).  PRESK_HIP_ATTN_GRAD writes those of dq, dk and dv whose p is
@@ -357,8 +360,9 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * between each other's do not).  Nothing is allocated, and only kernels are
  * launched, so the calls may be captured; lens, first and mask are read then.
  * Storage types f32 (head_dim to 128), bf16 and f16 (to 256), others are E7005;
- * q_len, k_len, mask_cols and window below 2^28; a row's stride (seq) at least
- * head_dim elements and below 2^25 bytes. */
+ * q_len, k_len, mask_cols and window below 2^28, a mask of batch * q_len * mask_cols
+ * below 2^35 (of lengths in whole 32s); a row's stride (seq) at least head_dim
+ * elements and below 2^25 bytes. */
 typedef struct {
     void* p;
     int64_t batch, seq, head;

@@ -34,6 +34,7 @@ struct Geo {
     static constexpr int ES = ST == kF32 ? 4 : 2, PITCH = ND <= 2 ? 64 : ND <= 4 ? 128 : 256;
     static constexpr int ROW = PITCH * ES, CPR = ROW / 16, EPC = 16 / ES;
     static constexpr int STEPS = ND * 32 / (2 * EPC);     // 16-byte reads of a row a lane (its half of each pair of chunks)
+    static constexpr int KSTEPS = ST == kF32 ? STEPS / 2 : STEPS;     // matrix instructions' k of a row
     static constexpr int TILE = ROW <= 256 ? 64 : 32;     // rows of a tile
     __host__ __device__ static constexpr int swz(int r) {
         if constexpr (CPR == 8) return ((r & 2) << 1) | ((r & 4) >> 1) | ((r ^ (r >> 3)) & 1);
@@ -41,20 +42,21 @@ struct Geo {
     }
 };
 
-// 16 bytes of a row: one matrix instruction's k in 16 bits, four's in f32
+// 16 bytes of a row
 template <int ST> struct FragOf { typedef u16x8 T; };
 template <> struct FragOf<kF32> { typedef f32x4 T; };
 
-template <int ST>
-__device__ __forceinline__ f32x16 mma_row(typename FragOf<ST>::T a, typename FragOf<ST>::T b, f32x16 acc) {
-    if constexpr (ST == kF32) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
-        return acc;
-    } else {
-        return mfma32<ST>(a, b, acc);
-    }
-}
+// A matrix instruction's eight elements a lane.  f32 in three parts of 8 bits
+// each, rounded to nearest, which are all of its 24: of a product's nine six are
+// taken (the three left are below 2^-24 of it together, f32's own rounding), by
+// bf16 instructions, of which six take 3/8 of the time of f32's own (64 x 6 heads x
+// 256 x 64, causal: the value 63 -> 50 us, the queries' gradient 87 -> 64, the keys'
+// 121 -> 98, with errors against 64 bits as before; bound now by the eleven vector
+// instructions that two elements' parts take, in every wave that reads them).  An
+// infinite element, or one that rounds to it, has a second part that is no number:
+// what reads it is NaN.
+template <int ST> struct Part { u16x8 p[1]; };
+template <> struct Part<kF32> { u16x8 p[3]; };
 
 // Two values rounded into one word.  (The compiler's own conversion: it knows that
 // an exponential's result needs a wait before it is read, which assembly would not get.)
@@ -62,6 +64,50 @@ template <int ST>
 __device__ __forceinline__ unsigned pack2(float a, float b) {
     if constexpr (ST == kBF16) return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
     else return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+
+__device__ __forceinline__ Part<kF32> parts_of(const float (&x)[8]) {
+    unsigned w[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = x[2 * e], b = x[2 * e + 1];
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            w[n][e] = pack2<kBF16>(a, b);
+            a -= __builtin_bit_cast(float, w[n][e] << 16);
+            b -= __builtin_bit_cast(float, w[n][e] & 0xffff0000u);
+        }
+    }
+    Part<kF32> f;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) f.p[n] = __builtin_bit_cast(u16x8, i32x4{(int)w[n][0], (int)w[n][1], (int)w[n][2], (int)w[n][3]});
+    return f;
+}
+// The elements as they are read, and their parts.
+struct Raw32 { f32x4 a, b; };
+template <int ST> struct RawOf { typedef Part<ST> T; };
+template <> struct RawOf<kF32> { typedef Raw32 T; };
+__device__ __forceinline__ Part<kF32> parts_of(f32x4 a, f32x4 b) {
+    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return parts_of(x);
+}
+
+__device__ __forceinline__ Part<kF32> part_of(const Raw32& r) { return parts_of(r.a, r.b); }
+template <int ST>
+__device__ __forceinline__ const Part<ST>& part_of(const Part<ST>& p) { return p; }
+
+template <int ST>
+__device__ __forceinline__ f32x16 mma_row(const Part<ST>& a, const Part<ST>& b, f32x16 acc) {
+    if constexpr (ST == kF32) {
+        // the smallest first
+#pragma unroll
+        for (int n = 2; n >= 0; --n)
+#pragma unroll
+            for (int i = 0; i <= n; ++i) acc = mfma32<kBF16>(a.p[i], b.p[n - i], acc);
+        return acc;
+    } else {
+        return mfma32<ST>(a.p[0], b.p[0], acc);
+    }
 }
 
 // The weights of 32 tile rows as a product's operand.
@@ -89,8 +135,12 @@ __device__ __forceinline__ void left_in(f32x16& p, const Weights<ST>& w) {
 }
 template <>
 struct Weights<kF32> {
-    f32x16 w;
-    __device__ __forceinline__ void set(const f32x16& p) { w = p; }
+    Part<kF32> w[2];
+    __device__ __forceinline__ void set(const f32x16& p) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) w[s] = parts_of(f32x4{p[8 * s], p[8 * s + 1], p[8 * s + 2], p[8 * s + 3]},
+                                                    f32x4{p[8 * s + 4], p[8 * s + 5], p[8 * s + 6], p[8 * s + 7]});
+    }
 };
 
 // The tile row, of 32, of a lane's sum e.
@@ -129,10 +179,12 @@ __device__ __forceinline__ T lds_read(unsigned at) {
     return *(__attribute__((address_space(3))) T*)at;
 }
 
-// A lane's part of its row at step `st` (its half of chunks 2 st and 2 st + 1).
+// A lane's part of its row at step `st` (its half of chunks 2 st and 2 st + 1; in
+// f32 of the four from 4 st on).
 template <int ST>
-__device__ __forceinline__ typename FragOf<ST>::T frag_row(unsigned row, int st, unsigned off = 0) {
-    return lds_read<typename FragOf<ST>::T>((row ^ (unsigned)(st << 5)) + off);
+__device__ __forceinline__ typename RawOf<ST>::T frag_row(unsigned row, int st, unsigned off = 0) {
+    if constexpr (ST == kF32) return Raw32{lds_read<f32x4>((row ^ (unsigned)(st << 6)) + off), lds_read<f32x4>((row ^ (unsigned)(st << 6 | 32)) + off)};
+    else return Part<ST>{{lds_read<u16x8>((row ^ (unsigned)(st << 5)) + off)}};
 }
 
 // acc[n][dt] += X^T . w[n] over 32 rows of a tile, for NB blocks of kept rows.  f32
@@ -142,23 +194,28 @@ __device__ __forceinline__ void mma_col(unsigned col, unsigned off, const Weight
     typedef Geo<ST, ND> G;
     if constexpr (ST == kF32) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            // (the row without the half-wave's 4, which `col` has)
-            const int r = 8 * (e >> 2) + (e & 3);
-            const unsigned at = (col ^ (unsigned)(G::swz(r) << 4)) + (unsigned)(r * G::ROW) + off;
-            float x[ND];
-            if constexpr (ND == 4) {
-                const f32x4 v = lds_read<f32x4>(at);
+        for (int q = 0; q < 2; ++q) {
+            float x[ND][8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = v[i];
-            } else {
-                const f32x2 v = lds_read<f32x2>(at);
-                x[0] = v[0], x[1] = v[1];
+            for (int e = 0; e < 8; ++e) {
+                // (the row without the half-wave's 4, which `col` has)
+                const int r = 16 * q + 8 * (e >> 2) + (e & 3);
+                const unsigned at = (col ^ (unsigned)(G::swz(r) << 4)) + (unsigned)(r * G::ROW) + off;
+                if constexpr (ND == 4) {
+                    const f32x4 v = lds_read<f32x4>(at);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i][e] = v[i];
+                } else {
+                    const f32x2 v = lds_read<f32x2>(at);
+                    x[0][e] = v[0], x[1][e] = v[1];
+                }
             }
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int dt = 0; dt < ND; ++dt) {
+                const Part<kF32> f = parts_of(x[dt]);
 #pragma unroll
-                for (int dt = 0; dt < ND; ++dt) acc[n][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[dt], w[n].w[e], acc[n][dt], 0, 0, 0);
+                for (int n = 0; n < NB; ++n) acc[n][dt] = mma_row<kF32>(f, w[n].w[q], acc[n][dt]);
+            }
         }
     } else {
         constexpr unsigned FLIP = (unsigned)((G::swz(8) ^ G::swz(0)) << 4);      // of a row 8 further on
@@ -213,24 +270,36 @@ __device__ __forceinline__ const void* row_at(const AttnTensor& t, int b, long l
 // A kept row: a lane's 16 bytes of every step.  Rows that are no whole vectors
 // pass through the lane's own 16 bytes a step of `lds` (the wave's 1 KB a step),
 // in a loop that is not unrolled.
-template <int ST, int ND>
+template <int ST, int ND, typename P>
 __device__ __forceinline__ void load_kept(const AttnTensor& t, int b, long long i, int head, int d, bool in, int lane, unsigned char* lds,
-                                          typename FragOf<ST>::T (&x)[Geo<ST, ND>::STEPS]) {
+                                          P (&x)[Geo<ST, ND>::KSTEPS]) {
     typedef typename FragOf<ST>::T F;
+    constexpr int EACH = ST == kF32 ? 2 : 1;
     const void* const row = row_at<ST>(t, b, in ? i : 0, head);
     const int h = lane >> 5;
     if (t.vec) {
+        F f[Geo<ST, ND>::STEPS];
 #pragma unroll
         for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) {
             const int c = 2 * st + h;
-            x[st] = in && c * Geo<ST, ND>::EPC < d ? *(const F*)((const char*)row + 16 * c) : F{};
+            f[st] = in && c * Geo<ST, ND>::EPC < d ? *(const F*)((const char*)row + 16 * c) : F{};
+        }
+#pragma unroll
+        for (int st = 0; st < Geo<ST, ND>::KSTEPS; ++st) {
+            if constexpr (ST != kF32) x[st].p[0] = f[st];
+            else if constexpr (sizeof(P) == sizeof(Raw32)) x[st] = Raw32{f[EACH * st], f[EACH * st + 1]};
+            else x[st] = parts_of(f[EACH * st], f[EACH * st + 1]);
         }
     } else {
         F* const mine = (F*)lds + lane;
 #pragma unroll 1
         for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) mine[64 * st] = chunk_of<ST>(row, 2 * st + h, d, in);
 #pragma unroll
-        for (int st = 0; st < Geo<ST, ND>::STEPS; ++st) x[st] = mine[64 * st];
+        for (int st = 0; st < Geo<ST, ND>::KSTEPS; ++st) {
+            if constexpr (ST != kF32) x[st].p[0] = mine[64 * st];
+            else if constexpr (sizeof(P) == sizeof(Raw32)) x[st] = Raw32{mine[64 * EACH * st], mine[64 * (EACH * st + 1)]};
+            else x[st] = parts_of(mine[64 * EACH * st], mine[64 * (EACH * st + 1)]);
+        }
     }
 }
 
@@ -529,20 +598,13 @@ __device__ __forceinline__ void take(const unsigned char* at, int lane, f32x16 (
         }
 }
 
-// f32's heads of 64 elements in tiles of 32 keys, so that a CU has three workgroups
-// (64 x 6 heads x 256 x 64, causal: 66 -> 63 us, the gradient 90 -> 87)
-template <int ST, int ND, int SW>
-constexpr bool three() { return ST == kF32 && ND == 2 && SW == 1; }
-template <int ST, int ND, int SW>
-constexpr int tile_of() { return three<ST, ND, SW>() ? 32 : Geo<ST, ND>::TILE; }
-
 // One workgroup: 128 rows of a head (of a group's heads beside each other), 32 a
 // wave, over the keys that any of them reads, or a share of those.  SW 2: eight
 // waves, two of which share 32 rows and take half of each tile's keys each.
 template <int ST, int ND, int SW>
-__global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : 2) attn_fwd_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256 * SW, ST == kF32 && ND >= 4 ? 1 : 2) attn_fwd_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
-    constexpr int TILE = tile_of<ST, ND, SW>();
+    constexpr int TILE = G::TILE;
     typedef Rows<ST, ND, TILE, 256 * SW> Tile;
     constexpr int NB = TILE / 32 / SW;
     static_assert(NB >= 1, "a tile has a block for each");
@@ -598,7 +660,7 @@ __global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : 2) attn_
         vt.issue(k0, khi - k0, stage, smem + Tile::BYTES, tid);
     };
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
-    typename FragOf<ST>::T q[G::STEPS];
+    Part<ST> q[G::KSTEPS];
     load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
     if (!a.q.vec) __syncthreads();
     if (nt > 0) fetch(0);
@@ -642,7 +704,7 @@ __global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : 2) attn_
             }
             s[kb] = f32x16{};
 #pragma unroll
-            for (int st = 0; st < G::STEPS; ++st) s[kb] = mma_row<ST>(frag_row<ST>(at.row, st, kb * 32 * G::ROW), q[st], s[kb]);
+            for (int st = 0; st < G::KSTEPS; ++st) s[kb] = mma_row<ST>(part_of(frag_row<ST>(at.row, st, kb * 32 * G::ROW)), q[st], s[kb]);
             if (masked) {
                 bits = (bits & range_of(rlo - base, rhi - base)) >> (4 * h);
 #pragma unroll
@@ -789,7 +851,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
     const int i = live ? r / a.pack : a.tq - 1, head = hk * a.pack + (live ? r % a.pack : 0);
     const int rlo = keys.lo(a, i), rhi = keys.hi(a, i);
     const unsigned line = (unsigned)((b * a.bits_batch + i) * a.words);
-    typename FragOf<ST>::T q[G::STEPS];
+    Part<ST> q[G::KSTEPS];
     if (!a.q.vec) {
         load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q);
         __builtin_amdgcn_s_waitcnt(0xc07f);     // LDS: the reads are done before a tile lands there
@@ -816,7 +878,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
         const Places<ST, ND> at = places.from((unsigned)(t & 1) * STAGE);
         f32x16 s = f32x16{};
 #pragma unroll
-        for (int st = 0; st < G::STEPS; ++st) s = mma_row<ST>(frag_row<ST>(at.row, st), q[st], s);
+        for (int st = 0; st < G::KSTEPS; ++st) s = mma_row<ST>(part_of(frag_row<ST>(at.row, st)), q[st], s);
         if (k0 < surelo || k0 + 32 > surehi) {
             unsigned bits = ~0u;
             if (a.cols && k0 + 32 > keys.first) {
@@ -1015,11 +1077,11 @@ constexpr float kShift = 8.f;
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
 // the queries'.
 template <int ST, int ND, int SW>
-constexpr int dq_lds() { return 4 * Rows<ST, ND, tile_of<ST, ND, SW>(), 256 * SW>::BYTES; }
+constexpr int dq_lds() { return 4 * Rows<ST, ND, Geo<ST, ND>::TILE, 256 * SW>::BYTES; }
 template <int ST, int ND, int SW>
 __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned total, unsigned char* smem) {
     typedef Geo<ST, ND> G;
-    constexpr int TILE = tile_of<ST, ND, SW>();
+    constexpr int TILE = G::TILE;
     typedef Rows<ST, ND, TILE, 256 * SW> Tile;
     constexpr int NB = 1;
     constexpr int WROWS = 32 * NB, ROWS = 4 * WROWS, PAIR = SW == 2 ? 4096 * ND : 32 * G::ROW;
@@ -1056,7 +1118,7 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
     const int w0 = r0 + rw * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
     const int wlo = keys.lo(a, w0 < r1 ? w0 : r1), whi = w0 <= r1 ? keys.hi(a, w1) : 0;
     const bool fine = fine_of<ST>(a, keys, w0 < r1 ? w0 : r1, w1);
-    typename FragOf<ST>::T q[NB][G::STEPS], dout[NB][G::STEPS];
+    Part<ST> q[NB][G::KSTEPS], dout[NB][G::KSTEPS];
     float lse[NB], delta[NB];
     f32x16 dq[NB][ND];
 #pragma unroll
@@ -1098,12 +1160,12 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = dp[n] = f32x16{};
 #pragma unroll
-        for (int st = 0; st < G::STEPS; ++st) {
+        for (int st = 0; st < G::KSTEPS; ++st) {
             const auto fk = frag_row<ST>(at.row, st), fv = frag_row<ST>(at.row, st, Tile::BYTES);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                s[n] = mma_row<ST>(fk, q[n][st], s[n]);
-                dp[n] = mma_row<ST>(fv, dout[n][st], dp[n]);
+                s[n] = mma_row<ST>(part_of(fk), q[n][st], s[n]);
+                dp[n] = mma_row<ST>(part_of(fv), dout[n][st], dp[n]);
             }
         }
         Weights<ST> w[NB];
@@ -1255,7 +1317,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     };
 
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
-    typename FragOf<ST>::T k[KL ? 1 : NB][G::STEPS], v[VL ? 1 : NB][G::STEPS];
+    typename RawOf<ST>::T k[KL ? 1 : NB][G::KSTEPS], v[VL ? 1 : NB][G::KSTEPS];
     f32x16 dk[NB][ND], dv[NB][ND];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -1315,7 +1377,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
         for (int n = 0; n < NB; ++n) s[n] = dp[n] = f32x16{};
         // a step's reads a step ahead of its products, and no further, or the
         // registers do not hold them
-        typedef typename FragOf<ST>::T F;
+        typedef typename RawOf<ST>::T F;
         F fq, fd, fv[NB], fk;
         auto read = [&](int st) {
             fq = frag_row<ST>(at.row, st);
@@ -1329,17 +1391,19 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
         };
         read(0);
 #pragma unroll
-        for (int st = 0; st < G::STEPS; ++st) {
-            const F cq = fq, cd = fd, ck = KL ? fk : k[0][KL ? 0 : st];
-            F cv[NB];
+        for (int st = 0; st < G::KSTEPS; ++st) {
+            const F cq = fq, cd = fd;
+            F ck = KL ? fk : k[0][KL ? 0 : st], cv[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n) cv[n] = VL ? fv[n] : v[VL ? 0 : n][st];
-            if (st + 1 < G::STEPS) read(st + 1);
+            // (the compiler would keep their parts, which the registers do not hold)
+            if constexpr (ST == kF32) asm volatile("" : "+v"(ck.a), "+v"(ck.b), "+v"(cv[0].a), "+v"(cv[0].b));
+            if (st + 1 < G::KSTEPS) read(st + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                s[n] = mma_row<ST>(cq, ck, s[n]);
-                if (DK) dp[n] = mma_row<ST>(cd, cv[n], dp[n]);
+                s[n] = mma_row<ST>(part_of(cq), part_of(ck), s[n]);
+                if (DK) dp[n] = mma_row<ST>(part_of(cd), part_of(cv[n]), dp[n]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -1453,7 +1517,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
 }
 
 template <int ST, int ND, int SW>
-__global__ void __launch_bounds__(256 * SW, (three<ST, ND, SW>()) ? 3 : ND >= 8 || (ST == kF32 && ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256 * SW, ND >= 8 || (ST == kF32 && ND >= 4) ? 1 : 2) attn_dq_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[dq_lds<ST, ND, SW>()];
     dq_of<ST, ND, SW>(a, blockIdx.x, gridDim.x, smem);
 }
@@ -1530,14 +1594,15 @@ hipError_t fwd(const AttnArgs& a, hipStream_t s) {
 
 template <int ST, int ND>
 hipError_t bwd(const AttnArgs& a, hipStream_t s) {
+    constexpr bool WIDE = Geo<ST, ND>::ROW == 256;      // (two waves a SIMD have no registers for the values too)
     const long long all = (long long)a.batch * a.heads * a.tq;
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
     const long long nq = a.dq.p ? (long long)((a.tq + 127) / 128) * a.batch * a.heads : 0;
     long long nkv = a.dk.p || a.dv.p ? (long long)((a.tk + 127) / 128) * a.batch * a.kv * a.parts : 0;
     if constexpr (Geo<ST, ND>::TILE == 64)
         if (nkv && (a.parts > 1 || eight<ST, ND>(nkv))) {      // (parts are those kernels' alone)
-            if (nq && nq <= 1024) attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
-            else attn_dkv_kernel<ST, ND, 2, 64, true, true, ND == 4, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
+            if (nq && nq <= 1024) attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
+            else attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
             if (a.parts > 1) {
                 const long long n = 2LL * a.batch * a.kv * a.tk * 8 * ND;
                 attn_sum_kernel<ST, ND><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
@@ -1560,7 +1625,7 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
         } else if constexpr (ST == kF32 && ND == 4) {
             attn_dkv_kernel<ST, ND, 1, 32, true, true, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         } else {
-            attn_dkv_kernel<ST, ND, 1, ND == 4 ? 32 : 64, true, true, ND == 4, 2, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
+            attn_dkv_kernel<ST, ND, 1, WIDE ? 32 : 64, true, true, WIDE, 2, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         }
     }
     return hipGetLastError();
