@@ -103,6 +103,8 @@ Plan plan_of(const presk_hip_attn& a, int what) {
         if (grad) p.bits_t = take(4 * a.batch * a.mask_cols * p.words_t);
         p.any = take(a.batch * p.words_t * p.words);
     }
+    const long long per = a.heads / a.kv_heads;
+    if (a.q_len < kAttnTile) p.pack = (int)per;
     if (grad) {
         p.rows = take(8 * all);
         // the keys' and values' gradients in parts of their rows, where one
@@ -111,10 +113,10 @@ Plan plan_of(const presk_hip_attn& a, int what) {
         // to a workgroup a CU, and four tiles each at least (32 heads in groups of
         // four x 1024 x 128, causal, all gradients: 133 -> 82 us in four parts, 40
         // heads in groups of eight x 2048: 481 -> 250 in three)
-        const long long units = a.batch * a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile), per = a.heads / a.kv_heads;
+        const long long units = a.batch * a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile);
         const long long span = a.window ? std::min<long long>(a.window + kAttnTile, 1 << 28) : 1 << 28;
         const long long own = per * (up(std::min<long long>(a.q_len, span), 64) / 64);
-        const long long queries = a.batch * a.heads * (up(a.q_len, kAttnTile) / kAttnTile) * (up(std::min<long long>(a.k_len, span), 64) / 64);
+        const long long queries = a.batch * (a.heads / p.pack) * (up(a.q_len * p.pack, kAttnTile) / kAttnTile) * (up(std::min<long long>(a.k_len, span), 64) / 64);
         if (p.nd <= (p.st == kF32 ? 2 : 4) && units && own) {
             const long long mean = std::max<long long>(1, (units * own + queries) / (a.causal && !a.window ? 512 : 256));
             p.parts = (int)std::max<long long>(1, std::min({256 / units, own / 4, (own + mean / 2) / mean}));
@@ -122,8 +124,6 @@ Plan plan_of(const presk_hip_attn& a, int what) {
         if (p.parts > 1) p.part = take(8 * p.parts * a.batch * a.kv_heads * a.k_len * p.nd * 32);
         return p;
     }
-    const long long per = a.heads / a.kv_heads;
-    if (a.q_len < kAttnTile) p.pack = (int)per;
     const long long rows = a.q_len * p.pack, units = a.batch * (a.heads / p.pack);
     // few rows in shares of the keys that come to four rounds of the CUs, a workgroup
     // each (32 sequences' single tokens over 8192 keys: 1024 132 us, 768 137, 2048

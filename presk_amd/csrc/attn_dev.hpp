@@ -601,6 +601,12 @@ __device__ __forceinline__ void take(const unsigned char* at, int lane, f32x16 (
 // One workgroup: 128 rows of a head (of a group's heads beside each other), 32 a
 // wave, over the keys that any of them reads, or a share of those.  SW 2: eight
 // waves, two of which share 32 rows and take half of each tile's keys each.
+// Bound by the matrix instructions and the softmax's vector instructions, as many
+// cycles again, of which two waves a SIMD hide most: 4 x 32 heads x 4096 x 128 in
+// bf16, causal, 670 to 700 us, 800 TFLOP/s of the two products (all keys 895; a
+// large library product 1149); 32 heads x 2048 x 128 55 us.  Of a small call a
+// third is a launch, the first loads and the last stores (2 x 12 heads x 1024 x 64
+// with a mask 20 us, of which 8 with no tile at all).
 template <int ST, int ND, int SW>
 __global__ void __launch_bounds__(256 * SW, ST == kF32 && ND >= 4 ? 1 : 2) attn_fwd_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
@@ -811,7 +817,9 @@ __device__ __forceinline__ bool put(void* row, int at, int d, float v) {
 // Few rows (a group's heads beside each other, 32 at most) over many keys: all
 // of a workgroup's NW waves have the same rows, and blocks of 32 keys in turn,
 // which each loads for itself two at a time, so that no wave waits for another
-// until their sums meet in LDS at the end.
+// until their sums meet in LDS at the end.  Bound by reading the keys and values:
+// 32 sequences of 2048 to 8192, 8 key heads x 128 in bf16, 132 us, 5.2 TB/s (a large
+// copy reads and writes 4.9).
 template <int ST, int ND, int NW>
 __global__ void __launch_bounds__(64 * NW, 1) attn_few_kernel(AttnArgs a) {
     typedef Geo<ST, ND> G;
@@ -1037,7 +1045,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 
 // ---- the gradients --------------------------------------------------------------------
 
-// A row's -lse log2 e, and behind all of them its -sum do o.  16 lanes a row.
+// A row's -lse log2 e, and behind all of them its -sum do o.  16 lanes a row.  One
+// pass over o and do: 4 x 4096 x 32 x 128 in bf16 57 us, 4.7 TB/s.
 template <int ST>
 __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
     const long long all = (long long)a.batch * a.heads * a.tq, row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -1075,7 +1084,9 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
 constexpr float kShift = 8.f;
 
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
-// the queries'.
+// the queries' (4 x 32 heads x 4096 x 128, causal, 840 to 880 us, 960 TFLOP/s of the
+// three products, where a large library product has 1149).  Rows of a group's heads
+// stand beside each other where a head's do not fill a workgroup, as there.
 template <int ST, int ND, int SW>
 constexpr int dq_lds() { return 4 * Rows<ST, ND, Geo<ST, ND>::TILE, 256 * SW>::BYTES; }
 template <int ST, int ND, int SW>
@@ -1089,18 +1100,19 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
     const int rw = wave & 3, kw = wave >> 2;      // which rows, and which of a tile's keys
-    const int tiles = (a.tq + ROWS - 1) / ROWS;
+    const int rows = a.tq * a.pack, tiles = (rows + ROWS - 1) / ROWS;
     const unsigned at = item_of(id, total);
     const int tile = tiles - 1 - (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
-    int b, hk, head;
-    head_of(a, unit, a.per, &b, &hk, &head);
-    const int r0 = tile * ROWS, r1 = (a.tq < r0 + ROWS ? a.tq : r0 + ROWS) - 1;
+    int b, hk, hx;
+    head_of(a, unit, a.per / a.pack, &b, &hk, &hx);
+    const int r0 = tile * ROWS, r1 = (rows < r0 + ROWS ? rows : r0 + ROWS) - 1;
 
     Keys keys;
     keys.init(a, b);
-    int klo = keys.lo(a, r0), khi = keys.hi(a, r1);
-    by_mask(a, keys, b, r0, r1, &klo, &khi);
-    const int surelo = keys.lo(a, r1), surehi = keys.sure(a, r0);
+    const int ifirst = r0 / a.pack, ilast = r1 / a.pack;
+    int klo = keys.lo(a, ifirst), khi = keys.hi(a, ilast);
+    by_mask(a, keys, b, ifirst, ilast, &klo, &khi);
+    const int surelo = keys.lo(a, ilast), surehi = keys.sure(a, ifirst);
     const int nt = khi > klo ? (khi - klo + TILE - 1) / TILE : 0;
 
     Tile kt, vt;
@@ -1116,16 +1128,19 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
 
     const int w0 = r0 + rw * WROWS, w1 = w0 + WROWS - 1 < r1 ? w0 + WROWS - 1 : r1;
-    const int wlo = keys.lo(a, w0 < r1 ? w0 : r1), whi = w0 <= r1 ? keys.hi(a, w1) : 0;
-    const bool fine = fine_of<ST>(a, keys, w0 < r1 ? w0 : r1, w1);
+    const int wfirst = (w0 < r1 ? w0 : r1) / a.pack, wlast = w1 / a.pack;
+    const int wlo = keys.lo(a, wfirst), whi = w0 <= r1 ? keys.hi(a, wlast) : 0;
+    const bool fine = fine_of<ST>(a, keys, wfirst, wlast);
+    // this lane's row
+    const bool live = w0 + (lane & 31) <= r1;
+    const int mine = live ? w0 + (lane & 31) : r1, i = mine / a.pack, head = hx * a.pack + mine % a.pack;
     Part<ST> q[NB][G::KSTEPS], dout[NB][G::KSTEPS];
     float lse[NB], delta[NB];
     f32x16 dq[NB][ND];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-        const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
-        load_kept<ST, ND>(a.q, b, i, head, a.d, r <= r1, lane, own, q[n]);
-        load_kept<ST, ND>(a.dout, b, i, head, a.d, r <= r1, lane, own, dout[n]);
+        load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q[n]);
+        load_kept<ST, ND>(a.dout, b, i, head, a.d, live, lane, own, dout[n]);
         const float* const x = a.rows + ((long long)b * a.heads + head) * a.tq + i;
         lse[n] = x[0], delta[n] = x[(long long)a.batch * a.heads * a.tq];
 #pragma unroll
@@ -1139,7 +1154,7 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
     places = places.from(lds);
     constexpr int MINE = TILE / 32 / SW;     // blocks of a tile that are the wave's
     MaskBits ahead[MINE], now[MINE];
-    const unsigned line = (unsigned)((b * a.bits_batch + (w0 + (lane & 31) <= r1 ? w0 + (lane & 31) : r1)) * a.words);
+    const unsigned line = (unsigned)((b * a.bits_batch + i) * a.words);
     auto load_bits = [&](int t) {
         if (a.cols)
 #pragma unroll
@@ -1174,7 +1189,6 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], a.c, lse[n])) * (dp[n][e] + delta[n]);
             if (masked) {
-                const int r = w0 + 32 * n + (lane & 31), i = r <= r1 ? r : r1;
                 const unsigned in = (bits[n] & range_of(keys.lo(a, i) - base, keys.hi(a, i) - base)) >> (4 * h);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] = where_bit(in, e, s[n][e], 0.f);
@@ -1218,8 +1232,8 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
         if (kw == 1) return;
         take<ND>(pair, lane, dq[0], 1.f, 1.f);
     }
-    store_kept<ST, ND>(dq[0], a.scale, a.d, a.dq.vec, w0 + (lane & 31) <= r1, [&](int x) -> const void* {
-        return w0 + x <= r1 ? row_at<ST>(a.dq, b, w0 + x, head) : nullptr;
+    store_kept<ST, ND>(dq[0], a.scale, a.d, a.dq.vec, live, [&](int x) -> const void* {
+        return w0 + x <= r1 ? row_at<ST>(a.dq, b, (w0 + x) / a.pack, hx * a.pack + (w0 + x) % a.pack) : nullptr;
     }, pair, lane, a.flag);
 }
 
@@ -1233,7 +1247,11 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 // (3 x 10 heads, 5 of keys, 777 x 1021 x 80, 120 and 210 workgroups: 38 + 18 -> 41
 // us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves a
 // tile's rows may be in parts of theirs (AttnArgs::parts), whose sums in f32
-// attn_sum_kernel adds.
+// attn_sum_kernel adds.  Bound by LDS: of a tile of 32 rows a wave of the four
+// reads 40 KB beside 32 matrix instructions, eight waves a CU 156 bytes a cycle of
+// the 128 there are (4 x 32 heads in groups of four x 4096 x 128 in bf16, causal,
+// 1410 to 1440 us, 775 TFLOP/s of the four products; with 64 keys a wave and one
+// wave a SIMD, which read half as much, 2070).
 template <int ST, int ND, int SW, int QT, bool DK, bool DV, bool VL, int OCC, bool DQ>
 __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, unsigned nkv) {
     typedef Geo<ST, ND> G;
@@ -1597,17 +1615,22 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     constexpr bool WIDE = Geo<ST, ND>::ROW == 256;      // (two waves a SIMD have no registers for the values too)
     const long long all = (long long)a.batch * a.heads * a.tq;
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
-    const long long nq = a.dq.p ? (long long)((a.tq + 127) / 128) * a.batch * a.heads : 0;
+    const long long nq = a.dq.p ? ((long long)a.tq * a.pack + 127) / 128 * a.batch * (a.heads / a.pack) : 0;
     long long nkv = a.dk.p || a.dv.p ? (long long)((a.tk + 127) / 128) * a.batch * a.kv * a.parts : 0;
     if constexpr (Geo<ST, ND>::TILE == 64)
         if (nkv && (a.parts > 1 || eight<ST, ND>(nkv))) {      // (parts are those kernels' alone)
-            if (nq && nq <= 1024) attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
+            // the queries' beside them, unless there are many short ones, whose own
+            // launch has two workgroups a CU (14 x 64 heads in groups of eight x 40 x
+            // 128: 45 us in one launch, 40 in two; but 6 x 48 x 333 x 96, 864
+            // workgroups, 98 and 103, 40 x 2048 x 128, 640 of them, 241 and 284)
+            const bool one = nq <= 256 || (nq <= 1024 && a.tk > 256);
+            if (nq && one) attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
             else attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
             if (a.parts > 1) {
                 const long long n = 2LL * a.batch * a.kv * a.tk * 8 * ND;
                 attn_sum_kernel<ST, ND><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
             }
-            if (!nq || nq <= 1024) return hipGetLastError();
+            if (one) return hipGetLastError();
             nkv = 0;
         }
     if (nq) {
