@@ -601,8 +601,8 @@ __device__ __forceinline__ void take(const unsigned char* at, int lane, f32x16 (
 // One workgroup: 128 rows of a head (of a group's heads beside each other), 32 a
 // wave, over the keys that any of them reads, or a share of those.  SW 2: eight
 // waves, two of which share 32 rows and take half of each tile's keys each.
-// Bound by the matrix instructions and the softmax's vector instructions, as many
-// cycles again, of which two waves a SIMD hide most: 4 x 32 heads x 4096 x 128 in
+// Bound by the matrix instructions, 42 % of the cycles, and the softmax's vector
+// instructions, nearly as many, of which two waves a SIMD hide a part: 4 x 32 heads x 4096 x 128 in
 // bf16, causal, 670 to 700 us, 800 TFLOP/s of the two products (all keys 895; a
 // large library product 1149); 32 heads x 2048 x 128 55 us.  Of a small call a
 // third is a launch, the first loads and the last stores (2 x 12 heads x 1024 x 64
@@ -1247,11 +1247,12 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 // (3 x 10 heads, 5 of keys, 777 x 1021 x 80, 120 and 210 workgroups: 38 + 18 -> 41
 // us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves a
 // tile's rows may be in parts of theirs (AttnArgs::parts), whose sums in f32
-// attn_sum_kernel adds.  Bound by LDS: of a tile of 32 rows a wave of the four
-// reads 40 KB beside 32 matrix instructions, eight waves a CU 156 bytes a cycle of
-// the 128 there are (4 x 32 heads in groups of four x 4096 x 128 in bf16, causal,
-// 1410 to 1440 us, 775 TFLOP/s of the four products; with 64 keys a wave and one
-// wave a SIMD, which read half as much, 2070).
+// attn_sum_kernel adds.  4 x 32 heads in groups of four x 4096 x 128 in
+// bf16, causal, 1400 to 1440 us, 775 TFLOP/s of the four products: matrix
+// instructions in 40 % of the cycles, vector ones in 25, LDS in 30, each waiting for
+// the others' results in turn with two waves a SIMD, which is what the registers
+// hold (64 keys a wave and one wave a SIMD: 2070; waves' priorities raised for the
+// products: 1490).
 template <int ST, int ND, int SW, int QT, bool DK, bool DV, bool VL, int OCC, bool DQ>
 __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, unsigned nkv) {
     typedef Geo<ST, ND> G;
