@@ -34,7 +34,8 @@ struct PlainBuffer {
 };
 
 // Why a tensor's strides are refused, or "".  The kernels reach a tile's rows by
-// 32-bit offsets; an output's elements are distinct.
+// 32-bit offsets (of 128 rows below 2^31, which stands for an element that is
+// not there); an output's elements are distinct.
 inline std::string heads_check(const HeadsBuffer& b, int esz) {
     if (b.count() == 0) return "";
     if (!b.t->p) return b.need ? std::string(b.name) + " is null" : "";
@@ -43,7 +44,7 @@ inline std::string heads_check(const HeadsBuffer& b, int esz) {
     for (int64_t s : {b.t->batch, b.t->seq, b.t->head})
         if (s < 0 || s > kMost) return std::string(b.name) + " has a stride of " + std::to_string(s);
     if (b.seq > 1 && b.t->seq < b.d) return std::string(b.name) + " has rows of " + std::to_string(b.d) + " elements " + std::to_string(b.t->seq) + " apart";
-    if (b.seq > 1 && b.t->seq * esz >= 1ll << 25) return std::string(b.name) + " has rows 2^25 bytes apart or more";
+    if (b.seq > 1 && b.t->seq * esz >= 1ll << 24) return std::string(b.name) + " has rows 2^24 bytes apart or more";
     if (b.out) {
         std::vector<std::pair<int64_t, int64_t>> axes;   // stride, length
         if (b.batch > 1) axes.push_back({b.t->batch, b.batch});

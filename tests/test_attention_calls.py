@@ -211,6 +211,16 @@ def test_strides_that_are_refused(calls):
         op.value(**{**b, "k": far})
 
 
+def test_rows_far_apart(calls):
+    """A tile's rows lie within 2^31 bytes, past which an offset stands for none."""
+    op = attention(batch=1, heads=1, kv_heads=1)
+    b = {n: dev(1, 8, 1, 64) for n in ("q", "k", "v", "o")}
+    wide = torch.empty(7 * 2 ** 23 + 64, dtype=BF)
+    op.value(**{**b, "k": wide.as_strided((1, 8, 1, 64), (0, 2 ** 23 - 8, 0, 1)).as_subclass(Tensor)})
+    with pytest.raises(hip.HipError, match=r"k has rows 2\^24 bytes apart or more"):
+        op.value(**{**b, "k": wide.as_strided((1, 8, 1, 64), (0, 2 ** 23, 0, 1)).as_subclass(Tensor)})
+
+
 def test_the_own_workspace_is_a_streams_and_devices(calls, monkeypatch):
     op = attention()
     for s in (0x10, 0x20, 0x10, 0):
