@@ -353,7 +353,8 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * `what`: PRESK_HIP_ATTN_VALUE writes o and, where it is not null, lse (f32 [batch,
  * heads, q_len]).  PRESK_HIP_ATTN_GRAD writes those of dq, dk and dv whose p is
  * not null from the forward's o and lse.  f16 outputs that overflow set bit 0 of
- * *flag (if flag is not null).
+ * *flag (if flag is not null), of gradients any that is not finite: where ds
+ * overflows they are not, whatever their sums would be.
  * `work`: device memory of presk_hip_attention_workspace bytes (from the sizes
  * alone), 16-byte aligned, this call's until it has run; nothing in it is kept
  * between calls.  An output may not meet another buffer (tensors whose rows lie

@@ -377,8 +377,9 @@ struct Rows {
 // A wave's 32 rows of sums, a lane's times its own f, in the storage type: through
 // the wave's 32 rows of `lds` (which no other wave reads any more), so that a row
 // leaves in 16-byte vectors beside each other.  `where(r)`: row r's address, null
-// where there is none.
-template <int ST, int ND, typename W>
+// where there is none.  GRAD: an element that is not finite counts as one that
+// overflows, since the cotangents of the weights may have.
+template <int ST, int ND, bool GRAD, typename W>
 __device__ __forceinline__ void store_kept(const f32x16 (&acc)[ND], float f, int d, bool vec, bool live, W where, unsigned char* lds, int lane,
                                            unsigned* flag) {
     typedef Geo<ST, ND> G;
@@ -403,7 +404,7 @@ __device__ __forceinline__ void store_kept(const f32x16 (&acc)[ND], float f, int
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[e] = acc[dt][4 * g + e] * f;
-                    if (ST == kF16) ovf |= pk_overflows_f16(x[e]);
+                    if (ST == kF16) ovf |= GRAD ? !(__builtin_fabsf(x[e]) < 65520.f) : pk_overflows_f16(x[e]);
                 }
                 *(unsigned long long*)(lds + r * G::ROW + ((((at >> 3) ^ G::swz(r)) << 4) | ((at & 4) << 1))) =
                     pack2<ST>(x[0], x[1]) | (unsigned long long)pack2<ST>(x[2], x[3]) << 32;
@@ -796,7 +797,7 @@ __global__ void __launch_bounds__(256 * SW, ST == kF32 && ND >= 4 ? 1 : 2) attn_
         }
         return;
     }
-    store_kept<ST, ND>(o[0], l == 0.f ? 0.f : 1.f / l, a.d, a.o.vec, live, [&](int n) -> const void* {
+    store_kept<ST, ND, false>(o[0], l == 0.f ? 0.f : 1.f / l, a.d, a.o.vec, live, [&](int n) -> const void* {
         const int x = r0 + rw * 32 + n;
         return x < rows ? row_at<ST>(a.o, b, x / a.pack, hx * a.pack + x % a.pack) : nullptr;
     }, pair, lane, a.flag);
@@ -1232,7 +1233,7 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
         if (kw == 1) return;
         take<ND>(pair, lane, dq[0], 1.f, 1.f);
     }
-    store_kept<ST, ND>(dq[0], a.scale, a.d, a.dq.vec, live, [&](int x) -> const void* {
+    store_kept<ST, ND, true>(dq[0], a.scale, a.d, a.dq.vec, live, [&](int x) -> const void* {
         return w0 + x <= r1 ? row_at<ST>(a.dq, b, (w0 + x) / a.pack, hx * a.pack + (w0 + x) % a.pack) : nullptr;
     }, pair, lane, a.flag);
 }
@@ -1531,8 +1532,8 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     auto where = [&](const AttnTensor& t) {
         return [&, t](int x) -> const void* { return jw + x < k1 ? row_at<ST>(t, b, jw + x, hk) : nullptr; };
     };
-    if (DK && a.dk.p) store_kept<ST, ND>(dk[0], a.scale, a.d, a.dk.vec, exists, where(a.dk), pair, lane, a.flag);
-    if (DV && a.dv.p) store_kept<ST, ND>(dv[0], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), pair, lane, a.flag);
+    if (DK && a.dk.p) store_kept<ST, ND, true>(dk[0], a.scale, a.d, a.dk.vec, exists, where(a.dk), pair, lane, a.flag);
+    if (DV && a.dv.p) store_kept<ST, ND, true>(dv[0], ST == kF16 ? 0.00390625f : 1.f, a.d, a.dv.vec, exists, where(a.dv), pair, lane, a.flag);
 }
 
 template <int ST, int ND, int SW>
@@ -1567,13 +1568,14 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             x[e] *= f;
-            ovf |= ST == kF16 && pk_overflows_f16(x[e]);
+            ovf |= ST == kF16 && !(__builtin_fabsf(x[e]) < 65520.f);
         }
         if constexpr (ST != kF32)
             *(unsigned long long*)((unsigned short*)out + at) = pack2<ST>(x[0], x[1]) | (unsigned long long)pack2<ST>(x[2], x[3]) << 32;
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ovf |= put<ST, ND>(out, at + e, a.d, x[e] * f);
+        for (int e = 0; e < 4; ++e)
+            ovf |= put<ST, ND>(out, at + e, a.d, x[e] * f) || (ST == kF16 && at + e < a.d && !(__builtin_fabsf(x[e] * f) < 65520.f));
     }
     if (ovf && a.flag) atomicOr(a.flag, 1u);
 }

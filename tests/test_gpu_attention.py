@@ -374,6 +374,27 @@ def test_f16_gradients_that_overflow_set_the_flag():
     assert int(flag) == 1
 
 
+def test_f16_weights_cotangents_that_overflow_set_the_flag():
+    """p (do . v - do . o) past f16, whose sums would not be: two keys of opposite
+    values, so that the cotangents are half of 64 * 4000, times keys of 0.01."""
+    hip.init(0)
+    q, do = torch.zeros(1, 4, 1, 64), torch.full((1, 4, 1, 64), 4000.0)
+    v = torch.ones(1, 2, 1, 64)
+    v[:, 1] = -1
+    q, k, v, do = (x.half().to(DEV) for x in (q, torch.full((1, 2, 1, 64), 0.01), v, do))
+    op = hip.Attention("f16", 1, 1, 1, 4, 2, 64)
+    o, lse, flag = torch.empty_like(q), torch.empty(1, 1, 4, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    op.value(q, k, v, o, lse=lse, flag=flag)
+    dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
+    op.vjp(q, k, v, o, lse, do / 16, dq=dq, dk=dk, dv=dv, flag=flag)
+    assert int(flag) == 0 and bool(torch.isfinite(dq).all())
+    op.vjp(q, k, v, o, lse, do, dq=dq, flag=flag)
+    assert int(flag) == 1
+    flag.zero_()
+    op.vjp(q + 1, k, v, o, lse, do, dk=dk, flag=flag)
+    assert int(flag) == 1
+
+
 def test_a_long_cache():
     """Keys whose elements lie past 2^31 elements and 2^32 bytes: the last ones'
     rows alone are read, by a window."""
