@@ -112,25 +112,33 @@ Plan plan_of(const presk_hip_attn& a, int what) {
         // queries' among them (of a causal square's the longest has twice the mean):
         // to a workgroup a CU, and four tiles each at least (32 heads in groups of
         // four x 1024 x 128, causal, all gradients: 133 -> 82 us in four parts, 40
-        // heads in groups of eight x 2048: 481 -> 250 in three)
+        // heads in groups of eight x 2048: 481 -> 250 in three; heads past 128, whose keys'
+        // have launches of their own, whenever there is room)
         const long long units = a.batch * a.kv_heads * (up(a.k_len, kAttnTile) / kAttnTile);
         const long long span = a.window ? std::min<long long>(a.window + kAttnTile, 1 << 28) : 1 << 28;
         const long long own = per * (up(std::min<long long>(a.q_len, span), 64) / 64);
         const long long queries = a.batch * (a.heads / p.pack) * (up(a.q_len * p.pack, kAttnTile) / kAttnTile) * (up(std::min<long long>(a.k_len, span), 64) / 64);
-        if (p.nd <= (p.st == kF32 ? 2 : 4) && units && own) {
+        if ((p.st != kF32 || p.nd == 2) && units && own) {
             const long long mean = std::max<long long>(1, (units * own + queries) / (a.causal && !a.window ? 512 : 256));
-            p.parts = (int)std::max<long long>(1, std::min({256 / units, own / 4, (own + mean / 2) / mean}));
+            p.parts = (int)std::max<long long>(1, std::min({256 / units, own / 4, p.nd == 8 ? 256 : (own + mean / 2) / mean}));
         }
         if (p.parts > 1) p.part = take(8 * p.parts * a.batch * a.kv_heads * a.k_len * p.nd * 32);
         return p;
     }
     const long long rows = a.q_len * p.pack, units = a.batch * (a.heads / p.pack);
     // few rows in shares of the keys that come to four rounds of the CUs, a workgroup
-    // each (32 sequences' single tokens over 8192 keys: 1024 132 us, 768 137, 2048
-    // 145); others to one (8 x 24 drafted tokens over 4096: 34 us with the join, in
-    // two rounds 35, in four 41)
-    if (rows <= kAttnFew) p.chunk = chunk_of(units, a.k_len, 1024, 256);
-    else if (up(rows, kAttnTile) / kAttnTile * units < 128) p.chunk = chunk_of(up(rows, kAttnTile) / kAttnTile * units, a.k_len, 256, 256);
+    // each (32 sequences' single tokens over 8192 keys: 1024 132 us, 768 137, 2048 145)
+    if (rows <= kAttnFew) {
+        p.chunk = chunk_of(units, a.k_len, 1024, 256);
+    } else {
+        // others to one (8 x 24 drafted tokens over 4096: 34 us with the join, in two
+        // rounds 35, in four 41), where the longest is so much shorter that it pays for
+        // the join: 128 workgroups in two shares each of 4096 keys 77 -> 65 us, of 2048
+        // 42 -> 40, but of 1024 26 -> 32; 64 in four of 1024 25 -> 23, in three of 600
+        // 19 -> 23; in f32, whose keys take longer, 128 in two of 1024 53 -> 42
+        p.chunk = chunk_of(up(rows, kAttnTile) / kAttnTile * units, a.k_len, 256, 256);
+        if ((a.k_len - p.chunk) * (p.st == kF32 ? 2 : 1) < 768) p.chunk = 0;
+    }
     p.splits = p.chunk ? (int)std::max<long long>(1, (a.k_len + p.chunk - 1) / p.chunk) : 1;
     if (p.splits > 1) {
         p.part = take(4 * all * p.splits * p.nd * 32);

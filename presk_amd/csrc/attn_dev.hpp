@@ -1246,9 +1246,9 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 // workgroup a CU has the room, the keys beside them.  DQ: the queries' workgroups
 // follow the `nkv` of the keys in one launch, where either would leave CUs idle
 // (3 x 10 heads, 5 of keys, 777 x 1021 x 80, 120 and 210 workgroups: 38 + 18 -> 41
-// us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves a
-// tile's rows may be in parts of theirs (AttnArgs::parts), whose sums in f32
-// attn_sum_kernel adds.  4 x 32 heads in groups of four x 4096 x 128 in
+// us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves, or
+// heads past 128, a tile's rows may be in parts of theirs (AttnArgs::parts), whose
+// sums in f32 attn_sum_kernel adds.  4 x 32 heads in groups of four x 4096 x 128 in
 // bf16, causal, 1400 to 1440 us, 775 TFLOP/s of the four products: matrix
 // instructions in 40 % of the cycles, vector ones in 25, LDS in 30, each waiting for
 // the others' results in turn with two waves a SIMD, which is what the registers
@@ -1270,8 +1270,9 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     const int rw = wave & 3, kw = wave >> 2;      // which keys, and which of a tile's rows
     const int tiles = (a.tk + KEYS - 1) / KEYS;
     unsigned at = item_of(blockIdx.x, DQ ? nkv : gridDim.x);
-    const int part = SW == 2 ? (int)(at % (unsigned)a.parts) : 0;
-    if (SW == 2) at /= (unsigned)a.parts;
+    constexpr bool PARTS = SW == 2 || ND == 8;      // (the kernels of small launches)
+    const int part = PARTS ? (int)(at % (unsigned)a.parts) : 0;
+    if (PARTS) at /= (unsigned)a.parts;
     const int tile = (int)(at % (unsigned)tiles), unit = (int)(at / (unsigned)tiles);
     const int b = unit % a.batch, hk = unit / a.batch;
     const int k0 = tile * KEYS, k1 = a.tk < k0 + KEYS ? a.tk : k0 + KEYS;
@@ -1303,7 +1304,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     const int nt1 = ihi > ilo ? (ihi - ilo + QT - 1) / QT : 0;
     int nt = nt1 * a.per, t0 = 0;
     int fi = ilo, fg = 0;       // the next tile's first row, and its head in the group
-    if (SW == 2 && a.parts > 1) {
+    if (PARTS && a.parts > 1) {
         const int share = (nt + a.parts - 1) / a.parts;
         t0 = part * share < nt ? part * share : nt;
         nt = t0 + share < nt ? t0 + share : nt;
@@ -1516,16 +1517,16 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     if (j >= keys.len)
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) dk[0][dt] = dv[0][dt] = f32x16{};
-    if (SW == 2 && a.parts > 1) {
-        // (kw 0: the waves that have both halves)
+    if (PARTS && a.parts > 1) {
+        // (of eight waves those that have both halves)
         const long long all = (long long)a.batch * a.kv * a.tk, row = part * all + ((long long)b * a.kv + hk) * a.tk + j;
         if (exists)
 #pragma unroll
             for (int g = 0; g < 4 * ND; ++g) {
                 float* const to = a.part + row * (ND * 32) + g / 4 * 32 + 8 * (g & 3) + 4 * h;
                 const f32x16 &x = dk[0][g / 4], &y = dv[0][g / 4];
-                *(f32x4*)to = f32x4{x[g % 4 * 4], x[g % 4 * 4 + 1], x[g % 4 * 4 + 2], x[g % 4 * 4 + 3]};
-                *(f32x4*)(to + a.parts * all * (ND * 32)) = f32x4{y[g % 4 * 4], y[g % 4 * 4 + 1], y[g % 4 * 4 + 2], y[g % 4 * 4 + 3]};
+                if (DK) *(f32x4*)to = f32x4{x[g % 4 * 4], x[g % 4 * 4 + 1], x[g % 4 * 4 + 2], x[g % 4 * 4 + 3]};
+                if (DV) *(f32x4*)(to + a.parts * all * (ND * 32)) = f32x4{y[g % 4 * 4], y[g % 4 * 4 + 1], y[g % 4 * 4 + 2], y[g % 4 * 4 + 3]};
             }
         return;
     }
@@ -1620,6 +1621,10 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
     if (all) attn_rows_kernel<ST><<<(unsigned)((all + 15) / 16), 256, 0, s>>>(a);
     const long long nq = a.dq.p ? ((long long)a.tq * a.pack + 127) / 128 * a.batch * (a.heads / a.pack) : 0;
     long long nkv = a.dk.p || a.dv.p ? (long long)((a.tk + 127) / 128) * a.batch * a.kv * a.parts : 0;
+    const auto add_parts = [&] {
+        const long long n = 2LL * a.batch * a.kv * a.tk * 8 * ND;
+        if (a.parts > 1) attn_sum_kernel<ST, ND><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    };
     if constexpr (Geo<ST, ND>::TILE == 64)
         if (nkv && (a.parts > 1 || eight<ST, ND>(nkv))) {      // (parts are those kernels' alone)
             // the queries' beside them, unless there are many short ones, whose own
@@ -1629,10 +1634,7 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
             const bool one = nq <= 256 || (nq <= 1024 && a.tk > 256);
             if (nq && one) attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, true><<<(unsigned)(nkv + nq), 512, 0, s>>>(a, (unsigned)nkv);
             else attn_dkv_kernel<ST, ND, 2, 64, true, true, WIDE, 2, false><<<(unsigned)nkv, 512, 0, s>>>(a, (unsigned)nkv);
-            if (a.parts > 1) {
-                const long long n = 2LL * a.batch * a.kv * a.tk * 8 * ND;
-                attn_sum_kernel<ST, ND><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
-            }
+            add_parts();
             if (one) return hipGetLastError();
             nkv = 0;
         }
@@ -1648,6 +1650,7 @@ hipError_t bwd(const AttnArgs& a, hipStream_t s) {
             // (both sums of 256 elements and both kept rows do not fit the registers)
             if (a.dk.p) attn_dkv_kernel<ST, ND, 1, 32, true, false, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
             if (a.dv.p) attn_dkv_kernel<ST, ND, 1, 32, false, true, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
+            add_parts();
         } else if constexpr (ST == kF32 && ND == 4) {
             attn_dkv_kernel<ST, ND, 1, 32, true, true, false, 1, false><<<(unsigned)nkv, 256, 0, s>>>(a, (unsigned)nkv);
         } else {

@@ -87,10 +87,12 @@ def test_all_workgroups_on_the_chip_at_once(dtype, size):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("kind", ["all", "causal", "window", "lengths", "mask", "dk", "dv"])
-@pytest.mark.parametrize("d", [20, 64, 128])
+@pytest.mark.parametrize("d", [20, 64, 128, 200])
 def test_few_keys_and_many_rows(dtype, kind, d):
     """Keys' gradients that one workgroup a tile would leave CUs idle for: in parts
     of the rows, of which some may have none."""
+    if dtype == "f32" and d > 128:
+        pytest.skip("f32 heads end at 128")
     b, h, kv, tq, tk = 2, 6, 2, 610, 200
     q, k, v, do = tensors(dtype, b, h, kv, tq, tk, d, seed=d)
     g = torch.Generator().manual_seed(d)
