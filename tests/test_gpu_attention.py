@@ -339,6 +339,53 @@ def test_a_captured_call_replays():
         assert all(torch.equal(x, y) for x, y in zip(got, again)), step
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_captured_shares_and_parts(dtype):
+    """Keys in shares, their gradients in parts beside the queries', single tokens:
+    two graphs of them that share one workspace, replayed in turn with eager calls
+    between, over inputs that change."""
+    hip.init(0)
+    b, h, kv, tq, tk, d = 1, 8, 2, 300, 2100, 64
+    q, k, v, do = (x.to(DEV) for x in tensors(dtype, b, h, kv, tq, tk, d))
+    lens, first = torch.tensor([1200], device=DEV), torch.tensor([900], device=DEV)
+    op, one = hip.Attention(dtype, b, h, kv, tq, tk, d, causal=True), hip.Attention(dtype, b, h, kv, 1, tk, d, causal=True)
+    need = max(op.workspace("value"), op.workspace("vjp"), one.workspace("value"))
+    rows = 4 * b * h * tq
+    assert op.workspace("value") > 64 * rows and op.workspace("vjp") > 2 * rows + 4 * 2 * b * kv * tk * d     # (shares, parts)
+    work = torch.empty(need, dtype=torch.uint8, device=DEV)
+
+    def call(outs, work, i):
+        o, lse, dq, dk, dv, o1 = outs
+        if i == 0:
+            op.value(q, k, v, o, lse=lse, lens=lens, first=first, work=work)
+            op.vjp(q, k, v, o, lse, do, dq=dq, dk=dk, dv=dv, lens=lens, first=first, work=work)
+        else:
+            one.value(q[:, -1:], k, v, o1, lens=lens, first=last, work=work)
+
+    def outs():
+        return [torch.empty_like(q), torch.empty(b, h, tq, device=DEV), *(torch.empty_like(x) for x in (q, k, v)), torch.empty_like(q[:, -1:])]
+
+    last = lens - 1
+    mine, graphs = outs(), []
+    for i in (0, 1):
+        call(mine, work, i)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            call(mine, work, i)
+    for step in range(3):
+        lens.add_(300), first.add_(300), last.add_(300)
+        k.mul_(1.1)
+        for x in mine:
+            x.fill_(9.0)
+        graphs[0].replay(), graphs[1].replay()
+        again = outs()
+        for i in (0, 1):
+            call(again, torch.empty_like(work), i)
+        torch.cuda.synchronize()
+        assert [n for n, x, y in zip(("o", "lse", "dq", "dk", "dv", "o1"), mine, again) if not torch.equal(x, y)] == [], step
+
+
 def test_two_streams():
     """Calls of one object on two streams with no wait between them."""
     hip.init(0)
