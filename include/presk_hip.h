@@ -363,7 +363,7 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * Storage types f32 (head_dim to 128), bf16 and f16 (to 256), others are E7005;
  * q_len, k_len, mask_cols and window below 2^28, a mask of batch * q_len * mask_cols
  * below 2^35 (of lengths in whole 32s); a row's stride (seq) at least head_dim
- * elements and below 2^24 bytes. */
+ * elements and below 2^24 bytes, of a single row anything from 0 to 2^40. */
 typedef struct {
     void* p;
     int64_t batch, seq, head;

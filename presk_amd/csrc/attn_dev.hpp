@@ -1325,6 +1325,8 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
             qt.init(a.q, b, head, a.d, tid, lds);
             dt_.init(a.dout, b, head, a.d, tid, lds + Tile::BYTES);
         }
+        // (rows past ihi are zeros, the cotangent's and both sums' too, and so add nothing
+        // where no mask leaves them out)
         const int left = ihi - i0;
         qt.issue(i0, left, stage, smem, tid);
         dt_.issue(i0, left, stage, smem + Tile::BYTES, tid);

@@ -460,3 +460,49 @@ def test_a_long_cache():
     op.value(q.to(DEV), k, v, o)
     case = A.Case("bf16", q, kl, vl, A.allowed(1, 3, w, True, w - 2), op.scale)
     A.check("o", o, *case.value()["o"])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("stride", [0, 1, 2 ** 26, 2 ** 40])
+@pytest.mark.parametrize("tq, tk", [(1, 5), (1, 300), (70, 1)])
+def test_one_row_whose_stride_says_nothing(dtype, causal, stride, tq, tk):
+    """A length of one leaves a tensor's row stride free: that of an expanded tensor is
+    0, and a large one times a tile's row numbers would pass 32 bits."""
+    hip.init(0)
+    b, h, kv, d = 2, 4, 2, 64
+    q, k, v, do = tensors(dtype, b, h, kv, tq, tk, d)
+
+    def far(x):
+        x = x.to(DEV)
+        return x.as_strided(x.shape, (x.stride(0), stride, d, 1)) if x.shape[1] == 1 else x
+
+    op = hip.Attention(dtype, b, h, kv, tq, tk, d, causal=causal)
+    Q, K, V, DO = map(far, (q, k, v, do))
+    o, dq, dk, dv = (far(torch.full_like(x, 9.0)) for x in (q, q, k, v))
+    lse = torch.empty(b, h, tq, device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    op.vjp(Q, K, V, o, lse, DO, dq=dq, dk=dk, dv=dv)
+    case = A.Case(dtype, q, k, v, A.allowed(b, tq, tk, causal), op.scale, do)
+    A.check("o", o, *case.value()["o"])
+    want = case.vjp(o.cpu(), lse.cpu())
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        A.check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_cotangent_that_is_shared(dtype):
+    """One query's, of one row for all sequences and heads by expansion."""
+    hip.init(0)
+    b, h, kv, tk, d = 3, 4, 2, 200, 64
+    q, k, v, _ = tensors(dtype, b, h, kv, 1, tk, d)
+    do = torch.linspace(-1, 2, d).to(A.TORCH[dtype]).expand(b, 1, h, d)
+    op = hip.Attention(dtype, b, h, kv, 1, tk, d)
+    Q, K, V = (x.to(DEV) for x in (q, k, v))
+    o, lse = torch.empty_like(Q), torch.empty(b, h, 1, device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    grads = {n: torch.empty_like(x) for n, x in (("dq", Q), ("dk", K), ("dv", V))}
+    op.vjp(Q, K, V, o, lse, do[0, 0, 0].to(DEV).expand(b, 1, h, d), **grads)
+    want = A.Case(dtype, q, k, v, A.allowed(b, 1, tk), op.scale, do).vjp(o.cpu(), lse.cpu())
+    for n, g in grads.items():
+        A.check(n, g, *want[n])
