@@ -220,6 +220,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
                     // the hardware's root, refined once
                     const float m = __builtin_fmaf(over_lanes(ss, a.lanes), a.per_d, a.eps), r = __builtin_amdgcn_rsqf(m);
                     rstd = !(m >= 1e-30f && m <= 1e30f) ? 1.f / sqrtf(m) : __builtin_fmaf(__builtin_fmaf(-m * r, r, 1.f), 0.5f * r, r);
+                    // (lanes without a head would have 1 / sqrt(eps), infinite for none, times
+                    // their zeros in the gains' sums)
+                    if (GRAD && head >= end) rstd = 0.f;
                 }
                 if constexpr (MODE == kNormed)
 #pragma unroll

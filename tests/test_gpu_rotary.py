@@ -158,3 +158,28 @@ def test_a_captured_call_replays():
         call(*again, torch.empty_like(work))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, again)), step
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("size", [(1, 3, 3, 1, 64), (2, 33, 4, 2, 128), (1, 5, 7, 8, 64), (2, 9, 3, 2, 33)], ids=str)
+def test_a_norm_without_eps(dtype, eps, size):
+    """Lanes beyond the last head have no elements, whose norm would be infinite."""
+    hip.init(0)
+    b, n, h, kv, d = size
+    q, k, dyq, dyk, gq, gk = tensors(dtype, *size, seed=d)
+    rot = d // 2 * 2
+    op = hip.HeadRotary(dtype, b, n, h, kv, d, rotary=rot, norm=True, eps=eps)
+    freq = torch.from_numpy(hip.rotary_frequencies(rot))
+    Q, K, DYQ, DYK, GQ, GK = (x.to(DEV) for x in (q, k, dyq, dyk, gq, gk))
+    yq, yk, dq, dk = (torch.full_like(x, 9.0) for x in (Q, K, Q, K))
+    dgq, dgk = torch.full_like(GQ, 9.0), torch.full_like(GK, 9.0)
+    op.value(Q, freq.to(DEV), yq, k=K, yk=yk, gq=GQ, gk=GK)
+    op.vjp(freq.to(DEV), DYQ, dq, dyk=DYK, dk=dk, q=Q, k=K, gq=GQ, gk=GK, dgq=dgq, dgk=dgk)
+    at = torch.arange(n).expand(b, n)
+    for x, g, dy, y, dx, dg in ((q, gq, dyq, yq, dq, dgq), (k, gk, dyk, yk, dk, dgk)):
+        spec = (dtype, x, g, freq, at, rot, True, eps, False)
+        A.check("y", y, *A.rotary(*spec))
+        want = A.rotary(*spec, dy=dy)
+        A.check("dx", dx, *want["dx"])
+        A.check("dg", dg, *want["dg"])
