@@ -409,9 +409,10 @@ int presk_hip_batch_add_attention(presk_hip_batch* b, const presk_hip_attn* a, i
  * PRESK_HIP_ROT_VALUE writes yq and yk (which may be q and k themselves);
  * PRESK_HIP_ROT_GRAD, from their cotangents dyq and dyk and, with `norm`, q and k,
  * writes dq and dk (which may be dyq and dyk) and those of dgq and dgk ([head_dim])
- * that are not null.  Sums in f32, angles in f64 (so that one of 2^30
- * radians is right to 2^-23); tensors, f16's flag, `work` (null and 0 bytes do but for a gradient with
- * `norm`), streams and graphs as presk_hip_attention's. */
+ * that are not null.  Sums in f32, angles in f64 (so that the cosine and sine of one
+ * of 2^30 radians are within 2^-23 of those of its f64 product); tensors, f16's flag,
+ * `work` (null and 0 bytes do but for a gradient with `norm`), streams and graphs as
+ * presk_hip_attention's. */
 typedef struct {
     const char* dtype;
     int64_t batch, seq, heads, kv_heads, head_dim, rotary;

@@ -6,8 +6,8 @@
 // A wave takes a token and some of its heads of q, or of k: a head is `lanes` lanes,
 // each with two runs of EC elements that are each other's partners, so that no lane
 // needs another's; the angles, the same for all heads, are worked out once a wave.
-// They are turns in f64, of which whole quarters drop out before f32: a position of
-// 10^6 keeps what an angle near zero has.
+// They are f64, of which whole quarter turns drop out before f32: a position of 10^6
+// keeps what an angle near zero has.
 // Bound by its bytes, x read and y written once, as long as the work on them stays
 // at a few instructions an element: one kernel that told q from k and pairs from
 // halves as it went took 47 an element, and 44 us for 2 x 4096 x (32 + 8) heads x 128
@@ -83,11 +83,13 @@ struct alignas(EC * sizeof(typename Elem<ST>::T)) Run {
     typename Elem<ST>::T v[EC];
 };
 
-// cos and sin of `turns` quarter turns: the nearest whole one taken off in f64,
-// the rest, at most pi / 4, by the series (to 2e-9).
-__device__ __forceinline__ void turned(double quarters, float* c, float* s) {
-    const double n = __builtin_rint(quarters);
-    const float x = (float)((quarters - n) * 1.5707963267948966);
+// cos and sin of an angle: the nearest number of quarter turns taken off in f64, pi / 2
+// in two parts by an fma each (Cody and Waite's reduction), the rest, at most pi / 4,
+// by the series (to 2e-9).  An angle of 2^30 radians loses nothing that its f64 has:
+// 4096 angles below it 6.6e-8 off, by one product with 2 / pi 1.8e-7.
+__device__ __forceinline__ void turned(double angle, float* c, float* s) {
+    const double n = __builtin_rint(angle * 0.63661977236758134);
+    const float x = (float)__builtin_fma(-n, 6.1232339957367660e-17, __builtin_fma(-n, 1.5707963267948966, angle));
     const float z = x * x;
     float a = __builtin_fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
     a = __builtin_fmaf(z, a, 8.3333333e-3f);
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
             for (int e = 0; e < EC; ++e) {
                 cs[k][e] = 1.f, sn[k][e] = 0.f;
                 // (neighbours paired: the two runs' EC pairs in order)
-                if (turns[k]) turned(at * a.freq[EC * (mine + k * a.lanes) + e] * 0.6366197723675814, &cs[k][e], &sn[k][e]);
+                if (turns[k]) turned(at * a.freq[EC * (mine + k * a.lanes) + e], &cs[k][e], &sn[k][e]);
                 sn[k][e] *= a.sign;
             }
         for (int h0 = first; h0 < end; h0 += U * beside) {

@@ -183,3 +183,28 @@ def test_a_norm_without_eps(dtype, eps, size):
         want = A.rotary(*spec, dy=dy)
         A.check("dx", dx, *want["dx"])
         A.check("dg", dg, *want["dg"])
+
+
+@pytest.mark.parametrize("pairs", ["half", "even"])
+@pytest.mark.parametrize("d", [2, 64])
+def test_an_angle_of_2_30_radians(pairs, d):
+    """Is right to 2^-23 of its f64 product's: whole turns are taken off without loss, so
+    that what is left is f32's rounding of the angle (2^-25 at most), of its cosine
+    or sine (2^-25) and of their series."""
+    hip.init(0)
+    n = 4096
+    g = torch.Generator().manual_seed(d)
+    at = (2 ** 30 - torch.randint(0, 2 ** 28, (2, n), generator=g)).contiguous()
+    freq = 1.0 - torch.rand(d // 2, generator=g, dtype=torch.float64) * 0.2
+    x = torch.zeros(2, n, 1, d)
+    first = x[..., 0::2] if pairs == "even" else x[..., :d // 2]
+    first += 1.0
+    op = hip.HeadRotary("f32", 2, n, 1, 0, d, pairs=pairs)
+    y = torch.empty_like(x, device=DEV)
+    op.value(x.to(DEV), freq.to(DEV), y, at=at.to(DEV))
+    y = y.cpu().double()
+    angle = at.double()[:, :, None, None] * freq
+    c, s = (y[..., 0::2], y[..., 1::2]) if pairs == "even" else (y[..., :d // 2], y[..., d // 2:])
+    worst = max(float((c - torch.cos(angle)).abs().max()), float((s - torch.sin(angle)).abs().max()))
+    print(f"{worst:.3g}", flush=True)
+    assert worst <= 2.0 ** -23
