@@ -506,3 +506,34 @@ def test_a_cotangent_that_is_shared(dtype):
     want = A.Case(dtype, q, k, v, A.allowed(b, 1, tk), op.scale, do).vjp(o.cpu(), lse.cpu())
     for n, g in grads.items():
         A.check(n, g, *want[n])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["all", "causal", "window", "lengths", "mask"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_more_workgroups_than_cus(dtype, kind, d):
+    """528 tiles of queries and of keys: the kernels of four waves, each gradient's a
+    launch of its own."""
+    b, h, n = 33, 8, 130
+    q, k, v, do = tensors(dtype, b, h, h, n, n, d, seed=d)
+    g = torch.Generator().manual_seed(d)
+    lens = torch.randint(0, n + 1, (b,), generator=g)
+    mask = torch.rand(b, n, n, generator=g) < 0.3
+    mask[::3, 32:, 32:96] = False                    # (whole blocks without any)
+    more = {"all": {}, "causal": {"causal": True}, "window": {"causal": True, "window": 50, "first": torch.randint(-40, 40, (b,), generator=g)},
+            "lengths": {"lens": lens, "causal": True, "first": lens - n}, "mask": {"mask": mask}}[kind]
+    run(dtype, q, k, v, do, **more)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [(14, 64, 8, 40, 40, 128), (14, 64, 8, 40, 40, 64), (1, 40, 2, 3400, 130, 64), (1, 40, 2, 3400, 130, 128),
+                                  (2, 12, 4, 2100, 70, 96)], ids=str)
+def test_the_queries_gradient_after_the_keys(dtype, size):
+    """Few tiles of keys, whose kernel has eight waves, and many of queries."""
+    run(dtype, *tensors(dtype, *size, seed=5), causal=size[3] == size[4])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_of_a_grouped_step(dtype):
+    """Heads in groups of four, over 256 tiles of either, head after head."""
+    run(dtype, *tensors(dtype, 9, 32, 8, 400, 400, 64, seed=2), causal=True)
