@@ -537,3 +537,20 @@ def test_the_queries_gradient_after_the_keys(dtype, size):
 def test_rows_of_a_grouped_step(dtype):
     """Heads in groups of four, over 256 tiles of either, head after head."""
     run(dtype, *tensors(dtype, 9, 32, 8, 400, 400, 64, seed=2), causal=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [(4, 2, 1, 1, 6000, 64), (2, 8, 2, 3, 9000, 128), (1, 3, 1, 5, 5000, 80)], ids=str)
+def test_many_shares_of_the_keys(dtype, size):
+    """More than 16 shares of a sequence's keys, which a workgroup's waves join; some
+    sequences have fewer, and none."""
+    lens = torch.tensor([size[4], 300, 0, 4500])[:size[0]]
+    run(dtype, *tensors(dtype, *size, seed=7), lens=lens, grad=False)
+    run(dtype, *tensors(dtype, *size, seed=8), grad=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_shares_than_a_waves_lanes(dtype):
+    """274 shares, 64 times 4 and the rest."""
+    run(dtype, *tensors(dtype, 1, 2, 1, 1, 70000, 64, seed=9), grad=False)
+    run(dtype, *tensors(dtype, 1, 2, 1, 2, 70000, 64, seed=10), causal=True, grad=False)
