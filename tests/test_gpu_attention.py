@@ -554,3 +554,73 @@ def test_more_shares_than_a_waves_lanes(dtype):
     """274 shares, 64 times 4 and the rest."""
     run(dtype, *tensors(dtype, 1, 2, 1, 1, 70000, 64, seed=9), grad=False)
     run(dtype, *tensors(dtype, 1, 2, 1, 2, 70000, 64, seed=10), causal=True, grad=False)
+
+
+def sum_error(rows, d, lse, value=False):
+    """What f32 sums over `rows` random terms p x may be off by, root mean square over
+    that of the sums, and half as much again; in half steps (2^-24) of them:
+    the sums: one rounding every 32 rows, 0.41 on average of a partial one's, which
+    grow as a random walk's: 0.41 sqrt(rows / 32 / 2);
+    a matrix instruction: a step at most, 0.82 on average, six every 16 elements of a
+    score and of a cotangent, and as many every 16 of the 32 rows;
+    a number between 2^e and 2^(e + 1): 0.58 2^e.  p = exp2(s log2 e - lse log2 e) has
+    that difference's, times ln 2, and lse's: in log 2 and times ln 2, as it is
+    stored, and times log2 e again, and of the weights' sum, whose partial ones grow
+    evenly, 0.41 sqrt(keys / 32 / 3).  The value has the sum's and the difference's."""
+    product, block = 0.82 * math.sqrt(6 * d / 16 / 2), 0.82 * math.sqrt(12 / 2)
+    step = lambda x: 0.58 * 2.0 ** math.floor(math.log2(x))  # noqa: E731
+    log2 = step(lse / math.log(2)) * math.log(2)
+    weights = 0.41 * math.sqrt(math.exp(lse) / 32 / 3)
+    terms = [product, block, log2, weights] + ([] if value else [product, log2, step(lse), log2])
+    return 1.5 * A.F * math.sqrt(0.41 ** 2 * rows / 32 / 2 + sum(x * x for x in terms))
+
+
+def off(got, want):
+    return float((got.double() - want).square().mean().sqrt() / want.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kv", [128, 129])
+def test_f32_sums_over_a_groups_rows(d, kv):
+    """Keys' and values' gradients over 4 x 4096 rows, by eight waves and by four."""
+    hip.init(0)
+    per, tq, tk = 4, 4096, 256
+    g = torch.Generator(DEV).manual_seed(d + kv)
+    q, k, v, do = (torch.randn(1, n, h, d, generator=g, device=DEV) for n, h in ((tq, per * kv), (tk, kv), (tk, kv), (tq, per * kv)))
+    op = hip.Attention("f32", 1, per * kv, kv, tq, tk, d)
+    o, lse = torch.empty_like(q), torch.empty(1, per * kv, tq, device=DEV)
+    op.value(q, k, v, o, lse=lse)
+    dk, dv = torch.empty_like(k), torch.empty_like(v)
+    op.vjp(q, k, v, o, lse, do, dk=dk, dv=dv)
+    for head in (0, kv - 1):
+        x, y = (t[0, :, head * per:(head + 1) * per].double().transpose(0, 1) for t in (q, do))
+        kd, vd = k[0, :, head].double(), v[0, :, head].double()
+        p = torch.softmax(x @ kd.T * op.scale, -1)
+        dp = y @ vd.T
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * op.scale
+        worst = {"dv": off(dv[0, :, head], sum(p[n].T @ y[n] for n in range(per))), "dk": off(dk[0, :, head], sum(ds[n].T @ x[n] for n in range(per)))}
+        print({n: f"{e:.3g}" for n, e in worst.items()}, flush=True)
+        assert max(worst.values()) <= sum_error(per * tq, d, math.log(tk) + 0.5), worst
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [256, 264])
+def test_f32_sums_over_many_keys(d, heads):
+    """The value and the queries' gradient over 16384 keys."""
+    hip.init(0)
+    kv, tq, tk = 8, 128, 16384
+    g = torch.Generator(DEV).manual_seed(d + heads)
+    q, k, v, do = (torch.randn(1, n, h, d, generator=g, device=DEV) for n, h in ((tq, heads), (tk, kv), (tk, kv), (tq, heads)))
+    op = hip.Attention("f32", 1, heads, kv, tq, tk, d)
+    o, lse, dq = torch.empty_like(q), torch.empty(1, heads, tq, device=DEV), torch.empty_like(q)
+    op.value(q, k, v, o, lse=lse)
+    op.vjp(q, k, v, o, lse, do, dq=dq)
+    for head in (0, heads - 1):
+        x, y, kd, vd = (t[0, :, n].double() for t, n in ((q, head), (do, head), (k, head * kv // heads), (v, head * kv // heads)))
+        p = torch.softmax(x @ kd.T * op.scale, -1)
+        dp = y @ vd.T
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * op.scale
+        worst = {"o": off(o[0, :, head], p @ vd), "dq": off(dq[0, :, head], ds @ kd)}
+        print({n: f"{e:.3g}" for n, e in worst.items()}, flush=True)
+        assert worst["o"] <= sum_error(tk, d, math.log(tk) + 0.5, value=True), worst
+        assert worst["dq"] <= sum_error(tk, d, math.log(tk) + 0.5), worst
