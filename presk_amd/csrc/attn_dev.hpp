@@ -47,8 +47,10 @@ template <int ST> struct FragOf { typedef u16x8 T; };
 template <> struct FragOf<kF32> { typedef f32x4 T; };
 
 // A matrix instruction's eight elements a lane.  f32 in three parts of 8 bits
-// each, rounded to nearest, which are all of its 24: of a product's nine six are
-// taken (the three left are below 2^-24 of it together, f32's own rounding), by
+// each, rounded to nearest, which are all of its 24 down to 2^-110 (where the last
+// part's come to bf16's smallest step, 2^-133: scaling that away is an instruction an
+// element more, and a second pass for the large ones, on what these kernels are
+// bound by): of a product's nine six are taken (the three left are below 2^-24 of it together, f32's own rounding), by
 // bf16 instructions, of which six take 3/8 of the time of f32's own (64 x 6 heads x
 // 256 x 64, causal: the value 63 -> 50 us, the queries' gradient 87 -> 64, the keys'
 // 121 -> 98, with errors against 64 bits as before; bound now by the eleven vector

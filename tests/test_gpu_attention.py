@@ -624,3 +624,26 @@ def test_f32_sums_over_many_keys(d, heads):
         print({n: f"{e:.3g}" for n, e in worst.items()}, flush=True)
         assert worst["o"] <= sum_error(tk, d, math.log(tk) + 0.5, value=True), worst
         assert worst["dq"] <= sum_error(tk, d, math.log(tk) + 0.5), worst
+
+
+@pytest.mark.parametrize("n", [40, 400])
+def test_f32_small_elements(n):
+    """Three bf16 parts are all of an element down to 2^-110; below, the last is a
+    multiple of bf16's smallest step, 2^-133, of which half may be lost."""
+    hip.init(0)
+    g = torch.Generator().manual_seed(n)
+    v = torch.randn(1, 1, 60, 64, generator=g, dtype=torch.float64) * 2.0 ** -torch.arange(100, 130, 0.5, dtype=torch.float64)[None, None, :, None]
+    v = v.float().transpose(1, 2).contiguous()                  # [1, 60 keys, 1, 64]
+    q = torch.zeros(1, n, 1, 64)
+    k = torch.zeros(1, 60, 1, 64)
+    i = torch.arange(n) % 60
+    first = torch.tensor([0])
+    mask = torch.zeros(n, 60, dtype=torch.bool)
+    mask[torch.arange(n), i] = True                             # query i reads one key
+    op = hip.Attention("f32", 1, 1, 1, n, 60, 64, mask_cols=60)
+    o = torch.empty(1, n, 1, 64, device=DEV)
+    op.value(q.to(DEV), k.to(DEV), v.to(DEV), o, first=first.to(DEV), mask=mask.to(DEV))
+    want = v[0, i, 0].double()
+    err = (o.cpu()[0, :, 0].double() - want).abs()
+    print(float((err / (2.0 ** -134 + 2.0 ** -24 * want.abs())).max()))
+    assert (err <= 2.0 ** -134 + 2.0 ** -24 * want.abs()).all()
