@@ -346,7 +346,8 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * Products accumulate in f32, and so do the sums of a softmax.  In 16-bit storage
  * the weights p and their cotangents ds are rounded to the storage type before
  * the products they enter, ds with what that rounding left as a second term where
- * queries read fewer than 64 keys or a mask says which.  f32 elements enter as
+ * queries read fewer than 64 keys or a mask says which; in f16 ds times a power of
+ * two, 1 or more, that keeps small ones' bits and is taken out of the sums.  f32 elements enter as
  * three bf16 parts, which are all of one of 2^-110 or more (below, what is left of it
  * may be off by 2^-134), and six of their nine products (the rest is below 2^-24);
  * one that is infinite, or above 0x1.ffp127, gives NaN.

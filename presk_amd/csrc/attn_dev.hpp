@@ -1094,6 +1094,43 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
 
 // In f16 the weights, most of them far below one, enter their product times 2^8.
 constexpr float kShift = 8.f;
+// Their cotangents, of whatever size the gradient's are (a mean loss's 10^-4 left
+// them f16's last bits, and the gradients 4 times the error), times a power of two of
+// the wave's own, 2^up: as large a one as leaves the largest so far below 2^15 (those
+// of 2^-22 of it and more are whole), and one at least, so that those past f16 still
+// show.  As with a softmax's maximum, the sums go along with it where it has to fall,
+// then by so much that the largest is past 2^8.  (Gradients of 4 x 32 heads in groups of four
+// x 4096 x 128, causal: 2400 us without it, 2540 so, 2730 with a power for each kept row,
+// which takes registers; shorter ones 2 to 6 % more than without.)
+constexpr int kUp = 60;     // (2^60 times the largest of them, 2^41, stays in f32)
+template <int ND>
+__device__ __forceinline__ void fit_f16(f32x16& s, f32x16 (&acc)[ND], int& up, bool live) {
+    float mx = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, __builtin_fabsf(s[e]));
+    // (a lane without a row has scores of 0, and weights of any size)
+    mx = live ? mx : 0.f;
+    if (up == 0 || !__any(mx > 32768.f)) return;
+    const unsigned top = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(unsigned, all_of<64>(mx, nullptr, max_f)));
+    const int by = max(135 - (int)(top >> 23), -up);
+    const float f = __builtin_ldexpf(1.f, by);
+    up += by;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= f;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] *= f;
+}
+// The sums as they are.
+template <int ND>
+__device__ __forceinline__ void unfit_f16(f32x16 (&acc)[ND], int up) {
+    const float f = __builtin_ldexpf(1.f, -up);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] *= f;
+}
 
 // The queries' gradient: as the value's kernel, with the cotangent's rows beside
 // the queries' (4 x 32 heads x 4096 x 128, causal, 840 to 880 us, 960 TFLOP/s of the
@@ -1149,6 +1186,7 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
     Part<ST> q[NB][G::KSTEPS], dout[NB][G::KSTEPS];
     float lse[NB], delta[NB];
     f32x16 dq[NB][ND];
+    int up = kUp;       // (f16)
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         load_kept<ST, ND>(a.q, b, i, head, a.d, live, lane, own, q[n]);
@@ -1198,13 +1236,15 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
         Weights<ST> w[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
+            const float row = ST == kF16 ? lse[n] + (float)up : lse[n];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], a.c, lse[n])) * (dp[n][e] + delta[n]);
+            for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], a.c, row)) * (dp[n][e] + delta[n]);
             if (masked) {
                 const unsigned in = (bits[n] & range_of(keys.lo(a, i) - base, keys.hi(a, i) - base)) >> (4 * h);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[n][e] = where_bit(in, e, s[n][e], 0.f);
             }
+            if (ST == kF16) fit_f16<ND>(s[n], dq[n], up, live);
             w[n].set(s[n]);
         }
         mma_col<ST, ND, NB, ST == kF32>(at.col, 0, w, dq);
@@ -1237,6 +1277,7 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
         for (int kb = kw; kb < TILE / 32; kb += SW) body(k0 < surelo || k0 + TILE > surehi, t, kb);
     }
     __syncthreads();
+    if (ST == kF16) unfit_f16<ND>(dq[0], up);
     unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same rows
     if constexpr (SW == 2) {
         give<ND>(pair, lane, dq[0], kw == 1);
@@ -1353,6 +1394,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
     unsigned char* const own = smem + wave * 32 * G::ROW;   // the wave's part of LDS where no tile is
     typename RawOf<ST>::T k[KL ? 1 : NB][G::KSTEPS], v[VL ? 1 : NB][G::KSTEPS];
     f32x16 dk[NB][ND], dv[NB][ND];
+    int up = kUp;       // of dk's (f16)
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const int j = jw + 32 * n + (lane & 31);
@@ -1462,8 +1504,12 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
             }
             if (DV) w[n].set(s[n]);
         }
-        if (DV) mma_col<ST, ND, NB, true>(at.col, Tile::BYTES, w, dv);
+        // (f16's cotangents first, whose largest is looked for: the registers hold no
+        // more beside the values' products)
+        if (DV && ST != kF16) mma_col<ST, ND, NB, true>(at.col, Tile::BYTES, w, dv);
         if (DK) {
+            const float fit = __builtin_ldexpf(1.f, up - (int)kShift);
+            Weights<ST> z[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -1472,22 +1518,24 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float y = s[n][4 * g + e];
-                        s[n][4 * g + e] = (ST == kF16 ? y * 0.00390625f : y) * (dp[n][4 * g + e] + x[e]);
+                        s[n][4 * g + e] = (ST == kF16 ? y * fit : y) * (dp[n][4 * g + e] + x[e]);
                     }
                 }
-                w[n].set(s[n]);
+                if (ST == kF16) fit_f16<ND>(s[n], dk[n], up, jw + (lane & 31) < (k1 < keys.len ? k1 : keys.len));
+                z[n].set(s[n]);
             }
-            mma_col<ST, ND, NB, true>(at.col, 0, w, dk);
+            mma_col<ST, ND, NB, true>(at.col, 0, z, dk);
             if constexpr (ST != kF32)
                 if (fine_of<ST>(a, keys, i0, i0 + 31 < a.tq ? i0 + 31 : a.tq - 1)) {
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        left_in<ST>(s[n], w[n]);
-                        w[n].set(s[n]);
+                        left_in<ST>(s[n], z[n]);
+                        z[n].set(s[n]);
                     }
-                    mma_col<ST, ND, NB, true>(at.col, 0, w, dk);
+                    mma_col<ST, ND, NB, true>(at.col, 0, z, dk);
                 }
         }
+        if (DV && ST == kF16) mma_col<ST, ND, NB, true>(at.col, Tile::BYTES, w, dv);
     };
     if (nt > t0) load_bits(i00);
     for (int t = t0, ti = i00; t < nt; ++t, ti = ti + QT < ihi ? ti + QT : ilo) {
@@ -1512,6 +1560,7 @@ __global__ void __launch_bounds__(256 * SW, OCC) attn_dkv_kernel(AttnArgs a, uns
         }
     }
     __syncthreads();
+    if (DK && ST == kF16) unfit_f16<ND>(dk[0], up);
     unsigned char* const pair = smem + rw * PAIR;      // the LDS of the waves of the same keys
     if constexpr (SW == 2) {
         static_assert(sizeof(smem) >= 4 * PAIR, "the waves' sums in LDS");

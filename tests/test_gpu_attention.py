@@ -647,3 +647,63 @@ def test_f32_small_elements(n):
     err = (o.cpu()[0, :, 0].double() - want).abs()
     print(float((err / (2.0 ** -134 + 2.0 ** -24 * want.abs())).max()))
     assert (err <= 2.0 ** -134 + 2.0 ** -24 * want.abs()).all()
+
+
+F16_SIZES = [(1, 4, 2, 1024, 1024, 64), (33, 8, 8, 130, 130, 64), (33, 4, 4, 200, 200, 128), (1, 2, 1, 300, 600, 200), (14, 8, 1, 40, 90, 96)]
+
+
+def f16_gradients(size, do, q=None, k=None, causal=True, last=0):
+    """The largest root mean square error of f16's gradients, over that of rounding the
+    exact ones to f16.  (Without a head's first element: where the scores hang on
+    that one, the cotangents' roundings are times it; `last`: of that many rows.)"""
+    hip.init(0)
+    q0, k0, v, _ = tensors("f16", *size)
+    q, k = q0 if q is None else q, k0 if k is None else k
+    op = hip.Attention("f16", *size, causal=causal)
+    Q, K, V, DO = (x.to(DEV) for x in (q, k, v, do))
+    o, lse = torch.empty_like(Q), torch.empty(size[0], size[1], size[3], device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    grads = {n: torch.empty_like(x) for n, x in (("dq", Q), ("dk", K), ("dv", V))}
+    op.vjp(Q, K, V, o, lse, DO, **grads)
+    want = A.Case("f16", q, k, v, A.allowed(size[0], size[3], size[4], causal), op.scale, do).vjp(o.cpu(), lse.cpu())
+    rms = lambda x: float(x.square().mean().sqrt())  # noqa: E731
+    out = {}
+    for n, g in grads.items():
+        x = want[n][0]
+        A.check(n, g, *want[n])
+        out[n] = rms((g.cpu().double() - x)[:, -last:, :, 1:]) / rms((x.half().double() - x)[:, -last:, :, 1:])
+    print({n: round(e, 2) for n, e in out.items()}, flush=True)
+    return max(out.values())
+
+
+@pytest.mark.parametrize("power", [0, -10, -13])
+@pytest.mark.parametrize("size", F16_SIZES, ids=str)
+def test_f16_gradients_of_small_cotangents(size, power):
+    """A mean loss's: the weights' cotangents, rounded to f16, add as much as the
+    gradients' own rounding does, whose errors are then 1.41 times those alone (and a
+    tenth for the sample), not what f16 has left at that size."""
+    do = (tensors("f16", *size)[3].float() * 2.0 ** power).half()
+    worst = f16_gradients(size, do)
+    assert worst <= 1.41 * 1.1
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("size", F16_SIZES, ids=str)
+def test_f16_gradients_of_cotangents_far_apart(size, turned):
+    """From 2^-20 to 2^6 along the rows, either way."""
+    do = tensors("f16", *size)[3].float()
+    power = torch.linspace(-20, 6, size[3])
+    do = (do * torch.exp2(power.flip(0) if turned else power)[None, :, None, None]).half()
+    worst = f16_gradients(size, do)
+    assert worst <= 1.41 * 1.1
+
+
+@pytest.mark.parametrize("size", [(2, 4, 2, 1001, 1000, 64), (9, 8, 8, 1001, 1000, 128), (1, 2, 1, 601, 600, 200)], ids=str)
+def test_f16_gradients_of_low_scores(size):
+    """Scores of -32 and less: a lane without a row or a key, beside the last ones of
+    them, has scores of 0 in their place and weights of 10^13, which say nothing of
+    the others' size."""
+    q, k, _, do = tensors("f16", *size)
+    q[..., 0], k[..., 0] = 16, -16 * (size[5] / 64) ** 0.5
+    worst = f16_gradients(size, (do.float() * 2.0 ** -12).half(), q, k, False, last=8)
+    assert worst <= 1.41 * 1.1
