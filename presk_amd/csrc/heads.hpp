@@ -60,19 +60,33 @@ inline std::string heads_check(const HeadsBuffer& b, int esz) {
     return "";
 }
 
-// Whether two tensors' elements meet.  Where their bytes interleave, rows of
-// equal stride that never share a place in it do not.
+// Whether two tensors' elements meet.  Where their bytes interleave (slices of a
+// packed buffer's rows, of its batches, of its heads) they do not if some stride of
+// theirs is a period in which both keep to places of their own: axes whose
+// strides are multiples of it stay in place, the others spread a tensor out.
 inline bool heads_meet(const HeadsBuffer& a, const HeadsBuffer& b, int esz) {
     if (a.count() == 0 || b.count() == 0 || !a.t->p || !b.t->p) return false;
     const uintptr_t x = (uintptr_t)a.t->p, y = (uintptr_t)b.t->p;
     if (!(x < y + (uintptr_t)(b.extent() * esz) && y < x + (uintptr_t)(a.extent() * esz))) return false;
-    const int64_t s = a.t->seq;
-    if (a.seq < 2 || b.seq < 2 || s != b.t->seq || (a.batch > 1 && a.t->batch % s) || (b.batch > 1 && b.t->batch % s)) return true;
-    const int64_t wa = (a.heads - 1) * a.t->head + a.d, wb = (b.heads - 1) * b.t->head + b.d;
     const int64_t gap = (int64_t)(y > x ? y - x : x - y);
-    if (wa > s || wb > s || gap % esz) return true;
-    const int64_t at = y > x ? gap / esz % s : (s - gap / esz % s) % s;    // b's place in a's rows
-    return at < wa || at + wb > s;
+    if (gap % esz) return true;
+    typedef std::pair<int64_t, int64_t> Axis;      // stride, length
+    auto axes = [](const HeadsBuffer& h) { return std::vector<Axis>{{h.t->batch, h.batch}, {h.t->seq, h.seq}, {h.t->head, h.heads}}; };
+    const std::vector<Axis> as = axes(a), bs = axes(b);
+    auto apart = [&](int64_t period) {
+        auto width = [&](const std::vector<Axis>& v, int64_t d) {
+            for (const Axis& e : v)
+                if (e.second > 1 && e.first % period) d += (e.second - 1) * e.first;
+            return d;
+        };
+        const int64_t wa = width(as, a.d), wb = width(bs, b.d);
+        const int64_t at = y > x ? gap / esz % period : (period - gap / esz % period) % period;    // b's place in a's period
+        return at >= wa && at + wb <= period;
+    };
+    for (const auto* v : {&as, &bs})
+        for (const Axis& e : *v)
+            if (e.second > 1 && e.first > 0 && apart(e.first)) return false;
+    return true;
 }
 
 inline bool bytes_meet(const void* p, int64_t n, const void* q, int64_t m) {

@@ -299,3 +299,34 @@ def test_workspaces_come_from_the_sizes():
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
     masked = attention(mask_cols=300, k_len=300, q_len=100)
     assert masked.workspace("vjp") == up(4 * 2 * 100 * 10) + up(4 * 2 * 300 * 4) + up(2 * 4 * 10) + up(8 * 2 * 4 * 100)
+
+
+def test_buffers_between_each_other(calls):
+    """Outputs whose elements lie between other tensors' are apart from them: single
+    tokens of a packed projection, and heads before rows in one buffer."""
+    op = attention(q_len=1, k_len=1)
+    one = lambda: dev(2, 1, 8, 64).split((4, 2, 2), 2)  # noqa: E731
+    (q, k, v), (dq, dk, dv) = one(), one()
+    lse = dev(2, 4, 1, dtype=torch.float32)
+    b = {"q": q, "k": k, "v": v, "o": dev(2, 1, 4, 64), "lse": lse, "do": dev(2, 1, 4, 64), "dq": dq, "dk": dk, "dv": dv}
+    op.vjp(**b)
+    rotary(seq=1).value(q, dev(32, dtype=torch.float64), q, k=k, yk=k)
+    for same in ({"dk": dv}, {"dk": dq[:, :, 3:].expand(2, 1, 2, 64)}, {"dv": q[:, :, 2:]}):
+        with pytest.raises(hip.HipError, match="meet"):
+            op.vjp(**{**b, **same})
+    (q, k, v), (dq, dk, dv) = (dev(2, 3, 4, 8, 64).unbind(1) for _ in range(2))
+    op = attention(kv_heads=4, layout="bhsd")
+    b = {"q": q, "k": k, "v": v, "o": dev(2, 4, 8, 64), "lse": dev(2, 4, 8, dtype=torch.float32), "do": dev(2, 4, 8, 64), "dq": dq, "dk": dk, "dv": dv}
+    op.vjp(**b)
+    # a cache's next row, beside those that the call reads
+    cache = dev(2, 4, 9, 64)
+    attention(kv_heads=4, layout="bhsd").value(**{**{n: b[n] for n in ("q", "v", "o", "lse")}, "k": cache[:, :, :8]})
+    rotary(seq=1, heads=4, kv_heads=0, layout="bhsd").value(cache[:, :, 8:], dev(32, dtype=torch.float64), cache[:, :, 8:])
+    assert len(calls) == 5
+    for same in ({"dk": dq}, {"dk": dev(2, 4, 8, 64), "dv": q}):
+        with pytest.raises(hip.HipError, match="meets"):
+            op.vjp(**{**b, **same})
+    flat = dev(2 * 4 * 8 * 64 + 32)
+    cut = lambda at: flat[at:at + 2 * 4 * 8 * 64].view(2, 4, 8, 64)  # noqa: E731
+    with pytest.raises(hip.HipError, match="dv meets dk|dk meets dv"):
+        op.vjp(**{**b, "dk": cut(0), "dv": cut(32)})
