@@ -160,8 +160,9 @@ def storage_inputs(p: Program, host: dict) -> dict:
                                 Q.Quant(q.bits, over, q.scheme))
                 env[name], env[name + "#scales"] = qt.data, qt.scales
             elif ty == "int8":
-                # a mask's bytes
-                env[name] = np.ascontiguousarray(v, dtype=np.uint8).ravel()
+                # a mask's bytes, those that the sequences share once for each
+                m = (np.asarray(v) != 0).astype(np.uint8).ravel()
+                env[name] = np.tile(m, count // m.size) if 0 < m.size < count and count % m.size == 0 else m
             elif np.asarray(v).dtype == np.float64:
                 # the host's f64 values (literals, drawn inputs): one Buf::of
                 env[name] = encode64(np.asarray(v).reshape(-1)[:max(count, 1)], ty)

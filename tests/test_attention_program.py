@@ -1,8 +1,9 @@
 """Attention and head rotations as steps of a program, without a GPU: what they
 refuse, what they read, and that a program without them is as it was."""
+import numpy as np
 import pytest
 
-from presk_amd import gpt, hip, llama
+from presk_amd import configs, gpt, hip, llama
 from presk_amd import lower as L
 from presk_amd.gpt import A, Builder
 from presk_amd.program import Program
@@ -82,3 +83,17 @@ def test_views_and_axes():
     assert [a.len for a in b.axes[o]] == [2, 4, 16] and [a.len for a in b.axes[lse]] == [2, 2, 4]
     grads = b.attention_vjp(q, "kv", "kv", o, lse, "do", 2, 1, name="g")
     assert grads == ("g.dq", "g.dk", "g.dv") and [[a.len for a in b.axes[g]] for g in grads] == [[2, 4, 16], [2, 4, 8], [2, 4, 8]]
+
+
+def test_a_masks_host_values():
+    """Anything but 0 is a key that is read, and a mask without a batch is every
+    sequence's."""
+    p = Program("t", hip.FAST)
+    p.add_attention("value", {**QKV, "o": "o", "mask": "m"}, **{**SIZES, "causal": False, "mask_cols": 4})
+    rng = np.random.default_rng(1)
+    want = rng.random((2, 4, 4)) < 0.5
+    for m in (want, want.astype(np.uint8) * 255, want * 256, want * 0.25, np.where(want, -1.0, 0.0)):
+        got = configs.storage_inputs(p, {"m": m})["m"]
+        assert got.dtype == np.uint8 and ((got != 0) == want.ravel()).all()
+    got = configs.storage_inputs(p, {"m": want[0]})["m"]
+    assert got.size == 32 and ((got.reshape(2, 4, 4) != 0) == want[0]).all()
