@@ -451,7 +451,11 @@ void presk_hip_release(presk_hip_kernel* h) {
 }
 
 int presk_hip_alloc(size_t bytes, void** dev) {
+    // (allowed while a stream is captured, of which it records nothing)
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool other = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
     hipError_t e = hipMalloc(dev, bytes ? bytes : 1);
+    if (other) (void)hipThreadExchangeStreamCaptureMode(&mode);
     return e == hipSuccess ? PRESK_HIP_OK : hip_fail(e, "hipMalloc");
 }
 int presk_hip_free(void* dev) {

@@ -409,7 +409,8 @@ class Distill:
     with tensors that names no stream goes to torch's current one, others to
     the null stream.  `work` is workspace(kind) bytes of the caller's, or, not
     given, a buffer that this object keeps for the call's stream (with any
-    smaller one outgrown, which a captured call may still use): calls that
+    smaller one outgrown, which a captured call's graph may still use, and the
+    object with it): calls that
     share a workspace, their captured graphs among them, run one after another."""
 
     head = False
@@ -651,8 +652,9 @@ class Attention(_HeadsCall):
     are given.  Buffers are DeviceBuffers or torch tensors; a call with tensors
     that names no stream goes to torch's current one, others to the null stream.
     `work` is workspace(kind) bytes of the caller's, or, not given, a buffer that
-    this object keeps for the call's stream: calls that share a workspace, their
-    captured graphs among them, run one after another."""
+    this object keeps for the call's stream (a captured call's graph needs the object
+    as long as it is replayed): calls that share a workspace, their captured graphs
+    among them, run one after another."""
 
     _name = "attention"
     _launch = staticmethod(lambda lib: lib.presk_hip_attention)

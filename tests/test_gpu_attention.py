@@ -707,3 +707,38 @@ def test_f16_gradients_of_low_scores(size):
     q[..., 0], k[..., 0] = 16, -16 * (size[5] / 64) ** 0.5
     worst = f16_gradients(size, (do.float() * 2.0 ** -12).half(), q, k, False, last=8)
     assert worst <= 1.41 * 1.1
+
+
+def test_captured_calls_take_their_own_workspace():
+    """A first call while its stream is captured, without one of the caller's."""
+    hip.init(0)
+    b, n, h, kv, d = 2, 70, 4, 2, 64
+    q, k, v, do = (x.to(DEV) for x in tensors("bf16", b, h, kv, n, n, d))
+    freq, g = torch.from_numpy(hip.rotary_frequencies(d)).to(DEV), torch.ones(d, dtype=torch.bfloat16, device=DEV)
+
+    def ops():
+        return hip.Attention("bf16", b, h, kv, n, n, d, causal=True), hip.HeadRotary("bf16", b, n, h, kv, d, norm=True)
+
+    def call(op, rot, outs):
+        o, lse, dq, dk, dv, tq, tk, dg = outs
+        op.value(q, k, v, o, lse=lse)
+        op.vjp(q, k, v, o, lse, do, dq=dq, dk=dk, dv=dv)
+        rot.vjp(freq, dq, tq, dyk=dk, dk=tk, q=q, k=k, gq=g, gk=g, dgq=dg)
+
+    def outs():
+        return [torch.empty_like(q), torch.empty(b, h, n, device=DEV), *(torch.empty_like(x) for x in (q, k, v, q, k, g))]
+
+    captured, eager, mine = ops(), ops(), outs()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(*captured, mine)
+    for step in range(3):
+        q.mul_(1.1)
+        for x in mine:
+            x.fill_(9.0)
+        graph.replay()
+        again = outs()
+        call(*eager, again)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(mine, again)), step
