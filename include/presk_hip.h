@@ -337,8 +337,8 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  *   neither:        always.
  * `first` null: k_len - q_len (the queries are the last keys), of a mask k_len -
  * mask_cols.  A key at or past lens[b] is not read, whatever it holds, and its
- * rows of dk and dv are 0; one that only some queries read enters the others
- * times 0, so it must be finite.
+ * rows of dk and dv are 0; any other enters the sums of queries that may not read
+ * it times 0, so it must be finite, also where no query reads it.
  * A tensor's element (b, i, h, d) is at p + b * batch + i * seq + h * head + d,
  * strides in elements and not negative, those of an input over batch or heads 0
  * where it is shared.  Rows of whole 16-byte vectors (address, strides and
@@ -412,8 +412,9 @@ int presk_hip_batch_add_attention(presk_hip_batch* b, const presk_hip_attn* a, i
  * PRESK_HIP_ROT_GRAD, from their cotangents dyq and dyk and, with `norm`, q and k,
  * writes dq and dk (which may be dyq and dyk) and those of dgq and dgk ([head_dim])
  * that are not null.  Sums in f32, angles in f64 (so that the cosine and sine of one
- * of 2^30 radians are within 2^-23 of those of its f64 product); tensors, f16's flag,
- * `work` (null and 0 bytes do but for a gradient with `norm`), streams and graphs as
+ * of 2^30 radians are within 2^-23 of those of its f64 product).  f16 outputs
+ * that overflow set bit 0 of *flag (if flag is not null).  Tensors, `work` (null and 0
+ * bytes do but for a gradient with `norm`), streams and graphs as
  * presk_hip_attention's. */
 typedef struct {
     const char* dtype;

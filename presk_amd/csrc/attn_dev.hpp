@@ -50,10 +50,10 @@ template <> struct FragOf<kF32> { typedef f32x4 T; };
 // each, rounded to nearest, which are all of its 24 down to 2^-110 (where the last
 // part's come to bf16's smallest step, 2^-133: scaling that away is an instruction an
 // element more, and a second pass for the large ones, on what these kernels are
-// bound by): of a product's nine six are taken (the three left are below 2^-24 of it together, f32's own rounding), by
-// bf16 instructions, of which six take 3/8 of the time of f32's own (64 x 6 heads x
-// 256 x 64, causal: the value 63 -> 50 us, the queries' gradient 87 -> 64, the keys'
-// 121 -> 98, with errors against 64 bits as before; bound now by the eleven vector
+// bound by).  Of a product's nine six are taken (the three left are below 2^-24 of it
+// together, f32's own rounding), by bf16 instructions, of which six take 3/8 of the
+// time of f32's own (64 x 6 heads x 256 x 64, causal: the value 63 -> 52 us, the
+// queries' gradient 87 -> 68, the keys' 121 -> 105; bound now by the eleven vector
 // instructions that two elements' parts take, in every wave that reads them).  An
 // infinite element, or one that rounds to it, has a second part that is no number:
 // what reads it is NaN.
@@ -1298,9 +1298,10 @@ __device__ __forceinline__ void dq_of(const AttnArgs& a, unsigned id, unsigned t
 // workgroup a CU has the room, the keys beside them.  DQ: the queries' workgroups
 // follow the `nkv` of the keys in one launch, where either would leave CUs idle
 // (3 x 10 heads, 5 of keys, 777 x 1021 x 80, 120 and 210 workgroups: 38 + 18 -> 41
-// us; 2 x 12 heads x 1024 x 64, 192 each: 27 + 24 -> 39).  With eight waves, or
-// heads past 128, a tile's rows may be in parts of theirs (AttnArgs::parts), whose
-// sums in f32 attn_sum_kernel adds.  4 x 32 heads in groups of four x 4096 x 128 in
+// us, in f16 44 with its cotangents' powers; 2 x 12 heads x 1024 x 64, 192 each:
+// 27 + 24 -> 39).  With eight waves, or heads past 128, a tile's rows may be in parts
+// of theirs (AttnArgs::parts), whose sums in f32 attn_sum_kernel adds.  4 x 32 heads
+// in groups of four x 4096 x 128 in
 // bf16, causal, 1400 to 1440 us, 775 TFLOP/s of the four products: matrix
 // instructions in 40 % of the cycles, vector ones in 25, LDS in 30, each waiting for
 // the others' results in turn with two waves a SIMD, which is what the registers
