@@ -347,10 +347,10 @@ int presk_hip_batch_add_distill(presk_hip_batch* b, const presk_hip_loss* a, int
  * the weights p and their cotangents ds are rounded to the storage type before
  * the products they enter, ds with what that rounding left as a second term where
  * queries read fewer than 64 keys or a mask says which; in f16 ds times a power of
- * two, 1 or more, that keeps small ones' bits and is taken out of the sums.  f32 elements enter as
- * three bf16 parts, which are all of one of 2^-110 or more (below, what is left of it
- * may be off by 2^-134), and six of their nine products (the rest is below 2^-24);
- * one that is infinite, or above 0x1.ffp127, gives NaN.
+ * two, 1 or more, that keeps small ones' bits and is taken out of the sums.  f32
+ * elements enter as three bf16 parts, which are all of one of 2^-110 or more (a
+ * smaller one may lose 2^-134), and six of their nine products (the rest is below
+ * 2^-24); one that is infinite, or above 0x1.ffp127, gives NaN.
  *
  * `what`: PRESK_HIP_ATTN_VALUE writes o and, where it is not null, lse (f32 [batch,
  * heads, q_len]).  PRESK_HIP_ATTN_GRAD writes those of dq, dk and dv whose p is

@@ -234,8 +234,8 @@ hipError_t attn_run(const presk_hip_attn& a, int what, hipStream_t s) {
     auto tensor = [&](const presk_hip_heads& t, int64_t seq, int64_t heads) {
         auto whole = [&](int64_t n, int64_t stride) { return n < 2 || stride * esz % 16 == 0; };
         const bool vec = (uintptr_t)t.p % 16 == 0 && a.head_dim * esz % 16 == 0 && whole(a.batch, t.batch) && whole(seq, t.seq) && whole(heads, t.head);
-        // (a single row's stride is the caller's whim, and the kernels multiply it by a
-        // tile's row numbers: what they find past the row has to be zero)
+        // (a single row's stride may be anything, and the kernels multiply it by a tile's
+        // row numbers: what they find past the row has to be zero)
         return AttnTensor{t.p, t.batch, seq < 2 ? a.head_dim : t.seq, t.head, vec};
     };
     auto queries = [&](const presk_hip_heads& t) { return tensor(t, a.q_len, a.heads); };

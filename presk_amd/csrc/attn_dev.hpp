@@ -1099,9 +1099,9 @@ constexpr float kShift = 8.f;
 // the wave's own, 2^up: as large a one as leaves the largest so far below 2^15 (those
 // of 2^-22 of it and more are whole), and one at least, so that those past f16 still
 // show.  As with a softmax's maximum, the sums go along with it where it has to fall,
-// then by so much that the largest is past 2^8.  (Gradients of 4 x 32 heads in groups of four
-// x 4096 x 128, causal: 2400 us without it, 2540 so, 2730 with a power for each kept row,
-// which takes registers; shorter ones 2 to 6 % more than without.)
+// then by so much that the largest is past 2^8.  (Gradients of 4 x 32 heads in groups
+// of four x 4096 x 128, causal: 2400 us without it, 2540 so, 2730 with a power for each
+// kept row, which takes registers; shorter ones 2 to 8 % more than without.)
 constexpr int kUp = 60;     // (2^60 times the largest of them, 2^41, stays in f32)
 template <int ND>
 __device__ __forceinline__ void fit_f16(f32x16& s, f32x16 (&acc)[ND], int& up, bool live) {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -71,10 +72,11 @@ inline bool heads_meet(const HeadsBuffer& a, const HeadsBuffer& b, int esz) {
     const int64_t gap = (int64_t)(y > x ? y - x : x - y);
     if (gap % esz) return true;
     typedef std::pair<int64_t, int64_t> Axis;      // stride, length
-    auto axes = [](const HeadsBuffer& h) { return std::vector<Axis>{{h.t->batch, h.batch}, {h.t->seq, h.seq}, {h.t->head, h.heads}}; };
-    const std::vector<Axis> as = axes(a), bs = axes(b);
+    typedef std::array<Axis, 3> Axes;
+    auto axes = [](const HeadsBuffer& h) { return Axes{{{h.t->batch, h.batch}, {h.t->seq, h.seq}, {h.t->head, h.heads}}}; };
+    const Axes as = axes(a), bs = axes(b);
     auto apart = [&](int64_t period) {
-        auto width = [&](const std::vector<Axis>& v, int64_t d) {
+        auto width = [&](const Axes& v, int64_t d) {
             for (const Axis& e : v)
                 if (e.second > 1 && e.first % period) d += (e.second - 1) * e.first;
             return d;

@@ -742,3 +742,29 @@ def test_captured_calls_take_their_own_workspace():
         call(*eager, again)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(mine, again)), step
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_single_tokens_of_packed_projections(dtype):
+    """One token a sequence, rotated in place and then read where the projection left
+    it, its gradients side by side in one buffer."""
+    hip.init(0)
+    b, h, kv, d = 5, 4, 2, 64
+    q, k, v, do = tensors(dtype, b, h, kv, 1, 1, d)
+    packed, grads = torch.cat((q, k, v), 2).to(DEV), torch.full((b, 1, h + 2 * kv, d), 9.0, dtype=q.dtype, device=DEV)
+    (Q, K, V), (dq, dk, dv) = (x.split((h, kv, kv), 2) for x in (packed, grads))
+    freq, at = torch.from_numpy(hip.rotary_frequencies(d)), torch.arange(b)[:, None] * 100
+    hip.HeadRotary(dtype, b, 1, h, kv, d).value(Q, freq.to(DEV), Q, k=K, yk=K, at=at.to(DEV))
+    for x, y in ((q, Q), (k, K)):
+        A.check("y", y, *A.rotary(dtype, x, None, freq, at, d, False, 0.0, False))
+    assert torch.equal(V.cpu(), v)
+    q, k = Q.cpu(), K.cpu()
+    op = hip.Attention(dtype, b, h, kv, 1, 1, d, causal=True)
+    o, lse = torch.empty(b, 1, h, d, dtype=q.dtype, device=DEV), torch.empty(b, h, 1, device=DEV)
+    op.value(Q, K, V, o, lse=lse)
+    op.vjp(Q, K, V, o, lse, do.to(DEV), dq=dq, dk=dk, dv=dv)
+    case = A.Case(dtype, q, k, v, A.allowed(b, 1, 1, True), op.scale, do)
+    A.check("o", o, *case.value()["o"])
+    want = case.vjp(o.cpu(), lse.cpu())
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        A.check(name, got, *want[name])
